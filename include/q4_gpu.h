@@ -457,6 +457,57 @@ bool q4_gpu_kv_prefill(const q4_gpu_kv *kv, uint32_t layer, const void *q_bf16, 
                        void *out_bf16, uint32_t n_head, uint32_t n_tok, uint32_t kv_base,
                        float scale);
 
+/* ---- a paged KV cache for many requests in one pool (no counterpart in the reference: one contiguous cache per session).  A
+ * request's rows lie in pages of page_rows positions, named by its row of a block table; a step brings `add` new tokens per
+ * request: one (decoding), a few (drafts) or many (a chunk of prompt), all requests in one call.  Per step:
+ *     q4_gpu_pages_plan(...);                              pages, slots and positions of the step's tokens
+ *     per layer: q4_gpu_pages_append(...); q4_gpu_pages_attend(...);
+ * and q4_gpu_pages_trim when requests end or are rewound.  All lengths and maps live on the device, so a step can be captured
+ * in a graph and replayed while they change.
+ * Memory is the caller's: `mem` (q4_gpu_pages_bytes, 16-byte aligned), the stack of free pages `free_list` [n_pages] with its
+ * height `n_free` (one word), both on the device; a new pool's stack holds all page numbers.  Pages may be named by several
+ * tables for reading (a shared prefix of whole pages), but must be given back once.
+ * mem: [layer][page][kv head][tile of 16 rows].  q8_0 tile: 16 records {K codes hd | V codes hd | K scales hd/32 fp16 | V scales},
+ * padded to 16 bytes (144, 272, 544 at hd 64, 128, 256).  fp16 tile: K then V, each hd/64 blocks of 16 rows x 128 bytes whose
+ * 16-byte piece c of row r lies at c ^ (r & 7).  kind is 1 (fp16) or 2 (q8_0); hd 64, 128 or 256; page_rows a power of two, 16
+ * to 256; n_pages * page_rows below 2^31. */
+typedef struct q4_gpu_pages {
+    void *mem;
+    int32_t *free_list, *n_free;     /* plan and trim only */
+    uint32_t n_layers, n_kvh, hd, n_pages, page_rows;
+    int kind;
+} q4_gpu_pages;
+uint64_t q4_gpu_pages_bytes(uint32_t n_layers, uint32_t n_kvh, uint32_t hd, uint32_t n_pages, uint32_t page_rows, int kind);
+/* Request r holds rows[r] rows and gets add[r] more tokens (0 or less: none): ceil((rows + add) / page_rows) - ceil(rows / page_rows)
+ * pages from the top of the stack, in the order of the requests, go into its row of table [n_req][table_stride]; start [n_req + 1]
+ * are the exclusive sums of the tokens; token t = start[r] + j has req[t] = r, pos[t] = rows[r] + j and slot[t] = page * page_rows +
+ * row in the page.  slot, pos and req have max_tok entries; those behind the step's tokens are -1.  Requests are served up to the
+ * first one that does not fit (pages left, max_tok): it and those behind it get nothing (their start does not move) and status bit
+ * 8 is set.  A request that would pass its table's row (or rows < 0) gets nothing and sets status bit 4.  n_req <= 8192. */
+bool q4_gpu_pages_plan(const q4_gpu_pages *pg, const int32_t *rows, const int32_t *add, uint32_t n_req, int32_t *table,
+                       uint32_t table_stride, int32_t *start, int32_t *slot, int32_t *pos, int32_t *req, uint32_t max_tok);
+/* Request r, which holds rows[r] rows, keeps the first keep[r] of them (0 or less: none): the pages behind those go back on the
+ * stack, in the order in which a plan that is taken back took them.  Table entries stay as they are.  More pages than are out
+ * (one given back twice): nothing is done, status bit 4. */
+bool q4_gpu_pages_trim(const q4_gpu_pages *pg, const int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table,
+                       uint32_t table_stride);
+/* k, v [n_tok][n_kvh * hd] fp32: row t of one layer into slot[t] (below 0: skipped; beyond the pool: skipped, status bit 4),
+ * quantised as q4_gpu_kv_append does or rounded to fp16. */
+bool q4_gpu_pages_append(const q4_gpu_pages *pg, uint32_t layer, const float *k, const float *v, const int32_t *slot, uint32_t n_tok);
+/* The rows of slots as fp32 (code * scale), [n_tok][n_kvh * hd]; k or v may be NULL.  A slot below 0 gives zeros. */
+bool q4_gpu_pages_gather(const q4_gpu_pages *pg, uint32_t layer, const int32_t *slot, uint32_t n_tok, float *k, float *v);
+/* Attention of a step's tokens: token start[r] + j attends positions [0, rows[r] + j] of request r, found through its row of the
+ * table; rows is what the requests held before the step, and the step's own rows are appended already.
+ *   q, out   [n_tok][n_head][hd], bf16 or fp32; n_head / n_kvh 1 to 16; rows of out behind start[n_req] are not written
+ *   gate     [n_tok][n_head][hd] fp32 or NULL; out = softmax(q.k * scale) v * sigmoid(gate)
+ *   max_add  the most tokens of one request, as far as the host knows (0: it does not).  It chooses between kernels only: results
+ *            are right for any value
+ * A request whose rows pass its table's row is left out (status bit 4); positions on a page that is not the pool's are skipped
+ * (status bit 4); a token with nothing to attend gets 0.  Scratch grows outside a capture only (status bit 8 inside one). */
+bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, int q_bf16, const float *gate, void *out, int out_bf16,
+                         uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
+                         uint32_t table_stride, uint32_t max_add, float scale);
+
 #ifdef __cplusplus
 }
 #endif

@@ -228,6 +228,10 @@ struct q4_gpu_xchg {
 /* wait-and-merge half alone (q4_decode.cu): the records of the latest push on every rank -> out */
 bool q4i_xchg_merge(const q4_gpu_xchg *x, const float *gate, float *out);
 
+/* pools of pages (q4_pages.cu): bytes of K and V of one position and kv head; whether a descriptor holds together */
+uint32_t q4i_pages_row_bytes(uint32_t hd, int kind);
+bool q4i_pages_ok(const q4_gpu_pages *pg);
+
 /* frees the prefill staging buffer (q4_prefill.cu) / the session-file staging (q4_sess.cu); called at shutdown */
 void q4i_prefill_release();
 void q4i_sess_release();

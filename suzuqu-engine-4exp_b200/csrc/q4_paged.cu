@@ -1,0 +1,655 @@
+/*
+ * Attention of a step's new tokens over a pool of pages: token j that request r brings attends positions [0, rows[r] + j] of
+ * that request, with the query heads of a kv head sharing every row that is read.
+ *
+ *     o = sum_p w_p v_p / sum_p w_p,  w_p = 2^(scale log2(e) q.k_p - m),  m the running maximum;  out = o sigmoid(gate)
+ *
+ * q4_pg_few_k, tokens of requests that bring few.  Bound by memory: every row is read once, for 8 to 32 (token, head) pairs.
+ * Both contractions run on warp-level MMA with the positions as M, so that 8 pairs are a whole tile of the product:
+ * S^T = K Q^T and O^T += V^T P^T, 16 positions per step of a warp.
+ *
+ * Requests differ in length by orders of magnitude, so blocks are not given requests but equal shares of the step's whole work:
+ * the steps (128 positions) of all units (request, kv head, group of tokens) lie one behind the other, and block c takes steps
+ * [T c / C, T (c + 1) / C).  Where a share ends inside a unit the block leaves (acc, m, l) records, at most two, and q4_pg_merge_k
+ * joins a unit's records; the block that holds the unit's end tells it which.  The division is computed by every block
+ * itself from the lengths on the device (one scan), which the host need not know.
+ */
+#include <cuda_bf16.h>
+#include <math_constants.h>
+#include <string.h>
+
+#include "q4_internal.h"
+
+namespace {
+
+constexpr uint32_t PG_SPIN_LIMIT = 1u << 20;
+
+struct PagedParams {
+    const uint8_t *mem;          /* of the layer */
+    uint64_t page_bytes;         /* of all kv heads */
+    uint32_t part_bytes;         /* of one kv head */
+    uint32_t n_pages, page_shift, n_kvh, n_head, gqa, tpg /* tokens per group */;
+    const int32_t *rows, *start, *table;
+    uint32_t table_stride, n_req, n_tok;
+    const void *q;
+    const float *gate;
+    void *out;
+    int q_bf16, out_bf16;
+    float scale_log2e;
+    float *part;                 /* [block][2][rows of a group][hd + 4] */
+    int4 *ends;                  /* [block] {first block of the unit that ends here, or -1; its first token; its rows; its kv head} */
+    uint32_t *err;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0u;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+/* fp16 1024 + 128 + code has (code ^ 0x80) in its low byte: two bytes picked out of word x (its codes ^ 0x80) become the exact codes */
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) {
+    return h2u(__hsub2(u2h(__byte_perm(x, 0x64646464u, SEL)), u2h(0x64806480u)));
+}
+
+template <int KIND, int HD>
+struct PgTile {
+    static constexpr uint32_t ROW = KIND == Q4K_Q8 ? (2u * HD + HD / 8u + 15u) / 16u * 16u : 4u * HD, BYTES = 16u * ROW;
+};
+/* warps per block, blocks per SM, tiles of a warp's ring: as many bytes in flight as an SM's shared memory holds */
+template <int KIND, int HD, int NT>
+struct FewCfg {
+    static constexpr uint32_t TILE = PgTile<KIND, HD>::BYTES;
+    static constexpr uint32_t ROWS = 8u * NT;
+    static constexpr uint32_t CTAS = (TILE <= 4352u && NT * HD <= 256) ? 2u : 1u;
+    static constexpr uint32_t WARPS = TILE > 8704u ? 4u : 8u;
+    static constexpr uint32_t DEPTH = TILE <= 2304u ? 4u : 3u;
+    static constexpr uint32_t THREADS = WARPS * 32u;
+    static constexpr uint32_t STEP = WARPS * 16u;            /* positions per step */
+    static constexpr uint32_t Q_STRIDE = HD * 2u + 32u;      /* the four rows of a half-warp's 8-byte reads on different banks */
+    static constexpr uint32_t RING = WARPS * DEPTH * TILE;
+    static constexpr uint32_t REC = HD + 4u;
+    /* fragments of half of the warps on the way to the others, and the block's record, reuse the ring */
+    static constexpr uint32_t FRAG = (HD / 16u * 4u + 4u) * NT * 32u * 4u;
+    static_assert(WARPS / 2u * FRAG <= RING && ROWS * REC * 4u <= RING, "merge does not fit");
+    static constexpr uint32_t SMEM = RING + ROWS * Q_STRIDE + WARPS * DEPTH * 8u + 1024u;
+};
+
+/* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */
+struct PgReq { uint32_t held, add, tok0; };
+__device__ __forceinline__ PgReq pg_request(const PagedParams &P, uint32_t r, bool &bad) {
+    const int32_t s0 = P.start[r], s1 = P.start[r + 1u], h = P.rows[r];
+    PgReq q = {0u, 0u, 0u};
+    bad = false;
+    if (s1 <= s0) return q;
+    if (h < 0 || s0 < 0 || (uint32_t)s1 > P.n_tok || (uint64_t)(uint32_t)h + (uint32_t)(s1 - s0) > ((uint64_t)P.table_stride << P.page_shift)) {
+        bad = true;
+        return q;
+    }
+    q.held = (uint32_t)h; q.add = (uint32_t)(s1 - s0); q.tok0 = (uint32_t)s0;
+    return q;
+}
+
+template <int KIND, int HD, int NT>
+__global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD, NT>::CTAS) q4_pg_few_k(const PagedParams P) {
+    using C = FewCfg<KIND, HD, NT>;
+    constexpr uint32_t TILE = C::TILE, WARPS = C::WARPS, DEPTH = C::DEPTH, STEP = C::STEP, MT = HD / 16u;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t s_sum[WARPS];
+    __shared__ uint64_t s_off;
+    __shared__ uint32_t s_req;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t s_base = (smem_u32(smem) + 1023u) & ~1023u;   /* swizzled tiles are anchored to multiples of 1024 */
+    uint8_t *base = smem + (s_base - smem_u32(smem));
+    const uint32_t ring = s_base + warp * DEPTH * TILE, s_q = s_base + C::RING, bars = s_q + C::ROWS * C::Q_STRIDE + warp * DEPTH * 8u;
+    if (lane == 0)
+        for (uint32_t i = 0; i < DEPTH; i++) bar_init(bars + 8u * i, 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    q4d_pdl_wait();
+
+    /* ---- this block's share of all steps */
+    auto steps_of = [&](uint32_t r, bool &bad) -> uint64_t {
+        const PgReq q = pg_request(P, r, bad);
+        return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh * ((q.held + q.add + STEP - 1u) / STEP);   /* no tokens: 0 groups */
+    };
+    const uint32_t per = (P.n_req + C::THREADS - 1u) / C::THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
+    uint64_t mine = 0, total = 0, before = 0;
+    bool bad, any_bad = false;
+    for (uint32_t r = r0; r < r1; r++) {
+        mine += steps_of(r, bad);
+        any_bad |= bad;
+    }
+    {
+        uint64_t x = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= (uint32_t)d) x += y;
+        }
+        if (lane == 31u) s_sum[warp] = x;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < WARPS; w++) {
+            if (w < warp) before += s_sum[w];
+            total += s_sum[w];
+        }
+        before += x - mine;
+    }
+    if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    const uint64_t blocks = min((uint64_t)gridDim.x, total);
+    if (blockIdx.x >= blocks) {
+        if (tid == 0) P.ends[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    uint64_t s = total * blockIdx.x / blocks;
+    const uint64_t s_end = total * (blockIdx.x + 1u) / blocks;
+    if (before <= s && s < before + mine)
+        for (uint32_t r = r0; r < r1; r++) {
+            const uint64_t n = steps_of(r, bad);
+            if (s < before + n) {
+                s_req = r;
+                s_off = s - before;
+                break;
+            }
+            before += n;
+        }
+    __syncthreads();
+    uint32_t req = s_req, issued = 0, taken = 0;   /* of the warp's ring, over all pieces */
+    uint64_t off = s_off;
+    int4 end_of = make_int4(-1, 0, 0, 0);
+    bool ok = true;
+
+    /* ---- pieces of units */
+    while (s < s_end) {
+        const PgReq R = pg_request(P, req, bad);
+        const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = (R.held + R.add + STEP - 1u) / STEP;
+        if (off >= (uint64_t)groups * P.n_kvh * n_steps) {   /* on to the next request; requests without tokens are passed over */
+            off -= (uint64_t)groups * P.n_kvh * n_steps;
+            req++;
+            continue;
+        }
+        const uint32_t unit = (uint32_t)(off / n_steps), st = (uint32_t)(off - (uint64_t)unit * n_steps);
+        const uint32_t here = (uint32_t)min((uint64_t)(n_steps - st), s_end - s);
+        const uint32_t kh = unit / groups, j0 = (unit - kh * groups) * P.tpg, n_here = min(P.tpg, R.add - j0);
+        const uint32_t n_kv = R.held + j0 + n_here, live_rows = n_here * P.gqa, tok0 = R.tok0 + j0;
+
+        /* ---- the unit's queries as fp16 */
+        __syncthreads();   /* the piece before has been read */
+        for (uint32_t i = tid; i < C::ROWS * (HD / 4u); i += C::THREADS) {
+            const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < live_rows) {
+                const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
+                if (P.q_bf16) {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + at);
+                    x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+                } else {
+                    x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(P.q) + at);
+                }
+            }
+            const uint32_t lo = h2u(__floats2half2_rn(x.x, x.y)), hi = h2u(__floats2half2_rn(x.z, x.w)), a = s_q + row * C::Q_STRIDE;
+            if (KIND == Q4K_Q8) {
+                /* lane t feeds dims 4 t .. 4 t + 3 of 16, as it gets the codes */
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a + d * 2u), "r"(lo), "r"(hi) : "memory");
+            } else {
+                /* lane t feeds dims 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of 16: one behind the other */
+                const uint32_t in = d & 15u, p = a + (d & ~15u) * 2u + (in & 7u) / 2u * 8u + (in >> 3) * 4u;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(lo) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p + 8u), "r"(hi) : "memory");
+            }
+        }
+        __syncthreads();
+
+        /* positions that column 2 t + e of row tile i may see */
+        uint32_t lim[NT][2], lim_min = n_kv;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (uint32_t e = 0; e < 2; e++) {
+                const uint32_t row = 8u * i + 2u * t + e;
+                lim[i][e] = row < live_rows ? R.held + j0 + row / P.gqa + 1u : n_kv;
+                lim_min = min(lim_min, lim[i][e]);
+            }
+        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+
+        /* ---- this warp's tiles of the piece, numbered i = 0 .. : tile (st + i) * WARPS + warp of the unit */
+        const uint32_t tiles = (n_kv + 15u) / 16u;
+        uint32_t n_my = 0;
+        if (ok && st * WARPS + warp < tiles) n_my = min(here, (tiles - 1u - st * WARPS - warp) / WARPS + 1u);
+        const int32_t *tab = P.table + (size_t)req * P.table_stride;
+        auto entry = [&](uint32_t i) -> int32_t { return i < n_my ? tab[(((st + i) * WARPS + warp) * 16u) >> P.page_shift] : 0; };
+        int32_t cur = -1, nxt = entry(lane);
+        uint32_t dead = 0, dead_nxt = 0;   /* tiles of the present / the next 32 whose page is not the pool's */
+        const uint8_t *src = P.mem;
+        uint32_t ahead = 0;
+        auto issue = [&]() {   /* tile `ahead`, by the lane that holds its page */
+            if ((ahead & 31u) == 0u) {
+                cur = nxt;
+                nxt = entry(ahead + 32u + lane);
+                const uint32_t p = ((st + ahead + lane) * WARPS + warp) * 16u;
+                const bool there = cur >= 0 && (uint32_t)cur < P.n_pages;
+                src = P.mem + (uint64_t)(there ? (uint32_t)cur : 0u) * P.page_bytes + (uint64_t)kh * P.part_bytes + ((p & ((1u << P.page_shift) - 1u)) >> 4) * TILE;
+                cur = there ? 0 : -1;
+                dead_nxt = __ballot_sync(0xffffffffu, !there);
+                if (ahead == 0u) dead = dead_nxt;
+            }
+            const uint32_t slot = issued % DEPTH;
+            if (lane == (ahead & 31u)) {
+                if (cur >= 0) {
+                    bar_expect(bars + 8u * slot, TILE);
+                    bulk_load(ring + slot * TILE, src, TILE, bars + 8u * slot);
+                } else {
+                    bar_arrive(bars + 8u * slot);
+                    atomicOr(P.err, (uint32_t)Q4E_RANGE);
+                }
+            }
+            ahead++;
+            issued++;
+        };
+        while (ahead < n_my && ahead < DEPTH) issue();
+
+        float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            m[i][0] = m[i][1] = -CUDART_INF_F;
+            l[i][0] = l[i][1] = 0.f;
+#pragma unroll
+            for (uint32_t k = 0; k < MT; k++) o[k][i][0] = o[k][i][1] = o[k][i][2] = o[k][i][3] = 0.f;
+        }
+        for (uint32_t i = 0; i < n_my; i++) {
+            const uint32_t slot = taken % DEPTH, phase = (taken / DEPTH) & 1u, sb = ring + slot * TILE;
+            const uint32_t p0 = ((st + i) * WARPS + warp) * 16u;
+            taken++;
+            for (uint32_t spin = 0; !bar_test(bars + 8u * slot, phase); spin++)
+                if (spin >= PG_SPIN_LIMIT) { ok = false; break; }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const bool gone = (dead >> (i & 31u)) & 1u;
+            if ((i & 31u) == 31u) dead = dead_nxt;
+            if (!gone) {
+                /* ---- scores: c0, c1 of position g, c2, c3 of position g + 8, columns 2 t and 2 t + 1 */
+                float sc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+                const uint32_t mrow = (lane & 7u) + ((lane >> 3) & 1u) * 8u, mchunk = lane >> 4;   /* of ldmatrix: the row and 16-byte piece this lane addresses */
+                if constexpr (KIND == Q4K_Q8) {
+                    constexpr uint32_t NB = HD / 32u;
+                    uint32_t k0[NB / 2], k1[NB / 2];   /* K scales of positions g and g + 8 */
+                    const uint32_t ka = sb + g * C::TILE / 16u + 2u * HD, kb = ka + 8u * (C::TILE / 16u);
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; b++) { k0[b] = lds32(ka + 4u * b); k1[b] = lds32(kb + 4u * b); }
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; b++) {
+                        uint32_t w[4], a0[4], a1[4];
+                        ldmatrix_x4(w, sb + mrow * (TILE / 16u) + (2u * b + mchunk) * 16u);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
+                        a0[0] = codes2<0x4140>(w[0]); a0[2] = codes2<0x4342>(w[0]); a0[1] = codes2<0x4140>(w[1]); a0[3] = codes2<0x4342>(w[1]);
+                        a1[0] = codes2<0x4140>(w[2]); a1[2] = codes2<0x4342>(w[2]); a1[1] = codes2<0x4140>(w[3]); a1[3] = codes2<0x4342>(w[3]);
+                        const float2 f0 = __half22float2(u2h(k0[b / 2])), f1 = __half22float2(u2h(k1[b / 2]));
+                        const float e0 = b & 1u ? f0.y : f0.x, e1 = b & 1u ? f1.y : f1.x;
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const uint32_t qa = s_q + (8u * n + g) * C::Q_STRIDE + b * 64u + t * 8u;
+                            const uint2 qx = lds64(qa), qy = lds64(qa + 32u);
+                            float c[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma16816(c, a0, qx.x, qx.y);
+                            mma16816(c, a1, qy.x, qy.y);
+                            sc[n][0] = fmaf(c[0], e0, sc[n][0]); sc[n][1] = fmaf(c[1], e0, sc[n][1]);
+                            sc[n][2] = fmaf(c[2], e1, sc[n][2]); sc[n][3] = fmaf(c[3], e1, sc[n][3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t ks = 0; ks < MT; ks++) {
+                        uint32_t a[4];
+                        const uint32_t c = 2u * ks + mchunk;
+                        ldmatrix_x4(a, sb + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const uint2 qx = lds64(s_q + (8u * n + g) * C::Q_STRIDE + ks * 32u + t * 8u);
+                            mma16816(sc[n], a, qx.x, qx.y);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sc[n][k] *= P.scale_log2e;
+                if (p0 + 16u > lim_min) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (p0 + g + (k >> 1) * 8u >= lim[n][k & 1]) sc[n][k] = -CUDART_INF_F;
+                }
+                /* ---- the maxima move only where a score is above them: seldom, after the first tiles */
+                bool grow = false;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) grow = grow || fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e];
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float x = fmaxf(sc[n][e], sc[n][e + 2]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            if (x > m[n][e]) {
+                                const float f = ex2(m[n][e] - x);
+                                m[n][e] = x;
+                                l[n][e] *= f;
+#pragma unroll
+                                for (uint32_t k = 0; k < MT; k++) { o[k][n][e] *= f; o[k][n][e + 2] *= f; }
+                            }
+                        }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float m0 = m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m1 = m[n][1] == -CUDART_INF_F ? 0.f : m[n][1];
+                    const float x0 = ex2(sc[n][0] - m0), x1 = ex2(sc[n][1] - m1), x2 = ex2(sc[n][2] - m0), x3 = ex2(sc[n][3] - m1);
+                    l[n][0] += x0 + x2;
+                    l[n][1] += x1 + x3;
+                    pb[n][0] = movmatrix_t(h2u(__floats2half2_rn(x0, x1)));
+                    pb[n][1] = movmatrix_t(h2u(__floats2half2_rn(x2, x3)));
+                }
+                /* ---- O^T += V^T P^T.  Rows behind the last position hold anything: 0 x NaN has to stay 0 */
+                const bool tail = p0 + 16u > n_kv;
+                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+                if (tail) {
+                    const uint32_t p = p0 + 2u * t;
+                    keep0 = (p < n_kv ? 0xffffu : 0u) | (p + 1u < n_kv ? 0xffff0000u : 0u);
+                    keep1 = (p + 8u < n_kv ? 0xffffu : 0u) | (p + 9u < n_kv ? 0xffff0000u : 0u);
+                }
+                if constexpr (KIND == Q4K_Q8) {
+                    constexpr uint32_t NB = HD / 32u;
+                    uint32_t v0[NB / 2], v1[NB / 2], v2[NB / 2], v3[NB / 2];   /* V scales of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9 */
+                    const uint32_t va = sb + 2u * t * (TILE / 16u) + 2u * HD + NB * 2u;
+#pragma unroll
+                    for (uint32_t b = 0; b < NB / 2; b++) {
+                        v0[b] = lds32(va + 4u * b); v1[b] = lds32(va + TILE / 16u + 4u * b);
+                        v2[b] = lds32(va + 8u * (TILE / 16u) + 4u * b); v3[b] = lds32(va + 9u * (TILE / 16u) + 4u * b);
+                    }
+#pragma unroll
+                    for (uint32_t b = 0; b < NB; b++) {
+                        const uint32_t sel = b & 1u ? 0x7632u : 0x5410u;
+                        const __half2 f0 = u2h(__byte_perm(v0[b / 2], v1[b / 2], sel) & keep0), f1 = u2h(__byte_perm(v2[b / 2], v3[b / 2], sel) & keep1);
+                        uint32_t w[4];
+                        ldmatrix_x4_trans(w, sb + mrow * (TILE / 16u) + HD + (2u * b + mchunk) * 16u);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
+#pragma unroll
+                        for (uint32_t c = 0; c < 2; c++) {
+                            /* dims 2 g (rows g) and 2 g + 1 (rows g + 8) of 16; fp16(code x scale): 2^-12 of a value on average, as P is rounded */
+                            uint32_t a[4] = {h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c])), f0)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c])), f0)),
+                                             h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c + 1])), f1)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c + 1])), f1))};
+#pragma unroll
+                            for (int n = 0; n < NT; n++) mma16816(o[2 * b + c][n], a, pb[n][0], pb[n][1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < MT; k++) {
+                        uint32_t w[4];
+                        const uint32_t c = 2u * k + mchunk;
+                        ldmatrix_x4_trans(w, sb + TILE / 2u + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
+                        uint32_t a[4] = {w[0], w[2], w[1], w[3]};
+                        if (tail) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
+#pragma unroll
+                        for (int n = 0; n < NT; n++) mma16816(o[k][n], a, pb[n][0], pb[n][1]);
+                    }
+                }
+            }
+            __syncwarp();   /* all lanes have read the slot */
+            if (ahead < n_my) issue();
+        }
+
+        /* ---- the warps' results are joined in pairs through shared memory (the rings are empty: all that was issued was taken) */
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+                l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+                l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+            }
+        float *xch = reinterpret_cast<float *>(base);
+#pragma unroll 1
+        for (uint32_t half = WARPS / 2u; half > 0; half >>= 1) {
+            __syncthreads();
+            if (warp >= half && warp < 2u * half) {
+                float *to = xch + (warp - half) * (C::FRAG / 4u) + lane;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) { to[(n * 4 + e) * 32] = m[n][e]; to[(n * 4 + 2 + e) * 32] = l[n][e]; }
+#pragma unroll
+                    for (uint32_t k = 0; k < MT; k++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) to[(NT * 4 + (n * MT + k) * 4 + e) * 32] = o[k][n][e];
+                }
+            }
+            __syncthreads();
+            if (warp < half) {
+                const float *from = xch + warp * (C::FRAG / 4u) + lane;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float mo = from[(n * 4 + e) * 32], lo = from[(n * 4 + 2 + e) * 32];
+                        const float M = fmaxf(m[n][e], mo), Mu = M == -CUDART_INF_F ? 0.f : M;
+                        const float fa = ex2(m[n][e] - Mu), fb = ex2(mo - Mu);
+                        m[n][e] = M;
+                        l[n][e] = l[n][e] * fa + lo * fb;
+#pragma unroll
+                        for (uint32_t k = 0; k < MT; k++) {
+                            o[k][n][e] = o[k][n][e] * fa + from[(NT * 4 + (n * MT + k) * 4 + e) * 32] * fb;
+                            o[k][n][e + 2] = o[k][n][e + 2] * fa + from[(NT * 4 + (n * MT + k) * 4 + e + 2) * 32] * fb;
+                        }
+                    }
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {   /* [row][hd + 4]: acc, m, l */
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float *rec = xch + (8u * n + 2u * t + e) * C::REC;
+#pragma unroll
+                    for (uint32_t k = 0; k < MT; k++) {
+                        rec[16u * k + (KIND == Q4K_Q8 ? 2u * g : g)] = o[k][n][e];
+                        rec[16u * k + (KIND == Q4K_Q8 ? 2u * g + 1u : g + 8u)] = o[k][n][e + 2];
+                    }
+                    if (g == 0) { rec[HD] = m[n][e]; rec[HD + 1] = l[n][e]; }
+                }
+        }
+        __syncthreads();
+        const bool whole = st == 0u && here == n_steps;
+        float *part = P.part + ((size_t)blockIdx.x * 2u + (st == 0u ? 1u : 0u)) * C::ROWS * C::REC;
+        for (uint32_t i = tid; i < live_rows * (HD / 4u); i += C::THREADS) {
+            const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
+            const float *rec = xch + row * C::REC;
+            float4 x = *reinterpret_cast<const float4 *>(rec + d);
+            const float L = rec[HD + 1];
+            if (whole) {
+                const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+                const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
+                x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+                if (P.gate) {
+                    const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
+                    x.x *= 1.f / (1.f + __expf(-gt.x)); x.y *= 1.f / (1.f + __expf(-gt.y));
+                    x.z *= 1.f / (1.f + __expf(-gt.z)); x.w *= 1.f / (1.f + __expf(-gt.w));
+                }
+                if (P.out_bf16) {
+                    const __nv_bfloat162 b0 = __floats2bfloat162_rn(x.x, x.y), b1 = __floats2bfloat162_rn(x.z, x.w);
+                    *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
+                } else {
+                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = x;
+                }
+            } else {
+                *reinterpret_cast<float4 *>(part + row * C::REC + d) = x;
+                if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(rec[HD], L);
+            }
+        }
+        if (st > 0u && st + here == n_steps) {   /* the unit ends here; it began in block .. */
+            const uint64_t first = s - st;
+            end_of = make_int4((int32_t)(((first + 1u) * blocks - 1u) / total), (int32_t)tok0, (int32_t)live_rows, (int32_t)kh);
+        }
+        s += here;
+        off += here;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   /* the next bulk copies overwrite what was stored here */
+    }
+    if (tid == 0) P.ends[blockIdx.x] = end_of;
+    if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
+        if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
+        for (; taken < issued; taken++)
+            for (uint32_t i = 0; i < 4096u && !bar_test(bars + 8u * (taken % DEPTH), (taken / DEPTH) & 1u); i++) {}
+    }
+}
+
+/* Joins the records of the unit that ends in block blockIdx.x, row blockIdx.y of its group: a lane has 4 dims, the warps
+ * share out the records. */
+template <int HD>
+__global__ void __launch_bounds__(256) q4_pg_merge_k(const PagedParams P, uint32_t rows_max) {
+    constexpr uint32_t LANES = HD / 4u, SETS = 256u / LANES, REC = HD + 4u;
+    __shared__ float4 s_acc[SETS][LANES];
+    __shared__ float2 s_ml[SETS];
+    q4d_pdl_wait();
+    const int4 e = P.ends[blockIdx.x];
+    const uint32_t row = blockIdx.y, last = blockIdx.x;
+    if (e.x < 0 || row >= (uint32_t)e.z) return;
+    const uint32_t set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u, first = (uint32_t)e.x;
+    float M = -CUDART_INF_F, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto join = [&](float m, float l, float4 x) {
+        const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m - Mu);
+        M = Mn;
+        L = L * fa + l * fb;
+        A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
+    };
+#pragma unroll 4
+    for (uint32_t c = first + set; c <= last; c += SETS) {
+        const float *rec = P.part + (((size_t)c * 2u + (c == first ? 1u : 0u)) * rows_max + row) * REC;
+        const float2 ml = *reinterpret_cast<const float2 *>(rec + HD);
+        const float4 x = *reinterpret_cast<const float4 *>(rec + d);
+        join(ml.x, ml.y, x);
+    }
+    s_acc[set][d / 4u] = A;
+    if (d == 0u) s_ml[set] = make_float2(M, L);
+    __syncthreads();
+    if (set) return;
+    for (uint32_t k = 1; k < SETS; k++) join(s_ml[k].x, s_ml[k].y, s_acc[k][d / 4u]);
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const uint32_t kh = (uint32_t)e.w;
+    const size_t at = ((size_t)((uint32_t)e.y + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
+    A.x *= inv; A.y *= inv; A.z *= inv; A.w *= inv;
+    if (P.gate) {
+        const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
+        A.x *= 1.f / (1.f + __expf(-gt.x)); A.y *= 1.f / (1.f + __expf(-gt.y));
+        A.z *= 1.f / (1.f + __expf(-gt.z)); A.w *= 1.f / (1.f + __expf(-gt.w));
+    }
+    if (P.out_bf16) {
+        const __nv_bfloat162 b0 = __floats2bfloat162_rn(A.x, A.y), b1 = __floats2bfloat162_rn(A.z, A.w);
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
+    } else {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = A;
+    }
+}
+
+template <int KIND, int HD, int NT>
+bool few(PagedParams &p) {
+    using C = FewCfg<KIND, HD, NT>;
+    static bool attr = false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_few_k<KIND, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
+    attr = true;
+    const uint32_t blocks = (uint32_t)g_q4.sm_count * C::CTAS;
+    const size_t recs = (size_t)blocks * 2u * C::ROWS * C::REC;
+    if (!q4i_scratch(recs + (size_t)blocks * 4u, 0)) return false;
+    p.part = g_q4.part;
+    p.ends = reinterpret_cast<int4 *>(g_q4.part + recs);
+    p.tpg = C::ROWS / p.gqa;
+    return q4i_launch_pdl("pages_attend launch", q4_pg_few_k<KIND, HD, NT>, dim3(blocks), C::THREADS, C::SMEM, p) &&
+           q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<HD>, dim3(blocks, C::ROWS), 256u, 0, p, C::ROWS);
+}
+template <int KIND, int HD>
+bool few_by_rows(PagedParams &p, uint32_t rows) {
+    if (rows <= 8u) return few<KIND, HD, 1>(p);
+    if (rows <= 16u || HD == 256) return few<KIND, HD, 2>(p);
+    return few<KIND, HD, HD == 256 ? 2 : 4>(p);
+}
+bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
+
+}  // namespace
+
+extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, int q_bf16, const float *gate, void *out, int out_bf16,
+                                    uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
+                                    uint32_t table_stride, uint32_t max_add, float scale) {
+    if (!g_q4.ok) return q4i_fail(Q4E_INIT, "pages_attend: library not initialised");
+    Q4_REQUIRE(q4i_pages_ok(pg) && pg->mem && aligned16(pg->mem) && layer < pg->n_layers, "pages_attend: bad pool or layer");
+    Q4_REQUIRE(q && out && rows && start && table && n_req && n_tok && table_stride && n_head, "pages_attend: bad argument");
+    Q4_REQUIRE(n_head % pg->n_kvh == 0 && n_head / pg->n_kvh <= 16, "pages_attend: n_head/n_kvh must be 1..16");
+    Q4_REQUIRE(aligned16(q) && aligned16(gate) && aligned16(out), "pages_attend: q, gate and out must be 16-byte aligned");
+    Q4_REQUIRE(scale > 0.f, "pages_attend: scale must be positive");
+    Q4_REQUIRE(n_tok <= 0x7fffffffu && (uint64_t)table_stride * pg->page_rows <= 0x7fffffffu, "pages_attend: a block table's rows pass 2^31 - 1");
+    PagedParams p = {};
+    const uint32_t row = q4i_pages_row_bytes(pg->hd, pg->kind);
+    p.part_bytes = row * pg->page_rows;
+    p.page_bytes = (uint64_t)p.part_bytes * pg->n_kvh;
+    p.mem = (const uint8_t *)pg->mem + (uint64_t)layer * p.page_bytes * pg->n_pages;
+    p.n_pages = pg->n_pages; p.page_shift = (uint32_t)__builtin_ctz(pg->page_rows);
+    p.n_kvh = pg->n_kvh; p.n_head = n_head; p.gqa = n_head / pg->n_kvh;
+    p.rows = rows; p.start = start; p.table = table; p.table_stride = table_stride; p.n_req = n_req; p.n_tok = n_tok;
+    p.q = q; p.q_bf16 = q_bf16; p.gate = gate; p.out = out; p.out_bf16 = out_bf16;
+    p.scale_log2e = scale * 1.4426950408889634f;
+    p.err = g_q4.err_d;
+    const uint64_t most = (uint64_t)(max_add && max_add < n_tok ? max_add : n_tok) * p.gqa;
+    const uint32_t want = most < 64u ? (uint32_t)most : 64u;
+    if (pg->kind == Q4K_Q8) return pg->hd == 64 ? few_by_rows<Q4K_Q8, 64>(p, want) : pg->hd == 128 ? few_by_rows<Q4K_Q8, 128>(p, want) : few_by_rows<Q4K_Q8, 256>(p, want);
+    return pg->hd == 64 ? few_by_rows<Q4K_F16, 64>(p, want) : pg->hd == 128 ? few_by_rows<Q4K_F16, 128>(p, want) : few_by_rows<Q4K_F16, 256>(p, want);
+}

@@ -93,7 +93,20 @@ SIGNATURES = {
     "q4_gpu_batch_decode": (_b, [_v, _u32, _v, _i, _v, _v, _v, _u32, _u32, _u32, _u32, _f]),
     "q4_gpu_batch_append_decode": (_b, [_v, _u32, _v, _v, _v, _i, _v, _v, _v, _u32, _u32, _u32, _u32, _f]),
     "q4_gpu_kv_append_decode_d": (_b, [_v, _u32, _v, _v, _v, _i, _v, _v, _u32, _v, _u32, _u32, _f]),
+    "q4_gpu_pages_bytes": (_u64, [_u32, _u32, _u32, _u32, _u32, _i]),
+    "q4_gpu_pages_plan": (_b, [_v, _v, _v, _u32, _v, _u32, _v, _v, _v, _v, _u32]),
+    "q4_gpu_pages_trim": (_b, [_v, _v, _v, _u32, _v, _u32]),
+    "q4_gpu_pages_append": (_b, [_v, _u32, _v, _v, _v, _u32]),
+    "q4_gpu_pages_gather": (_b, [_v, _u32, _v, _u32, _v, _v]),
+    "q4_gpu_pages_attend": (_b, [_v, _u32, _v, _i, _v, _v, _i, _u32, _v, _v, _u32, _u32, _v, _u32, _u32, _f]),
 }
+
+
+class PagesDesc(C.Structure):
+    """q4_gpu_pages of include/q4_gpu.h: a pool of pages in the caller's memory"""
+    _fields_ = [("mem", C.c_void_p), ("free_list", C.c_void_p), ("n_free", C.c_void_p), ("n_layers", C.c_uint32), ("n_kvh", C.c_uint32),
+                ("hd", C.c_uint32), ("n_pages", C.c_uint32), ("page_rows", C.c_uint32), ("kind", C.c_int)]
+
 
 class SessDesc(C.Structure):
     """q4_gpu_sess_desc of include/q4_gpu.h: the host's part of a version-5 session file"""
@@ -379,3 +392,53 @@ class Batch:
         check(self.L.q4_gpu_batch_append_decode(self.h, layer, _ptr(k), _ptr(v), _ptr(q), int(q_bf16), _ptr(gate),
                                                 _ptr(out), _ptr(idx), width, idx_kvh_stride, idx_sess_stride,
                                                 n_head, scale), "q4_gpu_batch_append_decode")
+
+
+class PagePool:
+    """A paged KV cache for many requests (q4_gpu_pages_*).  Arrays are torch tensors on the device; the pool's memory and its stack
+    of free pages are allocated here unless they are given.  Per step: plan, then append and attend for every layer."""
+
+    def __init__(self, n_layers, n_kvh, hd, n_pages, page_rows=64, kind=KIND_Q8, mem=None, free=None, n_free=None):
+        import torch
+        self.L = init()
+        size = self.L.q4_gpu_pages_bytes(n_layers, n_kvh, hd, n_pages, page_rows, kind)
+        if not size:
+            raise RuntimeError("q4_gpu_pages_bytes: a pool of kind f16 or q8_0, hd 64 / 128 / 256, page_rows 16 .. 256 is needed")
+        on = torch.device("cuda", self.L.q4_gpu_device())
+        own_mem = free is None and mem is None
+        if own_mem:
+            mem = torch.empty(size, dtype=torch.uint8, device=on)
+            free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=on)   # page 0 is on top
+            n_free = torch.full((1,), n_pages, dtype=torch.int32, device=on)
+        if mem is not None and mem.numel() * mem.element_size() < size:
+            raise RuntimeError("the pool's memory is smaller than q4_gpu_pages_bytes (%d)" % size)
+        self.mem, self.free, self.n_free = mem, free, n_free
+        self.n_layers, self.n_kvh, self.hd, self.n_pages, self.page_rows, self.kind = n_layers, n_kvh, hd, n_pages, page_rows, kind
+        self.desc = PagesDesc(_ptr(mem), _ptr(free), _ptr(n_free), n_layers, n_kvh, hd, n_pages, page_rows, kind)
+        self.p = C.addressof(self.desc)
+
+    def plan(self, rows, add, table, start, slot, pos, req):
+        """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok]"""
+        n, stride = table.shape
+        check(self.L.q4_gpu_pages_plan(self.p, _ptr(rows), _ptr(add), n, _ptr(table), stride, _ptr(start), _ptr(slot), _ptr(pos),
+                                       _ptr(req), slot.shape[0]), "q4_gpu_pages_plan")
+
+    def trim(self, rows, keep, table):
+        """the pages behind the first keep[r] of rows[r] rows go back"""
+        n, stride = table.shape
+        check(self.L.q4_gpu_pages_trim(self.p, _ptr(rows), _ptr(keep), n, _ptr(table), stride), "q4_gpu_pages_trim")
+
+    def append(self, layer, k, v, slot):
+        check(self.L.q4_gpu_pages_append(self.p, layer, _ptr(k), _ptr(v), _ptr(slot), slot.shape[0]), "q4_gpu_pages_append")
+
+    def gather(self, layer, slot, k, v):
+        check(self.L.q4_gpu_pages_gather(self.p, layer, _ptr(slot), slot.shape[0], _ptr(k), _ptr(v)), "q4_gpu_pages_gather")
+
+    def attend(self, layer, q, out, rows, start, table, n_head, scale, gate=None, max_add=0):
+        """attention of the step's tokens: q, out [n_tok][n_head][hd], bf16 or fp32; rows as they were given to plan"""
+        import torch
+        n, stride = table.shape
+        n_tok = q.numel() // (n_head * self.hd)
+        check(self.L.q4_gpu_pages_attend(self.p, layer, _ptr(q), q.dtype == torch.bfloat16, _ptr(gate), _ptr(out),
+                                         out.dtype == torch.bfloat16, n_head, _ptr(rows), _ptr(start), n, n_tok, _ptr(table), stride,
+                                         max_add, scale), "q4_gpu_pages_attend")
