@@ -18,28 +18,11 @@
 #include <math_constants.h>
 #include <string.h>
 
-#include "q4_internal.h"
+#include "q4_paged.h"
 
 namespace {
 
 constexpr uint32_t PG_SPIN_LIMIT = 1u << 20;
-
-struct PagedParams {
-    const uint8_t *mem;          /* of the layer */
-    uint64_t page_bytes;         /* of all kv heads */
-    uint32_t part_bytes;         /* of one kv head */
-    uint32_t n_pages, page_shift, n_kvh, n_head, gqa, tpg /* tokens per group */;
-    const int32_t *rows, *start, *table;
-    uint32_t table_stride, n_req, n_tok;
-    const void *q;
-    const float *gate;
-    void *out;
-    int q_bf16, out_bf16;
-    float scale_log2e;
-    float *part;                 /* [block][2][rows of a group][hd + 4] */
-    int4 *ends;                  /* [block] {first block of the unit that ends here, or -1; its first token; its rows; its kv head} */
-    uint32_t *err;
-};
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ float ex2(float x) {
@@ -93,10 +76,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
     return h2u(__hsub2(u2h(__byte_perm(x, 0x64646464u, SEL)), u2h(0x64806480u)));
 }
 
-template <int KIND, int HD>
-struct PgTile {
-    static constexpr uint32_t ROW = KIND == Q4K_Q8 ? (2u * HD + HD / 8u + 15u) / 16u * 16u : 4u * HD, BYTES = 16u * ROW;
-};
 /* warps per block, blocks per SM, tiles of a warp's ring: as many bytes in flight as an SM's shared memory holds */
 template <int KIND, int HD, int NT>
 struct FewCfg {
@@ -116,19 +95,23 @@ struct FewCfg {
     static constexpr uint32_t SMEM = RING + ROWS * Q_STRIDE + WARPS * DEPTH * 8u + 1024u;
 };
 
-/* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */
-struct PgReq { uint32_t held, add, tok0; };
-__device__ __forceinline__ PgReq pg_request(const PagedParams &P, uint32_t r, bool &bad) {
-    const int32_t s0 = P.start[r], s1 = P.start[r + 1u], h = P.rows[r];
-    PgReq q = {0u, 0u, 0u};
-    bad = false;
-    if (s1 <= s0) return q;
-    if (h < 0 || s0 < 0 || (uint32_t)s1 > P.n_tok || (uint64_t)(uint32_t)h + (uint32_t)(s1 - s0) > ((uint64_t)P.table_stride << P.page_shift)) {
-        bad = true;
-        return q;
+/* four dims of a row: acc / l * sigmoid(gate).  A row that attended nothing is 0, one with a NaN among its scores stays NaN */
+template <int HD>
+__device__ __forceinline__ void pg_store(const PagedParams &P, uint32_t tok, uint32_t head, uint32_t d, float4 x, float L) {
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const size_t at = ((size_t)tok * P.n_head + head) * HD + d;
+    x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+    if (P.gate) {
+        const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
+        x.x *= 1.f / (1.f + __expf(-gt.x)); x.y *= 1.f / (1.f + __expf(-gt.y));
+        x.z *= 1.f / (1.f + __expf(-gt.z)); x.w *= 1.f / (1.f + __expf(-gt.w));
     }
-    q.held = (uint32_t)h; q.add = (uint32_t)(s1 - s0); q.tok0 = (uint32_t)s0;
-    return q;
+    if (P.out_bf16) {
+        const __nv_bfloat162 b0 = __floats2bfloat162_rn(x.x, x.y), b1 = __floats2bfloat162_rn(x.z, x.w);
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
+    } else {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = x;
+    }
 }
 
 template <int KIND, int HD, int NT>
@@ -149,8 +132,13 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     q4d_pdl_wait();
 
     /* ---- this block's share of all steps */
+    auto mine_of = [&](uint32_t r, bool &bad) -> PgReq {
+        PgReq q = pg_request(P, r, bad);
+        if (q.add > P.add_split) q.add = 0u;
+        return q;
+    };
     auto steps_of = [&](uint32_t r, bool &bad) -> uint64_t {
-        const PgReq q = pg_request(P, r, bad);
+        const PgReq q = mine_of(r, bad);
         return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh * ((q.held + q.add + STEP - 1u) / STEP);   /* no tokens: 0 groups */
     };
     const uint32_t per = (P.n_req + C::THREADS - 1u) / C::THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
@@ -202,7 +190,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
 
     /* ---- pieces of units */
     while (s < s_end) {
-        const PgReq R = pg_request(P, req, bad);
+        const PgReq R = mine_of(req, bad);
         const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = (R.held + R.add + STEP - 1u) / STEP;
         if (off >= (uint64_t)groups * P.n_kvh * n_steps) {   /* on to the next request; requests without tokens are passed over */
             off -= (uint64_t)groups * P.n_kvh * n_steps;
@@ -515,23 +503,10 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         for (uint32_t i = tid; i < live_rows * (HD / 4u); i += C::THREADS) {
             const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
             const float *rec = xch + row * C::REC;
-            float4 x = *reinterpret_cast<const float4 *>(rec + d);
+            const float4 x = *reinterpret_cast<const float4 *>(rec + d);
             const float L = rec[HD + 1];
             if (whole) {
-                const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-                const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
-                x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
-                if (P.gate) {
-                    const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
-                    x.x *= 1.f / (1.f + __expf(-gt.x)); x.y *= 1.f / (1.f + __expf(-gt.y));
-                    x.z *= 1.f / (1.f + __expf(-gt.z)); x.w *= 1.f / (1.f + __expf(-gt.w));
-                }
-                if (P.out_bf16) {
-                    const __nv_bfloat162 b0 = __floats2bfloat162_rn(x.x, x.y), b1 = __floats2bfloat162_rn(x.z, x.w);
-                    *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
-                } else {
-                    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = x;
-                }
+                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, x, L);
             } else {
                 *reinterpret_cast<float4 *>(part + row * C::REC + d) = x;
                 if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(rec[HD], L);
@@ -539,7 +514,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         }
         if (st > 0u && st + here == n_steps) {   /* the unit ends here; it began in block .. */
             const uint64_t first = s - st;
-            end_of = make_int4((int32_t)(((first + 1u) * blocks - 1u) / total), (int32_t)tok0, (int32_t)live_rows, (int32_t)kh);
+            end_of = make_int4((int32_t)(((first + 1u) * blocks - 1u) / total), (int32_t)tok0, (int32_t)n_here, (int32_t)kh);
         }
         s += here;
         off += here;
@@ -553,79 +528,87 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     }
 }
 
-/* Joins the records of the unit that ends in block blockIdx.x, row blockIdx.y of its group: a lane has 4 dims, the warps
- * share out the records. */
+/* Joins the records of the unit that ends in block blockIdx.x: 4 dims per thread, so that 256 threads have SETS rows at a time;
+ * where a unit lies in many blocks, one row, whose records they share out. */
 template <int HD>
-__global__ void __launch_bounds__(256) q4_pg_merge_k(const PagedParams P, uint32_t rows_max) {
+__global__ void __launch_bounds__(256) q4_pg_merge_k(const PagedParams P, uint32_t unit_rows) {
     constexpr uint32_t LANES = HD / 4u, SETS = 256u / LANES, REC = HD + 4u;
     __shared__ float4 s_acc[SETS][LANES];
     __shared__ float2 s_ml[SETS];
     q4d_pdl_wait();
     const int4 e = P.ends[blockIdx.x];
-    const uint32_t row = blockIdx.y, last = blockIdx.x;
-    if (e.x < 0 || row >= (uint32_t)e.z) return;
-    const uint32_t set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u, first = (uint32_t)e.x;
-    float M = -CUDART_INF_F, L = 0.f;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto join = [&](float m, float l, float4 x) {
-        const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m - Mu);
-        M = Mn;
-        L = L * fa + l * fb;
-        A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
-    };
+    const uint32_t first = (uint32_t)e.x, last = blockIdx.x;
+    if (e.x < 0) return;
+    const uint32_t set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u;
+    const bool wide = last - first >= 2u * SETS;   /* 18 records and more at hd 128 */
+    const uint32_t at_once = wide ? 1u : SETS, step = wide ? SETS : 1u;
+    for (uint32_t r0 = blockIdx.y * at_once; r0 < unit_rows; r0 += gridDim.y * at_once) {
+        const uint32_t row = wide ? r0 : r0 + set, group = row / P.group_rows, in = row - group * P.group_rows, tl = in / P.gqa, tok = group * P.tpg + tl;
+        const bool live = row < unit_rows && tl < P.tpg && tok < (uint32_t)e.z;
+        float M = -CUDART_INF_F, L = 0.f;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto join = [&](float m, float l, float4 x) {
+            const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m - Mu);
+            M = Mn;
+            L = L * fa + l * fb;
+            A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
+        };
+        if (live) {
 #pragma unroll 4
-    for (uint32_t c = first + set; c <= last; c += SETS) {
-        const float *rec = P.part + (((size_t)c * 2u + (c == first ? 1u : 0u)) * rows_max + row) * REC;
-        const float2 ml = *reinterpret_cast<const float2 *>(rec + HD);
-        const float4 x = *reinterpret_cast<const float4 *>(rec + d);
-        join(ml.x, ml.y, x);
-    }
-    s_acc[set][d / 4u] = A;
-    if (d == 0u) s_ml[set] = make_float2(M, L);
-    __syncthreads();
-    if (set) return;
-    for (uint32_t k = 1; k < SETS; k++) join(s_ml[k].x, s_ml[k].y, s_acc[k][d / 4u]);
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    const uint32_t kh = (uint32_t)e.w;
-    const size_t at = ((size_t)((uint32_t)e.y + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
-    A.x *= inv; A.y *= inv; A.z *= inv; A.w *= inv;
-    if (P.gate) {
-        const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
-        A.x *= 1.f / (1.f + __expf(-gt.x)); A.y *= 1.f / (1.f + __expf(-gt.y));
-        A.z *= 1.f / (1.f + __expf(-gt.z)); A.w *= 1.f / (1.f + __expf(-gt.w));
-    }
-    if (P.out_bf16) {
-        const __nv_bfloat162 b0 = __floats2bfloat162_rn(A.x, A.y), b1 = __floats2bfloat162_rn(A.z, A.w);
-        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
-    } else {
-        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = A;
+            for (uint32_t c = first + (wide ? set : 0u); c <= last; c += step) {
+                const float *rec = P.part + (((size_t)c * 2u + (c == first ? 1u : 0u)) * unit_rows + row) * REC;
+                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(rec + HD));
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(rec + d));
+                join(ml.x, ml.y, x);
+            }
+        }
+        if (wide) {
+            __syncthreads();   /* the row before has been joined */
+            s_acc[set][d / 4u] = A;
+            if (d == 0u) s_ml[set] = make_float2(M, L);
+            __syncthreads();
+            if (set) continue;
+            for (uint32_t k = 1; k < SETS; k++) join(s_ml[k].x, s_ml[k].y, s_acc[k][d / 4u]);
+        }
+        if (live) pg_store<HD>(P, (uint32_t)e.y + tok, (uint32_t)e.w * P.gqa + in - tl * P.gqa, d, A, L);
     }
 }
 
 template <int KIND, int HD, int NT>
-bool few(PagedParams &p) {
+bool few(PagedParams &p, float *scratch) {
     using C = FewCfg<KIND, HD, NT>;
     static bool attr = false;
     if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_few_k<KIND, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
     attr = true;
     const uint32_t blocks = (uint32_t)g_q4.sm_count * C::CTAS;
     const size_t recs = (size_t)blocks * 2u * C::ROWS * C::REC;
-    if (!q4i_scratch(recs + (size_t)blocks * 4u, 0)) return false;
-    p.part = g_q4.part;
-    p.ends = reinterpret_cast<int4 *>(g_q4.part + recs);
+    if (!scratch) {
+        if (!q4i_scratch(recs + (size_t)blocks * 4u, 0)) return false;
+        scratch = g_q4.part;
+    }
+    p.part = scratch;
+    p.ends = reinterpret_cast<int4 *>(scratch + recs);
     p.tpg = C::ROWS / p.gqa;
-    return q4i_launch_pdl("pages_attend launch", q4_pg_few_k<KIND, HD, NT>, dim3(blocks), C::THREADS, C::SMEM, p) &&
-           q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<HD>, dim3(blocks, C::ROWS), 256u, 0, p, C::ROWS);
+    p.group_rows = C::ROWS;
+    return q4i_launch_pdl("pages_attend launch", q4_pg_few_k<KIND, HD, NT>, dim3(blocks), C::THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
 }
 template <int KIND, int HD>
-bool few_by_rows(PagedParams &p, uint32_t rows) {
-    if (rows <= 8u) return few<KIND, HD, 1>(p);
-    if (rows <= 16u || HD == 256) return few<KIND, HD, 2>(p);
-    return few<KIND, HD, HD == 256 ? 2 : 4>(p);
+bool few_by_rows(PagedParams &p, uint32_t rows, float *scratch) {
+    if (rows <= 8u) return few<KIND, HD, 1>(p, scratch);
+    if (rows <= 16u || HD == 256) return few<KIND, HD, 2>(p, scratch);
+    return few<KIND, HD, HD == 256 ? 2 : 4>(p, scratch);
 }
 bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 
 }  // namespace
+
+bool q4i_paged_merge(const PagedParams &p, uint32_t hd, uint32_t blocks, uint32_t unit_rows) {
+    const uint32_t at_once = 1024u / hd, y = unit_rows / at_once < 16u ? unit_rows / at_once : 16u;
+    const dim3 grid(blocks, y < 8u ? 8u : y);
+    if (hd == 64) return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<64>, grid, 256u, 0, p, unit_rows);
+    if (hd == 128) return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<128>, grid, 256u, 0, p, unit_rows);
+    return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<256>, grid, 256u, 0, p, unit_rows);
+}
 
 extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, int q_bf16, const float *gate, void *out, int out_bf16,
                                     uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
@@ -648,8 +631,22 @@ extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, cons
     p.q = q; p.q_bf16 = q_bf16; p.gate = gate; p.out = out; p.out_bf16 = out_bf16;
     p.scale_log2e = scale * 1.4426950408889634f;
     p.err = g_q4.err_d;
-    const uint64_t most = (uint64_t)(max_add && max_add < n_tok ? max_add : n_tok) * p.gqa;
-    const uint32_t want = most < 64u ? (uint32_t)most : 64u;
-    if (pg->kind == Q4K_Q8) return pg->hd == 64 ? few_by_rows<Q4K_Q8, 64>(p, want) : pg->hd == 128 ? few_by_rows<Q4K_Q8, 128>(p, want) : few_by_rows<Q4K_Q8, 256>(p, want);
-    return pg->hd == 64 ? few_by_rows<Q4K_F16, 64>(p, want) : pg->hd == 128 ? few_by_rows<Q4K_F16, 128>(p, want) : few_by_rows<Q4K_F16, 256>(p, want);
+    const uint32_t most = max_add && max_add < n_tok ? max_add : n_tok;
+    uint32_t few_rows = (uint32_t)(most * (uint64_t)p.gqa < 64u ? most * p.gqa : 64u);   /* (token, head) pairs that q4_pg_few_k takes at once */
+    float *scratch = nullptr;
+    p.add_split = 0xffffffffu;
+    if (few_rows > (pg->hd == 256 ? 16u : 32u)) {
+        /* requests that bring more than fits the smallest tile go to the tensor cores; a single request in any case */
+        few_rows = p.gqa <= 8u ? 8u : 16u;
+        p.add_split = n_req == 1u ? 0u : few_rows / p.gqa;
+        /* records of both kernels: the second's must not fall on the first's while those are joined */
+        const size_t chunk = q4i_paged_chunk_floats(pg->hd), rest = (size_t)g_q4.sm_count * 2u * (2u * 32u * (256u + 4u) + 4u);
+        if (!q4i_scratch(chunk + rest, 0)) return false;
+        if (!q4i_paged_chunk(p, pg->kind, pg->hd, g_q4.part)) return false;
+        if (n_req == 1u) return true;
+        scratch = g_q4.part + chunk;
+    }
+    if (pg->kind == Q4K_Q8)
+        return pg->hd == 64 ? few_by_rows<Q4K_Q8, 64>(p, few_rows, scratch) : pg->hd == 128 ? few_by_rows<Q4K_Q8, 128>(p, few_rows, scratch) : few_by_rows<Q4K_Q8, 256>(p, few_rows, scratch);
+    return pg->hd == 64 ? few_by_rows<Q4K_F16, 64>(p, few_rows, scratch) : pg->hd == 128 ? few_by_rows<Q4K_F16, 128>(p, few_rows, scratch) : few_by_rows<Q4K_F16, 256>(p, few_rows, scratch);
 }

@@ -1,0 +1,807 @@
+/*
+ * Attention of chunks of new tokens over a pool of pages on the tensor cores (tcgen05.mma, accumulators in tensor memory): the
+ * requests that bring more tokens than q4_pg_few_k takes at once.  Token j of request r attends [0, rows[r] + j].
+ *
+ * One block per SM, each with an equal share of the step's work: the tiles of 128 positions of all units (request, kv head, group of
+ * tokens) one behind the other, cut into as many shares as there are blocks.  Lengths are read from the device.  A unit's
+ * tokens fill the rows of the products: 2 x 128 (token, head) pairs at hd 64 and 128, 128 at hd 256 (whose outputs take half
+ * of tensor memory).  What a share holds of a unit is a piece; a piece that is not the whole unit leaves (acc, m, l) records.
+ *
+ *   warps 0 - 7    softmax: thread r owns row r (hd 256: two threads, half of a unit's positions each): its scores out of tensor
+ *                  memory, causal mask, running maximum with lazy rescale, weights as fp16 back into the columns they came from
+ *   warps 8 - 11   producers: K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads
+ *                  them: bulk copies.  q8_0: codes and scales into registers, a slot ahead of their use, fp16(code x scale) into
+ *                  the slot (7 instructions per 4 values: a fifth of the issue slots that the products leave)
+ *   warp 12        issues the products: O += P V of a unit of positions as its weights appear, then the scores that take over the
+ *                  buffer
+ * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
+ *
+ * Every wait is bounded: on expiry the block's waits all end, Q4E_CUDA is set, and tensor memory is freed.
+ */
+#include <cuda_bf16.h>
+#include <math_constants.h>
+#include <string.h>
+
+#include "q4_paged.h"
+#include "q4_tc.h"
+
+using namespace q4tc;
+
+namespace {
+
+constexpr uint32_t CK_THREADS = 512, CK_BN = 128;
+constexpr uint32_t CK_SPIN_LIMIT = 1u << 22;
+constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
+constexpr uint32_t PIECES = 4;          /* pieces that are walked ahead */
+constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the reference moves */
+
+template <int HD>
+struct ChunkCfg {
+    static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
+    static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : 5u;
+    static constexpr uint32_t PARTS = HD == 256 ? 2u : 1u;        /* slots of a K or a V tile: K by 128 dims, V by 64 positions */
+    static constexpr uint32_t QG = 128u * HD * 2u;                /* one group's queries */
+    static constexpr uint32_t REC = HD + 4u;
+    static constexpr uint32_t BARS = 768u + (NQ == 1u ? 1024u : 0u);
+    static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + BARS + 1024u;
+    static constexpr uint32_t UN = NQ == 2u ? 64u : 128u;         /* positions of a unit of scores */
+    static_assert(SMEM <= 232448u, "shared memory");
+};
+
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t block_bytes) {
+    /* dims contiguous: blocks of 64 dims (block_bytes apart), in them rows of 128 bytes per position, swizzled in groups of eight
+     * (1024 bytes apart) */
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+/* fp16 1024 + 128 + code has (code ^ 0x80) in its low byte: two bytes picked out of word x (its codes ^ 0x80) become the exact codes */
+template <uint32_t SEL>
+__device__ __forceinline__ __half2 codes2(uint32_t x) {
+    const uint32_t u = __byte_perm(x, 0x64646464u, SEL), off = 0x64806480u;
+    return __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&off));
+}
+
+/* the rest of a wait whose first test found the phase incomplete (in line: ptxas does not allocate calls beside setmaxnreg) */
+__device__ __forceinline__ bool ck_wait_on(uint32_t bar, uint32_t parity, uint32_t s_abort) {
+    const unsigned long long t0 = global_ns();
+    for (uint32_t i = 0; i < CK_SPIN_LIMIT; i++) {
+        if (mbar_test<OWN>(bar, parity)) return true;
+        if ((i & 63u) == 63u) {
+            uint32_t a;
+            asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(a) : "r"(s_abort) : "memory");
+            if (a) return false;
+            if (global_ns() - t0 > CK_LIMIT_NS) break;
+        }
+    }
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(1u) : "memory");
+    return false;
+}
+/* by a whole warp, which goes on as one */
+__device__ __forceinline__ bool ck_all_wait(uint32_t bar, uint32_t parity, uint32_t s_abort) {
+    if (__builtin_expect(__all_sync(0xffffffffu, mbar_test<OWN>(bar, parity)), 1)) return true;
+    return __all_sync(0xffffffffu, ck_wait_on(bar, parity, s_abort));
+}
+
+/* sum of floor((a i + b) / m) over i < n (Euclid's steps on a and m) */
+__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
+    uint64_t r = 0;
+    while (n) {
+        if (a >= m) { r += (n - 1u) * n / 2u * (a / m); a %= m; }
+        if (b >= m) { r += n * (b / m); b %= m; }
+        const uint64_t y = (uint64_t)a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const uint32_t t = m;
+        m = a;
+        a = t;
+    }
+    return r;
+}
+/* tiles of a unit, and of the first g of a request's units on one kv head */
+__device__ __forceinline__ uint32_t unit_tiles(const PgReq &R, uint32_t tpu, uint32_t g) {
+    return (R.held + min((uint32_t)min((uint64_t)(g + 1u) * tpu, (uint64_t)R.add), R.add) + CK_BN - 1u) / CK_BN;
+}
+__device__ __forceinline__ uint64_t tiles_before(const PgReq &R, uint32_t tpu, uint32_t g) { return floor_sum(g, CK_BN, tpu, (uint64_t)R.held + tpu + CK_BN - 1u); }   /* g below the last */
+__device__ __forceinline__ PgReq chunk_request(const PagedParams &P, uint32_t r, bool &bad) {
+    PgReq q = pg_request(P, r, bad);
+    if (q.add <= P.add_split) q.add = 0u;
+    return q;
+}
+__device__ __forceinline__ uint64_t request_tiles(const PagedParams &P, const PgReq &R, uint32_t tpu) {
+    if (!R.add) return 0u;
+    const uint32_t groups = (R.add + tpu - 1u) / tpu;
+    return (tiles_before(R, tpu, groups - 1u) + unit_tiles(R, tpu, groups - 1u)) * P.n_kvh;
+}
+
+/* A share's pieces, one after the other: one warp walks them ahead of the others and leaves them in shared memory */
+struct Piece {
+    uint32_t before;             /* rows of the request before the unit's first token: it attends those and itself */
+    uint32_t tok0, n_here, kh;   /* the unit's first token, its tokens, its kv head */
+    uint32_t req, st, here;      /* the piece: tiles [st, st + here) of the unit; here = 0: there are no more */
+    uint32_t tiles;              /* of the unit */
+};
+struct Walk {
+    uint64_t left;               /* tiles of the share still to come */
+    uint32_t req, kh, g, st;
+    PgReq R;
+    __device__ __forceinline__ void begin(const PagedParams &P, uint64_t n, uint32_t r, uint32_t kh_, uint32_t g_, uint32_t st_) {
+        bool bad;
+        left = n; req = r; kh = kh_; g = g_; st = st_;
+        R = chunk_request(P, r, bad);
+    }
+    __device__ __forceinline__ bool next(const PagedParams &P, uint32_t tpu, Piece &p) {
+        if (!left) return false;
+        bool bad;
+        while (!R.add) R = chunk_request(P, ++req, bad);   /* `left` tiles lie ahead: there is one with tokens */
+        p.tiles = unit_tiles(R, tpu, g);
+        p.n_here = min(tpu, R.add - g * tpu);
+        p.before = R.held + g * tpu; p.tok0 = R.tok0 + g * tpu; p.kh = kh; p.req = req; p.st = st;
+        p.here = (uint32_t)min((uint64_t)(p.tiles - st), left);
+        left -= p.here;
+        st += p.here;
+        if (st == p.tiles) {
+            st = 0;
+            if (++g * (uint64_t)tpu >= R.add) {
+                g = 0;
+                if (++kh == P.n_kvh) {
+                    kh = 0;
+                    R.add = 0;
+                }
+            }
+        }
+        return true;
+    }
+};
+
+template <int KIND, int HD>
+__global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
+    using C = ChunkCfg<HD>;
+    constexpr uint32_t NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
+    constexpr uint32_t O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
+    extern __shared__ uint8_t smem_dyn[];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT;
+    const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
+                   s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 288, s_sum = bars + 320, w_full = bars + 448,
+                   w_empty = w_full + 8u * PIECES, s_piece = w_empty + 8u * PIECES, s_xch = bars + 768;
+    uint8_t *base = smem_dyn + (sQ - smem_u32(smem_dyn));
+    const uint32_t tpu = P.tpg * NQ;
+
+    if (warp == 12u) {
+        if (lane == 0) {
+            for (uint32_t s = 0; s < SLOTS; s++) {
+                mbar_init(full + 8 * s, KIND == Q4K_Q8 ? 4u : 1u);
+                mbar_init(empty + 8 * s, 1);
+            }
+            for (uint32_t s = 0; s < 4; s++) {
+                mbar_init(bar_s + 8 * s, 1);
+                mbar_init(bar_p + 8 * s, NQ == 2u ? 128u : 256u);
+            }
+            mbar_init(bar_o, 1);
+            mbar_init(bar_o + 8, 1);
+            mbar_init(bar_q, 256);
+            for (uint32_t s = 0; s < PIECES; s++) {
+                mbar_init(w_full + 8 * s, 1);
+                mbar_init(w_empty + 8 * s, 9u + (KIND == Q4K_Q8 ? 4u : 1u));   /* a warp each of softmax, issuer and producers */
+            }
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(0u) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_tmem), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    q4d_pdl_wait();
+
+    /* ---- this block's share */
+    uint64_t total = 0, s_begin, s_end, blocks;
+    {
+        const uint32_t per = (P.n_req + CK_THREADS - 1u) / CK_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
+        uint64_t mine = 0, before = 0;
+        bool bad, any_bad = false;
+        for (uint32_t r = r0; r < r1; r++) {
+            mine += request_tiles(P, chunk_request(P, r, bad), tpu);
+            any_bad |= bad;
+        }
+        uint64_t x = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= (uint32_t)d) x += y;
+        }
+        uint64_t *sums = reinterpret_cast<uint64_t *>(base + (s_sum - sQ));
+        if (lane == 31u) sums[warp] = x;
+        __syncthreads();
+        for (uint32_t w = 0; w < CK_THREADS / 32u; w++) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        before += x - mine;
+        if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+        blocks = min((uint64_t)gridDim.x, total);
+        s_begin = blockIdx.x < blocks ? total * blockIdx.x / blocks : 0u;
+        s_end = blockIdx.x < blocks ? total * (blockIdx.x + 1u) / blocks : 0u;
+        if (s_begin < s_end && before <= s_begin && s_begin < before + mine)
+            for (uint32_t r = r0; r < r1; r++) {
+                const PgReq R = chunk_request(P, r, bad);
+                const uint64_t n = request_tiles(P, R, tpu);
+                if (s_begin < before + n) {
+                    const uint64_t per_kh = n / P.n_kvh, off = s_begin - before;
+                    const uint32_t kh = (uint32_t)(off / per_kh), groups = (R.add + tpu - 1u) / tpu;
+                    const uint64_t in = off - (uint64_t)kh * per_kh;
+                    uint32_t lo = 0, hi = groups - 1u;   /* the last group that begins at or before `in` */
+                    while (lo < hi) {
+                        const uint32_t mid = (lo + hi + 1u) >> 1;
+                        if (tiles_before(R, tpu, mid) <= in) lo = mid;
+                        else hi = mid - 1u;
+                    }
+                    const uint32_t st = (uint32_t)(in - tiles_before(R, tpu, lo));
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"(kh), "r"(lo), "r"(st) : "memory");
+                    break;
+                }
+                before += n;
+            }
+    }
+    tc_fence_before();
+    __syncthreads();   /* barriers initialised, tensor memory allocated, the share's place found */
+    tc_fence_after();
+    uint32_t tmem, w_req, w_kh, w_g, w_st;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w_req), "=r"(w_kh), "=r"(w_g), "=r"(w_st) : "r"(s_at));
+    bool ok = true;
+    /* the next piece, by a whole warp; its place is given back with piece_done */
+    uint32_t n_piece = 0;
+    auto next_piece = [&](Piece &p) -> bool {
+        const uint32_t e = n_piece % PIECES, a = s_piece + e * 32u;
+        if (!ck_all_wait(w_full + 8 * e, (n_piece / PIECES) & 1u, s_abort)) {
+            ok = false;
+            return false;
+        }
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.before), "=r"(p.tok0), "=r"(p.n_here), "=r"(p.kh) : "r"(a) : "memory");
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.req), "=r"(p.st), "=r"(p.here), "=r"(p.tiles) : "r"(a + 16u) : "memory");
+        return p.here != 0u;
+    };
+    auto piece_done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(w_empty + 8 * (n_piece % PIECES));
+        n_piece++;
+    };
+    Piece p;
+
+    if (warp >= 12u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12u) {
+            /* ================= issuer: a converged warp, one elected lane ================= */
+            constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(UN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const uint32_t el = elect_one();
+            uint32_t slot = 0, phase = 0, use[2] = {0u, 0u};   /* use: units of scores so far, per group */
+            auto take = [&]() -> uint32_t {
+                const uint32_t s = slot;
+                ok = ok && ck_all_wait(full + 8 * s, phase, s_abort);
+                if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
+                return s;
+            };
+            const uint64_t q_desc = umma_desc(sQ), k_desc = umma_desc(sR), vt_desc = v_desc(sR, HD == 256 ? 64u * 128u : 128u * 128u);
+            /* scores of a unit (row0: its first position in the tile) of group g from K slot s, dims 128 c .. */
+            auto qk = [&](uint32_t col, uint32_t g, uint32_t c, uint32_t s, uint32_t row0) {
+                const uint64_t qd = q_desc + ((g * C::QG + c * (2u * 16384u)) >> 4), kd = k_desc + ((s * SLOT + row0 * 128u) >> 4);
+#pragma unroll
+                for (uint32_t kk = 0; kk < (HD == 64 ? 4u : 8u); kk++)
+                    umma_f16<false>(el, tmem + col, qd + (((kk >> 2) * 16384u + (kk & 3u) * 32u) >> 4), kd + (((kk >> 2) * 16384u + (kk & 3u) * 32u) >> 4), IDESC_QK, (c | kk) > 0u);
+            };
+            /* 64 positions, from byte `at` of V slot s */
+            auto pv = [&](uint32_t col, uint32_t g, uint32_t s, uint32_t at, bool first) {
+                const uint64_t vd = vt_desc + ((s * SLOT + at) >> 4);
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; kk++)
+                    umma_f16_ta<false>(el, tmem + O_COL + g * 128u, tmem + col + kk * 8u, vd + kk * (2048u >> 4), IDESC_PV, (first && kk == 0u) ? 0u : 1u);
+            };
+            while (ok && next_piece(p)) {
+                const uint32_t groups = NQ == 2u && p.n_here > P.tpg ? 2u : 1u;
+                ok = ck_all_wait(bar_q, n_piece & 1u, s_abort);
+                piece_done();
+                if (NQ == 2u) {
+                    uint32_t ks = take();
+                    tc_fence_after();
+                    if (!ok) break;
+                    for (uint32_t e = 0; e < 2; e++)
+                        for (uint32_t g = 0; g < groups; g++) {
+                            qk(g * 128u + e * 64u, g, 0u, ks, e * 64u);
+                            umma_commit<false>(el, bar_s + 8 * (g * 2u + e));
+                        }
+                    umma_commit<false>(el, empty + 8 * ks);
+                    for (uint32_t j = 0; j < p.here && ok; j++) {
+                        const uint32_t sv = take();
+                        const bool more = j + 1u < p.here;
+                        if (more) ks = take();
+                        tc_fence_after();
+#pragma unroll
+                        for (uint32_t e = 0; e < 2; e++)
+                            for (uint32_t g = 0; g < groups; g++) {
+                                ok = ok && ck_all_wait(bar_p + 8 * (g * 2u + e), (use[g] >> 1) & 1u, s_abort);
+                                tc_fence_after();
+                                if (!ok) break;
+                                use[g]++;
+                                pv(g * 128u + e * 64u, g, sv, e * (64u * 128u), j == 0u && e == 0u);
+                                umma_commit<false>(el, bar_o + 8 * g);
+                                if (e == 1u && g + 1u == groups) umma_commit<false>(el, empty + 8 * sv);
+                                if (more) {
+                                    qk(g * 128u + e * 64u, g, 0u, ks, e * 64u);
+                                    umma_commit<false>(el, bar_s + 8 * (g * 2u + e));
+                                }
+                            }
+                        if (more && ok) umma_commit<false>(el, empty + 8 * ks);
+                    }
+                } else {
+                    uint32_t issued = use[0];
+                    auto issue_qk = [&]() {
+                        const uint32_t b = issued & 1u;
+                        for (uint32_t c = 0; c < PARTS; c++) {
+                            const uint32_t s = take();
+                            tc_fence_after();
+                            if (!ok) return;
+                            qk(b * 128u, 0u, c, s, 0u);
+                            umma_commit<false>(el, empty + 8 * s);
+                        }
+                        umma_commit<false>(el, bar_s + 8 * b);
+                        issued++;
+                    };
+                    issue_qk();
+                    if (ok && p.here > 1u) issue_qk();
+                    for (uint32_t j = 0; j < p.here && ok; j++) {
+                        const uint32_t b = use[0] & 1u;
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; h++) {
+                            const uint32_t sv = take();
+                            if (h == 0u) ok = ok && ck_all_wait(bar_p + 8 * b, (use[0] >> 1) & 1u, s_abort);
+                            tc_fence_after();
+                            if (!ok) break;
+                            pv(b * 128u + h * 64u, 0u, sv, 0u, j == 0u && h == 0u);
+                            umma_commit<false>(el, empty + 8 * sv);
+                        }
+                        if (!ok) break;
+                        use[0]++;
+                        umma_commit<false>(el, bar_o);
+                        if (j + 2u < p.here) issue_qk();
+                    }
+                }
+            }
+        }
+        if (warp == 13u) {
+            /* ================= walker: the share's pieces, and the unit that ends in this block ================= */
+            int4 end_of = make_int4(-1, 0, 0, 0);
+            uint64_t s_now = s_begin;
+            Walk W;
+            W.left = 0;
+            if (s_begin < s_end) W.begin(P, s_end - s_begin, w_req, w_kh, w_g, w_st);
+            for (uint32_t n = 0; ok; n++) {
+                const uint32_t e = n % PIECES, a = s_piece + e * 32u;
+                p.here = 0;
+                const bool more = W.next(P, tpu, p);
+                if (n >= PIECES) ok = ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
+                if (!ok) break;
+                if (lane == 0) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here), "r"(p.kh) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
+                    mbar_arrive(w_full + 8 * e);
+                }
+                if (!more) break;
+                if (p.st > 0u && p.st + p.here == p.tiles)   /* the unit ends here; it began in block .. */
+                    end_of = make_int4((int32_t)((((s_now - p.st) + 1u) * blocks - 1u) / total), (int32_t)p.tok0, (int32_t)p.n_here, (int32_t)p.kh);
+                s_now += p.here;
+            }
+            if (lane == 0) P.ends[blockIdx.x] = end_of;
+        }
+    } else if (warp >= 8u) {
+        /* ================= producers ================= */
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        const uint32_t ptid = tid - 256u, mask = (1u << P.page_shift) - 1u;
+        if (KIND == Q4K_Q8 || warp == 8u) {
+            uint32_t at = 0;                          /* slots so far */
+            uint32_t kt = 0, vt = 0, part = 0, n_kv = 0;   /* of the piece: next K and V tile, slot of the tile; positions */
+            uint32_t k_count = 0;
+            const int32_t *tab = nullptr;
+            const uint8_t *kh_base = nullptr;
+            int32_t e_next = 0, h0 = -1, h1 = -1;     /* lane i: the page of 16 positions i of the next K tile, of the last one, of the one before */
+            p.here = 0;
+            struct Job { uint32_t p0, part; bool v; int32_t pages; };
+            auto entry = [&](uint32_t tile) -> int32_t {
+                const uint32_t q = (p.st + tile) * CK_BN + (lane & 7u) * 16u;
+                return tile < p.here && q < n_kv ? tab[q >> P.page_shift] : 0;
+            };
+            auto next_job = [&](Job &job) -> bool {
+                if (vt == p.here) {
+                    if (!ok || !next_piece(p)) return false;
+                    piece_done();
+                    kt = vt = part = 0;
+                    n_kv = p.before + p.n_here;
+                    tab = P.table + (size_t)p.req * P.table_stride;
+                    kh_base = P.mem + (uint64_t)p.kh * P.part_bytes;
+                    e_next = entry(0);
+                }
+                /* K runs ahead of V as far as the scores run ahead of the outputs */
+                const bool k = kt < p.here && kt <= vt + (NQ == 1u ? 1u : 0u);
+                job.v = !k;
+                job.part = part;
+                if (k) {
+                    if (part == 0u) {
+                        h1 = h0;
+                        h0 = e_next;
+                        if (h0 < 0 || (uint32_t)h0 >= P.n_pages) h0 = -1;
+                        e_next = entry(kt + 1u);
+                        const uint32_t gone = __ballot_sync(0xffffffffu, h0 < 0) & 0xffu;
+                        if (gone && ptid == 0u) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+                        /* read by the softmax warps once the scores of the tile are there */
+                        if (ptid == 0u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (k_count & 7u)), "r"(gone) : "memory");
+                        k_count++;
+                    }
+                    job.p0 = (p.st + kt) * CK_BN;
+                    job.pages = h0;
+                    if (++part == PARTS) { part = 0; kt++; }
+                } else {
+                    job.p0 = (p.st + vt) * CK_BN;
+                    job.pages = kt - 1u == vt ? h0 : h1;
+                    if (++part == PARTS) { part = 0; vt++; }
+                }
+                return true;
+            };
+            auto wait_empty = [&]() {
+                const uint32_t s = at % SLOTS, n = at / SLOTS;
+                if (n > 0u) ok = ok && ck_all_wait(empty + 8 * s, (n - 1u) & 1u, s_abort);
+            };
+            auto sub_tile = [&](int32_t page, uint32_t q) -> const uint8_t * {   /* the tile of 16 rows at position q, on that page */
+                return kh_base + (uint64_t)(uint32_t)page * P.page_bytes + ((q & mask) >> 4) * TILE;
+            };
+            if constexpr (KIND == Q4K_Q8) {
+                /* 16 codes per item; CH items to a row of the slot, RB rows per pass of the 128 threads */
+                constexpr uint32_t ITEMS = SLOT / 32u / 128u;
+                struct Raw { uint4 w[ITEMS]; uint16_t s[ITEMS]; };
+                auto load = [&](Raw &r, const Job &job, uint32_t ch) {
+                    const uint32_t rb = 128u / ch, c = ptid % ch, row0 = ptid / ch;
+                    const uint32_t p0 = job.p0 + (HD == 256 && job.v ? job.part * 64u : 0u), cc = c + (HD == 256 && !job.v ? job.part * 8u : 0u);
+#pragma unroll
+                    for (uint32_t it = 0; it < ITEMS; it++) {
+                        const uint32_t row = row0 + it * rb, q = p0 + row;
+                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)((q - job.p0) >> 4));
+                        r.w[it] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                        r.s[it] = 0;
+                        if (q < n_kv && page >= 0) {
+                            const uint8_t *rec = sub_tile(page, q) + (q & 15u) * ROW;
+                            r.w[it] = *reinterpret_cast<const uint4 *>(rec + (job.v ? HD : 0) + cc * 16u);
+                            r.s[it] = *reinterpret_cast<const uint16_t *>(rec + 2u * HD + (job.v ? HD / 16u : 0u) + (cc >> 1) * 2u);
+                        }
+                    }
+                };
+                auto store = [&](const Raw &r, const Job &job, uint32_t ch) {
+                    wait_empty();
+                    if (!ok) return;
+                    const uint32_t rb = 128u / ch, c = ptid % ch, row0 = ptid / ch, dst = sR + (at % SLOTS) * SLOT;
+                    const uint32_t block = HD == 256 && job.v ? 64u * 128u : 128u * 128u;
+#pragma unroll
+                    for (uint32_t it = 0; it < ITEMS; it++) {
+                        const uint32_t row = row0 + it * rb;
+                        const __half2 sc = __half2half2(__ushort_as_half(r.s[it]));
+                        const uint32_t w[4] = {r.w[it].x ^ 0x80808080u, r.w[it].y ^ 0x80808080u, r.w[it].z ^ 0x80808080u, r.w[it].w ^ 0x80808080u};
+                        uint32_t o[8];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            o[2 * k] = h2u(__hmul2(codes2<0x4140>(w[k]), sc));
+                            o[2 * k + 1] = h2u(__hmul2(codes2<0x4342>(w[k]), sc));
+                        }
+                        /* lanes of the upper block begin with their second piece: they would meet the lower's banks */
+                        const uint32_t a = dst + (c >> 2) * block + row * 128u, c0 = (c & 3u) * 2u, odd = (c >> 2) & 1u;
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; k++) {
+                            const uint32_t second = k ^ odd;
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a + (((c0 + second) ^ (row & 7u)) << 4)),
+                                         "r"(second ? o[4] : o[0]), "r"(second ? o[5] : o[1]), "r"(second ? o[6] : o[2]), "r"(second ? o[7] : o[3]) : "memory");
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
+                    at++;
+                };
+                constexpr uint32_t CHK = HD == 64 ? 4u : 8u, CHV = HD / 16u;
+                Raw r0, r1;
+                Job j0, j1;
+                bool more = next_job(j0);
+                if (more) load(r0, j0, j0.v ? CHV : CHK);
+                while (more && ok) {
+                    more = next_job(j1);
+                    if (more) load(r1, j1, j1.v ? CHV : CHK);
+                    store(r0, j0, j0.v ? CHV : CHK);
+                    if (!more || !ok) break;
+                    more = next_job(j0);
+                    if (more) load(r0, j0, j0.v ? CHV : CHK);
+                    store(r1, j1, j1.v ? CHV : CHK);
+                }
+            } else {
+                Job job;
+                while (ok && next_job(job)) {
+                    wait_empty();
+                    if (!ok) break;
+                    const uint32_t s = at % SLOTS, dst = sR + s * SLOT, bar = full + 8 * s;
+                    const uint32_t rows = HD == 256 && job.v ? 64u : 128u, p0 = job.p0 + (HD == 256 && job.v ? job.part * 64u : 0u);
+                    constexpr uint32_t BLOCKS = HD == 256 ? 2u : HD / 64u;
+                    const uint32_t blocks_here = HD == 256 && job.v ? 4u : BLOCKS, block0 = HD == 256 && !job.v ? job.part * 2u : 0u;
+                    /* lane i < rows / 16: 16 positions; whole rows of 128 bytes of every block, as many as there are */
+                    const uint32_t q = p0 + lane * 16u;
+                    const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)(((q - job.p0) >> 4) & 7u));
+                    uint32_t live = lane * 16u < rows && page >= 0 && q < n_kv ? min(16u, n_kv - q) : 0u;
+                    const uint32_t all = __reduce_add_sync(0xffffffffu, live);
+                    if (job.v && all < rows) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
+                        for (uint32_t i = lane; i < rows; i += 32u) {
+                            const uint32_t there = __shfl_sync(0xffffffffu, live, (int)(i >> 4));
+                            if ((i & 15u) >= there)
+                                for (uint32_t b = 0; b < blocks_here; b++)
+#pragma unroll
+                                    for (uint32_t c = 0; c < 8; c++)
+                                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + b * rows * 128u + i * 128u + c * 16u), "r"(0u) : "memory");
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+                        if (all) mbar_expect_tx(bar, all * 128u * blocks_here);
+                        else mbar_arrive(bar);
+                    }
+                    __syncwarp();
+                    if (live) {
+                        const uint8_t *src = sub_tile(page, q) + (job.v ? TILE / 2u : 0u) + block0 * 2048u;
+                        for (uint32_t b = 0; b < blocks_here; b++) bulk_load(dst + b * rows * 128u + lane * 2048u, src + b * 2048u, live * 128u, bar);
+                    }
+                    at++;
+                }
+                /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
+                if (!ok)
+                    for (uint32_t t = at > SLOTS ? at - SLOTS : 0u; t < at; t++)
+                        for (uint32_t i = 0; i < 4096u && !mbar_test<OWN>(full + 8 * (t % SLOTS), (t / SLOTS) & 1u); i++) {}
+            }
+        }
+    } else {
+        /* ================= softmax ================= */
+        /* 128 threads x (2 x 168 + 120 + 56) registers: the block's 512 x 128 */
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const uint32_t g = NQ == 2u ? warp >> 2 : 0u, h = NQ == 2u ? 0u : warp >> 2, r = tid & 127u, t_lane = tmem + (((warp & 3u) * 32u) << 16);
+        const uint32_t tl = r / P.gqa, head_in = r - tl * P.gqa;
+        auto pair_sync = [&]() {   /* the two warps of the same 32 rows (hd 256) */
+            __syncwarp();
+            asm volatile("bar.sync %0, 64;" ::"r"(1u + (warp & 3u)) : "memory");
+        };
+        auto pair_any = [&](bool x) -> bool {
+            uint32_t any;
+            __syncwarp();
+            asm volatile("{ .reg .pred p, q; setp.ne.u32 q, %1, 0; bar.red.or.pred p, %2, 64, q; selp.u32 %0, 1, 0, p; }"
+                         : "=r"(any) : "r"((uint32_t)x), "r"(1u + (warp & 3u)) : "memory");
+            return any != 0u;
+        };
+        auto partner = [&](float x) -> float {   /* the other half's value of this row; a meeting lies between two calls */
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(s_xch + 4u * tid), "f"(x) : "memory");
+            pair_sync();
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(s_xch + 4u * (tid ^ 128u)) : "memory");
+            return x;
+        };
+        uint32_t use = 0, tiles_seen = 0;   /* units of this group so far; K tiles so far */
+        while (ok && next_piece(p)) {
+            const bool active = g == 0u || p.n_here > P.tpg;
+            /* ---- queries as fp16, swizzled rows of 64 dims: the products of the piece before have read theirs (its last scores are here) */
+            {
+                constexpr uint32_t PER = HD / 8u, T = NQ == 2u ? 128u : 256u, STEPS = 128u * PER / T, BATCH = 8u;
+                const uint32_t qt = NQ == 2u ? r : tid;
+                if (active) {
+#pragma unroll 1
+                    for (uint32_t k0 = 0; k0 < STEPS; k0 += BATCH) {
+                        uint4 w[BATCH][2];
+#pragma unroll
+                        for (uint32_t k = 0; k < BATCH; k++) {
+                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER, ql = row / P.gqa, qtok = g * P.tpg + ql;
+                            w[k][0] = w[k][1] = make_uint4(0u, 0u, 0u, 0u);
+                            if (ql < P.tpg && qtok < p.n_here) {
+                                const size_t off = ((size_t)(p.tok0 + qtok) * P.n_head + (size_t)p.kh * P.gqa + (row - ql * P.gqa)) * HD + c * 8u;
+                                if (P.q_bf16) {
+                                    w[k][0] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + off);
+                                } else {
+                                    w[k][0] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(P.q) + off);
+                                    w[k][1] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(P.q) + off + 4);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < BATCH; k++) {
+                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER;
+                            const uint32_t in[8] = {w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w, w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                o[e] = P.q_bf16 ? h2u(__floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u)))
+                                                : h2u(__floats2half2_rn(__uint_as_float(in[2 * e]), __uint_as_float(in[2 * e + 1])));
+                            const uint32_t a = sQ + g * C::QG + (c >> 3) * 16384u + row * 128u + (((c & 7u) ^ (row & 7u)) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                        }
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(bar_q);
+                /* a group without tokens would run ahead, and its next arrival count for this piece */
+                if (!active) ok = ck_all_wait(bar_q, n_piece & 1u, s_abort);
+            }
+            const uint32_t tok = g * P.tpg + tl;
+            const bool row_live = tl < P.tpg && tok < p.n_here;
+            /* this row attends positions [0, row_nkv); padding rows (queries of zeros, never stored) need no mask */
+            const uint32_t row_nkv = row_live ? p.before + tok + 1u : 0xffffffffu;
+            const uint32_t warp_min = __reduce_min_sync(0xffffffffu, row_nkv);
+            const uint32_t n_seq = active ? (NQ == 2u ? 2u * p.here : p.here) : 0u;
+            float m_ref = -CUDART_INF_F, l_run = 0.f;
+            for (uint32_t u = 0; u < n_seq && (NQ == 1u || ok); u++, use++) {
+                const uint32_t b = g * 2u + (use & 1u), p0 = p.st * CK_BN + u * UN + h * TU;
+                const uint32_t t_s = t_lane + (NQ == 2u ? g * 128u + (use & 1u) * 64u : (use & 1u) * 128u + h * TU);
+                ok = ok && ck_all_wait(bar_s + 8 * b, (use >> 1) & 1u, s_abort);
+                if (NQ == 1u && !ok) {
+                    if (u == 0u || pair_any(false)) partner(0.f);
+                    continue;
+                }
+                tc_fence_after();
+                float s[TU];
+#pragma unroll
+                for (int c = 0; c < (int)TU / 32; c++) tmem_ld32(t_s + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
+                tmem_wait_ld();
+                uint32_t gone;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(gone) : "r"(s_gone + 4u * ((tiles_seen + (NQ == 2u ? u >> 1 : u)) & 7u)) : "memory");
+                if (__builtin_expect(gone != 0u, 0)) {   /* positions on pages that are not the pool's */
+#pragma unroll
+                    for (int k = 0; k < (int)TU; k++)
+                        if ((gone >> (((p0 & 127u) + k) >> 4)) & 1u) s[k] = -CUDART_INF_F;
+                }
+                if (__builtin_expect(p0 + TU > warp_min, 0)) {
+#pragma unroll
+                    for (int k = 0; k < (int)TU; k++)
+                        if (p0 + k >= row_nkv) s[k] = -CUDART_INF_F;
+                }
+                uint32_t pk[TU / 2];
+                uint64_t ls[2];
+                auto exps = [&]() {
+                    const float mneg = m_ref == -CUDART_INF_F ? 0.f : -m_ref;
+                    const uint64_t sc2 = pack2(P.scale_log2e, P.scale_log2e), mn2 = pack2(mneg, mneg);
+                    ls[0] = ls[1] = 0ull;
+#pragma unroll
+                    for (int k = 0; k < (int)TU / 2; k++) {
+                        const float2 x = unpack2(fma2(pack2(s[2 * k], s[2 * k + 1]), sc2, mn2));
+                        const float e0 = ex2f(x.x), e1 = ex2f(x.y);
+                        ls[k & 1] = add2(ls[k & 1], pack2(e0, e1));
+                        pk[k] = h2u(__floats2half2_rn(e0, e1));
+                    }
+                };
+                /* the exponentials start against the maximum of the units before, while this unit's own is being formed; where that
+                 * is not within 2^8 the reference moves and they are taken again */
+                if (u > 0u) exps();
+                float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                for (int k = 0; k < (int)TU; k += 8) {
+                    mx[0] = fmaxf(fmaxf(mx[0], s[k]), s[k + 1]); mx[1] = fmaxf(fmaxf(mx[1], s[k + 2]), s[k + 3]);
+                    mx[2] = fmaxf(fmaxf(mx[2], s[k + 4]), s[k + 5]); mx[3] = fmaxf(fmaxf(mx[3], s[k + 6]), s[k + 7]);
+                }
+                float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2e;   /* scale > 0 */
+                bool grow = m_new > m_ref + CK_RESCALE_TAU;   /* also true on the first live unit (m_ref = -inf) */
+                const bool any = u == 0u || (NQ == 2u ? __any_sync(0xffffffffu, grow) : pair_any(grow));
+                if (__builtin_expect(any, 0)) {
+                    if (NQ == 1u) {   /* both halves of a row keep one reference: they share its O */
+                        m_new = fmaxf(m_new, partner(m_new));
+                        grow = m_new > m_ref + CK_RESCALE_TAU;
+                    }
+                    float alpha = 1.f;
+                    if (grow) {
+                        alpha = ex2f(m_ref - m_new);
+                        m_ref = m_new;
+                        l_run *= alpha;
+                    }
+                    exps();
+                    if (u > 0u) {   /* O is rescaled only here; the group's last product must have drained */
+                        ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort) && ok;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (uint32_t c = h * (HD / 64); c < (NQ == 2u ? HD / 32 : (h + 1u) * (HD / 64)); c++) {
+                            float o[32];
+                            tmem_ld32(t_lane + O_COL + g * 128u + 32 * c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k++) o[k] *= alpha;
+                            tmem_st32(t_lane + O_COL + g * 128u + 32 * c, o);
+                        }
+                    }
+                }
+                tmem_st32(t_s, *reinterpret_cast<const float(*)[32]>(&pk[0]));
+                tmem_wait_st();
+                /* a parity wait can tell the present phase from the one before it, no further, and bar_o's are not followed unit by
+                 * unit: the phase before the last is waited for here, while the last cannot complete without this thread */
+                if (u > 0u && u + 1u == n_seq) ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort) && ok;
+                tc_fence_before();
+                mbar_arrive(bar_p + 8 * b);
+                const float2 l0 = unpack2(ls[0]), l1 = unpack2(ls[1]);
+                l_run += (l0.x + l0.y) + (l1.x + l1.y);
+            }
+            tiles_seen += p.here;
+            if (NQ == 1u) {
+                pair_sync();
+                l_run += partner(l_run);
+                pair_sync();   /* before the next piece's first exchange */
+            }
+            /* ---- the piece's outputs: a thread has a row (hd 256: half of its columns) */
+            if (active && ok) ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort);
+            tc_fence_after();
+            const bool whole = p.st == 0u && p.here == p.tiles;
+            if (active && ok) {
+                const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
+                const size_t off = ((size_t)(p.tok0 + tok) * P.n_head + (size_t)p.kh * P.gqa + head_in) * HD;
+                float *rec = P.part + (((size_t)blockIdx.x * 2u + (p.st == 0u ? 1u : 0u)) * C::ROWS + g * 128u + r) * C::REC;
+                if (!whole && row_live && h == 0u) *reinterpret_cast<float2 *>(rec + HD) = make_float2(m_ref, l_run);
+#pragma unroll 1
+                for (uint32_t c = h * (HD / 64); c < (NQ == 2u ? HD / 32 : (h + 1u) * (HD / 64)); c++) {
+                    float o[32];
+                    tmem_ld32(t_lane + O_COL + g * 128u + 32 * c, o);
+                    tmem_wait_ld();
+                    if (!row_live) continue;
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(rec + 32u * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        continue;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k++) o[k] *= inv;
+                    if (P.gate) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            const float4 gt = *reinterpret_cast<const float4 *>(P.gate + off + 32u * c + k);
+                            o[k] = gated(o[k], gt.x); o[k + 1] = gated(o[k + 1], gt.y); o[k + 2] = gated(o[k + 2], gt.z); o[k + 3] = gated(o[k + 3], gt.w);
+                        }
+                    }
+                    if (P.out_bf16) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            __nv_bfloat162 x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] = __floats2bfloat162_rn(o[k + 2 * e], o[k + 2 * e + 1]);
+                            *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + off + 32u * c + k) = *reinterpret_cast<const uint4 *>(x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + off + 32u * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    }
+                }
+            }
+            tc_fence_before();   /* the next piece's first product overwrites O behind this thread's next arrival */
+            if (NQ == 1u) ok = !pair_any(!ok);   /* the two warps of a row leave together */
+            piece_done();
+        }
+    }
+    if (!ok && lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+}
+
+template <int KIND, int HD>
+bool chunk(PagedParams p, float *scratch) {
+    using C = ChunkCfg<HD>;
+    static bool attr = false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_chunk_k<KIND, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
+    attr = true;
+    const uint32_t blocks = (uint32_t)g_q4.sm_count;
+    p.part = scratch;
+    p.ends = reinterpret_cast<int4 *>(scratch + (size_t)blocks * 2u * C::ROWS * C::REC);
+    p.tpg = 128u / p.gqa;
+    p.group_rows = 128u;
+    return q4i_launch_pdl("pages_attend launch", q4_pg_chunk_k<KIND, HD>, dim3(blocks), CK_THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
+}
+
+}  // namespace
+
+size_t q4i_paged_chunk_floats(uint32_t hd) {
+    const size_t rows = hd == 256 ? 128u : 256u;
+    return (size_t)g_q4.sm_count * (2u * rows * (hd + 4u) + 4u);
+}
+bool q4i_paged_chunk(const PagedParams &p, int kind, uint32_t hd, float *scratch) {
+    if (kind == Q4K_Q8) return hd == 64 ? chunk<Q4K_Q8, 64>(p, scratch) : hd == 128 ? chunk<Q4K_Q8, 128>(p, scratch) : chunk<Q4K_Q8, 256>(p, scratch);
+    return hd == 64 ? chunk<Q4K_F16, 64>(p, scratch) : hd == 128 ? chunk<Q4K_F16, 128>(p, scratch) : chunk<Q4K_F16, 256>(p, scratch);
+}
