@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 #include <math_constants.h>
 #include <string.h>
+#include <type_traits>
 
 #include "q4_paged.h"
 #include "q4_tc.h"
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
             constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(UN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             const uint32_t el = elect_one();
-            uint32_t slot = 0, phase = 0, use[2] = {0u, 0u};   /* use: units of scores so far, per group */
+            uint32_t slot = 0, phase = 0, use0 = 0, use1 = 0;   /* two groups: phase of their score buffers; one: units so far */
             auto take = [&]() -> uint32_t {
                 const uint32_t s = slot;
                 ok = ok && ck_all_wait(full + 8 * s, phase, s_abort);
@@ -305,10 +306,12 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                     uint32_t ks = take();
                     tc_fence_after();
                     if (!ok) break;
-                    for (uint32_t e = 0; e < 2; e++)
-                        for (uint32_t g = 0; g < groups; g++) {
-                            qk(g * 128u + e * 64u, g, 0u, ks, e * 64u);
-                            umma_commit<false>(el, bar_s + 8 * (g * 2u + e));
+                    const bool two = groups == 2u;
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++)   /* half e >> 1 of the tile, group e & 1 */
+                        if (two || !(e & 1u)) {
+                            qk((e & 1u) * 128u + (e >> 1) * 64u, e & 1u, 0u, ks, (e >> 1) * 64u);
+                            umma_commit<false>(el, bar_s + 8 * ((e & 1u) * 2u + (e >> 1)));
                         }
                     umma_commit<false>(el, empty + 8 * ks);
                     for (uint32_t j = 0; j < p.here && ok; j++) {
@@ -317,24 +320,26 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                         if (more) ks = take();
                         tc_fence_after();
 #pragma unroll
-                        for (uint32_t e = 0; e < 2; e++)
-                            for (uint32_t g = 0; g < groups; g++) {
-                                ok = ok && ck_all_wait(bar_p + 8 * (g * 2u + e), (use[g] >> 1) & 1u, s_abort);
-                                tc_fence_after();
-                                if (!ok) break;
-                                use[g]++;
-                                pv(g * 128u + e * 64u, g, sv, e * (64u * 128u), j == 0u && e == 0u);
-                                umma_commit<false>(el, bar_o + 8 * g);
-                                if (e == 1u && g + 1u == groups) umma_commit<false>(el, empty + 8 * sv);
-                                if (more) {
-                                    qk(g * 128u + e * 64u, g, 0u, ks, e * 64u);
-                                    umma_commit<false>(el, bar_s + 8 * (g * 2u + e));
-                                }
+                        for (uint32_t e = 0; e < 4; e++) {
+                            if (!two && (e & 1u)) continue;
+                            const uint32_t b = (e & 1u) * 2u + (e >> 1), col = (e & 1u) * 128u + (e >> 1) * 64u;
+                            ok = ok && ck_all_wait(bar_p + 8 * b, e & 1u ? use1 : use0, s_abort);
+                            tc_fence_after();
+                            if (!ok) break;
+                            pv(col, e & 1u, sv, (e >> 1) * (64u * 128u), j == 0u && e < 2u);
+                            umma_commit<false>(el, bar_o + 8 * (e & 1u));
+                            if (e == (two ? 3u : 2u)) umma_commit<false>(el, empty + 8 * sv);
+                            if (more) {
+                                qk(col, e & 1u, 0u, ks, (e >> 1) * 64u);
+                                umma_commit<false>(el, bar_s + 8 * b);
                             }
+                        }
+                        use0 ^= 1u;
+                        use1 ^= two ? 1u : 0u;
                         if (more && ok) umma_commit<false>(el, empty + 8 * ks);
                     }
                 } else {
-                    uint32_t issued = use[0];
+                    uint32_t issued = use0;
                     auto issue_qk = [&]() {
                         const uint32_t b = issued & 1u;
                         for (uint32_t c = 0; c < PARTS; c++) {
@@ -350,18 +355,18 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                     issue_qk();
                     if (ok && p.here > 1u) issue_qk();
                     for (uint32_t j = 0; j < p.here && ok; j++) {
-                        const uint32_t b = use[0] & 1u;
+                        const uint32_t b = use0 & 1u;
 #pragma unroll
                         for (uint32_t h = 0; h < 2; h++) {
                             const uint32_t sv = take();
-                            if (h == 0u) ok = ok && ck_all_wait(bar_p + 8 * b, (use[0] >> 1) & 1u, s_abort);
+                            if (h == 0u) ok = ok && ck_all_wait(bar_p + 8 * b, (use0 >> 1) & 1u, s_abort);
                             tc_fence_after();
                             if (!ok) break;
                             pv(b * 128u + h * 64u, 0u, sv, 0u, j == 0u && h == 0u);
                             umma_commit<false>(el, empty + 8 * sv);
                         }
                         if (!ok) break;
-                        use[0]++;
+                        use0++;
                         umma_commit<false>(el, bar_o);
                         if (j + 2u < p.here) issue_qk();
                     }
@@ -454,68 +459,84 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 return kh_base + (uint64_t)(uint32_t)page * P.page_bytes + ((q & mask) >> 4) * TILE;
             };
             if constexpr (KIND == Q4K_Q8) {
-                /* 16 codes per item; CH items to a row of the slot, RB rows per pass of the 128 threads */
+                /* An item is 16 codes: one 16-byte load, two 16-byte pieces of fp16.  A pass of a warp is 8 rows x 64 dims: four lanes to
+                 * a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has SUB tiles of 16
+                 * rows of the slot, NB blocks of 64 dims each, two passes to a block: pages are looked up once per tile and the rest are
+                 * constant offsets. */
                 constexpr uint32_t ITEMS = SLOT / 32u / 128u;
-                struct Raw { uint4 w[ITEMS]; uint16_t s[ITEMS]; };
-                auto load = [&](Raw &r, const Job &job, uint32_t ch) {
-                    const uint32_t rb = 128u / ch, c = ptid % ch, row0 = ptid / ch;
-                    const uint32_t p0 = job.p0 + (HD == 256 && job.v ? job.part * 64u : 0u), cc = c + (HD == 256 && !job.v ? job.part * 8u : 0u);
+                constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
+                struct Raw { uint4 w[ITEMS]; uint32_t s[ITEMS]; };   /* codes; the two scales of 64 dims of a row */
+                const uint32_t wi = warp - 8u, r8 = lane >> 2, c4 = lane & 3u;
+                auto load = [&](Raw &r, const Job &job, auto nb) {
+                    constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB;
+                    const uint32_t sub0 = (HD == 256 && job.v ? job.part * 4u : 0u) + wi * SUB, col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
+                    const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
 #pragma unroll
-                    for (uint32_t it = 0; it < ITEMS; it++) {
-                        const uint32_t row = row0 + it * rb, q = p0 + row;
-                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)((q - job.p0) >> 4));
-                        r.w[it] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                        r.s[it] = 0;
-                        if (q < n_kv && page >= 0) {
-                            const uint8_t *rec = sub_tile(page, q) + (q & 15u) * ROW;
-                            r.w[it] = *reinterpret_cast<const uint4 *>(rec + (job.v ? HD : 0) + cc * 16u);
-                            r.s[it] = *reinterpret_cast<const uint16_t *>(rec + 2u * HD + (job.v ? HD / 16u : 0u) + (cc >> 1) * 2u);
+                    for (uint32_t i = 0; i < SUB; i++) {
+                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)(sub0 + i));
+                        const uint32_t q = job.p0 + (sub0 + i) * 16u;
+                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + r8 * ROW;
+#pragma unroll
+                        for (uint32_t x = 0; x < 2; x++) {   /* rows r8 and r8 + 8 */
+                            const bool there = page >= 0 && q + r8 + 8u * x < n_kv;
+#pragma unroll
+                            for (uint32_t b = 0; b < NB; b++) {
+                                const uint32_t k = (i * 2u + x) * NB + b;
+                                r.w[k] = make_uint4(0u, 0u, 0u, 0u);
+                                r.s[k] = 0u;
+                                if (there) {
+                                    r.w[k] = *reinterpret_cast<const uint4 *>(rec + 8u * x * ROW + col + b * 64u);
+                                    r.s[k] = *reinterpret_cast<const uint32_t *>(rec + 8u * x * ROW + sc + b * 4u);
+                                }
+                            }
                         }
                     }
                 };
-                auto store = [&](const Raw &r, const Job &job, uint32_t ch) {
+                const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
+                auto store = [&](const Raw &r, const Job &job, auto nb) {
+                    constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
                     wait_empty();
                     if (!ok) return;
-                    const uint32_t rb = 128u / ch, c = ptid % ch, row0 = ptid / ch, dst = sR + (at % SLOTS) * SLOT;
-                    const uint32_t block = HD == 256 && job.v ? 64u * 128u : 128u * 128u;
+                    const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * SUB * 16u + r8) * 128u;
+                    const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
 #pragma unroll
-                    for (uint32_t it = 0; it < ITEMS; it++) {
-                        const uint32_t row = row0 + it * rb;
-                        const __half2 sc = __half2half2(__ushort_as_half(r.s[it]));
-                        const uint32_t w[4] = {r.w[it].x ^ 0x80808080u, r.w[it].y ^ 0x80808080u, r.w[it].z ^ 0x80808080u, r.w[it].w ^ 0x80808080u};
+                    for (uint32_t k = 0; k < ITEMS; k++) {
+                        const uint32_t sc = __byte_perm(r.s[k], 0u, scale_sel), off = k / NB * 1024u + k % NB * BLOCK;
+                        const uint32_t w[4] = {r.w[k].x ^ 0x80808080u, r.w[k].y ^ 0x80808080u, r.w[k].z ^ 0x80808080u, r.w[k].w ^ 0x80808080u};
                         uint32_t o[8];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            o[2 * k] = h2u(__hmul2(codes2<0x4140>(w[k]), sc));
-                            o[2 * k + 1] = h2u(__hmul2(codes2<0x4342>(w[k]), sc));
+                        for (int e = 0; e < 4; e++) {
+                            o[2 * e] = h2u(__hmul2(codes2<0x4140>(w[e]), *reinterpret_cast<const __half2 *>(&sc)));
+                            o[2 * e + 1] = h2u(__hmul2(codes2<0x4342>(w[e]), *reinterpret_cast<const __half2 *>(&sc)));
                         }
-                        /* lanes of the upper block begin with their second piece: they would meet the lower's banks */
-                        const uint32_t a = dst + (c >> 2) * block + row * 128u, c0 = (c & 3u) * 2u, odd = (c >> 2) & 1u;
-#pragma unroll
-                        for (uint32_t k = 0; k < 2; k++) {
-                            const uint32_t second = k ^ odd;
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a + (((c0 + second) ^ (row & 7u)) << 4)),
-                                         "r"(second ? o[4] : o[0]), "r"(second ? o[5] : o[1]), "r"(second ? o[6] : o[2]), "r"(second ? o[7] : o[3]) : "memory");
-                        }
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a0 + off), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a1 + off), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
                     }
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
                     at++;
                 };
-                constexpr uint32_t CHK = HD == 64 ? 4u : 8u, CHV = HD / 16u;
+                auto load_job = [&](Raw &r, const Job &job) {
+                    if (NBK != NBV && job.v) load(r, job, std::integral_constant<uint32_t, NBV>());
+                    else load(r, job, std::integral_constant<uint32_t, NBK>());
+                };
+                auto store_job = [&](const Raw &r, const Job &job) {
+                    if (NBK != NBV && job.v) store(r, job, std::integral_constant<uint32_t, NBV>());
+                    else store(r, job, std::integral_constant<uint32_t, NBK>());
+                };
                 Raw r0, r1;
                 Job j0, j1;
                 bool more = next_job(j0);
-                if (more) load(r0, j0, j0.v ? CHV : CHK);
+                if (more) load_job(r0, j0);
                 while (more && ok) {
                     more = next_job(j1);
-                    if (more) load(r1, j1, j1.v ? CHV : CHK);
-                    store(r0, j0, j0.v ? CHV : CHK);
+                    if (more) load_job(r1, j1);
+                    store_job(r0, j0);
                     if (!more || !ok) break;
                     more = next_job(j0);
-                    if (more) load(r0, j0, j0.v ? CHV : CHK);
-                    store(r1, j1, j1.v ? CHV : CHK);
+                    if (more) load_job(r0, j0);
+                    store_job(r1, j1);
                 }
             } else {
                 Job job;
