@@ -10,8 +10,8 @@
  *   warps 0 - 7    softmax: thread r owns row r (hd 256: two threads, half of a unit's positions each): its scores out of tensor
  *                  memory, causal mask, running maximum with lazy rescale, weights as fp16 back into the columns they came from
  *   warps 8 - 11   producers: K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads
- *                  them: bulk copies.  q8_0: codes and scales into registers, a slot ahead of their use, fp16(code x scale) into
- *                  the slot (7 instructions per 4 values: a fifth of the issue slots that the products leave)
+ *                  them: bulk copies.  q8_0: codes and scales by asynchronous copies, three slots ahead, then fp16(code x scale)
+ *                  into the slot (7 instructions per 4 values)
  *   warp 12        issues the products: O += P V of a unit of positions as its weights appear, then the scores that take over the
  *                  buffer
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
@@ -36,15 +36,18 @@ constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
 constexpr uint32_t PIECES = 4;          /* pieces that are walked ahead */
 constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the reference moves */
 
-template <int HD>
+constexpr uint32_t RAWS = 3;            /* slots of q8_0 codes on their way */
+template <int KIND, int HD>
 struct ChunkCfg {
     static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
-    static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : 5u;
+    static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : KIND == Q4K_Q8 ? 3u : 5u;
+    static constexpr uint32_t ITEMS = SLOT / 32u / 128u;          /* of 16 codes, per producer thread and slot */
+    static constexpr uint32_t RAW = KIND == Q4K_Q8 ? 4u * ITEMS * 544u : 0u;   /* codes and scales of a slot */
     static constexpr uint32_t PARTS = HD == 256 ? 2u : 1u;        /* slots of a K or a V tile: K by 128 dims, V by 64 positions */
     static constexpr uint32_t QG = 128u * HD * 2u;                /* one group's queries */
     static constexpr uint32_t REC = HD + 4u;
     static constexpr uint32_t BARS = 768u + (NQ == 1u ? 1024u : 0u);
-    static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + BARS + 1024u;
+    static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + RAWS * RAW + BARS + 1024u;
     static constexpr uint32_t UN = NQ == 2u ? 64u : 128u;         /* positions of a unit of scores */
     static_assert(SMEM <= 232448u, "shared memory");
 };
@@ -61,6 +64,16 @@ __device__ __forceinline__ __half2 codes2(uint32_t x) {
     return __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&off));
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool there) {   /* zeros where there is nothing */
+    if (there) {
+        if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + i), "r"(0u) : "memory");
+    }
+}
 /* the rest of a wait whose first test found the phase incomplete (in line: ptxas does not allocate calls beside setmaxnreg) */
 __device__ __forceinline__ bool ck_wait_on(uint32_t bar, uint32_t parity, uint32_t s_abort) {
     const unsigned long long t0 = global_ns();
@@ -156,12 +169,12 @@ struct Walk {
 
 template <int KIND, int HD>
 __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
-    using C = ChunkCfg<HD>;
+    using C = ChunkCfg<KIND, HD>;
     constexpr uint32_t NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
     constexpr uint32_t O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT;
+    const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + RAWS * C::RAW;
     const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
                    s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 288, s_sum = bars + 320, w_full = bars + 448,
                    w_empty = w_full + 8u * PIECES, s_piece = w_empty + 8u * PIECES, s_xch = bars + 768;
@@ -459,85 +472,93 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 return kh_base + (uint64_t)(uint32_t)page * P.page_bytes + ((q & mask) >> 4) * TILE;
             };
             if constexpr (KIND == Q4K_Q8) {
-                /* An item is 16 codes: one 16-byte load, two 16-byte pieces of fp16.  A pass of a warp is 8 rows x 64 dims: four lanes to
-                 * a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has SUB tiles of 16
-                 * rows of the slot, NB blocks of 64 dims each, two passes to a block: pages are looked up once per tile and the rest are
-                 * constant offsets. */
-                constexpr uint32_t ITEMS = SLOT / 32u / 128u;
+                /* An item is 16 codes: 16 bytes that come in, two 16-byte pieces of fp16 that go out.  A pass of a warp is 8 rows x 64
+                 * dims: four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has
+                 * SUB tiles of 16 rows of the slot, NB blocks of 64 dims each, two passes to a block: pages are looked up once per tile
+                 * and the rest are constant offsets.  Codes and scales arrive by asynchronous copies, RAWS slots ahead, in places that
+                 * this warp alone uses (through registers, a slot ahead: 8192 tokens over 16 384 1813 us, heads of 256 8650). */
+                constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / 4u;
                 constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
-                struct Raw { uint4 w[ITEMS]; uint32_t s[ITEMS]; };   /* codes; the two scales of 64 dims of a row */
                 const uint32_t wi = warp - 8u, r8 = lane >> 2, c4 = lane & 3u;
-                auto load = [&](Raw &r, const Job &job, auto nb) {
+                const uint32_t raw0 = sR + SLOTS * SLOT + wi * WARP_RAW;
+                uint32_t asked = 0, is_v = 0;             /* slots requested so far; bit i: slot i of the last 32 is of V */
+                auto request = [&](const Job &job, auto nb) {
                     constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB;
+                    const uint32_t raw = raw0 + asked % RAWS * C::RAW;
                     const uint32_t sub0 = (HD == 256 && job.v ? job.part * 4u : 0u) + wi * SUB, col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
                     const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
 #pragma unroll
                     for (uint32_t i = 0; i < SUB; i++) {
                         const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)(sub0 + i));
                         const uint32_t q = job.p0 + (sub0 + i) * 16u;
-                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + r8 * ROW;
+                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + r8 * ROW + col;
 #pragma unroll
                         for (uint32_t x = 0; x < 2; x++) {   /* rows r8 and r8 + 8 */
                             const bool there = page >= 0 && q + r8 + 8u * x < n_kv;
 #pragma unroll
-                            for (uint32_t b = 0; b < NB; b++) {
-                                const uint32_t k = (i * 2u + x) * NB + b;
-                                r.w[k] = make_uint4(0u, 0u, 0u, 0u);
-                                r.s[k] = 0u;
-                                if (there) {
-                                    r.w[k] = *reinterpret_cast<const uint4 *>(rec + 8u * x * ROW + col + b * 64u);
-                                    r.s[k] = *reinterpret_cast<const uint32_t *>(rec + 8u * x * ROW + sc + b * 4u);
-                                }
-                            }
+                            for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + ((i * 2u + x) * NB + b) * 512u + lane * 16u, rec + 8u * x * ROW + b * 64u, there);
                         }
+                    }
+                    if (SUB == 2u || lane < 16u) {   /* the scales of a row of this warp's */
+                        const uint32_t q = job.p0 + sub0 * 16u + lane;
+                        const int32_t page = __shfl_sync(SUB == 2u ? 0xffffffffu : 0xffffu, job.pages, (int)(sub0 + (lane >> 4)));
+                        copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), sub_tile(page < 0 ? 0 : page, q) + (q & 15u) * ROW + sc, page >= 0 && q < n_kv);
                     }
                 };
                 const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
-                auto store = [&](const Raw &r, const Job &job, auto nb) {
+                auto convert = [&](auto nb) {
                     constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
+                    const uint32_t raw = raw0 + at % RAWS * C::RAW;
+                    uint4 w[ITEMS];
+                    uint32_t sc[ITEMS];
+#pragma unroll
+                    for (uint32_t k = 0; k < ITEMS; k++) {
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w) : "r"(raw + k * 512u + lane * 16u) : "memory");
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k]) : "r"(raw + ITEMS * 512u + ((k / NB >> 1) * 16u + (k / NB & 1u) * 8u + r8) * (NB * 4u) + k % NB * 4u) : "memory");
+                    }
                     wait_empty();
                     if (!ok) return;
                     const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * SUB * 16u + r8) * 128u;
                     const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
 #pragma unroll
                     for (uint32_t k = 0; k < ITEMS; k++) {
-                        const uint32_t sc = __byte_perm(r.s[k], 0u, scale_sel), off = k / NB * 1024u + k % NB * BLOCK;
-                        const uint32_t w[4] = {r.w[k].x ^ 0x80808080u, r.w[k].y ^ 0x80808080u, r.w[k].z ^ 0x80808080u, r.w[k].w ^ 0x80808080u};
+                        const uint32_t s2 = __byte_perm(sc[k], 0u, scale_sel), off = k / NB * 1024u + k % NB * BLOCK;
+                        const uint32_t u[4] = {w[k].x ^ 0x80808080u, w[k].y ^ 0x80808080u, w[k].z ^ 0x80808080u, w[k].w ^ 0x80808080u};
                         uint32_t o[8];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            o[2 * e] = h2u(__hmul2(codes2<0x4140>(w[e]), *reinterpret_cast<const __half2 *>(&sc)));
-                            o[2 * e + 1] = h2u(__hmul2(codes2<0x4342>(w[e]), *reinterpret_cast<const __half2 *>(&sc)));
+                            o[2 * e] = h2u(__hmul2(codes2<0x4140>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
+                            o[2 * e + 1] = h2u(__hmul2(codes2<0x4342>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
                         }
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a0 + off), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a1 + off), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
                     }
                     fence_async_smem();
-                    __syncwarp();
+                    __syncwarp();   /* and the raw slot has been read by all lanes */
                     if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
                     at++;
                 };
-                auto load_job = [&](Raw &r, const Job &job) {
-                    if (NBK != NBV && job.v) load(r, job, std::integral_constant<uint32_t, NBV>());
-                    else load(r, job, std::integral_constant<uint32_t, NBK>());
+                bool more = true;
+                auto request_next = [&]() {   /* a group per call, so that they can be counted */
+                    Job job;
+                    more = more && next_job(job);
+                    if (more) {
+                        if (NBK != NBV && job.v) request(job, std::integral_constant<uint32_t, NBV>());
+                        else request(job, std::integral_constant<uint32_t, NBK>());
+                        is_v = (is_v & ~(1u << (asked & 31u))) | (job.v ? 1u : 0u) << (asked & 31u);
+                        asked++;
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
                 };
-                auto store_job = [&](const Raw &r, const Job &job) {
-                    if (NBK != NBV && job.v) store(r, job, std::integral_constant<uint32_t, NBV>());
-                    else store(r, job, std::integral_constant<uint32_t, NBK>());
-                };
-                Raw r0, r1;
-                Job j0, j1;
-                bool more = next_job(j0);
-                if (more) load_job(r0, j0);
-                while (more && ok) {
-                    more = next_job(j1);
-                    if (more) load_job(r1, j1);
-                    store_job(r0, j0);
-                    if (!more || !ok) break;
-                    more = next_job(j0);
-                    if (more) load_job(r0, j0);
-                    store_job(r1, j1);
+                for (uint32_t d = 0; d < RAWS; d++) request_next();
+                while (ok && at < asked) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(RAWS - 1u) : "memory");
+                    __syncwarp();
+                    if (NBK != NBV && (is_v >> (at & 31u)) & 1u) convert(std::integral_constant<uint32_t, NBV>());
+                    else convert(std::integral_constant<uint32_t, NBK>());
+                    if (ok) request_next();
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
             } else {
                 Job job;
                 while (ok && next_job(job)) {
@@ -804,7 +825,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
 
 template <int KIND, int HD>
 bool chunk(PagedParams p, float *scratch) {
-    using C = ChunkCfg<HD>;
+    using C = ChunkCfg<KIND, HD>;
     static bool attr = false;
     if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_chunk_k<KIND, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
     attr = true;
