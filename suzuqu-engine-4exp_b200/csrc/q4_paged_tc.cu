@@ -9,11 +9,11 @@
  *
  *   warps 0 - 7    softmax: thread r owns row r (hd 256: two threads, half of a unit's positions each): its scores out of tensor
  *                  memory, causal mask, running maximum with lazy rescale, weights as fp16 back into the columns they came from
- *   warps 8 - 11   producers: K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads
- *                  them: bulk copies.  q8_0: codes and scales by asynchronous copies, three slots ahead, then fp16(code x scale)
- *                  into the slot (7 instructions per 4 values)
- *   warp 12        issues the products: O += P V of a unit of positions as its weights appear, then the scores that take over the
- *                  buffer
+ *   producers      K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads them: bulk copies.
+ *                  q8_0: codes and scales by asynchronous copies, three slots ahead, then fp16(code x scale) into the slot
+ *                  (7 instructions per 4 values)
+ *   issuer         the products: O += P V of a unit of positions as its weights appear, then the scores that take over the buffer
+ *   walker         the share's pieces, ahead of the others
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
  *
  * Every wait is bounded: on expiry the block's waits all end, Q4E_CUDA is set, and tensor memory is freed.
@@ -30,7 +30,7 @@ using namespace q4tc;
 
 namespace {
 
-constexpr uint32_t CK_THREADS = 512, CK_BN = 128;
+constexpr uint32_t CK_BN = 128;
 constexpr uint32_t CK_SPIN_LIMIT = 1u << 22;
 constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
 constexpr uint32_t PIECES = 4;          /* pieces that are walked ahead */
@@ -41,8 +41,13 @@ template <int KIND, int HD>
 struct ChunkCfg {
     static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
     static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : KIND == Q4K_Q8 ? 3u : 5u;
-    static constexpr uint32_t ITEMS = SLOT / 32u / 128u;          /* of 16 codes, per producer thread and slot */
-    static constexpr uint32_t RAW = KIND == Q4K_Q8 ? 4u * ITEMS * 544u : 0u;   /* codes and scales of a slot */
+    static constexpr uint32_t PW = 4u;                            /* producer warps */
+    static constexpr uint32_t ISSUER = 8u + PW, WALKER = ISSUER + 1u, THREADS = (ISSUER + 4u) * 32u;
+    static constexpr uint32_t ITEMS = SLOT / 32u / (PW * 32u);    /* of 16 codes, per producer thread and slot */
+    static constexpr uint32_t RAW = KIND == Q4K_Q8 ? PW * ITEMS * 544u : 0u;   /* codes and scales of a slot */
+    /* registers of a thread: the block's 512 x 128 are 128 threads x (2 softmax + producers + the rest) */
+    static constexpr uint32_t R_SOFTMAX = KIND == Q4K_Q8 ? 168u : 184u, R_PRODUCER = KIND == Q4K_Q8 ? 120u : 88u, R_REST = 56u;
+    static_assert(2u * R_SOFTMAX + R_PRODUCER + R_REST <= 512u, "register split");
     static constexpr uint32_t PARTS = HD == 256 ? 2u : 1u;        /* slots of a K or a V tile: K by 128 dims, V by 64 positions */
     static constexpr uint32_t QG = 128u * HD * 2u;                /* one group's queries */
     static constexpr uint32_t REC = HD + 4u;
@@ -133,6 +138,7 @@ struct Piece {
     uint32_t tok0, n_here, kh;   /* the unit's first token, its tokens, its kv head */
     uint32_t req, st, here;      /* the piece: tiles [st, st + here) of the unit; here = 0: there are no more */
     uint32_t tiles;              /* of the unit */
+    bool gone;                   /* some of its positions are on pages that are not the pool's */
 };
 struct Walk {
     uint64_t left;               /* tiles of the share still to come */
@@ -168,9 +174,9 @@ struct Walk {
 };
 
 template <int KIND, int HD>
-__global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
+__global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
     using C = ChunkCfg<KIND, HD>;
-    constexpr uint32_t NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
+    constexpr uint32_t CK_THREADS = C::THREADS, NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
     constexpr uint32_t O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -181,10 +187,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
     uint8_t *base = smem_dyn + (sQ - smem_u32(smem_dyn));
     const uint32_t tpu = P.tpg * NQ;
 
-    if (warp == 12u) {
+    if (warp == C::ISSUER) {
         if (lane == 0) {
             for (uint32_t s = 0; s < SLOTS; s++) {
-                mbar_init(full + 8 * s, KIND == Q4K_Q8 ? 4u : 1u);
+                mbar_init(full + 8 * s, C::PW);
                 mbar_init(empty + 8 * s, 1);
             }
             for (uint32_t s = 0; s < 4; s++) {
@@ -196,7 +202,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
             mbar_init(bar_q, 256);
             for (uint32_t s = 0; s < PIECES; s++) {
                 mbar_init(w_full + 8 * s, 1);
-                mbar_init(w_empty + 8 * s, 9u + (KIND == Q4K_Q8 ? 4u : 1u));   /* a warp each of softmax, issuer and producers */
+                mbar_init(w_empty + 8 * s, 9u + C::PW);   /* a warp each of softmax, issuer and producers */
             }
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(0u) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -273,6 +279,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
         }
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.before), "=r"(p.tok0), "=r"(p.n_here), "=r"(p.kh) : "r"(a) : "memory");
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p.req), "=r"(p.st), "=r"(p.here), "=r"(p.tiles) : "r"(a + 16u) : "memory");
+        p.gone = p.n_here >> 31;
+        p.n_here &= 0x7fffffffu;
         return p.here != 0u;
     };
     auto piece_done = [&]() {
@@ -282,9 +290,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
     };
     Piece p;
 
-    if (warp >= 12u) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12u) {
+    if (warp >= C::ISSUER) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
+        if (warp == C::ISSUER) {
             /* ================= issuer: a converged warp, one elected lane ================= */
             constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(UN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -386,7 +394,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 }
             }
         }
-        if (warp == 13u) {
+        if (warp == C::WALKER) {
             /* ================= walker: the share's pieces, and the unit that ends in this block ================= */
             int4 end_of = make_int4(-1, 0, 0, 0);
             uint64_t s_now = s_begin;
@@ -397,10 +405,18 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 const uint32_t e = n % PIECES, a = s_piece + e * 32u;
                 p.here = 0;
                 const bool more = W.next(P, tpu, p);
+                bool gone = false;
+                if (more) {   /* the softmax looks for missing pages only where there are any */
+                    const uint32_t last = min((p.st + p.here) * CK_BN, p.before + p.n_here) - 1u;
+                    const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
+                    for (uint32_t i = (p.st * CK_BN >> P.page_shift) + lane; i <= last >> P.page_shift; i += 32u) gone |= (uint32_t)tab[i] >= P.n_pages;
+                    gone = __any_sync(0xffffffffu, gone);
+                    if (gone && lane == 0) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+                }
                 if (n >= PIECES) ok = ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
                 if (!ok) break;
                 if (lane == 0) {
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here), "r"(p.kh) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here | (gone ? 0x80000000u : 0u)), "r"(p.kh) : "memory");
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
                     mbar_arrive(w_full + 8 * e);
                 }
@@ -413,9 +429,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
         }
     } else if (warp >= 8u) {
         /* ================= producers ================= */
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_PRODUCER));
         const uint32_t ptid = tid - 256u, mask = (1u << P.page_shift) - 1u;
-        if (KIND == Q4K_Q8 || warp == 8u) {
+        {
             uint32_t at = 0;                          /* slots so far */
             uint32_t kt = 0, vt = 0, part = 0, n_kv = 0;   /* of the piece: next K and V tile, slot of the tile; positions */
             uint32_t k_count = 0;
@@ -449,7 +465,6 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                         if (h0 < 0 || (uint32_t)h0 >= P.n_pages) h0 = -1;
                         e_next = entry(kt + 1u);
                         const uint32_t gone = __ballot_sync(0xffffffffu, h0 < 0) & 0xffu;
-                        if (gone && ptid == 0u) atomicOr(P.err, (uint32_t)Q4E_RANGE);
                         /* read by the softmax warps once the scores of the tile are there */
                         if (ptid == 0u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (k_count & 7u)), "r"(gone) : "memory");
                         k_count++;
@@ -474,51 +489,48 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
             if constexpr (KIND == Q4K_Q8) {
                 /* An item is 16 codes: 16 bytes that come in, two 16-byte pieces of fp16 that go out.  A pass of a warp is 8 rows x 64
                  * dims: four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has
-                 * SUB tiles of 16 rows of the slot, NB blocks of 64 dims each, two passes to a block: pages are looked up once per tile
-                 * and the rest are constant offsets.  Codes and scales arrive by asynchronous copies, RAWS slots ahead, in places that
-                 * this warp alone uses (through registers, a slot ahead: 8192 tokens over 16 384 1813 us, heads of 256 8650). */
-                constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / 4u;
+                 * RG groups of 8 rows of the slot, NB blocks of 64 dims (passes) to each.  Codes and scales arrive by asynchronous
+                 * copies, RAWS slots ahead, in places that this warp alone uses (through registers, a slot ahead, 8192 tokens over
+                 * 16 384 took 1813 us instead of 1451, with heads of 256 8650 instead of 4570). */
+                constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / C::PW;
                 constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
                 const uint32_t wi = warp - 8u, r8 = lane >> 2, c4 = lane & 3u;
                 const uint32_t raw0 = sR + SLOTS * SLOT + wi * WARP_RAW;
                 uint32_t asked = 0, is_v = 0;             /* slots requested so far; bit i: slot i of the last 32 is of V */
                 auto request = [&](const Job &job, auto nb) {
-                    constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB;
+                    constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB;
                     const uint32_t raw = raw0 + asked % RAWS * C::RAW;
-                    const uint32_t sub0 = (HD == 256 && job.v ? job.part * 4u : 0u) + wi * SUB, col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
+                    const uint32_t g0 = (HD == 256 && job.v ? job.part * 8u : 0u) + wi * RG, col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
                     const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
 #pragma unroll
-                    for (uint32_t i = 0; i < SUB; i++) {
-                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)(sub0 + i));
-                        const uint32_t q = job.p0 + (sub0 + i) * 16u;
-                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + r8 * ROW + col;
+                    for (uint32_t i = 0; i < RG; i++) {
+                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)((g0 + i) >> 1));
+                        const uint32_t q = job.p0 + (g0 + i) * 8u;
+                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + ((q & 8u) + r8) * ROW + col;
+                        const bool there = page >= 0 && q + r8 < n_kv;
 #pragma unroll
-                        for (uint32_t x = 0; x < 2; x++) {   /* rows r8 and r8 + 8 */
-                            const bool there = page >= 0 && q + r8 + 8u * x < n_kv;
-#pragma unroll
-                            for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + ((i * 2u + x) * NB + b) * 512u + lane * 16u, rec + 8u * x * ROW + b * 64u, there);
-                        }
+                        for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, rec + b * 64u, there);
                     }
-                    if (SUB == 2u || lane < 16u) {   /* the scales of a row of this warp's */
-                        const uint32_t q = job.p0 + sub0 * 16u + lane;
-                        const int32_t page = __shfl_sync(SUB == 2u ? 0xffffffffu : 0xffffu, job.pages, (int)(sub0 + (lane >> 4)));
+                    if (lane < RG * 8u) {   /* the scales of a row of this warp's */
+                        const uint32_t q = job.p0 + g0 * 8u + lane;
+                        const int32_t page = __shfl_sync((uint32_t)((1ull << RG * 8u) - 1u), job.pages, (int)((g0 + (lane >> 3)) >> 1));
                         copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), sub_tile(page < 0 ? 0 : page, q) + (q & 15u) * ROW + sc, page >= 0 && q < n_kv);
                     }
                 };
                 const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
                 auto convert = [&](auto nb) {
-                    constexpr uint32_t NB = decltype(nb)::value, SUB = ITEMS / 2u / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
+                    constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
                     const uint32_t raw = raw0 + at % RAWS * C::RAW;
                     uint4 w[ITEMS];
                     uint32_t sc[ITEMS];
 #pragma unroll
                     for (uint32_t k = 0; k < ITEMS; k++) {
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w) : "r"(raw + k * 512u + lane * 16u) : "memory");
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k]) : "r"(raw + ITEMS * 512u + ((k / NB >> 1) * 16u + (k / NB & 1u) * 8u + r8) * (NB * 4u) + k % NB * 4u) : "memory");
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k]) : "r"(raw + ITEMS * 512u + (k / NB * 8u + r8) * (NB * 4u) + k % NB * 4u) : "memory");
                     }
                     wait_empty();
                     if (!ok) return;
-                    const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * SUB * 16u + r8) * 128u;
+                    const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * RG * 8u + r8) * 128u;
                     const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
 #pragma unroll
                     for (uint32_t k = 0; k < ITEMS; k++) {
@@ -560,40 +572,36 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
             } else {
+                /* a slot is 16 units of 2 KB (8 at hd 64): 16 rows of a block of 64 dims.  One bulk copy each, shared out over the warps: a
+                 * warp issues one in about 100 cycles */
+                constexpr uint32_t UNITS = SLOT / 2048u / C::PW;
                 Job job;
                 while (ok && next_job(job)) {
                     wait_empty();
                     if (!ok) break;
                     const uint32_t s = at % SLOTS, dst = sR + s * SLOT, bar = full + 8 * s;
-                    const uint32_t rows = HD == 256 && job.v ? 64u : 128u, p0 = job.p0 + (HD == 256 && job.v ? job.part * 64u : 0u);
-                    constexpr uint32_t BLOCKS = HD == 256 ? 2u : HD / 64u;
-                    const uint32_t blocks_here = HD == 256 && job.v ? 4u : BLOCKS, block0 = HD == 256 && !job.v ? job.part * 2u : 0u;
-                    /* lane i < rows / 16: 16 positions; whole rows of 128 bytes of every block, as many as there are */
-                    const uint32_t q = p0 + lane * 16u;
-                    const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)(((q - job.p0) >> 4) & 7u));
-                    uint32_t live = lane * 16u < rows && page >= 0 && q < n_kv ? min(16u, n_kv - q) : 0u;
-                    const uint32_t all = __reduce_add_sync(0xffffffffu, live);
-                    if (job.v && all < rows) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
-                        for (uint32_t i = lane; i < rows; i += 32u) {
-                            const uint32_t there = __shfl_sync(0xffffffffu, live, (int)(i >> 4));
-                            if ((i & 15u) >= there)
-                                for (uint32_t b = 0; b < blocks_here; b++)
+                    const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u;
+                    const uint32_t unit = (warp - 8u) * UNITS + (lane & (UNITS - 1u)), tile = unit / nblk, b = unit - tile * nblk;
+                    const uint32_t in = (HD == 256 && job.v ? job.part * 4u : 0u) + tile, q = job.p0 + in * 16u;
+                    const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)in);
+                    const uint32_t live = page >= 0 && q < n_kv ? min(16u, n_kv - q) : 0u, to = dst + b * rows * 128u + tile * 2048u;
+                    const uint32_t all = __reduce_add_sync(0xffffffffu, lane < UNITS ? live : 0u);
+                    if (job.v && all < 16u * UNITS) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
+                        for (uint32_t u = 0; u < UNITS; u++) {
+                            const uint32_t there = __shfl_sync(0xffffffffu, live, (int)u), a = __shfl_sync(0xffffffffu, to, (int)u);
 #pragma unroll
-                                    for (uint32_t c = 0; c < 8; c++)
-                                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + b * rows * 128u + i * 128u + c * 16u), "r"(0u) : "memory");
+                            for (uint32_t i = 0; i < 4; i++)
+                                if (i * 4u + (lane >> 3) >= there) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a + i * 512u + lane * 16u), "r"(0u) : "memory");
                         }
                         fence_async_smem();
                         __syncwarp();
                     }
                     if (lane == 0) {
-                        if (all) mbar_expect_tx(bar, all * 128u * blocks_here);
+                        if (all) mbar_expect_tx(bar, all * 128u);
                         else mbar_arrive(bar);
                     }
                     __syncwarp();
-                    if (live) {
-                        const uint8_t *src = sub_tile(page, q) + (job.v ? TILE / 2u : 0u) + block0 * 2048u;
-                        for (uint32_t b = 0; b < blocks_here; b++) bulk_load(dst + b * rows * 128u + lane * 2048u, src + b * 2048u, live * 128u, bar);
-                    }
+                    if (lane < UNITS && live) bulk_load(to, sub_tile(page, q) + (job.v ? TILE / 2u : 0u) + ((HD == 256 && !job.v ? job.part * 2u : 0u) + b) * 2048u, live * 128u, bar);
                     at++;
                 }
                 /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
@@ -604,8 +612,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
         }
     } else {
         /* ================= softmax ================= */
-        /* 128 threads x (2 x 168 + 120 + 56) registers: the block's 512 x 128 */
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFTMAX));
         const uint32_t g = NQ == 2u ? warp >> 2 : 0u, h = NQ == 2u ? 0u : warp >> 2, r = tid & 127u, t_lane = tmem + (((warp & 3u) * 32u) << 16);
         const uint32_t tl = r / P.gqa, head_in = r - tl * P.gqa;
         auto pair_sync = [&]() {   /* the two warps of the same 32 rows (hd 256) */
@@ -689,9 +696,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
 #pragma unroll
                 for (int c = 0; c < (int)TU / 32; c++) tmem_ld32(t_s + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
                 tmem_wait_ld();
-                uint32_t gone;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(gone) : "r"(s_gone + 4u * ((tiles_seen + (NQ == 2u ? u >> 1 : u)) & 7u)) : "memory");
-                if (__builtin_expect(gone != 0u, 0)) {   /* positions on pages that are not the pool's */
+                if (__builtin_expect(p.gone, 0)) {   /* positions on pages that are not the pool's */
+                    uint32_t gone;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(gone) : "r"(s_gone + 4u * ((tiles_seen + (NQ == 2u ? u >> 1 : u)) & 7u)) : "memory");
 #pragma unroll
                     for (int k = 0; k < (int)TU; k++)
                         if ((gone >> (((p0 & 127u) + k) >> 4)) & 1u) s[k] = -CUDART_INF_F;
@@ -717,7 +724,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 };
                 /* the exponentials start against the maximum of the units before, while this unit's own is being formed; where that
                  * is not within 2^8 the reference moves and they are taken again */
-                if (u > 0u) exps();
+                if (NQ == 2u || u > 0u) exps();   /* of a short chunk's halves the first unit is a good part */
                 float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
                 for (int k = 0; k < (int)TU; k += 8) {
@@ -726,7 +733,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
                 }
                 float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2e;   /* scale > 0 */
                 bool grow = m_new > m_ref + CK_RESCALE_TAU;   /* also true on the first live unit (m_ref = -inf) */
-                const bool any = u == 0u || (NQ == 2u ? __any_sync(0xffffffffu, grow) : pair_any(grow));
+                const bool any = NQ == 2u ? __any_sync(0xffffffffu, grow) : u == 0u || pair_any(grow);
                 if (__builtin_expect(any, 0)) {
                     if (NQ == 1u) {   /* both halves of a row keep one reference: they share its O */
                         m_new = fmaxf(m_new, partner(m_new));
@@ -820,7 +827,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) q4_pg_chunk_k(const PagedParams
     if (!ok && lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
     tc_fence_before();
     __syncthreads();
-    if (warp == 12u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    if (warp == C::ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
 template <int KIND, int HD>
@@ -834,7 +841,7 @@ bool chunk(PagedParams p, float *scratch) {
     p.ends = reinterpret_cast<int4 *>(scratch + (size_t)blocks * 2u * C::ROWS * C::REC);
     p.tpg = 128u / p.gqa;
     p.group_rows = 128u;
-    return q4i_launch_pdl("pages_attend launch", q4_pg_chunk_k<KIND, HD>, dim3(blocks), CK_THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
+    return q4i_launch_pdl("pages_attend launch", q4_pg_chunk_k<KIND, HD>, dim3(blocks), C::THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
 }
 
 }  // namespace
