@@ -36,6 +36,9 @@ constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
 constexpr uint32_t PIECES = 4;          /* pieces that are walked ahead */
 constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the reference moves */
 
+/* A piece costs about as much besides its tiles (queries in, outputs out, the first scores) as this many of them: a unit counts as so
+ * many more steps when the work is shared out.  Only tiles are walked; a share may hold none. */
+constexpr uint32_t CK_EXTRA = 2;
 constexpr uint32_t RAWS = 3;            /* slots of q8_0 codes on their way */
 template <int KIND, int HD>
 struct ChunkCfg {
@@ -126,10 +129,10 @@ __device__ __forceinline__ PgReq chunk_request(const PagedParams &P, uint32_t r,
     if (q.add <= P.add_split) q.add = 0u;
     return q;
 }
-__device__ __forceinline__ uint64_t request_tiles(const PagedParams &P, const PgReq &R, uint32_t tpu) {
+__device__ __forceinline__ uint64_t request_steps(const PagedParams &P, const PgReq &R, uint32_t tpu) {
     if (!R.add) return 0u;
     const uint32_t groups = (R.add + tpu - 1u) / tpu;
-    return (tiles_before(R, tpu, groups - 1u) + unit_tiles(R, tpu, groups - 1u)) * P.n_kvh;
+    return (tiles_before(R, tpu, groups - 1u) + unit_tiles(R, tpu, groups - 1u) + (uint64_t)CK_EXTRA * groups) * P.n_kvh;
 }
 
 /* A share's pieces, one after the other: one warp walks them ahead of the others and leaves them in shared memory */
@@ -141,35 +144,44 @@ struct Piece {
     bool gone;                   /* some of its positions are on pages that are not the pool's */
 };
 struct Walk {
-    uint64_t left;               /* tiles of the share still to come */
+    uint64_t left;               /* steps of the share still to come */
+    uint64_t now;                /* of all steps, the next one */
+    uint64_t unit_at;            /* of all steps, the first tile of the unit of the last piece */
     uint32_t req, kh, g, st;
     PgReq R;
-    __device__ __forceinline__ void begin(const PagedParams &P, uint64_t n, uint32_t r, uint32_t kh_, uint32_t g_, uint32_t st_) {
+    __device__ __forceinline__ void begin(const PagedParams &P, uint64_t s0, uint64_t n, uint32_t r, uint32_t kh_, uint32_t g_, uint32_t st_) {
         bool bad;
-        left = n; req = r; kh = kh_; g = g_; st = st_;
+        left = n; now = s0; req = r; kh = kh_; g = g_; st = st_;
         R = chunk_request(P, r, bad);
     }
     __device__ __forceinline__ bool next(const PagedParams &P, uint32_t tpu, Piece &p) {
-        if (!left) return false;
-        bool bad;
-        while (!R.add) R = chunk_request(P, ++req, bad);   /* `left` tiles lie ahead: there is one with tokens */
-        p.tiles = unit_tiles(R, tpu, g);
-        p.n_here = min(tpu, R.add - g * tpu);
-        p.before = R.held + g * tpu; p.tok0 = R.tok0 + g * tpu; p.kh = kh; p.req = req; p.st = st;
-        p.here = (uint32_t)min((uint64_t)(p.tiles - st), left);
-        left -= p.here;
-        st += p.here;
-        if (st == p.tiles) {
-            st = 0;
-            if (++g * (uint64_t)tpu >= R.add) {
-                g = 0;
-                if (++kh == P.n_kvh) {
-                    kh = 0;
-                    R.add = 0;
+        while (left) {
+            bool bad;
+            while (!R.add) R = chunk_request(P, ++req, bad);   /* `left` steps lie ahead: there is one with tokens */
+            p.tiles = unit_tiles(R, tpu, g);
+            p.n_here = min(tpu, R.add - g * tpu);
+            p.before = R.held + g * tpu; p.tok0 = R.tok0 + g * tpu; p.kh = kh; p.req = req;
+            const uint32_t here = (uint32_t)min((uint64_t)(p.tiles + CK_EXTRA - st), left), end = st + here;
+            unit_at = now - st + CK_EXTRA;
+            p.st = max(st, CK_EXTRA) - CK_EXTRA;
+            p.here = max(end, CK_EXTRA) - CK_EXTRA - p.st;
+            left -= here;
+            now += here;
+            st = end;
+            if (st == p.tiles + CK_EXTRA) {
+                st = 0;
+                if (++g * (uint64_t)tpu >= R.add) {
+                    g = 0;
+                    if (++kh == P.n_kvh) {
+                        kh = 0;
+                        R.add = 0;
+                    }
                 }
             }
+            if (p.here) return true;
         }
-        return true;
+        p.here = 0;
+        return false;
     }
 };
 
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         uint64_t mine = 0, before = 0;
         bool bad, any_bad = false;
         for (uint32_t r = r0; r < r1; r++) {
-            mine += request_tiles(P, chunk_request(P, r, bad), tpu);
+            mine += request_steps(P, chunk_request(P, r, bad), tpu);
             any_bad |= bad;
         }
         uint64_t x = mine;
@@ -244,7 +256,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         if (s_begin < s_end && before <= s_begin && s_begin < before + mine)
             for (uint32_t r = r0; r < r1; r++) {
                 const PgReq R = chunk_request(P, r, bad);
-                const uint64_t n = request_tiles(P, R, tpu);
+                const uint64_t n = request_steps(P, R, tpu);
                 if (s_begin < before + n) {
                     const uint64_t per_kh = n / P.n_kvh, off = s_begin - before;
                     const uint32_t kh = (uint32_t)(off / per_kh), groups = (R.add + tpu - 1u) / tpu;
@@ -252,10 +264,10 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     uint32_t lo = 0, hi = groups - 1u;   /* the last group that begins at or before `in` */
                     while (lo < hi) {
                         const uint32_t mid = (lo + hi + 1u) >> 1;
-                        if (tiles_before(R, tpu, mid) <= in) lo = mid;
+                        if (tiles_before(R, tpu, mid) + (uint64_t)CK_EXTRA * mid <= in) lo = mid;
                         else hi = mid - 1u;
                     }
-                    const uint32_t st = (uint32_t)(in - tiles_before(R, tpu, lo));
+                    const uint32_t st = (uint32_t)(in - (tiles_before(R, tpu, lo) + (uint64_t)CK_EXTRA * lo));
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"(kh), "r"(lo), "r"(st) : "memory");
                     break;
                 }
@@ -397,13 +409,11 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         if (warp == C::WALKER) {
             /* ================= walker: the share's pieces, and the unit that ends in this block ================= */
             int4 end_of = make_int4(-1, 0, 0, 0);
-            uint64_t s_now = s_begin;
             Walk W;
             W.left = 0;
-            if (s_begin < s_end) W.begin(P, s_end - s_begin, w_req, w_kh, w_g, w_st);
+            if (s_begin < s_end) W.begin(P, s_begin, s_end - s_begin, w_req, w_kh, w_g, w_st);
             for (uint32_t n = 0; ok; n++) {
                 const uint32_t e = n % PIECES, a = s_piece + e * 32u;
-                p.here = 0;
                 const bool more = W.next(P, tpu, p);
                 bool gone = false;
                 if (more) {   /* the softmax looks for missing pages only where there are any */
@@ -412,6 +422,16 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     for (uint32_t i = (p.st * CK_BN >> P.page_shift) + lane; i <= last >> P.page_shift; i += 32u) gone |= (uint32_t)tab[i] >= P.n_pages;
                     gone = __any_sync(0xffffffffu, gone);
                     if (gone && lane == 0) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+                }
+                if (more) {   /* its queries, and the gates if it is a whole unit, are on their way when it begins */
+                    const bool whole = p.st == 0u && p.here == p.tiles;
+                    const uint32_t q_line = P.gqa * HD * (P.q_bf16 ? 2u : 4u) / 128u, g_line = whole && P.gate ? P.gqa * HD / 32u : 0u;   /* lines of 128 bytes per token */
+                    for (uint32_t i = lane; i < p.n_here * (q_line + g_line); i += 32u) {
+                        const uint32_t t = i / (q_line + g_line), x = i - t * (q_line + g_line);
+                        const size_t at = ((size_t)(p.tok0 + t) * P.n_head + (size_t)p.kh * P.gqa) * HD;
+                        const uint8_t *line = x < q_line ? (const uint8_t *)P.q + at * (P.q_bf16 ? 2u : 4u) + x * 128u : (const uint8_t *)(P.gate + at) + (x - q_line) * 128u;
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+                    }
                 }
                 if (n >= PIECES) ok = ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
                 if (!ok) break;
@@ -422,8 +442,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 }
                 if (!more) break;
                 if (p.st > 0u && p.st + p.here == p.tiles)   /* the unit ends here; it began in block .. */
-                    end_of = make_int4((int32_t)((((s_now - p.st) + 1u) * blocks - 1u) / total), (int32_t)p.tok0, (int32_t)p.n_here, (int32_t)p.kh);
-                s_now += p.here;
+                    end_of = make_int4((int32_t)(((W.unit_at + 1u) * blocks - 1u) / total), (int32_t)p.tok0, (int32_t)p.n_here, (int32_t)p.kh);
             }
             if (lane == 0) P.ends[blockIdx.x] = end_of;
         }
@@ -614,7 +633,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         /* ================= softmax ================= */
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFTMAX));
         const uint32_t g = NQ == 2u ? warp >> 2 : 0u, h = NQ == 2u ? 0u : warp >> 2, r = tid & 127u, t_lane = tmem + (((warp & 3u) * 32u) << 16);
-        const uint32_t tl = r / P.gqa, head_in = r - tl * P.gqa;
+        const uint32_t inv_gqa = 65536u / P.gqa + 1u;   /* row / gqa = row * inv_gqa >> 16 for rows below 128, gqa up to 16 */
+        const uint32_t tl = r * inv_gqa >> 16;
         auto pair_sync = [&]() {   /* the two warps of the same 32 rows (hd 256) */
             __syncwarp();
             asm volatile("bar.sync %0, 64;" ::"r"(1u + (warp & 3u)) : "memory");
@@ -632,8 +652,17 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(s_xch + 4u * (tid ^ 128u)) : "memory");
             return x;
         };
+        /* whether x holds for all warps of the group (hd 256: all eight): they take up and leave pieces together, whichever of them gave up */
+        auto agree = [&](bool x) -> bool {
+            uint32_t all;
+            __syncwarp();
+            asm volatile("{ .reg .pred p, q; setp.ne.u32 q, %1, 0; bar.red.and.pred p, %2, %3, q; selp.u32 %0, 1, 0, p; }"
+                         : "=r"(all) : "r"((uint32_t)x), "r"(NQ == 2u ? 5u + g : 5u), "n"(NQ == 2u ? 128 : 256) : "memory");
+            return all != 0u;
+        };
         uint32_t use = 0, tiles_seen = 0;   /* units of this group so far; K tiles so far */
-        while (ok && next_piece(p)) {
+        while (ok) {
+            if (!agree(next_piece(p))) break;
             const bool active = g == 0u || p.n_here > P.tpg;
             /* ---- queries as fp16, swizzled rows of 64 dims: the products of the piece before have read theirs (its last scores are here) */
             {
@@ -645,7 +674,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         uint4 w[BATCH][2];
 #pragma unroll
                         for (uint32_t k = 0; k < BATCH; k++) {
-                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER, ql = row / P.gqa, qtok = g * P.tpg + ql;
+                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER, ql = row * inv_gqa >> 16, qtok = g * P.tpg + ql;
                             w[k][0] = w[k][1] = make_uint4(0u, 0u, 0u, 0u);
                             if (ql < P.tpg && qtok < p.n_here) {
                                 const size_t off = ((size_t)(p.tok0 + qtok) * P.n_head + (size_t)p.kh * P.gqa + (row - ql * P.gqa)) * HD + c * 8u;
@@ -776,51 +805,75 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 l_run += partner(l_run);
                 pair_sync();   /* before the next piece's first exchange */
             }
-            /* ---- the piece's outputs: a thread has a row (hd 256: half of its columns) */
+            /* ---- the piece's outputs.  32 columns at a time go through the warp's share of the query tiles (read by no product any
+             * more), so that rows leave in whole lines: step q of a column block is 4 rows of 32 columns, 8 lanes each.  (From
+             * the threads that hold the rows a piece took 8000 cycles.) */
+            const bool whole = p.st == 0u && p.here == p.tiles;
+            const uint32_t w_row0 = (warp & 3u) * 32u;
+            uint32_t off[8], live = 0;   /* in 16-byte units from the unit's first token */
+#pragma unroll
+            for (uint32_t q = 0; q < 8; q++) {
+                const uint32_t row = w_row0 + 4u * q + (lane >> 3), ti = row * inv_gqa >> 16;
+                if (ti < P.tpg && g * P.tpg + ti < p.n_here) live |= 1u << q;
+                off[q] = whole ? ((g * P.tpg + ti) * P.n_head + p.kh * P.gqa + (row - ti * P.gqa)) * (HD / 4u) + (lane & 7u) : (g * 128u + row) * (C::REC / 4u) + (lane & 7u);
+            }
+            const size_t first = (size_t)p.tok0 * P.n_head * (HD / 4u);
+            float *rec = P.part + ((size_t)blockIdx.x * 2u + (p.st == 0u ? 1u : 0u)) * C::ROWS * C::REC;
             if (active && ok) ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort);
             tc_fence_after();
-            const bool whole = p.st == 0u && p.here == p.tiles;
             if (active && ok) {
                 const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
-                const size_t off = ((size_t)(p.tok0 + tok) * P.n_head + (size_t)p.kh * P.gqa + head_in) * HD;
-                float *rec = P.part + (((size_t)blockIdx.x * 2u + (p.st == 0u ? 1u : 0u)) * C::ROWS + g * 128u + r) * C::REC;
-                if (!whole && row_live && h == 0u) *reinterpret_cast<float2 *>(rec + HD) = make_float2(m_ref, l_run);
+                const uint32_t buf = sQ + warp * (NQ * C::QG / 8u);   /* [32 rows][8 x 16 bytes], piece k of row r at k ^ (r & 7) */
+                if (!whole && row_live && h == 0u) *reinterpret_cast<float2 *>(rec + (size_t)(g * 128u + r) * C::REC + HD) = make_float2(m_ref, l_run);
 #pragma unroll 1
                 for (uint32_t c = h * (HD / 64); c < (NQ == 2u ? HD / 32 : (h + 1u) * (HD / 64)); c++) {
                     float o[32];
+                    float4 x[8], gt[8];
                     tmem_ld32(t_lane + O_COL + g * 128u + 32 * c, o);
+                    if (whole && P.gate) {
+#pragma unroll
+                        for (int q = 0; q < 8; q++)
+                            if ((live >> q) & 1u) gt[q] = reinterpret_cast<const float4 *>(P.gate)[first + off[q] + 8u * c];
+                    }
                     tmem_wait_ld();
-                    if (!row_live) continue;
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k++)
+                        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(buf + lane * 128u + ((k ^ (lane & 7u)) << 4)), "f"(o[4 * k] * inv), "f"(o[4 * k + 1] * inv), "f"(o[4 * k + 2] * inv), "f"(o[4 * k + 3] * inv) : "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t q = 0; q < 8; q++) {
+                        const uint32_t row = 4u * q + (lane >> 3);
+                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x[q].x), "=f"(x[q].y), "=f"(x[q].z), "=f"(x[q].w) : "r"(buf + row * 128u + (((lane & 7u) ^ (row & 7u)) << 4)) : "memory");
+                    }
                     if (!whole) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(rec + 32u * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        for (int q = 0; q < 8; q++)
+                            if ((live >> q) & 1u) reinterpret_cast<float4 *>(rec)[off[q] + 8u * c] = x[q];
                         continue;
                     }
-#pragma unroll
-                    for (int k = 0; k < 32; k++) o[k] *= inv;
                     if (P.gate) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            const float4 gt = *reinterpret_cast<const float4 *>(P.gate + off + 32u * c + k);
-                            o[k] = gated(o[k], gt.x); o[k + 1] = gated(o[k + 1], gt.y); o[k + 2] = gated(o[k + 2], gt.z); o[k + 3] = gated(o[k + 3], gt.w);
-                        }
+                        for (int q = 0; q < 8; q++)
+                            if ((live >> q) & 1u) {
+                                x[q].x = gated(x[q].x, gt[q].x); x[q].y = gated(x[q].y, gt[q].y);
+                                x[q].z = gated(x[q].z, gt[q].z); x[q].w = gated(x[q].w, gt[q].w);
+                            }
                     }
-                    if (P.out_bf16) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            __nv_bfloat162 x[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) x[e] = __floats2bfloat162_rn(o[k + 2 * e], o[k + 2 * e + 1]);
-                            *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + off + 32u * c + k) = *reinterpret_cast<const uint4 *>(x);
+                    for (int q = 0; q < 8; q++) {
+                        if (!((live >> q) & 1u)) continue;
+                        if (P.out_bf16) {
+                            const __nv_bfloat162 b0 = __floats2bfloat162_rn(x[q].x, x[q].y), b1 = __floats2bfloat162_rn(x[q].z, x[q].w);
+                            reinterpret_cast<uint2 *>(P.out)[first + off[q] + 8u * c] = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
+                        } else {
+                            reinterpret_cast<float4 *>(P.out)[first + off[q] + 8u * c] = x[q];
                         }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + off + 32u * c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                 }
             }
             tc_fence_before();   /* the next piece's first product overwrites O behind this thread's next arrival */
-            if (NQ == 1u) ok = !pair_any(!ok);   /* the two warps of a row leave together */
+            ok = agree(ok);   /* and the next piece's queries may come where the outputs were */
             piece_done();
         }
     }
