@@ -13,7 +13,7 @@
  *                  q8_0: codes and scales by asynchronous copies, three slots ahead, then fp16(code x scale) into the slot
  *                  (7 instructions per 4 values)
  *   issuer         the products: O += P V of a unit of positions as its weights appear, then the scores that take over the buffer
- *   walker         the share's pieces, ahead of the others
+ *   walker, finder the share's pieces, and where the rows of their tiles lie, ahead of the others
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
  *
  * Every wait is bounded: on expiry the block's waits all end, Q4E_CUDA is set, and tensor memory is freed.
@@ -33,7 +33,7 @@ namespace {
 constexpr uint32_t CK_BN = 128;
 constexpr uint32_t CK_SPIN_LIMIT = 1u << 22;
 constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
-constexpr uint32_t PIECES = 4;          /* pieces that are walked ahead */
+constexpr uint32_t PIECES = 4, TILES = 4;   /* pieces that are walked ahead, tiles whose pages are found ahead */
 constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the reference moves */
 
 /* A piece costs about as much besides its tiles (queries in, outputs out, the first scores) as this many of them: a unit counts as so
@@ -45,16 +45,16 @@ struct ChunkCfg {
     static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
     static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : KIND == Q4K_Q8 ? 3u : 5u;
     static constexpr uint32_t PW = 4u;                            /* producer warps */
-    static constexpr uint32_t ISSUER = 8u + PW, WALKER = ISSUER + 1u, THREADS = (ISSUER + 4u) * 32u;
+    static constexpr uint32_t ISSUER = 8u + PW, WALKER = ISSUER + 1u, FINDER = ISSUER + 2u, THREADS = (ISSUER + 4u) * 32u;
     static constexpr uint32_t ITEMS = SLOT / 32u / (PW * 32u);    /* of 16 codes, per producer thread and slot */
     static constexpr uint32_t RAW = KIND == Q4K_Q8 ? PW * ITEMS * 544u : 0u;   /* codes and scales of a slot */
     /* registers of a thread: the block's 512 x 128 are 128 threads x (2 softmax + producers + the rest) */
-    static constexpr uint32_t R_SOFTMAX = KIND == Q4K_Q8 ? 168u : 184u, R_PRODUCER = KIND == Q4K_Q8 ? 120u : 88u, R_REST = 56u;
+    static constexpr uint32_t R_SOFTMAX = KIND == Q4K_Q8 ? 168u : 176u, R_PRODUCER = KIND == Q4K_Q8 ? 104u : 88u, R_REST = 72u;
     static_assert(2u * R_SOFTMAX + R_PRODUCER + R_REST <= 512u, "register split");
     static constexpr uint32_t PARTS = HD == 256 ? 2u : 1u;        /* slots of a K or a V tile: K by 128 dims, V by 64 positions */
     static constexpr uint32_t QG = 128u * HD * 2u;                /* one group's queries */
     static constexpr uint32_t REC = HD + 4u;
-    static constexpr uint32_t BARS = 768u + (NQ == 1u ? 1024u : 0u);
+    static constexpr uint32_t BARS = 1024u + (NQ == 1u ? 1024u : 0u);
     static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + RAWS * RAW + BARS + 1024u;
     static constexpr uint32_t UN = NQ == 2u ? 64u : 128u;         /* positions of a unit of scores */
     static_assert(SMEM <= 232448u, "shared memory");
@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + RAWS * C::RAW;
     const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
-                   s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 288, s_sum = bars + 320, w_full = bars + 448,
-                   w_empty = w_full + 8u * PIECES, s_piece = w_empty + 8u * PIECES, s_xch = bars + 768;
+                   s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 320, s_sum = bars + 352, w_full = bars + 480,
+                   w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_xch = bars + 1024;
     uint8_t *base = smem_dyn + (sQ - smem_u32(smem_dyn));
     const uint32_t tpu = P.tpg * NQ;
 
@@ -214,7 +214,11 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             mbar_init(bar_q, 256);
             for (uint32_t s = 0; s < PIECES; s++) {
                 mbar_init(w_full + 8 * s, 1);
-                mbar_init(w_empty + 8 * s, 9u + C::PW);   /* a warp each of softmax, issuer and producers */
+                mbar_init(w_empty + 8 * s, 10u + C::PW);   /* a warp each of softmax, issuer, finder and producers */
+            }
+            for (uint32_t s = 0; s < TILES; s++) {
+                mbar_init(t_full + 8 * s, 1);
+                mbar_init(t_empty + 8 * s, C::PW);
             }
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(0u) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -446,188 +450,212 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             }
             if (lane == 0) P.ends[blockIdx.x] = end_of;
         }
+        if (warp == C::FINDER) {
+            /* ================= finder: where the 16-position tiles of every tile of 128 lie ================= */
+            uint32_t n = 0;
+            const uint32_t per_page = P.part_bytes / TILE;
+            while (ok && next_piece(p)) {
+                piece_done();
+                const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
+                const uint32_t n_kv = p.before + p.n_here, q0 = p.st * CK_BN + (lane & 7u) * 16u;
+                auto entry = [&](uint32_t tile) -> int32_t { return tile < p.here && q0 + tile * CK_BN < n_kv ? tab[(q0 + tile * CK_BN) >> P.page_shift] : 0; };
+                int32_t next = entry(0);
+                for (uint32_t tile = 0; tile < p.here && ok; tile++, n++) {
+                    const int32_t page = next;
+                    next = entry(tile + 1u);
+                    const uint32_t q = q0 + tile * CK_BN, e = n % TILES, a = s_tile + e * 48u;
+                    const bool there = page >= 0 && (uint32_t)page < P.n_pages;
+                    const uint32_t at = there ? ((uint32_t)page * P.n_kvh + p.kh) * per_page + ((q & ((1u << P.page_shift) - 1u)) >> 4) : 0u;   /* in tiles of 16 positions */
+                    const uint32_t gone = __ballot_sync(0xffffffffu, !there) & 0xffu, first = (p.st + tile) * CK_BN;
+                    if (n >= TILES) ok = ck_all_wait(t_empty + 8 * e, (n / TILES - 1u) & 1u, s_abort);
+                    if (!ok) break;
+                    if (lane < 8u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(a + lane * 4u), "r"(at) : "memory");
+                    if (lane == 8u) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a + 32u), "r"(n_kv - first), "r"(gone) : "memory");
+                    if (lane == 9u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (n & 15u)), "r"(gone) : "memory");   /* for the softmax, once the tile's scores are there */
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(t_full + 8 * e);
+                }
+            }
+        }
     } else if (warp >= 8u) {
         /* ================= producers ================= */
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_PRODUCER));
-        const uint32_t ptid = tid - 256u, mask = (1u << P.page_shift) - 1u;
-        {
-            uint32_t at = 0;                          /* slots so far */
-            uint32_t kt = 0, vt = 0, part = 0, n_kv = 0;   /* of the piece: next K and V tile, slot of the tile; positions */
-            uint32_t k_count = 0;
-            const int32_t *tab = nullptr;
-            const uint8_t *kh_base = nullptr;
-            int32_t e_next = 0, h0 = -1, h1 = -1;     /* lane i: the page of 16 positions i of the next K tile, of the last one, of the one before */
-            p.here = 0;
-            struct Job { uint32_t p0, part; bool v; int32_t pages; };
-            auto entry = [&](uint32_t tile) -> int32_t {
-                const uint32_t q = (p.st + tile) * CK_BN + (lane & 7u) * 16u;
-                return tile < p.here && q < n_kv ? tab[q >> P.page_shift] : 0;
-            };
-            auto next_job = [&](Job &job) -> bool {
-                if (vt == p.here) {
-                    if (!ok || !next_piece(p)) return false;
-                    piece_done();
-                    kt = vt = part = 0;
-                    n_kv = p.before + p.n_here;
-                    tab = P.table + (size_t)p.req * P.table_stride;
-                    kh_base = P.mem + (uint64_t)p.kh * P.part_bytes;
-                    e_next = entry(0);
+        const uint32_t wi = warp - 8u;
+        uint32_t at = 0, n_k = 0, n_v = 0;            /* slots; K and V tiles so far */
+        uint32_t k_end = 0, part = 0;                 /* tiles of all pieces taken up; slot of the tile */
+        struct Job { uint32_t tile, part; bool v; };  /* tile: its place in the finder's ring */
+        auto next_job = [&](Job &job) -> bool {
+            if (n_v == k_end) {
+                if (!ok || !next_piece(p)) return false;
+                piece_done();
+                k_end += p.here;
+            }
+            /* K runs ahead of V as far as the scores run ahead of the outputs */
+            job.v = !(n_k < k_end && n_k <= n_v + (NQ == 1u ? 1u : 0u));
+            job.part = part;
+            const uint32_t n = job.v ? n_v : n_k;
+            job.tile = s_tile + n % TILES * 48u;
+            if (!job.v && part == 0u) ok = ok && ck_all_wait(t_full + 8 * (n % TILES), (n / TILES) & 1u, s_abort);
+            if (++part == PARTS) {
+                part = 0;
+                if (job.v) n_v++;
+                else n_k++;
+            }
+            return ok;
+        };
+        auto tile_read = [&](const Job &job) {        /* the last that the tile's places were needed for */
+            if (job.v && job.part + 1u == PARTS) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(t_empty + 8 * ((n_v - 1u) % TILES));
+            }
+        };
+        auto wait_empty = [&]() {
+            const uint32_t s = at % SLOTS, n = at / SLOTS;
+            if (n > 0u) ok = ok && ck_all_wait(empty + 8 * s, (n - 1u) & 1u, s_abort);
+        };
+        auto lds = [&](uint32_t a) -> uint32_t {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+            return v;
+        };
+        if constexpr (KIND == Q4K_Q8) {
+            /* An item is 16 codes: 16 bytes that come in, two 16-byte pieces of fp16 that go out.  A pass of a warp is 8 rows x 64 dims:
+             * four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has RG groups
+             * of 8 rows of the slot, NB blocks of 64 dims (passes) to each.  Codes and scales arrive by asynchronous copies, RAWS slots
+             * ahead, in places that this warp alone uses.  A warp here is alone on its scheduler with two of the softmax and issues
+             * once in four cycles: what counts is the number of its instructions, hence the finder. */
+            constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / C::PW;
+            constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
+            const uint32_t r8 = lane >> 2, c4 = lane & 3u;
+            const uint32_t raw0 = sR + SLOTS * SLOT + wi * WARP_RAW;
+            uint32_t asked = 0, is_v = 0;             /* slots requested so far; bit i: slot i of the last 32 is of V */
+            auto request = [&](const Job &job, auto nb) {
+                constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, T = RG > 1u ? RG / 2u : 1u;   /* T: tiles of 16 rows that the warp's rows lie in */
+                const uint32_t raw = raw0 + asked % RAWS * C::RAW;
+                const uint32_t g0 = (HD == 256 && job.v ? job.part * 8u : 0u) + wi * RG;   /* the first group of 8 rows, in the tile of 128 */
+                const uint32_t col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
+                const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
+                const uint32_t live = lds(job.tile + 32u), gone = lds(job.tile + 36u);
+                const uint8_t *rec[T];
+#pragma unroll
+                for (uint32_t i = 0; i < T; i++) rec[i] = P.mem + (uint64_t)lds(job.tile + ((g0 >> 1) + i) * 4u) * TILE + (RG == 1u ? (g0 & 1u) * 8u * ROW : 0u);
+                const uint32_t srow = lane < RG * 8u ? lane : 0u;   /* the row whose scales this lane brings */
+                const uint8_t *srec = (T == 2u && srow >= 16u ? rec[T - 1] : rec[0]) + (srow & 15u) * ROW + sc;
+                if (live >= CK_BN && !gone) {
+#pragma unroll
+                    for (uint32_t i = 0; i < RG; i++)
+#pragma unroll
+                        for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, rec[i / 2u] + ((i & 1u) * 8u + r8) * ROW + col + b * 64u, true);
+                    if (lane < RG * 8u) copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), srec, true);
+                } else {   /* zeros for rows that are not there */
+                    auto there = [&](uint32_t row) -> bool { return row < live && !((gone >> (row >> 4)) & 1u); };
+#pragma unroll 1
+                    for (uint32_t i = 0; i < RG; i++)
+#pragma unroll
+                        for (uint32_t b = 0; b < NB; b++)
+                            copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, (T == 2u && i >= 2u ? rec[T - 1] : rec[0]) + ((i & 1u) * 8u + r8) * ROW + col + b * 64u, there((g0 + i) * 8u + r8));
+                    if (lane < RG * 8u) copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), srec, there(g0 * 8u + lane));
                 }
-                /* K runs ahead of V as far as the scores run ahead of the outputs */
-                const bool k = kt < p.here && kt <= vt + (NQ == 1u ? 1u : 0u);
-                job.v = !k;
-                job.part = part;
-                if (k) {
-                    if (part == 0u) {
-                        h1 = h0;
-                        h0 = e_next;
-                        if (h0 < 0 || (uint32_t)h0 >= P.n_pages) h0 = -1;
-                        e_next = entry(kt + 1u);
-                        const uint32_t gone = __ballot_sync(0xffffffffu, h0 < 0) & 0xffu;
-                        /* read by the softmax warps once the scores of the tile are there */
-                        if (ptid == 0u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (k_count & 7u)), "r"(gone) : "memory");
-                        k_count++;
-                    }
-                    job.p0 = (p.st + kt) * CK_BN;
-                    job.pages = h0;
-                    if (++part == PARTS) { part = 0; kt++; }
-                } else {
-                    job.p0 = (p.st + vt) * CK_BN;
-                    job.pages = kt - 1u == vt ? h0 : h1;
-                    if (++part == PARTS) { part = 0; vt++; }
+                tile_read(job);
+            };
+            const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
+            auto convert = [&](auto nb) {
+                constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
+                const uint32_t raw = raw0 + at % RAWS * C::RAW;
+                uint4 w[ITEMS];
+                uint32_t sc[ITEMS];
+#pragma unroll
+                for (uint32_t k = 0; k < ITEMS; k++)
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w) : "r"(raw + k * 512u + lane * 16u) : "memory");
+#pragma unroll
+                for (uint32_t i = 0; i < RG; i++) {   /* all scales of the row's part */
+                    const uint32_t a = raw + ITEMS * 512u + (i * 8u + r8) * (NB * 4u);
+                    if constexpr (NB == 1u) sc[i] = lds(a);
+                    else if constexpr (NB == 2u) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[2 * i]), "=r"(sc[2 * i + 1]) : "r"(a) : "memory");
+                    else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(sc[4 * i]), "=r"(sc[4 * i + 1]), "=r"(sc[4 * i + 2]), "=r"(sc[4 * i + 3]) : "r"(a) : "memory");
                 }
-                return true;
-            };
-            auto wait_empty = [&]() {
-                const uint32_t s = at % SLOTS, n = at / SLOTS;
-                if (n > 0u) ok = ok && ck_all_wait(empty + 8 * s, (n - 1u) & 1u, s_abort);
-            };
-            auto sub_tile = [&](int32_t page, uint32_t q) -> const uint8_t * {   /* the tile of 16 rows at position q, on that page */
-                return kh_base + (uint64_t)(uint32_t)page * P.page_bytes + ((q & mask) >> 4) * TILE;
-            };
-            if constexpr (KIND == Q4K_Q8) {
-                /* An item is 16 codes: 16 bytes that come in, two 16-byte pieces of fp16 that go out.  A pass of a warp is 8 rows x 64
-                 * dims: four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has
-                 * RG groups of 8 rows of the slot, NB blocks of 64 dims (passes) to each.  Codes and scales arrive by asynchronous
-                 * copies, RAWS slots ahead, in places that this warp alone uses (through registers, a slot ahead, 8192 tokens over
-                 * 16 384 took 1813 us instead of 1451, with heads of 256 8650 instead of 4570). */
-                constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / C::PW;
-                constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
-                const uint32_t wi = warp - 8u, r8 = lane >> 2, c4 = lane & 3u;
-                const uint32_t raw0 = sR + SLOTS * SLOT + wi * WARP_RAW;
-                uint32_t asked = 0, is_v = 0;             /* slots requested so far; bit i: slot i of the last 32 is of V */
-                auto request = [&](const Job &job, auto nb) {
-                    constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB;
-                    const uint32_t raw = raw0 + asked % RAWS * C::RAW;
-                    const uint32_t g0 = (HD == 256 && job.v ? job.part * 8u : 0u) + wi * RG, col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
-                    const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
+                wait_empty();
+                if (!ok) return;
+                const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * RG * 8u + r8) * 128u;
+                const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
 #pragma unroll
-                    for (uint32_t i = 0; i < RG; i++) {
-                        const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)((g0 + i) >> 1));
-                        const uint32_t q = job.p0 + (g0 + i) * 8u;
-                        const uint8_t *rec = sub_tile(page < 0 ? 0 : page, q) + ((q & 8u) + r8) * ROW + col;
-                        const bool there = page >= 0 && q + r8 < n_kv;
+                for (uint32_t k = 0; k < ITEMS; k++) {
+                    const uint32_t s2 = __byte_perm(sc[k], 0u, scale_sel), off = k / NB * 1024u + k % NB * BLOCK;
+                    const uint32_t u[4] = {w[k].x ^ 0x80808080u, w[k].y ^ 0x80808080u, w[k].z ^ 0x80808080u, w[k].w ^ 0x80808080u};
+                    uint32_t o[8];
 #pragma unroll
-                        for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, rec + b * 64u, there);
+                    for (int e = 0; e < 4; e++) {
+                        o[2 * e] = h2u(__hmul2(codes2<0x4140>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
+                        o[2 * e + 1] = h2u(__hmul2(codes2<0x4342>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
                     }
-                    if (lane < RG * 8u) {   /* the scales of a row of this warp's */
-                        const uint32_t q = job.p0 + g0 * 8u + lane;
-                        const int32_t page = __shfl_sync((uint32_t)((1ull << RG * 8u) - 1u), job.pages, (int)((g0 + (lane >> 3)) >> 1));
-                        copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), sub_tile(page < 0 ? 0 : page, q) + (q & 15u) * ROW + sc, page >= 0 && q < n_kv);
-                    }
-                };
-                const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
-                auto convert = [&](auto nb) {
-                    constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
-                    const uint32_t raw = raw0 + at % RAWS * C::RAW;
-                    uint4 w[ITEMS];
-                    uint32_t sc[ITEMS];
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a0 + off), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a1 + off), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                }
+                fence_async_smem();
+                __syncwarp();   /* and the raw slot has been read by all lanes */
+                if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
+                at++;
+            };
+            bool more = true;
+            auto request_next = [&]() {   /* a group per call, so that they can be counted */
+                Job job;
+                more = more && next_job(job);
+                if (more) {
+                    if (NBK != NBV && job.v) request(job, std::integral_constant<uint32_t, NBV>());
+                    else request(job, std::integral_constant<uint32_t, NBK>());
+                    is_v = (is_v & ~(1u << (asked & 31u))) | (job.v ? 1u : 0u) << (asked & 31u);
+                    asked++;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            for (uint32_t d = 0; d < RAWS; d++) request_next();
+            while (ok && at < asked) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(RAWS - 1u) : "memory");
+                __syncwarp();
+                if (NBK != NBV && (is_v >> (at & 31u)) & 1u) convert(std::integral_constant<uint32_t, NBV>());
+                else convert(std::integral_constant<uint32_t, NBK>());
+                if (ok) request_next();
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            /* a slot is 16 units of 2 KB (8 at hd 64): 16 rows of a block of 64 dims.  One bulk copy each, shared out over the warps: a
+             * warp issues one in about 100 cycles */
+            constexpr uint32_t UNITS = SLOT / 2048u / C::PW;
+            Job job;
+            while (ok && next_job(job)) {
+                const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u;
+                const uint32_t unit = wi * UNITS + (lane & (UNITS - 1u)), tile = unit / nblk, b = unit - tile * nblk;
+                const uint32_t in = (HD == 256 && job.v ? job.part * 4u : 0u) + tile;
+                const uint32_t lies = lds(job.tile + in * 4u), left = lds(job.tile + 32u), gone = lds(job.tile + 36u);
+                const uint32_t live = (gone >> in) & 1u || left <= in * 16u ? 0u : min(16u, left - in * 16u);
+                tile_read(job);
+                wait_empty();
+                if (!ok) break;
+                const uint32_t s = at % SLOTS, bar = full + 8 * s, to = sR + s * SLOT + b * rows * 128u + tile * 2048u;
+                const uint32_t all = __reduce_add_sync(0xffffffffu, lane < UNITS ? live : 0u);
+                if (job.v && all < 16u * UNITS) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
+                    for (uint32_t u = 0; u < UNITS; u++) {
+                        const uint32_t there = __shfl_sync(0xffffffffu, live, (int)u), a = __shfl_sync(0xffffffffu, to, (int)u);
 #pragma unroll
-                    for (uint32_t k = 0; k < ITEMS; k++) {
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w) : "r"(raw + k * 512u + lane * 16u) : "memory");
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[k]) : "r"(raw + ITEMS * 512u + (k / NB * 8u + r8) * (NB * 4u) + k % NB * 4u) : "memory");
-                    }
-                    wait_empty();
-                    if (!ok) return;
-                    const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * RG * 8u + r8) * 128u;
-                    const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
-#pragma unroll
-                    for (uint32_t k = 0; k < ITEMS; k++) {
-                        const uint32_t s2 = __byte_perm(sc[k], 0u, scale_sel), off = k / NB * 1024u + k % NB * BLOCK;
-                        const uint32_t u[4] = {w[k].x ^ 0x80808080u, w[k].y ^ 0x80808080u, w[k].z ^ 0x80808080u, w[k].w ^ 0x80808080u};
-                        uint32_t o[8];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            o[2 * e] = h2u(__hmul2(codes2<0x4140>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
-                            o[2 * e + 1] = h2u(__hmul2(codes2<0x4342>(u[e]), *reinterpret_cast<const __half2 *>(&s2)));
-                        }
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a0 + off), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a1 + off), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                        for (uint32_t i = 0; i < 4; i++)
+                            if (i * 4u + (lane >> 3) >= there) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a + i * 512u + lane * 16u), "r"(0u) : "memory");
                     }
                     fence_async_smem();
-                    __syncwarp();   /* and the raw slot has been read by all lanes */
-                    if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
-                    at++;
-                };
-                bool more = true;
-                auto request_next = [&]() {   /* a group per call, so that they can be counted */
-                    Job job;
-                    more = more && next_job(job);
-                    if (more) {
-                        if (NBK != NBV && job.v) request(job, std::integral_constant<uint32_t, NBV>());
-                        else request(job, std::integral_constant<uint32_t, NBK>());
-                        is_v = (is_v & ~(1u << (asked & 31u))) | (job.v ? 1u : 0u) << (asked & 31u);
-                        asked++;
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                };
-                for (uint32_t d = 0; d < RAWS; d++) request_next();
-                while (ok && at < asked) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(RAWS - 1u) : "memory");
                     __syncwarp();
-                    if (NBK != NBV && (is_v >> (at & 31u)) & 1u) convert(std::integral_constant<uint32_t, NBV>());
-                    else convert(std::integral_constant<uint32_t, NBK>());
-                    if (ok) request_next();
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-            } else {
-                /* a slot is 16 units of 2 KB (8 at hd 64): 16 rows of a block of 64 dims.  One bulk copy each, shared out over the warps: a
-                 * warp issues one in about 100 cycles */
-                constexpr uint32_t UNITS = SLOT / 2048u / C::PW;
-                Job job;
-                while (ok && next_job(job)) {
-                    wait_empty();
-                    if (!ok) break;
-                    const uint32_t s = at % SLOTS, dst = sR + s * SLOT, bar = full + 8 * s;
-                    const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u;
-                    const uint32_t unit = (warp - 8u) * UNITS + (lane & (UNITS - 1u)), tile = unit / nblk, b = unit - tile * nblk;
-                    const uint32_t in = (HD == 256 && job.v ? job.part * 4u : 0u) + tile, q = job.p0 + in * 16u;
-                    const int32_t page = __shfl_sync(0xffffffffu, job.pages, (int)in);
-                    const uint32_t live = page >= 0 && q < n_kv ? min(16u, n_kv - q) : 0u, to = dst + b * rows * 128u + tile * 2048u;
-                    const uint32_t all = __reduce_add_sync(0xffffffffu, lane < UNITS ? live : 0u);
-                    if (job.v && all < 16u * UNITS) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
-                        for (uint32_t u = 0; u < UNITS; u++) {
-                            const uint32_t there = __shfl_sync(0xffffffffu, live, (int)u), a = __shfl_sync(0xffffffffu, to, (int)u);
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; i++)
-                                if (i * 4u + (lane >> 3) >= there) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(a + i * 512u + lane * 16u), "r"(0u) : "memory");
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                    }
-                    if (lane == 0) {
-                        if (all) mbar_expect_tx(bar, all * 128u);
-                        else mbar_arrive(bar);
-                    }
-                    __syncwarp();
-                    if (lane < UNITS && live) bulk_load(to, sub_tile(page, q) + (job.v ? TILE / 2u : 0u) + ((HD == 256 && !job.v ? job.part * 2u : 0u) + b) * 2048u, live * 128u, bar);
-                    at++;
+                if (lane == 0) {
+                    if (all) mbar_expect_tx(bar, all * 128u);
+                    else mbar_arrive(bar);
                 }
-                /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
-                if (!ok)
-                    for (uint32_t t = at > SLOTS ? at - SLOTS : 0u; t < at; t++)
-                        for (uint32_t i = 0; i < 4096u && !mbar_test<OWN>(full + 8 * (t % SLOTS), (t / SLOTS) & 1u); i++) {}
+                __syncwarp();
+                if (lane < UNITS && live)
+                    bulk_load(to, P.mem + (uint64_t)lies * TILE + (job.v ? TILE / 2u : 0u) + ((HD == 256 && !job.v ? job.part * 2u : 0u) + b) * 2048u, live * 128u, bar);
+                at++;
             }
+            /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
+            if (!ok)
+                for (uint32_t t = at > SLOTS ? at - SLOTS : 0u; t < at; t++)
+                    for (uint32_t i = 0; i < 4096u && !mbar_test<OWN>(full + 8 * (t % SLOTS), (t / SLOTS) & 1u); i++) {}
         }
     } else {
         /* ================= softmax ================= */
@@ -716,8 +744,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 const uint32_t b = g * 2u + (use & 1u), p0 = p.st * CK_BN + u * UN + h * TU;
                 const uint32_t t_s = t_lane + (NQ == 2u ? g * 128u + (use & 1u) * 64u : (use & 1u) * 128u + h * TU);
                 ok = ok && ck_all_wait(bar_s + 8 * b, (use >> 1) & 1u, s_abort);
-                if (NQ == 1u && !ok) {
-                    if (u == 0u || pair_any(false)) partner(0.f);
+                if (NQ == 1u && !ok) {   /* the other warp of the rows may have gone on: its meetings are kept */
+                    if (pair_any(false)) partner(0.f);
                     continue;
                 }
                 tc_fence_after();
@@ -725,21 +753,27 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
 #pragma unroll
                 for (int c = 0; c < (int)TU / 32; c++) tmem_ld32(t_s + 32 * c, *reinterpret_cast<float(*)[32]>(&s[32 * c]));
                 tmem_wait_ld();
-                if (__builtin_expect(p.gone, 0)) {   /* positions on pages that are not the pool's */
-                    uint32_t gone;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(gone) : "r"(s_gone + 4u * ((tiles_seen + (NQ == 2u ? u >> 1 : u)) & 7u)) : "memory");
+                if (__builtin_expect(p0 + TU > warp_min || p.gone, 0)) {
+                    uint32_t keep[2];   /* of 32 positions each */
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; k++) keep[k] = row_nkv >= p0 + 32u * k + 32u ? 0xffffffffu : row_nkv > p0 + 32u * k ? (1u << (row_nkv - (p0 + 32u * k))) - 1u : 0u;
+                    if (p.gone) {   /* positions on pages that are not the pool's */
+                        uint32_t gone;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(gone) : "r"(s_gone + 4u * ((tiles_seen + (NQ == 2u ? u >> 1 : u)) & 15u)) : "memory");
+                        gone >>= (p0 & 127u) >> 4;
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; k++) keep[k] &= ~((gone >> (2u * k) & 1u ? 0xffffu : 0u) | (gone >> (2u * k + 1u) & 1u ? 0xffff0000u : 0u));
+                    }
 #pragma unroll
                     for (int k = 0; k < (int)TU; k++)
-                        if ((gone >> (((p0 & 127u) + k) >> 4)) & 1u) s[k] = -CUDART_INF_F;
-                }
-                if (__builtin_expect(p0 + TU > warp_min, 0)) {
-#pragma unroll
-                    for (int k = 0; k < (int)TU; k++)
-                        if (p0 + k >= row_nkv) s[k] = -CUDART_INF_F;
+                        if (!((keep[k / 32] >> (k & 31)) & 1u)) s[k] = -CUDART_INF_F;
                 }
                 uint32_t pk[TU / 2];
                 uint64_t ls[2];
-                auto exps = [&]() {
+                /* The exponentials start against the maximum of the units before, while this unit's own is being formed; where that
+                 * is not within 2^8 the reference moves and they are taken again (by the same code: instructions that do not fit
+                 * the SM's cache together cost the roles more than this loop). */
+                for (bool again = false;; again = true) {
                     const float mneg = m_ref == -CUDART_INF_F ? 0.f : -m_ref;
                     const uint64_t sc2 = pack2(P.scale_log2e, P.scale_log2e), mn2 = pack2(mneg, mneg);
                     ls[0] = ls[1] = 0ull;
@@ -750,20 +784,16 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         ls[k & 1] = add2(ls[k & 1], pack2(e0, e1));
                         pk[k] = h2u(__floats2half2_rn(e0, e1));
                     }
-                };
-                /* the exponentials start against the maximum of the units before, while this unit's own is being formed; where that
-                 * is not within 2^8 the reference moves and they are taken again */
-                if (NQ == 2u || u > 0u) exps();   /* of a short chunk's halves the first unit is a good part */
-                float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                    if (__builtin_expect(again, 0)) break;
+                    float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-                for (int k = 0; k < (int)TU; k += 8) {
-                    mx[0] = fmaxf(fmaxf(mx[0], s[k]), s[k + 1]); mx[1] = fmaxf(fmaxf(mx[1], s[k + 2]), s[k + 3]);
-                    mx[2] = fmaxf(fmaxf(mx[2], s[k + 4]), s[k + 5]); mx[3] = fmaxf(fmaxf(mx[3], s[k + 6]), s[k + 7]);
-                }
-                float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2e;   /* scale > 0 */
-                bool grow = m_new > m_ref + CK_RESCALE_TAU;   /* also true on the first live unit (m_ref = -inf) */
-                const bool any = NQ == 2u ? __any_sync(0xffffffffu, grow) : u == 0u || pair_any(grow);
-                if (__builtin_expect(any, 0)) {
+                    for (int k = 0; k < (int)TU; k += 8) {
+                        mx[0] = fmaxf(fmaxf(mx[0], s[k]), s[k + 1]); mx[1] = fmaxf(fmaxf(mx[1], s[k + 2]), s[k + 3]);
+                        mx[2] = fmaxf(fmaxf(mx[2], s[k + 4]), s[k + 5]); mx[3] = fmaxf(fmaxf(mx[3], s[k + 6]), s[k + 7]);
+                    }
+                    float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * P.scale_log2e;   /* scale > 0 */
+                    bool grow = m_new > m_ref + CK_RESCALE_TAU;   /* also true on the first live unit (m_ref = -inf) */
+                    if (__builtin_expect(!(NQ == 2u ? __any_sync(0xffffffffu, grow) : pair_any(grow)), 1)) break;
                     if (NQ == 1u) {   /* both halves of a row keep one reference: they share its O */
                         m_new = fmaxf(m_new, partner(m_new));
                         grow = m_new > m_ref + CK_RESCALE_TAU;
@@ -774,7 +804,6 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         m_ref = m_new;
                         l_run *= alpha;
                     }
-                    exps();
                     if (u > 0u) {   /* O is rescaled only here; the group's last product must have drained */
                         ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort) && ok;
                         tc_fence_after();
