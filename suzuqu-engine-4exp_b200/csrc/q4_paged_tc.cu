@@ -9,11 +9,11 @@
  *
  *   warps 0 - 7    softmax: thread r owns row r (hd 256: two threads, half of a unit's positions each): its scores out of tensor
  *                  memory, causal mask, running maximum with lazy rescale, weights as fp16 back into the columns they came from
- *   producers      K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads them: bulk copies.
- *                  q8_0: codes and scales by asynchronous copies, three slots ahead, then fp16(code x scale) into the slot
- *                  (7 instructions per 4 values)
+ *   producers      (one team of four warps, or three of two) K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads them: bulk copies.
+ *                  q8_0: codes and scales by asynchronous copies, then fp16(code x scale) into the slot (7 instructions
+ *                  per 4 values)
  *   issuer         the products: O += P V of a unit of positions as its weights appear, then the scores that take over the buffer
- *   walker, finder the share's pieces, and where the rows of their tiles lie, ahead of the others
+ *   walker         the share's pieces, and where the rows of their tiles lie, ahead of the others
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
  *
  * Every wait is bounded: on expiry the block's waits all end, Q4E_CUDA is set, and tensor memory is freed.
@@ -39,23 +39,27 @@ constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the referenc
 /* A piece costs about as much besides its tiles (queries in, outputs out, the first scores) as this many of them: a unit counts as so
  * many more steps when the work is shared out.  Only tiles are walked; a share may hold none. */
 constexpr uint32_t CK_EXTRA = 2;
-constexpr uint32_t RAWS = 3;            /* slots of q8_0 codes on their way */
 template <int KIND, int HD>
 struct ChunkCfg {
     static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
     static constexpr uint32_t SLOT = HD == 64 ? 16384u : 32768u, SLOTS = HD == 64 ? 10u : KIND == Q4K_Q8 ? 3u : 5u;
-    static constexpr uint32_t PW = 4u;                            /* producer warps */
-    static constexpr uint32_t ISSUER = 8u + PW, WALKER = ISSUER + 1u, FINDER = ISSUER + 2u, THREADS = (ISSUER + 4u) * 32u;
-    static constexpr uint32_t ITEMS = SLOT / 32u / (PW * 32u);    /* of 16 codes, per producer thread and slot */
-    static constexpr uint32_t RAW = KIND == Q4K_Q8 ? PW * ITEMS * 544u : 0u;   /* codes and scales of a slot */
-    /* registers of a thread: the block's 512 x 128 are 128 threads x (2 softmax + producers + the rest) */
-    static constexpr uint32_t R_SOFTMAX = KIND == Q4K_Q8 ? 168u : 176u, R_PRODUCER = KIND == Q4K_Q8 ? 104u : 88u, R_REST = 72u;
-    static_assert(2u * R_SOFTMAX + R_PRODUCER + R_REST <= 512u, "register split");
+    static constexpr uint32_t ISSUER = 8u, WALKER = 9u, PRODUCER = 10u, THREADS = 512u;   /* first warps of the roles */
+    /* Producer warps: TEAMS x WPT, a slot is one team's.  At hd 256 three slots are worked at at once, or the fixed part of a slot (900
+     * of 1640 cycles) is not hidden: 8192 tokens over 16 384 5060 -> 3600 us; where the scores set the pace short slots leave more of
+     * the ring free: 512 tokens over 16 001 at hd 128 98 us, by two teams of two warps 110. */
+    static constexpr uint32_t TEAMS = HD == 256 ? 3u : 1u, WPT = HD == 256 ? 2u : 4u;
+    static constexpr uint32_t RPS = HD == 256 ? 2u : 1u;          /* rounds of a slot */
+    static constexpr uint32_t ITEMS = SLOT / 32u / (WPT * 32u * RPS);   /* of 16 codes, per producer thread and round */
+    static constexpr uint32_t ROUNDS = HD == 256 ? 2u : 3u;       /* rounds of codes on their way to a warp */
+    static constexpr uint32_t RAW = KIND == Q4K_Q8 ? ITEMS * 544u : 0u;   /* codes and scales of a warp's round */
+    /* registers of a thread: the block's 512 x 128 are 256 threads x (softmax + the others) */
+    static constexpr uint32_t R_SOFTMAX = 168u, R_OTHERS = 88u;
+    static_assert(R_SOFTMAX + R_OTHERS <= 256u, "register split");
     static constexpr uint32_t PARTS = HD == 256 ? 2u : 1u;        /* slots of a K or a V tile: K by 128 dims, V by 64 positions */
     static constexpr uint32_t QG = 128u * HD * 2u;                /* one group's queries */
     static constexpr uint32_t REC = HD + 4u;
     static constexpr uint32_t BARS = 1024u + (NQ == 1u ? 1024u : 0u);
-    static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + RAWS * RAW + BARS + 1024u;
+    static constexpr uint32_t SMEM = NQ * QG + SLOTS * SLOT + TEAMS * WPT * ROUNDS * RAW + BARS + 1024u;
     static constexpr uint32_t UN = NQ == 2u ? 64u : 128u;         /* positions of a unit of scores */
     static_assert(SMEM <= 232448u, "shared memory");
 };
@@ -188,11 +192,11 @@ struct Walk {
 template <int KIND, int HD>
 __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
     using C = ChunkCfg<KIND, HD>;
-    constexpr uint32_t CK_THREADS = C::THREADS, NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
+    constexpr uint32_t CK_THREADS = C::THREADS, TEAMS = C::TEAMS, WPT = C::WPT, NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
     constexpr uint32_t O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + RAWS * C::RAW;
+    const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + TEAMS * WPT * C::ROUNDS * C::RAW;
     const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
                    s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 320, s_sum = bars + 352, w_full = bars + 480,
                    w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_xch = bars + 1024;
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     if (warp == C::ISSUER) {
         if (lane == 0) {
             for (uint32_t s = 0; s < SLOTS; s++) {
-                mbar_init(full + 8 * s, C::PW);
+                mbar_init(full + 8 * s, WPT);
                 mbar_init(empty + 8 * s, 1);
             }
             for (uint32_t s = 0; s < 4; s++) {
@@ -214,11 +218,11 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             mbar_init(bar_q, 256);
             for (uint32_t s = 0; s < PIECES; s++) {
                 mbar_init(w_full + 8 * s, 1);
-                mbar_init(w_empty + 8 * s, 10u + C::PW);   /* a warp each of softmax, issuer, finder and producers */
+                mbar_init(w_empty + 8 * s, 9u + TEAMS * WPT);   /* a warp each of softmax, issuer and producers */
             }
             for (uint32_t s = 0; s < TILES; s++) {
                 mbar_init(t_full + 8 * s, 1);
-                mbar_init(t_empty + 8 * s, C::PW);
+                mbar_init(t_empty + 8 * s, WPT * PARTS * 2u);   /* the warps of every slot of its K and V */
             }
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(0u) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -306,8 +310,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     };
     Piece p;
 
-    if (warp >= C::ISSUER) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_REST));
+    if (warp >= 8u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_OTHERS));
         if (warp == C::ISSUER) {
             /* ================= issuer: a converged warp, one elected lane ================= */
             constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(UN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -411,7 +415,9 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             }
         }
         if (warp == C::WALKER) {
-            /* ================= walker: the share's pieces, and the unit that ends in this block ================= */
+            /* ================= walker: the share's pieces, where their tiles lie, and the unit that ends in this block ================= */
+            uint32_t n_tile = 0;
+            const uint32_t per_page = P.part_bytes / TILE;
             int4 end_of = make_int4(-1, 0, 0, 0);
             Walk W;
             W.left = 0;
@@ -445,69 +451,69 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     mbar_arrive(w_full + 8 * e);
                 }
                 if (!more) break;
+                /* tile by tile: where its eight tiles of 16 positions lie, in units of such tiles; its live positions; those without a page */
+                const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
+                const uint32_t n_kv = p.before + p.n_here, q0 = p.st * CK_BN + (lane & 7u) * 16u;
+                auto entry = [&](uint32_t tile) -> int32_t { return tile < p.here && q0 + tile * CK_BN < n_kv ? tab[(q0 + tile * CK_BN) >> P.page_shift] : 0; };
+                int32_t next = entry(0);
+                for (uint32_t tile = 0; tile < p.here && ok; tile++, n_tile++) {
+                    const int32_t page = next;
+                    next = entry(tile + 1u);
+                    const uint32_t q = q0 + tile * CK_BN, te = n_tile % TILES, ta = s_tile + te * 48u;
+                    const bool there = (uint32_t)page < P.n_pages;
+                    const uint32_t at = there ? ((uint32_t)page * P.n_kvh + p.kh) * per_page + ((q & ((1u << P.page_shift) - 1u)) >> 4) : 0u;
+                    const uint32_t gone8 = __ballot_sync(0xffffffffu, !there) & 0xffu;
+                    if (n_tile >= TILES) ok = ck_all_wait(t_empty + 8 * te, (n_tile / TILES - 1u) & 1u, s_abort);
+                    if (!ok) break;
+                    if (lane < 8u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ta + lane * 4u), "r"(at) : "memory");
+                    if (lane == 8u) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(ta + 32u), "r"(n_kv - (p.st + tile) * CK_BN), "r"(gone8) : "memory");
+                    if (lane == 9u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (n_tile & 15u)), "r"(gone8) : "memory");   /* for the softmax, once the tile's scores are there */
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(t_full + 8 * te);
+                }
                 if (p.st > 0u && p.st + p.here == p.tiles)   /* the unit ends here; it began in block .. */
                     end_of = make_int4((int32_t)(((W.unit_at + 1u) * blocks - 1u) / total), (int32_t)p.tok0, (int32_t)p.n_here, (int32_t)p.kh);
             }
             if (lane == 0) P.ends[blockIdx.x] = end_of;
         }
-        if (warp == C::FINDER) {
-            /* ================= finder: where the 16-position tiles of every tile of 128 lie ================= */
-            uint32_t n = 0;
-            const uint32_t per_page = P.part_bytes / TILE;
-            while (ok && next_piece(p)) {
-                piece_done();
-                const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
-                const uint32_t n_kv = p.before + p.n_here, q0 = p.st * CK_BN + (lane & 7u) * 16u;
-                auto entry = [&](uint32_t tile) -> int32_t { return tile < p.here && q0 + tile * CK_BN < n_kv ? tab[(q0 + tile * CK_BN) >> P.page_shift] : 0; };
-                int32_t next = entry(0);
-                for (uint32_t tile = 0; tile < p.here && ok; tile++, n++) {
-                    const int32_t page = next;
-                    next = entry(tile + 1u);
-                    const uint32_t q = q0 + tile * CK_BN, e = n % TILES, a = s_tile + e * 48u;
-                    const bool there = page >= 0 && (uint32_t)page < P.n_pages;
-                    const uint32_t at = there ? ((uint32_t)page * P.n_kvh + p.kh) * per_page + ((q & ((1u << P.page_shift) - 1u)) >> 4) : 0u;   /* in tiles of 16 positions */
-                    const uint32_t gone = __ballot_sync(0xffffffffu, !there) & 0xffu, first = (p.st + tile) * CK_BN;
-                    if (n >= TILES) ok = ck_all_wait(t_empty + 8 * e, (n / TILES - 1u) & 1u, s_abort);
-                    if (!ok) break;
-                    if (lane < 8u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(a + lane * 4u), "r"(at) : "memory");
-                    if (lane == 8u) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a + 32u), "r"(n_kv - first), "r"(gone) : "memory");
-                    if (lane == 9u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (n & 15u)), "r"(gone) : "memory");   /* for the softmax, once the tile's scores are there */
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(t_full + 8 * e);
-                }
-            }
-        }
-    } else if (warp >= 8u) {
+        if (warp >= C::PRODUCER && warp < C::PRODUCER + TEAMS * WPT) {
         /* ================= producers ================= */
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_PRODUCER));
-        const uint32_t wi = warp - 8u;
-        uint32_t at = 0, n_k = 0, n_v = 0;            /* slots; K and V tiles so far */
-        uint32_t k_end = 0, part = 0;                 /* tiles of all pieces taken up; slot of the tile */
-        struct Job { uint32_t tile, part; bool v; };  /* tile: its place in the finder's ring */
+        const uint32_t team = (warp - C::PRODUCER) / WPT, share = (warp - C::PRODUCER) % WPT;   /* its share of every slot of the team */
+        uint32_t at = team, in_piece = team, tiles_before = 0;   /* the team's next slot: of all, in the piece; tiles of earlier pieces */
+        bool have = false;
+        struct Job { uint32_t tile, part; bool v; };             /* tile: its place in the ring of tiles found */
+        /* The slots of a piece in the order of their use.  Two groups: K0 V0 K1 V1 ..; one: K0 K1 V0 K2 V1 .. V(n-1), two slots each (the
+         * scores run a tile and two tiles ahead of the outputs) */
         auto next_job = [&](Job &job) -> bool {
-            if (n_v == k_end) {
+            while (!have || in_piece >= 2u * PARTS * p.here) {
+                if (have) {
+                    in_piece -= 2u * PARTS * p.here;
+                    tiles_before += p.here;
+                }
                 if (!ok || !next_piece(p)) return false;
                 piece_done();
-                k_end += p.here;
+                have = true;
             }
-            /* K runs ahead of V as far as the scores run ahead of the outputs */
-            job.v = !(n_k < k_end && n_k <= n_v + (NQ == 1u ? 1u : 0u));
-            job.part = part;
-            const uint32_t n = job.v ? n_v : n_k;
-            job.tile = s_tile + n % TILES * 48u;
-            if (!job.v && part == 0u) ok = ok && ck_all_wait(t_full + 8 * (n % TILES), (n / TILES) & 1u, s_abort);
-            if (++part == PARTS) {
-                part = 0;
-                if (job.v) n_v++;
-                else n_k++;
+            const uint32_t m = in_piece / PARTS;
+            uint32_t tile;
+            if (NQ == 2u) {
+                job.v = m & 1u;
+                tile = m >> 1;
+            } else {
+                const bool last = m == 2u * p.here - 1u;
+                job.v = last || (m && !(m & 1u));
+                tile = last ? p.here - 1u : m == 0u ? 0u : m & 1u ? (m + 1u) >> 1 : (m >> 1) - 1u;
             }
+            job.part = in_piece % PARTS;
+            tile += tiles_before;
+            job.tile = tile % TILES;
+            ok = ck_all_wait(t_full + 8 * job.tile, (tile / TILES) & 1u, s_abort);
+            in_piece += TEAMS;
             return ok;
         };
-        auto tile_read = [&](const Job &job) {        /* the last that the tile's places were needed for */
-            if (job.v && job.part + 1u == PARTS) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(t_empty + 8 * ((n_v - 1u) % TILES));
-            }
+        auto tile_read = [&](const Job &job) {                   /* its place is not needed any more */
+            __syncwarp();
+            if (lane == 0) mbar_arrive(t_empty + 8 * job.tile);
         };
         auto wait_empty = [&]() {
             const uint32_t s = at % SLOTS, n = at / SLOTS;
@@ -520,27 +526,25 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         };
         if constexpr (KIND == Q4K_Q8) {
             /* An item is 16 codes: 16 bytes that come in, two 16-byte pieces of fp16 that go out.  A pass of a warp is 8 rows x 64 dims:
-             * four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp has RG groups
-             * of 8 rows of the slot, NB blocks of 64 dims (passes) to each.  Codes and scales arrive by asynchronous copies, RAWS slots
-             * ahead, in places that this warp alone uses.  A warp here is alone on its scheduler with two of the softmax and issues
-             * once in four cycles: what counts is the number of its instructions, hence the finder. */
-            constexpr uint32_t ITEMS = C::ITEMS, WARP_RAW = C::RAW / C::PW;
-            constexpr uint32_t NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
+             * four lanes to a row, so that the eight lanes whose stores go together (two rows) meet no bank twice.  A warp's share of a
+             * slot is RPS rounds of RG groups of 8 rows x NB blocks of 64 dims (passes) each; the codes and scales of the next rounds
+             * arrive by asynchronous copies meanwhile, in places that this warp alone uses.  A warp here issues once in three to five
+             * cycles, beside two of the softmax: where things lie is found for it. */
+            constexpr uint32_t ITEMS = C::ITEMS, NBK = HD == 64 ? 1u : 2u, NBV = HD / 64u;
             const uint32_t r8 = lane >> 2, c4 = lane & 3u;
-            const uint32_t raw0 = sR + SLOTS * SLOT + wi * WARP_RAW;
-            uint32_t asked = 0, is_v = 0;             /* slots requested so far; bit i: slot i of the last 32 is of V */
-            auto request = [&](const Job &job, auto nb) {
-                constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, T = RG > 1u ? RG / 2u : 1u;   /* T: tiles of 16 rows that the warp's rows lie in */
-                const uint32_t raw = raw0 + asked % RAWS * C::RAW;
-                const uint32_t g0 = (HD == 256 && job.v ? job.part * 8u : 0u) + wi * RG;   /* the first group of 8 rows, in the tile of 128 */
+            const uint32_t raw0 = sR + SLOTS * SLOT + (warp - C::PRODUCER) * C::ROUNDS * C::RAW;
+            auto request = [&](const Job &job, uint32_t round, uint32_t raw, auto nb) {
+                constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, T = RG > 2u ? 2u : 1u;
+                static_assert(RG <= 4u, "a lane brings the scales of one row");   /* T: tiles of 16 rows of a round */
+                const uint32_t place = s_tile + job.tile * 48u;
+                const uint32_t g0 = (HD == 256 && job.v ? job.part * 8u : 0u) + (share * C::RPS + round) * RG;   /* the first group of 8 rows, in the tile of 128 */
                 const uint32_t col = (job.v ? HD : 0u) + (HD == 256 && !job.v ? job.part * 128u : 0u) + c4 * 16u;
                 const uint32_t sc = 2u * HD + (job.v ? HD / 16u : 0u) + (HD == 256 && !job.v ? job.part * 8u : 0u);
-                const uint32_t live = lds(job.tile + 32u), gone = lds(job.tile + 36u);
+                const uint32_t live = lds(place + 32u), gone = lds(place + 36u);
                 const uint8_t *rec[T];
 #pragma unroll
-                for (uint32_t i = 0; i < T; i++) rec[i] = P.mem + (uint64_t)lds(job.tile + ((g0 >> 1) + i) * 4u) * TILE + (RG == 1u ? (g0 & 1u) * 8u * ROW : 0u);
-                const uint32_t srow = lane < RG * 8u ? lane : 0u;   /* the row whose scales this lane brings */
-                const uint8_t *srec = (T == 2u && srow >= 16u ? rec[T - 1] : rec[0]) + (srow & 15u) * ROW + sc;
+                for (uint32_t i = 0; i < T; i++) rec[i] = P.mem + (uint64_t)lds(place + ((g0 >> 1) + i) * 4u) * TILE;
+                const uint8_t *srec = (T == 2u && lane >= 16u ? rec[T - 1] : rec[0]) + (lane & 15u) * ROW + sc;   /* of the row whose scales this lane brings */
                 if (live >= CK_BN && !gone) {
 #pragma unroll
                     for (uint32_t i = 0; i < RG; i++)
@@ -556,12 +560,11 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                             copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, (T == 2u && i >= 2u ? rec[T - 1] : rec[0]) + ((i & 1u) * 8u + r8) * ROW + col + b * 64u, there((g0 + i) * 8u + r8));
                     if (lane < RG * 8u) copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), srec, there(g0 * 8u + lane));
                 }
-                tile_read(job);
+                if (round + 1u == C::RPS) tile_read(job);
             };
             const uint32_t scale_sel = c4 & 2u ? 0x3232u : 0x1010u;
-            auto convert = [&](auto nb) {
+            auto convert = [&](uint32_t round, uint32_t raw, auto nb) {
                 constexpr uint32_t NB = decltype(nb)::value, RG = ITEMS / NB, BLOCK = NB == 4u ? 64u * 128u : 128u * 128u;
-                const uint32_t raw = raw0 + at % RAWS * C::RAW;
                 uint4 w[ITEMS];
                 uint32_t sc[ITEMS];
 #pragma unroll
@@ -574,9 +577,9 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     else if constexpr (NB == 2u) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sc[2 * i]), "=r"(sc[2 * i + 1]) : "r"(a) : "memory");
                     else asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(sc[4 * i]), "=r"(sc[4 * i + 1]), "=r"(sc[4 * i + 2]), "=r"(sc[4 * i + 3]) : "r"(a) : "memory");
                 }
-                wait_empty();
+                if (round == 0u) wait_empty();
                 if (!ok) return;
-                const uint32_t dst = sR + (at % SLOTS) * SLOT + (wi * RG * 8u + r8) * 128u;
+                const uint32_t dst = sR + (at % SLOTS) * SLOT + ((share * C::RPS + round) * RG * 8u + r8) * 128u;
                 const uint32_t a0 = dst + (((2u * c4) ^ r8) << 4), a1 = dst + (((2u * c4 + 1u) ^ r8) << 4);
 #pragma unroll
                 for (uint32_t k = 0; k < ITEMS; k++) {
@@ -591,42 +594,53 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a0 + off), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a1 + off), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
                 }
-                fence_async_smem();
-                __syncwarp();   /* and the raw slot has been read by all lanes */
-                if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
-                at++;
             };
+            Job job;
             bool more = true;
-            auto request_next = [&]() {   /* a group per call, so that they can be counted */
-                Job job;
-                more = more && next_job(job);
+            uint32_t asked = 0, is_v = 0, done = 0;              /* rounds asked for; bit i: slot i of the team's last 32 is of V; rounds converted */
+            auto request_next = [&]() {                          /* a group per call in any case, so that they can be counted */
+                const uint32_t slot = asked / C::RPS & 31u, round = asked % C::RPS, raw = raw0 + asked % C::ROUNDS * C::RAW;
+                if (round == 0u) {
+                    more = more && next_job(job);
+                    is_v = (is_v & ~(1u << slot)) | (job.v ? 1u : 0u) << slot;
+                }
                 if (more) {
-                    if (NBK != NBV && job.v) request(job, std::integral_constant<uint32_t, NBV>());
-                    else request(job, std::integral_constant<uint32_t, NBK>());
-                    is_v = (is_v & ~(1u << (asked & 31u))) | (job.v ? 1u : 0u) << (asked & 31u);
+                    if (NBK != NBV && job.v) request(job, round, raw, std::integral_constant<uint32_t, NBV>());
+                    else request(job, round, raw, std::integral_constant<uint32_t, NBK>());
                     asked++;
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            for (uint32_t d = 0; d < RAWS; d++) request_next();
-            while (ok && at < asked) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(RAWS - 1u) : "memory");
+#pragma unroll 1
+            for (uint32_t d = 0; d < C::ROUNDS; d++) request_next();
+            while (ok && done < asked) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(C::ROUNDS - 1u) : "memory");
                 __syncwarp();
-                if (NBK != NBV && (is_v >> (at & 31u)) & 1u) convert(std::integral_constant<uint32_t, NBV>());
-                else convert(std::integral_constant<uint32_t, NBK>());
-                if (ok) request_next();
+                const uint32_t round = done % C::RPS, raw = raw0 + done % C::ROUNDS * C::RAW;
+                if (NBK != NBV && (is_v >> (done / C::RPS & 31u)) & 1u) convert(round, raw, std::integral_constant<uint32_t, NBV>());
+                else convert(round, raw, std::integral_constant<uint32_t, NBK>());
+                if (!ok) break;
+                done++;
+                if (round + 1u == C::RPS) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + 8 * (at % SLOTS));
+                    at += TEAMS;
+                }
+                __syncwarp();       /* the round's codes have been read by all lanes */
+                request_next();
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else {
             /* a slot is 16 units of 2 KB (8 at hd 64): 16 rows of a block of 64 dims.  One bulk copy each, shared out over the warps: a
              * warp issues one in about 100 cycles */
-            constexpr uint32_t UNITS = SLOT / 2048u / C::PW;
+            constexpr uint32_t UNITS = SLOT / 2048u / WPT;
             Job job;
             while (ok && next_job(job)) {
-                const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u;
-                const uint32_t unit = wi * UNITS + (lane & (UNITS - 1u)), tile = unit / nblk, b = unit - tile * nblk;
+                const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u, place = s_tile + job.tile * 48u;
+                const uint32_t unit = share * UNITS + (lane & (UNITS - 1u)), tile = unit / nblk, b = unit - tile * nblk;
                 const uint32_t in = (HD == 256 && job.v ? job.part * 4u : 0u) + tile;
-                const uint32_t lies = lds(job.tile + in * 4u), left = lds(job.tile + 32u), gone = lds(job.tile + 36u);
+                const uint32_t lies = lds(place + in * 4u), left = lds(place + 32u), gone = lds(place + 36u);
                 const uint32_t live = (gone >> in) & 1u || left <= in * 16u ? 0u : min(16u, left - in * 16u);
                 tile_read(job);
                 wait_empty();
@@ -650,12 +664,15 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 __syncwarp();
                 if (lane < UNITS && live)
                     bulk_load(to, P.mem + (uint64_t)lies * TILE + (job.v ? TILE / 2u : 0u) + ((HD == 256 && !job.v ? job.part * 2u : 0u) + b) * 2048u, live * 128u, bar);
-                at++;
+                at += TEAMS;
             }
             /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
             if (!ok)
-                for (uint32_t t = at > SLOTS ? at - SLOTS : 0u; t < at; t++)
+                for (uint32_t t = at; t >= TEAMS && at - t < SLOTS;) {
+                    t -= TEAMS;
                     for (uint32_t i = 0; i < 4096u && !mbar_test<OWN>(full + 8 * (t % SLOTS), (t / SLOTS) & 1u); i++) {}
+                }
+        }
         }
     } else {
         /* ================= softmax ================= */
