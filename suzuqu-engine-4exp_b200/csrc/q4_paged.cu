@@ -10,9 +10,9 @@
  *
  * Requests differ in length by orders of magnitude, so blocks are not given requests but equal shares of the step's whole work:
  * the steps (128 positions) of all units (request, kv head, group of tokens) lie one behind the other, and block c takes steps
- * [T c / C, T (c + 1) / C).  Where a share ends inside a unit the block leaves (acc, m, l) records, at most two, and q4_pg_merge_k
- * joins a unit's records; the block that holds the unit's end tells it which.  The division is computed by every block
- * itself from the lengths on the device (one scan), which the host need not know.
+ * [T c / C, T (c + 1) / C).  Where a share ends inside a unit the block leaves (acc, m, l) records, at most two, and the unit's
+ * blocks meet and join them.  The division is computed by every block itself from the lengths on the device (one scan), which
+ * the host need not know.
  */
 #include <cuda_bf16.h>
 #include <math_constants.h>
@@ -23,6 +23,7 @@
 namespace {
 
 constexpr uint32_t PG_SPIN_LIMIT = 1u << 20;
+__device__ uint32_t g_few_meet[2u * PG_MAX_BLOCKS];
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ float ex2(float x) {
@@ -95,25 +96,6 @@ struct FewCfg {
     static constexpr uint32_t SMEM = RING + ROWS * Q_STRIDE + WARPS * DEPTH * 8u + 1024u;
 };
 
-/* four dims of a row: acc / l * sigmoid(gate).  A row that attended nothing is 0, one with a NaN among its scores stays NaN */
-template <int HD>
-__device__ __forceinline__ void pg_store(const PagedParams &P, uint32_t tok, uint32_t head, uint32_t d, float4 x, float L) {
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    const size_t at = ((size_t)tok * P.n_head + head) * HD + d;
-    x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
-    if (P.gate) {
-        const float4 gt = *reinterpret_cast<const float4 *>(P.gate + at);
-        x.x *= 1.f / (1.f + __expf(-gt.x)); x.y *= 1.f / (1.f + __expf(-gt.y));
-        x.z *= 1.f / (1.f + __expf(-gt.z)); x.w *= 1.f / (1.f + __expf(-gt.w));
-    }
-    if (P.out_bf16) {
-        const __nv_bfloat162 b0 = __floats2bfloat162_rn(x.x, x.y), b1 = __floats2bfloat162_rn(x.z, x.w);
-        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&b0), *reinterpret_cast<const uint32_t *>(&b1));
-    } else {
-        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.out) + at) = x;
-    }
-}
-
 template <int KIND, int HD, int NT>
 __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD, NT>::CTAS) q4_pg_few_k(const PagedParams P) {
     using C = FewCfg<KIND, HD, NT>;
@@ -166,10 +148,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     }
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     const uint64_t blocks = min((uint64_t)gridDim.x, total);
-    if (blockIdx.x >= blocks) {
-        if (tid == 0) P.ends[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        return;
-    }
+    if (blockIdx.x >= blocks) return;
     uint64_t s = total * blockIdx.x / blocks;
     const uint64_t s_end = total * (blockIdx.x + 1u) / blocks;
     if (before <= s && s < before + mine)
@@ -185,7 +164,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     __syncthreads();
     uint32_t req = s_req, issued = 0, taken = 0;   /* of the warp's ring, over all pieces */
     uint64_t off = s_off;
-    int4 end_of = make_int4(-1, 0, 0, 0);
+    PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* units that began before this block; that go on behind it */
     bool ok = true;
 
     /* ---- pieces of units */
@@ -506,21 +485,26 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
             const float4 x = *reinterpret_cast<const float4 *>(rec + d);
             const float L = rec[HD + 1];
             if (whole) {
-                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, x, L);
+                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, x, L, P.gate ? P.gate + ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d : nullptr);
             } else {
                 *reinterpret_cast<float4 *>(part + row * C::REC + d) = x;
                 if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(rec[HD], L);
             }
         }
-        if (st > 0u && st + here == n_steps) {   /* the unit ends here; it began in block .. */
-            const uint64_t first = s - st;
-            end_of = make_int4((int32_t)(((first + 1u) * blocks - 1u) / total), (int32_t)tok0, (int32_t)n_here, (int32_t)kh);
+        if (!whole) {
+            const uint64_t first = s - st;   /* the unit's first step; step x is block ((x + 1) blocks - 1) / total's */
+            split[st == 0u] = {(uint32_t)(((first + 1u) * blocks - 1u) / total), (uint32_t)(((first + n_steps) * blocks - 1u) / total), tok0, n_here, kh};
         }
         s += here;
         off += here;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   /* the next bulk copies overwrite what was stored here */
     }
-    if (tid == 0) P.ends[blockIdx.x] = end_of;
+    __syncthreads();
+    if (tid == 0) {
+        pg_arrive(P, split[0]);
+        pg_arrive(P, split[1]);
+    }
+    pg_join<HD, C::THREADS>(P, split[0], C::ROWS, base, C::RING);
     if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
         if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
         for (; taken < issued; taken++)
@@ -528,69 +512,28 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     }
 }
 
-/* Joins the records of the unit that ends in block blockIdx.x: 4 dims per thread, so that 256 threads have SETS rows at a time;
- * where a unit lies in many blocks, one row, whose records they share out. */
-template <int HD>
-__global__ void __launch_bounds__(256) q4_pg_merge_k(const PagedParams P, uint32_t unit_rows) {
-    constexpr uint32_t LANES = HD / 4u, SETS = 256u / LANES, REC = HD + 4u;
-    __shared__ float4 s_acc[SETS][LANES];
-    __shared__ float2 s_ml[SETS];
-    q4d_pdl_wait();
-    const int4 e = P.ends[blockIdx.x];
-    const uint32_t first = (uint32_t)e.x, last = blockIdx.x;
-    if (e.x < 0) return;
-    const uint32_t set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4u;
-    const bool wide = last - first >= 2u * SETS;   /* 18 records and more at hd 128 */
-    const uint32_t at_once = wide ? 1u : SETS, step = wide ? SETS : 1u;
-    for (uint32_t r0 = blockIdx.y * at_once; r0 < unit_rows; r0 += gridDim.y * at_once) {
-        const uint32_t row = wide ? r0 : r0 + set, group = row / P.group_rows, in = row - group * P.group_rows, tl = in / P.gqa, tok = group * P.tpg + tl;
-        const bool live = row < unit_rows && tl < P.tpg && tok < (uint32_t)e.z;
-        float M = -CUDART_INF_F, L = 0.f;
-        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto join = [&](float m, float l, float4 x) {
-            const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m - Mu);
-            M = Mn;
-            L = L * fa + l * fb;
-            A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
-        };
-        if (live) {
-#pragma unroll 4
-            for (uint32_t c = first + (wide ? set : 0u); c <= last; c += step) {
-                const float *rec = P.part + (((size_t)c * 2u + (c == first ? 1u : 0u)) * unit_rows + row) * REC;
-                const float2 ml = __ldcg(reinterpret_cast<const float2 *>(rec + HD));
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(rec + d));
-                join(ml.x, ml.y, x);
-            }
-        }
-        if (wide) {
-            __syncthreads();   /* the row before has been joined */
-            s_acc[set][d / 4u] = A;
-            if (d == 0u) s_ml[set] = make_float2(M, L);
-            __syncthreads();
-            if (set) continue;
-            for (uint32_t k = 1; k < SETS; k++) join(s_ml[k].x, s_ml[k].y, s_acc[k][d / 4u]);
-        }
-        if (live) pg_store<HD>(P, (uint32_t)e.y + tok, (uint32_t)e.w * P.gqa + in - tl * P.gqa, d, A, L);
-    }
-}
-
 template <int KIND, int HD, int NT>
 bool few(PagedParams &p, float *scratch) {
     using C = FewCfg<KIND, HD, NT>;
-    static bool attr = false;
-    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_few_k<KIND, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
-    attr = true;
-    const uint32_t blocks = (uint32_t)g_q4.sm_count * C::CTAS;
+    static int per_sm = 0;
+    if (!per_sm && (!q4i_check(cudaFuncSetAttribute(q4_pg_few_k<KIND, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute") ||
+                    !q4i_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, q4_pg_few_k<KIND, HD, NT>, (int)C::THREADS, C::SMEM), "pages_attend occupancy")))
+        return false;
+    const uint32_t blocks = (uint32_t)g_q4.sm_count * ((uint32_t)per_sm < C::CTAS ? (uint32_t)per_sm : C::CTAS);   /* all resident: they meet */
+    if (!blocks) return q4i_fail(Q4E_CUDA, "pages_attend: no block fits an SM");
+    if (blocks > PG_MAX_BLOCKS) return q4i_fail(Q4E_CUDA, "pages_attend: more SMs than the counters are for");
     const size_t recs = (size_t)blocks * 2u * C::ROWS * C::REC;
     if (!scratch) {
-        if (!q4i_scratch(recs + (size_t)blocks * 4u, 0)) return false;
+        if (!q4i_scratch(recs, 0)) return false;
         scratch = g_q4.part;
     }
     p.part = scratch;
-    p.ends = reinterpret_cast<int4 *>(scratch + recs);
     p.tpg = C::ROWS / p.gqa;
     p.group_rows = C::ROWS;
-    return q4i_launch_pdl("pages_attend launch", q4_pg_few_k<KIND, HD, NT>, dim3(blocks), C::THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
+    static uint32_t *meet = nullptr;
+    if (!meet && !q4i_check(cudaGetSymbolAddress((void **)&meet, g_few_meet), "pages_attend counters")) return false;
+    p.meet = meet;
+    return q4i_launch_pdl("pages_attend launch", q4_pg_few_k<KIND, HD, NT>, dim3(blocks), C::THREADS, C::SMEM, p);
 }
 template <int KIND, int HD>
 bool few_by_rows(PagedParams &p, uint32_t rows, float *scratch) {
@@ -601,14 +544,6 @@ bool few_by_rows(PagedParams &p, uint32_t rows, float *scratch) {
 bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 
 }  // namespace
-
-bool q4i_paged_merge(const PagedParams &p, uint32_t hd, uint32_t blocks, uint32_t unit_rows) {
-    const uint32_t at_once = 1024u / hd, y = unit_rows / at_once < 16u ? unit_rows / at_once : 16u;
-    const dim3 grid(blocks, y < 8u ? 8u : y);
-    if (hd == 64) return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<64>, grid, 256u, 0, p, unit_rows);
-    if (hd == 128) return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<128>, grid, 256u, 0, p, unit_rows);
-    return q4i_launch_pdl("pages_attend merge", q4_pg_merge_k<256>, grid, 256u, 0, p, unit_rows);
-}
 
 extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, int q_bf16, const float *gate, void *out, int out_bf16,
                                     uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
@@ -640,7 +575,7 @@ extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, cons
         few_rows = p.gqa <= 8u ? 8u : 16u;
         p.add_split = n_req == 1u ? 0u : few_rows / p.gqa;
         /* records of both kernels: the second's must not fall on the first's while those are joined */
-        const size_t chunk = q4i_paged_chunk_floats(pg->hd), rest = (size_t)g_q4.sm_count * 2u * (2u * 32u * (256u + 4u) + 4u);
+        const size_t chunk = q4i_paged_chunk_floats(pg->hd), rest = (size_t)g_q4.sm_count * 2u * 2u * 32u * (256u + 4u);
         if (!q4i_scratch(chunk + rest, 0)) return false;
         if (!q4i_paged_chunk(p, pg->kind, pg->hd, g_q4.part)) return false;
         if (n_req == 1u) return true;

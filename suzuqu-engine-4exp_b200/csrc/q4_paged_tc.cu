@@ -30,6 +30,7 @@ using namespace q4tc;
 
 namespace {
 
+__device__ uint32_t g_chunk_meet[2u * PG_MAX_BLOCKS];
 constexpr uint32_t CK_BN = 128;
 constexpr uint32_t CK_SPIN_LIMIT = 1u << 22;
 constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
@@ -107,13 +108,14 @@ __device__ __forceinline__ bool ck_all_wait(uint32_t bar, uint32_t parity, uint3
     return __all_sync(0xffffffffu, ck_wait_on(bar, parity, s_abort));
 }
 
-/* sum of floor((a i + b) / m) over i < n (Euclid's steps on a and m) */
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a, uint64_t b) {
+/* sum of floor((a i + b) / 128) over i < n, a up to 256 and a n + b below 2^32 (Euclid's steps on a and 128) */
+__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t a, uint32_t b) {
     uint64_t r = 0;
+    uint32_t m = 128u;
     while (n) {
-        if (a >= m) { r += (n - 1u) * n / 2u * (a / m); a %= m; }
-        if (b >= m) { r += n * (b / m); b %= m; }
-        const uint64_t y = (uint64_t)a * n + b;
+        if (a >= m) { r += (uint64_t)n * (n - 1u) / 2u * (a / m); a %= m; }
+        if (b >= m) { r += (uint64_t)n * (b / m); b %= m; }
+        const uint32_t y = a * n + b;
         if (y < m) break;
         n = y / m;
         b = y % m;
@@ -127,7 +129,7 @@ __device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint32_t m, uint32_t a
 __device__ __forceinline__ uint32_t unit_tiles(const PgReq &R, uint32_t tpu, uint32_t g) {
     return (R.held + min((uint32_t)min((uint64_t)(g + 1u) * tpu, (uint64_t)R.add), R.add) + CK_BN - 1u) / CK_BN;
 }
-__device__ __forceinline__ uint64_t tiles_before(const PgReq &R, uint32_t tpu, uint32_t g) { return floor_sum(g, CK_BN, tpu, (uint64_t)R.held + tpu + CK_BN - 1u); }   /* g below the last */
+__device__ __forceinline__ uint64_t tiles_before(const PgReq &R, uint32_t tpu, uint32_t g) { return floor_sum(g, tpu, R.held + tpu + CK_BN - 1u); }   /* g below the last */
 __device__ __forceinline__ PgReq chunk_request(const PagedParams &P, uint32_t r, bool &bad) {
     PgReq q = pg_request(P, r, bad);
     if (q.add <= P.add_split) q.add = 0u;
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + TEAMS * WPT * C::ROUNDS * C::RAW;
     const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
                    s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 320, s_sum = bars + 352, w_full = bars + 480,
-                   w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_xch = bars + 1024;
+                   w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_split = bars + 928, s_xch = bars + 1024;
     uint8_t *base = smem_dyn + (sQ - smem_u32(smem_dyn));
     const uint32_t tpu = P.tpg * NQ;
 
@@ -263,24 +265,34 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         s_end = blockIdx.x < blocks ? total * (blockIdx.x + 1u) / blocks : 0u;
         if (s_begin < s_end && before <= s_begin && s_begin < before + mine)
             for (uint32_t r = r0; r < r1; r++) {
-                const PgReq R = chunk_request(P, r, bad);
-                const uint64_t n = request_steps(P, R, tpu);
+                const uint64_t n = request_steps(P, chunk_request(P, r, bad), tpu);
                 if (s_begin < before + n) {
-                    const uint64_t per_kh = n / P.n_kvh, off = s_begin - before;
-                    const uint32_t kh = (uint32_t)(off / per_kh), groups = (R.add + tpu - 1u) / tpu;
-                    const uint64_t in = off - (uint64_t)kh * per_kh;
-                    uint32_t lo = 0, hi = groups - 1u;   /* the last group that begins at or before `in` */
-                    while (lo < hi) {
-                        const uint32_t mid = (lo + hi + 1u) >> 1;
-                        if (tiles_before(R, tpu, mid) + (uint64_t)CK_EXTRA * mid <= in) lo = mid;
-                        else hi = mid - 1u;
-                    }
-                    const uint32_t st = (uint32_t)(in - (tiles_before(R, tpu, lo) + (uint64_t)CK_EXTRA * lo));
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"(kh), "r"(lo), "r"(st) : "memory");
+                    const uint64_t per_kh = n / P.n_kvh, off = s_begin - before, kh = off / per_kh, in = off - kh * per_kh;
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"((uint32_t)kh), "r"((uint32_t)in), "r"((uint32_t)(in >> 32)) : "memory");
                     break;
                 }
                 before += n;
             }
+        __syncthreads();
+        if (s_begin < s_end && warp == C::WALKER) {   /* the last group that begins at or before step `in`: 32 places at a time */
+            uint32_t r, kh, in0, in1;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r), "=r"(kh), "=r"(in0), "=r"(in1) : "r"(s_at));
+            const uint64_t in = (uint64_t)in1 << 32 | in0;
+            const PgReq R = chunk_request(P, r, bad);
+            uint32_t lo = 0, n = (R.add + tpu - 1u) / tpu;   /* it is lo or one of the n - 1 behind it */
+            uint64_t at = 0;
+            while (true) {
+                const uint32_t step = (n + 31u) / 32u, g = lo + lane * step;
+                const uint64_t s = tiles_before(R, tpu, g) + (uint64_t)CK_EXTRA * g;
+                const uint32_t below = __ballot_sync(0xffffffffu, lane * step < n && s <= in);   /* lane 0 always */
+                const uint32_t last = 31u - (uint32_t)__clz((int)below);
+                at = __shfl_sync(0xffffffffu, s, (int)last);
+                n = min(step, n - last * step);
+                lo += last * step;
+                if (step == 1u) break;
+            }
+            if (lane == 0) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(s_at + 8u), "r"(lo), "r"((uint32_t)(in - at)) : "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();   /* barriers initialised, tensor memory allocated, the share's place found */
@@ -415,14 +427,14 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             }
         }
         if (warp == C::WALKER) {
-            /* ================= walker: the share's pieces, where their tiles lie, and the unit that ends in this block ================= */
+            /* ================= walker: the share's pieces, where their tiles lie, and the units that are not this block's alone ================= */
             uint32_t n_tile = 0;
             const uint32_t per_page = P.part_bytes / TILE;
-            int4 end_of = make_int4(-1, 0, 0, 0);
+            PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* that began before this block; that go on behind it */
             Walk W;
             W.left = 0;
             if (s_begin < s_end) W.begin(P, s_begin, s_end - s_begin, w_req, w_kh, w_g, w_st);
-            for (uint32_t n = 0; ok; n++) {
+            for (uint32_t n = 0;; n++) {   /* to the end also where the others gave up: who meets whom does not change */
                 const uint32_t e = n % PIECES, a = s_piece + e * 32u;
                 const bool more = W.next(P, tpu, p);
                 bool gone = false;
@@ -443,9 +455,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
                     }
                 }
-                if (n >= PIECES) ok = ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
-                if (!ok) break;
-                if (lane == 0) {
+                if (n >= PIECES) ok = ok && ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
+                if (ok && lane == 0) {
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here | (gone ? 0x80000000u : 0u)), "r"(p.kh) : "memory");
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
                     mbar_arrive(w_full + 8 * e);
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     const bool there = (uint32_t)page < P.n_pages;
                     const uint32_t at = there ? ((uint32_t)page * P.n_kvh + p.kh) * per_page + ((q & ((1u << P.page_shift) - 1u)) >> 4) : 0u;
                     const uint32_t gone8 = __ballot_sync(0xffffffffu, !there) & 0xffu;
-                    if (n_tile >= TILES) ok = ck_all_wait(t_empty + 8 * te, (n_tile / TILES - 1u) & 1u, s_abort);
+                    if (n_tile >= TILES) ok = ok && ck_all_wait(t_empty + 8 * te, (n_tile / TILES - 1u) & 1u, s_abort);
                     if (!ok) break;
                     if (lane < 8u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ta + lane * 4u), "r"(at) : "memory");
                     if (lane == 8u) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(ta + 32u), "r"(n_kv - (p.st + tile) * CK_BN), "r"(gone8) : "memory");
@@ -471,10 +482,10 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     __syncwarp();
                     if (lane == 0) mbar_arrive(t_full + 8 * te);
                 }
-                if (p.st > 0u && p.st + p.here == p.tiles)   /* the unit ends here; it began in block .. */
-                    end_of = make_int4((int32_t)(((W.unit_at + 1u) * blocks - 1u) / total), (int32_t)p.tok0, (int32_t)p.n_here, (int32_t)p.kh);
+                if (p.st > 0u || p.here < p.tiles)   /* step x is block ((x + 1) blocks - 1) / total's */
+                    split[p.st == 0u] = {(uint32_t)(((W.unit_at + 1u) * blocks - 1u) / total), (uint32_t)(((W.unit_at + p.tiles) * blocks - 1u) / total), p.tok0, p.n_here, p.kh};
             }
-            if (lane == 0) P.ends[blockIdx.x] = end_of;
+            if (lane < 2u) *reinterpret_cast<PgSplit *>(base + (s_split - sQ) + lane * sizeof(PgSplit)) = lane ? split[1] : split[0];
         }
         if (warp >= C::PRODUCER && warp < C::PRODUCER + TEAMS * WPT) {
         /* ================= producers ================= */
@@ -924,9 +935,16 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         }
     }
     if (!ok && lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
+    __threadfence();             /* this thread's records */
     tc_fence_before();
     __syncthreads();
     if (warp == C::ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    const PgSplit *split = reinterpret_cast<const PgSplit *>(base + (s_split - sQ));
+    if (tid == 0) {
+        pg_arrive(P, split[0]);
+        pg_arrive(P, split[1]);
+    }
+    pg_join<HD, CK_THREADS>(P, split[0], C::ROWS, base, NQ * C::QG + SLOTS * SLOT);
 }
 
 template <int KIND, int HD>
@@ -936,18 +954,21 @@ bool chunk(PagedParams p, float *scratch) {
     if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_chunk_k<KIND, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM), "pages_attend smem attribute")) return false;
     attr = true;
     const uint32_t blocks = (uint32_t)g_q4.sm_count;
+    if (blocks > PG_MAX_BLOCKS) return q4i_fail(Q4E_CUDA, "pages_attend: more SMs than the counters are for");
     p.part = scratch;
-    p.ends = reinterpret_cast<int4 *>(scratch + (size_t)blocks * 2u * C::ROWS * C::REC);
     p.tpg = 128u / p.gqa;
     p.group_rows = 128u;
-    return q4i_launch_pdl("pages_attend launch", q4_pg_chunk_k<KIND, HD>, dim3(blocks), C::THREADS, C::SMEM, p) && q4i_paged_merge(p, HD, blocks, C::ROWS);
+    static uint32_t *meet = nullptr;
+    if (!meet && !q4i_check(cudaGetSymbolAddress((void **)&meet, g_chunk_meet), "pages_attend counters")) return false;
+    p.meet = meet;
+    return q4i_launch_pdl("pages_attend launch", q4_pg_chunk_k<KIND, HD>, dim3(blocks), C::THREADS, C::SMEM, p);
 }
 
 }  // namespace
 
 size_t q4i_paged_chunk_floats(uint32_t hd) {
     const size_t rows = hd == 256 ? 128u : 256u;
-    return (size_t)g_q4.sm_count * (2u * rows * (hd + 4u) + 4u);
+    return (size_t)g_q4.sm_count * 2u * rows * (hd + 4u);
 }
 bool q4i_paged_chunk(const PagedParams &p, int kind, uint32_t hd, float *scratch) {
     if (kind == Q4K_Q8) return hd == 64 ? chunk<Q4K_Q8, 64>(p, scratch) : hd == 128 ? chunk<Q4K_Q8, 128>(p, scratch) : chunk<Q4K_Q8, 256>(p, scratch);
