@@ -87,6 +87,8 @@ struct FewCfg {
     static constexpr uint32_t DEPTH = TILE <= 2304u ? 4u : 3u;
     static constexpr uint32_t THREADS = WARPS * 32u;
     static constexpr uint32_t STEP = WARPS * 16u;            /* positions per step */
+    static constexpr uint32_t EXTRA = 3u;                    /* steps that a piece costs besides its own */
+    using Shares = PgShares<EXTRA, 8u, 4u>;
     static constexpr uint32_t Q_STRIDE = HD * 2u + 32u;      /* the four rows of a half-warp's 8-byte reads on different banks */
     static constexpr uint32_t RING = WARPS * DEPTH * TILE;
     static constexpr uint32_t REC = HD + 4u;
@@ -99,10 +101,10 @@ struct FewCfg {
 template <int KIND, int HD, int NT>
 __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD, NT>::CTAS) q4_pg_few_k(const PagedParams P) {
     using C = FewCfg<KIND, HD, NT>;
-    constexpr uint32_t TILE = C::TILE, WARPS = C::WARPS, DEPTH = C::DEPTH, STEP = C::STEP, MT = HD / 16u;
+    constexpr uint32_t TILE = C::TILE, WARPS = C::WARPS, DEPTH = C::DEPTH, STEP = C::STEP, EXTRA = C::EXTRA, MT = HD / 16u;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t s_sum[WARPS];
-    __shared__ uint64_t s_off;
+    __shared__ uint64_t s_off, s_end2[2];
     __shared__ uint32_t s_req;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t s_base = (smem_u32(smem) + 1023u) & ~1023u;   /* swizzled tiles are anchored to multiples of 1024 */
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     };
     auto steps_of = [&](uint32_t r, bool &bad) -> uint64_t {
         const PgReq q = mine_of(r, bad);
-        return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh * ((q.held + q.add + STEP - 1u) / STEP);   /* no tokens: 0 groups */
+        return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh * ((q.held + q.add + STEP - 1u) / STEP + EXTRA);   /* no tokens: 0 groups */
     };
     const uint32_t per = (P.n_req + C::THREADS - 1u) / C::THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
     uint64_t mine = 0, total = 0, before = 0;
@@ -147,37 +149,50 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         before += x - mine;
     }
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-    const uint64_t blocks = min((uint64_t)gridDim.x, total);
-    if (blockIdx.x >= blocks) return;
-    uint64_t s = total * blockIdx.x / blocks;
-    const uint64_t s_end = total * (blockIdx.x + 1u) / blocks;
-    if (before <= s && s < before + mine)
+    typename C::Shares shares;
+    shares.set(total);
+    if (blockIdx.x >= shares.blocks) return;
+    if (tid == 0) s_end2[0] = s_end2[1] = total;
+    __syncthreads();
+    for (uint32_t i = 0; i < 2u && mine && blockIdx.x + i < shares.blocks; i++) {   /* the two cuts */
+        const uint64_t x = shares.cut(blockIdx.x + i);
+        if (x < before || x >= before + mine) continue;
+        uint64_t at = before;
         for (uint32_t r = r0; r < r1; r++) {
+            const PgReq q = mine_of(r, bad);
+            const uint32_t steps = (q.held + q.add + STEP - 1u) / STEP + EXTRA;
             const uint64_t n = steps_of(r, bad);
-            if (s < before + n) {
-                s_req = r;
-                s_off = s - before;
+            if (x < at + n) {
+                const uint64_t in = x - at, u0 = in >> 32 ? in / steps * steps : (uint32_t)in / steps * steps, to = u0 + C::Shares::snap(in - u0, steps);
+                if (i == 0u) {
+                    s_req = r;
+                    s_off = to;
+                }
+                s_end2[i] = at + to;
                 break;
             }
-            before += n;
+            at += n;
         }
+    }
     __syncthreads();
     uint32_t req = s_req, issued = 0, taken = 0;   /* of the warp's ring, over all pieces */
-    uint64_t off = s_off;
+    uint64_t off = s_off, s = s_end2[0];
+    const uint64_t s_end = s_end2[1];
     PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* units that began before this block; that go on behind it */
     bool ok = true;
 
     /* ---- pieces of units */
     while (s < s_end) {
         const PgReq R = mine_of(req, bad);
-        const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = (R.held + R.add + STEP - 1u) / STEP;
-        if (off >= (uint64_t)groups * P.n_kvh * n_steps) {   /* on to the next request; requests without tokens are passed over */
-            off -= (uint64_t)groups * P.n_kvh * n_steps;
+        const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = (R.held + R.add + STEP - 1u) / STEP, steps = n_steps + EXTRA;
+        if (off >= (uint64_t)groups * P.n_kvh * steps) {   /* on to the next request; requests without tokens are passed over */
+            off -= (uint64_t)groups * P.n_kvh * steps;
             req++;
             continue;
         }
-        const uint32_t unit = (uint32_t)(off / n_steps), st = (uint32_t)(off - (uint64_t)unit * n_steps);
-        const uint32_t here = (uint32_t)min((uint64_t)(n_steps - st), s_end - s);
+        const uint32_t unit = off >> 32 ? (uint32_t)(off / steps) : (uint32_t)off / steps, at = (uint32_t)(off - (uint64_t)unit * steps);
+        const uint32_t take = (uint32_t)min((uint64_t)(steps - at), s_end - s);
+        const uint32_t st = max(at, EXTRA) - EXTRA, here = max(at + take, EXTRA) - EXTRA - st;   /* the first EXTRA steps are none */
         const uint32_t kh = unit / groups, j0 = (unit - kh * groups) * P.tpg, n_here = min(P.tpg, R.add - j0);
         const uint32_t n_kv = R.held + j0 + n_here, live_rows = n_here * P.gqa, tok0 = R.tok0 + j0;
 
@@ -491,12 +506,9 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                 if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(rec[HD], L);
             }
         }
-        if (!whole) {
-            const uint64_t first = s - st;   /* the unit's first step; step x is block ((x + 1) blocks - 1) / total's */
-            split[st == 0u] = {(uint32_t)(((first + 1u) * blocks - 1u) / total), (uint32_t)(((first + n_steps) * blocks - 1u) / total), tok0, n_here, kh};
-        }
-        s += here;
-        off += here;
+        if (!whole) split[st == 0u] = {shares.first(s - at, s - at + steps), shares.last(s - at, s - at + steps), tok0, n_here, kh};
+        s += take;
+        off += take;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   /* the next bulk copies overwrite what was stored here */
     }
     __syncthreads();
@@ -504,7 +516,8 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         pg_arrive(P, split[0]);
         pg_arrive(P, split[1]);
     }
-    pg_join<HD, C::THREADS>(P, split[0], C::ROWS, base, C::RING);
+    for (uint32_t i = 0; i < 2u; i++)
+        if (i == 0u || split[1].last - split[1].first <= 2u) pg_join<HD, C::THREADS>(P, split[i], C::ROWS, base, C::RING, s_q + C::ROWS * C::Q_STRIDE + WARPS * DEPTH * 8u);
     if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
         if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
         for (; taken < issued; taken++)

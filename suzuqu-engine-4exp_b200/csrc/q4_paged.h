@@ -77,28 +77,78 @@ __device__ __forceinline__ void pg_store(const PagedParams &P, uint32_t tok, uin
     }
 }
 
+/* ---- shares.  `total` steps in `blocks` shares: share c begins at cut(c).  A cut that falls into a unit of at most SHORT steps, or
+ * within NEAR steps of the end of a longer one, goes to the unit's nearer end: that costs less than another piece and records that
+ * have to be joined. */
+template <uint32_t NEAR, uint32_t SHORT, uint32_t LEAST>
+struct PgShares {
+    uint64_t total;
+    uint32_t blocks;
+    /* as many shares as there are blocks, but none of fewer than LEAST steps */
+    __device__ __forceinline__ void set(uint64_t n) {
+        total = n;
+        blocks = (uint32_t)min((uint64_t)gridDim.x, n >> 32 ? n : max((uint32_t)n / LEAST, n ? 1u : 0u));
+    }
+    __device__ __forceinline__ uint64_t cut(uint32_t c) const {
+        return total >> 22 ? total * c / blocks : (uint32_t)total * c / blocks;   /* up to 1024 blocks */
+    }
+    __device__ __forceinline__ uint32_t of(uint64_t step) const {   /* the share that step would be in if no cut moved */
+        return total >> 21 ? (uint32_t)(((step + 1u) * blocks - 1u) / total) : (((uint32_t)step + 1u) * blocks - 1u) / (uint32_t)total;
+    }
+    /* where in a unit of `steps` steps a cut that falls on its step st lies */
+    static __device__ __forceinline__ uint64_t snap(uint64_t st, uint64_t steps) {
+        const uint64_t left = steps - st;
+        return steps > SHORT && st > NEAR && left > NEAR ? st : st <= left ? 0u : steps;
+    }
+    /* the shares that the first and the last step of the unit [u0, u1) are in */
+    __device__ __forceinline__ uint32_t first(uint64_t u0, uint64_t u1) const {
+        uint32_t c = of(u0);
+        while (c + 1u < blocks) {
+            const uint64_t b = cut(c + 1u);
+            if (b > u1 || snap(b - u0, u1 - u0) != 0u) break;
+            c++;
+        }
+        return c;
+    }
+    __device__ __forceinline__ uint32_t last(uint64_t u0, uint64_t u1) const {
+        uint32_t c = of(u1 - 1u);
+        while (c > 0u) {
+            const uint64_t b = cut(c);
+            if (b <= u0 || snap(b - u0, u1 - u0) != u1 - u0) break;
+            c--;
+        }
+        return c;
+    }
+};
 /* A unit that lies in several blocks, first to last; last < first: none */
 struct PgSplit { uint32_t first, last, tok0, n_here, kh; };
-/* The blocks of a split unit meet at a counter, and all but the first, which has the end of another unit to see to, join its
- * records, each an equal part of the rows.  All blocks of the launch are resident (the grid is what the SMs hold), and end their
- * shares within a few microseconds of one another; a launch of its own for this took 8 to 12 us (one request over 262 144 rows
- * 44 us with it).  The wait is bounded.  Every block arrives and goes once, whatever happened before, and the last to go leaves
- * the counters at zero.
- * What a block joins, and its gates, come to shared memory by asynchronous copies, all at once; then a thread has four dims of a
- * row, or shares them with others that take the other records. */
+/* The blocks of a split unit meet at a counter and join its records, each an equal part (the first, which may have the end of another
+ * unit to see to, only of a unit of two or three blocks: one block alone takes 15 us for it): some of the rows, or, where there are more blocks than rows, a half, a quarter .. of one.  All blocks
+ * of the launch are resident (the grid is what the SMs hold), and end their shares within a few microseconds of one another; a
+ * launch of its own for this took 8 to 12 us (one request over 262 144 rows 44 us with it).  The wait is bounded.  Every block
+ * arrives and goes once, whatever happened before, and the last to go leaves the counters at zero.
+ * What a block joins, and its gates, come to shared memory by bulk copies, all at once (16 bytes per thread and step: 6 to 10 us for
+ * 160 KB); then a thread has four dims of a row, or shares them with others that take the other records. */
 __device__ __forceinline__ void pg_arrive(const PagedParams &P, const PgSplit &u) {   /* one thread, behind the block's records and a barrier */
     if (u.last < u.first) return;
+    asm volatile("fence.proxy.async;" ::: "memory");   /* the records are read by bulk copies */
     __threadfence();
     atomicAdd(P.meet + 2u * u.first, 1u);
 }
+/* bar: 8 bytes of shared memory for a barrier, not in use by anything */
 template <int HD, uint32_t THREADS>
-__device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes) {
-    constexpr uint32_t REC = HD + 4u, PIECES = REC / 4u, WARPS = THREADS / 32u;   /* of 16 bytes */
+__device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes, uint32_t bar) {
+    constexpr uint32_t REC = HD + 4u;
     if (u.last < u.first) return;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, k = u.last - u.first + 1u, mine = blockIdx.x - u.first - 1u;
-    const uint32_t r_begin = unit_rows * mine / (k - 1u), r_end = unit_rows * (mine + 1u) / (k - 1u);
-    if (r_begin < r_end) {
+    const uint32_t tid = threadIdx.x, k = u.last - u.first + 1u, joiners = k <= 3u ? k : k - 1u, mine = blockIdx.x - u.last + joiners - 1u;   /* the last ones */
+    if (mine >= joiners) return;
+    uint32_t cut = 0;   /* a row is 1 << cut slices of at least 32 dims */
+    while (cut < (HD == 64 ? 1u : HD == 128 ? 2u : 3u) && unit_rows << cut < joiners) cut++;
+    const uint32_t wide = (uint32_t)HD >> cut, slices = unit_rows << cut;
+    const uint32_t s_begin = slices * mine / joiners, s_end = slices * (mine + 1u) / joiners;
+    if (s_begin < s_end) {
         if (tid == 0) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
             unsigned long long t0, t;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
             for (uint32_t i = 0;; i++) {
@@ -115,84 +165,103 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
             }
             __threadfence();
         }
-        __syncthreads();
         float4 *s_a = reinterpret_cast<float4 *>(smem);                      /* [thread] */
         float2 *s_ml = reinterpret_cast<float2 *>(smem + THREADS * 16u);     /* [thread] */
-        float *s_gate = reinterpret_cast<float *>(smem + THREADS * 24u);     /* [row][hd] */
-        /* as many rows at once as fit with all their records; or one row, and its records in turn */
-        const uint32_t room = smem_bytes - THREADS * 24u, gate_bytes = P.gate ? HD * 4u : 0u, fit = room / (k * REC * 4u + gate_bytes);
-        const uint32_t rows_at_once = fit ? fit : 1u, recs_at_once = fit ? k : (room - gate_bytes) / (REC * 4u);
-        for (uint32_t r0 = r_begin; r0 < r_end; r0 += rows_at_once) {
-        const uint32_t rows = min(rows_at_once, r_end - r0), items = rows * (HD / 4u), padded = (items + 31u) & ~31u, groups = padded < THREADS ? THREADS / padded : 1u;
-        float *s_rec = s_gate + (P.gate ? rows * HD : 0u);                   /* [record][row][hd + 4] */
-        /* token and head of a row of these; false: a row without a token */
-        auto place = [&](uint32_t rl, uint32_t &tok, uint32_t &head) -> bool {
-            const uint32_t row = r0 + rl, tg = row / P.group_rows, in = row - tg * P.group_rows, tl = in / P.gqa;
-            tok = tg * P.tpg + tl;
-            head = u.kh * P.gqa + in - tl * P.gqa;
-            const bool live = tl < P.tpg && tok < u.n_here;
-            tok += u.tok0;
-            return live;
-        };
-        auto copy = [&](float *to, const float *from) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-        };
-        auto bring = [&](uint32_t c0, uint32_t n) {   /* a row of a record per warp and step */
-            for (uint32_t pair = warp; pair < n * rows; pair += WARPS) {
-                const uint32_t c = pair / rows, rl = pair - c * rows, b = u.first + c0 + c;
-                const float *src = P.part + (((size_t)b * 2u + (b == u.first ? 1u : 0u)) * unit_rows + r0 + rl) * REC;
-                for (uint32_t x = lane; x < PIECES; x += 32u) copy(s_rec + (size_t)pair * REC + x * 4u, src + x * 4u);
-            }
-            if (P.gate && c0 == 0u)
-                for (uint32_t rl = warp; rl < rows; rl += WARPS) {
-                    uint32_t tok, head;
-                    if (place(rl, tok, head))
-                        for (uint32_t x = lane; x < HD / 4u; x += 32u) copy(s_gate + rl * HD + x * 4u, P.gate + ((size_t)tok * P.n_head + head) * HD + x * 4u);
-                }
-            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-            __syncthreads();
-        };
-        __syncthreads();   /* the rows before have been read */
-        bring(0u, recs_at_once);
-        for (uint32_t item0 = 0; item0 < items; item0 += groups > 1u ? padded : THREADS) {
-            const uint32_t group = groups > 1u ? tid / padded : 0u, item = item0 + (groups > 1u ? tid - group * padded : tid);
-            const uint32_t rl = item / (HD / 4u), d = item % (HD / 4u) * 4u;
-            uint32_t tok, head;
-            const bool live = item < items && group < groups && place(rl, tok, head);
-            float M = -CUDART_INF_F, L = 0.f;
-            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto join = [&](float m, float l, float4 x) {
-                const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = pg_ex2(M - Mu), fb = pg_ex2(m - Mu);
-                M = Mn;
-                L = L * fa + l * fb;
-                A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
+        float *s_gate = reinterpret_cast<float *>(smem + THREADS * 24u);     /* [slice][its dims] */
+        /* as many slices at once as fit with all their records; or one, and its records in turn */
+        const uint32_t stride = wide + 4u, room = smem_bytes - THREADS * 24u, gate_bytes = P.gate ? wide * 4u : 0u, fit = room / (k * stride * 4u + gate_bytes);
+        const uint32_t at_once = fit ? fit : 1u, recs_at_once = fit ? k : (room - gate_bytes) / (stride * 4u);
+        uint32_t phase = 0;
+        for (uint32_t s0 = s_begin; s0 < s_end; s0 += at_once) {
+            const uint32_t n_s = min(at_once, s_end - s0), items = n_s * (wide / 4u), padded = (items + 31u) & ~31u, groups = padded < THREADS ? THREADS / padded : 1u;
+            float *s_rec = s_gate + (P.gate ? n_s * wide : 0u);              /* [record][slice][its dims, m, l, -, -] */
+            /* token and head of a slice's row; false: a row without a token */
+            auto place = [&](uint32_t s, uint32_t &tok, uint32_t &head) -> bool {
+                const uint32_t row = (s0 + s) >> cut, tg = row / P.group_rows, in = row - tg * P.group_rows, tl = in / P.gqa;
+                tok = tg * P.tpg + tl;
+                head = u.kh * P.gqa + in - tl * P.gqa;
+                const bool live = tl < P.tpg && tok < u.n_here;
+                tok += u.tok0;
+                return live;
             };
-            for (uint32_t c0 = 0; c0 < k; c0 += recs_at_once) {   /* more than one turn: one row, and at most a thread per item */
-                const uint32_t n = min(recs_at_once, k - c0);
-                if (c0) {
-                    __syncthreads();   /* the records before have been read */
-                    bring(c0, n);
-                }
-                if (live)
-                    for (uint32_t c = group; c < n; c += groups) {
-                        const float *rec = s_rec + ((size_t)c * rows + rl) * REC;
-                        const float2 ml = *reinterpret_cast<const float2 *>(rec + HD);
-                        join(ml.x, ml.y, *reinterpret_cast<const float4 *>(rec + d));
-                    }
-            }
-            if (groups > 1u) {
-                s_a[tid] = A;
-                s_ml[tid] = make_float2(M, L);
+            auto copy = [&](float *to, const float *from, uint32_t bytes) {
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                             ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(bytes), "r"(bar) : "memory");
+            };
+            auto bring = [&](uint32_t c0, uint32_t n, bool gates) {
+                asm volatile("fence.proxy.async;" ::: "memory");             /* what lies there was used by ordinary accesses, and the records were written by such */
                 __syncthreads();
-                if (live && group == 0u)
-                    for (uint32_t o = 1; o < groups; o++) join(s_ml[o * padded + tid].x, s_ml[o * padded + tid].y, s_a[o * padded + tid]);
+                if (tid == 0) {
+                    uint32_t bytes = n * n_s * stride * 4u;
+                    if (gates) bytes += n_s * wide * 4u;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+                }
+                __syncthreads();
+                if (cut == 0u) {                                             /* whole rows lie one behind the other */
+                    for (uint32_t c = tid; c < n; c += THREADS) {
+                        const uint32_t b = u.first + c0 + c;
+                        copy(s_rec + (size_t)c * n_s * REC, P.part + (((size_t)b * 2u + (b == u.first ? 1u : 0u)) * unit_rows + s0) * REC, n_s * REC * 4u);
+                    }
+                } else {
+                    for (uint32_t i = tid; i < n * n_s; i += THREADS) {
+                        const uint32_t c = i / n_s, s = i - c * n_s, b = u.first + c0 + c, row = (s0 + s) >> cut, part = (s0 + s) & ((1u << cut) - 1u);
+                        const float *rec = P.part + (((size_t)b * 2u + (b == u.first ? 1u : 0u)) * unit_rows + row) * REC;
+                        copy(s_rec + (size_t)i * stride, rec + part * wide, wide * 4u);
+                        copy(s_rec + (size_t)i * stride + wide, rec + HD, 16u);
+                    }
+                }
+                if (gates)
+                    for (uint32_t s = tid; s < n_s; s += THREADS) {
+                        uint32_t tok, head;
+                        if (!place(s, tok, head)) tok = u.tok0, head = u.kh * P.gqa;   /* any gate: not used */
+                        copy(s_gate + s * wide, P.gate + ((size_t)tok * P.n_head + head) * HD + ((s0 + s) & ((1u << cut) - 1u)) * wide, wide * 4u);
+                    }
+                for (uint32_t i = 0; i < (1u << 20); i++) {                  /* bounded: a copy ends by itself */
+                    uint32_t done;
+                    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                                 : "=r"(done) : "r"(bar), "r"(phase) : "memory");
+                    if (done) break;
+                }
+                phase ^= 1u;
+            };
+            bring(0u, recs_at_once < k ? recs_at_once : k, P.gate != nullptr);
+            for (uint32_t item0 = 0; item0 < items; item0 += groups > 1u ? padded : THREADS) {
+                const uint32_t group = groups > 1u ? tid / padded : 0u, item = item0 + (groups > 1u ? tid - group * padded : tid);
+                const uint32_t s = item / (wide / 4u), d = item % (wide / 4u) * 4u;
+                uint32_t tok, head;
+                const bool live = item < items && group < groups && place(s, tok, head);
+                float M = -CUDART_INF_F, L = 0.f;
+                float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+                auto join = [&](float m, float l, float4 x) {
+                    const float Mn = fmaxf(M, m), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = pg_ex2(M - Mu), fb = pg_ex2(m - Mu);
+                    M = Mn;
+                    L = L * fa + l * fb;
+                    A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
+                };
+                for (uint32_t c0 = 0; c0 < k; c0 += recs_at_once) {          /* more than one turn: one slice, and at most a thread per item */
+                    const uint32_t n = min(recs_at_once, k - c0);
+                    if (c0) bring(c0, n, false);
+                    if (live)
+                        for (uint32_t c = group; c < n; c += groups) {
+                            const float *rec = s_rec + ((size_t)c * n_s + s) * stride;
+                            const float2 ml = *reinterpret_cast<const float2 *>(rec + wide);
+                            join(ml.x, ml.y, *reinterpret_cast<const float4 *>(rec + d));
+                        }
+                }
+                if (groups > 1u) {
+                    s_a[tid] = A;
+                    s_ml[tid] = make_float2(M, L);
+                    __syncthreads();
+                    if (live && group == 0u)
+                        for (uint32_t o = 1; o < groups; o++) join(s_ml[o * padded + tid].x, s_ml[o * padded + tid].y, s_a[o * padded + tid]);
+                }
+                if (live && group == 0u) pg_store<HD>(P, tok, head, ((s0 + s) & ((1u << cut) - 1u)) * wide + d, A, L, P.gate ? s_gate + s * wide + d : nullptr);
             }
-            if (live && group == 0u) pg_store<HD>(P, tok, head, d, A, L, P.gate ? s_gate + rl * HD + d : nullptr);
-        }
         }
     }
     __syncthreads();
-    if (tid == 0 && atomicAdd(P.meet + 2u * u.first + 1u, 1u) == k - 2u) {
+    if (tid == 0 && s_begin < s_end) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    if (tid == 0 && atomicAdd(P.meet + 2u * u.first + 1u, 1u) == joiners - 1u) {
         P.meet[2u * u.first] = 0u;
         P.meet[2u * u.first + 1u] = 0u;
     }

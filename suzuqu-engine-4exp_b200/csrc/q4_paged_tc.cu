@@ -37,9 +37,6 @@ constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
 constexpr uint32_t PIECES = 4, TILES = 4;   /* pieces that are walked ahead, tiles whose pages are found ahead */
 constexpr float CK_RESCALE_TAU = 8.f;   /* weights reach 2^8 before the reference moves */
 
-/* A piece costs about as much besides its tiles (queries in, outputs out, the first scores) as this many of them: a unit counts as so
- * many more steps when the work is shared out.  Only tiles are walked; a share may hold none. */
-constexpr uint32_t CK_EXTRA = 2;
 template <int KIND, int HD>
 struct ChunkCfg {
     static constexpr uint32_t NQ = HD == 256 ? 1u : 2u, ROWS = NQ * 128u;
@@ -53,6 +50,11 @@ struct ChunkCfg {
     static constexpr uint32_t ITEMS = SLOT / 32u / (WPT * 32u * RPS);   /* of 16 codes, per producer thread and round */
     static constexpr uint32_t ROUNDS = HD == 256 ? 2u : 3u;       /* rounds of codes on their way to a warp */
     static constexpr uint32_t RAW = KIND == Q4K_Q8 ? ITEMS * 544u : 0u;   /* codes and scales of a warp's round */
+    /* A piece takes 7.7 us (hd 256: 8.7) besides its tiles (queries in, the first scores, outputs out), a tile 2.2 (hd 256: 1.4 in fp16, 3.2
+     * in q8_0): a unit counts as EXTRA more steps when the work is shared out.  Only tiles are walked.  512 tokens over 16 001 rows
+     * 109 us with EXTRA 2, 98 with 3. */
+    static constexpr uint32_t EXTRA = HD == 256 ? (KIND == Q4K_Q8 ? 3u : 6u) : KIND == Q4K_Q8 ? 3u : 4u;
+    using Shares = PgShares<EXTRA, HD == 256 ? 4u * EXTRA : 16u, EXTRA + 2u>;
     /* registers of a thread: the block's 512 x 128 are 256 threads x (softmax + the others) */
     static constexpr uint32_t R_SOFTMAX = 168u, R_OTHERS = 88u;
     static_assert(R_SOFTMAX + R_OTHERS <= 256u, "register split");
@@ -135,6 +137,7 @@ __device__ __forceinline__ PgReq chunk_request(const PagedParams &P, uint32_t r,
     if (q.add <= P.add_split) q.add = 0u;
     return q;
 }
+template <uint32_t CK_EXTRA>
 __device__ __forceinline__ uint64_t request_steps(const PagedParams &P, const PgReq &R, uint32_t tpu) {
     if (!R.add) return 0u;
     const uint32_t groups = (R.add + tpu - 1u) / tpu;
@@ -149,10 +152,11 @@ struct Piece {
     uint32_t tiles;              /* of the unit */
     bool gone;                   /* some of its positions are on pages that are not the pool's */
 };
+template <uint32_t CK_EXTRA>
 struct Walk {
     uint64_t left;               /* steps of the share still to come */
     uint64_t now;                /* of all steps, the next one */
-    uint64_t unit_at;            /* of all steps, the first tile of the unit of the last piece */
+    uint64_t unit_at;            /* of all steps, the first of the unit of the last piece */
     uint32_t req, kh, g, st;
     PgReq R;
     __device__ __forceinline__ void begin(const PagedParams &P, uint64_t s0, uint64_t n, uint32_t r, uint32_t kh_, uint32_t g_, uint32_t st_) {
@@ -168,7 +172,7 @@ struct Walk {
             p.n_here = min(tpu, R.add - g * tpu);
             p.before = R.held + g * tpu; p.tok0 = R.tok0 + g * tpu; p.kh = kh; p.req = req;
             const uint32_t here = (uint32_t)min((uint64_t)(p.tiles + CK_EXTRA - st), left), end = st + here;
-            unit_at = now - st + CK_EXTRA;
+            unit_at = now - st;
             p.st = max(st, CK_EXTRA) - CK_EXTRA;
             p.here = max(end, CK_EXTRA) - CK_EXTRA - p.st;
             left -= here;
@@ -195,7 +199,7 @@ template <int KIND, int HD>
 __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(const PagedParams P) {
     using C = ChunkCfg<KIND, HD>;
     constexpr uint32_t CK_THREADS = C::THREADS, TEAMS = C::TEAMS, WPT = C::WPT, NQ = C::NQ, SLOT = C::SLOT, SLOTS = C::SLOTS, PARTS = C::PARTS, UN = C::UN, TU = 64;
-    constexpr uint32_t O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
+    constexpr uint32_t CK_EXTRA = C::EXTRA, O_COL = 256, TMEM_COLS = 512, TILE = PgTile<KIND, HD>::BYTES, ROW = PgTile<KIND, HD>::ROW;
     extern __shared__ uint8_t smem_dyn[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + TEAMS * WPT * C::ROUNDS * C::RAW;
@@ -235,14 +239,16 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     }
     q4d_pdl_wait();
 
-    /* ---- this block's share */
-    uint64_t total = 0, s_begin, s_end, blocks;
+    /* ---- this block's share: the steps of all requests by one scan, the two places where it is cut by two warps */
+    typename C::Shares shares;
     {
         const uint32_t per = (P.n_req + CK_THREADS - 1u) / CK_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
-        uint64_t mine = 0, before = 0;
+        uint64_t mine = 0, before = 0, total = 0;
         bool bad, any_bad = false;
+        PgReq R = {0u, 0u, 0u};
         for (uint32_t r = r0; r < r1; r++) {
-            mine += request_steps(P, chunk_request(P, r, bad), tpu);
+            R = chunk_request(P, r, bad);
+            mine += request_steps<CK_EXTRA>(P, R, tpu);
             any_bad |= bad;
         }
         uint64_t x = mine;
@@ -260,46 +266,74 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         }
         before += x - mine;
         if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-        blocks = min((uint64_t)gridDim.x, total);
-        s_begin = blockIdx.x < blocks ? total * blockIdx.x / blocks : 0u;
-        s_end = blockIdx.x < blocks ? total * (blockIdx.x + 1u) / blocks : 0u;
-        if (s_begin < s_end && before <= s_begin && s_begin < before + mine)
-            for (uint32_t r = r0; r < r1; r++) {
-                const uint64_t n = request_steps(P, chunk_request(P, r, bad), tpu);
-                if (s_begin < before + n) {
-                    const uint64_t per_kh = n / P.n_kvh, off = s_begin - before, kh = off / per_kh, in = off - kh * per_kh;
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"((uint32_t)kh), "r"((uint32_t)in), "r"((uint32_t)(in >> 32)) : "memory");
-                    break;
-                }
-                before += n;
-            }
+        shares.set(total);
+        if (tid < 2u) asm volatile("st.shared.v2.u64 [%0], {%1, %1};" ::"r"(s_at + 16u), "l"(total) : "memory");   /* begin and end: none yet, the last share's end */
         __syncthreads();
-        if (s_begin < s_end && warp == C::WALKER) {   /* the last group that begins at or before step `in`: 32 places at a time */
-            uint32_t r, kh, in0, in1;
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r), "=r"(kh), "=r"(in0), "=r"(in1) : "r"(s_at));
-            const uint64_t in = (uint64_t)in1 << 32 | in0;
-            const PgReq R = chunk_request(P, r, bad);
+        if (mine && blockIdx.x < shares.blocks) {
+#pragma unroll 1
+            for (uint32_t i = 0; i < 2u; i++) {
+                if (blockIdx.x + i >= shares.blocks) break;
+                const uint64_t s = shares.cut(blockIdx.x + i);
+                if (s < before || s >= before + mine) continue;
+                uint64_t at = before;
+                for (uint32_t r = r0; r < r1; r++) {
+                    if (per > 1u) R = chunk_request(P, r, bad);
+                    const uint64_t n = per > 1u ? request_steps<CK_EXTRA>(P, R, tpu) : mine;
+                    if (s < at + n) {
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_piece + 64u * i), "r"(r), "r"(R.held), "r"(R.add), "r"(R.tok0) : "memory");
+                        asm volatile("st.shared.v2.u64 [%0], {%1, %2};" ::"r"(s_piece + 64u * i + 16u), "l"(s), "l"(s - at) : "memory");
+                        asm volatile("st.shared.u64 [%0], %1;" ::"r"(s_piece + 64u * i + 32u), "l"(n) : "memory");
+                        break;
+                    }
+                    at += n;
+                }
+            }
+        }
+        __syncthreads();
+        const uint32_t which = warp - C::WALKER;
+        if (which < 2u && blockIdx.x + which < shares.blocks) {   /* the last group that begins at or before the cut: 32 places at a time */
+            uint32_t r;
+            uint64_t s, in, n_all;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r), "=r"(R.held), "=r"(R.add), "=r"(R.tok0) : "r"(s_piece + 64u * which));
+            asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(s), "=l"(in) : "r"(s_piece + 64u * which + 16u));
+            asm volatile("ld.shared.u64 %0, [%1];" : "=l"(n_all) : "r"(s_piece + 64u * which + 32u));
+            uint32_t kh;
+            if (n_all >> 32) {
+                const uint64_t per_kh = n_all / P.n_kvh;
+                kh = (uint32_t)(in / per_kh);
+                in -= kh * per_kh;
+            } else {
+                const uint32_t per_kh = (uint32_t)n_all / P.n_kvh;
+                kh = (uint32_t)in / per_kh;
+                in -= kh * per_kh;
+            }
             uint32_t lo = 0, n = (R.add + tpu - 1u) / tpu;   /* it is lo or one of the n - 1 behind it */
             uint64_t at = 0;
             while (true) {
                 const uint32_t step = (n + 31u) / 32u, g = lo + lane * step;
-                const uint64_t s = tiles_before(R, tpu, g) + (uint64_t)CK_EXTRA * g;
-                const uint32_t below = __ballot_sync(0xffffffffu, lane * step < n && s <= in);   /* lane 0 always */
+                const uint64_t x2 = tiles_before(R, tpu, g) + (uint64_t)CK_EXTRA * g;
+                const uint32_t below = __ballot_sync(0xffffffffu, lane * step < n && x2 <= in);   /* lane 0 always */
                 const uint32_t last = 31u - (uint32_t)__clz((int)below);
-                at = __shfl_sync(0xffffffffu, s, (int)last);
+                at = __shfl_sync(0xffffffffu, x2, (int)last);
                 n = min(step, n - last * step);
                 lo += last * step;
                 if (step == 1u) break;
             }
-            if (lane == 0) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(s_at + 8u), "r"(lo), "r"((uint32_t)(in - at)) : "memory");
+            const uint32_t st = (uint32_t)(in - at), to = (uint32_t)C::Shares::snap(st, unit_tiles(R, tpu, lo) + CK_EXTRA);
+            if (lane == 0) {
+                if (which == 0u) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"(kh), "r"(lo), "r"(to) : "memory");
+                asm volatile("st.shared.u64 [%0], %1;" ::"r"(s_at + 16u + 8u * which), "l"(s - st + to) : "memory");
+            }
         }
     }
     tc_fence_before();
     __syncthreads();   /* barriers initialised, tensor memory allocated, the share's place found */
     tc_fence_after();
     uint32_t tmem, w_req, w_kh, w_g, w_st;
+    uint64_t s_begin, s_end;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w_req), "=r"(w_kh), "=r"(w_g), "=r"(w_st) : "r"(s_at));
+    asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(s_begin), "=l"(s_end) : "r"(s_at + 16u));
     bool ok = true;
     /* the next piece, by a whole warp; its place is given back with piece_done */
     uint32_t n_piece = 0;
@@ -431,21 +465,32 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             uint32_t n_tile = 0;
             const uint32_t per_page = P.part_bytes / TILE;
             PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* that began before this block; that go on behind it */
-            Walk W;
+            Walk<CK_EXTRA> W;
             W.left = 0;
             if (s_begin < s_end) W.begin(P, s_begin, s_end - s_begin, w_req, w_kh, w_g, w_st);
             for (uint32_t n = 0;; n++) {   /* to the end also where the others gave up: who meets whom does not change */
                 const uint32_t e = n % PIECES, a = s_piece + e * 32u;
                 const bool more = W.next(P, tpu, p);
+                const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
+                const uint32_t n_kv = p.before + p.n_here, q0 = p.st * CK_BN + (lane & 7u) * 16u;
+                auto entry = [&](uint32_t tile) -> int32_t { return tile < p.here && q0 + tile * CK_BN < n_kv ? tab[(q0 + tile * CK_BN) >> P.page_shift] : 0; };
+                int32_t next = entry(0);
                 bool gone = false;
                 if (more) {   /* the softmax looks for missing pages only where there are any */
-                    const uint32_t last = min((p.st + p.here) * CK_BN, p.before + p.n_here) - 1u;
-                    const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
+                    const uint32_t last = min((p.st + p.here) * CK_BN, n_kv) - 1u;
+#pragma unroll 4
                     for (uint32_t i = (p.st * CK_BN >> P.page_shift) + lane; i <= last >> P.page_shift; i += 32u) gone |= (uint32_t)tab[i] >= P.n_pages;
                     gone = __any_sync(0xffffffffu, gone);
                     if (gone && lane == 0) atomicOr(P.err, (uint32_t)Q4E_RANGE);
                 }
-                if (more) {   /* its queries, and the gates if it is a whole unit, are on their way when it begins */
+                if (n >= PIECES) ok = ok && ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
+                if (ok && lane == 0) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here | (gone ? 0x80000000u : 0u)), "r"(p.kh) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
+                    mbar_arrive(w_full + 8 * e);
+                }
+                if (!more) break;
+                if (n) {   /* its queries, and the gates if it is a whole unit, are on their way when it begins (the first piece begins at once) */
                     const bool whole = p.st == 0u && p.here == p.tiles;
                     const uint32_t q_line = P.gqa * HD * (P.q_bf16 ? 2u : 4u) / 128u, g_line = whole && P.gate ? P.gqa * HD / 32u : 0u;   /* lines of 128 bytes per token */
                     for (uint32_t i = lane; i < p.n_here * (q_line + g_line); i += 32u) {
@@ -455,18 +500,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
                     }
                 }
-                if (n >= PIECES) ok = ok && ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
-                if (ok && lane == 0) {
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here | (gone ? 0x80000000u : 0u)), "r"(p.kh) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
-                    mbar_arrive(w_full + 8 * e);
-                }
-                if (!more) break;
                 /* tile by tile: where its eight tiles of 16 positions lie, in units of such tiles; its live positions; those without a page */
-                const int32_t *tab = P.table + (size_t)p.req * P.table_stride;
-                const uint32_t n_kv = p.before + p.n_here, q0 = p.st * CK_BN + (lane & 7u) * 16u;
-                auto entry = [&](uint32_t tile) -> int32_t { return tile < p.here && q0 + tile * CK_BN < n_kv ? tab[(q0 + tile * CK_BN) >> P.page_shift] : 0; };
-                int32_t next = entry(0);
                 for (uint32_t tile = 0; tile < p.here && ok; tile++, n_tile++) {
                     const int32_t page = next;
                     next = entry(tile + 1u);
@@ -482,8 +516,10 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     __syncwarp();
                     if (lane == 0) mbar_arrive(t_full + 8 * te);
                 }
-                if (p.st > 0u || p.here < p.tiles)   /* step x is block ((x + 1) blocks - 1) / total's */
-                    split[p.st == 0u] = {(uint32_t)(((W.unit_at + 1u) * blocks - 1u) / total), (uint32_t)(((W.unit_at + p.tiles) * blocks - 1u) / total), p.tok0, p.n_here, p.kh};
+                if (p.st > 0u || p.here < p.tiles) {
+                    const uint64_t u1 = W.unit_at + p.tiles + CK_EXTRA;
+                    split[p.st == 0u] = {shares.first(W.unit_at, u1), shares.last(W.unit_at, u1), p.tok0, p.n_here, p.kh};
+                }
             }
             if (lane < 2u) *reinterpret_cast<PgSplit *>(base + (s_split - sQ) + lane * sizeof(PgSplit)) = lane ? split[1] : split[0];
         }
@@ -722,7 +758,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             const bool active = g == 0u || p.n_here > P.tpg;
             /* ---- queries as fp16, swizzled rows of 64 dims: the products of the piece before have read theirs (its last scores are here) */
             {
-                constexpr uint32_t PER = HD / 8u, T = NQ == 2u ? 128u : 256u, STEPS = 128u * PER / T, BATCH = 8u;
+                constexpr uint32_t PER = HD / 8u, T = NQ == 2u ? 128u : 256u, STEPS = 128u * PER / T, BATCH = 8u;   /* loads in flight before the first store */
                 const uint32_t qt = NQ == 2u ? r : tid;
                 if (active) {
 #pragma unroll 1
@@ -944,7 +980,9 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         pg_arrive(P, split[0]);
         pg_arrive(P, split[1]);
     }
-    pg_join<HD, CK_THREADS>(P, split[0], C::ROWS, base, NQ * C::QG + SLOTS * SLOT);
+    const PgSplit ends = split[0], begins = split[1];   /* what follows uses the shared memory */
+    pg_join<HD, CK_THREADS>(P, ends, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
+    if (begins.last - begins.first <= 2u) pg_join<HD, CK_THREADS>(P, begins, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
 }
 
 template <int KIND, int HD>
