@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <math_constants.h>
 #include <string.h>
+#include <type_traits>
 
 #include "q4_paged.h"
 
@@ -66,25 +67,30 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+/* the same with an initial accumulator of its own, one value per column */
+__device__ __forceinline__ void mma16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-/* fp16 1024 + 128 + code has (code ^ 0x80) in its low byte: two bytes picked out of word x (its codes ^ 0x80) become the exact codes */
+/* fp16 1024 + 128 + code has (code ^ 0x80) in its low byte: two bytes picked out of word x (its codes ^ 0x80), and the exact codes */
 template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-    return h2u(__hsub2(u2h(__byte_perm(x, 0x64646464u, SEL)), u2h(0x64806480u)));
-}
+__device__ __forceinline__ uint32_t raised2(uint32_t x) { return __byte_perm(x, 0x64646464u, SEL); }
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) { return h2u(__hsub2(u2h(raised2<SEL>(x)), u2h(0x64806480u))); }
 
 /* warps per block, blocks per SM, tiles of a warp's ring: as many bytes in flight as an SM's shared memory holds */
 template <int KIND, int HD, int NT>
 struct FewCfg {
     static constexpr uint32_t TILE = PgTile<KIND, HD>::BYTES;
     static constexpr uint32_t ROWS = 8u * NT;
-    static constexpr uint32_t CTAS = (TILE <= 4352u && NT * HD <= 256) ? 2u : 1u;
+    static constexpr uint32_t CTAS = (TILE <= 4352u && NT * HD <= 128) ? 2u : 1u;   /* 128 registers: more columns do not fit */
     static constexpr uint32_t WARPS = TILE > 8704u ? 4u : 8u;
-    static constexpr uint32_t DEPTH = TILE <= 2304u ? 4u : 3u;
+    static constexpr uint32_t FIT = 209000u / (CTAS * WARPS * TILE), DEPTH = FIT < 6u ? FIT : 6u;
     static constexpr uint32_t THREADS = WARPS * 32u;
     static constexpr uint32_t STEP = WARPS * 16u;            /* positions per step */
     static constexpr uint32_t EXTRA = 3u;                    /* steps that a piece costs besides its own */
@@ -92,9 +98,10 @@ struct FewCfg {
     static constexpr uint32_t Q_STRIDE = HD * 2u + 32u;      /* the four rows of a half-warp's 8-byte reads on different banks */
     static constexpr uint32_t RING = WARPS * DEPTH * TILE;
     static constexpr uint32_t REC = HD + 4u;
-    /* fragments of half of the warps on the way to the others, and the block's record, reuse the ring */
-    static constexpr uint32_t FRAG = (HD / 16u * 4u + 4u) * NT * 32u * 4u;
-    static_assert(WARPS / 2u * FRAG <= RING && ROWS * REC * 4u <= RING, "merge does not fit");
+    /* the warps' records reuse the ring: of all warps at once, or of half of them, which have taken over the others' fragments */
+    static constexpr uint32_t FRAG = (HD / 16u * 4u + 4u) * NT * 32u * 4u, PARTS = WARPS * ROWS * REC * 4u <= RING ? WARPS : WARPS / 2u;
+    static_assert(WARPS / 2u * FRAG <= RING && PARTS * ROWS * REC * 4u <= RING, "merge does not fit");
+    static constexpr uint32_t DIRECT = 16u;                  /* records that the unit's last block joins alone */
     static constexpr uint32_t SMEM = RING + ROWS * Q_STRIDE + WARPS * DEPTH * 8u + 1024u;
 };
 
@@ -105,7 +112,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t s_sum[WARPS];
     __shared__ uint64_t s_off, s_end2[2];
-    __shared__ uint32_t s_req;
+    __shared__ uint32_t s_req, s_last;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t s_base = (smem_u32(smem) + 1023u) & ~1023u;   /* swizzled tiles are anchored to multiples of 1024 */
     uint8_t *base = smem + (s_base - smem_u32(smem));
@@ -196,33 +203,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         const uint32_t kh = unit / groups, j0 = (unit - kh * groups) * P.tpg, n_here = min(P.tpg, R.add - j0);
         const uint32_t n_kv = R.held + j0 + n_here, live_rows = n_here * P.gqa, tok0 = R.tok0 + j0;
 
-        /* ---- the unit's queries as fp16 */
         __syncthreads();   /* the piece before has been read */
-        for (uint32_t i = tid; i < C::ROWS * (HD / 4u); i += C::THREADS) {
-            const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row < live_rows) {
-                const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
-                if (P.q_bf16) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + at);
-                    x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-                } else {
-                    x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(P.q) + at);
-                }
-            }
-            const uint32_t lo = h2u(__floats2half2_rn(x.x, x.y)), hi = h2u(__floats2half2_rn(x.z, x.w)), a = s_q + row * C::Q_STRIDE;
-            if (KIND == Q4K_Q8) {
-                /* lane t feeds dims 4 t .. 4 t + 3 of 16, as it gets the codes */
-                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a + d * 2u), "r"(lo), "r"(hi) : "memory");
-            } else {
-                /* lane t feeds dims 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of 16: one behind the other */
-                const uint32_t in = d & 15u, p = a + (d & ~15u) * 2u + (in & 7u) / 2u * 8u + (in >> 3) * 4u;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(lo) : "memory");
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p + 8u), "r"(hi) : "memory");
-            }
-        }
-        __syncthreads();
-
         /* positions that column 2 t + e of row tile i may see */
         uint32_t lim[NT][2], lim_min = n_kv;
 #pragma unroll
@@ -271,6 +252,33 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         };
         while (ahead < n_my && ahead < DEPTH) issue();
 
+        /* ---- the unit's queries as fp16, while the first tiles come in */
+        for (uint32_t i = tid; i < C::ROWS * (HD / 4u); i += C::THREADS) {
+            const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row < live_rows) {
+                const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
+                if (P.q_bf16) {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + at);
+                    x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+                } else {
+                    x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(P.q) + at);
+                }
+            }
+            const uint32_t lo = h2u(__floats2half2_rn(x.x, x.y)), hi = h2u(__floats2half2_rn(x.z, x.w)), a = s_q + row * C::Q_STRIDE;
+            if (KIND == Q4K_Q8) {
+                /* lane t feeds dims 4 t .. 4 t + 3 of 16, as it gets the codes */
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a + d * 2u), "r"(lo), "r"(hi) : "memory");
+            } else {
+                /* lane t feeds dims 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of 16: one behind the other */
+                const uint32_t in = d & 15u, p = a + (d & ~15u) * 2u + (in & 7u) / 2u * 8u + (in >> 3) * 4u;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(lo) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(p + 8u), "r"(hi) : "memory");
+            }
+        }
+        __syncthreads();
+
+
         float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int i = 0; i < NT; i++) {
@@ -279,159 +287,204 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
 #pragma unroll
             for (uint32_t k = 0; k < MT; k++) o[k][i][0] = o[k][i][1] = o[k][i][2] = o[k][i][3] = 0.f;
         }
-        for (uint32_t i = 0; i < n_my; i++) {
-            const uint32_t slot = taken % DEPTH, phase = (taken / DEPTH) & 1u, sb = ring + slot * TILE;
-            const uint32_t p0 = ((st + i) * WARPS + warp) * 16u;
-            taken++;
+        /* codes enter K Q^T raised by 1152: the product starts from -1152 times the sum of the queries over the block (exact
+         * codes to fp32 sums; two subtractions per word less).  More columns take the subtractions. */
+        constexpr bool RAISED = KIND == Q4K_Q8 && NT == 1;
+        float below[RAISED ? HD / 32 : 1][2];
+        if constexpr (RAISED) {
+#pragma unroll
+            for (uint32_t b = 0; b < HD / 32u; b++)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; e++) {
+                    /* lane (g, t) sums dims 4 g .. 4 g + 3 of column 2 t + e, the eight lanes of a column then one another's */
+                    const uint2 w = lds64(s_q + (2u * t + e) * C::Q_STRIDE + b * 64u + g * 8u);
+                    const float2 f0 = __half22float2(u2h(w.x)), f1 = __half22float2(u2h(w.y));
+                    float x = (f0.x + f0.y) + (f1.x + f1.y);
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    below[b][e] = -1152.f * x;
+                }
+        }
+        const uint32_t mrow = (lane & 7u) + ((lane >> 3) & 1u) * 8u, mchunk = lane >> 4;   /* of ldmatrix: the row and 16-byte piece this lane addresses */
+        uint32_t slot = taken % DEPTH, phase = (taken / DEPTH) & 1u;                       /* of the next tile to wait for */
+        auto landed = [&]() -> uint32_t {   /* waits for it, and goes on */
+            const uint32_t sb = ring + slot * TILE;
             for (uint32_t spin = 0; !bar_test(bars + 8u * slot, phase); spin++)
                 if (spin >= PG_SPIN_LIMIT) { ok = false; break; }
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const bool gone = (dead >> (i & 31u)) & 1u;
-            if ((i & 31u) == 31u) dead = dead_nxt;
-            if (!gone) {
-                /* ---- scores: c0, c1 of position g, c2, c3 of position g + 8, columns 2 t and 2 t + 1 */
-                float sc[NT][4];
+            if (++slot == DEPTH) { slot = 0u; phase ^= 1u; }
+            taken++;
+            return sb;
+        };
+        /* scores of the tile at sb: c0, c1 of position g, c2, c3 of position g + 8, columns 2 t and 2 t + 1 */
+        auto scores = [&](uint32_t sb, float (&sc)[NT][4]) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-                const uint32_t mrow = (lane & 7u) + ((lane >> 3) & 1u) * 8u, mchunk = lane >> 4;   /* of ldmatrix: the row and 16-byte piece this lane addresses */
-                if constexpr (KIND == Q4K_Q8) {
-                    constexpr uint32_t NB = HD / 32u;
-                    uint32_t k0[NB / 2], k1[NB / 2];   /* K scales of positions g and g + 8 */
-                    const uint32_t ka = sb + g * C::TILE / 16u + 2u * HD, kb = ka + 8u * (C::TILE / 16u);
+            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            if constexpr (KIND == Q4K_Q8) {
+                constexpr uint32_t NB = HD / 32u;
+                uint32_t k0[NB / 2], k1[NB / 2];   /* K scales of positions g and g + 8 */
+                const uint32_t ka = sb + g * (TILE / 16u) + 2u * HD, kb = ka + 8u * (TILE / 16u);
 #pragma unroll
-                    for (uint32_t b = 0; b < NB / 2; b++) { k0[b] = lds32(ka + 4u * b); k1[b] = lds32(kb + 4u * b); }
+                for (uint32_t b = 0; b < NB / 2; b++) { k0[b] = lds32(ka + 4u * b); k1[b] = lds32(kb + 4u * b); }
 #pragma unroll
-                    for (uint32_t b = 0; b < NB; b++) {
-                        uint32_t w[4], a0[4], a1[4];
-                        ldmatrix_x4(w, sb + mrow * (TILE / 16u) + (2u * b + mchunk) * 16u);
+                for (uint32_t b = 0; b < NB; b++) {
+                    uint32_t w[4], a0[4], a1[4];
+                    ldmatrix_x4(w, sb + mrow * (TILE / 16u) + (2u * b + mchunk) * 16u);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
+                    for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
+                    if constexpr (RAISED) {
+                        a0[0] = raised2<0x4140>(w[0]); a0[2] = raised2<0x4342>(w[0]); a0[1] = raised2<0x4140>(w[1]); a0[3] = raised2<0x4342>(w[1]);
+                        a1[0] = raised2<0x4140>(w[2]); a1[2] = raised2<0x4342>(w[2]); a1[1] = raised2<0x4140>(w[3]); a1[3] = raised2<0x4342>(w[3]);
+                    } else {
                         a0[0] = codes2<0x4140>(w[0]); a0[2] = codes2<0x4342>(w[0]); a0[1] = codes2<0x4140>(w[1]); a0[3] = codes2<0x4342>(w[1]);
                         a1[0] = codes2<0x4140>(w[2]); a1[2] = codes2<0x4342>(w[2]); a1[1] = codes2<0x4140>(w[3]); a1[3] = codes2<0x4342>(w[3]);
-                        const float2 f0 = __half22float2(u2h(k0[b / 2])), f1 = __half22float2(u2h(k1[b / 2]));
-                        const float e0 = b & 1u ? f0.y : f0.x, e1 = b & 1u ? f1.y : f1.x;
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const uint32_t qa = s_q + (8u * n + g) * C::Q_STRIDE + b * 64u + t * 8u;
-                            const uint2 qx = lds64(qa), qy = lds64(qa + 32u);
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma16816(c, a0, qx.x, qx.y);
-                            mma16816(c, a1, qy.x, qy.y);
-                            sc[n][0] = fmaf(c[0], e0, sc[n][0]); sc[n][1] = fmaf(c[1], e0, sc[n][1]);
-                            sc[n][2] = fmaf(c[2], e1, sc[n][2]); sc[n][3] = fmaf(c[3], e1, sc[n][3]);
-                        }
                     }
-                } else {
+                    const float2 f0 = __half22float2(u2h(k0[b / 2])), f1 = __half22float2(u2h(k1[b / 2]));
+                    const float e0 = b & 1u ? f0.y : f0.x, e1 = b & 1u ? f1.y : f1.x;
 #pragma unroll
-                    for (uint32_t ks = 0; ks < MT; ks++) {
-                        uint32_t a[4];
-                        const uint32_t c = 2u * ks + mchunk;
-                        ldmatrix_x4(a, sb + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const uint2 qx = lds64(s_q + (8u * n + g) * C::Q_STRIDE + ks * 32u + t * 8u);
-                            mma16816(sc[n], a, qx.x, qx.y);
-                        }
+                    for (int n = 0; n < NT; n++) {
+                        const uint32_t qa = s_q + (8u * n + g) * C::Q_STRIDE + b * 64u + t * 8u;
+                        const uint2 qx = lds64(qa), qy = lds64(qa + 32u);
+                        float c[4];
+                        if constexpr (RAISED) mma16816_from(c, a0, qx.x, qx.y, below[b][0], below[b][1]);
+                        else mma16816_from(c, a0, qx.x, qx.y, 0.f, 0.f);
+                        mma16816(c, a1, qy.x, qy.y);
+                        sc[n][0] = fmaf(c[0], e0, sc[n][0]); sc[n][1] = fmaf(c[1], e0, sc[n][1]);
+                        sc[n][2] = fmaf(c[2], e1, sc[n][2]); sc[n][3] = fmaf(c[3], e1, sc[n][3]);
                     }
                 }
+            } else {
+#pragma unroll
+                for (uint32_t ks = 0; ks < MT; ks++) {
+                    uint32_t a[4];
+                    const uint32_t c = 2u * ks + mchunk;
+                    ldmatrix_x4(a, sb + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint2 qx = lds64(s_q + (8u * n + g) * C::Q_STRIDE + ks * 32u + t * 8u);
+                        mma16816(sc[n], a, qx.x, qx.y);
+                    }
+                }
+            }
+        };
+        /* Tile i at sb, whose scores are in sc.  The scores of the next one are computed beside its P V: neither needs the other, and a
+         * warp's chain of one tile alone (4000 cycles) left a third of the issue slots empty. */
+        float sc[NT][4];
+        uint32_t sb = 0;
+        auto step = [&](uint32_t i, auto more) {
+            const uint32_t p0 = ((st + i) * WARPS + warp) * 16u;
+            uint32_t sb_next = 0;
+            if constexpr (decltype(more)::value) {
+                sb_next = landed();
+                if (!ok) return;
+            }
+            const bool gone = (dead >> (i & 31u)) & 1u;   /* its page is not the pool's: all masked */
+            if ((i & 31u) == 31u) dead = dead_nxt;
+            const bool tail = p0 + 16u > n_kv || gone;
+            if (p0 + 16u > lim_min || gone) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) sc[n][k] *= P.scale_log2e;
-                if (p0 + 16u > lim_min) {
+                    for (int k = 0; k < 4; k++)
+                        if (gone || p0 + g + (k >> 1) * 8u >= lim[n][k & 1]) sc[n][k] = -CUDART_INF_F;
+            }
+            /* the maxima (of scores times scale_log2e) move only where a score is above them: seldom, after the first tiles */
+            bool grow = false;
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            if (p0 + g + (k >> 1) * 8u >= lim[n][k & 1]) sc[n][k] = -CUDART_INF_F;
-                }
-                /* ---- the maxima move only where a score is above them: seldom, after the first tiles */
-                bool grow = false;
+                for (int k = 0; k < 4; k++) sc[n][k] *= P.scale_log2e;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) grow = grow || fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e];
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) grow = grow || fmaxf(sc[n][e], sc[n][e + 2]) > m[n][e];
-                if (__any_sync(0xffffffffu, grow)) {
+                    for (int e = 0; e < 2; e++) {
+                        float x = fmaxf(sc[n][e], sc[n][e + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        if (x > m[n][e]) {
+                            const float f = ex2(m[n][e] - x);
+                            m[n][e] = x;
+                            l[n][e] *= f;
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float x = fmaxf(sc[n][e], sc[n][e + 2]);
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            if (x > m[n][e]) {
-                                const float f = ex2(m[n][e] - x);
-                                m[n][e] = x;
-                                l[n][e] *= f;
-#pragma unroll
-                                for (uint32_t k = 0; k < MT; k++) { o[k][n][e] *= f; o[k][n][e + 2] *= f; }
-                            }
-                        }
-                }
-                uint32_t pb[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float m0 = m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m1 = m[n][1] == -CUDART_INF_F ? 0.f : m[n][1];
-                    const float x0 = ex2(sc[n][0] - m0), x1 = ex2(sc[n][1] - m1), x2 = ex2(sc[n][2] - m0), x3 = ex2(sc[n][3] - m1);
-                    l[n][0] += x0 + x2;
-                    l[n][1] += x1 + x3;
-                    pb[n][0] = movmatrix_t(h2u(__floats2half2_rn(x0, x1)));
-                    pb[n][1] = movmatrix_t(h2u(__floats2half2_rn(x2, x3)));
-                }
-                /* ---- O^T += V^T P^T.  Rows behind the last position hold anything: 0 x NaN has to stay 0 */
-                const bool tail = p0 + 16u > n_kv;
-                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                if (tail) {
-                    const uint32_t p = p0 + 2u * t;
-                    keep0 = (p < n_kv ? 0xffffu : 0u) | (p + 1u < n_kv ? 0xffff0000u : 0u);
-                    keep1 = (p + 8u < n_kv ? 0xffffu : 0u) | (p + 9u < n_kv ? 0xffff0000u : 0u);
-                }
-                if constexpr (KIND == Q4K_Q8) {
-                    constexpr uint32_t NB = HD / 32u;
-                    uint32_t v0[NB / 2], v1[NB / 2], v2[NB / 2], v3[NB / 2];   /* V scales of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9 */
-                    const uint32_t va = sb + 2u * t * (TILE / 16u) + 2u * HD + NB * 2u;
-#pragma unroll
-                    for (uint32_t b = 0; b < NB / 2; b++) {
-                        v0[b] = lds32(va + 4u * b); v1[b] = lds32(va + TILE / 16u + 4u * b);
-                        v2[b] = lds32(va + 8u * (TILE / 16u) + 4u * b); v3[b] = lds32(va + 9u * (TILE / 16u) + 4u * b);
-                    }
-#pragma unroll
-                    for (uint32_t b = 0; b < NB; b++) {
-                        const uint32_t sel = b & 1u ? 0x7632u : 0x5410u;
-                        const __half2 f0 = u2h(__byte_perm(v0[b / 2], v1[b / 2], sel) & keep0), f1 = u2h(__byte_perm(v2[b / 2], v3[b / 2], sel) & keep1);
-                        uint32_t w[4];
-                        ldmatrix_x4_trans(w, sb + mrow * (TILE / 16u) + HD + (2u * b + mchunk) * 16u);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
-#pragma unroll
-                        for (uint32_t c = 0; c < 2; c++) {
-                            /* dims 2 g (rows g) and 2 g + 1 (rows g + 8) of 16; fp16(code x scale): 2^-12 of a value on average, as P is rounded */
-                            uint32_t a[4] = {h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c])), f0)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c])), f0)),
-                                             h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c + 1])), f1)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c + 1])), f1))};
-#pragma unroll
-                            for (int n = 0; n < NT; n++) mma16816(o[2 * b + c][n], a, pb[n][0], pb[n][1]);
+                            for (uint32_t k = 0; k < MT; k++) { o[k][n][e] *= f; o[k][n][e + 2] *= f; }
                         }
                     }
-                } else {
+            }
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;   /* rows behind the last position hold anything: 0 x NaN has to stay 0 */
+            if (tail) {
+                const uint32_t p = p0 + 2u * t, end = gone ? 0u : n_kv;
+                keep0 = (p < end ? 0xffffu : 0u) | (p + 1u < end ? 0xffff0000u : 0u);
+                keep1 = (p + 8u < end ? 0xffffu : 0u) | (p + 9u < end ? 0xffff0000u : 0u);
+            }
+            uint32_t pb[NT][2];
 #pragma unroll
-                    for (uint32_t k = 0; k < MT; k++) {
-                        uint32_t w[4];
-                        const uint32_t c = 2u * k + mchunk;
-                        ldmatrix_x4_trans(w, sb + TILE / 2u + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
-                        uint32_t a[4] = {w[0], w[2], w[1], w[3]};
-                        if (tail) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
+            for (int n = 0; n < NT; n++) {
+                const float m0 = m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m1 = m[n][1] == -CUDART_INF_F ? 0.f : m[n][1];
+                const float x0 = ex2(sc[n][0] - m0), x1 = ex2(sc[n][1] - m1), x2 = ex2(sc[n][2] - m0), x3 = ex2(sc[n][3] - m1);
+                l[n][0] += x0 + x2;
+                l[n][1] += x1 + x3;
+                pb[n][0] = movmatrix_t(h2u(__floats2half2_rn(x0, x1)));
+                pb[n][1] = movmatrix_t(h2u(__floats2half2_rn(x2, x3)));
+            }
+            if constexpr (decltype(more)::value) scores(sb_next, sc);
+            /* ---- O^T += V^T P^T */
+            if constexpr (KIND == Q4K_Q8) {
+                constexpr uint32_t NB = HD / 32u;
+                uint32_t v0[NB / 2], v1[NB / 2], v2[NB / 2], v3[NB / 2];   /* V scales of positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9 */
+                const uint32_t va = sb + 2u * t * (TILE / 16u) + 2u * HD + NB * 2u;
 #pragma unroll
-                        for (int n = 0; n < NT; n++) mma16816(o[k][n], a, pb[n][0], pb[n][1]);
+                for (uint32_t b = 0; b < NB / 2; b++) {
+                    v0[b] = lds32(va + 4u * b); v1[b] = lds32(va + TILE / 16u + 4u * b);
+                    v2[b] = lds32(va + 8u * (TILE / 16u) + 4u * b); v3[b] = lds32(va + 9u * (TILE / 16u) + 4u * b);
+                }
+#pragma unroll
+                for (uint32_t b = 0; b < NB; b++) {
+                    const uint32_t sel = b & 1u ? 0x7632u : 0x5410u;
+                    const __half2 f0 = u2h(__byte_perm(v0[b / 2], v1[b / 2], sel) & keep0), f1 = u2h(__byte_perm(v2[b / 2], v3[b / 2], sel) & keep1);
+                    uint32_t w[4];
+                    ldmatrix_x4_trans(w, sb + mrow * (TILE / 16u) + HD + (2u * b + mchunk) * 16u);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] ^= 0x80808080u;
+#pragma unroll
+                    for (uint32_t c = 0; c < 2; c++) {
+                        /* dims 2 g (rows g) and 2 g + 1 (rows g + 8) of 16; fp16(code x scale): 2^-12 of a value on average, as P is rounded */
+                        uint32_t a[4] = {h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c])), f0)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c])), f0)),
+                                         h2u(__hmul2(u2h(codes2<0x4240>(w[2 * c + 1])), f1)), h2u(__hmul2(u2h(codes2<0x4341>(w[2 * c + 1])), f1))};
+#pragma unroll
+                        for (int n = 0; n < NT; n++) mma16816(o[2 * b + c][n], a, pb[n][0], pb[n][1]);
                     }
+                }
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < MT; k++) {
+                    uint32_t w[4];
+                    const uint32_t c = 2u * k + mchunk;
+                    ldmatrix_x4_trans(w, sb + TILE / 2u + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
+                    uint32_t a[4] = {w[0], w[2], w[1], w[3]};
+                    if (tail) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma16816(o[k][n], a, pb[n][0], pb[n][1]);
                 }
             }
             __syncwarp();   /* all lanes have read the slot */
             if (ahead < n_my) issue();
+            sb = sb_next;
+        };
+        if (n_my) {
+            sb = landed();
+            if (ok) scores(sb, sc);
+            for (uint32_t i = 0; ok && i + 1u < n_my; i++) step(i, std::true_type());
+            if (ok) step(n_my - 1u, std::false_type());
         }
 
-        /* ---- the warps' results are joined in pairs through shared memory (the rings are empty: all that was issued was taken) */
+        /* ---- the warps' results are joined through shared memory (the rings are empty: all that was issued was taken) */
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -441,10 +494,10 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                 l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
             }
         float *xch = reinterpret_cast<float *>(base);
-#pragma unroll 1
-        for (uint32_t half = WARPS / 2u; half > 0; half >>= 1) {
+        if constexpr (C::PARTS < WARPS) {
+            constexpr uint32_t half = WARPS / 2u;
             __syncthreads();
-            if (warp >= half && warp < 2u * half) {
+            if (warp >= half) {
                 float *to = xch + (warp - half) * (C::FRAG / 4u) + lane;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
@@ -477,36 +530,95 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
             }
         }
         __syncthreads();
-        if (warp == 0) {   /* [row][hd + 4]: acc, m, l */
+        if (warp < C::PARTS) {   /* [warp][row][hd + 4]: acc, m, l */
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float *rec = xch + (8u * n + 2u * t + e) * C::REC;
+                    float *rec = xch + (warp * C::ROWS + 8u * n + 2u * t + e) * C::REC;
 #pragma unroll
                     for (uint32_t k = 0; k < MT; k++) {
-                        rec[16u * k + (KIND == Q4K_Q8 ? 2u * g : g)] = o[k][n][e];
-                        rec[16u * k + (KIND == Q4K_Q8 ? 2u * g + 1u : g + 8u)] = o[k][n][e + 2];
+                        if (KIND == Q4K_Q8) {
+                            *reinterpret_cast<float2 *>(rec + 16u * k + 2u * g) = make_float2(o[k][n][e], o[k][n][e + 2]);
+                        } else {
+                            rec[16u * k + g] = o[k][n][e];
+                            rec[16u * k + g + 8u] = o[k][n][e + 2];
+                        }
                     }
-                    if (g == 0) { rec[HD] = m[n][e]; rec[HD + 1] = l[n][e]; }
+                    if (g == 0) *reinterpret_cast<float2 *>(rec + HD) = make_float2(m[n][e], l[n][e]);
                 }
         }
         __syncthreads();
         const bool whole = st == 0u && here == n_steps;
+        const uint32_t first = whole ? 0u : shares.first(s - at, s - at + steps), last = whole ? 0u : shares.last(s - at, s - at + steps), n_recs = last - first + 1u;
+        float M, L;
+        float4 A;
+        auto join = [&](float m1, float l1, float4 x) {
+            const float Mn = fmaxf(M, m1), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m1 - Mu);
+            M = Mn;
+            L = L * fa + l1 * fb;
+            A.x = A.x * fa + x.x * fb; A.y = A.y * fa + x.y * fb; A.z = A.z * fa + x.z * fb; A.w = A.w * fa + x.w * fb;
+        };
+        auto gate_of = [&](uint32_t row, uint32_t d) -> const float * {
+            return P.gate ? P.gate + ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d : nullptr;
+        };
         float *part = P.part + ((size_t)blockIdx.x * 2u + (st == 0u ? 1u : 0u)) * C::ROWS * C::REC;
         for (uint32_t i = tid; i < live_rows * (HD / 4u); i += C::THREADS) {
             const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
             const float *rec = xch + row * C::REC;
-            const float4 x = *reinterpret_cast<const float4 *>(rec + d);
-            const float L = rec[HD + 1];
+            const float2 ml0 = *reinterpret_cast<const float2 *>(rec + HD);
+            M = ml0.x; L = ml0.y;
+            A = *reinterpret_cast<const float4 *>(rec + d);
+#pragma unroll
+            for (uint32_t w = 1; w < C::PARTS; w++) {
+                const float *r2 = rec + w * (C::ROWS * C::REC);
+                const float2 ml = *reinterpret_cast<const float2 *>(r2 + HD);
+                join(ml.x, ml.y, *reinterpret_cast<const float4 *>(r2 + d));
+            }
             if (whole) {
-                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, x, L, P.gate ? P.gate + ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d : nullptr);
+                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
             } else {
-                *reinterpret_cast<float4 *>(part + row * C::REC + d) = x;
-                if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(rec[HD], L);
+                *reinterpret_cast<float4 *>(part + row * C::REC + d) = A;
+                if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(M, L);
             }
         }
-        if (!whole) split[st == 0u] = {shares.first(s - at, s - at + steps), shares.last(s - at, s - at + steps), tok0, n_here, kh};
+        if (!whole) {
+            if (n_recs <= C::DIRECT) {   /* few records: the block that comes last joins them, the others go on */
+                __syncthreads();
+                if (tid == 0) {
+                    __threadfence();
+                    s_last = atomicAdd(P.meet + 2u * first, 1u) == n_recs - 1u;
+                    if (s_last) P.meet[2u * first] = 0u;
+                }
+                __syncthreads();
+                if (s_last) {
+                    __threadfence();
+                    for (uint32_t i = tid; i < live_rows * (HD / 4u); i += C::THREADS) {
+                        const uint32_t row = i / (HD / 4u), d = i % (HD / 4u) * 4u;
+                        constexpr uint32_t BATCH = 4u;
+                        M = -CUDART_INF_F; L = 0.f;
+                        A = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (uint32_t c0 = first; c0 <= last; c0 += BATCH) {
+                            float2 ml[BATCH];
+                            float4 x[BATCH];
+#pragma unroll
+                            for (uint32_t b = 0; b < BATCH; b++) {
+                                const uint32_t c = min(c0 + b, last);
+                                const float *rec = P.part + (((size_t)c * 2u + (c == first ? 1u : 0u)) * C::ROWS + row) * C::REC;
+                                ml[b] = __ldcg(reinterpret_cast<const float2 *>(rec + HD));
+                                x[b] = __ldcg(reinterpret_cast<const float4 *>(rec + d));
+                            }
+#pragma unroll
+                            for (uint32_t b = 0; b < BATCH; b++)
+                                if (c0 + b <= last) join(ml[b].x, ml[b].y, x[b]);
+                        }
+                        pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
+                    }
+                }
+            } else {
+                split[st == 0u] = {first, last, tok0, n_here, kh};
+            }
+        }
         s += take;
         off += take;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   /* the next bulk copies overwrite what was stored here */
@@ -516,8 +628,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         pg_arrive(P, split[0]);
         pg_arrive(P, split[1]);
     }
-    for (uint32_t i = 0; i < 2u; i++)
-        if (i == 0u || split[1].last - split[1].first <= 2u) pg_join<HD, C::THREADS>(P, split[i], C::ROWS, base, C::RING, s_q + C::ROWS * C::Q_STRIDE + WARPS * DEPTH * 8u);
+    pg_join<HD, C::THREADS>(P, split[0], C::ROWS, base, C::RING, s_q + C::ROWS * C::Q_STRIDE + WARPS * DEPTH * 8u);
     if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
         if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
         for (; taken < issued; taken++)

@@ -53,7 +53,7 @@ struct ChunkCfg {
     /* A piece takes 7.7 us (hd 256: 8.7) besides its tiles (queries in, the first scores, outputs out), a tile 2.2 (hd 256: 1.4 in fp16, 3.2
      * in q8_0): a unit counts as EXTRA more steps when the work is shared out.  Only tiles are walked.  512 tokens over 16 001 rows
      * 109 us with EXTRA 2, 98 with 3. */
-    static constexpr uint32_t EXTRA = HD == 256 ? (KIND == Q4K_Q8 ? 3u : 6u) : KIND == Q4K_Q8 ? 3u : 4u;
+    static constexpr uint32_t EXTRA = HD == 256 && KIND == Q4K_F16 ? 6u : 3u;
     using Shares = PgShares<EXTRA, HD == 256 ? 4u * EXTRA : 16u, EXTRA + 2u>;
     /* registers of a thread: the block's 512 x 128 are 256 threads x (softmax + the others) */
     static constexpr uint32_t R_SOFTMAX = 168u, R_OTHERS = 88u;
