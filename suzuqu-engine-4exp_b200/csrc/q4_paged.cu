@@ -93,8 +93,7 @@ struct FewCfg {
     static constexpr uint32_t FIT = 209000u / (CTAS * WARPS * TILE), DEPTH = FIT < 6u ? FIT : 6u;
     static constexpr uint32_t THREADS = WARPS * 32u;
     static constexpr uint32_t STEP = WARPS * 16u;            /* positions per step */
-    static constexpr uint32_t EXTRA = 3u;                    /* steps that a piece costs besides its own */
-    using Shares = PgShares<EXTRA, 8u, 4u>;
+    static constexpr uint32_t EXTRA = 3u;                    /* steps that a piece costs besides its own, where blocks have several */
     static constexpr uint32_t Q_STRIDE = HD * 2u + 32u;      /* the four rows of a half-warp's 8-byte reads on different banks */
     static constexpr uint32_t RING = WARPS * DEPTH * TILE;
     static constexpr uint32_t REC = HD + 4u;
@@ -108,10 +107,12 @@ struct FewCfg {
 template <int KIND, int HD, int NT>
 __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD, NT>::CTAS) q4_pg_few_k(const PagedParams P) {
     using C = FewCfg<KIND, HD, NT>;
-    constexpr uint32_t TILE = C::TILE, WARPS = C::WARPS, DEPTH = C::DEPTH, STEP = C::STEP, EXTRA = C::EXTRA, MT = HD / 16u;
+    constexpr uint32_t TILE = C::TILE, WARPS = C::WARPS, DEPTH = C::DEPTH, STEP = C::STEP, MT = HD / 16u;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t s_sum[WARPS];
+    __shared__ uint64_t s_sum[2u * WARPS];
     __shared__ uint64_t s_off, s_end2[2];
+    __shared__ PgShares s_shares;   /* what only the ends of pieces need is kept here: registers are short in the loop between */
+    __shared__ PgSplit s_split[2];  /* units that began before this block; that go on behind it */
     __shared__ uint32_t s_req, s_last;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t s_base = (smem_u32(smem) + 1023u) & ~1023u;   /* swizzled tiles are anchored to multiples of 1024 */
@@ -128,49 +129,62 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         if (q.add > P.add_split) q.add = 0u;
         return q;
     };
-    auto steps_of = [&](uint32_t r, bool &bad) -> uint64_t {
-        const PgReq q = mine_of(r, bad);
-        return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh * ((q.held + q.add + STEP - 1u) / STEP + EXTRA);   /* no tokens: 0 groups */
-    };
     const uint32_t per = (P.n_req + C::THREADS - 1u) / C::THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
-    uint64_t mine = 0, total = 0, before = 0;
+    uint64_t mine = 0, units = 0, total, all_units, before, units_before;
     bool bad, any_bad = false;
+    PgReq mine_is = {0u, 0u, 0u};
+    auto units_of = [&](const PgReq &q) -> uint64_t { return (uint64_t)((q.add + P.tpg - 1u) / P.tpg) * P.n_kvh; };   /* no tokens: none */
+    auto steps_in = [&](const PgReq &q) -> uint32_t { return (q.held + q.add + STEP - 1u) / STEP; };
     for (uint32_t r = r0; r < r1; r++) {
-        mine += steps_of(r, bad);
+        mine_is = mine_of(r, bad);
+        units += units_of(mine_is);
+        mine += units_of(mine_is) * steps_in(mine_is);
         any_bad |= bad;
     }
     {
-        uint64_t x = mine;
+        uint64_t x = mine, y = units;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= (uint32_t)d) x += y;
+            const uint64_t u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+            if (lane >= (uint32_t)d) { x += u; y += v; }
         }
-        if (lane == 31u) s_sum[warp] = x;
+        if (lane == 31u) { s_sum[warp] = x; s_sum[WARPS + warp] = y; }
         __syncthreads();
+        total = all_units = before = units_before = 0;
 #pragma unroll
         for (uint32_t w = 0; w < WARPS; w++) {
-            if (w < warp) before += s_sum[w];
+            if (w < warp) { before += s_sum[w]; units_before += s_sum[WARPS + w]; }
             total += s_sum[w];
+            all_units += s_sum[WARPS + w];
         }
         before += x - mine;
+        units_before += y - units;
     }
+    /* Where the blocks have many steps each, a unit counts as EXTRA more, that a piece costs, and short ones stay whole (a token of 64
+     * sessions 116 -> 113 us).  Where they have few, the way through the launch counts: units are cut as finely as there are
+     * blocks, down to one step (a token of four short chats 13.4 us whole, 11.5 so). */
+    const uint32_t extra = total >= 4u * gridDim.x ? C::EXTRA : 0u;   /* also shares.near */
+    total += all_units * extra; before += units_before * extra; mine += units * extra;
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-    typename C::Shares shares;
-    shares.set(total);
+    PgShares shares;
+    shares.set(total, extra, extra ? 8u : 0u, extra ? 4u : 1u);
     if (blockIdx.x >= shares.blocks) return;
-    if (tid == 0) s_end2[0] = s_end2[1] = total;
+    if (tid == 0) {
+        s_end2[0] = s_end2[1] = total;
+        s_shares = shares;
+        s_split[0] = s_split[1] = {1u, 0u, 0u, 0u, 0u};
+    }
     __syncthreads();
     for (uint32_t i = 0; i < 2u && mine && blockIdx.x + i < shares.blocks; i++) {   /* the two cuts */
         const uint64_t x = shares.cut(blockIdx.x + i);
         if (x < before || x >= before + mine) continue;
         uint64_t at = before;
         for (uint32_t r = r0; r < r1; r++) {
-            const PgReq q = mine_of(r, bad);
-            const uint32_t steps = (q.held + q.add + STEP - 1u) / STEP + EXTRA;
-            const uint64_t n = steps_of(r, bad);
+            if (per > 1u) mine_is = mine_of(r, bad);
+            const uint32_t steps = steps_in(mine_is) + extra;
+            const uint64_t n = units_of(mine_is) * steps;
             if (x < at + n) {
-                const uint64_t in = x - at, u0 = in >> 32 ? in / steps * steps : (uint32_t)in / steps * steps, to = u0 + C::Shares::snap(in - u0, steps);
+                const uint64_t in = x - at, u0 = in >> 32 ? in / steps * steps : (uint32_t)in / steps * steps, to = u0 + shares.snap(in - u0, steps);
                 if (i == 0u) {
                     s_req = r;
                     s_off = to;
@@ -184,22 +198,20 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     __syncthreads();
     uint32_t req = s_req, issued = 0, taken = 0;   /* of the warp's ring, over all pieces */
     uint64_t off = s_off, s = s_end2[0];
-    const uint64_t s_end = s_end2[1];
-    PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* units that began before this block; that go on behind it */
     bool ok = true;
 
     /* ---- pieces of units */
-    while (s < s_end) {
+    while (s < s_end2[1]) {
         const PgReq R = mine_of(req, bad);
-        const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = (R.held + R.add + STEP - 1u) / STEP, steps = n_steps + EXTRA;
+        const uint32_t groups = (R.add + P.tpg - 1u) / P.tpg, n_steps = steps_in(R), extra = s_shares.near, steps = n_steps + extra;
         if (off >= (uint64_t)groups * P.n_kvh * steps) {   /* on to the next request; requests without tokens are passed over */
             off -= (uint64_t)groups * P.n_kvh * steps;
             req++;
             continue;
         }
         const uint32_t unit = off >> 32 ? (uint32_t)(off / steps) : (uint32_t)off / steps, at = (uint32_t)(off - (uint64_t)unit * steps);
-        const uint32_t take = (uint32_t)min((uint64_t)(steps - at), s_end - s);
-        const uint32_t st = max(at, EXTRA) - EXTRA, here = max(at + take, EXTRA) - EXTRA - st;   /* the first EXTRA steps are none */
+        const uint32_t take = (uint32_t)min((uint64_t)(steps - at), s_end2[1] - s);
+        const uint32_t st = max(at, extra) - extra, here = max(at + take, extra) - extra - st;   /* the first `extra` steps are none */
         const uint32_t kh = unit / groups, j0 = (unit - kh * groups) * P.tpg, n_here = min(P.tpg, R.add - j0);
         const uint32_t n_kv = R.held + j0 + n_here, live_rows = n_here * P.gqa, tok0 = R.tok0 + j0;
 
@@ -550,7 +562,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         }
         __syncthreads();
         const bool whole = st == 0u && here == n_steps;
-        const uint32_t first = whole ? 0u : shares.first(s - at, s - at + steps), last = whole ? 0u : shares.last(s - at, s - at + steps), n_recs = last - first + 1u;
+        const uint32_t first = whole ? 0u : s_shares.first(s - at, s - at + steps), last = whole ? 0u : s_shares.last(s - at, s - at + steps), n_recs = last - first + 1u;
         float M, L;
         float4 A;
         auto join = [&](float m1, float l1, float4 x) {
@@ -615,20 +627,73 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                         pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
                     }
                 }
-            } else {
-                split[st == 0u] = {first, last, tok0, n_here, kh};
+            } else if (tid == 0) {
+                s_split[st == 0u] = {first, last, tok0, n_here, kh};
             }
         }
         s += take;
         off += take;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   /* the next bulk copies overwrite what was stored here */
     }
+    /* ---- units of many records: their blocks meet, and each joins slices of 32 dims of a row: eight lanes to a slice, the records
+     * shared out over the block's groups of eight lanes.  (All of a row by one block: 2 us more.) */
     __syncthreads();
     if (tid == 0) {
-        pg_arrive(P, split[0]);
-        pg_arrive(P, split[1]);
+        pg_arrive(P, s_split[0]);
+        pg_arrive(P, s_split[1]);
     }
-    pg_join<HD, C::THREADS>(P, split[0], C::ROWS, base, C::RING, s_q + C::ROWS * C::Q_STRIDE + WARPS * DEPTH * 8u);
+    if (s_split[0].last >= s_split[0].first) {
+        const PgSplit u = s_split[0];
+        const uint32_t k = u.last - u.first + 1u, joiners = k - 1u, mine_no = blockIdx.x - u.first - 1u;   /* all but the first, which has another's end */
+        constexpr uint32_t GROUPS = C::THREADS / 8u, BATCH = 5u;
+        float4 *s_a = reinterpret_cast<float4 *>(base);
+        float2 *s_ml = reinterpret_cast<float2 *>(base + C::THREADS * 16u);
+        const uint32_t slices = u.n_here * P.gqa * (HD / 32u), per_joiner = (slices + joiners - 1u) / joiners, x0 = min(mine_no * per_joiner, slices), x1 = min(x0 + per_joiner, slices);
+        if (x0 < x1) pg_wait(P, u, k);
+        for (uint32_t x = x0; x < x1; x++) {
+            const uint32_t row = x / (HD / 32u), d = x % (HD / 32u) * 32u + (lane & 7u) * 4u, group = tid >> 3;
+            const float *gate = P.gate ? P.gate + ((size_t)(u.tok0 + row / P.gqa) * P.n_head + u.kh * P.gqa + row % P.gqa) * HD + d : nullptr;
+            float M = -CUDART_INF_F, L = 0.f;
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto join = [&](float m1, float l1, float4 v) {
+                const float Mn = fmaxf(M, m1), Mu = Mn == -CUDART_INF_F ? 0.f : Mn, fa = ex2(M - Mu), fb = ex2(m1 - Mu);
+                M = Mn;
+                L = L * fa + l1 * fb;
+                A.x = A.x * fa + v.x * fb; A.y = A.y * fa + v.y * fb; A.z = A.z * fa + v.z * fb; A.w = A.w * fa + v.w * fb;
+            };
+            for (uint32_t c0 = u.first + group; c0 <= u.last; c0 += GROUPS * BATCH) {
+                float2 ml[BATCH];
+                float4 v[BATCH];
+#pragma unroll
+                for (uint32_t b = 0; b < BATCH; b++) {
+                    const uint32_t c = min(c0 + b * GROUPS, u.last);
+                    const float *rec = P.part + (((size_t)c * 2u + (c == u.first ? 1u : 0u)) * C::ROWS + row) * C::REC;
+                    ml[b] = __ldcg(reinterpret_cast<const float2 *>(rec + HD));
+                    v[b] = __ldcg(reinterpret_cast<const float4 *>(rec + d));
+                }
+#pragma unroll
+                for (uint32_t b = 0; b < BATCH; b++)
+                    if (c0 + b * GROUPS <= u.last) join(ml[b].x, ml[b].y, v[b]);
+            }
+#pragma unroll
+            for (int o2 = 8; o2 < 32; o2 <<= 1) {
+                const float m1 = __shfl_xor_sync(0xffffffffu, M, o2), l1 = __shfl_xor_sync(0xffffffffu, L, o2);
+                const float4 v = make_float4(__shfl_xor_sync(0xffffffffu, A.x, o2), __shfl_xor_sync(0xffffffffu, A.y, o2), __shfl_xor_sync(0xffffffffu, A.z, o2), __shfl_xor_sync(0xffffffffu, A.w, o2));
+                join(m1, l1, v);
+            }
+            __syncthreads();   /* the slice before has been joined */
+            if (lane < 8u) {
+                s_a[warp * 8u + lane] = A;
+                s_ml[warp * 8u + lane] = make_float2(M, L);
+            }
+            __syncthreads();
+            if (tid < 8u) {
+                for (uint32_t w = 1; w < WARPS; w++) join(s_ml[w * 8u + tid].x, s_ml[w * 8u + tid].y, s_a[w * 8u + tid]);
+                pg_store<HD>(P, u.tok0 + row / P.gqa, u.kh * P.gqa + row % P.gqa, d, A, L, gate);
+            }
+        }
+        pg_leave(P, u, joiners);
+    }
     if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
         if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
         for (; taken < issued; taken++)

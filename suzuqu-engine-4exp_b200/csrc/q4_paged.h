@@ -77,17 +77,16 @@ __device__ __forceinline__ void pg_store(const PagedParams &P, uint32_t tok, uin
     }
 }
 
-/* ---- shares.  `total` steps in `blocks` shares: share c begins at cut(c).  A cut that falls into a unit of at most SHORT steps, or
- * within NEAR steps of the end of a longer one, goes to the unit's nearer end: that costs less than another piece and records that
- * have to be joined. */
-template <uint32_t NEAR, uint32_t SHORT, uint32_t LEAST>
+/* ---- shares.  `total` steps in `blocks` shares: share c begins at cut(c).  A cut that falls into a unit of at most `little` steps, or
+ * within `near` steps of the end of a longer one, goes to the unit's nearer end: that costs less than another piece and records
+ * that have to be joined.  near is at least what a unit counts besides its own steps (a cut among those would be of no use). */
 struct PgShares {
     uint64_t total;
-    uint32_t blocks;
-    /* as many shares as there are blocks, but none of fewer than LEAST steps */
-    __device__ __forceinline__ void set(uint64_t n) {
-        total = n;
-        blocks = (uint32_t)min((uint64_t)gridDim.x, n >> 32 ? n : max((uint32_t)n / LEAST, n ? 1u : 0u));
+    uint32_t blocks, near, little;
+    /* as many shares as there are blocks, but none of fewer than `least` steps */
+    __device__ __forceinline__ void set(uint64_t n, uint32_t near_, uint32_t little_, uint32_t least) {
+        total = n; near = near_; little = little_;
+        blocks = (uint32_t)min((uint64_t)gridDim.x, n >> 32 ? n : max((uint32_t)n / least, n ? 1u : 0u));
     }
     __device__ __forceinline__ uint64_t cut(uint32_t c) const {
         return total >> 22 ? total * c / blocks : (uint32_t)total * c / blocks;   /* up to 1024 blocks */
@@ -96,9 +95,9 @@ struct PgShares {
         return total >> 21 ? (uint32_t)(((step + 1u) * blocks - 1u) / total) : (((uint32_t)step + 1u) * blocks - 1u) / (uint32_t)total;
     }
     /* where in a unit of `steps` steps a cut that falls on its step st lies */
-    static __device__ __forceinline__ uint64_t snap(uint64_t st, uint64_t steps) {
+    __device__ __forceinline__ uint64_t snap(uint64_t st, uint64_t steps) const {
         const uint64_t left = steps - st;
-        return steps > SHORT && st > NEAR && left > NEAR ? st : st <= left ? 0u : steps;
+        return steps > little && st > near && left > near ? st : st <= left ? 0u : steps;
     }
     /* the shares that the first and the last step of the unit [u0, u1) are in */
     __device__ __forceinline__ uint32_t first(uint64_t u0, uint64_t u1) const {
@@ -127,15 +126,42 @@ struct PgSplit { uint32_t first, last, tok0, n_here, kh; };
  * of the launch are resident (the grid is what the SMs hold), and end their shares within a few microseconds of one another; a
  * launch of its own for this took 8 to 12 us (one request over 262 144 rows 44 us with it).  The wait is bounded.  Every block
  * arrives and goes once, whatever happened before, and the last to go leaves the counters at zero.
- * What a block joins, and its gates, come to shared memory by bulk copies, all at once (16 bytes per thread and step: 6 to 10 us for
- * 160 KB); then a thread has four dims of a row, or shares them with others that take the other records. */
+ */
 __device__ __forceinline__ void pg_arrive(const PagedParams &P, const PgSplit &u) {   /* one thread, behind the block's records and a barrier */
     if (u.last < u.first) return;
-    asm volatile("fence.proxy.async;" ::: "memory");   /* the records are read by bulk copies */
     __threadfence();
     atomicAdd(P.meet + 2u * u.first, 1u);
 }
-/* bar: 8 bytes of shared memory for a barrier, not in use by anything */
+/* the whole block, until k have arrived */
+__device__ __forceinline__ void pg_wait(const PagedParams &P, const PgSplit &u, uint32_t k) {
+    if (threadIdx.x == 0) {
+        unsigned long long t0, t;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+        for (uint32_t i = 0;; i++) {
+            uint32_t n;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(P.meet + 2u * u.first) : "memory");
+            if (n >= k) break;
+            if ((i & 63u) == 63u) {
+                asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+                if (t - t0 > 2000000000ull) {
+                    atomicOr(P.err, (uint32_t)Q4E_CUDA);
+                    break;
+                }
+            }
+        }
+        __threadfence();
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void pg_leave(const PagedParams &P, const PgSplit &u, uint32_t joiners) {
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(P.meet + 2u * u.first + 1u, 1u) == joiners - 1u) {
+        P.meet[2u * u.first] = 0u;
+        P.meet[2u * u.first + 1u] = 0u;
+    }
+}
+/* What a block joins, and its gates, come to shared memory by bulk copies, all at once; then a thread has four dims of a row, or
+ * shares them with others that take the other records.  bar: 8 bytes of shared memory for a barrier, not in use by anything */
 template <int HD, uint32_t THREADS>
 __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes, uint32_t bar) {
     constexpr uint32_t REC = HD + 4u;
@@ -147,24 +173,8 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
     const uint32_t wide = (uint32_t)HD >> cut, slices = unit_rows << cut;
     const uint32_t s_begin = slices * mine / joiners, s_end = slices * (mine + 1u) / joiners;
     if (s_begin < s_end) {
-        if (tid == 0) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
-            unsigned long long t0, t;
-            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-            for (uint32_t i = 0;; i++) {
-                uint32_t n;
-                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(P.meet + 2u * u.first) : "memory");
-                if (n >= k) break;
-                if ((i & 63u) == 63u) {
-                    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-                    if (t - t0 > 2000000000ull) {
-                        atomicOr(P.err, (uint32_t)Q4E_CUDA);
-                        break;
-                    }
-                }
-            }
-            __threadfence();
-        }
+        if (tid == 0) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+        pg_wait(P, u, k);
         float4 *s_a = reinterpret_cast<float4 *>(smem);                      /* [thread] */
         float2 *s_ml = reinterpret_cast<float2 *>(smem + THREADS * 16u);     /* [thread] */
         float *s_gate = reinterpret_cast<float *>(smem + THREADS * 24u);     /* [slice][its dims] */
@@ -261,10 +271,7 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
     }
     __syncthreads();
     if (tid == 0 && s_begin < s_end) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-    if (tid == 0 && atomicAdd(P.meet + 2u * u.first + 1u, 1u) == joiners - 1u) {
-        P.meet[2u * u.first] = 0u;
-        P.meet[2u * u.first + 1u] = 0u;
-    }
+    pg_leave(P, u, joiners);
 }
 #endif
 

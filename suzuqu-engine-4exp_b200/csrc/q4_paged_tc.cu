@@ -54,7 +54,7 @@ struct ChunkCfg {
      * in q8_0): a unit counts as EXTRA more steps when the work is shared out.  Only tiles are walked.  512 tokens over 16 001 rows
      * 109 us with EXTRA 2, 98 with 3. */
     static constexpr uint32_t EXTRA = HD == 256 && KIND == Q4K_F16 ? 6u : 3u;
-    using Shares = PgShares<EXTRA, HD == 256 ? 4u * EXTRA : 16u, EXTRA + 2u>;
+    static constexpr uint32_t LITTLE = HD == 256 ? 4u * EXTRA : 16u;
     /* registers of a thread: the block's 512 x 128 are 256 threads x (softmax + the others) */
     static constexpr uint32_t R_SOFTMAX = 168u, R_OTHERS = 88u;
     static_assert(R_SOFTMAX + R_OTHERS <= 256u, "register split");
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     q4d_pdl_wait();
 
     /* ---- this block's share: the steps of all requests by one scan, the two places where it is cut by two warps */
-    typename C::Shares shares;
+    PgShares shares;
     {
         const uint32_t per = (P.n_req + CK_THREADS - 1u) / CK_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
         uint64_t mine = 0, before = 0, total = 0;
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         }
         before += x - mine;
         if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-        shares.set(total);
+        shares.set(total, CK_EXTRA, C::LITTLE, CK_EXTRA + 2u);
         if (tid < 2u) asm volatile("st.shared.v2.u64 [%0], {%1, %1};" ::"r"(s_at + 16u), "l"(total) : "memory");   /* begin and end: none yet, the last share's end */
         __syncthreads();
         if (mine && blockIdx.x < shares.blocks) {
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 lo += last * step;
                 if (step == 1u) break;
             }
-            const uint32_t st = (uint32_t)(in - at), to = (uint32_t)C::Shares::snap(st, unit_tiles(R, tpu, lo) + CK_EXTRA);
+            const uint32_t st = (uint32_t)(in - at), to = (uint32_t)shares.snap(st, unit_tiles(R, tpu, lo) + CK_EXTRA);
             if (lane == 0) {
                 if (which == 0u) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(s_at), "r"(r), "r"(kh), "r"(lo), "r"(to) : "memory");
                 asm volatile("st.shared.u64 [%0], %1;" ::"r"(s_at + 16u + 8u * which), "l"(s - st + to) : "memory");
@@ -971,7 +971,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         }
     }
     if (!ok && lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
-    __threadfence();             /* this thread's records */
+    asm volatile("fence.proxy.async;" ::: "memory");   /* this thread's records, which others read by bulk copies */
+    __threadfence();
     tc_fence_before();
     __syncthreads();
     if (warp == C::ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
