@@ -503,7 +503,10 @@ bool q4_gpu_pages_gather(const q4_gpu_pages *pg, uint32_t layer, const int32_t *
  *   max_add  the most tokens of one request, as far as the host knows (0: it does not).  It chooses between kernels only: results
  *            are right for any value
  * A request whose rows pass its table's row is left out (status bit 4); positions on a page that is not the pool's are skipped
- * (status bit 4); a token with nothing to attend gets 0.  Scratch grows outside a capture only (status bit 8 inside one). */
+ * (status bit 4); a token with nothing to attend gets 0.  Scratch grows outside a capture only (status bit 8 inside one).
+ * Queries, rows and weights enter the products as fp16 (q8_0: fp16(code * scale)): beyond 65504 in size they are not finite there.
+ * What is not finite stays with the tokens that attend it: a V that is not makes their outputs so in its dims, a new row's also in
+ * others. */
 bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, int q_bf16, const float *gate, void *out, int out_bf16,
                          uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
                          uint32_t table_stride, uint32_t max_add, float scale);

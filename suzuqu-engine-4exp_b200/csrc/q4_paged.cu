@@ -83,6 +83,29 @@ __device__ __forceinline__ uint32_t raised2(uint32_t x) { return __byte_perm(x, 
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t codes2(uint32_t x) { return h2u(__hsub2(u2h(raised2<SEL>(x)), u2h(0x64806480u))); }
 
+/* the rows of the tile at sb (by a whole warp) whose V holds a number that is not finite; rows behind the last position may be among them */
+template <int KIND, int HD>
+__device__ __forceinline__ uint32_t not_finite(uint32_t sb, uint32_t lane) {
+    constexpr uint32_t TILE = PgTile<KIND, HD>::BYTES;
+    uint32_t rows = 0;
+    if constexpr (KIND == Q4K_Q8) {   /* fp16(127 x scale) is not from 516 on */
+        const uint32_t a = sb + (lane & 15u) * (TILE / 16u) + 2u * HD + HD / 16u;
+#pragma unroll
+        for (uint32_t b = 0; b < HD / 64u; b++) {
+            const uint32_t x = lds32(a + 4u * b);
+            if ((x & 0x7fffu) > 0x6007u || (x >> 16 & 0x7fffu) > 0x6007u) rows = 1u << (lane & 15u);
+        }
+    } else {   /* exponents of ones only */
+#pragma unroll 4
+        for (uint32_t i = 0; i < HD / 8u; i++) {   /* 8 bytes at a time: two rows of a block of 64 dims */
+            const uint2 w = lds64(sb + TILE / 2u + i * 256u + lane * 8u);
+            const bool x = (w.x & 0x7c00u) == 0x7c00u || (w.x & 0x7c000000u) == 0x7c000000u || (w.y & 0x7c00u) == 0x7c00u || (w.y & 0x7c000000u) == 0x7c000000u;
+            if (x) rows |= 1u << ((2u * i + (lane >> 4)) & 15u);
+        }
+    }
+    return __reduce_or_sync(0xffffffffu, rows);
+}
+
 /* warps per block, blocks per SM, tiles of a warp's ring: as many bytes in flight as an SM's shared memory holds */
 template <int KIND, int HD, int NT>
 struct FewCfg {
@@ -99,6 +122,7 @@ struct FewCfg {
     static constexpr uint32_t REC = HD + 4u;
     /* the warps' records reuse the ring: of all warps at once, or of half of them, which have taken over the others' fragments */
     static constexpr uint32_t FRAG = (HD / 16u * 4u + 4u) * NT * 32u * 4u, PARTS = WARPS * ROWS * REC * 4u <= RING ? WARPS : WARPS / 2u;
+    static_assert(ROWS <= (WARPS - 1u) * 16u + 1u, "masks in a warp's last tile only");
     static_assert(WARPS / 2u * FRAG <= RING && PARTS * ROWS * REC * 4u <= RING, "merge does not fit");
     static constexpr uint32_t DIRECT = 16u;                  /* records that the unit's last block joins alone */
     static constexpr uint32_t SMEM = RING + ROWS * Q_STRIDE + WARPS * DEPTH * 8u + 1024u;
@@ -162,12 +186,12 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     }
     /* Where the blocks have many steps each, a unit counts as EXTRA more, that a piece costs, and short ones stay whole (a token of 64
      * sessions 116 -> 113 us).  Where they have few, the way through the launch counts: units are cut as finely as there are
-     * blocks, down to one step (a token of four short chats 13.4 us whole, 11.5 so). */
+     * blocks, down to one step (a token of four short chats 13.4 us whole, 11.4 so), but where a unit has three at most (one such chat 9.7 us cut, 8.5 whole). */
     const uint32_t extra = total >= 4u * gridDim.x ? C::EXTRA : 0u;   /* also shares.near */
     total += all_units * extra; before += units_before * extra; mine += units * extra;
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     PgShares shares;
-    shares.set(total, extra, extra ? 8u : 0u, extra ? 4u : 1u);
+    shares.set(total, extra, extra ? 8u : 3u, extra ? 4u : 1u);
     if (blockIdx.x >= shares.blocks) return;
     if (tid == 0) {
         s_end2[0] = s_end2[1] = total;
@@ -393,13 +417,34 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
             }
             const bool gone = (dead >> (i & 31u)) & 1u;   /* its page is not the pool's: all masked */
             if ((i & 31u) == 31u) dead = dead_nxt;
-            const bool tail = p0 + 16u > n_kv || gone;
-            if (p0 + 16u > lim_min || gone) {
+            /* Rows whose V is taken: a weight of 0 does not keep one that is not finite from a sum.  Those behind the last position hold
+             * anything; one that some columns attend and some do not is left out too, and makes the former NaN by their scores.
+             * Both can be in a warp's last tile only: the positions from lim_min on lie in consecutive tiles of different warps. */
+            uint32_t live16 = gone ? 0u : 0xffffu;
+            if (gone) {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = -CUDART_INF_F;
+            }
+            if constexpr (!decltype(more)::value) {
+                if (p0 + 16u > lim_min && !gone) {
+                    if (p0 + 16u > n_kv) live16 = (1u << (n_kv - p0)) - 1u;
+                    if (lim_min < n_kv) {
+                        const uint32_t bad = not_finite<KIND, HD>(sb, lane);
+                        if (bad) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (gone || p0 + g + (k >> 1) * 8u >= lim[n][k & 1]) sc[n][k] = -CUDART_INF_F;
+                            for (int n = 0; n < NT; n++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    if ((bad >> (g + (k >> 1) * 8u)) & 1u) sc[n][k] = CUDART_NAN_F;
+                            live16 &= ~bad;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (p0 + g + (k >> 1) * 8u >= lim[n][k & 1]) sc[n][k] = -CUDART_INF_F;
+                }
             }
             /* the maxima (of scores times scale_log2e) move only where a score is above them: seldom, after the first tiles */
             bool grow = false;
@@ -429,11 +474,11 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                         }
                     }
             }
-            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;   /* rows behind the last position hold anything: 0 x NaN has to stay 0 */
-            if (tail) {
-                const uint32_t p = p0 + 2u * t, end = gone ? 0u : n_kv;
-                keep0 = (p < end ? 0xffffu : 0u) | (p + 1u < end ? 0xffff0000u : 0u);
-                keep1 = (p + 8u < end ? 0xffffu : 0u) | (p + 9u < end ? 0xffff0000u : 0u);
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+            if (live16 != 0xffffu) {
+                const uint32_t rows = live16 >> (2u * t);
+                keep0 = (rows & 1u ? 0xffffu : 0u) | (rows & 2u ? 0xffff0000u : 0u);
+                keep1 = (rows & 0x100u ? 0xffffu : 0u) | (rows & 0x200u ? 0xffff0000u : 0u);
             }
             uint32_t pb[NT][2];
 #pragma unroll
@@ -480,7 +525,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                     const uint32_t c = 2u * k + mchunk;
                     ldmatrix_x4_trans(w, sb + TILE / 2u + (c >> 3) * 2048u + mrow * 128u + (((c & 7u) ^ (mrow & 7u)) << 4));
                     uint32_t a[4] = {w[0], w[2], w[1], w[3]};
-                    if (tail) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
+                    if (live16 != 0xffffu) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
 #pragma unroll
                     for (int n = 0; n < NT; n++) mma16816(o[k][n], a, pb[n][0], pb[n][1]);
                 }

@@ -16,6 +16,11 @@
  *   walker         the share's pieces, and where the rows of their tiles lie, ahead of the others
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
  *
+ * A weight of 0 does not keep a V that is not finite from a sum.  Rows behind the last position are zeros in the slot.  Of the
+ * unit's own tokens, which earlier ones do not attend, the walker looks through the rows before it hands their tile on; where
+ * there is a V that is not finite the producers take the tile's rows by a slower way, with zeros in its place, and a row that
+ * attends the first of them is NaN, by its sum.  (What lies before the unit's tokens is attended by every row.)
+ *
  * Every wait is bounded: on expiry the block's waits all end, Q4E_CUDA is set, and tensor memory is freed.
  */
 #include <cuda_bf16.h>
@@ -89,6 +94,21 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool t
         for (int i = 0; i < BYTES; i += 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + i), "r"(0u) : "memory");
     }
 }
+constexpr uint32_t TILE_BAD = 0x100u;   /* beside the eight bits of a tile's places without a page: new rows whose V is not finite */
+/* whether the V of a record is not finite as fp16(code x scale): the largest code is 127, which reaches 65520 from 516 on */
+template <int HD>
+__device__ __forceinline__ bool not_finite_q8(const uint8_t *rec) {
+    bool bad = false;
+#pragma unroll
+    for (uint32_t b = 0; b < HD / 64u; b++) {
+        const uint32_t x = __ldcg(reinterpret_cast<const uint32_t *>(rec + 2u * HD + HD / 16u) + b);
+        bad |= (x & 0x7fffu) > 0x6007u || (x >> 16 & 0x7fffu) > 0x6007u;
+    }
+    return bad;
+}
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {   /* all ones for a half whose exponent is */
+    return ((x & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
 /* the rest of a wait whose first test found the phase incomplete (in line: ptxas does not allocate calls beside setmaxnreg) */
 __device__ __forceinline__ bool ck_wait_on(uint32_t bar, uint32_t parity, uint32_t s_abort) {
     const unsigned long long t0 = global_ns();
@@ -149,6 +169,7 @@ struct Piece {
     uint32_t before;             /* rows of the request before the unit's first token: it attends those and itself */
     uint32_t tok0, n_here, kh;   /* the unit's first token, its tokens, its kv head */
     uint32_t req, st, here;      /* the piece: tiles [st, st + here) of the unit; here = 0: there are no more */
+                                 /* (in the ring the first new position whose V is not finite has the place of req, which only the walker uses) */
     uint32_t tiles;              /* of the unit */
     bool gone;                   /* some of its positions are on pages that are not the pool's */
 };
@@ -205,7 +226,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     const uint32_t sQ = (smem_u32(smem_dyn) + 1023u) & ~1023u, sR = sQ + NQ * C::QG, bars = sR + SLOTS * SLOT + TEAMS * WPT * C::ROUNDS * C::RAW;
     const uint32_t full = bars, empty = bars + 80, bar_s = bars + 160, bar_p = bars + 192, bar_o = bars + 224, bar_q = bars + 240,
                    s_tmem = bars + 248, s_abort = bars + 252, s_gone = bars + 256, s_at = bars + 320, s_sum = bars + 352, w_full = bars + 480,
-                   w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_split = bars + 928, s_xch = bars + 1024;
+                   w_empty = bars + 512, t_full = bars + 544, t_empty = bars + 576, s_piece = bars + 608, s_tile = bars + 736, s_split = bars + 928, checks = bars + 968, s_xch = bars + 1024;
     uint8_t *base = smem_dyn + (sQ - smem_u32(smem_dyn));
     const uint32_t tpu = P.tpg * NQ;
 
@@ -230,6 +251,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 mbar_init(t_full + 8 * s, 1);
                 mbar_init(t_empty + 8 * s, WPT * PARTS * 2u);   /* the warps of every slot of its K and V */
             }
+            for (uint32_t s = 0; s < TEAMS * WPT; s++) mbar_init(checks + 8 * s, 1);
             asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_abort), "r"(0u) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -465,6 +487,36 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             uint32_t n_tile = 0;
             const uint32_t per_page = P.part_bytes / TILE;
             PgSplit split[2] = {{1u, 0u, 0u, 0u, 0u}, {1u, 0u, 0u, 0u, 0u}};   /* that began before this block; that go on behind it */
+            /* the first of rows r0 .. r1 - 1 of a tile of 128 positions whose V is not finite (none: all ones); lane i knows where its rows
+             * from 16 i on lie */
+            auto look = [&](uint32_t at, uint32_t gone8, uint32_t r0, uint32_t r1) -> uint32_t {
+                uint32_t bad = 0xffffffffu;
+                if constexpr (KIND == Q4K_Q8) {
+#pragma unroll 1
+                    for (uint32_t i = r0; i < r1; i += 32u) {
+                        const uint32_t row = min(i + lane, r1 - 1u), lies = __shfl_sync(0xffffffffu, at, (int)(row >> 4));
+                        if (not_finite_q8<HD>(P.mem + (uint64_t)lies * TILE + (row & 15u) * ROW) && !((gone8 >> (row >> 4)) & 1u)) bad = min(bad, row);
+                    }
+                } else {   /* 16 bytes of a row per lane, four loads on their way */
+                    constexpr uint32_t LANES = HD / 8u, RPL = 32u / LANES, BATCH = 4u;   /* lanes of a row, rows of a load */
+                    const uint32_t x = lane % LANES, in_row = TILE / 2u + (x >> 3) * 2048u + (x & 7u) * 16u;
+#pragma unroll 1
+                    for (uint32_t i = r0; i < r1; i += RPL * BATCH) {
+                        uint4 w[BATCH];
+#pragma unroll
+                        for (uint32_t k = 0; k < BATCH; k++) {
+                            const uint32_t row = min(i + k * RPL + lane / LANES, r1 - 1u), lies = __shfl_sync(0xffffffffu, at, (int)(row >> 4));
+                            w[k] = __ldcg(reinterpret_cast<const uint4 *>(P.mem + (uint64_t)lies * TILE + in_row + (row & 15u) * 128u));
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < BATCH; k++) {
+                            const uint32_t row = min(i + k * RPL + lane / LANES, r1 - 1u);
+                            if ((not_finite2(w[k].x) | not_finite2(w[k].y) | not_finite2(w[k].z) | not_finite2(w[k].w)) && !((gone8 >> (row >> 4)) & 1u)) bad = min(bad, row);
+                        }
+                    }
+                }
+                return __reduce_min_sync(0xffffffffu, bad);
+            };
             Walk<CK_EXTRA> W;
             W.left = 0;
             if (s_begin < s_end) W.begin(P, s_begin, s_end - s_begin, w_req, w_kh, w_g, w_st);
@@ -486,7 +538,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 if (n >= PIECES) ok = ok && ck_all_wait(w_empty + 8 * e, (n / PIECES - 1u) & 1u, s_abort);
                 if (ok && lane == 0) {
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(p.before), "r"(p.tok0), "r"(p.n_here | (gone ? 0x80000000u : 0u)), "r"(p.kh) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(p.req), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a + 16u), "r"(0xffffffffu), "r"(p.st), "r"(p.here), "r"(p.tiles) : "memory");
                     mbar_arrive(w_full + 8 * e);
                 }
                 if (!more) break;
@@ -500,6 +552,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
                     }
                 }
+                const uint32_t first_new = p.n_here > 1u ? p.before + 1u : 0xffffffffu;   /* from here on some rows attend a position and some do not */
+                bool bad_yet = false;
                 /* tile by tile: where its eight tiles of 16 positions lie, in units of such tiles; its live positions; those without a page */
                 for (uint32_t tile = 0; tile < p.here && ok; tile++, n_tile++) {
                     const int32_t page = next;
@@ -507,12 +561,20 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                     const uint32_t q = q0 + tile * CK_BN, te = n_tile % TILES, ta = s_tile + te * 48u;
                     const bool there = (uint32_t)page < P.n_pages;
                     const uint32_t at = there ? ((uint32_t)page * P.n_kvh + p.kh) * per_page + ((q & ((1u << P.page_shift) - 1u)) >> 4) : 0u;
-                    const uint32_t gone8 = __ballot_sync(0xffffffffu, !there) & 0xffu;
+                    uint32_t gone8 = __ballot_sync(0xffffffffu, !there) & 0xffu;
+                    if ((p.st + tile + 1u) * CK_BN > first_new) {   /* new rows whose V is not finite */
+                        const uint32_t t0 = (p.st + tile) * CK_BN, r0 = max(first_new, t0) - t0, r1 = min(n_kv - t0, CK_BN), bad = look(at, gone8, r0, r1);
+                        if (bad != 0xffffffffu) {
+                            gone8 |= TILE_BAD;
+                            if (!bad_yet && ok && lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(a + 16u), "r"(t0 + bad) : "memory");
+                            bad_yet = true;
+                        }
+                    }
                     if (n_tile >= TILES) ok = ok && ck_all_wait(t_empty + 8 * te, (n_tile / TILES - 1u) & 1u, s_abort);
                     if (!ok) break;
                     if (lane < 8u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ta + lane * 4u), "r"(at) : "memory");
                     if (lane == 8u) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(ta + 32u), "r"(n_kv - (p.st + tile) * CK_BN), "r"(gone8) : "memory");
-                    if (lane == 9u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (n_tile & 15u)), "r"(gone8) : "memory");   /* for the softmax, once the tile's scores are there */
+                    if (lane == 9u) asm volatile("st.shared.u32 [%0], %1;" ::"r"(s_gone + 4u * (n_tile & 15u)), "r"(gone8 & 0xffu) : "memory");   /* for the softmax, once the tile's scores are there */
                     __syncwarp();
                     if (lane == 0) mbar_arrive(t_full + 8 * te);
                 }
@@ -598,8 +660,13 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
 #pragma unroll
                         for (uint32_t b = 0; b < NB; b++) copy_async<16>(raw + (i * NB + b) * 512u + lane * 16u, rec[i / 2u] + ((i & 1u) * 8u + r8) * ROW + col + b * 64u, true);
                     if (lane < RG * 8u) copy_async<NB * 4>(raw + ITEMS * 512u + lane * (NB * 4u), srec, true);
-                } else {   /* zeros for rows that are not there */
-                    auto there = [&](uint32_t row) -> bool { return row < live && !((gone >> (row >> 4)) & 1u); };
+                } else {   /* zeros for rows that are not there, and V that is not finite, where that matters */
+                    uint32_t bad = 0;   /* of the round's rows */
+                    if (gone & TILE_BAD && job.v) {
+                        const uint32_t row = min(g0 * 8u + lane, CK_BN - 1u);
+                        bad = __ballot_sync(0xffffffffu, not_finite_q8<HD>(P.mem + (uint64_t)lds(place + (row >> 4) * 4u) * TILE + (row & 15u) * ROW));
+                    }
+                    auto there = [&](uint32_t row) -> bool { return row < live && !((gone >> (row >> 4)) & 1u) && !((bad >> (row - g0 * 8u)) & 1u); };
 #pragma unroll 1
                     for (uint32_t i = 0; i < RG; i++)
 #pragma unroll
@@ -682,6 +749,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             /* a slot is 16 units of 2 KB (8 at hd 64): 16 rows of a block of 64 dims.  One bulk copy each, shared out over the warps: a
              * warp issues one in about 100 cycles */
             constexpr uint32_t UNITS = SLOT / 2048u / WPT;
+            const uint32_t check_bar = checks + 8u * (warp - C::PRODUCER);
+            uint32_t n_check = 0;
             Job job;
             while (ok && next_job(job)) {
                 const uint32_t nblk = HD == 256 ? (job.v ? 4u : 2u) : HD / 64u, rows = HD == 256 && job.v ? 64u : 128u, place = s_tile + job.tile * 48u;
@@ -692,7 +761,8 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 tile_read(job);
                 wait_empty();
                 if (!ok) break;
-                const uint32_t s = at % SLOTS, bar = full + 8 * s, to = sR + s * SLOT + b * rows * 128u + tile * 2048u;
+                const bool check = job.v && gone & TILE_BAD;
+                const uint32_t s = at % SLOTS, bar = check ? check_bar : full + 8 * s, to = sR + s * SLOT + b * rows * 128u + tile * 2048u;
                 const uint32_t all = __reduce_add_sync(0xffffffffu, lane < UNITS ? live : 0u);
                 if (job.v && all < 16u * UNITS) {   /* what is not copied has to be 0: weights there are 0, and 0 x NaN is not */
                     for (uint32_t u = 0; u < UNITS; u++) {
@@ -711,6 +781,24 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
                 __syncwarp();
                 if (lane < UNITS && live)
                     bulk_load(to, P.mem + (uint64_t)lies * TILE + (job.v ? TILE / 2u : 0u) + ((HD == 256 && !job.v ? job.part * 2u : 0u) + b) * 2048u, live * 128u, bar);
+                if (__builtin_expect(check, 0)) {   /* zeros for what is not finite, before the slot is handed on */
+                    n_check++;
+                    ok = ck_all_wait(check_bar, (n_check - 1u) & 1u, s_abort);
+                    if (!ok) {   /* its copies land all the same (bounded) */
+                        for (uint32_t i = 0; i < 4096u && !mbar_test<OWN>(check_bar, (n_check - 1u) & 1u); i++) {}
+                        break;
+                    }
+#pragma unroll 1
+                    for (uint32_t u = 0; u < UNITS * 4u; u++) {
+                        const uint32_t a = __shfl_sync(0xffffffffu, to, (int)(u >> 2)) + (u & 3u) * 512u + lane * 16u;
+                        uint4 w;
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(a) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(w.x & ~not_finite2(w.x)), "r"(w.y & ~not_finite2(w.y)), "r"(w.z & ~not_finite2(w.z)), "r"(w.w & ~not_finite2(w.w)) : "memory");
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + 8 * s);
+                }
                 at += TEAMS;
             }
             /* gave up: copies in flight land before the block's shared memory is another's (bounded) */
@@ -914,6 +1002,11 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             float *rec = P.part + ((size_t)blockIdx.x * 2u + (p.st == 0u ? 1u : 0u)) * C::ROWS * C::REC;
             if (active && ok) ok = ck_all_wait(bar_o + 8 * g, (use - 1u) & 1u, s_abort);
             tc_fence_after();
+            {
+                uint32_t bad;   /* the first position whose V is not finite */
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bad) : "r"(s_piece + n_piece % PIECES * 32u + 16u) : "memory");
+                if (row_live && row_nkv > bad) l_run = CUDART_NAN_F;
+            }
             if (active && ok) {
                 const float inv = whole ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
                 const uint32_t buf = sQ + warp * (NQ * C::QG / 8u);   /* [32 rows][8 x 16 bytes], piece k of row r at k ^ (r & 7) */

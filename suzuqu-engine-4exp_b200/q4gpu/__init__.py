@@ -148,13 +148,18 @@ def init():
 
 def _ptr(t):
     """Device (or host) address of a torch tensor / numpy array / int / None."""
-    if t is None:
-        return None
-    if isinstance(t, int):
+    if t is None or isinstance(t, int):
         return t
-    if hasattr(t, "data_ptr"):
+    try:
         return t.data_ptr()
-    return t.ctypes.data
+    except AttributeError:
+        return t.ctypes.data
+
+
+def _dense(*tensors):
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            raise RuntimeError("a dense tensor is needed, not one with strides %s" % (t.stride(),))
 
 
 def check(ok, what):
@@ -395,8 +400,8 @@ class Batch:
 
 
 class PagePool:
-    """A paged KV cache for many requests (q4_gpu_pages_*).  Arrays are torch tensors on the device; the pool's memory and its stack
-    of free pages are allocated here unless they are given.  Per step: plan, then append and attend for every layer."""
+    """A paged KV cache for many requests (q4_gpu_pages_*).  Arrays are dense torch tensors on the device; the pool's memory and its
+    stack of free pages are allocated here unless they are given.  Per step: plan, then append and attend for every layer."""
 
     def __init__(self, n_layers, n_kvh, hd, n_pages, page_rows=64, kind=KIND_Q8, mem=None, free=None, n_free=None):
         import torch
@@ -419,24 +424,31 @@ class PagePool:
 
     def plan(self, rows, add, table, start, slot, pos, req):
         """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok]"""
+        _dense(rows, add, table, start, slot, pos, req)
         n, stride = table.shape
         check(self.L.q4_gpu_pages_plan(self.p, _ptr(rows), _ptr(add), n, _ptr(table), stride, _ptr(start), _ptr(slot), _ptr(pos),
                                        _ptr(req), slot.shape[0]), "q4_gpu_pages_plan")
 
     def trim(self, rows, keep, table):
         """the pages behind the first keep[r] of rows[r] rows go back"""
+        _dense(rows, keep, table)
         n, stride = table.shape
         check(self.L.q4_gpu_pages_trim(self.p, _ptr(rows), _ptr(keep), n, _ptr(table), stride), "q4_gpu_pages_trim")
 
     def append(self, layer, k, v, slot):
+        """k, v [slot.shape[0]][n_kvh * hd] fp32; slots below 0 are skipped"""
+        _dense(k, v, slot)
         check(self.L.q4_gpu_pages_append(self.p, layer, _ptr(k), _ptr(v), _ptr(slot), slot.shape[0]), "q4_gpu_pages_append")
 
     def gather(self, layer, slot, k, v):
+        """the rows of the slots as fp32, the reverse of append; k or v may be None"""
+        _dense(slot, k, v)
         check(self.L.q4_gpu_pages_gather(self.p, layer, _ptr(slot), slot.shape[0], _ptr(k), _ptr(v)), "q4_gpu_pages_gather")
 
     def attend(self, layer, q, out, rows, start, table, n_head, scale, gate=None, max_add=0):
         """attention of the step's tokens: q, out [n_tok][n_head][hd], bf16 or fp32; rows as they were given to plan"""
         import torch
+        _dense(q, out, rows, start, table, gate)
         n, stride = table.shape
         n_tok = q.numel() // (n_head * self.hd)
         check(self.L.q4_gpu_pages_attend(self.p, layer, _ptr(q), q.dtype == torch.bfloat16, _ptr(gate), _ptr(out),
