@@ -24,6 +24,8 @@ struct PagedParams {
     float *part;                 /* [block][2][rows of a unit][hd + 4]: acc, m (log2 units, scale folded in), l */
     uint32_t *meet;              /* [block][2]: arrived, gone, of the blocks of the unit that begins in the block; zero between launches */
     uint32_t *err;
+    const uint32_t *fits;        /* not NULL: the launch has work only if this word is `fits_is` (q4i_paged_stage's) */
+    uint32_t fits_is;
 };
 
 template <int KIND, int HD>
@@ -37,6 +39,11 @@ constexpr uint32_t PG_MAX_BLOCKS = 1024;
  * at least q4i_paged_chunk_floats floats.  hd 64, 128 or 256, kind fp16 or q8_0. */
 size_t q4i_paged_chunk_floats(uint32_t hd);
 bool q4i_paged_chunk(const PagedParams &p, int kind, uint32_t hd, float *scratch);
+
+/* A copy in fp16 of the pages of those requests (pool of q8_0): at most cap pages of page_rows rows and all kv heads, their table, and
+ * whether they were that few (q4_paged_stage.cu).  n_req up to PG_STAGE_REQ. */
+constexpr uint32_t PG_STAGE_REQ = 8192;
+bool q4i_paged_stage(const PagedParams &p, uint32_t hd, uint8_t *to, int32_t *table, uint32_t cap, uint32_t *fits);
 
 #ifdef __CUDACC__
 /* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */

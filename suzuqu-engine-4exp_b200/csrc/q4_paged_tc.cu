@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     /* ---- this block's share: the steps of all requests by one scan, the two places where it is cut by two warps */
     PgShares shares;
     {
-        const uint32_t per = (P.n_req + CK_THREADS - 1u) / CK_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
+        const uint32_t n_req = P.fits && *P.fits != P.fits_is ? 0u : P.n_req, per = (n_req + CK_THREADS - 1u) / CK_THREADS, r0 = min(tid * per, n_req), r1 = min(r0 + per, n_req);
         uint64_t mine = 0, before = 0, total = 0;
         bool bad, any_bad = false;
         PgReq R = {0u, 0u, 0u};

@@ -29,7 +29,7 @@ BAD = [float("inf"), -float("inf"), float("nan"), 1e6]
 
 @pytest.mark.parametrize("kind", ["q8_0", "f16"])
 @pytest.mark.parametrize("n_head,n_kvh,hd", [(16, 2, 128), (12, 2, 64), (24, 2, 256), (4, 2, 256)])
-@pytest.mark.parametrize("held,n,at", [(37, 3, 1), (0, 3, 2), (120, 70, 9), (0, 200, 128), (1000, 40, 39), (6007, 150, 1), (31, 4, 3)])
+@pytest.mark.parametrize("held,n,at", [(37, 3, 1), (0, 3, 2), (120, 70, 9), (0, 200, 128), (1000, 40, 39), (6007, 150, 1), (31, 4, 3), (100, 1500, 700)])
 def test_new_rows_that_are_not_finite_stay_with_the_tokens_that_attend_them(kind, n_head, n_kvh, hd, held, n, at):
     """a weight of 0 times a V that is not finite is no 0.  Tokens before `at` have to come out bit by bit as without it"""
     s, k, v = step_of([held, 50], [n, 2], kind, n_kvh, hd)
@@ -90,6 +90,74 @@ def test_one_token_each(kind, n_head, n_kvh, hd, rows):
                                       ([5000], [17]), ([0, 128, 127, 1], [128, 128, 1, 127])])
 def test_several_tokens(kind, n_head, n_kvh, hd, rows, add):
     run_attend(rows, add, n_head, n_kvh, hd, kind, page=64, gate=True, max_add=max(add))
+
+
+# many tokens over q8_0: rows are read from a copy in fp16
+@pytest.mark.parametrize("n_head,n_kvh,hd", [(16, 2, 128), (32, 2, 64), (24, 2, 256), (16, 1, 256)])
+@pytest.mark.parametrize("rows,add", [([300], [1500]), ([0, 77, 1000], [1300, 1999, 900]), ([33, 0, 5, 128], [1200, 0, 1, 2600])])
+def test_many_tokens(n_head, n_kvh, hd, rows, add):
+    run_attend(rows, add, n_head, n_kvh, hd, "q8_0", page=32, max_add=max(add))
+
+
+def test_many_tokens_with_pages_that_are_not_the_pool_s():
+    L = lib()
+    n_head, n_kvh, hd = 16, 2, 128
+    s, k, v = step_of([200, 64], [2200, 1], "q8_0", n_kvh, hd, page=16)
+    s.pool.append(0, k, v, s.slot[:2201])
+    q = torch.randn(2201, n_head, hd, device="cuda")
+    out, short = torch.empty_like(q), torch.empty_like(q)
+    scale = float(hd ** -0.5)
+    bad = s.d_table.clone()
+    bad[0, 3], bad[0, 140] = -1, s.pool.n_pages        # positions 48 to 63 and 2240 to 2255
+    s.pool.attend(0, q, out, s.d_rows, s.start, bad, n_head, scale)
+    assert L.q4_gpu_last_error() == 4
+    s.pool.attend(0, q[:2200], short[:2200], s.d_rows, ints([0, 0, 0]), bad, n_head, scale)   # no tokens: nothing
+    assert L.q4_gpu_last_error() == 0
+    table = s.d_table[0].tolist()
+    kr, vr = torch.empty(2, 2400, n_kvh * hd, device="cuda")
+    s.pool.gather(0, ints([table[p // 16] * 16 + p % 16 for p in range(2400)]), kr, vr)
+    keep = torch.ones(2400, dtype=torch.bool, device="cuda")
+    keep[48:64] = keep[2240:2256] = False
+    kr, vr = (x.view(-1, n_kvh, hd).double().repeat_interleave(n_head // n_kvh, 1) for x in (kr, vr))
+    for j in (0, 700, 2039, 2040, 2199):
+        p = torch.arange(2400, device="cuda")
+        w = torch.einsum("hd,phd->hp", q[j].double(), kr) * scale
+        w = w.masked_fill((p > 200 + j) | ~keep, -torch.inf)
+        want = torch.einsum("hp,phd->hd", torch.softmax(w, -1), vr)
+        assert ((out[j].double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+
+
+def test_many_tokens_that_the_copy_has_no_room_for():
+    """a table wide enough for more rows than the copy may hold: used where the step's rows fit, and not where they do not"""
+    L = lib()
+    n_head, n_kvh, hd, page, wide = 16, 8, 256, 256, 400   # 2 MB of copy per page: 256 of them at most
+    s = Step([0], [1100], page, n_pages=300, stride=wide, n_kvh=n_kvh, hd=hd, kind=q4gpu.KIND_Q8)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    s.plan()
+    k, v = torch.randn(2, 1100, n_kvh * hd, device="cuda", generator=g)
+    s.pool.append(0, k, v, s.slot[:1100])
+    q = torch.randn(1100, n_head, hd, device="cuda", generator=g)
+    out = torch.empty(1100, n_head, hd, device="cuda")
+    scale = float(hd ** -0.5)
+    s.pool.attend(0, q, out, s.d_rows, s.start, s.d_table, n_head, scale, max_add=1100)
+    kr, vr = torch.empty(2, 1100, n_kvh * hd, device="cuda")
+    s.pool.gather(0, s.slot[:1100], kr, vr)
+    want = attend_exact(q, kr.view(-1, n_kvh, hd), vr.view(-1, n_kvh, hd), None, 0, scale)
+    assert ((out.double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+    # 290 pages before the same tokens: all of the first 286 the same page, whose rows are zeros but for V
+    s.pool.append(0, torch.zeros(256, n_kvh * hd, device="cuda"), torch.ones(256, n_kvh * hd, device="cuda"), torch.arange(256, dtype=torch.int32, device="cuda") + s.free_now()[0] * page)
+    table = torch.full_like(s.d_table, -1)
+    table[0, :286] = s.free_now()[0]
+    table[0, 286:291] = s.d_table[0, :5]
+    s.pool.attend(0, q, out, ints([286 * 256]), s.start, table, n_head, scale, max_add=1100)
+    assert L.q4_gpu_last_error() == 0
+    # 73 216 weights of exp(0) on ones beside the tokens' own
+    kr, vr = (x.view(-1, n_kvh, hd).double().repeat_interleave(2, 1) for x in (kr, vr))
+    for j in (0, 500, 1099):
+        w = torch.einsum("hd,phd->hp", q[j].double(), kr[: j + 1]) * scale
+        e = torch.exp(w)
+        want = (286 * 256 + torch.einsum("hp,phd->hd", e, vr[: j + 1])) / (286 * 256 + e.sum(-1, keepdim=True))
+        assert ((out[j].double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
 
 
 @pytest.mark.parametrize("hint", [0, 1, 2, 5, 100000])
