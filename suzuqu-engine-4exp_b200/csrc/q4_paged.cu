@@ -763,7 +763,6 @@ bool few(PagedParams &p, float *scratch) {
     }
     p.part = scratch;
     p.tpg = C::ROWS / p.gqa;
-    p.group_rows = C::ROWS;
     static uint32_t *meet = nullptr;
     if (!meet && !q4i_check(cudaGetSymbolAddress((void **)&meet, g_few_meet), "pages_attend counters")) return false;
     p.meet = meet;

@@ -12,7 +12,7 @@ struct PagedParams {
     uint64_t page_bytes;         /* of all kv heads */
     uint32_t part_bytes;         /* of one kv head */
     uint32_t n_pages, page_shift, n_kvh, n_head, gqa;
-    uint32_t tpg, group_rows;    /* tokens of a group, rows that a group takes (the last ones may be empty) */
+    uint32_t tpg;                /* tokens of a group of rows (128 in q4_pg_chunk_k, of which the last ones may be empty) */
     uint32_t add_split;          /* requests that bring at most so many tokens are q4_pg_few_k's, the others q4_pg_chunk_k's */
     const int32_t *rows, *start, *table;
     uint32_t table_stride, n_req, n_tok;
@@ -189,12 +189,13 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
         const uint32_t stride = wide + 4u, room = smem_bytes - THREADS * 24u, gate_bytes = P.gate ? wide * 4u : 0u, fit = room / (k * stride * 4u + gate_bytes);
         const uint32_t at_once = fit ? fit : 1u, recs_at_once = fit ? k : (room - gate_bytes) / (stride * 4u);
         uint32_t phase = 0;
+        const uint32_t inv_gqa = 65536u / P.gqa + 1u, per_slice = (HD == 64 ? 4u : HD == 128 ? 5u : 6u) - cut;   /* in / gqa = in * inv_gqa >> 16 for in below 128, gqa up to 16; log2 of a slice's items */
         for (uint32_t s0 = s_begin; s0 < s_end; s0 += at_once) {
             const uint32_t n_s = min(at_once, s_end - s0), items = n_s * (wide / 4u), padded = (items + 31u) & ~31u, groups = padded < THREADS ? THREADS / padded : 1u;
             float *s_rec = s_gate + (P.gate ? n_s * wide : 0u);              /* [record][slice][its dims, m, l, -, -] */
             /* token and head of a slice's row; false: a row without a token */
             auto place = [&](uint32_t s, uint32_t &tok, uint32_t &head) -> bool {
-                const uint32_t row = (s0 + s) >> cut, tg = row / P.group_rows, in = row - tg * P.group_rows, tl = in / P.gqa;
+                const uint32_t row = (s0 + s) >> cut, tg = row >> 7, in = row & 127u, tl = in * inv_gqa >> 16;
                 tok = tg * P.tpg + tl;
                 head = u.kh * P.gqa + in - tl * P.gqa;
                 const bool live = tl < P.tpg && tok < u.n_here;
@@ -244,7 +245,7 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
             bring(0u, recs_at_once < k ? recs_at_once : k, P.gate != nullptr);
             for (uint32_t item0 = 0; item0 < items; item0 += groups > 1u ? padded : THREADS) {
                 const uint32_t group = groups > 1u ? tid / padded : 0u, item = item0 + (groups > 1u ? tid - group * padded : tid);
-                const uint32_t s = item / (wide / 4u), d = item % (wide / 4u) * 4u;
+                const uint32_t s = item >> per_slice, d = (item & ((1u << per_slice) - 1u)) * 4u;
                 uint32_t tok, head;
                 const bool live = item < items && group < groups && place(s, tok, head);
                 float M = -CUDART_INF_F, L = 0.f;

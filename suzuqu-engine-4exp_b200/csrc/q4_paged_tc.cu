@@ -1089,7 +1089,6 @@ bool chunk(PagedParams p, float *scratch) {
     if (blocks > PG_MAX_BLOCKS) return q4i_fail(Q4E_CUDA, "pages_attend: more SMs than the counters are for");
     p.part = scratch;
     p.tpg = 128u / p.gqa;
-    p.group_rows = 128u;
     static uint32_t *meet = nullptr;
     if (!meet && !q4i_check(cudaGetSymbolAddress((void **)&meet, g_chunk_meet), "pages_attend counters")) return false;
     p.meet = meet;
