@@ -156,10 +156,13 @@ def _ptr(t):
         return t.ctypes.data
 
 
-def _dense(*tensors):
-    for t in tensors:
-        if t is not None and not t.is_contiguous():
-            raise RuntimeError("a dense tensor is needed, not one with strides %s" % (t.stride(),))
+def _dense(t, dtype):
+    """address of a dense tensor of that type; None stays None"""
+    if t is None:
+        return None
+    if t.dtype is not dtype or not t.is_contiguous():
+        raise RuntimeError("a dense tensor of %s is needed, not one of %s with strides %s" % (dtype, t.dtype, t.stride()))
+    return t.data_ptr()
 
 
 def check(ok, what):
@@ -421,36 +424,37 @@ class PagePool:
         self.n_layers, self.n_kvh, self.hd, self.n_pages, self.page_rows, self.kind = n_layers, n_kvh, hd, n_pages, page_rows, kind
         self.desc = PagesDesc(_ptr(mem), _ptr(free), _ptr(n_free), n_layers, n_kvh, hd, n_pages, page_rows, kind)
         self.p = C.addressof(self.desc)
+        self.calls = [getattr(self.L, "q4_gpu_pages_" + name) for name in ("plan", "trim", "append", "gather", "attend")]
+        self.i32, self.f32, self.bf16 = torch.int32, torch.float32, torch.bfloat16
+
+    # a call costs the host as much as a small launch the device: addresses are taken once, functions looked up above
 
     def plan(self, rows, add, table, start, slot, pos, req):
         """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok]"""
-        _dense(rows, add, table, start, slot, pos, req)
-        n, stride = table.shape
-        check(self.L.q4_gpu_pages_plan(self.p, _ptr(rows), _ptr(add), n, _ptr(table), stride, _ptr(start), _ptr(slot), _ptr(pos),
-                                       _ptr(req), slot.shape[0]), "q4_gpu_pages_plan")
+        i, (n, stride) = self.i32, table.shape
+        if not self.calls[0](self.p, _dense(rows, i), _dense(add, i), n, _dense(table, i), stride, _dense(start, i), _dense(slot, i), _dense(pos, i), _dense(req, i), slot.shape[0]):
+            check(False, "q4_gpu_pages_plan")
 
     def trim(self, rows, keep, table):
         """the pages behind the first keep[r] of rows[r] rows go back"""
-        _dense(rows, keep, table)
-        n, stride = table.shape
-        check(self.L.q4_gpu_pages_trim(self.p, _ptr(rows), _ptr(keep), n, _ptr(table), stride), "q4_gpu_pages_trim")
+        i, (n, stride) = self.i32, table.shape
+        if not self.calls[1](self.p, _dense(rows, i), _dense(keep, i), n, _dense(table, i), stride):
+            check(False, "q4_gpu_pages_trim")
 
     def append(self, layer, k, v, slot):
         """k, v [slot.shape[0]][n_kvh * hd] fp32; slots below 0 are skipped"""
-        _dense(k, v, slot)
-        check(self.L.q4_gpu_pages_append(self.p, layer, _ptr(k), _ptr(v), _ptr(slot), slot.shape[0]), "q4_gpu_pages_append")
+        if not self.calls[2](self.p, layer, _dense(k, self.f32), _dense(v, self.f32), _dense(slot, self.i32), slot.shape[0]):
+            check(False, "q4_gpu_pages_append")
 
     def gather(self, layer, slot, k, v):
         """the rows of the slots as fp32, the reverse of append; k or v may be None"""
-        _dense(slot, k, v)
-        check(self.L.q4_gpu_pages_gather(self.p, layer, _ptr(slot), slot.shape[0], _ptr(k), _ptr(v)), "q4_gpu_pages_gather")
+        if not self.calls[3](self.p, layer, _dense(slot, self.i32), slot.shape[0], _dense(k, self.f32), _dense(v, self.f32)):
+            check(False, "q4_gpu_pages_gather")
 
     def attend(self, layer, q, out, rows, start, table, n_head, scale, gate=None, max_add=0):
         """attention of the step's tokens: q, out [n_tok][n_head][hd], bf16 or fp32; rows as they were given to plan"""
-        import torch
-        _dense(q, out, rows, start, table, gate)
-        n, stride = table.shape
-        n_tok = q.numel() // (n_head * self.hd)
-        check(self.L.q4_gpu_pages_attend(self.p, layer, _ptr(q), q.dtype == torch.bfloat16, _ptr(gate), _ptr(out),
-                                         out.dtype == torch.bfloat16, n_head, _ptr(rows), _ptr(start), n, n_tok, _ptr(table), stride,
-                                         max_add, scale), "q4_gpu_pages_attend")
+        i, (n, stride) = self.i32, table.shape
+        q_bf16, out_bf16 = q.dtype is self.bf16, out.dtype is self.bf16
+        if not self.calls[4](self.p, layer, _dense(q, self.bf16 if q_bf16 else self.f32), q_bf16, _dense(gate, self.f32), _dense(out, self.bf16 if out_bf16 else self.f32),
+                             out_bf16, n_head, _dense(rows, i), _dense(start, i), n, q.numel() // (n_head * self.hd), _dense(table, i), stride, max_add, scale):
+            check(False, "q4_gpu_pages_attend")

@@ -341,4 +341,9 @@ def test_dense_tensors_only():
         s.pool.plan(s.d_rows, s.d_add, s.d_table.t(), s.start, s.slot, s.pos, s.req)
     with pytest.raises(RuntimeError, match="dense"):
         s.pool.trim(s.d_rows, s.d_rows, s.d_table[:, ::2])
+    for q2, out2, rows in ((q[:, :16].half().contiguous(), out, s.d_rows), (q[:, :16].contiguous(), out.double(), s.d_rows), (q[:, :16].contiguous(), out, s.d_rows.long())):
+        with pytest.raises(RuntimeError, match="dense tensor of"):
+            s.pool.attend(0, q2, out2, rows, s.start, s.d_table, 16, 0.1)
+    with pytest.raises(RuntimeError, match="dense tensor of"):
+        s.pool.append(0, k[:, :256].to(torch.bfloat16).contiguous(), k[:, :256].contiguous(), s.slot[:2])
     assert lib().q4_gpu_last_error() == 0
