@@ -846,37 +846,35 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
             const bool active = g == 0u || p.n_here > P.tpg;
             /* ---- queries as fp16, swizzled rows of 64 dims: the products of the piece before have read theirs (its last scores are here) */
             {
-                constexpr uint32_t PER = HD / 8u, T = NQ == 2u ? 128u : 256u, STEPS = 128u * PER / T, BATCH = 8u;   /* loads in flight before the first store */
-                const uint32_t qt = NQ == 2u ? r : tid;
+                /* a thread keeps its 8 dims and goes down the rows, 8 or 16 at a time: its places in the swizzled tiles lie in line */
+                constexpr uint32_t PER = HD / 8u, T = NQ == 2u ? 128u : 256u, DOWN = T / PER, STEPS = 128u / DOWN, BATCH = 8u;   /* loads in flight before the first store */
+                static_assert(DOWN % 8u == 0u && STEPS % BATCH == 0u, "queries by rows");
+                const uint32_t qt = NQ == 2u ? r : tid, c = qt % PER, row0 = qt / PER, elem = P.q_bf16 ? 2u : 4u;
                 if (active) {
+                    const uint8_t *src = reinterpret_cast<const uint8_t *>(P.q) + (((size_t)(p.tok0 + g * P.tpg) * P.n_head + (size_t)p.kh * P.gqa) * HD + c * 8u) * elem;
+                    const uint32_t a = sQ + g * C::QG + (c >> 3) * 16384u + row0 * 128u + (((c & 7u) ^ (row0 & 7u)) << 4), n_q = min(P.tpg, p.n_here - g * P.tpg), skip = P.n_head - P.gqa;
 #pragma unroll 1
                     for (uint32_t k0 = 0; k0 < STEPS; k0 += BATCH) {
                         uint4 w[BATCH][2];
 #pragma unroll
                         for (uint32_t k = 0; k < BATCH; k++) {
-                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER, ql = row * inv_gqa >> 16, qtok = g * P.tpg + ql;
+                            const uint32_t row = row0 + (k0 + k) * DOWN, ql = row * inv_gqa >> 16;
                             w[k][0] = w[k][1] = make_uint4(0u, 0u, 0u, 0u);
-                            if (ql < P.tpg && qtok < p.n_here) {
-                                const size_t off = ((size_t)(p.tok0 + qtok) * P.n_head + (size_t)p.kh * P.gqa + (row - ql * P.gqa)) * HD + c * 8u;
-                                if (P.q_bf16) {
-                                    w[k][0] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + off);
-                                } else {
-                                    w[k][0] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(P.q) + off);
-                                    w[k][1] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(P.q) + off + 4);
-                                }
+                            if (ql < n_q) {
+                                const uint4 *x = reinterpret_cast<const uint4 *>(src + (uint64_t)(ql * skip + row) * (HD * elem));   /* ql whole tokens and the row's head */
+                                w[k][0] = *x;
+                                if (!P.q_bf16) w[k][1] = x[1];
                             }
                         }
 #pragma unroll
                         for (uint32_t k = 0; k < BATCH; k++) {
-                            const uint32_t i = qt + (k0 + k) * T, row = i / PER, c = i % PER;
                             const uint32_t in[8] = {w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w, w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w};
                             uint32_t o[4];
 #pragma unroll
                             for (int e = 0; e < 4; e++)
                                 o[e] = P.q_bf16 ? h2u(__floats2half2_rn(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u)))
                                                 : h2u(__floats2half2_rn(__uint_as_float(in[2 * e]), __uint_as_float(in[2 * e + 1])));
-                            const uint32_t a = sQ + g * C::QG + (c >> 3) * 16384u + row * 128u + (((c & 7u) ^ (row & 7u)) << 4);
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a + (k0 + k) * (DOWN * 128u)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
                         }
                     }
                 }
