@@ -145,7 +145,10 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     if (lane == 0)
         for (uint32_t i = 0; i < DEPTH; i++) bar_init(bars + 8u * i, 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    q4d_pdl_wait();
+    /* Beside the chunks of its own call it takes the SMs that they leave: that launch began behind everything before it, and nothing
+     * here reads what it writes (a mixed step 278 -> 256 us).  What it reads may be two launches old: by loads that do not look into L1.  The
+     * end of that launch is waited for at the end, for those behind this one. */
+    if (!P.beside) q4d_pdl_wait();
 
     /* ---- this block's share of all steps */
     auto mine_of = [&](uint32_t r, bool &bad) -> PgReq {
@@ -192,7 +195,10 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     PgShares shares;
     shares.set(total, extra, extra ? 8u : 3u, extra ? 4u : 1u);
-    if (blockIdx.x >= shares.blocks) return;
+    if (blockIdx.x >= shares.blocks) {
+        if (P.beside) q4d_pdl_wait();
+        return;
+    }
     if (tid == 0) {
         s_end2[0] = s_end2[1] = total;
         s_shares = shares;
@@ -256,8 +262,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         const uint32_t tiles = (n_kv + 15u) / 16u;
         uint32_t n_my = 0;
         if (ok && st * WARPS + warp < tiles) n_my = min(here, (tiles - 1u - st * WARPS - warp) / WARPS + 1u);
-        const int32_t *tab = P.table + (size_t)req * P.table_stride;
-        auto entry = [&](uint32_t i) -> int32_t { return i < n_my ? tab[(((st + i) * WARPS + warp) * 16u) >> P.page_shift] : 0; };
+        auto entry = [&](uint32_t i) -> int32_t { return i < n_my ? __ldcg(P.table + (size_t)req * P.table_stride + ((((st + i) * WARPS + warp) * 16u) >> P.page_shift)) : 0; };
         int32_t cur = -1, nxt = entry(lane);
         uint32_t dead = 0, dead_nxt = 0;   /* tiles of the present / the next 32 whose page is not the pool's */
         const uint8_t *src = P.mem;
@@ -295,10 +300,10 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
             if (row < live_rows) {
                 const size_t at = ((size_t)(tok0 + row / P.gqa) * P.n_head + kh * P.gqa + row % P.gqa) * HD + d;
                 if (P.q_bf16) {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + at);
+                    const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(P.q) + at));
                     x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
                 } else {
-                    x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(P.q) + at);
+                    x = __ldcg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(P.q) + at));
                 }
             }
             const uint32_t lo = h2u(__floats2half2_rn(x.x, x.y)), hi = h2u(__floats2half2_rn(x.z, x.w)), a = s_q + row * C::Q_STRIDE;
@@ -633,7 +638,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                 join(ml.x, ml.y, *reinterpret_cast<const float4 *>(r2 + d));
             }
             if (whole) {
-                pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
+                pg_store<HD, true>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
             } else {
                 *reinterpret_cast<float4 *>(part + row * C::REC + d) = A;
                 if (d == 0u) *reinterpret_cast<float2 *>(part + row * C::REC + HD) = make_float2(M, L);
@@ -669,7 +674,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                             for (uint32_t b = 0; b < BATCH; b++)
                                 if (c0 + b <= last) join(ml[b].x, ml[b].y, x[b]);
                         }
-                        pg_store<HD>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
+                        pg_store<HD, true>(P, tok0 + row / P.gqa, kh * P.gqa + row % P.gqa, d, A, L, gate_of(row, d));
                     }
                 }
             } else if (tid == 0) {
@@ -734,7 +739,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
             __syncthreads();
             if (tid < 8u) {
                 for (uint32_t w = 1; w < WARPS; w++) join(s_ml[w * 8u + tid].x, s_ml[w * 8u + tid].y, s_a[w * 8u + tid]);
-                pg_store<HD>(P, u.tok0 + row / P.gqa, u.kh * P.gqa + row % P.gqa, d, A, L, gate);
+                pg_store<HD, true>(P, u.tok0 + row / P.gqa, u.kh * P.gqa + row % P.gqa, d, A, L, gate);
             }
         }
         pg_leave(P, u, joiners);
@@ -744,6 +749,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         for (; taken < issued; taken++)
             for (uint32_t i = 0; i < 4096u && !bar_test(bars + 8u * (taken % DEPTH), (taken / DEPTH) & 1u); i++) {}
     }
+    if (P.beside) q4d_pdl_wait();
 }
 
 template <int KIND, int HD, int NT>
@@ -837,6 +843,7 @@ extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, cons
             return false;
         }
         if (n_req == 1u) return true;
+        p.beside = 1u;
         scratch = g_q4.part + chunk;
     }
     if (pg->kind == Q4K_Q8)

@@ -26,6 +26,7 @@ struct PagedParams {
     uint32_t *err;
     const uint32_t *fits;        /* not NULL: the launch has work only if this word is `fits_is` (q4i_paged_stage's) */
     uint32_t fits_is;
+    uint32_t beside;             /* q4_pg_few_k behind q4_pg_chunk_k of the same call: it need not wait for that one's end */
 };
 
 template <int KIND, int HD>
@@ -49,7 +50,7 @@ bool q4i_paged_stage(const PagedParams &p, uint32_t hd, uint8_t *to, int32_t *ta
 /* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */
 struct PgReq { uint32_t held, add, tok0; };
 __device__ __forceinline__ PgReq pg_request(const PagedParams &P, uint32_t r, bool &bad) {
-    const int32_t s0 = P.start[r], s1 = P.start[r + 1u], h = P.rows[r];
+    const int32_t s0 = __ldcg(P.start + r), s1 = __ldcg(P.start + r + 1u), h = __ldcg(P.rows + r);
     PgReq q = {0u, 0u, 0u};
     bad = false;
     if (s1 <= s0) return q;
@@ -65,14 +66,14 @@ __device__ __forceinline__ float pg_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-/* four dims of a row: acc / l * sigmoid(gate), where there are gates.  A row that attended nothing is 0, one with a NaN among its scores stays NaN */
-template <int HD>
+/* four dims of a row: acc / l * sigmoid(gate), where there are gates (LDCG: in global memory).  A row that attended nothing is 0, one with a NaN among its scores stays NaN */
+template <int HD, bool LDCG = false>
 __device__ __forceinline__ void pg_store(const PagedParams &P, uint32_t tok, uint32_t head, uint32_t d, float4 x, float L, const float *gate) {
     const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
     const size_t at = ((size_t)tok * P.n_head + head) * HD + d;
     x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
     if (gate) {
-        const float4 gt = *reinterpret_cast<const float4 *>(gate);
+        const float4 gt = LDCG ? __ldcg(reinterpret_cast<const float4 *>(gate)) : *reinterpret_cast<const float4 *>(gate);
         x.x *= 1.f / (1.f + __expf(-gt.x)); x.y *= 1.f / (1.f + __expf(-gt.y));
         x.z *= 1.f / (1.f + __expf(-gt.z)); x.w *= 1.f / (1.f + __expf(-gt.w));
     }

@@ -11,9 +11,9 @@ from test_gpu_pages import KINDS, Step, attend_exact, ints, run_attend
 pytestmark = pytest.mark.gpu
 
 
-def step_of(rows, add, kind, n_kvh, hd, page=16, seed=0):
+def step_of(rows, add, kind, n_kvh, hd, page=16, seed=0, n_pages=None):
     """requests whose rows are normal numbers, the step's own k and v not appended yet: (step, k, v)"""
-    s = Step(rows, add, page, n_kvh=n_kvh, hd=hd, kind=KINDS[kind], seed=seed)
+    s = Step(rows, add, page, n_pages, n_kvh=n_kvh, hd=hd, kind=KINDS[kind], seed=seed)
     g = torch.Generator(device="cuda").manual_seed(seed)
     slot = [s.table[r][p // page] * page + p % page for r, h in enumerate(rows) for p in range(h)]
     if slot:
@@ -187,6 +187,30 @@ def test_requests_that_share_pages(kind, add):
         at = r * add
         want = attend_exact(q[at: at + add], kr.view(-1, n_kvh, hd), vr.view(-1, n_kvh, hd), None, h, float(hd ** -0.5))
         assert ((out[at: at + add].double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+
+
+@pytest.mark.parametrize("kind,n_pages", [("f16", 2600), ("q8_0", 4700)])
+@pytest.mark.parametrize("add", [[1, 1, 1], [3, 70, 1], [1, 1, 1200]])
+def test_a_pool_of_more_than_4_gb(kind, n_pages, add):
+    """pages of 2 and 1.1 MB anywhere in it"""
+    n_head, n_kvh, hd, page, rows = 64, 8, 256, 256, [3000, 700, 5]
+    s, k, v = step_of(rows, add, kind, n_kvh, hd, page, n_pages=n_pages)
+    n = sum(add)
+    assert s.pool.mem.numel() > 1 << 32 and int(s.d_table.max()) * (s.pool.mem.numel() // n_pages) > 1 << 32
+    s.pool.append(0, k, v, s.slot[:n])
+    q = torch.randn(n, n_head, hd, device="cuda").to(torch.bfloat16)
+    out = torch.empty(n, n_head, hd, device="cuda")
+    s.pool.attend(0, q, out, s.d_rows, s.start, s.d_table, n_head, float(hd ** -0.5))
+    assert lib().q4_gpu_last_error() == 0
+    at = 0
+    for r, (h, m) in enumerate(zip(rows, add)):
+        table = s.d_table[r].tolist()
+        kr, vr = torch.empty(2, h + m, n_kvh * hd, device="cuda")
+        s.pool.gather(0, ints([table[p // page] * page + p % page for p in range(h + m)]), kr, vr)
+        assert torch.isfinite(kr).all() and (kr[h:] - k[at: at + m]).abs().max() < 4 / 127     # where append put them
+        want = attend_exact(q[at: at + m], kr.view(-1, n_kvh, hd), vr.view(-1, n_kvh, hd), None, h, float(hd ** -0.5))
+        assert ((out[at: at + m].double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+        at += m
 
 
 def test_rows_behind_the_step_s_tokens_are_left_alone():
