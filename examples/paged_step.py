@@ -1,10 +1,13 @@
 """A serving loop on the paged KV cache: chats come and go, and every step takes the next piece of each prompt and one token of each
 chat that answers, in one plan, and one append and one attention per layer.
 
-    python examples/paged_step.py [--layers 4] [--chats 12] [--steps 40] [--kind q8_0]
+    python examples/paged_step.py [--layers 4] [--chats 12] [--steps 40] [--pages 512] [--kind q8_0]
 
-Queries, keys and values are random, as there is no model here; every --check steps a layer's outputs are compared with softmax(q k) v
-in 64 bits over the rows that the pool holds.  Prints the tokens served and the time of a step.
+A plan serves the chats up to the first one that does not fit: a chat has as many rows more as `start` says that it was served, and where
+pages ran out the last chat that holds any gives them back and begins again.
+
+Queries, keys and values are random, as there is no model here; every --check steps the rows that the pool holds are compared with the ones
+that each chat was given, and a layer's outputs with softmax(q k) v in 64 bits over them.  Prints the tokens served and the time of a step.
 """
 import argparse
 import os
@@ -25,10 +28,12 @@ class Loop:
         self.pool = q4gpu.PagePool(layers, n_kvh, hd, n_pages, page_rows, kind)
         self.rng, self.gen = random.Random(seed), torch.Generator(device="cuda").manual_seed(seed)
         word = dict(dtype=torch.int32, device="cuda")
-        self.table = torch.full((places, n_pages // 4), -1, **word)
+        self.table = torch.full((places, max(n_pages // 4, -(-640 // page_rows))), -1, **word)
         self.start = torch.zeros(places + 1, **word)
         self.slot, self.pos, self.req = (torch.zeros(max_tok, **word) for _ in range(3))
         self.held, self.prompt, self.answer = [0] * places, [0] * places, [0] * places    # rows in the pool; tokens still to come
+        self.given = [[] for _ in range(places)]                                          # the last layer's K and V of the rows in the pool
+        self.again = 0                                                                    # chats that had to begin again
 
     def words(self, values):
         return torch.tensor(values, dtype=torch.int32).pin_memory().to("cuda", non_blocking=True)
@@ -53,38 +58,53 @@ class Loop:
             out = torch.empty_like(q)
             self.pool.append(layer, k, v, self.slot[:n_tok])
             self.pool.attend(layer, q, out, rows, self.start, self.table, self.n_head, self.hd**-0.5, max_add=max(add))
+        start = self.start.tolist()                                                              # a host waits here for the new tokens in any case
+        status = q4gpu.load().q4_gpu_last_error()
+        if status & ~8:                                                                          # 8: not all were served
+            raise RuntimeError("a step's status is 0x%x" % status)
+        got = [b - a for a, b in zip(start, start[1:])]
+        for r, n in enumerate(got):
+            if n:
+                self.given[r].append((k[start[r]: start[r + 1]], v[start[r]: start[r + 1]]))
         if check:
-            self.check(q, out, add)
-        self.held = [h + n for h, n in zip(self.held, add)]
-        keep = []
-        for r, n in enumerate(add):
+            self.check(q, out, start)
+        rows = self.held = [h + n for h, n in zip(self.held, got)]
+        for r, n in enumerate(got):
             if self.prompt[r]:
                 self.prompt[r] -= n
             else:
                 self.answer[r] -= n
-            keep.append(self.held[r] if self.prompt[r] + self.answer[r] else 0)                  # a chat that is over gives its pages back
-        if keep != self.held:
-            self.pool.trim(self.words(self.held), self.words(keep), self.table)
+        keep = [h if p + a else 0 for h, p, a in zip(rows, self.prompt, self.answer)]            # a chat that is over gives its pages back
+        if status & 8 and keep == rows:
+            last = max(r for r, h in enumerate(rows) if h)
+            self.prompt[last], keep[last] = self.prompt[last] + rows[last], 0
+            self.again += 1
+        if keep != rows:
+            self.pool.trim(self.words(rows), self.words(keep), self.table)
+            self.given = [g if h else [] for g, h in zip(self.given, keep)]
             self.held = keep
-        return n_tok
+        return start[-1]
 
-    def check(self, q, out, add):
-        """the last layer's outputs, request by request"""
-        at = 0
-        for r, (h, n) in enumerate(zip(self.held, add)):
+    def check(self, q, out, start):
+        """the last layer's rows and outputs, request by request"""
+        for r, h in enumerate(self.held):
+            at, n = start[r], start[r + 1] - start[r]
             if n == 0:
                 continue
             p = torch.arange(h + n, device="cuda")
             slot = (self.table[r].long()[p // self.page_rows] * self.page_rows + p % self.page_rows).int()
             k, v = torch.empty(2, h + n, self.n_kvh * self.hd, device="cuda")
             self.pool.gather(self.layers - 1, slot, k, v)
+            for x, mine in zip((k, v), zip(*self.given[r])):
+                mine = torch.cat(mine)
+                # codes are half of amax / 127 off, their scale 2^-11 of itself (127 codes of it: 0.06)
+                assert ((x - mine).abs() <= 0.6 / 127 * mine.abs().max()).all(), "rows of request %d" % r
             k, v = (x.view(-1, self.n_kvh, self.hd).double().repeat_interleave(self.n_head // self.n_kvh, 1) for x in (k, v))
             w = torch.einsum("thd,phd->htp", q[at: at + n].double(), k) * self.hd**-0.5
             w = w.masked_fill(p > h + torch.arange(n, device="cuda")[:, None], -torch.inf)
             want = torch.einsum("htp,phd->thd", torch.softmax(w, -1), v)
             # 2e-3 + 1e-3 |o| of the attention, 2^-8 of a bf16 output
             assert ((out[at: at + n].double() - want).abs() <= 2e-3 + (1e-3 + 2.0**-8) * want.abs()).all(), "request %d" % r
-            at += n
 
     def end(self):
         """all chats end; whether every page came back once"""
@@ -99,9 +119,10 @@ def main(argv=None):
     a.add_argument("--chats", type=int, default=12)
     a.add_argument("--steps", type=int, default=40)
     a.add_argument("--check", type=int, default=5, metavar="N")
+    a.add_argument("--pages", type=int, default=512, help="of 64 rows; a chat alone takes up to 10")
     a.add_argument("--kind", choices=("q8_0", "f16"), default="q8_0")
     a = a.parse_args(argv)
-    loop = Loop(a.layers, a.chats, kind=q4gpu.KIND_Q8 if a.kind == "q8_0" else q4gpu.KIND_F16)
+    loop = Loop(a.layers, a.chats, n_pages=a.pages, kind=q4gpu.KIND_Q8 if a.kind == "q8_0" else q4gpu.KIND_F16)
     times, tokens, checked = [], 0, 0
     for i in range(a.steps):
         begin, end = torch.cuda.Event(True), torch.cuda.Event(True)
@@ -116,8 +137,8 @@ def main(argv=None):
     ms = sorted(b.elapsed_time(e) for b, e in times)
     status = q4gpu.load().q4_gpu_last_error()
     back = loop.end()
-    print("%d tokens in %d steps of %d layers, %.3f ms per step (median); %d steps checked; status %d; pages back: %s"
-          % (tokens, a.steps, a.layers, ms[len(ms) // 2] if ms else 0.0, checked, status, back))
+    print("%d tokens in %d steps of %d layers, %.3f ms per step (median); %d steps checked; status %d; pages back: %s; begun again: %d"
+          % (tokens, a.steps, a.layers, ms[len(ms) // 2] if ms else 0.0, checked, status, back, loop.again))
     return 0 if back and status == 0 else 1
 
 

@@ -483,7 +483,9 @@ uint64_t q4_gpu_pages_bytes(uint32_t n_layers, uint32_t n_kvh, uint32_t hd, uint
  * are the exclusive sums of the tokens; token t = start[r] + j has req[t] = r, pos[t] = rows[r] + j and slot[t] = page * page_rows +
  * row in the page.  slot, pos and req have max_tok entries; those behind the step's tokens are -1.  Requests are served up to the
  * first one that does not fit (pages left, max_tok): it and those behind it get nothing (their start does not move) and status bit
- * 8 is set.  A request that would pass its table's row (or rows < 0) gets nothing and sets status bit 4.  n_req <= 8192. */
+ * 8 is set.  A request that would pass its table's row (or rows < 0) gets nothing and sets status bit 4.  n_req <= 8192.
+ * The next step's rows[r] are these plus start[r + 1] - start[r], what was served, never plus add[r]: the table's entries behind a
+ * request's rows are leftovers of earlier requests and may be others' pages by now, which nothing here can tell. */
 bool q4_gpu_pages_plan(const q4_gpu_pages *pg, const int32_t *rows, const int32_t *add, uint32_t n_req, int32_t *table,
                        uint32_t table_stride, int32_t *start, int32_t *slot, int32_t *pos, int32_t *req, uint32_t max_tok);
 /* Request r, which holds rows[r] rows, keeps the first keep[r] of them (0 or less: none): the pages behind those go back on the

@@ -430,7 +430,8 @@ class PagePool:
     # a call costs the host as much as a small launch the device: addresses are taken once, functions looked up above
 
     def plan(self, rows, add, table, start, slot, pos, req):
-        """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok]"""
+        """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok].  Request r
+        then holds start[r + 1] - start[r] rows more: all of add[r], or none where pages or max_tok ran out"""
         i, (n, stride) = self.i32, table.shape
         if not self.calls[0](self.p, _dense(rows, i), _dense(add, i), n, _dense(table, i), stride, _dense(start, i), _dense(slot, i), _dense(pos, i), _dense(req, i), slot.shape[0]):
             check(False, "q4_gpu_pages_plan")
