@@ -490,7 +490,7 @@ bool q4_gpu_pages_plan(const q4_gpu_pages *pg, const int32_t *rows, const int32_
                        uint32_t table_stride, int32_t *start, int32_t *slot, int32_t *pos, int32_t *req, uint32_t max_tok);
 /* Request r, which holds rows[r] rows, keeps the first keep[r] of them (0 or less: none): the pages behind those go back on the
  * stack, in the order in which a plan that is taken back took them.  Table entries stay as they are.  More pages than are out
- * (one given back twice): nothing is done, status bit 4. */
+ * (one given back twice), or an entry that is no page of the pool: no page goes back, status bit 4. */
 bool q4_gpu_pages_trim(const q4_gpu_pages *pg, const int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table,
                        uint32_t table_stride);
 /* k, v [n_tok][n_kvh * hd] fp32: row t of one layer into slot[t] (below 0: skipped; beyond the pool: skipped, status bit 4),

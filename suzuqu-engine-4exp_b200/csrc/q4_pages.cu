@@ -16,7 +16,7 @@ namespace {
 
 constexpr uint32_t PLAN_THREADS = 512, PLAN_MAX_REQ = 8192;
 
-/* blocks of a launch that have finished; zero between launches */
+/* blocks of a launch that have finished, in the upper half those that want the stack left alone; zero between launches */
 __device__ uint32_t g_plan_arrived;
 
 struct PlanParams {
@@ -51,14 +51,16 @@ __device__ __forceinline__ void block_scan2(uint64_t &a, uint64_t &b, uint64_t &
     b += pb - b0;
 }
 
-/* the last block to finish moves the stack's top: all of them have read it by then */
-__device__ __forceinline__ void move_top(int32_t *n_free, int32_t to) {
-    __syncthreads();
+/* the last block to finish moves the stack's top, unless a thread of any block says no: all of them have read it by then */
+__device__ __forceinline__ void move_top(int32_t *n_free, int32_t to, uint32_t *err, bool no = false) {
+    const bool stays = __syncthreads_or(no);
     if (threadIdx.x == 0) {
         __threadfence();
-        if (atomicAdd(&g_plan_arrived, 1u) == gridDim.x - 1u) {
+        const uint32_t mine = stays ? 0x10001u : 1u, all = atomicAdd(&g_plan_arrived, mine) + mine;
+        if ((all & 0xffffu) == gridDim.x) {
             g_plan_arrived = 0u;
-            *n_free = to;
+            if (all >> 16) atomicOr(err, (uint32_t)Q4E_RANGE);
+            else *n_free = to;
         }
     }
 }
@@ -163,11 +165,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_plan_k(const PlanParams P)
             }
         }
     }
-    move_top(P.n_free, (int32_t)(n_free - pages));
+    move_top(P.n_free, (int32_t)(n_free - pages), P.err);
 }
 
 /* Trim: pages ceil(kept / P) .. ceil(held / P) of every request go back, the last one of all lowest, so that a plan that is
- * taken back leaves the stack as it was. */
+ * taken back leaves the stack as it was.  An entry that is no page of the pool (rows that no plan served) leaves all of them out: on the
+ * stack it would be handed out in place of a page. */
 __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_trim_k(const PlanParams P) {
     extern __shared__ uint32_t s_plan[];
     uint32_t *page_end = s_plan;
@@ -197,6 +200,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_trim_k(const PlanParams P)
     const bool fits = n_free + all <= P.n_pages;   /* else a page would come back twice */
     if (blockIdx.x == 0 && (any_bad || (tid == 0 && !fits))) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     __syncthreads();
+    bool no_page = false;
     if (fits) {
         for (uint64_t i = (uint64_t)blockIdx.x * PLAN_THREADS + tid; i < all; i += (uint64_t)gridDim.x * PLAN_THREADS) {
             uint32_t lo = 0, hi = P.n_req - 1u;
@@ -208,10 +212,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_trim_k(const PlanParams P)
             const int32_t h = __ldcg(P.rows + lo);
             /* counted from the request's end */
             const uint32_t pg = (((uint32_t)h + mask) >> P.page_shift) - (page_end[lo] - (uint32_t)i);
-            P.free_list[n_free + all - 1u - i] = P.table[(size_t)lo * P.table_stride + pg];
+            const int32_t page = P.table[(size_t)lo * P.table_stride + pg];
+            no_page |= (uint32_t)page >= P.n_pages;
+            P.free_list[n_free + all - 1u - i] = page;   /* above the top: of no meaning until that moves */
         }
     }
-    move_top(P.n_free, fits ? (int32_t)(n_free + all) : top);
+    move_top(P.n_free, fits ? (int32_t)(n_free + all) : top, P.err, no_page);
 }
 
 struct RowParams {
