@@ -156,12 +156,13 @@ def _ptr(t):
         return t.ctypes.data
 
 
-def _dense(t, dtype):
-    """address of a dense tensor of that type; None stays None"""
+def _dense(t, dtype, n, gpu):
+    """address of a dense tensor of that type, of n numbers or more, on that GPU; None stays None"""
     if t is None:
         return None
-    if t.dtype is not dtype or not t.is_contiguous():
-        raise RuntimeError("a dense tensor of %s is needed, not one of %s with strides %s" % (dtype, t.dtype, t.stride()))
+    if t.dtype is not dtype or t.numel() < n or t.get_device() != gpu or not t.is_contiguous():
+        raise RuntimeError("a dense tensor of %s on GPU %d with %d numbers is needed, not one of %s on %s, %s with strides %s"
+                           % (dtype, gpu, n, t.dtype, t.device, tuple(t.shape), t.stride()))
     return t.data_ptr()
 
 
@@ -403,8 +404,9 @@ class Batch:
 
 
 class PagePool:
-    """A paged KV cache for many requests (q4_gpu_pages_*).  Arrays are dense torch tensors on the device; the pool's memory and its
-    stack of free pages are allocated here unless they are given.  Per step: plan, then append and attend for every layer."""
+    """A paged KV cache for many requests (q4_gpu_pages_*).  Arrays are dense torch tensors on the library's GPU, others are refused
+    (RuntimeError), as are ones too small for the call; the pool's memory and its stack of free pages are allocated here unless they
+    are given.  Per step: plan, then append and attend for every layer."""
 
     def __init__(self, n_layers, n_kvh, hd, n_pages, page_rows=64, kind=KIND_Q8, mem=None, free=None, n_free=None):
         import torch
@@ -412,18 +414,22 @@ class PagePool:
         size = self.L.q4_gpu_pages_bytes(n_layers, n_kvh, hd, n_pages, page_rows, kind)
         if not size:
             raise RuntimeError("q4_gpu_pages_bytes: a pool of kind f16 or q8_0, hd 64 / 128 / 256, page_rows 16 .. 256 is needed")
-        on = torch.device("cuda", self.L.q4_gpu_device())
-        own_mem = free is None and mem is None
+        self.gpu = gpu = self.L.q4_gpu_device()
+        on = torch.device("cuda", gpu)
+        own_mem = free is None and mem is None and n_free is None
         if own_mem:
             mem = torch.empty(size, dtype=torch.uint8, device=on)
             free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=on)   # page 0 is on top
             n_free = torch.full((1,), n_pages, dtype=torch.int32, device=on)
+        if (free is None) != (n_free is None):
+            raise RuntimeError("the stack of free pages and its height go together")
         if mem is not None and mem.numel() * mem.element_size() < size:
             raise RuntimeError("the pool's memory is smaller than q4_gpu_pages_bytes (%d)" % size)
         self.mem, self.free, self.n_free = mem, free, n_free
         self.n_layers, self.n_kvh, self.hd, self.n_pages, self.page_rows, self.kind = n_layers, n_kvh, hd, n_pages, page_rows, kind
-        self.desc = PagesDesc(_ptr(mem), _ptr(free), _ptr(n_free), n_layers, n_kvh, hd, n_pages, page_rows, kind)
-        self.p = C.addressof(self.desc)
+        at = (_dense(mem, None if mem is None else mem.dtype, 1, gpu), _dense(free, torch.int32, n_pages, gpu), _dense(n_free, torch.int32, 1, gpu))
+        self.desc = PagesDesc(*at, n_layers, n_kvh, hd, n_pages, page_rows, kind)
+        self.p, self.width = C.addressof(self.desc), n_kvh * hd
         self.calls = [getattr(self.L, "q4_gpu_pages_" + name) for name in ("plan", "trim", "append", "gather", "attend")]
         self.i32, self.f32, self.bf16 = torch.int32, torch.float32, torch.bfloat16
 
@@ -432,30 +438,38 @@ class PagePool:
     def plan(self, rows, add, table, start, slot, pos, req):
         """pages for add[r] more tokens of every request, and the step's maps; table [n_req][stride], slot / pos / req [max_tok].  Request r
         then holds start[r + 1] - start[r] rows more: all of add[r], or none where pages or max_tok ran out"""
-        i, (n, stride) = self.i32, table.shape
-        if not self.calls[0](self.p, _dense(rows, i), _dense(add, i), n, _dense(table, i), stride, _dense(start, i), _dense(slot, i), _dense(pos, i), _dense(req, i), slot.shape[0]):
+        i, gpu, (n, stride), m = self.i32, self.gpu, table.shape, slot.shape[0]
+        if not self.calls[0](self.p, _dense(rows, i, n, gpu), _dense(add, i, n, gpu), n, _dense(table, i, n * stride, gpu), stride, _dense(start, i, n + 1, gpu),
+                             _dense(slot, i, m, gpu), _dense(pos, i, m, gpu), _dense(req, i, m, gpu), m):
             check(False, "q4_gpu_pages_plan")
 
     def trim(self, rows, keep, table):
         """the pages behind the first keep[r] of rows[r] rows go back"""
-        i, (n, stride) = self.i32, table.shape
-        if not self.calls[1](self.p, _dense(rows, i), _dense(keep, i), n, _dense(table, i), stride):
+        i, gpu, (n, stride) = self.i32, self.gpu, table.shape
+        if not self.calls[1](self.p, _dense(rows, i, n, gpu), _dense(keep, i, n, gpu), n, _dense(table, i, n * stride, gpu), stride):
             check(False, "q4_gpu_pages_trim")
 
     def append(self, layer, k, v, slot):
         """k, v [slot.shape[0]][n_kvh * hd] fp32; slots below 0 are skipped"""
-        if not self.calls[2](self.p, layer, _dense(k, self.f32), _dense(v, self.f32), _dense(slot, self.i32), slot.shape[0]):
+        gpu, m = self.gpu, slot.shape[0]
+        x = m * self.width
+        if not self.calls[2](self.p, layer, _dense(k, self.f32, x, gpu), _dense(v, self.f32, x, gpu), _dense(slot, self.i32, m, gpu), m):
             check(False, "q4_gpu_pages_append")
 
     def gather(self, layer, slot, k, v):
         """the rows of the slots as fp32, the reverse of append; k or v may be None"""
-        if not self.calls[3](self.p, layer, _dense(slot, self.i32), slot.shape[0], _dense(k, self.f32), _dense(v, self.f32)):
+        gpu, m = self.gpu, slot.shape[0]
+        x = m * self.width
+        if not self.calls[3](self.p, layer, _dense(slot, self.i32, m, gpu), m, _dense(k, self.f32, x, gpu), _dense(v, self.f32, x, gpu)):
             check(False, "q4_gpu_pages_gather")
 
     def attend(self, layer, q, out, rows, start, table, n_head, scale, gate=None, max_add=0):
         """attention of the step's tokens: q, out [n_tok][n_head][hd], bf16 or fp32; rows as they were given to plan"""
-        i, (n, stride) = self.i32, table.shape
+        i, gpu, (n, stride), x, per = self.i32, self.gpu, table.shape, q.numel(), n_head * self.hd
+        if per <= 0 or x % per:
+            raise RuntimeError("queries of %s are no tokens of %d heads of %d" % (tuple(q.shape), n_head, self.hd))
         q_bf16, out_bf16 = q.dtype is self.bf16, out.dtype is self.bf16
-        if not self.calls[4](self.p, layer, _dense(q, self.bf16 if q_bf16 else self.f32), q_bf16, _dense(gate, self.f32), _dense(out, self.bf16 if out_bf16 else self.f32),
-                             out_bf16, n_head, _dense(rows, i), _dense(start, i), n, q.numel() // (n_head * self.hd), _dense(table, i), stride, max_add, scale):
+        if not self.calls[4](self.p, layer, _dense(q, self.bf16 if q_bf16 else self.f32, x, gpu), q_bf16, _dense(gate, self.f32, x, gpu),
+                             _dense(out, self.bf16 if out_bf16 else self.f32, x, gpu), out_bf16, n_head, _dense(rows, i, n, gpu), _dense(start, i, n + 1, gpu), n, x // per,
+                             _dense(table, i, n * stride, gpu), stride, max_add, scale):
             check(False, "q4_gpu_pages_attend")
