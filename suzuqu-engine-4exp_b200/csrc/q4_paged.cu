@@ -24,7 +24,7 @@
 namespace {
 
 constexpr uint32_t PG_SPIN_LIMIT = 1u << 20;
-__device__ uint32_t g_few_meet[2u * PG_MAX_BLOCKS];
+__device__ uint32_t g_few_meet[PG_MAX_BLOCKS];
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ float ex2(float x) {
@@ -649,8 +649,8 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                 __syncthreads();
                 if (tid == 0) {
                     __threadfence();
-                    s_last = atomicAdd(P.meet + 2u * first, 1u) == n_recs - 1u;
-                    if (s_last) P.meet[2u * first] = 0u;
+                    s_last = atomicAdd(P.meet + first, 1u) == n_recs - 1u;
+                    if (s_last) P.meet[first] = 0u;
                 }
                 __syncthreads();
                 if (s_last) {
@@ -689,12 +689,12 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
      * shared out over the block's groups of eight lanes.  (All of a row by one block: 2 us more.) */
     __syncthreads();
     if (tid == 0) {
-        pg_arrive(P, s_split[0]);
-        pg_arrive(P, s_split[1]);
+        pg_arrive(P, s_split[0], true);
+        pg_arrive(P, s_split[1], false);
     }
     if (s_split[0].last >= s_split[0].first) {
         const PgSplit u = s_split[0];
-        const uint32_t k = u.last - u.first + 1u, joiners = k - 1u, mine_no = blockIdx.x - u.first - 1u;   /* all but the first, which has another's end */
+        const uint32_t k = u.last - u.first + 1u, joiners = pg_joiners(k, false), mine_no = blockIdx.x - u.first - 1u;
         constexpr uint32_t GROUPS = C::THREADS / 8u, BATCH = 5u;
         float4 *s_a = reinterpret_cast<float4 *>(base);
         float2 *s_ml = reinterpret_cast<float2 *>(base + C::THREADS * 16u);
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
                 pg_store<HD, true>(P, u.tok0 + row / P.gqa, u.kh * P.gqa + row % P.gqa, d, A, L, gate);
             }
         }
-        pg_leave(P, u, joiners);
+        pg_leave(P, u);
     }
     if (!ok) {   /* gave up on a copy: those behind it land before the block's shared memory is another's (bounded as well) */
         if (lane == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);

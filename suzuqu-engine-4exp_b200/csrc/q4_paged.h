@@ -22,7 +22,7 @@ struct PagedParams {
     int q_bf16, out_bf16;
     float scale_log2e;
     float *part;                 /* [block][2][rows of a unit][hd + 4]: acc, m (log2 units, scale folded in), l */
-    uint32_t *meet;              /* [block][2]: arrived, gone, of the blocks of the unit that begins in the block; zero between launches */
+    uint32_t *meet;              /* [block]: the word at which the blocks of the unit that begins in the block meet; zero between launches */
     uint32_t *err;
     const uint32_t *fits;        /* not NULL: the launch has work only if this word is `fits_is` (q4i_paged_stage's) */
     uint32_t fits_is;
@@ -45,6 +45,17 @@ bool q4i_paged_chunk(const PagedParams &p, int kind, uint32_t hd, float *scratch
  * whether they were that few (q4_paged_stage.cu).  n_req up to PG_STAGE_REQ. */
 constexpr uint32_t PG_STAGE_REQ = 8192;
 bool q4i_paged_stage(const PagedParams &p, uint32_t hd, uint8_t *to, int32_t *table, uint32_t cap, uint32_t *fits);
+
+/* The word at which the blocks of a split unit meet counts in its lower half the blocks that have arrived, in its upper half those that
+ * will not look at it any more.  Every block counts once in each, whatever happened before, one that joins nothing in both at once, and
+ * whoever completes the upper half leaves zero: nothing comes to the word after that. */
+constexpr uint32_t PG_HERE = 1u, PG_GONE = 1u << 16;
+__host__ __device__ inline uint32_t pg_arrival(bool joins) { return joins ? PG_HERE : PG_HERE + PG_GONE; }
+__host__ __device__ inline bool pg_all_here(uint32_t word, uint32_t blocks) { return (word & (PG_GONE - 1u)) >= blocks; }
+__host__ __device__ inline bool pg_last_gone(uint32_t before, uint32_t blocks) { return before >> 16 == blocks - 1u; }   /* before the addition */
+/* the blocks of a unit that join its records; the first, which may have the end of another unit to see to, only where that is said */
+__host__ __device__ inline uint32_t pg_joiners(uint32_t blocks, bool first_too) { return first_too ? blocks : blocks - 1u; }
+__host__ __device__ inline bool pg_first_joins(uint32_t blocks) { return blocks <= 3u; }                               /* in q4_pg_chunk_k */
 
 #ifdef __CUDACC__
 /* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */
@@ -129,16 +140,21 @@ struct PgShares {
 };
 /* A unit that lies in several blocks, first to last; last < first: none */
 struct PgSplit { uint32_t first, last, tok0, n_here, kh; };
-/* The blocks of a split unit meet at a counter and join its records, each an equal part (the first, which may have the end of another
- * unit to see to, only of a unit of two or three blocks: one block alone takes 15 us for it): some of the rows, or, where there are more blocks than rows, a half, a quarter .. of one.  All blocks
- * of the launch are resident (the grid is what the SMs hold), and end their shares within a few microseconds of one another; a
- * launch of its own for this took 8 to 12 us (one request over 262 144 rows 44 us with it).  The wait is bounded.  Every block
- * arrives and goes once, whatever happened before, and the last to go leaves the counters at zero.
+/* The blocks of a split unit meet at a word and join its records, each an equal part (the first of many records not at all: one block
+ * alone takes 15 us for it): some of the rows, or, where there are more blocks than rows, a half, a quarter .. of one.  All blocks
+ * of the launch are resident in the end (the grid is what the SMs hold) and none waits for another before its share is done; a
+ * launch of its own for this took 8 to 12 us (one request over 262 144 rows 44 us with it).  They end their shares within a few
+ * microseconds of one another, but for q4_pg_few_k beside q4_pg_chunk_k, whose blocks come in as the chunks' leave: there a wait is up to
+ * the spread of those.  The wait is bounded (2 s).
  */
-__device__ __forceinline__ void pg_arrive(const PagedParams &P, const PgSplit &u) {   /* one thread, behind the block's records and a barrier */
+__device__ __forceinline__ void pg_meet(const PagedParams &P, const PgSplit &u, uint32_t what) {   /* one thread */
+    const uint32_t k = u.last - u.first + 1u, before = atomicAdd(P.meet + u.first, what);
+    if (what >= PG_GONE && pg_last_gone(before, k)) P.meet[u.first] = 0u;
+}
+__device__ __forceinline__ void pg_arrive(const PagedParams &P, const PgSplit &u, bool joins) {    /* one thread, behind the block's records and a barrier */
     if (u.last < u.first) return;
     __threadfence();
-    atomicAdd(P.meet + 2u * u.first, 1u);
+    pg_meet(P, u, pg_arrival(joins));
 }
 /* the whole block, until k have arrived */
 __device__ __forceinline__ void pg_wait(const PagedParams &P, const PgSplit &u, uint32_t k) {
@@ -147,8 +163,8 @@ __device__ __forceinline__ void pg_wait(const PagedParams &P, const PgSplit &u, 
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
         for (uint32_t i = 0;; i++) {
             uint32_t n;
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(P.meet + 2u * u.first) : "memory");
-            if (n >= k) break;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(P.meet + u.first) : "memory");
+            if (pg_all_here(n, k)) break;
             if ((i & 63u) == 63u) {
                 asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
                 if (t - t0 > 2000000000ull) {
@@ -161,12 +177,9 @@ __device__ __forceinline__ void pg_wait(const PagedParams &P, const PgSplit &u, 
     }
     __syncthreads();
 }
-__device__ __forceinline__ void pg_leave(const PagedParams &P, const PgSplit &u, uint32_t joiners) {
+__device__ __forceinline__ void pg_leave(const PagedParams &P, const PgSplit &u) {
     __syncthreads();
-    if (threadIdx.x == 0 && atomicAdd(P.meet + 2u * u.first + 1u, 1u) == joiners - 1u) {
-        P.meet[2u * u.first] = 0u;
-        P.meet[2u * u.first + 1u] = 0u;
-    }
+    if (threadIdx.x == 0) pg_meet(P, u, PG_GONE);
 }
 /* What a block joins, and its gates, come to shared memory by bulk copies, all at once; then a thread has four dims of a row, or
  * shares them with others that take the other records.  bar: 8 bytes of shared memory for a barrier, not in use by anything */
@@ -174,8 +187,8 @@ template <int HD, uint32_t THREADS>
 __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes, uint32_t bar) {
     constexpr uint32_t REC = HD + 4u;
     if (u.last < u.first) return;
-    const uint32_t tid = threadIdx.x, k = u.last - u.first + 1u, joiners = k <= 3u ? k : k - 1u, mine = blockIdx.x - u.last + joiners - 1u;   /* the last ones */
-    if (mine >= joiners) return;
+    const uint32_t tid = threadIdx.x, k = u.last - u.first + 1u, joiners = pg_joiners(k, pg_first_joins(k)), mine = blockIdx.x - u.last + joiners - 1u;   /* the last ones */
+    if (mine >= joiners) return;   /* the first of many: it arrived as one that joins nothing */
     uint32_t cut = 0;   /* a row is 1 << cut slices of at least 32 dims */
     while (cut < (HD == 64 ? 1u : HD == 128 ? 2u : 3u) && unit_rows << cut < joiners) cut++;
     const uint32_t wide = (uint32_t)HD >> cut, slices = unit_rows << cut;
@@ -280,7 +293,7 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
     }
     __syncthreads();
     if (tid == 0 && s_begin < s_end) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-    pg_leave(P, u, joiners);
+    pg_leave(P, u);
 }
 #endif
 

@@ -35,7 +35,7 @@ using namespace q4tc;
 
 namespace {
 
-__device__ uint32_t g_chunk_meet[2u * PG_MAX_BLOCKS];
+__device__ uint32_t g_chunk_meet[PG_MAX_BLOCKS];
 constexpr uint32_t CK_BN = 128;
 constexpr uint32_t CK_SPIN_LIMIT = 1u << 22;
 constexpr unsigned long long CK_LIMIT_NS = 2000000000ull;
@@ -1069,12 +1069,12 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
     if (warp == C::ISSUER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     const PgSplit *split = reinterpret_cast<const PgSplit *>(base + (s_split - sQ));
     if (tid == 0) {
-        pg_arrive(P, split[0]);
-        pg_arrive(P, split[1]);
+        pg_arrive(P, split[0], true);
+        pg_arrive(P, split[1], pg_first_joins(split[1].last - split[1].first + 1u));
     }
     const PgSplit ends = split[0], begins = split[1];   /* what follows uses the shared memory */
     pg_join<HD, CK_THREADS>(P, ends, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
-    if (begins.last - begins.first <= 2u) pg_join<HD, CK_THREADS>(P, begins, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
+    if (begins.last >= begins.first && pg_first_joins(begins.last - begins.first + 1u)) pg_join<HD, CK_THREADS>(P, begins, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
 }
 
 template <int KIND, int HD>
