@@ -56,6 +56,13 @@ __host__ __device__ inline bool pg_last_gone(uint32_t before, uint32_t blocks) {
 /* the blocks of a unit that join its records; the first, which may have the end of another unit to see to, only where that is said */
 __host__ __device__ inline uint32_t pg_joiners(uint32_t blocks, bool first_too) { return first_too ? blocks : blocks - 1u; }
 __host__ __device__ inline bool pg_first_joins(uint32_t blocks) { return blocks <= 3u; }                               /* in q4_pg_chunk_k */
+/* a wait: whether one of at most so many probes says yes */
+template <typename Probe>
+__host__ __device__ inline bool pg_within(uint32_t probes, Probe probe) {
+    for (uint32_t i = 0; i < probes; i++)
+        if (probe()) return true;
+    return false;
+}
 
 #ifdef __CUDACC__
 /* what the host or the device gave for request r: tokens (0: none of this launch's), rows before them */
@@ -182,9 +189,10 @@ __device__ __forceinline__ void pg_leave(const PagedParams &P, const PgSplit &u)
     if (threadIdx.x == 0) pg_meet(P, u, PG_GONE);
 }
 /* What a block joins, and its gates, come to shared memory by bulk copies, all at once; then a thread has four dims of a row, or
- * shares them with others that take the other records.  bar: 8 bytes of shared memory for a barrier, not in use by anything */
+ * shares them with others that take the other records.  bar: 8 bytes of shared memory for a barrier, not in use by anything.  ok: false
+ * once a wait for copies has run out (Q4E_CUDA): nothing more is brought or stored, by a later call neither */
 template <int HD, uint32_t THREADS>
-__device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes, uint32_t bar) {
+__device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, uint32_t unit_rows, uint8_t *smem, uint32_t smem_bytes, uint32_t bar, bool &ok) {
     constexpr uint32_t REC = HD + 4u;
     if (u.last < u.first) return;
     const uint32_t tid = threadIdx.x, k = u.last - u.first + 1u, joiners = pg_joiners(k, pg_first_joins(k)), mine = blockIdx.x - u.last + joiners - 1u;   /* the last ones */
@@ -193,7 +201,8 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
     while (cut < (HD == 64 ? 1u : HD == 128 ? 2u : 3u) && unit_rows << cut < joiners) cut++;
     const uint32_t wide = (uint32_t)HD >> cut, slices = unit_rows << cut;
     const uint32_t s_begin = slices * mine / joiners, s_end = slices * (mine + 1u) / joiners;
-    if (s_begin < s_end) {
+    const bool works = ok && s_begin < s_end;
+    if (works) {
         if (tid == 0) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
         pg_wait(P, u, k);
         float4 *s_a = reinterpret_cast<float4 *>(smem);                      /* [thread] */
@@ -203,8 +212,14 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
         const uint32_t stride = wide + 4u, room = smem_bytes - THREADS * 24u, gate_bytes = P.gate ? wide * 4u : 0u, fit = room / (k * stride * 4u + gate_bytes);
         const uint32_t at_once = fit ? fit : 1u, recs_at_once = fit ? k : (room - gate_bytes) / (stride * 4u);
         uint32_t phase = 0;
+        auto there = [&]() -> bool {
+            uint32_t done;
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done) : "r"(bar), "r"(phase) : "memory");
+            return done != 0u;
+        };
         const uint32_t inv_gqa = 65536u / P.gqa + 1u, per_slice = (HD == 64 ? 4u : HD == 128 ? 5u : 6u) - cut;   /* in / gqa = in * inv_gqa >> 16 for in below 128, gqa up to 16; log2 of a slice's items */
-        for (uint32_t s0 = s_begin; s0 < s_end; s0 += at_once) {
+        for (uint32_t s0 = s_begin; s0 < s_end && ok; s0 += at_once) {
             const uint32_t n_s = min(at_once, s_end - s0), items = n_s * (wide / 4u), padded = (items + 31u) & ~31u, groups = padded < THREADS ? THREADS / padded : 1u;
             float *s_rec = s_gate + (P.gate ? n_s * wide : 0u);              /* [record][slice][its dims, m, l, -, -] */
             /* token and head of a slice's row; false: a row without a token */
@@ -248,16 +263,11 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
                         if (!place(s, tok, head)) tok = u.tok0, head = u.kh * P.gqa;   /* any gate: not used */
                         copy(s_gate + s * wide, P.gate + ((size_t)tok * P.n_head + head) * HD + ((s0 + s) & ((1u << cut) - 1u)) * wide, wide * 4u);
                     }
-                for (uint32_t i = 0; i < (1u << 20); i++) {                  /* bounded: a copy ends by itself */
-                    uint32_t done;
-                    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                                 : "=r"(done) : "r"(bar), "r"(phase) : "memory");
-                    if (done) break;
-                }
-                phase ^= 1u;
+                ok = __syncthreads_and(pg_within(1u << 20, there));
+                if (ok) phase ^= 1u;
             };
             bring(0u, recs_at_once < k ? recs_at_once : k, P.gate != nullptr);
-            for (uint32_t item0 = 0; item0 < items; item0 += groups > 1u ? padded : THREADS) {
+            for (uint32_t item0 = 0; item0 < items && ok; item0 += groups > 1u ? padded : THREADS) {
                 const uint32_t group = groups > 1u ? tid / padded : 0u, item = item0 + (groups > 1u ? tid - group * padded : tid);
                 const uint32_t s = item >> per_slice, d = (item & ((1u << per_slice) - 1u)) * 4u;
                 uint32_t tok, head;
@@ -273,6 +283,7 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
                 for (uint32_t c0 = 0; c0 < k; c0 += recs_at_once) {          /* more than one turn: one slice, and at most a thread per item */
                     const uint32_t n = min(recs_at_once, k - c0);
                     if (c0) bring(c0, n, false);
+                    if (!ok) break;
                     if (live)
                         for (uint32_t c = group; c < n; c += groups) {
                             const float *rec = s_rec + ((size_t)c * n_s + s) * stride;
@@ -280,6 +291,7 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
                             join(ml.x, ml.y, *reinterpret_cast<const float4 *>(rec + d));
                         }
                 }
+                if (!ok) break;
                 if (groups > 1u) {
                     s_a[tid] = A;
                     s_ml[tid] = make_float2(M, L);
@@ -290,9 +302,14 @@ __device__ __forceinline__ void pg_join(const PagedParams &P, const PgSplit &u, 
                 if (live && group == 0u) pg_store<HD>(P, tok, head, ((s0 + s) & ((1u << cut) - 1u)) * wide + d, A, L, P.gate ? s_gate + s * wide + d : nullptr);
             }
         }
+        __syncthreads();
+        if (ok) {
+            if (tid == 0) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+        } else {
+            if (tid == 0) atomicOr(P.err, (uint32_t)Q4E_CUDA);
+            (void)pg_within(4096u, there);   /* those on their way land before the block's shared memory is another's */
+        }
     }
-    __syncthreads();
-    if (tid == 0 && s_begin < s_end) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     pg_leave(P, u);
 }
 #endif

@@ -1073,8 +1073,9 @@ __global__ void __launch_bounds__(ChunkCfg<KIND, HD>::THREADS, 1) q4_pg_chunk_k(
         pg_arrive(P, split[1], pg_first_joins(split[1].last - split[1].first + 1u));
     }
     const PgSplit ends = split[0], begins = split[1];   /* what follows uses the shared memory */
-    pg_join<HD, CK_THREADS>(P, ends, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
-    if (begins.last >= begins.first && pg_first_joins(begins.last - begins.first + 1u)) pg_join<HD, CK_THREADS>(P, begins, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum);
+    bool joining = true;
+    pg_join<HD, CK_THREADS>(P, ends, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum, joining);
+    if (begins.last >= begins.first && pg_first_joins(begins.last - begins.first + 1u)) pg_join<HD, CK_THREADS>(P, begins, C::ROWS, base, NQ * C::QG + SLOTS * SLOT, s_sum, joining);
 }
 
 template <int KIND, int HD>

@@ -84,3 +84,30 @@ def test_the_word_comes_back_to_zero(tmp_path):
     assert r.returncode == 0, r.stdout
     r = subprocess.run([str(exe)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout == "ok\n", r.stdout
+
+
+WAITS = r"""
+#include <stdio.h>
+#include "q4_paged.h"
+int main() {
+    for (uint32_t probes : {0u, 1u, 5u, 4096u})
+        for (uint32_t yes : {0u, 1u, 4u, 4095u, 4096u, 0xffffffffu}) {   /* the probe that says so */
+            uint32_t n = 0;
+            const bool got = pg_within(probes, [&]() { return n++ == yes; });
+            if (got != (yes < probes) || n != (got ? yes + 1u : probes)) return printf("%u probes, yes at %u: %d after %u\n", probes, yes, got, n), 1;
+        }
+    printf("ok\n");
+    return 0;
+}
+"""
+
+
+def test_a_wait_says_whether_it_ran_out(tmp_path):
+    """by it the join of records knows not to store what did not come"""
+    src, exe = tmp_path / "waits.cpp", tmp_path / "waits"
+    src.write_text(WAITS)
+    r = subprocess.run(["g++", "-std=c++17", "-O2", "-I", CSRC, "-I", "/usr/local/cuda/include", str(src), "-o", str(exe)],
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert r.returncode == 0, r.stdout
+    r = subprocess.run([str(exe)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout
