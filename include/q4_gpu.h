@@ -505,8 +505,9 @@ bool q4_gpu_pages_gather(const q4_gpu_pages *pg, uint32_t layer, const int32_t *
  *   max_add  the most tokens of one request, as far as the host knows (0: it does not).  It chooses between kernels only: results
  *            are right for any value
  * A request whose rows pass its table's row is left out (status bit 4); positions on a page that is not the pool's are skipped
- * (status bit 4); a token with nothing to attend gets 0.  Scratch grows outside a capture only (status bit 8 inside one);
- * many tokens per request over q8_0 pages are read from a copy of their rows in fp16 there, of at most 512 MB.
+ * (status bit 4); a token with nothing to attend gets 0.  Scratch (up to 60 MB of records) grows outside a capture only (status bit
+ * 8 inside one).  Many tokens per request over q8_0 pages are read from a copy of their rows in fp16 there, of at most 512 MB and
+ * the size of the block tables; where that is not to be had, or not there yet in a capture, they are read as they are, which is slower.
  * Queries, rows and weights enter the products as fp16 (q8_0: fp16(code * scale)): beyond 65504 in size they are not finite there.
  * What is not finite stays with the tokens that attend it: a V that is not makes their outputs so in its dims, a new row's also in
  * others. */

@@ -106,6 +106,7 @@ struct Q4State {
      * that then grows is kept until no graph is left (sizes grow by a quarter at least, so what is kept stays below four
      * times what is in use). */
     bool part_captured, counters_captured, stage_captured;
+    uint32_t spare_refused;      /* calls of q4i_scratch_spare still to pass before memory is asked for again */
     Q4PtrList graphs, kept;      /* instantiated and not yet freed; workspaces that one of them may use */
 };
 extern Q4State g_q4;
@@ -133,6 +134,7 @@ bool q4i_apart(const Q4Touch &touch);
 bool q4i_blocks_ahead(const void *p, uint64_t bytes, uint32_t ratio);
 inline void q4i_kv_written(q4_gpu_kv *kv, uint32_t layer) { kv->writes->at[layer] = g_q4.launches; }
 bool q4i_scratch(size_t part_floats, size_t n_counters); /* grows outside capture, fails inside */
+bool q4i_scratch_spare(size_t part_floats);              /* whether so much is there or to be had, for a launch that can do without: no status */
 void q4i_give_back(void *p, bool captured);              /* cudaFree, now or with the last graph */
 
 #define Q4_REQUIRE(cond, what)                    \

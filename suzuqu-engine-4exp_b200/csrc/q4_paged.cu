@@ -814,17 +814,18 @@ extern "C" bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, cons
         few_rows = p.gqa <= 8u ? 8u : 16u;
         p.add_split = n_req == 1u ? 0u : few_rows / p.gqa;
         /* Many units per request read its rows from a copy in fp16 (q4_paged_stage.cu), if it is not too large: on average 12 per request
-         * at hd 256, 32 at 64 and 128, and 1024 tokens in all.  Without and with, us: at hd 256 8192 tokens over 16 384 (820 units) 5760
-         * and 3260, three prompts (130) 201 and 132, 128 tokens each over 4000 rows (13) 99 and 90, 60 (6) 66 and 69, one prompt of
-         * 320 tokens 29 and 38; at hd 128 8192 over 16 384 (256) 1440 and 1270, 2048 over 16 001 (64) 350 and 318, 1024 (32) 192 and
+         * at hd 256, 32 at 64 and 128, and 1024 tokens in all.  Without and with, us: at hd 256 8192 tokens over 16 384 (820 units) 5700
+         * and 3350, three prompts (130) 201 and 132, 128 tokens each over 4000 rows (13) 99 and 90, 60 (6) 66 and 69, one prompt of
+         * 320 tokens 29 and 38; at hd 128 8192 over 16 384 (256) 1390 and 1225, 2048 over 16 001 (64) 323 and 302, 1024 (32) 192 and
          * 184, 512 (16) 106 and 106; three prompts (40) 73 and 75. */
         const uint32_t per_unit = 128u / p.gqa * (pg->hd == 256 ? 1u : 2u);
         const uint64_t img_page = (uint64_t)pg->page_rows * pg->n_kvh * pg->hd * 4u, places = (uint64_t)n_req * table_stride, most_pages = (512ull << 20) / img_page;
-        const bool stage = pg->kind == Q4K_Q8 && n_req <= PG_STAGE_REQ && places <= 1u << 24 && most_pages && n_tok >= 1024u && n_tok >= (uint64_t)n_req * per_unit * (pg->hd == 256 ? 12u : 32u);
+        bool stage = pg->kind == Q4K_Q8 && n_req <= PG_STAGE_REQ && places <= 1u << 24 && most_pages && n_tok >= 1024u && n_tok >= (uint64_t)n_req * per_unit * (pg->hd == 256 ? 12u : 32u);
         const uint32_t cap = stage ? (uint32_t)(places < most_pages ? places : most_pages) : 0u;
         /* records of both kernels: the second's must not fall on the first's while those are joined */
         const size_t chunk = (q4i_paged_chunk_floats(pg->hd) + 63u) / 64u * 64u, rest = (size_t)g_q4.sm_count * 2u * 2u * 32u * (256u + 4u), img = cap * (size_t)(img_page / 4u);
-        if (!q4i_scratch(chunk + rest + img + (stage ? (size_t)places + 1u : 0u), 0)) return false;
+        if (stage) stage = q4i_scratch_spare(chunk + rest + img + (size_t)places + 1u);   /* no room, or a capture before it was made: the pages as they are */
+        if (!q4i_scratch(chunk + rest, 0)) return false;
         if (stage) {
             PagedParams c = p;
             uint8_t *to = (uint8_t *)(g_q4.part + chunk + rest);

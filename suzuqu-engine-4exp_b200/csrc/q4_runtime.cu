@@ -176,6 +176,35 @@ bool q4i_scratch(size_t part_floats, size_t n_counters) {
     return true;
 }
 
+/* The records' scratch for something that can do without: what is there stays until the larger one is, and no memory, or a
+ * capture, is no error.  A request that was refused is not repeated for the next calls: each would cost the host a failing allocation. */
+bool q4i_scratch_spare(size_t part_floats) {
+    if (part_floats <= g_q4.part_floats) return true;
+    if (g_q4.capturing) return false;
+    if (g_q4.spare_refused) {
+        g_q4.spare_refused--;
+        return false;
+    }
+    const size_t grown = g_q4.part_floats + g_q4.part_floats / 4, want = part_floats > grown ? part_floats : grown;
+    float *p = nullptr;
+    const cudaError_t e = cudaMalloc(&p, want * sizeof(float));
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        if (e != cudaErrorMemoryAllocation) return q4i_check(e, "scratch alloc");
+        g_q4.spare_refused = 64;
+        return false;
+    }
+    if (!q4i_check(cudaStreamSynchronize(g_q4.stream), "scratch sync")) {
+        cudaFree(p);
+        return false;
+    }
+    q4i_give_back(g_q4.part, g_q4.part_captured);
+    g_q4.part = p;
+    g_q4.part_floats = want;
+    g_q4.part_captured = false;
+    return true;
+}
+
 extern "C" bool q4_hip_init(void) {
     if (g_q4.ok) return true;
     int n = 0;

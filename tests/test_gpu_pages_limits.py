@@ -5,7 +5,7 @@ import torch
 
 import q4gpu
 from gpu_util import lib
-from test_gpu_pages import KINDS, Step, attend_exact, ints, plan_plain
+from test_gpu_pages import Step, attend_exact, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,45 @@ def test_trim_does_not_look_at_entries_that_stay():
     s.pool.trim(s.d_rows, ints([5, 33]), table)
     assert lib().q4_gpu_last_error() == 0
     assert s.free_now() == s.free + s.table[0][1:5][::-1]
+
+
+def test_many_tokens_over_q8_0_without_scratch_for_their_copy():
+    """a capture for which only a short chunk's scratch is there: the pages are read as they are"""
+    L = lib()
+    L.q4_gpu_set_stream(None)
+    L.q4_hip_shutdown()                                   # gives back what other tests made it reserve
+    L = q4gpu.init()
+    n_head, n_kvh, hd, page, held, n = 16, 2, 128, 16, 77, 1300
+    scale = float(hd ** -0.5)
+    try:
+        with torch.cuda.stream(torch.cuda.ExternalStream(L.q4_gpu_stream())):
+            pool = q4gpu.PagePool(1, n_kvh, hd, 200, page, q4gpu.KIND_Q8)
+            table = torch.full((1, 16384), -1, dtype=torch.int32, device="cuda")     # a context of 262 144
+            start, maps = ints([0, 0]), [torch.empty(held + n, dtype=torch.int32, device="cuda") for _ in range(3)]
+            k, v = torch.randn(2, held + n, n_kvh * hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7))
+            q = torch.randn(held + n, n_head, hd, device="cuda").to(torch.bfloat16)
+            out = torch.empty(held + n, n_head, hd, device="cuda")
+            pool.plan(ints([0]), ints([held]), table, start, *maps)
+            pool.append(0, k[:held], v[:held], maps[0][:held])
+            pool.attend(0, q[:held], out[:held], ints([0]), start, table, n_head, scale, max_add=held)
+            rows, add = ints([held]), ints([n])
+            torch.cuda.synchronize()
+            assert L.q4_hip_graph_begin()
+            pool.plan(rows, add, table, start, *maps)
+            pool.append(0, k[held:], v[held:], maps[0][:n])
+            pool.attend(0, q[held:], out[held:], rows, start, table, n_head, scale, max_add=n)
+            graph = L.q4_hip_graph_end()
+            assert graph and L.q4_gpu_last_error() == 0
+            assert L.q4_hip_graph_launch(graph)
+            captured = out[held:].clone()
+            pool.attend(0, q[held:], out[held:], rows, start, table, n_head, scale, max_add=n)   # outside: by the copy
+            p = torch.arange(held + n, device="cuda")
+            kr, vr = torch.empty(2, held + n, n_kvh * hd, device="cuda")
+            pool.gather(0, (table[0].long()[p // page] * page + p % page).int(), kr, vr)
+            want = attend_exact(q[held:], kr.view(-1, n_kvh, hd), vr.view(-1, n_kvh, hd), None, held, scale)
+            for got in (captured, out[held:]):
+                assert ((got.double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+            L.q4_hip_graph_free(graph)
+    finally:
+        lib()
+    assert L.q4_gpu_last_error() == 0
