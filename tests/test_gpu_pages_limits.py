@@ -5,7 +5,7 @@ import torch
 
 import q4gpu
 from gpu_util import lib
-from test_gpu_pages import Step, attend_exact, ints
+from test_gpu_pages import KINDS, Step, attend_exact, ints, plan_plain
 
 pytestmark = pytest.mark.gpu
 
@@ -40,6 +40,51 @@ def test_trim_does_not_look_at_entries_that_stay():
     s.pool.trim(s.d_rows, ints([5, 33]), table)
     assert lib().q4_gpu_last_error() == 0
     assert s.free_now() == s.free + s.table[0][1:5][::-1]
+
+
+@pytest.mark.parametrize("rows,add,kw", [([0], [1], dict(n_pages=1, max_tok=1)), ([0], [17], dict(n_pages=1)), ([5], [12], dict(max_tok=12)), ([5], [12], dict(max_tok=11)),
+                                         ([-3], [1], {}), ([60], [5], dict(stride=4)), ([60], [4], dict(stride=4))])
+def test_status_of_a_plan_of_one_request(rows, add, kw):
+    s = Step(rows, add, **kw)
+    want = plan_plain(rows, add, s.table, s.free, s.page, s.max_tok)
+    L = lib()
+    L.q4_gpu_last_error()
+    s.plan()
+    assert L.q4_gpu_last_error() == want[6]
+    assert (s.d_table.tolist(), s.free_now(), s.start.tolist(), s.slot.tolist()) == (want[0], want[1], want[2], want[3])
+
+
+@pytest.mark.parametrize("kind", ["q8_0", "f16"])
+@pytest.mark.parametrize("idle", [40, 1000, 3000])
+@pytest.mark.parametrize("add", [[1, 1, 1], [1, 90, 3], [200, 1, 70]])
+def test_many_places_without_tokens(kind, idle, add):
+    """requests that bring tokens far apart among places that bring none, held rows or not"""
+    n_head, n_kvh, hd, page = 16, 2, 128, 16
+    n, at = 2 * idle + 3, [0, idle + 1, 2 * idle + 2]
+    rows, adds = [(r % 3) * 8 for r in range(n)], [0] * n
+    for r, h, a in zip(at, (700, 0, 333), add):
+        rows[r], adds[r] = h, a
+    s = Step(rows, adds, page, n_kvh=n_kvh, hd=hd, kind=KINDS[kind])
+    g = torch.Generator(device="cuda").manual_seed(idle)
+    slot = [s.table[r][p // page] * page + p % page for r in at for p in range(rows[r])]
+    k, v = torch.randn(2, len(slot), n_kvh * hd, generator=g, device="cuda")
+    s.pool.append(0, k, v, ints(slot))
+    s.plan()
+    total = sum(add)
+    k, v = torch.randn(2, total, n_kvh * hd, generator=g, device="cuda")
+    s.pool.append(0, k, v, s.slot[:total])
+    q = torch.randn(total, n_head, hd, generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.empty(total, n_head, hd, device="cuda")
+    s.pool.attend(0, q, out, s.d_rows, s.start, s.d_table, n_head, float(hd ** -0.5))
+    assert lib().q4_gpu_last_error() == 0
+    first = 0
+    for r, m in zip(at, add):
+        table = s.d_table[r].tolist()
+        kr, vr = torch.empty(2, rows[r] + m, n_kvh * hd, device="cuda")
+        s.pool.gather(0, ints([table[p // page] * page + p % page for p in range(rows[r] + m)]), kr, vr)
+        want = attend_exact(q[first: first + m], kr.view(-1, n_kvh, hd), vr.view(-1, n_kvh, hd), None, rows[r], float(hd ** -0.5))
+        assert ((out[first: first + m].double() - want).abs() <= 2e-3 + 1e-3 * want.abs()).all()
+        first += m
 
 
 def test_many_tokens_over_q8_0_without_scratch_for_their_copy():
