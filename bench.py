@@ -18,9 +18,7 @@ Extra objects on the same JSON line (rank 0, 1 GPU): `single_session_ctx262144` 
 1, us per layer under graph replay), `dense_ctx262144` (full attention over 262144 rows for q8_0 /
 f16 / f32), `roofline` for the dominant kernel and `cpu_baseline` (the CPU oracle on host cores).
 
-`--impl reference` times the reference's own CPU arithmetic for the same step (the oracle port:
-q8_0 quantise of the new rows + scalar attention over the dequantised selected rows) on all host
-threads, on a bounded sample of the sessions.
+`--impl reference` prints that the reference cannot run here, and why; `cpu_baseline` is the time of the oracle port of its CPU arithmetic.
 """
 import argparse
 import json
@@ -235,31 +233,11 @@ def cpu_baseline(ctxs, budget_s, n_sessions=4):
             "value_1_thread": v1, "sample_1_thread": "same sample, %d reps (%.1f s) on one thread" % (reps1, dt1)}
 
 
-def run_reference_arm(args, rank):
-    if rank != 0:
-        return
-    from oracle import q4_oracle as oracle
-    ctxs = draw_contexts(args.sessions)
-    n_s = 4
-    threads = max(1, oracle.host_procs())
-    items, news = cpu_sample_problem(ctxs, n_s, SEED + 9)
-    for _ in range(args.warmup):
-        cpu_step(items, news, threads)
-    t0 = time.perf_counter()
-    for _ in range(args.steps):
-        cpu_step(items, news, threads)
-    dt = time.perf_counter() - t0
-    v = n_s * args.steps / dt
-    line = {"impl": "reference", "metric": "decode_attn_session_tok_per_s", "value": v, "unit": "session*tok/s",
-            "n_gpus": args.gpus, "steps": args.steps, "warmup": args.warmup, "ms_per_step": 1e3 * dt / args.steps,
-            "higher_is_better": True, "scaling": "strong", "vs_baseline": None, "dtype": "q8_0+f32",
-            "data": "synthetic", "config": workload_config(args.sessions),
-            "cpu_baseline": {"value": v, "unit": "session*tok/s", "cores": threads, "kind": "port",
-                             "sample": "each step = %d of the 64 sessions x 12 layers (compact caches of the "
-                                       "selected rows), all host threads" % n_s},
-            "e2e": {"value": v, "unit": "session*tok/s", "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0},
-            "gpu_launches": 0}
-    print(json.dumps(line), flush=True)
+def run_reference_arm(rank):
+    """The reference's own code for this path is HIP (hipcc and an AMD GPU) or its CPU forward (an 80 GB model file), neither of which
+    can be had where this runs; the oracle port is no reference and is timed as `cpu_baseline` only."""
+    if rank == 0:
+        print(json.dumps({"impl": "reference", "unavailable": "its GPU path needs hipcc and an AMD GPU, its CPU path an 80 GB model file; neither is on this machine"}), flush=True)
 
 
 def workload_config(sessions):
@@ -1040,7 +1018,7 @@ def main():
     world = int(os.environ.get("WORLD_SIZE", "1"))
     local = int(os.environ.get("LOCAL_RANK", "0"))
     if args.impl == "reference":
-        run_reference_arm(args, rank)
+        run_reference_arm(rank)
         return
     if args.warmup < 3:
         args.warmup = 3
