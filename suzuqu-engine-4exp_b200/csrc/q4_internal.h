@@ -180,7 +180,7 @@ bool q4i_launch_pdl(const char *what, K kernel, dim3 grid, uint32_t threads, siz
     return q4i_launched(q4i_launch_dep(what, kernel, grid, threads, smem, args...));
 }
 /* ---- the q8_0 quantiser, one copy for every kernel that writes a cache row.  8 lanes share a block
- * of 32 values (4 each): d = amax / 127 and id = 1 / d as IEEE fp32 divisions, codes =
+ * of 32 values (4 each; in a pool of pages 4 lanes, 8 each): d = amax / 127 and id = 1 / d as IEEE fp32 divisions, codes =
  * clamp(rint(x * id), +-127), stored scale = fp16(d) (quantize_row_q8_0's arithmetic,
  * src/q4_quant.c / src/q4_rocm.cu f32_to_q8 kernels). */
 __device__ __forceinline__ uint32_t q4d_quant4(const float4 x, float id) {
@@ -191,14 +191,18 @@ __device__ __forceinline__ uint32_t q4d_quant4(const float4 x, float id) {
     return (uint32_t)(q0 & 0xff) | ((uint32_t)(q1 & 0xff) << 8) | ((uint32_t)(q2 & 0xff) << 16) |
            ((uint32_t)(q3 & 0xff) << 24);
 }
+/* d and 1/d of a block whose largest value is a */
+__device__ __forceinline__ void q4d_scale(float a, float &d, float &id) {
+    d = __fdiv_rn(a, 127.f);
+    id = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
+}
 /* amax over the 8 lanes that share a block (all 32 lanes of the warp must call), then d and 1/d */
 __device__ __forceinline__ void q4d_block_scale(const float4 x, float &d, float &id) {
     float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 4));
-    d = __fdiv_rn(a, 127.f);
-    id = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
+    q4d_scale(a, d, id);
 }
 #endif
 

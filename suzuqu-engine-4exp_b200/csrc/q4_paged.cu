@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(FewCfg<KIND, HD, NT>::THREADS, FewCfg<KIND, HD
         for (uint32_t i = 0; i < DEPTH; i++) bar_init(bars + 8u * i, 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     /* Beside the chunks of its own call it takes the SMs that they leave: that launch began behind everything before it, and nothing
-     * here reads what it writes (a mixed step 278 -> 256 us).  What it reads may be two launches old: by loads that do not look into L1.  The
+     * here reads what it writes (a mixed step 279 -> 256 us in a burst, 291 -> 273 over a second of them; in q8_0 297 -> 277 and 296 -> 281).  What it reads may be two launches old: by loads that do not look into L1.  The
      * end of that launch is waited for at the end, for those behind this one. */
     if (!P.beside) q4d_pdl_wait();
 

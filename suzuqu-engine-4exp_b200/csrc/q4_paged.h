@@ -1,4 +1,4 @@
-/* Shared by the two attention kernels over a pool of pages (q4_paged.cu, q4_paged_tc.cu; not installed). */
+/* Shared by the kernels over a pool of pages (q4_pages.cu, q4_paged.cu, q4_paged_tc.cu, q4_paged_stage.cu; not installed). */
 #ifndef Q4_PAGED_H
 #define Q4_PAGED_H
 
@@ -29,6 +29,7 @@ struct PagedParams {
     uint32_t beside;             /* q4_pg_few_k behind q4_pg_chunk_k of the same call: it need not wait for that one's end */
 };
 
+/* of 16 rows of a kv head, K and V; of one row */
 template <int KIND, int HD>
 struct PgTile {
     static constexpr uint32_t ROW = KIND == Q4K_Q8 ? (2u * HD + HD / 8u + 15u) / 16u * 16u : 4u * HD, BYTES = 16u * ROW;

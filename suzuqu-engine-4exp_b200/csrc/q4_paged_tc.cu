@@ -130,7 +130,9 @@ __device__ __forceinline__ bool ck_all_wait(uint32_t bar, uint32_t parity, uint3
     return __all_sync(0xffffffffu, ck_wait_on(bar, parity, s_abort));
 }
 
-/* sum of floor((a i + b) / 128) over i < n, a up to 256 and a n + b below 2^32 (Euclid's steps on a and 128) */
+/* sum of floor((a i + b) / 128) over i < n, a up to 256 and a n + b below 2^32: whole multiples are taken out of a and b, what is left is counted
+ * along the other axis of the lattice triangle, which swaps a and 128 (the reciprocity of floor sums, Graham, Knuth, Patashnik,
+ * Concrete Mathematics, section 3.5), as in Euclid's algorithm */
 __device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t a, uint32_t b) {
     uint64_t r = 0;
     uint32_t m = 128u;

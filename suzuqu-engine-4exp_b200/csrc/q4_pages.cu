@@ -10,7 +10,7 @@
  *         tiles one behind the other are the swizzled operand that the tensor core reads
  * Either way a tile is contiguous and arrives by bulk copies as it is used.
  */
-#include "q4_internal.h"
+#include "q4_paged.h"
 
 namespace {
 
@@ -229,10 +229,6 @@ struct RowParams {
     float *k_out, *v_out;        /* gather */
     uint32_t *err;
 };
-template <int KIND, int HD>
-struct PgTile {
-    static constexpr uint32_t ROW = KIND == Q4K_Q8 ? (2u * HD + HD / 8u + 15u) / 16u * 16u : 4u * HD, BYTES = 16u * ROW;
-};
 /* of the slot: its page's part of the kv head, its tile, its row of the tile */
 template <int KIND, int HD>
 __device__ __forceinline__ uint8_t *slot_tile(const RowParams &P, uint32_t slot, uint32_t kh) {
@@ -244,7 +240,7 @@ __device__ __forceinline__ uint8_t *slot_tile(const RowParams &P, uint32_t slot,
 /*
  * Append and gather: 8 dims per thread (two 16-byte loads of fp32; 8 codes or one 16-byte piece of fp16), K and V of them, so
  * that a thread has 64 bytes in flight.  Both are bound by memory: 4 bytes read per value for 1 or 2 written, or the reverse.
- * The quantiser's steps are those of q4d_block_scale and q4d_quant4, with four lanes to a block of 32 instead of eight.
+ * The quantiser is the store's (q4d_scale, q4d_quant4), with four lanes to a block of 32 instead of eight.
  */
 template <int KIND, int HD>
 __global__ void __launch_bounds__(256) q4_pg_append_k(const RowParams P) {
@@ -275,7 +271,8 @@ __global__ void __launch_bounds__(256) q4_pg_append_k(const RowParams P) {
                             fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float d = __fdiv_rn(m, 127.f), id = d > 0.f ? __fdiv_rn(1.f, d) : 0.f;
+            float d, id;
+            q4d_scale(m, d, id);
             if (store) {
                 uint8_t *rec = tile + in * PgTile<KIND, HD>::ROW;
                 *reinterpret_cast<uint2 *>(rec + w * HD + c * 8u) = make_uint2(q4d_quant4(a, id), q4d_quant4(b, id));
