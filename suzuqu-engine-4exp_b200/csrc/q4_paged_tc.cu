@@ -11,7 +11,8 @@
  *                  memory, causal mask, running maximum with lazy rescale, weights as fp16 back into the columns they came from
  *   producers      (one team of four warps, or three of two) K and V of a tile into a ring of operand slots.  fp16 pages hold tiles as the tensor core reads them: bulk copies.
  *                  q8_0: codes and scales by asynchronous copies, then fp16(code x scale) into the slot (7 instructions
- *                  per 4 values)
+ *                  per 4 values).  Scales on the scores instead, as for few tokens, would need a product and an accumulator per 32 dims, and
+ *                  their sums on the softmax warps, which set the pace
  *   issuer         the products: O += P V of a unit of positions as its weights appear, then the scores that take over the buffer
  *   walker         the share's pieces, and where the rows of their tiles lie, ahead of the others
  * V stays as it lies in the page, positions by dims: the product takes it as an operand whose dims are contiguous.
