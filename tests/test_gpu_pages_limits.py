@@ -42,6 +42,26 @@ def test_trim_does_not_look_at_entries_that_stay():
     assert s.free_now() == s.free + s.table[0][1:5][::-1]
 
 
+def test_tensors_on_the_host_and_ones_too_small_reach_no_kernel():
+    s = Step([5, 6], [1, 1], n_kvh=2, hd=128).plan()
+    p, before = s.pool, s.free_now()
+    q = torch.zeros(2, 16, 128, device="cuda")
+    k = torch.zeros(2, 256, device="cuda")
+    calls = [lambda: p.plan(s.d_rows.cpu(), s.d_add, s.d_table, s.start, s.slot, s.pos, s.req), lambda: p.plan(s.d_rows, s.d_add, s.d_table, s.start[:2], s.slot, s.pos, s.req),
+             lambda: p.plan(s.d_rows, s.d_add[:1], s.d_table, s.start, s.slot, s.pos, s.req), lambda: p.plan(s.d_rows, s.d_add, s.d_table, s.start, s.slot, s.pos[:3], s.req),
+             lambda: p.trim(s.d_rows, s.d_rows[:1], s.d_table), lambda: p.append(0, k[:1], k, s.slot[:2]), lambda: p.append(0, k, k.cpu(), s.slot[:2]),
+             lambda: p.gather(0, s.slot[:2], k, k[:1]), lambda: p.attend(0, q, q[:1].clone(), s.d_rows, s.start, s.d_table, 16, 0.1),
+             lambda: p.attend(0, q, q.clone(), s.d_rows, s.start, s.d_table.cpu(), 16, 0.1), lambda: p.attend(0, q, q.clone(), s.d_rows, s.start, s.d_table, 16, 0.1, gate=q[:1]),
+             lambda: p.attend(0, q, q.clone(), s.d_rows, s.start, s.d_table, 0, 0.1),
+             lambda: q4gpu.PagePool(1, 2, 128, p.n_pages, 16, q4gpu.KIND_Q8, mem=p.mem, free=p.free[:2], n_free=p.n_free),
+             lambda: q4gpu.PagePool(1, 2, 128, p.n_pages, 16, q4gpu.KIND_Q8, mem=p.mem.cpu())]
+    for i, call in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("call %d was taken" % i)
+    assert lib().q4_gpu_last_error() == 0 and s.free_now() == before
+
+
 @pytest.mark.parametrize("rows,add,kw", [([0], [1], dict(n_pages=1, max_tok=1)), ([0], [17], dict(n_pages=1)), ([5], [12], dict(max_tok=12)), ([5], [12], dict(max_tok=11)),
                                          ([-3], [1], {}), ([60], [5], dict(stride=4)), ([60], [4], dict(stride=4))])
 def test_status_of_a_plan_of_one_request(rows, add, kw):
