@@ -518,6 +518,90 @@ bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, 
                          uint32_t n_head, const int32_t *rows, const int32_t *start, uint32_t n_req, uint32_t n_tok, const int32_t *table,
                          uint32_t table_stride, uint32_t max_add, float scale);
 
+/* ---- what a step does around its attention.  Per step of a host whose requests share prefixes and are drafted for:
+ *     q4_gpu_pages_plan(...);
+ *     per layer: q4_gpu_pages_prep(...); q4_gpu_pages_attend(...);
+ *     q4_gpu_verify(...);                                  tokens kept, the next token, rows kept
+ *     q4_gpu_pages_release(...);                           in place of trim: pages with other holders stay out
+ * and q4_gpu_pages_fork when a request's prefix is taken over, q4_gpu_pages_compact when the pool is to be cut.
+ *
+ * Rotation of position p: pair i is turned by p * f_i, the pairs being dims (2 i, 2 i + 1) (half = 0) or (i, i + n_rot / 2) (half = 1)
+ * of the first n_rot dims; mag is on the turned dims.  turn[i] is f_i in turns as a fraction of 2^64: p * turn[i] modulo 2^64 is the angle
+ * without a rounding, at any position. */
+typedef struct q4_gpu_rope {
+    uint32_t n_rot;
+    int32_t half;
+    float mag;
+    uint32_t reserved;
+    uint64_t turn[128];
+} q4_gpu_rope;
+/* Fills in a descriptor, on the host (no device is needed).  f_i = base^(-2 i / n_rot), scaled for longer contexts than orig positions:
+ *   0  as they are                                                  (factor, orig, fast, slow: ignored)
+ *   1  linear   f_i / factor
+ *   2  ramp     f_i (1 - s) + f_i / factor s, s rising from 0 to 1 over the pairs, from the one that turns `fast` times in orig positions (rounded
+ *               down) to the one that turns `slow` times (rounded up)
+ *   3  smooth   the same with s = 1 - (turns in orig positions - slow) / (fast - slow), between 0 and 1
+ * n_rot even, up to 256 (0: no rotation), a multiple of 8 for half; base above 1 (scaling 2 and 3) or 0; factor, orig, mag above 0, fast above
+ * slow above 0. */
+bool q4_gpu_rope_set(q4_gpu_rope *r, uint32_t n_rot, int half, double base, int scaling, double factor, double orig, double fast,
+                     double slow, double mag);
+/* The projections of a step's tokens made ready for q4_gpu_pages_attend, one launch per layer: queries and keys are normed per head (x / sqrt(mean
+ * x^2 + eps) * w; eps below 0: no norm; w [hd] fp32 or NULL) and turned by pos[t], the gates split off, keys and values put into slot[t] as by
+ * q4_gpu_pages_append.  Replaces q4_hip_qsa_q_prep_n, q4_hip_qsa_k_prep_n and the append for steps of many requests, whose
+ * tokens have positions of their own (src/q4_fwd.c:881-891, 1734-1741 know one).
+ *   q        token t's row begins q_stride values behind token t - 1's: [n_head][hd], or [n_head][q hd | gate hd] where gate is not NULL
+ *   k, v     the same with kv_stride, [n_kvh][hd]; the three may lie in one fused row.  fp32, or bf16 (in_bf16); rows 16-byte aligned
+ *   q_out    [n_tok][n_head][hd], bf16 or fp32; gate [n_tok][n_head][hd] fp32 or NULL.  May not overlap the inputs.
+ * A token with pos[t] below 0 is left out, q_out and gate too; one with slot[t] below 0 only keeps no row; one beyond the pool sets status bit 4. */
+bool q4_gpu_pages_prep(const q4_gpu_pages *pg, uint32_t layer, const void *q, const void *k, const void *v, int in_bf16, uint64_t q_stride,
+                       uint64_t kv_stride, uint32_t n_head, const float *wq, const float *wk, float eps, const q4_gpu_rope *rope, const int32_t *pos,
+                       const int32_t *slot, uint32_t n_tok, void *q_out, int q_out_bf16, float *gate);
+
+/* Pages with several holders.  shares: int32 [3 * n_pages] on the device, zeros for a new pool, beside the stack: shares[p] is the number of
+ * requests that hold page p besides the first; the rest is the calls' own and zero between them.  A pool whose requests share pages
+ * gives them back by release, never by trim.
+ * fork: request dst[i], which holds nothing, gets the first len[i] rows of request src[i]: the whole pages among them are held by both from now on,
+ * the rows of the page that they end in are copied, in all layers, to a page from the stack (whole tiles of 16 rows).  rows [n_req] are what the
+ * requests hold: rows[dst[i]] becomes len[i].  All forks see the requests as they were before the call.  Forks are served up to the first one that
+ * finds no page: it and those behind it get nothing, status bit 8.  One that cannot be (src or dst not a request, dst the place of an earlier fork of
+ * the call or holding rows, len below 0 or above rows[src], src's rows passing its table's row) gets nothing, status bit 4; an entry of src's that is
+ * no page of the pool is taken over as it is, status bit 4.  n_req, n_fork <= 8192. */
+bool q4_gpu_pages_fork(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, uint32_t n_req, const int32_t *src, const int32_t *dst, const int32_t *len,
+                       uint32_t n_fork, int32_t *table, uint32_t table_stride);
+/* As q4_gpu_pages_trim for pages that may be shared: request r keeps the first keep[r] of its rows[r] rows (0 or less: none), and rows[r] becomes that
+ * (where keep is less).  A page goes back on the stack with its last holder, in the order of those, and otherwise has a holder less.  A request that
+ * would keep only a part of the rows of a page that others hold too is left as it is, status bit 4 (its next rows would overwrite theirs): fork it at
+ * that length and release it.  More pages than are out, a page given back by more than hold it, or an entry that is no page of the pool: nothing goes back, rows
+ * stay, status bit 4.  Table entries stay as they are.  n_req <= 8192. */
+bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table,
+                          uint32_t table_stride);
+/* Moves the pages in use (those not on the stack) to the low end of the pool, in all layers: page i of those that lie behind it, in ascending
+ * order, to the i-th free one in front.  Then pages [0, n_pages - n_free) are in use and the stack hands out the others in ascending order.  map [n_pages] tells
+ * each page's new number (-1: free); shares (may be NULL) move along; the tables' entries of the requests' rows are renamed.  Tables that
+ * are not given here are the host's to rename by map.  A stack that names a page twice, or one that is not the pool's: nothing moves, map is the
+ * identity, status bit 4; a table's entry that is no page in use stays as it is, status bit 4.  n_req may be 0 (rows and table NULL).  Scratch (4 bytes
+ * per page) grows outside a capture only. */
+bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t *rows, uint32_t n_req, int32_t *table, uint32_t table_stride, int32_t *map);
+
+/* Drafted tokens held against the target's distributions, and the token behind the last one that is kept (no counterpart in the reference).  Request r
+ * brought the tokens token[start[r] .. start[r + 1]), as q4_gpu_pages_plan lays them out: the first is known, the others are its drafts.  Row t of
+ * logits [n_tok][vocab] (rows ld values apart, fp32 or bf16) is the target's for the token behind token t, row t of draft the draft's, from which token
+ * t + 1 was drawn (rows draft_ld apart, of the same type); draft NULL: drafts are certain.  With p, q the softmax of a row over temp[r] (NULL: 1):
+ *     the draft behind row t is kept while u_accept[t] * q(d) < p(d)         (certain drafts: q(d) = 1, others 0)
+ *     next: the first token whose running sum of w exceeds u_next[r] times the whole sum, w = max(p - q, 0) in the row whose draft was
+ *     refused (p where that is 0 throughout), w = p in the last row if all are kept
+ * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Sums, probabilities and
+ * comparisons are in 64 bits.
+ *   accepted, next [n_req]   drafts kept, and the token behind them
+ *   logp [n_tok] or NULL     row t's log p of the token that it decided (a kept draft, next), 0 for greedy requests and in rows behind next's
+ *   rows, keep [n_req]       or both NULL: keep[r] = rows[r] + accepted[r] + 1, rows[r] being what the request held before the step: for q4_gpu_pages_release
+ * A request without tokens: accepted 0, next -1, keep[r] = rows[r].  Logits of minus infinity are tokens that cannot be; a row that is needed and has a NaN, a plus infinity or
+ * no token at all, a temperature that is negative or not finite: next -1, status bit 4.  A draft outside the vocabulary is refused, status bit 4.  u in [0, 1).
+ * n_req <= 8192.  Scratch (32 bytes per row and 8192 logits) grows outside a capture only. */
+bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const void *draft, uint64_t draft_ld, uint32_t vocab, const int32_t *token, const int32_t *start,
+                   uint32_t n_req, uint32_t n_tok, const float *temp, const float *u_accept, const float *u_next, int32_t *accepted, int32_t *next, float *logp,
+                   const int32_t *rows, int32_t *keep);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,10 +11,9 @@
  * Either way a tile is contiguous and arrives by bulk copies as it is used.
  */
 #include "q4_paged.h"
+#include "q4_pages_scan.h"
 
 namespace {
-
-constexpr uint32_t PLAN_THREADS = 512, PLAN_MAX_REQ = 8192;
 
 /* blocks of a launch that have finished, in the upper half those that want the stack left alone; zero between launches */
 __device__ uint32_t g_plan_arrived;
@@ -27,43 +26,6 @@ struct PlanParams {
     uint32_t vec;                /* the token arrays take 16-byte stores */
     uint32_t *err;
 };
-
-/* exclusive sums over the block's threads of (a, b), and their totals */
-__device__ __forceinline__ void block_scan2(uint64_t &a, uint64_t &b, uint64_t &ta, uint64_t &tb) {
-    __shared__ uint64_t s_a[PLAN_THREADS / 32], s_b[PLAN_THREADS / 32];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint64_t a0 = a, b0 = b;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint64_t x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, b, d);
-        if (lane >= (uint32_t)d) { a += x; b += y; }
-    }
-    if (lane == 31u) { s_a[warp] = a; s_b[warp] = b; }
-    __syncthreads();
-    uint64_t pa = 0, pb = 0;
-    ta = tb = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < PLAN_THREADS / 32; w++) {
-        if (w < warp) { pa += s_a[w]; pb += s_b[w]; }
-        ta += s_a[w]; tb += s_b[w];
-    }
-    a += pa - a0;
-    b += pb - b0;
-}
-
-/* the last block to finish moves the stack's top, unless a thread of any block says no: all of them have read it by then */
-__device__ __forceinline__ void move_top(int32_t *n_free, int32_t to, uint32_t *err, bool no = false) {
-    const bool stays = __syncthreads_or(no);
-    if (threadIdx.x == 0) {
-        __threadfence();
-        const uint32_t mine = stays ? 0x10001u : 1u, all = atomicAdd(&g_plan_arrived, mine) + mine;
-        if ((all & 0xffffu) == gridDim.x) {
-            g_plan_arrived = 0u;
-            if (all >> 16) atomicOr(err, (uint32_t)Q4E_RANGE);
-            else *n_free = to;
-        }
-    }
-}
 
 /*
  * Plan.  With h rows held and n new tokens request r takes need = ceil((h + n) / P) - ceil(h / P) pages; page i of all of them,
@@ -165,7 +127,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_plan_k(const PlanParams P)
             }
         }
     }
-    move_top(P.n_free, (int32_t)(n_free - pages), P.err);
+    move_top(&g_plan_arrived, P.n_free, (int32_t)(n_free - pages), P.err);
 }
 
 /* Trim: pages ceil(kept / P) .. ceil(held / P) of every request go back, the last one of all lowest, so that a plan that is
@@ -217,7 +179,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_trim_k(const PlanParams P)
             P.free_list[n_free + all - 1u - i] = page;   /* above the top: of no meaning until that moves */
         }
     }
-    move_top(P.n_free, fits ? (int32_t)(n_free + all) : top, P.err, no_page);
+    move_top(&g_plan_arrived, P.n_free, fits ? (int32_t)(n_free + all) : top, P.err, no_page);
 }
 
 struct RowParams {

@@ -1,0 +1,508 @@
+/*
+ * Pages with several holders, and pools that are cut: fork (a prefix is taken over), release (pages go back with their last holder),
+ * compact (the pages in use are moved to the low end).  No counterpart in the reference, whose session holds its one cache alone.
+ *
+ * shares[p] counts the holders of page p besides the first, so that pages which plan hands out need no count and those of a pool
+ * without forks stay at zero.  Behind the counts lie two words per page that are the calls' own and zero between them.
+ */
+#include "q4_paged.h"
+#include "q4_pages_scan.h"
+
+namespace {
+
+/* blocks of a launch that have finished, as in q4_pages.cu; of fork, of release */
+__device__ uint32_t g_fork_arrived, g_rel_arrived;
+
+/* 16 bytes, by copies that go past L1 and are not wanted again */
+__device__ __forceinline__ uint4 load16(const uint8_t *p) { return __ldcs(reinterpret_cast<const uint4 *>(p)); }
+__device__ __forceinline__ void store16(uint8_t *p, uint4 x) { __stcs(reinterpret_cast<uint4 *>(p), x); }
+/* n bytes (a multiple of 16) by a warp, 16 * BATCH per lane on their way */
+template <uint32_t BATCH>
+__device__ __forceinline__ void warp_copy(uint8_t *to, const uint8_t *from, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 31u;
+    for (uint32_t at = lane * 16u; at < n; at += 512u * BATCH) {
+        uint4 x[BATCH];
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++)
+            if (at + i * 512u < n) x[i] = load16(from + at + i * 512u);
+#pragma unroll
+        for (uint32_t i = 0; i < BATCH; i++)
+            if (at + i * 512u < n) store16(to + at + i * 512u, x[i]);
+    }
+}
+
+struct ForkParams {
+    uint8_t *mem;
+    uint64_t layer_bytes;        /* of all pages */
+    uint32_t n_layers, n_kvh, tile_bytes, tiles;   /* tiles: of a page and kv head */
+    uint32_t n_req, n_fork, table_stride, page_shift, n_pages;
+    const int32_t *src, *dst, *len;
+    int32_t *rows, *table, *free_list, *n_free, *shares;
+    uint32_t *err;
+};
+
+/*
+ * Fork.  Every block forms the sums over all forks itself, as plan does; then the table entries of whole pages are shared out by threads,
+ * the tiles to copy (fork, layer, kv head, 16 rows) by warps.  The last block to finish writes what the others have read: the stack's top
+ * and the children's rows.
+ */
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P) {
+    extern __shared__ uint32_t s_fork[];
+    __shared__ uint64_t s_entries, s_tiles, s_pages;
+    __shared__ uint32_t s_last;
+    uint32_t *owner = s_fork, *entry_end = owner + P.n_req, *tile_end = entry_end + P.n_fork, *page_at = tile_end + P.n_fork;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, mask = (1u << P.page_shift) - 1u;
+    const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
+    for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) owner[r] = 0xffffffffu;
+    if (tid == 0) s_entries = s_tiles = s_pages = s_last = 0;
+    __syncthreads();
+    q4d_pdl_wait();
+    const int32_t top = *P.n_free;
+    const uint64_t n_free = top < 0 ? 0u : min((uint32_t)top, P.n_pages);
+    for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS) {   /* a place is the first fork's that names it */
+        const uint32_t d = (uint32_t)__ldcg(P.dst + i);
+        if (d < P.n_req) atomicMin(owner + d, i);
+    }
+    __syncthreads();
+    const uint32_t per = (P.n_fork + PLAN_THREADS - 1u) / PLAN_THREADS, i0 = min(tid * per, P.n_fork), i1 = min(i0 + per, P.n_fork);
+    auto one = [&](uint32_t i, uint64_t &entries, uint32_t &tiles) -> bool {
+        const uint32_t s = (uint32_t)__ldcg(P.src + i), d = (uint32_t)__ldcg(P.dst + i);
+        const int32_t n = __ldcg(P.len + i);
+        entries = tiles = 0u;
+        if (s >= P.n_req || d >= P.n_req || owner[d] != i || n < 0) return false;
+        const int32_t held = __ldcg(P.rows + s);
+        if (n > max(held, 0) || (uint64_t)max(held, 0) > room || __ldcg(P.rows + d) > 0) return false;
+        entries = (uint32_t)n >> P.page_shift;
+        tiles = (((uint32_t)n & mask) + 15u) >> 4;
+        return true;
+    };
+    uint64_t e_sum = 0, p_sum = 0, t_sum = 0, none = 0, e_all, p_all, t_all, none_all, e;
+    uint32_t t;
+    bool any_bad = false;
+    for (uint32_t i = i0; i < i1; i++) {
+        any_bad |= !one(i, e, t);
+        e_sum += e; t_sum += t; p_sum += t ? 1u : 0u;
+    }
+    block_scan2(e_sum, p_sum, e_all, p_all);
+    __syncthreads();
+    block_scan2(t_sum, none, t_all, none_all);
+    uint64_t fit_e = 0, fit_t = 0, fit_p = 0;
+    for (uint32_t i = i0; i < i1; i++) {
+        page_at[i] = one(i, e, t) ? (uint32_t)p_sum : 0xffffffffu;   /* 0xffffffff: it cannot be */
+        e_sum += e; t_sum += t; p_sum += t ? 1u : 0u;
+        const bool fits = p_sum <= n_free && e_sum < 0xffffffffu;
+        if (fits) { fit_e = e_sum; fit_t = t_sum; fit_p = p_sum; }
+        entry_end[i] = fits ? (uint32_t)e_sum : 0xffffffffu;   /* 0xffffffff: not served */
+        tile_end[i] = fits ? (uint32_t)t_sum : 0xffffffffu;
+    }
+    if (fit_e) atomicMax((unsigned long long *)&s_entries, (unsigned long long)fit_e);
+    if (fit_t) atomicMax((unsigned long long *)&s_tiles, (unsigned long long)fit_t);
+    if (fit_p) atomicMax((unsigned long long *)&s_pages, (unsigned long long)fit_p);
+    __syncthreads();
+    const uint32_t entries = (uint32_t)s_entries, tiles = (uint32_t)s_tiles, pages = (uint32_t)s_pages;
+    if (blockIdx.x == 0) {
+        if (any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+        if (tid == 0 && (p_all > pages || e_all > entries)) atomicOr(P.err, (uint32_t)Q4E_SCRATCH);
+    }
+    bool no_page = false;
+    for (uint64_t x = (uint64_t)blockIdx.x * PLAN_THREADS + tid; x < entries; x += (uint64_t)gridDim.x * PLAN_THREADS) {
+        const uint32_t i = first_above(entry_end, P.n_fork, (uint32_t)x), col = (uint32_t)x - (i ? entry_end[i - 1u] : 0u);
+        const int32_t page = P.table[(size_t)__ldcg(P.src + i) * P.table_stride + col];
+        P.table[(size_t)__ldcg(P.dst + i) * P.table_stride + col] = page;
+        if ((uint32_t)page < P.n_pages) atomicAdd(P.shares + page, 1);
+        else no_page = true;
+    }
+    const uint64_t units = (uint64_t)tiles * P.n_layers * P.n_kvh;
+    for (uint64_t u = (uint64_t)blockIdx.x * (PLAN_THREADS / 32u) + (tid >> 5); u < units; u += (uint64_t)gridDim.x * (PLAN_THREADS / 32u)) {
+        const uint64_t lk = u / tiles;
+        const uint32_t x = (uint32_t)(u - lk * tiles), i = first_above(tile_end, P.n_fork, x), tile = x - (i ? tile_end[i - 1u] : 0u);
+        const uint32_t layer = (uint32_t)(lk / P.n_kvh), kh = (uint32_t)(lk - (uint64_t)layer * P.n_kvh), col = (uint32_t)__ldcg(P.len + i) >> P.page_shift;
+        const int32_t old = P.table[(size_t)__ldcg(P.src + i) * P.table_stride + col], page = __ldcg(P.free_list + (n_free - 1u - page_at[i]));
+        if (lk == 0u && tile == 0u && lane == 0u) P.table[(size_t)__ldcg(P.dst + i) * P.table_stride + col] = page;
+        if ((uint32_t)old >= P.n_pages || (uint32_t)page >= P.n_pages) {
+            no_page = true;
+            continue;
+        }
+        uint8_t *at = P.mem + layer * P.layer_bytes + (uint64_t)(kh * P.tiles + tile) * P.tile_bytes;
+        const uint64_t page_bytes = (uint64_t)P.n_kvh * P.tiles * P.tile_bytes;
+        warp_copy<4>(at + (uint32_t)page * page_bytes, at + (uint32_t)old * page_bytes, P.tile_bytes);
+    }
+    if (no_page) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    bool no;
+    if (last_arrives(&g_fork_arrived, false, no)) {
+        *P.n_free = (int32_t)(n_free - pages);
+        s_last = 1u;
+    }
+    __syncthreads();
+    if (s_last)
+        for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS)
+            if (entry_end[i] != 0xffffffffu && page_at[i] != 0xffffffffu) P.rows[__ldcg(P.dst + i)] = __ldcg(P.len + i);
+}
+
+struct ReleaseParams {
+    int32_t *rows;
+    const int32_t *keep, *table;
+    uint32_t n_req, table_stride, page_shift, n_pages;
+    int32_t *free_list, *n_free, *shares;
+    uint32_t *err;
+};
+constexpr uint32_t REL_MAX_BLOCKS = 1024;
+/* between the launches of a call: entries given up, up to and with each request; its rows afterwards; entries of each block with which a page goes back */
+__device__ uint32_t g_rel_end[PLAN_MAX_REQ], g_rel_count[REL_MAX_BLOCKS];
+__device__ int32_t g_rel_rows[PLAN_MAX_REQ];
+__device__ uint32_t g_rel_bad;   /* nothing goes back; zero between calls */
+
+/*
+ * Release.  The entries that requests give up are numbered in the requests' order.  A page goes back with the last of its entries, if there are
+ * as many as it has holders: the first launch counts every page's entries and keeps the largest number, the second counts the pages that go back
+ * per block, the third puts them on the stack.  Which entry is a page's last does not depend on the order of the atomics.
+ */
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_k(const ReleaseParams P) {
+    extern __shared__ uint32_t s_end[];
+    const uint32_t tid = threadIdx.x, mask = (1u << P.page_shift) - 1u;
+    const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
+    q4d_pdl_wait();
+    const uint32_t per = (P.n_req + PLAN_THREADS - 1u) / PLAN_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
+    auto one = [&](uint32_t r, int32_t &after, bool &bad) -> uint32_t {
+        const int32_t h = __ldcg(P.rows + r), k = max(__ldcg(P.keep + r), 0);
+        after = h;
+        bad = h > 0 && (uint64_t)h > room;
+        if (bad || h <= 0 || k >= h) return 0u;
+        if ((uint32_t)k & mask) {   /* its next rows go where others' may be */
+            const int32_t page = P.table[(size_t)r * P.table_stride + ((uint32_t)k >> P.page_shift)];
+            bad = (uint32_t)page < P.n_pages && __ldcg(P.shares + page) > 0;
+            if (bad) return 0u;
+        }
+        after = k;
+        return (((uint32_t)h + mask) >> P.page_shift) - (((uint32_t)k + mask) >> P.page_shift);
+    };
+    uint64_t sum = 0, all, none = 0, none_all;
+    int32_t after;
+    bool bad, any_bad = false;
+    for (uint32_t r = r0; r < r1; r++) {
+        sum += one(r, after, bad);
+        any_bad |= bad;
+    }
+    block_scan2(sum, none, all, none_all);
+    const bool too_many = all > 0x7fffffffu;
+    for (uint32_t r = r0; r < r1; r++) {
+        sum += one(r, after, bad);
+        s_end[r] = too_many ? 0u : (uint32_t)sum;
+        if (blockIdx.x == 0) {
+            g_rel_end[r] = s_end[r];
+            g_rel_rows[r] = after;
+        }
+    }
+    if (blockIdx.x == 0) {
+        if (any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+        if (too_many && tid == 0) atomicOr(&g_rel_bad, 1u);
+    }
+    __syncthreads();
+    bool no_page = false;
+    int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
+    const uint32_t total = too_many ? 0u : (uint32_t)all;
+    for (uint64_t x = (uint64_t)blockIdx.x * PLAN_THREADS + tid; x < total; x += (uint64_t)gridDim.x * PLAN_THREADS) {
+        const uint32_t r = first_above(s_end, P.n_req, (uint32_t)x);
+        /* counted from the request's end */
+        const uint32_t pg = (((uint32_t)__ldcg(P.rows + r) + mask) >> P.page_shift) - (s_end[r] - (uint32_t)x);
+        const int32_t page = P.table[(size_t)r * P.table_stride + pg];
+        if ((uint32_t)page < P.n_pages) {
+            atomicAdd(times + page, 1);
+            atomicMax(last + page, (int32_t)x + 1);
+        } else {
+            no_page = true;
+        }
+    }
+    if (no_page) atomicOr(&g_rel_bad, 1u);
+}
+/* the page of entry x */
+__device__ __forceinline__ int32_t given_page(const ReleaseParams &P, const uint32_t *ends, uint32_t x) {
+    const uint32_t r = first_above(ends, P.n_req, x);
+    const uint32_t pg = (((uint32_t)__ldcg(P.rows + r) + (1u << P.page_shift) - 1u) >> P.page_shift) - (ends[r] - x);
+    return P.table[(size_t)r * P.table_stride + pg];
+}
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_count_k(const ReleaseParams P) {
+    extern __shared__ uint32_t s_end[];
+    __shared__ uint32_t s_count;
+    const uint32_t tid = threadIdx.x;
+    if (tid == 0) s_count = 0;
+    q4d_pdl_wait();
+    for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) s_end[r] = __ldcg(g_rel_end + r);
+    __syncthreads();
+    const int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
+    const uint32_t total = s_end[P.n_req - 1u], share = (total + gridDim.x - 1u) / gridDim.x;
+    const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
+    uint32_t n = 0;
+    bool bad = false;
+    for (uint64_t x = x0 + tid; x < x1; x += PLAN_THREADS) {
+        const int32_t page = given_page(P, s_end, (uint32_t)x);
+        if ((uint32_t)page >= P.n_pages || __ldcg(last + page) != (int32_t)x + 1) continue;
+        const int32_t held = __ldcg(P.shares + page) + 1, given = __ldcg(times + page);
+        n += given == held;
+        bad |= given > held;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((tid & 31u) == 0u && n) atomicAdd(&s_count, n);
+    if (bad) atomicOr(&g_rel_bad, 1u);
+    __syncthreads();
+    if (tid == 0) g_rel_count[blockIdx.x] = s_count;
+}
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_back_k(const ReleaseParams P) {
+    extern __shared__ uint32_t s_end[];
+    __shared__ uint32_t s_before, s_all, s_warp[PLAN_THREADS / 32u], s_last;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    if (tid == 0) s_before = s_all = s_last = 0;
+    __syncthreads();
+    q4d_pdl_wait();
+    for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) s_end[r] = __ldcg(g_rel_end + r);
+    for (uint32_t b = tid; b < gridDim.x; b += PLAN_THREADS) {
+        const uint32_t n = __ldcg(g_rel_count + b);
+        if (n) atomicAdd(&s_all, n);
+        if (n && b < blockIdx.x) atomicAdd(&s_before, n);
+    }
+    const int32_t top = *P.n_free;
+    __syncthreads();
+    const uint32_t all = s_all;
+    const uint64_t n_free = top < 0 ? 0u : (uint32_t)top;
+    const bool good = !*(volatile uint32_t *)&g_rel_bad && n_free + all <= P.n_pages;
+    int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
+    const uint32_t total = s_end[P.n_req - 1u], share = (total + gridDim.x - 1u) / gridDim.x;
+    const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
+    uint32_t before = s_before;
+    for (uint64_t x = x0; x < x1; x += PLAN_THREADS) {   /* the block stays together */
+        int32_t page = -1;
+        bool mine = false, goes = false;
+        if (x + tid < x1) {
+            page = given_page(P, s_end, (uint32_t)(x + tid));
+            if ((uint32_t)page < P.n_pages) {
+                if (!good) {
+                    times[page] = last[page] = 0;
+                } else if (__ldcg(last + page) == (int32_t)(x + tid) + 1) {
+                    const int32_t held = __ldcg(P.shares + page) + 1, given = __ldcg(times + page);
+                    mine = true;
+                    goes = given == held;
+                    P.shares[page] = goes ? 0 : held - given - 1;
+                    times[page] = last[page] = 0;   /* the others of its entries find that they are not the last, whichever value they read */
+                }
+            }
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine && goes);
+        if (lane == 0) s_warp[warp] = __popc(votes);
+        __syncthreads();
+        uint32_t at = before;
+        for (uint32_t w = 0; w < PLAN_THREADS / 32u; w++) {
+            if (w < warp) at += s_warp[w];
+            before += s_warp[w];
+        }
+        if (mine && goes) P.free_list[n_free + all - 1u - (at + __popc(votes & ((1u << lane) - 1u)))] = page;
+        __syncthreads();
+    }
+    bool no;
+    if (last_arrives(&g_rel_arrived, !good, no)) {
+        if (no) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+        else *P.n_free = (int32_t)(n_free + all);
+        g_rel_bad = 0u;
+        s_last = no ? 0u : 1u;
+    }
+    __syncthreads();
+    if (s_last)
+        for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) P.rows[r] = __ldcg(g_rel_rows + r);
+}
+
+struct CompactParams {
+    uint8_t *mem;
+    uint64_t layer_bytes, page_bytes;
+    uint32_t n_layers, n_req, table_stride, page_shift, n_pages;
+    const int32_t *rows;
+    int32_t *table, *free_list, *n_free, *shares, *map;
+    int32_t *hole;               /* pages to fill, and behind as many of them as there are pages in use those to move, in ascending order */
+    uint32_t *err;
+};
+constexpr uint32_t CMP_THREADS = 1024, CMP_WORDS = 40960;   /* 160 KB: 1.3 M pages at once */
+__device__ uint32_t g_cmp_moves, g_cmp_good;
+
+/*
+ * Compact.  Which pages go where follows from the stack alone: one block marks the free pages as bits in shared memory and counts them off
+ * (65 536 pages: 8 KB of bits; larger pools in windows).  Then all copy.
+ */
+__global__ void __launch_bounds__(CMP_THREADS) q4_pg_cmp_plan_k(const CompactParams P) {
+    extern __shared__ uint32_t s_bits[];
+    __shared__ uint32_t s_hole[32], s_move[32];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    q4d_pdl_wait();
+    const int32_t top = *P.n_free;
+    const bool fits = top >= 0 && (uint32_t)top <= P.n_pages;
+    const uint32_t n_free = fits ? (uint32_t)top : 0u, live = P.n_pages - n_free;
+    int32_t *const moving = P.hole + live;
+    bool bad = !fits;
+    uint32_t n_hole = 0, n_move = 0;
+    for (uint32_t w0 = 0; w0 < P.n_pages; w0 += CMP_WORDS * 32u) {   /* below 2^31 - 2^21: no wrap */
+        const uint32_t pages = min(P.n_pages - w0, CMP_WORDS * 32u), words = (pages + 31u) / 32u;
+        for (uint32_t w = tid; w < words; w += CMP_THREADS) s_bits[w] = 0u;
+        __syncthreads();
+        for (uint32_t i = tid; i < n_free; i += CMP_THREADS) {
+            const uint32_t p = (uint32_t)__ldcg(P.free_list + i);
+            if (p >= P.n_pages) bad = true;
+            else if (p - w0 < pages) bad |= (atomicOr(s_bits + ((p - w0) >> 5), 1u << (p & 31u)) >> (p & 31u)) & 1u;
+        }
+        __syncthreads();
+        const uint32_t per = (words + CMP_THREADS - 1u) / CMP_THREADS, a = min(tid * per, words), b = min(a + per, words);
+        auto of = [&](uint32_t w, uint32_t &hole, uint32_t &move) {
+            const uint32_t p = w0 + w * 32u, bits = s_bits[w];
+            const uint32_t there = P.n_pages - p >= 32u ? 0xffffffffu : (1u << (P.n_pages - p)) - 1u;
+            const uint32_t low = p >= live ? 0u : live - p >= 32u ? 0xffffffffu : (1u << (live - p)) - 1u;
+            hole = bits & low;
+            move = ~bits & ~low & there;
+        };
+        uint32_t h = 0, m = 0, hole, move;
+        for (uint32_t w = a; w < b; w++) {
+            of(w, hole, move);
+            h += __popc(hole);
+            m += __popc(move);
+        }
+        uint32_t hs = h, ms = m;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, hs, d), y = __shfl_up_sync(0xffffffffu, ms, d);
+            if (lane >= (uint32_t)d) { hs += x; ms += y; }
+        }
+        if (lane == 31u) { s_hole[warp] = hs; s_move[warp] = ms; }
+        __syncthreads();
+        uint32_t hb = n_hole + hs - h, mb = n_move + ms - m;
+        for (uint32_t w = 0; w < 32u; w++) {
+            if (w < warp) { hb += s_hole[w]; mb += s_move[w]; }
+            n_hole += s_hole[w]; n_move += s_move[w];
+        }
+        for (uint32_t w = a; w < b; w++) {
+            of(w, hole, move);
+            for (; hole; hole &= hole - 1u) P.hole[hb++] = (int32_t)(w0 + w * 32u + (uint32_t)__ffs((int)hole) - 1u);
+            for (; move; move &= move - 1u) moving[mb++] = (int32_t)(w0 + w * 32u + (uint32_t)__ffs((int)move) - 1u);
+        }
+        for (uint32_t i = tid; i < pages; i += CMP_THREADS) P.map[w0 + i] = (s_bits[i >> 5] >> (i & 31u)) & 1u ? -1 : (int32_t)(w0 + i);
+        __syncthreads();
+    }
+    const bool good = !__syncthreads_or(bad) && n_hole == n_move;
+    if (good)
+        for (uint32_t k = tid; k < n_move; k += CMP_THREADS) P.map[moving[k]] = P.hole[k];
+    else
+        for (uint32_t p = tid; p < P.n_pages; p += CMP_THREADS) P.map[p] = (int32_t)p;
+    if (tid == 0) {
+        g_cmp_moves = good ? n_move : 0u;
+        g_cmp_good = good;
+        if (!good) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    }
+}
+constexpr uint32_t CMP_UNIT = 4096;   /* bytes that a warp moves at once */
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_cmp_move_k(const CompactParams P) {
+    const uint32_t tid = threadIdx.x, threads = gridDim.x * PLAN_THREADS, me = blockIdx.x * PLAN_THREADS + tid;
+    q4d_pdl_wait();
+    if (!__ldcg(&g_cmp_good)) return;
+    const uint32_t n_move = __ldcg(&g_cmp_moves), n_free = (uint32_t)__ldcg(P.n_free);
+    const int32_t *const moving = P.hole + (P.n_pages - n_free);
+    for (uint32_t i = me; i < n_free; i += threads) P.free_list[i] = (int32_t)(P.n_pages - 1u - i);
+    if (P.shares)
+        for (uint32_t k = me; k < n_move; k += threads) {
+            const int32_t from = __ldcg(moving + k);
+            P.shares[__ldcg(P.hole + k)] = P.shares[from];
+            P.shares[from] = 0;
+        }
+    bool bad = false;
+    for (uint32_t r = blockIdx.x; r < P.n_req; r += gridDim.x) {
+        const int32_t h = __ldcg(P.rows + r);
+        uint64_t n = h > 0 ? ((uint64_t)(uint32_t)h + (1u << P.page_shift) - 1u) >> P.page_shift : 0u;
+        if (n > P.table_stride) { n = P.table_stride; bad = true; }
+        for (uint32_t c = tid; c < n; c += PLAN_THREADS) {
+            int32_t *entry = P.table + (size_t)r * P.table_stride + c;
+            const uint32_t page = (uint32_t)*entry;
+            const int32_t to = page < P.n_pages ? __ldcg(P.map + page) : -1;
+            if (to < 0) bad = true;
+            else if ((uint32_t)to != page) *entry = to;
+        }
+    }
+    if (bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    const uint32_t parts = (uint32_t)((P.page_bytes + CMP_UNIT - 1u) / CMP_UNIT);
+    const uint64_t units = (uint64_t)n_move * P.n_layers * parts;
+    for (uint64_t u = me >> 5; u < units; u += threads >> 5) {
+        const uint64_t pl = u / parts;
+        const uint32_t at = (uint32_t)(u - pl * parts) * CMP_UNIT, k = (uint32_t)(pl / P.n_layers), layer = (uint32_t)(pl - (uint64_t)k * P.n_layers);
+        uint8_t *base = P.mem + layer * P.layer_bytes + at;
+        warp_copy<8>(base + (uint32_t)__ldcg(P.hole + k) * P.page_bytes, base + (uint32_t)__ldcg(moving + k) * P.page_bytes, (uint32_t)min((uint64_t)CMP_UNIT, P.page_bytes - at));
+    }
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
+uint64_t page_bytes_of(const q4_gpu_pages *pg) { return (uint64_t)q4i_pages_row_bytes(pg->hd, pg->kind) * pg->page_rows * pg->n_kvh; }
+/* blocks for so many items of a thread each, one per SM at most */
+uint32_t blocks_for(uint64_t items) {
+    const uint64_t want = (items + PLAN_THREADS - 1u) / PLAN_THREADS, cap = (uint64_t)g_q4.sm_count;
+    return (uint32_t)(want < 1u ? 1u : want < cap ? want : cap);
+}
+
+}  // namespace
+
+extern "C" bool q4_gpu_pages_fork(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, uint32_t n_req, const int32_t *src, const int32_t *dst, const int32_t *len,
+                                  uint32_t n_fork, int32_t *table, uint32_t table_stride) {
+    if (!g_q4.ok) return q4i_fail(Q4E_INIT, "pages_fork: library not initialised");
+    Q4_REQUIRE(q4i_pages_ok(pg) && pg->mem && aligned16(pg->mem) && pg->free_list && pg->n_free, "pages_fork: bad pool");
+    Q4_REQUIRE(shares && rows && src && dst && len && table && n_req && n_fork && table_stride, "pages_fork: bad argument");
+    Q4_REQUIRE(n_req <= PLAN_MAX_REQ && n_fork <= PLAN_MAX_REQ, "pages_fork: at most 8192 requests and forks");
+    Q4_REQUIRE((uint64_t)table_stride * pg->page_rows <= 0x7fffffffu, "pages_fork: a block table's rows pass 2^31 - 1");
+    ForkParams p = {};
+    p.mem = (uint8_t *)pg->mem;
+    p.layer_bytes = page_bytes_of(pg) * pg->n_pages;
+    p.n_layers = pg->n_layers; p.n_kvh = pg->n_kvh;
+    p.tile_bytes = 16u * q4i_pages_row_bytes(pg->hd, pg->kind); p.tiles = pg->page_rows / 16u;
+    p.n_req = n_req; p.n_fork = n_fork; p.table_stride = table_stride; p.n_pages = pg->n_pages;
+    p.page_shift = (uint32_t)__builtin_ctz(pg->page_rows);
+    p.src = src; p.dst = dst; p.len = len; p.rows = rows; p.table = table;
+    p.free_list = pg->free_list; p.n_free = pg->n_free; p.shares = shares;
+    p.err = g_q4.err_d;
+    static bool attr = false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_fork_k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(4u * PLAN_MAX_REQ * sizeof(uint32_t))), "pages_fork smem attribute")) return false;
+    attr = true;
+    /* a warp per tile to copy, or a thread per entry, up to two blocks per SM */
+    const uint64_t tiles = (uint64_t)n_fork * p.tiles * p.n_layers * p.n_kvh, items = tiles * 32u + (uint64_t)n_fork * table_stride, want = (items + PLAN_THREADS - 1u) / PLAN_THREADS, cap = 2u * (uint64_t)g_q4.sm_count;
+    return q4i_launch_pdl("pages_fork launch", q4_pg_fork_k, dim3((unsigned)(want < cap ? want : cap)), PLAN_THREADS, (n_req + 3u * (size_t)n_fork) * sizeof(uint32_t), p);
+}
+
+extern "C" bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table, uint32_t table_stride) {
+    if (!g_q4.ok) return q4i_fail(Q4E_INIT, "pages_release: library not initialised");
+    Q4_REQUIRE(q4i_pages_ok(pg) && pg->free_list && pg->n_free, "pages_release: bad pool");
+    Q4_REQUIRE(shares && rows && keep && table && n_req && table_stride, "pages_release: bad argument");
+    Q4_REQUIRE(n_req <= PLAN_MAX_REQ, "pages_release: at most 8192 requests");
+    Q4_REQUIRE((uint64_t)table_stride * pg->page_rows <= 0x7fffffffu, "pages_release: a block table's rows pass 2^31 - 1");
+    ReleaseParams p = {};
+    p.rows = rows; p.keep = keep; p.n_req = n_req; p.table = table; p.table_stride = table_stride; p.n_pages = pg->n_pages;
+    p.page_shift = (uint32_t)__builtin_ctz(pg->page_rows);
+    p.free_list = pg->free_list; p.n_free = pg->n_free; p.shares = shares;
+    p.err = g_q4.err_d;
+    const dim3 grid(blocks_for((uint64_t)n_req * table_stride));
+    if (grid.x > REL_MAX_BLOCKS) return q4i_fail(Q4E_CUDA, "pages_release: more SMs than the counts are for");
+    const size_t smem = n_req * sizeof(uint32_t);
+    return q4i_launch_pdl("pages_release launch", q4_pg_give_k, grid, PLAN_THREADS, smem, p) &&
+           q4i_launch_pdl("pages_release launch", q4_pg_give_count_k, grid, PLAN_THREADS, smem, p) &&
+           q4i_launch_pdl("pages_release launch", q4_pg_give_back_k, grid, PLAN_THREADS, smem, p);
+}
+
+extern "C" bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t *rows, uint32_t n_req, int32_t *table, uint32_t table_stride, int32_t *map) {
+    if (!g_q4.ok) return q4i_fail(Q4E_INIT, "pages_compact: library not initialised");
+    Q4_REQUIRE(q4i_pages_ok(pg) && pg->mem && aligned16(pg->mem) && pg->free_list && pg->n_free, "pages_compact: bad pool");
+    Q4_REQUIRE(map && (!n_req || (rows && table && table_stride)), "pages_compact: bad argument");
+    Q4_REQUIRE((uint64_t)table_stride * pg->page_rows <= 0x7fffffffu, "pages_compact: a block table's rows pass 2^31 - 1");
+    if (!q4i_scratch(pg->n_pages, 0)) return false;
+    CompactParams p = {};
+    p.mem = (uint8_t *)pg->mem;
+    p.page_bytes = page_bytes_of(pg);
+    p.layer_bytes = p.page_bytes * pg->n_pages;
+    p.n_layers = pg->n_layers; p.n_req = n_req; p.table_stride = table_stride; p.n_pages = pg->n_pages;
+    p.page_shift = (uint32_t)__builtin_ctz(pg->page_rows);
+    p.rows = rows; p.table = table; p.free_list = pg->free_list; p.n_free = pg->n_free; p.shares = shares; p.map = map;
+    p.hole = (int32_t *)g_q4.part;
+    p.err = g_q4.err_d;
+    const uint32_t words = (pg->n_pages + 31u) / 32u;
+    static bool attr = false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_cmp_plan_k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(CMP_WORDS * sizeof(uint32_t))), "pages_compact smem attribute")) return false;
+    attr = true;
+    return q4i_launch_pdl("pages_compact launch", q4_pg_cmp_plan_k, dim3(1), CMP_THREADS, (words < CMP_WORDS ? words : CMP_WORDS) * sizeof(uint32_t), p) &&
+           q4i_launch_pdl("pages_compact launch", q4_pg_cmp_move_k, dim3(2u * (unsigned)g_q4.sm_count), PLAN_THREADS, 0, p);
+}

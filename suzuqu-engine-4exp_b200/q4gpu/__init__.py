@@ -15,8 +15,8 @@ HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include", "
 KIND_F32, KIND_F16, KIND_Q8 = 0, 1, 2
 KIND_NAMES = {"f32": 0, "fp32": 0, "f16": 1, "fp16": 1, "q8": 2, "q8_0": 2}
 
-_b, _v, _u32, _i32, _u64, _f, _sz, _i = (C.c_bool, C.c_void_p, C.c_uint32, C.c_int32, C.c_uint64,
-                                        C.c_float, C.c_size_t, C.c_int)
+_b, _v, _u32, _i32, _u64, _f, _sz, _i, _d = (C.c_bool, C.c_void_p, C.c_uint32, C.c_int32, C.c_uint64,
+                                            C.c_float, C.c_size_t, C.c_int, C.c_double)
 
 # name -> (restype, argtypes); mirrors include/q4_gpu.h declaration by declaration
 SIGNATURES = {
@@ -99,6 +99,12 @@ SIGNATURES = {
     "q4_gpu_pages_append": (_b, [_v, _u32, _v, _v, _v, _u32]),
     "q4_gpu_pages_gather": (_b, [_v, _u32, _v, _u32, _v, _v]),
     "q4_gpu_pages_attend": (_b, [_v, _u32, _v, _i, _v, _v, _i, _u32, _v, _v, _u32, _u32, _v, _u32, _u32, _f]),
+    "q4_gpu_rope_set": (_b, [_v, _u32, _i, _d, _i, _d, _d, _d, _d, _d]),
+    "q4_gpu_pages_prep": (_b, [_v, _u32, _v, _v, _v, _i, _u64, _u64, _u32, _v, _v, _f, _v, _v, _v, _u32, _v, _i, _v]),
+    "q4_gpu_pages_fork": (_b, [_v, _v, _v, _u32, _v, _v, _v, _u32, _v, _u32]),
+    "q4_gpu_pages_release": (_b, [_v, _v, _v, _v, _u32, _v, _u32]),
+    "q4_gpu_pages_compact": (_b, [_v, _v, _v, _u32, _v, _u32, _v]),
+    "q4_gpu_verify": (_b, [_v, _i, _u64, _v, _u64, _u32, _v, _v, _u32, _u32, _v, _v, _v, _v, _v, _v, _v, _v]),
 }
 
 
@@ -106,6 +112,21 @@ class PagesDesc(C.Structure):
     """q4_gpu_pages of include/q4_gpu.h: a pool of pages in the caller's memory"""
     _fields_ = [("mem", C.c_void_p), ("free_list", C.c_void_p), ("n_free", C.c_void_p), ("n_layers", C.c_uint32), ("n_kvh", C.c_uint32),
                 ("hd", C.c_uint32), ("n_pages", C.c_uint32), ("page_rows", C.c_uint32), ("kind", C.c_int)]
+
+
+class Rope(C.Structure):
+    """q4_gpu_rope of include/q4_gpu.h: how positions turn the first n_rot dims of a head, in pairs (2 i, 2 i + 1) or, half, (i, i + n_rot / 2).
+    scaling: None, or for contexts longer than orig positions by factor "linear", "ramp" (over the pairs between those that turn fast and slow
+    times in orig positions) or "smooth" (over the turns from slow to fast).  Needs no device."""
+    _fields_ = [("n_rot", C.c_uint32), ("half", C.c_int32), ("mag", C.c_float), ("reserved", C.c_uint32), ("turn", C.c_uint64 * 128)]
+    SCALINGS = {None: 0, "linear": 1, "ramp": 2, "smooth": 3}
+
+    def __init__(self, n_rot, base, half=False, scaling=None, factor=1.0, orig=0.0, fast=32.0, slow=1.0, mag=1.0):
+        super().__init__()
+        if scaling not in self.SCALINGS or not 0 <= n_rot <= 256:
+            raise RuntimeError("a scaling of %s and up to 256 dims are needed, not %r and %r" % (list(self.SCALINGS), scaling, n_rot))
+        self.p = C.addressof(self)
+        check(load().q4_gpu_rope_set(self.p, n_rot, int(half), base, self.SCALINGS[scaling], factor, orig, fast, slow, mag), "q4_gpu_rope_set")
 
 
 class SessDesc(C.Structure):
@@ -164,6 +185,14 @@ def _dense(t, dtype, n, gpu):
         raise RuntimeError("a dense tensor of %s on GPU %d with %d numbers is needed, not one of %s on %s, %s with strides %s"
                            % (dtype, gpu, n, t.dtype, t.device, tuple(t.shape), t.stride()))
     return t.data_ptr()
+
+
+def _rows(t, dtype, n_rows, width, gpu):
+    """address and row stride of a tensor [n_rows or more][width or more] of that type on that GPU, whose rows are dense"""
+    if t.dtype is not dtype or t.get_device() != gpu or t.dim() != 2 or t.shape[0] < n_rows or t.shape[1] < width or t.stride(1) != 1 or t.stride(0) < width:
+        raise RuntimeError("rows of %d numbers of %s on GPU %d are needed, %d of them, not one of %s on %s, %s with strides %s"
+                           % (width, dtype, gpu, n_rows, t.dtype, t.device, tuple(t.shape), t.stride()))
+    return t.data_ptr(), t.stride(0)
 
 
 def check(ok, what):
@@ -408,7 +437,7 @@ class PagePool:
     (RuntimeError), as are ones too small for the call; the pool's memory and its stack of free pages are allocated here unless they
     are given.  Per step: plan, then append and attend for every layer."""
 
-    def __init__(self, n_layers, n_kvh, hd, n_pages, page_rows=64, kind=KIND_Q8, mem=None, free=None, n_free=None):
+    def __init__(self, n_layers, n_kvh, hd, n_pages, page_rows=64, kind=KIND_Q8, mem=None, free=None, n_free=None, shares=None):
         import torch
         self.L = init()
         size = self.L.q4_gpu_pages_bytes(n_layers, n_kvh, hd, n_pages, page_rows, kind)
@@ -421,16 +450,17 @@ class PagePool:
             mem = torch.empty(size, dtype=torch.uint8, device=on)
             free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=on)   # page 0 is on top
             n_free = torch.full((1,), n_pages, dtype=torch.int32, device=on)
+            shares = torch.zeros(3 * n_pages, dtype=torch.int32, device=on) if shares is None else shares
         if (free is None) != (n_free is None):
             raise RuntimeError("the stack of free pages and its height go together")
         if mem is not None and mem.numel() * mem.element_size() < size:
             raise RuntimeError("the pool's memory is smaller than q4_gpu_pages_bytes (%d)" % size)
-        self.mem, self.free, self.n_free = mem, free, n_free
+        self.mem, self.free, self.n_free, self.shares = mem, free, n_free, shares   # shares: holders besides the first, fork and release count them
         self.n_layers, self.n_kvh, self.hd, self.n_pages, self.page_rows, self.kind = n_layers, n_kvh, hd, n_pages, page_rows, kind
         at = (_dense(mem, None if mem is None else mem.dtype, 1, gpu), _dense(free, torch.int32, n_pages, gpu), _dense(n_free, torch.int32, 1, gpu))
         self.desc = PagesDesc(*at, n_layers, n_kvh, hd, n_pages, page_rows, kind)
-        self.p, self.width = C.addressof(self.desc), n_kvh * hd
-        self.calls = [getattr(self.L, "q4_gpu_pages_" + name) for name in ("plan", "trim", "append", "gather", "attend")]
+        self.p, self.width, self.shared = C.addressof(self.desc), n_kvh * hd, _dense(shares, torch.int32, 3 * n_pages, gpu)
+        self.calls = [getattr(self.L, "q4_gpu_pages_" + name) for name in ("plan", "trim", "append", "gather", "attend", "prep", "fork", "release", "compact")]
         self.i32, self.f32, self.bf16 = torch.int32, torch.float32, torch.bfloat16
 
     # a call costs the host as much as a small launch the device: addresses are taken once, functions looked up above
@@ -473,3 +503,56 @@ class PagePool:
                              _dense(out, self.bf16 if out_bf16 else self.f32, x, gpu), out_bf16, n_head, _dense(rows, i, n, gpu), _dense(start, i, n + 1, gpu), n, x // per,
                              _dense(table, i, n * stride, gpu), stride, max_add, scale):
             check(False, "q4_gpu_pages_attend")
+
+    def prep(self, layer, q, k, v, q_out, pos, slot, rope, wq=None, wk=None, eps=1e-6, gate=None):
+        """the projections' rows made ready for attend: q [n_tok][n_head * hd], or [n_head][q | gate] where gate is given, k and v [n_tok][n_kvh * hd], fp32 or
+        bf16, each dense in its rows (k and v at one stride); q_out [n_tok][n_head][hd], gate likewise fp32; pos and slot as plan made them; wq, wk [hd]; eps None: no norm"""
+        gpu, m, dtype = self.gpu, pos.shape[0], q.dtype
+        if q_out.dim() != 3 or q_out.shape[2] != self.hd or (dtype is not self.f32 and dtype is not self.bf16):
+            raise RuntimeError("queries of %s are no heads of %d, or those of %s neither fp32 nor bf16" % (tuple(q_out.shape), self.hd, dtype))
+        n_head, q_bf16 = q_out.shape[1], q_out.dtype is self.bf16
+        x = n_head * self.hd
+        (qp, qs), (kp, ks), (vp, vs) = _rows(q, dtype, m, x if gate is None else 2 * x, gpu), _rows(k, dtype, m, self.width, gpu), _rows(v, dtype, m, self.width, gpu)
+        if ks != vs:
+            raise RuntimeError("the rows of k and v are %d and %d apart: one stride is needed" % (ks, vs))
+        if not self.calls[5](self.p, layer, qp, kp, vp, dtype is self.bf16, qs, ks, n_head, _dense(wq, self.f32, self.hd, gpu), _dense(wk, self.f32, self.hd, gpu),
+                             -1.0 if eps is None else eps, rope.p, _dense(pos, self.i32, m, gpu), _dense(slot, self.i32, m, gpu), m,
+                             _dense(q_out, self.bf16 if q_bf16 else self.f32, m * x, gpu), q_bf16, _dense(gate, self.f32, m * x, gpu)):
+            check(False, "q4_gpu_pages_prep")
+
+    def fork(self, rows, src, dst, length, table):
+        """request dst[i], which holds nothing, gets the first length[i] rows of request src[i]; rows[dst[i]] becomes length[i]"""
+        i, gpu, (n, stride), m = self.i32, self.gpu, table.shape, src.shape[0]
+        if not self.calls[6](self.p, self.shared, _dense(rows, i, n, gpu), n, _dense(src, i, m, gpu), _dense(dst, i, m, gpu), _dense(length, i, m, gpu), m,
+                             _dense(table, i, n * stride, gpu), stride):
+            check(False, "q4_gpu_pages_fork")
+
+    def release(self, rows, keep, table):
+        """request r keeps the first keep[r] of its rows, which rows[r] becomes; pages go back with their last holder"""
+        i, gpu, (n, stride) = self.i32, self.gpu, table.shape
+        if not self.calls[7](self.p, self.shared, _dense(rows, i, n, gpu), _dense(keep, i, n, gpu), n, _dense(table, i, n * stride, gpu), stride):
+            check(False, "q4_gpu_pages_release")
+
+    def compact(self, rows, table, number):
+        """the pages in use to the low end of the pool; number [n_pages] gets every page's new one (-1: free).  rows and table None: the tables are renamed by the host"""
+        i, gpu = self.i32, self.gpu
+        n, stride = (0, 0) if table is None else table.shape
+        if (rows is None) != (table is None):
+            raise RuntimeError("a table and what its requests hold go together")
+        if not self.calls[8](self.p, self.shared, _dense(rows, i, n, gpu), n, _dense(table, i, n * stride, gpu), stride, _dense(number, i, self.n_pages, gpu)):
+            check(False, "q4_gpu_pages_compact")
+
+
+def verify(logits, token, start, u_accept, u_next, accepted, next, draft=None, temp=None, logp=None, rows=None, keep=None):
+    """drafted tokens held against the target's logits [n_tok][vocab] (fp32 or bf16, dense in its rows, as draft's), and the token behind the last one that is
+    kept (q4_gpu_verify): token [n_tok] and start [n_req + 1] as the step was planned, u_accept [n_tok], u_next, accepted, next, temp, rows and keep [n_req], logp [n_tok]"""
+    import torch
+    L = load()
+    gpu, (m, vocab), n, dtype, i, f = L.q4_gpu_device(), logits.shape, start.shape[0] - 1, logits.dtype, torch.int32, torch.float32
+    if dtype is not f and dtype is not torch.bfloat16:
+        raise RuntimeError("logits of %s are neither fp32 nor bf16" % dtype)
+    (p, ld), (d, draft_ld) = _rows(logits, dtype, m, vocab, gpu), (None, 0) if draft is None else _rows(draft, dtype, m, vocab, gpu)
+    if not L.q4_gpu_verify(p, dtype is torch.bfloat16, ld, d, draft_ld, vocab, _dense(token, i, m, gpu), _dense(start, i, n + 1, gpu), n, m, _dense(temp, f, n, gpu),
+                           _dense(u_accept, f, m, gpu), _dense(u_next, f, n, gpu), _dense(accepted, i, n, gpu), _dense(next, i, n, gpu), _dense(logp, f, m, gpu),
+                           _dense(rows, i, n, gpu), _dense(keep, i, n, gpu)):
+        check(False, "q4_gpu_verify")
