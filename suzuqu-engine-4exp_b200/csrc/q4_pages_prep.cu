@@ -17,14 +17,15 @@
 
 namespace {
 
-constexpr uint32_t PREP_THREADS = 256, PREP_WARPS = PREP_THREADS / 32u;
+constexpr uint32_t PREP_THREADS = 32;   /* warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 79 us, in pairs 99, in eights 115) */
 
 struct PrepParams {
     uint8_t *mem;                /* of the layer */
     uint32_t n_head, n_kvh, n_tok, page_shift;
     uint32_t slots;              /* n_pages << page_shift */
     uint32_t q_bf16;             /* the type of q_out */
-    uint32_t jobs, per;          /* of a token: pairs of rows (query and gate, K and V), in groups of lanes; of a block */
+    uint32_t q_units, units;     /* warps of a token: those for its queries (and gates), then those for its keys and values */
+    uint32_t q_per, kv_per;      /* turns of each; a turn is a row, and its gate or value, per group of lanes */
     const void *q, *k, *v;
     uint64_t q_stride, kv_stride;
     const float *wq, *wk;
@@ -36,157 +37,209 @@ struct PrepParams {
     q4_gpu_rope rope;
 };
 
-/* four values of a row, as they lie */
+/* eight values of a row, as they lie */
 template <bool BF16>
-struct Four {
-    typename std::conditional<BF16, uint2, float4>::type x;
-    __device__ __forceinline__ void load(const void *base, uint64_t at) {
-        if constexpr (BF16) x = __ldcs(reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(base) + at));
-        else x = __ldcs(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at));
+struct Eight {
+    uint4 x[BF16 ? 1 : 2];
+    __device__ __forceinline__ void load(const uint8_t *p, bool live) {
+#pragma unroll
+        for (int i = 0; i < (BF16 ? 1 : 2); i++) x[i] = live ? __ldcs(reinterpret_cast<const uint4 *>(p) + i) : make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ void none() {
-        if constexpr (BF16) x = make_uint2(0u, 0u);
-        else x = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __device__ __forceinline__ float4 get() const {
-        if constexpr (BF16)
-            return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u));
-        else return x;
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        const uint32_t *u = reinterpret_cast<const uint32_t *>(x);
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = __uint_as_float(BF16 ? (i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16) : u[BF16 ? 0 : i]);
     }
 };
-__device__ __forceinline__ uint2 to_bf16(float4 x) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-    return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+__device__ __forceinline__ void eight_floats(const float *p, float (&f)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void store_floats(float *p, const float (&f)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
 
-/* A row lies in LPR lanes, CH groups of four dims each, 128 dims apart: the eight lanes of a q8_0 block are neighbours at every head size, and
- * at hd 64 a warp has two rows.  A job is a query row and its gate, or a K row and its V: both are on their way at once. */
-template <int KIND, int HD, bool BF16, uint32_t TOK>
+/*
+ * A warp has a token's queries, or its keys and values, or a part of them where there are few tokens, and keeps what belongs to the token in registers:
+ * sines and cosines, with the weights in them.  Lanes hold eight dims of a row each, so that a warp has 1, 2 or 4 rows at a time (hd 256, 128, 64).  The
+ * warps' issue slots set the pace beside memory (16 001 rows of a fused bf16 projection 169 us with four dims per lane).  A turn's rows are requested
+ * before the one before them is worked at, the first before the token's position is there.
+ */
+template <int KIND, int HD, bool BF16, bool HALF, bool FULL>
 __global__ void __launch_bounds__(PREP_THREADS) q4_pg_prep_k(const __grid_constant__ PrepParams P) {
-    constexpr uint32_t LPR = HD == 64 ? 16u : 32u, RPW = 32u / LPR, CH = HD / (4u * LPR);
-    __shared__ float4 cs[TOK][64];       /* (cos, sin) of two pairs */
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, in = lane % LPR;
-    const uint32_t np = P.rope.n_rot / 2u, t0 = blockIdx.x * TOK;
+    constexpr uint32_t LPR = HD / 8u, RPW = 32u / LPR, U = BF16 ? 2u : 1u, SIZE = BF16 ? 2u : 4u;   /* U: turns at a time, as many bytes on their way in either type */
+    const uint32_t lane = threadIdx.x, in = lane % LPR, sub = lane / LPR, unit = blockIdx.x;
+    const uint32_t tok = unit / P.units, which = unit - tok * P.units;
+    const bool is_q = which < P.q_units;
+    const uint32_t heads = is_q ? P.n_head : P.n_kvh, per = is_q ? P.q_per : P.kv_per, first = (is_q ? which : which - P.q_units) * per * RPW + sub, behind = min(first - sub + per * RPW, heads);
     q4d_pdl_wait();
-    for (uint32_t i = tid; i < TOK * np; i += PREP_THREADS) {
-        const uint32_t t = TOK == 1u ? 0u : i / np, pair = i - t * np;
-        const int32_t pos = t0 + t < P.n_tok ? __ldcg(P.pos + t0 + t) : 0;
-        const uint64_t angle = (uint64_t)(uint32_t)pos * P.rope.turn[pair];
-        float s, c;
-        sincospif((float)(int32_t)(angle >> 32) * 4.656612873077393e-10f, &s, &c);   /* 2^-31: half turns */
-        reinterpret_cast<float2 *>(cs[t])[pair] = make_float2(c * P.rope.mag, s * P.rope.mag);
+    const int32_t pos = __ldcg(P.pos + tok);
+
+    /* rows of the group's heads: first, first + RPW .. */
+    const bool two = !is_q || P.gate;      /* a second row: gate or value */
+    const uint32_t step = RPW * HD * (is_q && P.gate ? 2u : 1u) * SIZE;
+    const uint64_t at = (is_q ? tok * P.q_stride : tok * P.kv_stride) + (uint64_t)first * (HD * (is_q && P.gate ? 2u : 1u)) + in * 8u;
+    const uint8_t *pa = (const uint8_t *)(is_q ? P.q : P.k) + at * SIZE, *pb = is_q ? pa + HD * SIZE : (const uint8_t *)P.v + at * SIZE;
+    Eight<BF16> a[U], b[U], a_next[U], b_next[U];
+    auto load = [&](uint32_t head, Eight<BF16> (&x)[U], Eight<BF16> (&y)[U]) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const bool live = head + u * RPW < behind;
+            x[u].load(pa, live);
+            if (two) y[u].load(pb, live);
+            pa += step;
+            pb += step;
+        }
+    };
+    load(first, a, b);
+
+    if (pos < 0) return;
+    /* The warp's lanes take the sines and cosines of the head's pairs, C consecutive ones each, for one another */
+    const uint32_t n_rot = P.rope.n_rot, np = n_rot / 2u;
+    constexpr uint32_t C = HD / 64u;
+    float cs[C], sn[C];
+    {
+        const uint64_t *turn;              /* as memory: the lanes' addresses differ, which the constant port takes one by one */
+        asm("mov.u64 %0, %1;" : "=l"(turn) : "l"(P.rope.turn));
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++) {
+            const uint64_t angle = (uint64_t)(uint32_t)pos * turn[lane * C + i];
+            sincospif((float)(int32_t)(angle >> 32) * 4.656612873077393e-10f, &sn[i], &cs[i]);   /* 2^-31: half turns */
+            cs[i] *= P.rope.mag;
+            sn[i] *= P.rope.mag;
+        }
     }
-    __syncthreads();
-    const uint32_t j0 = blockIdx.y * P.per, j1 = min(j0 + P.per, P.jobs), n_jobs = (j1 - j0) * TOK;
-    for (uint32_t g = (tid >> 5) * RPW + lane / LPR; g - lane / LPR < n_jobs; g += PREP_WARPS * RPW) {   /* the lanes of a warp stay together */
-        const uint32_t t = TOK == 1u ? 0u : g / (j1 - j0), job = j0 + g - t * (j1 - j0), tok = t0 + t;
-        const bool is_q = job < P.n_head, mine = g < n_jobs && tok < P.n_tok;
-        const uint32_t head = is_q ? job : job - P.n_head;
-        const int32_t pos = mine ? __ldcg(P.pos + tok) : -1;
-        const bool live = pos >= 0;
-        Four<BF16> a[CH], b[CH];
-        const uint64_t at = is_q ? tok * P.q_stride + (uint64_t)head * (P.gate ? 2u * HD : HD) : tok * P.kv_stride + (uint64_t)head * HD;
+    /* What a dim is made of: x fa + y fb, y the pair's other dim.  Both hold the weights.  Dims that are not turned: x fa */
+    float fa[8], fb[8];
+    uint32_t on = 0;                       /* dims that are turned */
+    const uint32_t quarter = np / 4u, swap = quarter & 1u;
+    uint32_t from[2] = {0u, 0u};           /* halves: the lanes where the other dims of the lane's two groups of four lie, in which of its groups is the same for all lanes */
+    {
+        const float *wn = P.eps >= 0.f ? (is_q ? P.wq : P.wk) : nullptr;
+        float w[8];
 #pragma unroll
-        for (uint32_t c = 0; c < CH; c++) {
-            const uint32_t d = c * 128u + in * 4u;
-            a[c].none(); b[c].none();
-            if (live) {
-                a[c].load(is_q ? P.q : P.k, at + d);
-                if (!is_q) b[c].load(P.v, at + d);
-                else if (P.gate) b[c].load(P.q, at + HD + d);
+        for (int i = 0; i < 8; i++) w[i] = 1.f;
+        if (wn) eight_floats(wn + in * 8u, w);
+        if constexpr (HALF) {
+#pragma unroll
+            for (uint32_t s = 0; s < 2u; s++) {
+                const uint32_t g = in * 2u + s, other = g < quarter ? g + quarter : g - quarter;
+                const bool turns = FULL || g < 2u * quarter;
+                from[s] = sub * LPR + ((other >> 1) & (LPR - 1u));
+                float v[4] = {1.f, 1.f, 1.f, 1.f};
+                if (wn && turns) *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(wn) + other);
+                const uint32_t pair = (g < quarter ? g : other) * 4u;   /* of the group's first dim */
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) {
+                    const uint32_t k = s * 4u + i, holder = ((pair + i) / C) & 31u;
+                    const float c = __shfl_sync(0xffffffffu, cs[i % C], holder), d = __shfl_sync(0xffffffffu, sn[i % C], holder);
+                    fa[k] = turns ? w[k] * c : w[k];
+                    fb[k] = v[i] * (g < quarter ? -d : d);
+                }
+                on |= turns ? 0xfu << (4u * s) : 0u;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) {
+                const uint32_t pair = in * 4u + i;
+                const float c = __shfl_sync(0xffffffffu, cs[i % C], pair / C), d = __shfl_sync(0xffffffffu, sn[i % C], pair / C);
+                const bool turns = FULL || pair < np;
+                fa[2 * i] = turns ? w[2 * i] * c : w[2 * i];
+                fa[2 * i + 1] = turns ? w[2 * i + 1] * c : w[2 * i + 1];
+                fb[2 * i] = w[2 * i + 1] * -d;
+                fb[2 * i + 1] = w[2 * i] * d;
+                on |= turns ? 3u << (2u * i) : 0u;
             }
         }
-        const float *wn = is_q ? P.wq : P.wk;
-        float4 x[CH];
+    }
+    const int32_t slot = is_q ? -1 : __ldcg(P.slot + tok);
+    const bool keeps = slot >= 0 && (uint32_t)slot < P.slots;
+    if (slot >= 0 && !keeps && lane == 0u) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    const uint32_t row = (uint32_t)(keeps ? slot : 0), page = row >> P.page_shift, in_page = row & ((1u << P.page_shift) - 1u), r16 = row & 15u;
+
+    for (uint32_t head0 = first; head0 - sub < behind; head0 += RPW * U) {
+        load(head0 + RPW * U, a_next, b_next);
 #pragma unroll
-        for (uint32_t c = 0; c < CH; c++) x[c] = a[c].get();
-        if (P.eps >= 0.f) {
-            float ss = 0.f;
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t head = head0 + u * RPW;
+            if (head - sub >= behind) break;
+            const bool live = head < behind;
+            float x[8];
+            a[u].get(x);
+            float r = 1.f;
+            if (P.eps >= 0.f) {
+                float ss = 0.f;
 #pragma unroll
-            for (uint32_t c = 0; c < CH; c++) ss += x[c].x * x[c].x + x[c].y * x[c].y + x[c].z * x[c].z + x[c].w * x[c].w;
+                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-            for (uint32_t o = LPR / 2u; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float r = 1.f / sqrtf(ss * (1.f / HD) + P.eps);
-#pragma unroll
-            for (uint32_t c = 0; c < CH; c++) {
-                const float4 w = wn ? __ldg(reinterpret_cast<const float4 *>(wn + c * 128u) + in) : make_float4(1.f, 1.f, 1.f, 1.f);
-                x[c].x *= r * w.x; x[c].y *= r * w.y; x[c].z *= r * w.z; x[c].w *= r * w.w;
+                for (uint32_t o = LPR / 2u; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                r = rsqrtf(fmaf(ss, 1.f / HD, P.eps));   /* 2 units in the last place at most */
             }
-        }
-        /* the rotation */
-        if (!P.rope.half) {
+            float y[8];
+            if constexpr (HALF) {
+                if (swap) {
 #pragma unroll
-            for (uint32_t c = 0; c < CH; c++) {
-                const uint32_t grp = c * 32u + in;
-                if (grp * 4u < P.rope.n_rot) {
-                    const float4 k = cs[t][grp];
-                    const float4 y = x[c];
-                    const bool both = grp * 4u + 2u < P.rope.n_rot;
-                    x[c].x = y.x * k.x - y.y * k.y; x[c].y = y.x * k.y + y.y * k.x;
-                    if (both) { x[c].z = y.z * k.z - y.w * k.w; x[c].w = y.z * k.w + y.w * k.z; }
+                    for (uint32_t i = 0; i < 8u; i++) y[i] = __shfl_sync(0xffffffffu, x[i ^ 4u], from[i >> 2]);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++) y[i] = __shfl_sync(0xffffffffu, x[i], from[i >> 2]);
                 }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++) y[i] = x[i ^ 1u];
             }
-        } else if (np) {
-            const uint32_t half = np / 4u;   /* groups of four dims */
-            float4 y[CH];
 #pragma unroll
-            for (uint32_t c = 0; c < CH; c++) {
-                const uint32_t grp = c * 32u + in, other = grp < half ? grp + half : grp - half, from = (lane & ~(LPR - 1u)) + (other & (LPR - 1u));
+            for (uint32_t i = 0; i < 8u; i++) {
+                const float z = x[i] * fa[i];
+                x[i] = r * (FULL || (on >> i) & 1u ? fmaf(y[i], fb[i], z) : z);   /* not turned: the other dim may be infinite */
+            }
+            if (is_q) {
+                if (!live) continue;
+                const uint64_t to = ((uint64_t)tok * P.n_head + head) * HD + in * 8u;
+                if (P.q_bf16) {
+                    __nv_bfloat162 h[4];
 #pragma unroll
-                for (uint32_t s = 0; s < CH; s++) {
-                    const float4 z = make_float4(__shfl_sync(0xffffffffu, x[s].x, from), __shfl_sync(0xffffffffu, x[s].y, from), __shfl_sync(0xffffffffu, x[s].z, from), __shfl_sync(0xffffffffu, x[s].w, from));
-                    if (s == 0u || other / LPR == s) y[c] = z;
+                    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(P.q_out) + to) = *reinterpret_cast<const uint4 *>(h);
+                } else {
+                    store_floats(reinterpret_cast<float *>(P.q_out) + to, x);
                 }
-            }
-#pragma unroll
-            for (uint32_t c = 0; c < CH; c++) {
-                const uint32_t grp = c * 32u + in;
-                if (grp < 2u * half) {
-                    const uint32_t i = (grp < half ? grp : grp - half) * 2u;
-                    const float4 k0 = cs[t][i], k1 = cs[t][i + 1u];
-                    const float sign = grp < half ? -1.f : 1.f;
-                    x[c].x = x[c].x * k0.x + sign * (y[c].x * k0.y); x[c].y = x[c].y * k0.z + sign * (y[c].y * k0.w);
-                    x[c].z = x[c].z * k1.x + sign * (y[c].z * k1.y); x[c].w = x[c].w * k1.z + sign * (y[c].w * k1.w);
+                if (two) {
+                    b[u].get(x);
+                    store_floats(P.gate + to, x);
                 }
-            }
-        }
-        if (is_q) {
-            if (live) {
-                const uint64_t to = ((uint64_t)tok * P.n_head + head) * HD + in * 4u;
+            } else {
+                uint8_t *tile = P.mem + ((((uint64_t)page * P.n_kvh + head) << (P.page_shift - 4u)) + (in_page >> 4)) * PgTile<KIND, HD>::BYTES;
 #pragma unroll
-                for (uint32_t c = 0; c < CH; c++) {
-                    if (P.q_bf16) *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(P.q_out) + to + c * 128u) = to_bf16(x[c]);
-                    else *reinterpret_cast<float4 *>(reinterpret_cast<float *>(P.q_out) + to + c * 128u) = x[c];
-                    if (P.gate) *reinterpret_cast<float4 *>(P.gate + to + c * 128u) = b[c].get();
-                }
-            }
-        }
-        if (RPW > 1u || !is_q) {
-            const int32_t slot = live && !is_q ? __ldcg(P.slot + tok) : -1;
-            const bool store = slot >= 0 && (uint32_t)slot < P.slots;
-            if (slot >= 0 && !store && in == 0u) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-            const uint32_t page = (uint32_t)(store ? slot : 0) >> P.page_shift, row = (uint32_t)(store ? slot : 0) & ((1u << P.page_shift) - 1u), r16 = row & 15u;
-            uint8_t *tile = P.mem + ((((uint64_t)page * P.n_kvh + head) << (P.page_shift - 4u)) + (row >> 4)) * PgTile<KIND, HD>::BYTES;
+                for (uint32_t v = 0; v < 2u; v++) {
+                    if (v) b[u].get(x);
+                    if constexpr (KIND == Q4K_Q8) {   /* four lanes to a block of 32 */
+                        float m = 0.f, d, id;
 #pragma unroll
-            for (uint32_t w = 0; w < 2u; w++)
-#pragma unroll
-                for (uint32_t c = 0; c < CH; c++) {
-                    const float4 y = w ? b[c].get() : x[c];
-                    const uint32_t d = c * 128u + in * 4u;
-                    if constexpr (KIND == Q4K_Q8) {
-                        float s, id;
-                        q4d_block_scale(y, s, id);
-                        if (store) {
+                        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                        q4d_scale(m, d, id);
+                        if (keeps && live) {
                             uint8_t *rec = tile + r16 * PgTile<KIND, HD>::ROW;
-                            *reinterpret_cast<uint32_t *>(rec + w * HD + d) = q4d_quant4(y, id);
-                            if ((in & 7u) == 0u) reinterpret_cast<__half *>(rec + 2u * HD)[w * (HD / 32u) + (d >> 5)] = __float2half_rn(s);
+                            *reinterpret_cast<uint2 *>(rec + v * HD + in * 8u) = make_uint2(q4d_quant4(make_float4(x[0], x[1], x[2], x[3]), id), q4d_quant4(make_float4(x[4], x[5], x[6], x[7]), id));
+                            if ((in & 3u) == 0u) reinterpret_cast<__half *>(rec + 2u * HD)[v * (HD / 32u) + (in >> 2)] = __float2half_rn(d);
                         }
-                    } else if (store) {
-                        const __half2 h0 = __floats2half2_rn(y.x, y.y), h1 = __floats2half2_rn(y.z, y.w);
-                        uint8_t *dst = tile + w * (PgTile<KIND, HD>::BYTES / 2u) + (d >> 6) * 2048u + r16 * 128u + ((((d >> 3) & 7u) ^ (r16 & 7u)) << 4) + (d & 4u) * 2u;
-                        *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&h0), *reinterpret_cast<const uint32_t *>(&h1));
+                    } else if (keeps && live) {
+                        __half2 h[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                        uint8_t *dst = tile + v * (PgTile<KIND, HD>::BYTES / 2u) + (in >> 3) * 2048u + r16 * 128u + (((in & 7u) ^ (r16 & 7u)) << 4);
+                        *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(h);
                     }
                 }
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            a[u] = a_next[u];
+            b[u] = b_next[u];
         }
     }
 }
@@ -195,14 +248,20 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 
 template <int KIND, int HD, bool BF16>
 bool prep_launch(PrepParams &p) {
-    const uint32_t sms = (uint32_t)g_q4.sm_count;
-    if (p.n_tok >= 4u * sms) {
-        p.per = p.jobs;
-        return q4i_launch_pdl("pages_prep launch", q4_pg_prep_k<KIND, HD, BF16, 4>, dim3((p.n_tok + 3u) / 4u), PREP_THREADS, 0, p);
-    }
-    const uint32_t one = PREP_WARPS * (HD == 64 ? 2u : 1u);   /* few tokens: a job per group of lanes */
-    p.per = p.n_tok < sms ? one : p.jobs;
-    return q4i_launch_pdl("pages_prep launch", q4_pg_prep_k<KIND, HD, BF16, 1>, dim3(p.n_tok, (p.jobs + p.per - 1u) / p.per), PREP_THREADS, 0, p);
+    constexpr uint32_t RPW = 256u / HD;
+    /* warps for every SM, several rounds of them where there is that much */
+    const uint32_t most = 108u * (uint32_t)g_q4.sm_count, want = (most + p.n_tok - 1u) / p.n_tok, q_turns = (p.n_head + RPW - 1u) / RPW, kv_turns = (p.n_kvh + RPW - 1u) / RPW;
+    const uint32_t per = (q_turns + kv_turns + want - 1u) / want;
+    p.q_per = per < q_turns ? per : q_turns;
+    p.kv_per = per < kv_turns ? per : kv_turns;
+    p.q_units = (q_turns + p.q_per - 1u) / p.q_per;
+    p.units = p.q_units + (kv_turns + p.kv_per - 1u) / p.kv_per;
+    const uint64_t blocks = (uint64_t)p.n_tok * p.units;
+    if (blocks > 0x7fffffffu) return q4i_fail(Q4E_ARG, "pages_prep: too many tokens for one call");
+    const bool full = p.rope.n_rot == HD;
+    auto start = [&](auto kernel) { return q4i_launch_pdl("pages_prep launch", kernel, dim3((unsigned)blocks), PREP_THREADS, 0, p); };
+    if (p.rope.half) return full ? start(q4_pg_prep_k<KIND, HD, BF16, true, true>) : start(q4_pg_prep_k<KIND, HD, BF16, true, false>);
+    return full ? start(q4_pg_prep_k<KIND, HD, BF16, false, true>) : start(q4_pg_prep_k<KIND, HD, BF16, false, false>);
 }
 
 }  // namespace
@@ -260,7 +319,6 @@ extern "C" bool q4_gpu_pages_prep(const q4_gpu_pages *pg, uint32_t layer, const 
     p.page_shift = (uint32_t)__builtin_ctz(pg->page_rows);
     p.slots = pg->n_pages << p.page_shift;
     p.q_bf16 = q_out_bf16 != 0;
-    p.jobs = n_head + pg->n_kvh;
     p.q = q; p.k = k; p.v = v; p.q_stride = q_stride; p.kv_stride = kv_stride;
     p.wq = wq; p.wk = wk; p.eps = eps;
     p.pos = pos; p.slot = slot; p.q_out = q_out; p.gate = gate;
