@@ -4,15 +4,15 @@
  *     p_i = exp((x_i - M) / T) / S,  S = sum exp((x_i - M) / T),  M the largest logit;  q likewise from the draft's logits
  *     draft d is kept while u q_d < p_d;  next = the first i with sum_{j <= i} w_j > u sum w,  w = max(p - q, 0), or p
  *
- * Two launches.  The first goes once through all rows, a block per row and CHUNK logits, and leaves (M, S) per chunk, relative to the chunk's own
- * largest logit: bound by memory, and by the 64-bit pipe, in which the exponentials and sums are taken (a token's border in the running sum may lie
- * anywhere; with 32 bits a draw over a flat distribution of 10^5 tokens falls on the wrong side once in some thousands).  The second decides per
- * request; the sums of the chunks tell in which one the next token lies, and only that one is looked through.  Where a draft was refused the
- * request's blocks go through that row of p and q once more for max(p - q, 0), and the last of them to finish looks.
+ * The first launch goes once through all rows, a warp per row and CHUNK logits, and leaves (M, S) per chunk.  The second decides, a block per request: the sums
+ * of the chunks tell in which one the next token lies, and only that one is looked through.  Where a draft was refused and has logits, the blocks of the
+ * third go through that row of p and q once more for the sums of max(p - q, 0), and the last of the request's to finish looks.
  *
- * The exponential: x log2(e) / T in steps of 1/32 is an integer K and a rest |r| <= 1/2; 2^((K + r) / 32) = 2^(K >> 5) 2^((K & 31) / 32) e^(r ln 2 / 32),
- * the second factor from a table of which each lane holds one entry, the third by its Taylor series up to r^5 (what is left out is below 2.3e-15):
- * 10 operations of the 64-bit pipe, the sum's among them, where a library exponential takes some 20 (48 x 5 drafts over 131 072 tokens 206 us with those).
+ * Exponentials and sums are in 64 bits: a token's border in the running sum may lie anywhere, and with 32 bits a draw over a flat distribution of 10^5 tokens
+ * falls on the wrong side of one once in some thousands.  x log2(e) / T in steps of 1/32 is an integer K and a rest |r| <= 1/2;
+ * 2^((K + r) / 32) = 2^(K >> 5) 2^((K & 31) / 32) e^(r ln 2 / 32), the second factor from a table of which each lane holds one entry, the third by its Taylor
+ * series up to r^5 (what is left out is below 2.3e-15): 9 operations of the 64-bit pipe, the sum's among them, where the library's exponential
+ * takes some 20.  The first launch is bound by its instructions, 15 per logit, beside memory.
  */
 #include <math_constants.h>
 
@@ -21,15 +21,19 @@
 
 namespace {
 
-constexpr uint32_t CHUNK = 4096, VF_THREADS = 128, EACH = CHUNK / VF_THREADS, PICK_THREADS = 512, PICK_EACH = CHUNK / PICK_THREADS;
+constexpr uint32_t EACH = 32, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
 constexpr float LARGEST = 3.402823466e38f;
 
-struct __align__(16) VfStat { double s; float m; int32_t at; };   /* of a chunk: sum relative to the largest logit, that logit (NaN or +inf: the row is no distribution), its first place (greedy) */
+/* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to m, m's first place (greedy) */
+struct __align__(16) VfStat { double s; float m; int32_t at; };
+struct Row { float m; double s; };   /* s relative to m */
+/* of a request: which row decides next (and how), for the launch that looks where p is over q; none: it has been decided */
+struct VfChoice { Row p, q; uint32_t stop, open; };
 
 struct VerifyParams {
     const uint8_t *logits, *draft;
     uint64_t ld, draft_ld;       /* bytes */
-    uint32_t vocab, chunks, n_req, n_tok;
+    uint32_t vocab, chunks, n_req, n_tok, rows_all;   /* rows_all: the target's, and the draft's if there are any */
     const int32_t *token, *start;
     const float *temp, *u_accept, *u_next;
     int32_t *accepted, *next;
@@ -37,6 +41,7 @@ struct VerifyParams {
     const int32_t *rows;
     int32_t *keep;
     VfStat *stat;                /* [target's rows, draft's rows][chunk] */
+    VfChoice *choice;            /* [request] */
     double *rest;                /* [request][chunk]: sums of max(p - q, 0) */
     uint32_t *err;
 };
@@ -53,6 +58,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
     return c;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float warp_max_nan(float m) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -63,43 +73,57 @@ __device__ __forceinline__ double warp_sum(double x) {
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
+/* sums up to and with each lane's */
+__device__ __forceinline__ double warp_scan(double x) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((threadIdx.x & 31u) >= (uint32_t)o) x += y;
+    }
+    return x;
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= LARGEST; }
 
-/* exp((x - M) / T) for the logits of a row whose largest is M.  fast: in steps of c per unit of x from the whole one e next to M, as above; it needs steps below
- * 2^50 and a logit 1000 powers of two below M that is still a number.  Else by the library's function. */
+/* exp((x - M) / T) for logits x up to M.  fast: relative to the whole step e next to M, as above; it needs steps below 2^40 and a logit 1000 powers of two
+ * below M that is still a number.  Else relative to M, by the library's function. */
 struct VfExp {
-    double c, e, inv, m;
+    double c, e, m, T;
     float low;                   /* what is below is nothing (2^-1000) */
     bool fast;
-    __device__ __forceinline__ void set(float largest, double inv_t, float T) {
+    __device__ __forceinline__ void set(float largest, float t) {
         m = largest;
-        inv = inv_t;
-        c = inv_t * STEPS;
-        const double at = m * c, far = m - 1000.0 * LN2 * (double)T;
+        T = t;
+        c = STEPS / T;
+        const double at = m * c, far = m - 1000.0 * LN2 * T;
         fast = fabs(at) < 1099511627776.0 && far > -1e38;
         e = rint(at);
         low = (float)far;
     }
-    /* the steps from e back to M, as a factor */
-    __device__ __forceinline__ double to_m() const { return fast ? exp2(fma(m, c, -e) * (-1.0 / 32.0)) : 1.0; }
-    /* relative to e where fast; pow: the lane's entry of the table.  By whole warps */
-    __device__ __forceinline__ double steps(float x, double pow) const {
+    __device__ __forceinline__ double slow(float x) const { return exp(((double)x - m) / T); }
+    /* what is relative to this as a factor relative to a logit of `to` */
+    __device__ __forceinline__ double over(double to) const { return fast ? exp2(fma(-to, c, e) * (1.0 / 32.0)) : exp((m - to) / T); }
+    /* table: the lane's entry, less its number at the exponent's lowest bits, which the whole step brings along.  By whole warps, x not below low.  The value is f * (what is returned) */
+    __device__ __forceinline__ double steps(float x, int2 table, double &f) const {
         constexpr double MAGIC = 6755399441055744.0;   /* 1.5 * 2^52: the sum's low word is the rounded integer */
         constexpr double L = LN2 / 32.0;
-        const double xd = (double)x, t = fma(xd, c, MAGIC - e);
-        const double r = fma(xd, c, -(t - (MAGIC - e)));
+        const double xd = (double)x, base = MAGIC - e, t = fma(xd, c, base), r = fma(xd, c, base - t);
         const int32_t k = __double2loint(t);
-        const int32_t hi = __shfl_sync(0xffffffffu, __double2hiint(pow), k), lo = __shfl_sync(0xffffffffu, __double2loint(pow), k);
-        const double p = fma(r, fma(r, fma(r, fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0), L * L * L / 6.0), L * L / 2.0), L);
-        const double f = __hiloint2double(hi + ((k & ~31) << 15), lo);
-        return fma(f * r, p, f);
+        const int32_t hi = __shfl_sync(0xffffffffu, table.y, k), lo = __shfl_sync(0xffffffffu, table.x, k);
+        f = __hiloint2double(hi + (k << 15), lo);
+        return fma(r, fma(r, fma(r, fma(r, fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0), L * L * L / 6.0), L * L / 2.0), L), 1.0);
     }
-    __device__ __forceinline__ double of(float x, double pow) const {
-        if (!fast) return exp(((double)x - m) * inv);
-        const double y = steps(fmaxf(x, low), pow);
-        return x < low ? 0.0 : y;
+    __device__ __forceinline__ double of(float x, int2 table) const {
+        if (!fast) return slow(x);
+        double f;
+        const double y = steps(fmaxf(x, low), table, f);
+        return x < low ? 0.0 : f * y;
     }
 };
+__device__ __forceinline__ int2 lane_table() {
+    const uint32_t lane = threadIdx.x & 31u;
+    const double x = __ldg(g_vf_pow + lane);
+    return make_int2(__double2loint(x), __double2hiint(x) - (int32_t)(lane << 15));
+}
 
 template <bool BF16>
 __device__ __forceinline__ float logit(const uint8_t *row, uint64_t at) {
@@ -127,22 +151,19 @@ __device__ __forceinline__ float temperature(const VerifyParams &P, uint32_t r) 
 __device__ __forceinline__ bool temperature_ok(float t) { return t >= 0.f && t <= LARGEST; }
 
 template <bool BF16>
-__global__ void __launch_bounds__(VF_THREADS) q4_vf_stat_k(const VerifyParams P) {
-    constexpr uint32_t PER = BF16 ? 8u : 4u, WARPS = VF_THREADS / 32u;
-    __shared__ float s_max[WARPS];
-    __shared__ double s_sum[WARPS], s_inv;
-    __shared__ uint32_t s_at;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    q4d_pdl_wait();
-    const uint32_t row = blockIdx.x / P.chunks, chunk = blockIdx.x - row * P.chunks;
+__global__ void __launch_bounds__(VF_THREADS, 7) q4_vf_stat_k(const VerifyParams P) {
+    constexpr uint32_t PER = BF16 ? 8u : 4u;
+    const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.chunks, chunk = unit - row * P.chunks;
     const bool drafts = row >= P.n_tok;
     const uint32_t t = drafts ? row - P.n_tok : row;
+    q4d_pdl_wait();
+    if (row >= P.rows_all) return;   /* warps behind the last row */
     const uint8_t *base = drafts ? P.draft + t * P.draft_ld : P.logits + t * P.ld;
     const uint32_t off = row_begins<BF16>(base);
     float x[EACH];
 #pragma unroll
     for (uint32_t k = 0; k < EACH / PER; k++) {
-        const int64_t i = (int64_t)chunk * CHUNK + (k * VF_THREADS + tid) * PER - off;
+        const int64_t i = (int64_t)chunk * CHUNK + (k * 32u + lane) * PER - off;
         if (i >= 0 && i + PER <= P.vocab) {
             const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(base + i * (BF16 ? 2 : 4)));
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -159,83 +180,80 @@ __global__ void __launch_bounds__(VF_THREADS) q4_vf_stat_k(const VerifyParams P)
     const float T = temperature(P, r);
     if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
     if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
-    const double pow = __ldg(g_vf_pow + lane);
-    float m = x[0];
+    const int2 table = lane_table();
+    float m = max_nan(x[0], x[1]);
 #pragma unroll
-    for (uint32_t k = 1; k < EACH; k++) m = max_nan(m, x[k]);
+    for (uint32_t k = 2; k < EACH; k += 2u) m = max_nan(m, x[k], x[k + 1u]);
     m = warp_max_nan(m);
-    if (lane == 0) s_max[warp] = m;
-    if (tid == 0) {
-        s_at = 0xffffffffu;
-        s_inv = 1.0 / (double)T;
-    }
-    __syncthreads();
-    m = s_max[0];
-#pragma unroll
-    for (uint32_t w = 1; w < WARPS; w++) m = max_nan(m, s_max[w]);
     VfStat *out = P.stat + (uint64_t)row * P.chunks + chunk;
     if (T == 0.f) {
         uint32_t at = 0xffffffffu;
 #pragma unroll
         for (uint32_t k = 0; k < EACH; k++)
-            if (x[k] == m) at = min(at, (k / PER * VF_THREADS + tid) * PER + k % PER);
-        atomicMin(&s_at, at);
-        __syncthreads();
-        if (tid == 0) *out = {1.0, m, (int32_t)(chunk * CHUNK + s_at - off)};
+            if (x[k] == m) at = min(at, (k / PER * 32u + lane) * PER + k % PER);
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) *out = {1.0, m, (int32_t)(chunk * CHUNK + at - off)};
         return;
     }
     double s = 0.0;
-    VfExp E;
-    E.set(m, s_inv, T);
-    if (!finite(m)) {   /* nothing in it, or no distribution */
-    } else if (E.fast) {
-        double s1 = 0.0;
+    if (finite(m)) {             /* else nothing is in it, or the row is no distribution */
+        VfExp E;
+        E.set(m, T);
+        if (E.fast) {
+            double s1 = 0.0, f;
 #pragma unroll
-        for (uint32_t k = 0; k < EACH; k += 2u) {
-            s += E.steps(fmaxf(x[k], E.low), pow);
-            s1 += E.steps(fmaxf(x[k + 1u], E.low), pow);
-        }
-        s += s1;
-    } else {
+            for (uint32_t k = 0; k < EACH; k += 2u) {
+                double y = E.steps(fmaxf(x[k], E.low), table, f);
+                s = fma(f, y, s);
+                y = E.steps(fmaxf(x[k + 1u], E.low), table, f);
+                s1 = fma(f, y, s1);
+            }
+            s += s1;
+        } else {
 #pragma unroll 1
-        for (uint32_t k = 0; k < EACH; k++) {
-            float y = x[0];
+            for (uint32_t k = 0; k < EACH; k++) {
+                float y = x[0];
 #pragma unroll
-            for (uint32_t j = 1; j < EACH; j++) y = j == k ? x[j] : y;
-            s += exp(((double)y - E.m) * E.inv);
+                for (uint32_t j = 1; j < EACH; j++) y = j == k ? x[j] : y;
+                s += E.slow(y);
+            }
         }
     }
     s = warp_sum(s);
-    if (lane == 0) s_sum[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
-        for (uint32_t w = 1; w < WARPS; w++) s += s_sum[w];
-        *out = {finite(m) ? s * E.to_m() : 0.0, m, 0};
-    }
+    if (lane == 0) *out = {s, m, 0};
 }
 
+__device__ __forceinline__ VfStat stat_at(const VfStat *p) {
+    const int4 x = __ldcg(reinterpret_cast<const int4 *>(p));
+    return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
+}
+/* the sum of a chunk relative to a logit of `to` */
+__device__ __forceinline__ double chunk_over(const VfStat &x, double to, float T) {
+    if (!(x.s > 0.0)) return 0.0;
+    VfExp E;
+    E.set(x.m, T);
+    return x.s * E.over(to);
+}
 /* a row's M and S from its chunks', by a whole warp; false: no distribution */
-struct Row { float m; double s; };
-__device__ __forceinline__ bool row_of(const VfStat *stat, uint32_t chunks, double inv, Row &R) {
+__device__ __forceinline__ bool row_of(const VfStat *stat, uint32_t chunks, float T, Row &R) {
+    constexpr uint32_t AT_ONCE = 4;   /* chunks of a lane */
     const uint32_t lane = threadIdx.x & 31u;
-    float m = -CUDART_INF_F, m0 = -CUDART_INF_F;
-    double s0 = 0.0;
-    for (uint32_t c = lane; c < chunks; c += 32u) {
-        const int4 x = __ldcg(reinterpret_cast<const int4 *>(stat + c));
-        if (c == lane) {
-            s0 = __hiloint2double(x.y, x.x);
-            m0 = __int_as_float(x.z);
-        }
-        m = max_nan(m, __int_as_float(x.z));
+    VfStat x[AT_ONCE];
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (uint32_t k = 0; k < AT_ONCE; k++) {
+        x[k] = {0.0, -CUDART_INF_F, 0};
+        if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
     }
+#pragma unroll
+    for (uint32_t k = 0; k < AT_ONCE; k++) m = max_nan(m, x[k].m);
+    for (uint32_t c = lane + 32u * AT_ONCE; c < chunks; c += 32u) m = max_nan(m, __ldcg(&stat[c].m));
     R.m = m = warp_max_nan(m);
     R.s = 0.0;
     if (!finite(m)) return false;
-    if (s0 > 0.0) R.s = s0 * exp(((double)m0 - (double)m) * inv);
-    for (uint32_t c = lane + 32u; c < chunks; c += 32u) {
-        const double s = __ldcg(&stat[c].s);
-        if (s > 0.0) R.s += s * exp(((double)__ldcg(&stat[c].m) - (double)m) * inv);
-    }
+#pragma unroll
+    for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_over(x[k], m, T);
+    for (uint32_t c = lane + 32u * AT_ONCE; c < chunks; c += 32u) R.s += chunk_over(stat_at(stat + c), m, T);
     R.s = warp_sum(R.s);
     return true;
 }
@@ -243,33 +261,147 @@ __device__ __forceinline__ bool row_of(const VfStat *stat, uint32_t chunks, doub
 __device__ __forceinline__ bool best_of(const VfStat *stat, uint32_t chunks, int32_t &at) {
     const uint32_t lane = threadIdx.x & 31u;
     float m = -CUDART_INF_F;
-    for (uint32_t c = lane; c < chunks; c += 32u) m = max_nan(m, __ldcg(&stat[c].m));
-    m = warp_max_nan(m);
     at = 0x7fffffff;
-    for (uint32_t c = lane; c < chunks; c += 32u)
-        if (__ldcg(&stat[c].m) == m) at = min(at, __ldcg(&stat[c].at));
-    at = __reduce_min_sync(0xffffffffu, at);
-    return finite(m);
+    for (uint32_t c = lane; c < chunks; c += 32u) {
+        const VfStat x = stat_at(stat + c);
+        const float top = max_nan(m, x.m);
+        if (x.m == top && (m < top || x.at < at)) at = x.at;
+        m = top;
+    }
+    const float all = warp_max_nan(m);
+    at = __reduce_min_sync(0xffffffffu, m == all ? at : 0x7fffffff);
+    return finite(all);
+}
+
+/* The place in w_0 w_1 .. w_(n - 1) (of(i, lane's turn): lanes ask for items of their own) at which the running sum passes u times the whole, and what is left for it;
+ * by a whole warp.  A lane sums n / 32 items, then the 32 share out those of the lane in whose sum it lies, and so on.  Where rounding leaves
+ * none: the last item with anything in it.  whole: the sum (0: nothing there) */
+template <typename F>
+__device__ __forceinline__ uint32_t place_of(uint32_t n, double u, double &left, double &whole, F of) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t lo = 0;
+    bool top = true;
+    left = 0.0;
+    while (top || n > 1u) {
+        const uint32_t step = (n + 31u) / 32u, i0 = min(lane * step, n), i1 = min(i0 + step, n);
+        double own = 0.0;
+#pragma unroll 4
+        for (uint32_t i = i0; i < i1; i++) own += of(lo + i);
+        const double x = warp_scan(own);
+        if (top) {
+            whole = __shfl_sync(0xffffffffu, x, 31);
+            if (!(whole > 0.0)) return 0u;
+            left = u * whole;
+            top = false;
+        }
+        const uint32_t above = __ballot_sync(0xffffffffu, x > left && own > 0.0), any = __ballot_sync(0xffffffffu, own > 0.0);
+        const uint32_t l = above ? (uint32_t)__ffs((int)above) - 1u : any ? 31u - (uint32_t)__clz((int)any) : 0u;
+        const double before = __shfl_up_sync(0xffffffffu, x, 1);
+        left = above ? left - __shfl_sync(0xffffffffu, lane ? before : 0.0, (int)l) : CUDART_INF;
+        n = min(step, n - min(l * step, n));
+        lo += l * step;
+    }
+    return lo;
+}
+
+/* a row's tokens by weight: p without the refused one where drafts are certain, or what p has over q */
+template <bool BF16>
+struct Weights {
+    const uint8_t *row_p, *row_q;
+    VfExp p, q;
+    double scale_p, scale_q;
+    int64_t off;
+    uint32_t vocab;
+    int32_t certain;             /* the token left out; -1: none */
+    bool over_q;
+    int2 table;
+    __device__ __forceinline__ void set(const VerifyParams &P, uint32_t row, const Row &rp, const Row &rq, float T, bool with_q, int32_t left_out) {
+        row_p = P.logits + row * P.ld;
+        row_q = with_q ? P.draft + row * P.draft_ld : nullptr;
+        off = row_begins<BF16>(row_p);
+        vocab = P.vocab;
+        certain = left_out;
+        over_q = with_q;
+        table = lane_table();
+        p.set(rp.m, T);
+        scale_p = p.over(rp.m) / rp.s;
+        q.set(with_q ? rq.m : 0.f, T);
+        scale_q = with_q ? q.over(rq.m) / rq.s : 0.0;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t c) const { return (uint32_t)max((int64_t)c * CHUNK - off, (int64_t)0); }
+    __device__ __forceinline__ uint32_t end(uint32_t c) const { return (uint32_t)min((int64_t)(c + 1u) * CHUNK - off, (int64_t)vocab); }
+    __device__ __forceinline__ void load(uint64_t i, uint32_t end, float &xp, float &xq) const {
+        xp = i < end ? logit<BF16>(row_p, i) : -CUDART_INF_F;
+        xq = over_q && i < end ? logit<BF16>(row_q, i) : -CUDART_INF_F;
+    }
+    __device__ __forceinline__ double of(float xp, float xq, uint32_t i) const {   /* by whole warps; minus infinity: nothing */
+        const double x = __dmul_rn(p.of(xp, table), scale_p);
+        if (over_q) return fmax(__dsub_rn(x, __dmul_rn(q.of(xq, table), scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
+        return (int32_t)i == certain ? 0.0 : x;
+    }
+};
+
+/* by a block: the token of chunk c at which the running sum passes `left`, and its log p */
+template <bool BF16>
+__device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> &W, uint32_t r, uint32_t stop, const Row &p, uint32_t c, double left) {
+    __shared__ double s_scan[PICK_WARPS];
+    __shared__ int32_t s_some[PICK_WARPS];
+    __shared__ uint32_t s_found;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, i0 = W.begin(c) + tid * PICK_EACH, i1 = W.end(c);
+    if (tid == 0) s_found = 0xffffffffu;
+    float xp[PICK_EACH], xq[PICK_EACH];
+#pragma unroll
+    for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k, i1, xp[k], xq[k]);
+    double w[PICK_EACH], sum = 0.0;
+    int32_t some = -1;
+#pragma unroll
+    for (uint32_t k = 0; k < PICK_EACH; k++) {
+        w[k] = W.of(xp[k], xq[k], i0 + k);
+        sum += w[k];
+        if (w[k] > 0.0) some = (int32_t)(i0 + k);
+    }
+    double before = warp_scan(sum);
+    some = (int32_t)__reduce_max_sync(0xffffffffu, (uint32_t)(some + 1)) - 1;
+    if (lane == 31u) s_scan[warp] = before;
+    if (lane == 0) s_some[warp] = some;
+    __syncthreads();
+    before -= sum;
+    for (uint32_t k = 0; k < warp; k++) before += s_scan[k];
+    if (before + sum > left && sum > 0.0) {   /* the first token above it; threads behind find later ones */
+        uint32_t found = 0xffffffffu;
+#pragma unroll
+        for (uint32_t k = 0; k < PICK_EACH; k++) {
+            before += w[k];
+            if (before > left && w[k] > 0.0 && found == 0xffffffffu) found = i0 + k;
+        }
+        if (found != 0xffffffffu) atomicMin(&s_found, found);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int32_t found = (int32_t)s_found;
+        if (s_found == 0xffffffffu)   /* rounding, or u not below 1: the last that can be */
+            for (uint32_t k = 0; k < PICK_WARPS; k++) found = max(found, s_some[k]);
+        P.next[r] = found;
+        if (P.logp) P.logp[stop] = found >= 0 ? (float)(((double)logit<BF16>(W.row_p, (uint32_t)found) - (double)p.m) / W.p.T - log(p.s)) : 0.f;
+    }
 }
 
 enum { VF_REFUSED = 0, VF_KEPT = 1, VF_NONE = 2 /* no distribution */, VF_LAST = 3 };
 
 template <bool BF16>
 __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams P) {
-    constexpr uint32_t WARPS = PICK_THREADS / 32u;
-    __shared__ Row s_p[WARPS], s_q[WARPS];
-    __shared__ uint32_t s_said[WARPS];
-    __shared__ int32_t s_best[WARPS], s_some[WARPS];
-    __shared__ double s_scan[WARPS], s_left, s_special;
-    __shared__ uint32_t s_chunk, s_found, s_last, s_over;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, chunk = blockIdx.x, r = blockIdx.y;
-    const bool first = chunk == 0u;
+    __shared__ Row s_p[PICK_WARPS], s_q[PICK_WARPS];
+    __shared__ uint32_t s_said[PICK_WARPS], s_chunk;
+    __shared__ int32_t s_best[PICK_WARPS], s_draft[PICK_WARPS];
+    __shared__ double s_left, s_part[PICK_WARPS];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.x;
     q4d_pdl_wait();
     const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
     const float T = temperature(P, r);
     const bool bounds = a >= 0 && b >= a && (uint32_t)b <= P.n_tok;
+    if (tid == 0 && P.draft) P.choice[r].open = 0u;
     if (!bounds || a == b) {
-        if (first && tid == 0) {
+        if (tid == 0) {
             P.accepted[r] = 0;
             P.next[r] = -1;
             if (P.keep) P.keep[r] = __ldcg(P.rows + r);
@@ -278,35 +410,35 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         return;
     }
     const bool greedy = T == 0.f;
-    const double inv = greedy ? 1.0 : 1.0 / (double)T, pow = __ldg(g_vf_pow + lane);
     const VfStat *stat_p = P.stat, *stat_q = P.stat + (uint64_t)P.n_tok * P.chunks;
     const uint32_t last = (uint32_t)b - 1u;
 
     /* ---- the request's rows, a warp each: whether the draft behind a row is kept.  The first that is not, or the last row, decides */
     uint32_t stop = (uint32_t)a, said = VF_NONE;
     Row p = {}, q = {};
-    int32_t best = -1;
+    int32_t best = -1, left_out = -1;   /* left_out: the draft behind the row that decides */
     bool out_of_vocab = false;
-    for (uint32_t t0 = (uint32_t)a; temperature_ok(T); t0 += WARPS) {
+    for (uint32_t t0 = (uint32_t)a; temperature_ok(T); t0 += PICK_WARPS) {
         const uint32_t t = t0 + warp;
         uint32_t mine = VF_KEPT;
+        int32_t d = -1;
         float lp = 0.f;
         if (t <= last) {
-            const int32_t d = t < last ? __ldcg(P.token + t + 1u) : -1;
+            if (t < last) d = __ldcg(P.token + t + 1u);
             const bool in = (uint32_t)d < P.vocab, with_q = t < last && P.draft;
             /* asked for ahead of the sums */
             const float xp = !greedy && in ? logit<BF16>(P.logits + t * P.ld, (uint32_t)d) : 0.f, xq = !greedy && in && with_q ? logit<BF16>(P.draft + t * P.draft_ld, (uint32_t)d) : 0.f;
             const float u = !greedy && t < last ? __ldcg(P.u_accept + t) : 0.f;
             if (greedy) {
                 mine = !best_of(stat_p + (uint64_t)t * P.chunks, P.chunks, best) ? VF_NONE : t == last ? VF_LAST : best == d ? VF_KEPT : VF_REFUSED;
-            } else if (!row_of(stat_p + (uint64_t)t * P.chunks, P.chunks, inv, p) || (with_q && !row_of(stat_q + (uint64_t)t * P.chunks, P.chunks, inv, q))) {
+            } else if (!row_of(stat_p + (uint64_t)t * P.chunks, P.chunks, T, p) || (with_q && !row_of(stat_q + (uint64_t)t * P.chunks, P.chunks, T, q))) {
                 mine = VF_NONE;
             } else if (t == last) {
                 mine = VF_LAST;
             } else if (in) {
-                const double pd = exp(((double)xp - (double)p.m) * inv) / p.s, qd = P.draft ? exp(((double)xq - (double)q.m) * inv) / q.s : 1.0;
+                const double pd = exp(((double)xp - (double)p.m) / (double)T) / p.s, qd = P.draft ? exp(((double)xq - (double)q.m) / (double)T) / q.s : 1.0;
                 mine = (double)u * qd < pd ? VF_KEPT : VF_REFUSED;
-                if (P.logp && first) lp = (float)(((double)xp - (double)p.m) * inv - log(p.s));
+                if (P.logp) lp = (float)(((double)xp - (double)p.m) / (double)T - log(p.s));
             } else {
                 mine = VF_REFUSED;
             }
@@ -318,11 +450,12 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             s_p[warp] = p;
             s_q[warp] = q;
             s_best[warp] = best;
+            s_draft[warp] = d;
         }
         __syncthreads();
-        const uint32_t others = __ballot_sync(0xffffffffu, lane < WARPS && s_said[lane & (WARPS - 1u)] != VF_KEPT);
-        const uint32_t n = others ? (uint32_t)__ffs((int)others) - 1u : WARPS;
-        if (first && lane == 0 && t < last) {
+        const uint32_t others = __ballot_sync(0xffffffffu, lane < PICK_WARPS && s_said[lane % PICK_WARPS] != VF_KEPT);
+        const uint32_t n = others ? (uint32_t)__ffs((int)others) - 1u : PICK_WARPS;
+        if (lane == 0 && t < last) {
             if (P.logp && warp < n) P.logp[t] = greedy ? 0.f : lp;
             if (out_of_vocab && warp <= n) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         }
@@ -332,193 +465,123 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             p = s_p[n];
             q = s_q[n];
             best = s_best[n];
+            left_out = s_draft[n];
             break;
         }
     }
-    if (first) {
-        if (P.logp)
-            for (uint32_t t = stop + 1u + tid; t <= last; t += PICK_THREADS) P.logp[t] = 0.f;
-        if (tid == 0) {
-            P.accepted[r] = (int32_t)(stop - (uint32_t)a);
-            if (P.keep) P.keep[r] = __ldcg(P.rows + r) + (int32_t)(stop - (uint32_t)a) + 1;
-            if (said == VF_NONE || greedy) {
-                P.next[r] = said == VF_NONE ? -1 : best;
-                if (P.logp) P.logp[stop] = 0.f;
-                if (said == VF_NONE) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-            }
+    if (P.logp)
+        for (uint32_t t = stop + 1u + tid; t <= last; t += PICK_THREADS) P.logp[t] = 0.f;
+    const bool refused = said == VF_REFUSED && !greedy, open = refused && P.draft;
+    if (tid == 0) {
+        P.accepted[r] = (int32_t)(stop - (uint32_t)a);
+        if (P.keep) P.keep[r] = __ldcg(P.rows + r) + (int32_t)(stop - (uint32_t)a) + 1;
+        if (said == VF_NONE || greedy) {
+            P.next[r] = said == VF_NONE ? -1 : best;
+            if (P.logp) P.logp[stop] = 0.f;
+            if (said == VF_NONE) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         }
+        if (open) P.choice[r] = {p, q, stop, 1u};
     }
-    if (said == VF_NONE || greedy) return;
-    const bool refused = said == VF_REFUSED, with_q = refused && P.draft;
-    if (!first && !with_q) return;
+    if (said == VF_NONE || greedy || open) return;
 
-    /* ---- weights of the row's tokens: p without the refused one where drafts are certain, or what p has over q */
-    const uint8_t *row_p = P.logits + stop * P.ld, *row_q = with_q ? P.draft + stop * P.draft_ld : nullptr;
-    const int64_t off = row_begins<BF16>(row_p);
-    const int32_t d = refused ? __ldcg(P.token + stop + 1u) : -1, certain = refused && !with_q ? d : -1;
-    VfExp Ep, Eq;
-    Ep.set(p.m, inv, T);
-    Eq.set(with_q ? q.m : 0.f, inv, T);
-    const double scale_p = Ep.to_m() / p.s, scale_q = with_q ? Eq.to_m() / q.s : 0.0;
-    auto begin_of = [&](uint32_t c) -> uint32_t { return (uint32_t)max((int64_t)c * CHUNK - off, (int64_t)0); };
-    auto end_of = [&](uint32_t c) -> uint32_t { return (uint32_t)min((int64_t)(c + 1u) * CHUNK - off, (int64_t)P.vocab); };
-    auto weight = [&](float xp, float xq, bool skip, bool over_q) -> double {   /* by whole warps; minus infinity: nothing */
-        const double x = __dmul_rn(Ep.of(xp, pow), scale_p);
-        if (!over_q) return skip ? 0.0 : x;
-        return fmax(__dsub_rn(x, __dmul_rn(Eq.of(xq, pow), scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
-    };
-    auto block_sum = [&](double x) -> double {
-        x = warp_sum(x);
-        __syncthreads();
-        if (lane == 0) s_scan[warp] = x;
-        __syncthreads();
-        x = s_scan[0];
+    /* ---- from p: the chunk, then the place in it.  The chunk with a certain draft that was refused is summed again without that */
+    Weights<BF16> W;
+    W.set(P, stop, p, q, T, false, left_out);
+    const uint32_t special = (uint32_t)W.certain < P.vocab ? (uint32_t)((W.certain + W.off) / CHUNK) : 0xffffffffu;
+    double without = 0.0;
+    if (special != 0xffffffffu) {
+        const uint32_t i0 = W.begin(special) + tid, i1 = W.end(special);
+        float xp[PICK_EACH], xq;
 #pragma unroll
-        for (uint32_t w = 1; w < WARPS; w++) x += s_scan[w];
-        return x;
-    };
-    auto chunk_sum = [&](uint32_t c, bool over_q) -> double {
-        const uint32_t i0 = begin_of(c), i1 = end_of(c);
-        float xp[PICK_EACH], xq[PICK_EACH];
+        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq);
 #pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) {
-            const uint64_t i = (uint64_t)i0 + k * PICK_THREADS + tid;
-            xp[k] = i < i1 ? logit<BF16>(row_p, i) : -CUDART_INF_F;
-            xq[k] = over_q && i < i1 ? logit<BF16>(row_q, i) : -CUDART_INF_F;
-        }
-        double x = 0.0;
-#pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) x += weight(xp[k], xq[k], (int32_t)(i0 + k * PICK_THREADS + tid) == certain, over_q);
-        return block_sum(x);
-    };
-    double *rest = P.rest + (uint64_t)r * P.chunks;
-    if (with_q) {
-        const double x = chunk_sum(chunk, true);
-        if (tid == 0) {
-            __stcg(rest + chunk, x);
-            __threadfence();
-            s_last = atomicAdd(&g_vf_arrived[r], 1u) == P.chunks - 1u;
-            if (s_last) g_vf_arrived[r] = 0u;
-            __threadfence();
-        }
+        for (uint32_t k = 0; k < PICK_EACH; k++) without += W.of(xp[k], 0.f, i0 + k * PICK_THREADS);
+        without = warp_sum(without);
+        if (lane == 0) s_part[warp] = without;
         __syncthreads();
-        if (!s_last) return;
+        without = 0.0;
+        for (uint32_t k = 0; k < PICK_WARPS; k++) without += s_part[k];
     }
-    /* ---- the chunk in which the running sum passes u times the whole, by a warp with a chunk per lane; then the place in it */
-    const uint32_t special_at = (uint32_t)certain < P.vocab ? (uint32_t)((certain + off) / CHUNK) : 0xffffffffu;
-    if (special_at != 0xffffffffu) {
-        const double x = chunk_sum(special_at, false);
-        if (tid == 0) s_special = x;
-        __syncthreads();
-    }
-    const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
     if (warp == 0) {
-        const double u = (double)__ldcg(P.u_next + r);
-        auto of_chunk = [&](uint32_t c, bool over_q) -> double {
-            if (c >= P.chunks) return 0.0;
-            if (over_q) return __ldcg(rest + c);
-            if (c == special_at) return s_special;
-            const int4 x = __ldcg(reinterpret_cast<const int4 *>(sp + c));
-            const double s = __hiloint2double(x.y, x.x);
-            return s > 0.0 ? s * exp(((double)__int_as_float(x.z) - (double)p.m) * inv) / p.s : 0.0;
-        };
-        /* sums up to and with every lane's chunk, from chunk c0 on; they are formed in one order for the whole and for the place */
-        auto scan = [&](uint32_t c0, double before, bool over_q, double &own) -> double {
-            double x = own = of_chunk(c0 + lane, over_q);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= (uint32_t)o) x += y;
-            }
-            return x + before;
-        };
-        bool over_q = with_q;
-        double all, own, x = 0.0;
-        for (;;) {
-            all = 0.0;
-            for (uint32_t c0 = 0; c0 < P.chunks; c0 += 32u) all = __shfl_sync(0xffffffffu, x = scan(c0, all, over_q, own), 31);
-            if (all > 0.0 || !over_q) break;
-            over_q = false;      /* p nowhere above q: as if none was refused */
-        }
-        const double want = u * all;
-        double before = 0.0, left = CUDART_INF;
-        uint32_t at = 0xffffffffu, some = 0;
-        for (uint32_t c0 = 0; c0 < P.chunks && at == 0xffffffffu; c0 += 32u) {
-            if (P.chunks > 32u) x = scan(c0, before, over_q, own);
-            const uint32_t above = __ballot_sync(0xffffffffu, x > want && own > 0.0), any = __ballot_sync(0xffffffffu, own > 0.0);
-            if (any) some = c0 + 31u - (uint32_t)__clz((int)any);
-            const double below = __shfl_up_sync(0xffffffffu, x, 1);
-            if (above) {
-                const uint32_t l = (uint32_t)__ffs((int)above) - 1u;
-                at = c0 + l;
-                left = want - __shfl_sync(0xffffffffu, lane ? below : before, (int)l);
-            }
-            before = __shfl_sync(0xffffffffu, x, 31);
-        }
+        const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
+        double left, whole;
+        const uint32_t c = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_over(stat_at(sp + i), p.m, T) / p.s; });
         if (lane == 0) {
-            s_chunk = at == 0xffffffffu ? some : at;   /* rounding, or u not below 1: the last with anything in it */
+            s_chunk = c;
             s_left = left;
-            s_over = over_q;
-            s_found = 0xffffffffu;
         }
     }
     __syncthreads();
-    const bool over_q = s_over;
-    const double want = s_left;
-    const uint32_t i0 = begin_of(s_chunk) + tid * PICK_EACH, i1 = end_of(s_chunk);
-    float xp[PICK_EACH], xq[PICK_EACH];
+    look<BF16>(P, W, r, stop, p, s_chunk, s_left);
+}
+
+/* what p has over q, a warp per chunk; the request's last block to finish looks for next */
+template <bool BF16>
+__global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams P) {
+    __shared__ uint32_t s_last, s_chunk, s_over;
+    __shared__ double s_left;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk = blockIdx.x * PICK_WARPS + warp;
+    q4d_pdl_wait();
+    const VfChoice *at = P.choice + r;
+    if (!__ldcg(&at->open)) return;
+    const Row p = {__ldcg(&at->p.m), __ldcg(&at->p.s)}, q = {__ldcg(&at->q.m), __ldcg(&at->q.s)};
+    const uint32_t stop = __ldcg(&at->stop);
+    const float T = temperature(P, r);
+    Weights<BF16> W;
+    W.set(P, stop, p, q, T, true, -1);
+    double *rest = P.rest + (uint64_t)r * P.chunks;
+    if (chunk < P.chunks) {
+        constexpr uint32_t AT_ONCE = 8;
+        const uint32_t i1 = W.end(chunk);
+        double x = 0.0;
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < EACH; k0 += AT_ONCE) {
+            const uint32_t i0 = W.begin(chunk) + k0 * 32u + lane;
+            float xp[AT_ONCE], xq[AT_ONCE];
 #pragma unroll
-    for (uint32_t k = 0; k < PICK_EACH; k++) {
-        const uint64_t i = (uint64_t)i0 + k;
-        xp[k] = i < i1 ? logit<BF16>(row_p, i) : -CUDART_INF_F;
-        xq[k] = over_q && i < i1 ? logit<BF16>(row_q, i) : -CUDART_INF_F;
-    }
-    double w[PICK_EACH], sum = 0.0;
-    int32_t some = -1;
+            for (uint32_t k = 0; k < AT_ONCE; k++) W.load((uint64_t)i0 + k * 32u, i1, xp[k], xq[k]);
 #pragma unroll
-    for (uint32_t k = 0; k < PICK_EACH; k++) {
-        w[k] = weight(xp[k], xq[k], (int32_t)(i0 + k) == certain, over_q);
-        sum += w[k];
-        if (w[k] > 0.0) some = (int32_t)(i0 + k);
-    }
-    double before = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= (uint32_t)o) before += x;
-    }
-    some = (int32_t)__reduce_max_sync(0xffffffffu, (uint32_t)(some + 1)) - 1;
-    __syncthreads();
-    if (lane == 31u) s_scan[warp] = before;
-    if (lane == 0) s_some[warp] = some;
-    __syncthreads();
-    before -= sum;
-    for (uint32_t k = 0; k < warp; k++) before += s_scan[k];
-    if (before + sum > want && sum > 0.0) {   /* the first token above it; threads behind find later ones */
-        uint32_t found = 0xffffffffu;
-#pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) {
-            before += w[k];
-            if (before > want && w[k] > 0.0 && found == 0xffffffffu) found = i0 + k;
+            for (uint32_t k = 0; k < AT_ONCE; k++) x += W.of(xp[k], xq[k], 0u);
         }
-        if (found != 0xffffffffu) atomicMin(&s_found, found);
+        x = warp_sum(x);
+        if (lane == 0) __stcg(rest + chunk, x);
     }
     __syncthreads();
     if (tid == 0) {
-        int32_t found = (int32_t)s_found;
-        if (s_found == 0xffffffffu)   /* rounding: the last that can be */
-            for (uint32_t k = 0; k < WARPS; k++) found = max(found, s_some[k]);
-        P.next[r] = found;
-        if (P.logp) P.logp[stop] = found >= 0 ? (float)(((double)logit<BF16>(row_p, (uint32_t)found) - (double)p.m) * inv - log(p.s)) : 0.f;
+        __threadfence();
+        s_last = atomicAdd(&g_vf_arrived[r], 1u) == gridDim.x - 1u;
+        if (s_last) g_vf_arrived[r] = 0u;
+        __threadfence();
     }
+    __syncthreads();
+    if (!s_last) return;
+    if (warp == 0) {
+        const double u = (double)__ldcg(P.u_next + r);
+        double left, whole;
+        uint32_t c = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return __ldcg(rest + i); });
+        const bool over_q = whole > 0.0;
+        if (!over_q) {           /* p nowhere above q: as if none was refused */
+            const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
+            c = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_over(stat_at(sp + i), p.m, T) / p.s; });
+        }
+        if (lane == 0) {
+            s_chunk = c;
+            s_left = left;
+            s_over = over_q;
+        }
+    }
+    __syncthreads();
+    W.over_q = s_over;
+    look<BF16>(P, W, r, stop, p, s_chunk, s_left);
 }
 
 template <bool BF16>
 bool verify_launch(const VerifyParams &p) {
-    const uint64_t blocks = (uint64_t)p.n_tok * (p.draft ? 2u : 1u) * p.chunks;
-    if (blocks > 0x7fffffffu) return q4i_fail(Q4E_ARG, "verify: too many rows for one call");
+    const uint64_t warps = (uint64_t)p.rows_all * p.chunks, blocks = (warps + VF_WARPS - 1u) / VF_WARPS;
+    if (warps > 0x7fffffffu) return q4i_fail(Q4E_ARG, "verify: too many rows for one call");
     return q4i_launch_pdl("verify launch", q4_vf_stat_k<BF16>, dim3((unsigned)blocks), VF_THREADS, 0, p) &&
-           q4i_launch_pdl("verify launch", q4_vf_pick_k<BF16>, dim3(p.draft ? p.chunks : 1u, p.n_req), PICK_THREADS, 0, p);
+           q4i_launch_pdl("verify launch", q4_vf_pick_k<BF16>, dim3(p.n_req), PICK_THREADS, 0, p) &&
+           (!p.draft || q4i_launch_pdl("verify launch", q4_vf_rest_k<BF16>, dim3((p.chunks + PICK_WARPS - 1u) / PICK_WARPS, p.n_req), PICK_THREADS, 0, p));
 }
 
 }  // namespace
@@ -537,12 +600,13 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t size = bf16 ? 2u : 4u;
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
-    p.n_req = n_req; p.n_tok = n_tok; p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
+    p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
     p.accepted = accepted; p.next = next; p.logp = logp; p.rows = rows; p.keep = keep;
     p.err = g_q4.err_d;
-    const uint64_t stats = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, rests = draft ? (uint64_t)n_req * p.chunks : 0u;
-    if (!q4i_scratch((size_t)(stats * 4u + rests * 2u), 0)) return false;
+    const uint64_t stats = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, rests = draft ? (uint64_t)n_req * p.chunks : 0u, choices = draft ? n_req : 0u;
+    if (!q4i_scratch((size_t)(stats * 4u + rests * 2u + choices * (sizeof(VfChoice) / 4u)), 0)) return false;
     p.stat = (VfStat *)g_q4.part;
     p.rest = (double *)(p.stat + stats);
+    p.choice = (VfChoice *)(p.rest + rests);
     return bf16 ? verify_launch<true>(p) : verify_launch<false>(p);
 }
