@@ -21,19 +21,22 @@
 
 namespace {
 
-constexpr uint32_t EACH = 32, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
+constexpr uint32_t EACH = 64, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
+constexpr uint32_t STAT_BLOCKS = 6;
 constexpr float LARGEST = 3.402823466e38f;
 
-/* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to m, m's first place (greedy) */
+/* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to the logit whose bits
+ * at is; greedy: at is m's first place */
 struct __align__(16) VfStat { double s; float m; int32_t at; };
-struct Row { float m; double s; };   /* s relative to m */
+struct Row { float m; double s; };   /* s relative to the place next to m */
 /* of a request: which row decides next (and how), for the launch that looks where p is over q; none: it has been decided */
 struct VfChoice { Row p, q; uint32_t stop, open; };
 
 struct VerifyParams {
     const uint8_t *logits, *draft;
     uint64_t ld, draft_ld;       /* bytes */
-    uint32_t vocab, chunks, n_req, n_tok, rows_all;   /* rows_all: the target's, and the draft's if there are any */
+    uint32_t vocab, n_req, n_tok;
+    uint32_t chunks, span, spans, rows_all;   /* of a row: chunks, those of a warp, warps; rows: the target's, and the draft's if there are any */
     const int32_t *token, *start;
     const float *temp, *u_accept, *u_next;
     int32_t *accepted, *next;
@@ -84,24 +87,27 @@ __device__ __forceinline__ double warp_scan(double x) {
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= LARGEST; }
 
-/* exp((x - M) / T) for logits x up to M.  fast: relative to the whole step e next to M, as above; it needs steps below 2^40 and a logit 1000 powers of two
- * below M that is still a number.  Else relative to M, by the library's function. */
+/* steps per unit of a logit, and 1000 powers of two in logits */
+struct VfScale {
+    double c, drop;
+    __device__ __forceinline__ explicit VfScale(float T) : c(STEPS / (double)T), drop(1000.0 * LN2 * (double)T) {}
+};
+/* exp((x - M) / T) for logits x up to some hundred powers of two above M.  fast: relative to the whole step e next to M, as above; it needs steps below 2^40 and
+ * a logit 1000 powers of two below M that is still a number.  Else relative to M, by the library's function. */
 struct VfExp {
-    double c, e, m, T;
+    double c, e, m;
     float low;                   /* what is below is nothing (2^-1000) */
     bool fast;
-    __device__ __forceinline__ void set(float largest, float t) {
+    __device__ __forceinline__ void set(float largest, const VfScale &S) {
         m = largest;
-        T = t;
-        c = STEPS / T;
-        const double at = m * c, far = m - 1000.0 * LN2 * T;
+        c = S.c;
+        const double at = m * c, far = m - S.drop;
         fast = fabs(at) < 1099511627776.0 && far > -1e38;
         e = rint(at);
         low = (float)far;
     }
-    __device__ __forceinline__ double slow(float x) const { return exp(((double)x - m) / T); }
-    /* what is relative to this as a factor relative to a logit of `to` */
-    __device__ __forceinline__ double over(double to) const { return fast ? exp2(fma(-to, c, e) * (1.0 / 32.0)) : exp((m - to) / T); }
+    __device__ __forceinline__ double place() const { return fast ? e : m * c; }   /* what values are relative to, in steps */
+    __device__ __forceinline__ double slow(float x) const { return exp2(((double)x - m) * c * (1.0 / 32.0)); }
     /* table: the lane's entry, less its number at the exponent's lowest bits, which the whole step brings along.  By whole warps, x not below low.  The value is f * (what is returned) */
     __device__ __forceinline__ double steps(float x, int2 table, double &f) const {
         constexpr double MAGIC = 6755399441055744.0;   /* 1.5 * 2^52: the sum's low word is the rounded integer */
@@ -118,6 +124,14 @@ struct VfExp {
         const double y = steps(fmaxf(x, low), table, f);
         return x < low ? 0.0 : f * y;
     }
+    /* what is relative to o's place (a chunk's) as a factor relative to this (its row's) */
+    __device__ __forceinline__ double from(const VfExp &o) const {
+        if (!fast || !o.fast) return exp2((fast || o.fast ? o.place() - place() : (o.m - m) * c) * (1.0 / 32.0));
+        const int32_t k = (int32_t)fmin(fmax(o.e - e, -32000.0), 32000.0);
+        return k <= -32000 ? 0.0 : __hiloint2double(__double2hiint(__ldg(g_vf_pow + (k & 31))) + (k >> 5) * 1048576, __double2loint(__ldg(g_vf_pow + (k & 31))));
+    }
+    /* log p of logit x, s being its row's sum relative to this */
+    __device__ __forceinline__ float log_p(float x, double s) const { return (float)((fast ? fma((double)x, c, -e) : ((double)x - m) * c) * (LN2 / 32.0) - log(s)); }
 };
 __device__ __forceinline__ int2 lane_table() {
     const uint32_t lane = threadIdx.x & 31u;
@@ -150,30 +164,57 @@ __device__ __forceinline__ uint32_t request_of(const int32_t *start, uint32_t n_
 __device__ __forceinline__ float temperature(const VerifyParams &P, uint32_t r) { return P.temp ? __ldcg(P.temp + r) : 1.f; }
 __device__ __forceinline__ bool temperature_ok(float t) { return t >= 0.f && t <= LARGEST; }
 
+/* 16 bytes of a row from its logit i on, around its ends: what is not its own is minus infinity */
 template <bool BF16>
-__global__ void __launch_bounds__(VF_THREADS, 7) q4_vf_stat_k(const VerifyParams P) {
-    constexpr uint32_t PER = BF16 ? 8u : 4u;
-    const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.chunks, chunk = unit - row * P.chunks;
-    const bool drafts = row >= P.n_tok;
-    const uint32_t t = drafts ? row - P.n_tok : row;
-    q4d_pdl_wait();
-    if (row >= P.rows_all) return;   /* warps behind the last row */
-    const uint8_t *base = drafts ? P.draft + t * P.draft_ld : P.logits + t * P.ld;
-    const uint32_t off = row_begins<BF16>(base);
-    float x[EACH];
+__device__ __noinline__ uint4 at_the_end(const uint8_t *base, int64_t i, uint32_t vocab) {
+    uint32_t u[4];
 #pragma unroll
-    for (uint32_t k = 0; k < EACH / PER; k++) {
-        const int64_t i = (int64_t)chunk * CHUNK + (k * 32u + lane) * PER - off;
-        if (i >= 0 && i + PER <= P.vocab) {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(base + i * (BF16 ? 2 : 4)));
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (uint32_t j = 0; j < PER; j++) x[k * PER + j] = __uint_as_float(!BF16 ? u[j & 3u] : j & 1u ? u[j / 2u] & 0xffff0000u : u[j / 2u] << 16);
+    for (uint32_t j = 0; j < 4u; j++) {
+        if constexpr (BF16) {
+            const int64_t a = i + 2 * j, b = a + 1;
+            u[j] = (a >= 0 && a < vocab ? __ldcg(reinterpret_cast<const unsigned short *>(base) + a) : 0xff80u) | (b >= 0 && b < vocab ? (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(base) + b) : 0xff80u) << 16;
         } else {
-#pragma unroll
-            for (uint32_t j = 0; j < PER; j++) x[k * PER + j] = i + j >= 0 && i + j < P.vocab ? logit<BF16>(base, (uint64_t)(i + j)) : -CUDART_INF_F;
+            u[j] = i + j >= 0 && i + j < vocab ? __ldcg(reinterpret_cast<const uint32_t *>(base) + i + j) : 0xff800000u;
         }
     }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+/* piece k of a chunk (which begins at logit i0, below 0 where the row begins in it): 16 bytes of a lane */
+template <bool BF16>
+struct Piece {
+    static constexpr uint32_t PER = BF16 ? 8u : 4u, PIECES = EACH / PER, RING = 8;   /* logits; of a chunk and lane; on their way to a lane */
+    uint4 v;
+    __device__ __forceinline__ void load(const uint8_t *base, int64_t i0, uint32_t k, uint32_t vocab) {
+        const int64_t i = i0 + (k * 32u + (threadIdx.x & 31u)) * PER;
+        if (i >= 0 && i + PER <= vocab) v = __ldcs(reinterpret_cast<const uint4 *>(base + i * (BF16 ? 2 : 4)));
+        else v = at_the_end<BF16>(base, i, vocab);
+    }
+    __device__ __forceinline__ void get(float (&x)[PER]) const {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (uint32_t j = 0; j < PER; j++) x[j] = __uint_as_float(!BF16 ? u[j & 3u] : j & 1u ? u[j / 2u] & 0xffff0000u : u[j / 2u] << 16);
+    }
+};
+
+/*
+ * A warp has `span` chunks of a row.  64-bit numbers reach 1000 powers of two either way, so that the sums need not be relative to the largest logit but to
+ * any that is not far from it: the first finite one's neighbourhood that the warp sees.  So every logit is taken up once, and its place in the
+ * ring refilled at once from the next pieces.  Where a chunk's largest logit turns out to lie too far above, it is summed again.
+ */
+template <bool BF16>
+__global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const VerifyParams P) {
+    using V = Piece<BF16>;
+    constexpr uint32_t PER = V::PER, RING = V::RING;
+    const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.spans, c0 = (unit - row * P.spans) * P.span, c1 = min(c0 + P.span, P.chunks);
+    q4d_pdl_wait();
+    if (row >= P.rows_all) return;   /* warps behind the last row */
+    const bool drafts = row >= P.n_tok;
+    const uint32_t t = drafts ? row - P.n_tok : row;
+    const uint8_t *base = drafts ? P.draft + t * P.draft_ld : P.logits + t * P.ld;
+    const int64_t off = row_begins<BF16>(base);
+    V ring[RING];
+#pragma unroll
+    for (uint32_t k = 0; k < RING; k++) ring[k].load(base, (int64_t)c0 * CHUNK - off, k, P.vocab);
     /* whose row it is, while the logits come */
     const uint32_t r = request_of(P.start, P.n_req, t);
     const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
@@ -181,82 +222,125 @@ __global__ void __launch_bounds__(VF_THREADS, 7) q4_vf_stat_k(const VerifyParams
     if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
     if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
     const int2 table = lane_table();
-    float m = max_nan(x[0], x[1]);
-#pragma unroll
-    for (uint32_t k = 2; k < EACH; k += 2u) m = max_nan(m, x[k], x[k + 1u]);
-    m = warp_max_nan(m);
-    VfStat *out = P.stat + (uint64_t)row * P.chunks + chunk;
-    if (T == 0.f) {
+    const bool greedy = T == 0.f;
+    const VfScale S(T);
+    VfStat *out = P.stat + (uint64_t)row * P.chunks;
+    VfExp E;
+    E.fast = false;
+    float ref = -CUDART_INF_F, high = -CUDART_INF_F;   /* high: 900 powers of two above ref */
+    for (uint32_t chunk = c0; chunk < c1; chunk++) {
+        const int64_t i0 = (int64_t)chunk * CHUNK - off;
+        float m = -CUDART_INF_F;
+        double s = 0.0, s1 = 0.0;
         uint32_t at = 0xffffffffu;
+        if (!greedy && !finite(ref)) {   /* of what is there: by and large the row's size */
 #pragma unroll
-        for (uint32_t k = 0; k < EACH; k++)
-            if (x[k] == m) at = min(at, (k / PER * 32u + lane) * PER + k % PER);
-        at = __reduce_min_sync(0xffffffffu, at);
-        if (lane == 0) *out = {1.0, m, (int32_t)(chunk * CHUNK + at - off)};
-        return;
-    }
-    double s = 0.0;
-    if (finite(m)) {             /* else nothing is in it, or the row is no distribution */
-        VfExp E;
-        E.set(m, T);
-        if (E.fast) {
-            double s1 = 0.0, f;
+            for (uint32_t k = 0; k < RING; k++) {
+                float x[PER];
+                ring[k].get(x);
 #pragma unroll
-            for (uint32_t k = 0; k < EACH; k += 2u) {
-                double y = E.steps(fmaxf(x[k], E.low), table, f);
-                s = fma(f, y, s);
-                y = E.steps(fmaxf(x[k + 1u], E.low), table, f);
-                s1 = fma(f, y, s1);
+                for (uint32_t j = 0; j < PER; j++) ref = fmaxf(ref, x[j]);
             }
-            s += s1;
-        } else {
-#pragma unroll 1
-            for (uint32_t k = 0; k < EACH; k++) {
-                float y = x[0];
-#pragma unroll
-                for (uint32_t j = 1; j < EACH; j++) y = j == k ? x[j] : y;
-                s += E.slow(y);
+            ref = warp_max_nan(ref);
+            if (finite(ref)) {
+                E.set(ref, S);
+                high = (float)(E.m + 0.9 * S.drop);
             }
         }
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < V::PIECES; k0 += RING)
+#pragma unroll
+        for (uint32_t k1 = 0; k1 < RING; k1++) {
+            const uint32_t k = k0 + k1;
+            float x[PER];
+            ring[k1].get(x);
+            if (k0 + RING < V::PIECES || chunk + 1u < c1) ring[k1].load(base, i0, k + RING, P.vocab);   /* of the next chunk, which lies behind */
+            if (greedy) {
+#pragma unroll
+                for (uint32_t j = 0; j < PER; j++) {
+                    if (x[j] > m || (at == 0xffffffffu && x[j] == m)) at = (k * 32u + lane) * PER + j;   /* the lane's first of the largest */
+                    m = max_nan(m, x[j]);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < PER; j += 2u) {
+                    m = max_nan(m, x[j], x[j + 1u]);
+                    double f, y = E.steps(fmaxf(x[j], E.low), table, f);
+                    s = fma(f, y, s);
+                    y = E.steps(fmaxf(x[j + 1u], E.low), table, f);
+                    s1 = fma(f, y, s1);
+                }
+            }
+        }
+        const float all = warp_max_nan(m);
+        if (greedy) {
+            at = __reduce_min_sync(0xffffffffu, m == all ? at : 0xffffffffu);
+            if (lane == 0) out[chunk] = {1.0, all, (int32_t)(chunk * CHUNK + at - off)};
+            continue;
+        }
+        s += s1;
+        float to = ref;
+        if (finite(all) && (!E.fast || all > high)) {   /* again, relative to its own largest */
+            VfExp O;
+            O.set(all, S);
+            to = all;
+            s = 0.0;
+            for (uint32_t k = 0; k < EACH; k++) {
+                const int64_t i = i0 + k * 32u + lane;
+                s += O.of(i >= 0 && i < P.vocab ? logit<BF16>(base, (uint64_t)i) : -CUDART_INF_F, table);
+            }
+        }
+        s = warp_sum(s);
+        if (lane == 0) out[chunk] = {finite(all) ? s : 0.0, all, __float_as_int(to)};
     }
-    s = warp_sum(s);
-    if (lane == 0) *out = {s, m, 0};
 }
 
 __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
     const int4 x = __ldcg(reinterpret_cast<const int4 *>(p));
     return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
 }
-/* the sum of a chunk relative to a logit of `to` */
-__device__ __forceinline__ double chunk_over(const VfStat &x, double to, float T) {
-    if (!(x.s > 0.0)) return 0.0;
+/* the sum of a chunk as one of its row's */
+__device__ __forceinline__ double chunk_in(const VfStat &x, const VfExp &row, const VfScale &S) {
     VfExp E;
-    E.set(x.m, T);
-    return x.s * E.over(to);
+    E.set(__int_as_float(x.at), S);
+    return x.s > 0.0 ? x.s * row.from(E) : 0.0;
 }
-/* a row's M and S from its chunks', by a whole warp; false: no distribution */
-__device__ __forceinline__ bool row_of(const VfStat *stat, uint32_t chunks, float T, Row &R) {
-    constexpr uint32_t AT_ONCE = 4;   /* chunks of a lane */
-    const uint32_t lane = threadIdx.x & 31u;
+/* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
+struct RowOf {
+    static constexpr uint32_t AT_ONCE = 2;   /* chunks of a lane */
     VfStat x[AT_ONCE];
-    float m = -CUDART_INF_F;
+    const VfStat *stat;
+    uint32_t chunks;
+    __device__ __forceinline__ void load(const VfStat *stat_, uint32_t chunks_) {
+        const uint32_t lane = threadIdx.x & 31u;
+        stat = stat_;
+        chunks = chunks_;
 #pragma unroll
-    for (uint32_t k = 0; k < AT_ONCE; k++) {
-        x[k] = {0.0, -CUDART_INF_F, 0};
-        if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
+        for (uint32_t k = 0; k < AT_ONCE; k++) {
+            x[k] = {0.0, -CUDART_INF_F, 0};
+            if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
+        }
     }
+    __device__ __forceinline__ bool get(const VfScale &S, Row &R) const {   /* false: no distribution */
+        const uint32_t lane = threadIdx.x & 31u;
+        float m = -CUDART_INF_F;
 #pragma unroll
-    for (uint32_t k = 0; k < AT_ONCE; k++) m = max_nan(m, x[k].m);
-    for (uint32_t c = lane + 32u * AT_ONCE; c < chunks; c += 32u) m = max_nan(m, __ldcg(&stat[c].m));
-    R.m = m = warp_max_nan(m);
-    R.s = 0.0;
-    if (!finite(m)) return false;
+        for (uint32_t k = 0; k < AT_ONCE; k++) m = max_nan(m, x[k].m);
+#pragma unroll 1
+        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) m = max_nan(m, __ldcg(&stat[i].m));
+        R.m = m = warp_max_nan(m);
+        R.s = 0.0;
+        if (!finite(m)) return false;
+        VfExp E;
+        E.set(m, S);
 #pragma unroll
-    for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_over(x[k], m, T);
-    for (uint32_t c = lane + 32u * AT_ONCE; c < chunks; c += 32u) R.s += chunk_over(stat_at(stat + c), m, T);
-    R.s = warp_sum(R.s);
-    return true;
-}
+        for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_in(x[k], E, S);
+#pragma unroll 1
+        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += chunk_in(stat_at(stat + i), E, S);
+        R.s = warp_sum(R.s);
+        return true;
+    }
+};
 /* the first place of a row's largest logit, by a whole warp */
 __device__ __forceinline__ bool best_of(const VfStat *stat, uint32_t chunks, int32_t &at) {
     const uint32_t lane = threadIdx.x & 31u;
@@ -304,18 +388,18 @@ __device__ __forceinline__ uint32_t place_of(uint32_t n, double u, double &left,
     return lo;
 }
 
-/* a row's tokens by weight: p without the refused one where drafts are certain, or what p has over q */
+/* a row's tokens by weight: p times its row's sum, without the refused one where drafts are certain, or what p has over q */
 template <bool BF16>
 struct Weights {
     const uint8_t *row_p, *row_q;
     VfExp p, q;
-    double scale_p, scale_q;
+    double scale_p, scale_q;     /* over q */
     int64_t off;
     uint32_t vocab;
     int32_t certain;             /* the token left out; -1: none */
     bool over_q;
     int2 table;
-    __device__ __forceinline__ void set(const VerifyParams &P, uint32_t row, const Row &rp, const Row &rq, float T, bool with_q, int32_t left_out) {
+    __device__ __forceinline__ void set(const VerifyParams &P, uint32_t row, const Row &rp, const Row &rq, const VfScale &S, bool with_q, int32_t left_out) {
         row_p = P.logits + row * P.ld;
         row_q = with_q ? P.draft + row * P.draft_ld : nullptr;
         off = row_begins<BF16>(row_p);
@@ -323,10 +407,10 @@ struct Weights {
         certain = left_out;
         over_q = with_q;
         table = lane_table();
-        p.set(rp.m, T);
-        scale_p = p.over(rp.m) / rp.s;
-        q.set(with_q ? rq.m : 0.f, T);
-        scale_q = with_q ? q.over(rq.m) / rq.s : 0.0;
+        p.set(rp.m, S);
+        q.set(with_q ? rq.m : 0.f, S);
+        scale_p = with_q ? 1.0 / rp.s : 1.0;
+        scale_q = with_q ? 1.0 / rq.s : 0.0;
     }
     __device__ __forceinline__ uint32_t begin(uint32_t c) const { return (uint32_t)max((int64_t)c * CHUNK - off, (int64_t)0); }
     __device__ __forceinline__ uint32_t end(uint32_t c) const { return (uint32_t)min((int64_t)(c + 1u) * CHUNK - off, (int64_t)vocab); }
@@ -335,15 +419,14 @@ struct Weights {
         xq = over_q && i < end ? logit<BF16>(row_q, i) : -CUDART_INF_F;
     }
     __device__ __forceinline__ double of(float xp, float xq, uint32_t i) const {   /* by whole warps; minus infinity: nothing */
-        const double x = __dmul_rn(p.of(xp, table), scale_p);
-        if (over_q) return fmax(__dsub_rn(x, __dmul_rn(q.of(xq, table), scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
+        const double x = p.of(xp, table);
+        if (over_q) return fmax(__dsub_rn(__dmul_rn(x, scale_p), __dmul_rn(q.of(xq, table), scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
         return (int32_t)i == certain ? 0.0 : x;
     }
 };
-
 /* by a block: the token of chunk c at which the running sum passes `left`, and its log p */
 template <bool BF16>
-__device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> &W, uint32_t r, uint32_t stop, const Row &p, uint32_t c, double left) {
+__device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> &W, uint32_t r, uint32_t stop, double sum_p, uint32_t c, double left) {
     __shared__ double s_scan[PICK_WARPS];
     __shared__ int32_t s_some[PICK_WARPS];
     __shared__ uint32_t s_found;
@@ -382,7 +465,7 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
         if (s_found == 0xffffffffu)   /* rounding, or u not below 1: the last that can be */
             for (uint32_t k = 0; k < PICK_WARPS; k++) found = max(found, s_some[k]);
         P.next[r] = found;
-        if (P.logp) P.logp[stop] = found >= 0 ? (float)(((double)logit<BF16>(W.row_p, (uint32_t)found) - (double)p.m) / W.p.T - log(p.s)) : 0.f;
+        if (P.logp) P.logp[stop] = found >= 0 ? W.p.log_p(logit<BF16>(W.row_p, (uint32_t)found), sum_p) : 0.f;
     }
 }
 
@@ -412,6 +495,8 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     const bool greedy = T == 0.f;
     const VfStat *stat_p = P.stat, *stat_q = P.stat + (uint64_t)P.n_tok * P.chunks;
     const uint32_t last = (uint32_t)b - 1u;
+    const VfScale S(T);
+    const int2 table = lane_table();
 
     /* ---- the request's rows, a warp each: whether the draft behind a row is kept.  The first that is not, or the last row, decides */
     uint32_t stop = (uint32_t)a, said = VF_NONE;
@@ -422,25 +507,38 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         const uint32_t t = t0 + warp;
         uint32_t mine = VF_KEPT;
         int32_t d = -1;
-        float lp = 0.f;
+        float xp = 0.f, xq = 0.f;
         if (t <= last) {
             if (t < last) d = __ldcg(P.token + t + 1u);
             const bool in = (uint32_t)d < P.vocab, with_q = t < last && P.draft;
             /* asked for ahead of the sums */
-            const float xp = !greedy && in ? logit<BF16>(P.logits + t * P.ld, (uint32_t)d) : 0.f, xq = !greedy && in && with_q ? logit<BF16>(P.draft + t * P.draft_ld, (uint32_t)d) : 0.f;
+            if (!greedy && in) xp = logit<BF16>(P.logits + t * P.ld, (uint32_t)d);
+            if (!greedy && in && with_q) xq = logit<BF16>(P.draft + t * P.draft_ld, (uint32_t)d);
             const float u = !greedy && t < last ? __ldcg(P.u_accept + t) : 0.f;
             if (greedy) {
                 mine = !best_of(stat_p + (uint64_t)t * P.chunks, P.chunks, best) ? VF_NONE : t == last ? VF_LAST : best == d ? VF_KEPT : VF_REFUSED;
-            } else if (!row_of(stat_p + (uint64_t)t * P.chunks, P.chunks, T, p) || (with_q && !row_of(stat_q + (uint64_t)t * P.chunks, P.chunks, T, q))) {
-                mine = VF_NONE;
-            } else if (t == last) {
-                mine = VF_LAST;
-            } else if (in) {
-                const double pd = exp(((double)xp - (double)p.m) / (double)T) / p.s, qd = P.draft ? exp(((double)xq - (double)q.m) / (double)T) / q.s : 1.0;
-                mine = (double)u * qd < pd ? VF_KEPT : VF_REFUSED;
-                if (P.logp) lp = (float)(((double)xp - (double)p.m) / (double)T - log(p.s));
             } else {
-                mine = VF_REFUSED;
+                RowOf rows[2];
+                rows[0].load(stat_p + (uint64_t)t * P.chunks, P.chunks);
+                rows[1].load(stat_q + (uint64_t)t * P.chunks, with_q ? P.chunks : 0u);
+                if (!rows[0].get(S, p) || (with_q && !rows[1].get(S, q))) {
+                    mine = VF_NONE;
+                } else if (t == last) {
+                    mine = VF_LAST;
+                } else if (in) {
+                    VfExp E;
+                    E.set(p.m, S);
+                    const double pd = E.of(xp, table);
+                    double qd = 1.0, qs = 1.0;
+                    if (with_q) {
+                        E.set(q.m, S);
+                        qd = E.of(xq, table);
+                        qs = q.s;
+                    }
+                    mine = (double)u * qd * p.s < pd * qs ? VF_KEPT : VF_REFUSED;   /* u q < p, by both sums */
+                } else {
+                    mine = VF_REFUSED;
+                }
             }
             out_of_vocab = t < last && !in;
         }
@@ -456,7 +554,11 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         const uint32_t others = __ballot_sync(0xffffffffu, lane < PICK_WARPS && s_said[lane % PICK_WARPS] != VF_KEPT);
         const uint32_t n = others ? (uint32_t)__ffs((int)others) - 1u : PICK_WARPS;
         if (lane == 0 && t < last) {
-            if (P.logp && warp < n) P.logp[t] = greedy ? 0.f : lp;
+            if (P.logp && warp < n) {
+                VfExp E;
+                E.set(p.m, S);
+                P.logp[t] = greedy ? 0.f : E.log_p(xp, p.s);
+            }
             if (out_of_vocab && warp <= n) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         }
         if (others) {
@@ -486,7 +588,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
 
     /* ---- from p: the chunk, then the place in it.  The chunk with a certain draft that was refused is summed again without that */
     Weights<BF16> W;
-    W.set(P, stop, p, q, T, false, left_out);
+    W.set(P, stop, p, q, S, false, left_out);
     const uint32_t special = (uint32_t)W.certain < P.vocab ? (uint32_t)((W.certain + W.off) / CHUNK) : 0xffffffffu;
     double without = 0.0;
     if (special != 0xffffffffu) {
@@ -505,48 +607,49 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     if (warp == 0) {
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
         double left, whole;
-        const uint32_t c = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_over(stat_at(sp + i), p.m, T) / p.s; });
+        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_in(stat_at(sp + i), W.p, S); });
         if (lane == 0) {
-            s_chunk = c;
+            s_chunk = at;
             s_left = left;
         }
     }
     __syncthreads();
-    look<BF16>(P, W, r, stop, p, s_chunk, s_left);
+    look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
 }
 
-/* what p has over q, a warp per chunk; the request's last block to finish looks for next */
+/* what p has over q, chunk by chunk; the request's last block to finish looks for next */
 template <bool BF16>
 __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams P) {
     __shared__ uint32_t s_last, s_chunk, s_over;
-    __shared__ double s_left;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk = blockIdx.x * PICK_WARPS + warp;
+    __shared__ double s_left, s_part[PICK_WARPS];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk0 = blockIdx.x;
     q4d_pdl_wait();
-    const VfChoice *at = P.choice + r;
-    if (!__ldcg(&at->open)) return;
-    const Row p = {__ldcg(&at->p.m), __ldcg(&at->p.s)}, q = {__ldcg(&at->q.m), __ldcg(&at->q.s)};
-    const uint32_t stop = __ldcg(&at->stop);
+    const VfChoice *choice = P.choice + r;
     const float T = temperature(P, r);
+    const Row p = {__ldcg(&choice->p.m), __ldcg(&choice->p.s)}, q = {__ldcg(&choice->q.m), __ldcg(&choice->q.s)};
+    const uint32_t stop = __ldcg(&choice->stop);
+    if (!__ldcg(&choice->open)) return;
     Weights<BF16> W;
-    W.set(P, stop, p, q, T, true, -1);
+    const VfScale S(T);
+    W.set(P, stop, p, q, S, true, -1);
     double *rest = P.rest + (uint64_t)r * P.chunks;
-    if (chunk < P.chunks) {
-        constexpr uint32_t AT_ONCE = 8;
-        const uint32_t i1 = W.end(chunk);
+    for (uint32_t chunk = chunk0; chunk < P.chunks; chunk += gridDim.x) {
+        const uint32_t i0 = W.begin(chunk) + tid, i1 = W.end(chunk);
+        float xp[PICK_EACH], xq[PICK_EACH];
+#pragma unroll
+        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq[k]);
         double x = 0.0;
-#pragma unroll 1
-        for (uint32_t k0 = 0; k0 < EACH; k0 += AT_ONCE) {
-            const uint32_t i0 = W.begin(chunk) + k0 * 32u + lane;
-            float xp[AT_ONCE], xq[AT_ONCE];
 #pragma unroll
-            for (uint32_t k = 0; k < AT_ONCE; k++) W.load((uint64_t)i0 + k * 32u, i1, xp[k], xq[k]);
-#pragma unroll
-            for (uint32_t k = 0; k < AT_ONCE; k++) x += W.of(xp[k], xq[k], 0u);
-        }
+        for (uint32_t k = 0; k < PICK_EACH; k++) x += W.of(xp[k], xq[k], 0u);
         x = warp_sum(x);
-        if (lane == 0) __stcg(rest + chunk, x);
+        __syncthreads();         /* the chunk before has been read */
+        if (lane == 0) s_part[warp] = x;
+        __syncthreads();
+        if (tid == 0) {
+            for (uint32_t k = 1; k < PICK_WARPS; k++) x += s_part[k];
+            __stcg(rest + chunk, x);
+        }
     }
-    __syncthreads();
     if (tid == 0) {
         __threadfence();
         s_last = atomicAdd(&g_vf_arrived[r], 1u) == gridDim.x - 1u;
@@ -558,30 +661,31 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
     if (warp == 0) {
         const double u = (double)__ldcg(P.u_next + r);
         double left, whole;
-        uint32_t c = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return __ldcg(rest + i); });
+        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return __ldcg(rest + i); });
         const bool over_q = whole > 0.0;
         if (!over_q) {           /* p nowhere above q: as if none was refused */
             const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
-            c = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_over(stat_at(sp + i), p.m, T) / p.s; });
+            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_in(stat_at(sp + i), W.p, S); });
         }
         if (lane == 0) {
-            s_chunk = c;
+            s_chunk = at;
             s_left = left;
             s_over = over_q;
         }
     }
     __syncthreads();
     W.over_q = s_over;
-    look<BF16>(P, W, r, stop, p, s_chunk, s_left);
+    look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
 }
 
 template <bool BF16>
 bool verify_launch(const VerifyParams &p) {
-    const uint64_t warps = (uint64_t)p.rows_all * p.chunks, blocks = (warps + VF_WARPS - 1u) / VF_WARPS;
+    const uint64_t warps = (uint64_t)p.rows_all * p.spans, blocks = (warps + VF_WARPS - 1u) / VF_WARPS;
     if (warps > 0x7fffffffu) return q4i_fail(Q4E_ARG, "verify: too many rows for one call");
+    const uint32_t rest_blocks = (8u * (uint32_t)g_q4.sm_count + p.n_req - 1u) / p.n_req;   /* of a request; most have nothing to do where few drafts are refused */
     return q4i_launch_pdl("verify launch", q4_vf_stat_k<BF16>, dim3((unsigned)blocks), VF_THREADS, 0, p) &&
            q4i_launch_pdl("verify launch", q4_vf_pick_k<BF16>, dim3(p.n_req), PICK_THREADS, 0, p) &&
-           (!p.draft || q4i_launch_pdl("verify launch", q4_vf_rest_k<BF16>, dim3((p.chunks + PICK_WARPS - 1u) / PICK_WARPS, p.n_req), PICK_THREADS, 0, p));
+           (!p.draft || q4i_launch_pdl("verify launch", q4_vf_rest_k<BF16>, dim3(rest_blocks < p.chunks ? rest_blocks : p.chunks, p.n_req), PICK_THREADS, 0, p));
 }
 
 }  // namespace
@@ -600,10 +704,14 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t size = bf16 ? 2u : 4u;
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
+    /* a warp's chunks: four, while there are warps for every SM several times over (one session's five drafts: one) */
+    const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 64u * (uint64_t)g_q4.sm_count;
+    p.span = all >= 4u * enough ? 4u : all >= 2u * enough ? 2u : 1u;
+    p.spans = (p.chunks + p.span - 1u) / p.span;
     p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
     p.accepted = accepted; p.next = next; p.logp = logp; p.rows = rows; p.keep = keep;
     p.err = g_q4.err_d;
-    const uint64_t stats = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, rests = draft ? (uint64_t)n_req * p.chunks : 0u, choices = draft ? n_req : 0u;
+    const uint64_t stats = all, rests = draft ? (uint64_t)n_req * p.chunks : 0u, choices = draft ? n_req : 0u;
     if (!q4i_scratch((size_t)(stats * 4u + rests * 2u + choices * (sizeof(VfChoice) / 4u)), 0)) return false;
     p.stat = (VfStat *)g_q4.part;
     p.rest = (double *)(p.stat + stats);
