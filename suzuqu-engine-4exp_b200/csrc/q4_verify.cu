@@ -22,7 +22,7 @@
 namespace {
 
 constexpr uint32_t EACH = 64, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-constexpr uint32_t STAT_BLOCKS = 6;
+constexpr uint32_t STAT_BLOCKS = 5;
 constexpr float LARGEST = 3.402823466e38f;
 
 /* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to the logit whose bits
@@ -196,10 +196,60 @@ struct Piece {
     }
 };
 
+/* Exponentials for sums, relative to a whole step e of which all that counts lies within 100 powers of two: as VfExp's, but in 32 bits and in two parts.
+ * x c comes to whole steps and a rest by a product in two words.  The table's entry is 2^(j / 32) rounded, its error goes into the rest's exponential less 1,
+ * q: the value is w + w q, where w is exact and q below 0.0109.  The sums are in 64 bits, but for up to eight w q at a time.  Errors, of the sum: steps 2.25 x 2^-25
+ * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's own last roundings 1.5 x 2^-25 x 0.0109: 5e-10;  seven additions
+ * 7 x 2^-25 x 0.0109: 2.3e-9.  Below 5e-9 in all, and for many tokens far below, as they are not all one way. */
+struct VfFast {
+    float c_hi, c_lo, base, low, high;
+    bool ok;
+    double sum;
+    __device__ __forceinline__ void set(const VfExp &E, const VfScale &S) {
+        constexpr double MAGIC = 12582912.0;   /* 1.5 * 2^23: the sum's low bits are the rounded integer */
+        ok = E.fast && fabs(E.e) < 2.0e6;
+        c_hi = (float)S.c;
+        c_lo = (float)(S.c - (double)c_hi);
+        base = (float)(MAGIC - E.e);
+        low = (float)(E.m - 0.1 * S.drop);
+        high = (float)(E.m + 0.1 * S.drop);
+    }
+    /* table: the lane's entry, less its number at the exponent's lowest bits; its error.  By whole warps */
+    template <uint32_t N>
+    __device__ __forceinline__ void add(const float (&x)[N], uint32_t table, float error) {
+        constexpr float L = (float)(LN2 / 32.0);
+        float rest = 0.f;
+#pragma unroll
+        for (uint32_t j = 0; j < N; j++) {
+            const float y = fmaxf(x[j], low), t = fmaf(y, c_hi, base), r = fmaf(y, c_lo, fmaf(y, c_hi, base - t));
+            const uint32_t k = __float_as_uint(t);
+            const float w = __uint_as_float(__shfl_sync(0xffffffffu, table, k) + (k << 18)), d = __shfl_sync(0xffffffffu, error, k);
+            const float q = fmaf(r, fmaf(r, fmaf(r, fmaf(r, L * L * L * L / 24.f, L * L * L / 6.f), L * L / 2.f), L), d);
+            sum += (double)w;
+            rest = fmaf(w, q, rest);
+        }
+        sum += (double)rest;
+    }
+};
+/* a lane's part of a chunk's sum relative to its largest logit, by the slow way */
+template <bool BF16>
+__device__ __noinline__ double sum_again(const uint8_t *base, int64_t i0, uint32_t vocab, float largest, const VfScale &S) {
+    VfExp E;
+    E.set(largest, S);
+    const int2 table = lane_table();
+    double s = 0.0;
+#pragma unroll 1
+    for (uint32_t k = 0; k < EACH; k++) {
+        const int64_t i = i0 + k * 32u + (threadIdx.x & 31u);
+        s += E.of(i >= 0 && i < vocab ? logit<BF16>(base, (uint64_t)i) : -CUDART_INF_F, table);
+    }
+    return s;
+}
+
 /*
- * A warp has `span` chunks of a row.  64-bit numbers reach 1000 powers of two either way, so that the sums need not be relative to the largest logit but to
- * any that is not far from it: the first finite one's neighbourhood that the warp sees.  So every logit is taken up once, and its place in the
- * ring refilled at once from the next pieces.  Where a chunk's largest logit turns out to lie too far above, it is summed again.
+ * A warp has `span` chunks of a row.  The sums need not be relative to the largest logit but to any within 100 powers of two of it: the largest of the first
+ * that the warp sees.  So every logit is taken up once, and its place in the ring is refilled at once from the pieces to come.  Where a
+ * chunk's largest logit turns out to lie farther off, it is summed again.
  */
 template <bool BF16>
 __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const VerifyParams P) {
@@ -221,17 +271,19 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
     const float T = temperature(P, r);
     if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
     if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
-    const int2 table = lane_table();
+    const double pow = __ldg(g_vf_pow + lane);
+    const float near = (float)pow, error = (float)((pow - (double)near) / (double)near);
+    const uint32_t table = __float_as_uint(near) - (lane << 18);
     const bool greedy = T == 0.f;
     const VfScale S(T);
     VfStat *out = P.stat + (uint64_t)row * P.chunks;
-    VfExp E;
-    E.fast = false;
-    float ref = -CUDART_INF_F, high = -CUDART_INF_F;   /* high: 900 powers of two above ref */
+    VfFast F;
+    F.ok = false;
+    F.c_hi = F.c_lo = F.base = F.low = F.high = 0.f;
+    float ref = -CUDART_INF_F;
     for (uint32_t chunk = c0; chunk < c1; chunk++) {
         const int64_t i0 = (int64_t)chunk * CHUNK - off;
         float m = -CUDART_INF_F;
-        double s = 0.0, s1 = 0.0;
         uint32_t at = 0xffffffffu;
         if (!greedy && !finite(ref)) {   /* of what is there: by and large the row's size */
 #pragma unroll
@@ -243,32 +295,33 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
             }
             ref = warp_max_nan(ref);
             if (finite(ref)) {
+                VfExp E;
                 E.set(ref, S);
-                high = (float)(E.m + 0.9 * S.drop);
+                F.set(E, S);
             }
         }
+        F.sum = 0.0;
 #pragma unroll 1
-        for (uint32_t k0 = 0; k0 < V::PIECES; k0 += RING)
+        for (uint32_t k0 = 0; k0 < V::PIECES; k0 += RING) {
+            const int64_t next = i0 + (int64_t)(k0 + RING) * (32u * PER);   /* of the next chunk, which lies behind, at last */
+            const bool more = k0 + RING < V::PIECES || chunk + 1u < c1, inside = more && next >= 0 && next + RING * 32u * PER <= P.vocab;
+            const uint4 *p = reinterpret_cast<const uint4 *>(base + next * (BF16 ? 2 : 4)) + lane;
 #pragma unroll
-        for (uint32_t k1 = 0; k1 < RING; k1++) {
-            const uint32_t k = k0 + k1;
-            float x[PER];
-            ring[k1].get(x);
-            if (k0 + RING < V::PIECES || chunk + 1u < c1) ring[k1].load(base, i0, k + RING, P.vocab);   /* of the next chunk, which lies behind */
-            if (greedy) {
+            for (uint32_t k = 0; k < RING; k++) {
+                float x[PER];
+                ring[k].get(x);
+                if (inside) ring[k].v = __ldcs(p + k * 32u);
+                else if (more) ring[k].load(base, next, k, P.vocab);
+                if (greedy) {
 #pragma unroll
-                for (uint32_t j = 0; j < PER; j++) {
-                    if (x[j] > m || (at == 0xffffffffu && x[j] == m)) at = (k * 32u + lane) * PER + j;   /* the lane's first of the largest */
-                    m = max_nan(m, x[j]);
-                }
-            } else {
+                    for (uint32_t j = 0; j < PER; j++) {
+                        if (x[j] > m || (at == 0xffffffffu && x[j] == m)) at = ((k0 + k) * 32u + lane) * PER + j;   /* the lane's first of the largest */
+                        m = max_nan(m, x[j]);
+                    }
+                } else {
 #pragma unroll
-                for (uint32_t j = 0; j < PER; j += 2u) {
-                    m = max_nan(m, x[j], x[j + 1u]);
-                    double f, y = E.steps(fmaxf(x[j], E.low), table, f);
-                    s = fma(f, y, s);
-                    y = E.steps(fmaxf(x[j + 1u], E.low), table, f);
-                    s1 = fma(f, y, s1);
+                    for (uint32_t j = 0; j < PER; j += 2u) m = max_nan(m, x[j], x[j + 1u]);
+                    F.add(x, table, error);
                 }
             }
         }
@@ -278,17 +331,11 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
             if (lane == 0) out[chunk] = {1.0, all, (int32_t)(chunk * CHUNK + at - off)};
             continue;
         }
-        s += s1;
+        double s = F.sum;
         float to = ref;
-        if (finite(all) && (!E.fast || all > high)) {   /* again, relative to its own largest */
-            VfExp O;
-            O.set(all, S);
+        if (finite(all) && (!F.ok || all > F.high || all < F.low)) {
             to = all;
-            s = 0.0;
-            for (uint32_t k = 0; k < EACH; k++) {
-                const int64_t i = i0 + k * 32u + lane;
-                s += O.of(i >= 0 && i < P.vocab ? logit<BF16>(base, (uint64_t)i) : -CUDART_INF_F, table);
-            }
+            s = sum_again<BF16>(base, i0, P.vocab, all, S);
         }
         s = warp_sum(s);
         if (lane == 0) out[chunk] = {finite(all) ? s : 0.0, all, __float_as_int(to)};
