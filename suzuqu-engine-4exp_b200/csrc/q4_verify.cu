@@ -22,7 +22,8 @@
 namespace {
 
 constexpr uint32_t EACH = 64, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-constexpr uint32_t STAT_BLOCKS = 5;
+constexpr uint32_t SPAN = 4;
+constexpr uint32_t STAT_BLOCKS = 7, VF_RING = 4;
 constexpr float LARGEST = 3.402823466e38f;
 
 /* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to the logit whose bits
@@ -30,7 +31,7 @@ constexpr float LARGEST = 3.402823466e38f;
 struct __align__(16) VfStat { double s; float m; int32_t at; };
 struct Row { float m; double s; };   /* s relative to the place next to m */
 /* of a request: which row decides next (and how), for the launch that looks where p is over q; none: it has been decided */
-struct VfChoice { Row p, q; uint32_t stop, open; };
+struct __align__(16) VfChoice { double c, drop, scale_p, scale_q, sum_p; float m_p, m_q; uint32_t stop, open; };
 
 struct VerifyParams {
     const uint8_t *logits, *draft;
@@ -67,9 +68,9 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return d;
 }
 __device__ __forceinline__ float warp_max_nan(float m) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
+    float all;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(all) : "f"(m));
+    return all;
 }
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
@@ -91,6 +92,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= LARGEST; }
 struct VfScale {
     double c, drop;
     __device__ __forceinline__ explicit VfScale(float T) : c(STEPS / (double)T), drop(1000.0 * LN2 * (double)T) {}
+    __device__ __forceinline__ VfScale(double c_, double drop_) : c(c_), drop(drop_) {}
 };
 /* exp((x - M) / T) for logits x up to some hundred powers of two above M.  fast: relative to the whole step e next to M, as above; it needs steps below 2^40 and
  * a logit 1000 powers of two below M that is still a number.  Else relative to M, by the library's function. */
@@ -125,10 +127,11 @@ struct VfExp {
         return x < low ? 0.0 : f * y;
     }
     /* what is relative to o's place (a chunk's) as a factor relative to this (its row's) */
-    __device__ __forceinline__ double from(const VfExp &o) const {
+    __device__ __forceinline__ double from(const VfExp &o, const double *pow) const {   /* pow: the table */
         if (!fast || !o.fast) return exp2((fast || o.fast ? o.place() - place() : (o.m - m) * c) * (1.0 / 32.0));
         const int32_t k = (int32_t)fmin(fmax(o.e - e, -32000.0), 32000.0);
-        return k <= -32000 ? 0.0 : __hiloint2double(__double2hiint(__ldg(g_vf_pow + (k & 31))) + (k >> 5) * 1048576, __double2loint(__ldg(g_vf_pow + (k & 31))));
+        const double x = pow[k & 31];
+        return k <= -32000 ? 0.0 : __hiloint2double(__double2hiint(x) + (k >> 5) * 1048576, __double2loint(x));
     }
     /* log p of logit x, s being its row's sum relative to this */
     __device__ __forceinline__ float log_p(float x, double s) const { return (float)((fast ? fma((double)x, c, -e) : ((double)x - m) * c) * (LN2 / 32.0) - log(s)); }
@@ -166,27 +169,26 @@ __device__ __forceinline__ bool temperature_ok(float t) { return t >= 0.f && t <
 
 /* 16 bytes of a row from its logit i on, around its ends: what is not its own is minus infinity */
 template <bool BF16>
-__device__ __noinline__ uint4 at_the_end(const uint8_t *base, int64_t i, uint32_t vocab) {
+__device__ __noinline__ uint4 at_the_end(const uint8_t *base, int32_t i, uint32_t vocab) {
     uint32_t u[4];
 #pragma unroll
     for (uint32_t j = 0; j < 4u; j++) {
         if constexpr (BF16) {
-            const int64_t a = i + 2 * j, b = a + 1;
-            u[j] = (a >= 0 && a < vocab ? __ldcg(reinterpret_cast<const unsigned short *>(base) + a) : 0xff80u) | (b >= 0 && b < vocab ? (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(base) + b) : 0xff80u) << 16;
+            const uint32_t a = i + 2 * j, b = a + 1;   /* below 0: beyond any vocabulary */
+            u[j] = (a < vocab ? __ldcg(reinterpret_cast<const unsigned short *>(base) + a) : 0xff80u) | (b < vocab ? (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(base) + b) : 0xff80u) << 16;
         } else {
-            u[j] = i + j >= 0 && i + j < vocab ? __ldcg(reinterpret_cast<const uint32_t *>(base) + i + j) : 0xff800000u;
+            u[j] = i + j < vocab ? __ldcg(reinterpret_cast<const uint32_t *>(base) + (i + j)) : 0xff800000u;
         }
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
-/* piece k of a chunk (which begins at logit i0, below 0 where the row begins in it): 16 bytes of a lane */
+/* 16 bytes of a row, a lane's: ring of them */
 template <bool BF16>
 struct Piece {
-    static constexpr uint32_t PER = BF16 ? 8u : 4u, PIECES = EACH / PER, RING = 8;   /* logits; of a chunk and lane; on their way to a lane */
+    static constexpr uint32_t PER = BF16 ? 8u : 4u, PIECES = EACH / PER, RING = VF_RING;   /* logits; of a chunk and lane; on their way to a lane */
     uint4 v;
-    __device__ __forceinline__ void load(const uint8_t *base, int64_t i0, uint32_t k, uint32_t vocab) {
-        const int64_t i = i0 + (k * 32u + (threadIdx.x & 31u)) * PER;
-        if (i >= 0 && i + PER <= vocab) v = __ldcs(reinterpret_cast<const uint4 *>(base + i * (BF16 ? 2 : 4)));
+    __device__ __forceinline__ void load(const uint8_t *base, int32_t i, uint32_t vocab) {   /* from logit i on, below 0 where the row begins in it */
+        if (i >= 0 && i + (int32_t)PER <= (int32_t)vocab) v = __ldcs(reinterpret_cast<const uint4 *>(base + (uint64_t)(uint32_t)i * (BF16 ? 2u : 4u)));
         else v = at_the_end<BF16>(base, i, vocab);
     }
     __device__ __forceinline__ void get(float (&x)[PER]) const {
@@ -199,8 +201,8 @@ struct Piece {
 /* Exponentials for sums, relative to a whole step e of which all that counts lies within 100 powers of two: as VfExp's, but in 32 bits and in two parts.
  * x c comes to whole steps and a rest by a product in two words.  The table's entry is 2^(j / 32) rounded, its error goes into the rest's exponential less 1,
  * q: the value is w + w q, where w is exact and q below 0.0109.  The sums are in 64 bits, but for up to eight w q at a time.  Errors, of the sum: steps 2.25 x 2^-25
- * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's own last roundings 1.5 x 2^-25 x 0.0109: 5e-10;  seven additions
- * 7 x 2^-25 x 0.0109: 2.3e-9.  Below 5e-9 in all, and for many tokens far below, as they are not all one way. */
+ * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's series, up to r^3: 6e-10, its last roundings 1.5 x 2^-25 x 0.0109: 5e-10;
+ * seven additions 7 x 2^-25 x 0.0109: 2.3e-9.  Below 5e-9 in all, and for many tokens far below, as they are not all one way. */
 struct VfFast {
     float c_hi, c_lo, base, low, high;
     bool ok;
@@ -224,7 +226,7 @@ struct VfFast {
             const float y = fmaxf(x[j], low), t = fmaf(y, c_hi, base), r = fmaf(y, c_lo, fmaf(y, c_hi, base - t));
             const uint32_t k = __float_as_uint(t);
             const float w = __uint_as_float(__shfl_sync(0xffffffffu, table, k) + (k << 18)), d = __shfl_sync(0xffffffffu, error, k);
-            const float q = fmaf(r, fmaf(r, fmaf(r, fmaf(r, L * L * L * L / 24.f, L * L * L / 6.f), L * L / 2.f), L), d);
+            const float q = fmaf(r, fmaf(r, fmaf(r, L * L * L / 6.f, L * L / 2.f), L), d);
             sum += (double)w;
             rest = fmaf(w, q, rest);
         }
@@ -233,17 +235,44 @@ struct VfFast {
 };
 /* a lane's part of a chunk's sum relative to its largest logit, by the slow way */
 template <bool BF16>
-__device__ __noinline__ double sum_again(const uint8_t *base, int64_t i0, uint32_t vocab, float largest, const VfScale &S) {
+__device__ __noinline__ double sum_again(const uint8_t *base, int32_t i0, uint32_t vocab, float largest, float T) {
     VfExp E;
-    E.set(largest, S);
+    E.set(largest, VfScale(T));
     const int2 table = lane_table();
     double s = 0.0;
 #pragma unroll 1
     for (uint32_t k = 0; k < EACH; k++) {
-        const int64_t i = i0 + k * 32u + (threadIdx.x & 31u);
-        s += E.of(i >= 0 && i < vocab ? logit<BF16>(base, (uint64_t)i) : -CUDART_INF_F, table);
+        const uint32_t i = i0 + k * 32u + (threadIdx.x & 31u);   /* below 0: beyond any vocabulary */
+        s += E.of(i < vocab ? logit<BF16>(base, i) : -CUDART_INF_F, table);
     }
     return s;
+}
+/* greedy rows: a chunk's largest logit and its first place */
+template <bool BF16>
+__device__ __noinline__ void best_in(const uint8_t *base, int32_t i0, uint32_t vocab, VfStat *out) {
+    using V = Piece<BF16>;
+    const uint32_t lane = threadIdx.x & 31u;
+    float m = -CUDART_INF_F;
+    uint32_t at = 0xffffffffu;
+#pragma unroll 1
+    for (uint32_t k0 = 0; k0 < V::PIECES; k0 += V::RING) {
+        V ring[V::RING];
+#pragma unroll
+        for (uint32_t k = 0; k < V::RING; k++) ring[k].load(base, i0 + (int32_t)((k0 + k) * 32u + lane) * (int32_t)V::PER, vocab);
+#pragma unroll
+        for (uint32_t k = 0; k < V::RING; k++) {
+            float x[V::PER];
+            ring[k].get(x);
+#pragma unroll
+            for (uint32_t j = 0; j < V::PER; j++) {
+                if (x[j] > m || (at == 0xffffffffu && x[j] == m)) at = ((k0 + k) * 32u + lane) * V::PER + j;   /* the lane's first of the largest */
+                m = max_nan(m, x[j]);
+            }
+        }
+    }
+    const float all = warp_max_nan(m);
+    at = __reduce_min_sync(0xffffffffu, m == all ? at : 0xffffffffu);
+    if (lane == 0) *out = {1.0, all, (int32_t)(i0 + at)};
 }
 
 /*
@@ -254,38 +283,42 @@ __device__ __noinline__ double sum_again(const uint8_t *base, int64_t i0, uint32
 template <bool BF16>
 __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const VerifyParams P) {
     using V = Piece<BF16>;
-    constexpr uint32_t PER = V::PER, RING = V::RING;
+    constexpr uint32_t PER = V::PER, RING = V::RING, HALF = RING * 32u * PER;   /* logits of a ring */
     const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.spans, c0 = (unit - row * P.spans) * P.span, c1 = min(c0 + P.span, P.chunks);
     q4d_pdl_wait();
     if (row >= P.rows_all) return;   /* warps behind the last row */
     const bool drafts = row >= P.n_tok;
-    const uint32_t t = drafts ? row - P.n_tok : row;
+    const uint32_t t = drafts ? row - P.n_tok : row, vocab = P.vocab;
     const uint8_t *base = drafts ? P.draft + t * P.draft_ld : P.logits + t * P.ld;
-    const int64_t off = row_begins<BF16>(base);
+    int32_t i0 = (int32_t)(c0 * CHUNK) - (int32_t)row_begins<BF16>(base);   /* the chunk's first logit */
     V ring[RING];
 #pragma unroll
-    for (uint32_t k = 0; k < RING; k++) ring[k].load(base, (int64_t)c0 * CHUNK - off, k, P.vocab);
+    for (uint32_t k = 0; k < RING; k++) ring[k].load(base, i0 + (int32_t)((k * 32u + lane) * PER), vocab);
     /* whose row it is, while the logits come */
-    const uint32_t r = request_of(P.start, P.n_req, t);
-    const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
-    const float T = temperature(P, r);
-    if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
-    if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
+    float T;
+    {
+        const uint32_t r = request_of(P.start, P.n_req, t);
+        const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
+        T = temperature(P, r);
+        if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
+        if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
+    }
+    VfStat *out = P.stat + (uint64_t)row * P.chunks + c0;
+    const uint32_t chunks = c1 - c0;
+    if (T == 0.f) {
+        for (uint32_t c = 0; c < chunks; c++, i0 += CHUNK) best_in<BF16>(base, i0, vocab, out + c);
+        return;
+    }
     const double pow = __ldg(g_vf_pow + lane);
     const float near = (float)pow, error = (float)((pow - (double)near) / (double)near);
     const uint32_t table = __float_as_uint(near) - (lane << 18);
-    const bool greedy = T == 0.f;
-    const VfScale S(T);
-    VfStat *out = P.stat + (uint64_t)row * P.chunks;
     VfFast F;
     F.ok = false;
     F.c_hi = F.c_lo = F.base = F.low = F.high = 0.f;
     float ref = -CUDART_INF_F;
-    for (uint32_t chunk = c0; chunk < c1; chunk++) {
-        const int64_t i0 = (int64_t)chunk * CHUNK - off;
+    for (uint32_t c = 0; c < chunks; c++, i0 += CHUNK) {
         float m = -CUDART_INF_F;
-        uint32_t at = 0xffffffffu;
-        if (!greedy && !finite(ref)) {   /* of what is there: by and large the row's size */
+        if (!finite(ref)) {          /* of what is there: by and large the row's size */
 #pragma unroll
             for (uint32_t k = 0; k < RING; k++) {
                 float x[PER];
@@ -295,6 +328,7 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
             }
             ref = warp_max_nan(ref);
             if (finite(ref)) {
+                const VfScale S(T);
                 VfExp E;
                 E.set(ref, S);
                 F.set(E, S);
@@ -302,43 +336,30 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
         }
         F.sum = 0.0;
 #pragma unroll 1
-        for (uint32_t k0 = 0; k0 < V::PIECES; k0 += RING) {
-            const int64_t next = i0 + (int64_t)(k0 + RING) * (32u * PER);   /* of the next chunk, which lies behind, at last */
-            const bool more = k0 + RING < V::PIECES || chunk + 1u < c1, inside = more && next >= 0 && next + RING * 32u * PER <= P.vocab;
-            const uint4 *p = reinterpret_cast<const uint4 *>(base + next * (BF16 ? 2 : 4)) + lane;
+        for (uint32_t k0 = 0; k0 < CHUNK; k0 += HALF) {
+            const int32_t next = i0 + (int32_t)(k0 + HALF);   /* of the next chunk, which lies behind, at last */
+            const bool more = k0 + HALF < CHUNK || c + 1u < chunks, inside = more && next >= 0 && next + HALF <= vocab;
+            const uint4 *p = reinterpret_cast<const uint4 *>(base + (int64_t)next * (BF16 ? 2 : 4)) + lane;
 #pragma unroll
             for (uint32_t k = 0; k < RING; k++) {
                 float x[PER];
                 ring[k].get(x);
                 if (inside) ring[k].v = __ldcs(p + k * 32u);
-                else if (more) ring[k].load(base, next, k, P.vocab);
-                if (greedy) {
+                else if (more) ring[k].load(base, next + (int32_t)((k * 32u + lane) * PER), vocab);
 #pragma unroll
-                    for (uint32_t j = 0; j < PER; j++) {
-                        if (x[j] > m || (at == 0xffffffffu && x[j] == m)) at = ((k0 + k) * 32u + lane) * PER + j;   /* the lane's first of the largest */
-                        m = max_nan(m, x[j]);
-                    }
-                } else {
-#pragma unroll
-                    for (uint32_t j = 0; j < PER; j += 2u) m = max_nan(m, x[j], x[j + 1u]);
-                    F.add(x, table, error);
-                }
+                for (uint32_t j = 0; j < PER; j += 2u) m = max_nan(m, x[j], x[j + 1u]);
+                F.add(x, table, error);
             }
         }
         const float all = warp_max_nan(m);
-        if (greedy) {
-            at = __reduce_min_sync(0xffffffffu, m == all ? at : 0xffffffffu);
-            if (lane == 0) out[chunk] = {1.0, all, (int32_t)(chunk * CHUNK + at - off)};
-            continue;
-        }
         double s = F.sum;
         float to = ref;
         if (finite(all) && (!F.ok || all > F.high || all < F.low)) {
             to = all;
-            s = sum_again<BF16>(base, i0, P.vocab, all, S);
+            s = sum_again<BF16>(base, i0, vocab, all, T);
         }
         s = warp_sum(s);
-        if (lane == 0) out[chunk] = {finite(all) ? s : 0.0, all, __float_as_int(to)};
+        if (lane == 0) out[c] = {finite(all) ? s : 0.0, all, __float_as_int(to)};
     }
 }
 
@@ -347,10 +368,10 @@ __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
     return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
 }
 /* the sum of a chunk as one of its row's */
-__device__ __forceinline__ double chunk_in(const VfStat &x, const VfExp &row, const VfScale &S) {
+__device__ __forceinline__ double chunk_in(const VfStat &x, const VfExp &row, const VfScale &S, const double *pow) {
     VfExp E;
     E.set(__int_as_float(x.at), S);
-    return x.s > 0.0 ? x.s * row.from(E) : 0.0;
+    return x.s > 0.0 ? x.s * row.from(E, pow) : 0.0;
 }
 /* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
 struct RowOf {
@@ -368,7 +389,7 @@ struct RowOf {
             if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
         }
     }
-    __device__ __forceinline__ bool get(const VfScale &S, Row &R) const {   /* false: no distribution */
+    __device__ __forceinline__ bool get(const VfScale &S, const double *pow, Row &R) const {   /* false: no distribution */
         const uint32_t lane = threadIdx.x & 31u;
         float m = -CUDART_INF_F;
 #pragma unroll
@@ -381,9 +402,9 @@ struct RowOf {
         VfExp E;
         E.set(m, S);
 #pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_in(x[k], E, S);
+        for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_in(x[k], E, S, pow);
 #pragma unroll 1
-        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += chunk_in(stat_at(stat + i), E, S);
+        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += chunk_in(stat_at(stat + i), E, S, pow);
         R.s = warp_sum(R.s);
         return true;
     }
@@ -446,7 +467,7 @@ struct Weights {
     int32_t certain;             /* the token left out; -1: none */
     bool over_q;
     int2 table;
-    __device__ __forceinline__ void set(const VerifyParams &P, uint32_t row, const Row &rp, const Row &rq, const VfScale &S, bool with_q, int32_t left_out) {
+    __device__ __forceinline__ void set(const VerifyParams &P, uint32_t row, float m_p, float m_q, double scale_p_, double scale_q_, const VfScale &S, bool with_q, int32_t left_out) {
         row_p = P.logits + row * P.ld;
         row_q = with_q ? P.draft + row * P.draft_ld : nullptr;
         off = row_begins<BF16>(row_p);
@@ -454,10 +475,10 @@ struct Weights {
         certain = left_out;
         over_q = with_q;
         table = lane_table();
-        p.set(rp.m, S);
-        q.set(with_q ? rq.m : 0.f, S);
-        scale_p = with_q ? 1.0 / rp.s : 1.0;
-        scale_q = with_q ? 1.0 / rq.s : 0.0;
+        p.set(m_p, S);
+        q.set(m_q, S);
+        scale_p = scale_p_;
+        scale_q = scale_q_;
     }
     __device__ __forceinline__ uint32_t begin(uint32_t c) const { return (uint32_t)max((int64_t)c * CHUNK - off, (int64_t)0); }
     __device__ __forceinline__ uint32_t end(uint32_t c) const { return (uint32_t)min((int64_t)(c + 1u) * CHUNK - off, (int64_t)vocab); }
@@ -523,15 +544,17 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     __shared__ Row s_p[PICK_WARPS], s_q[PICK_WARPS];
     __shared__ uint32_t s_said[PICK_WARPS], s_chunk;
     __shared__ int32_t s_best[PICK_WARPS], s_draft[PICK_WARPS];
-    __shared__ double s_left, s_part[PICK_WARPS];
+    __shared__ double s_left, s_part[PICK_WARPS], s_pow[32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.x;
-    q4d_pdl_wait();
+    /* The launch before this one began behind everything that its inputs come from: they are there.  What it writes is waited for below. */
+    if (tid < 32u) s_pow[tid] = __ldg(g_vf_pow + tid);
     const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
     const float T = temperature(P, r);
     const bool bounds = a >= 0 && b >= a && (uint32_t)b <= P.n_tok;
-    if (tid == 0 && P.draft) P.choice[r].open = 0u;
     if (!bounds || a == b) {
+        q4d_pdl_wait();
         if (tid == 0) {
+            if (P.draft) P.choice[r].open = 0u;
             P.accepted[r] = 0;
             P.next[r] = -1;
             if (P.keep) P.keep[r] = __ldcg(P.rows + r);
@@ -549,7 +572,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     uint32_t stop = (uint32_t)a, said = VF_NONE;
     Row p = {}, q = {};
     int32_t best = -1, left_out = -1;   /* left_out: the draft behind the row that decides */
-    bool out_of_vocab = false;
+    bool out_of_vocab = false, waited = false;
     for (uint32_t t0 = (uint32_t)a; temperature_ok(T); t0 += PICK_WARPS) {
         const uint32_t t = t0 + warp;
         uint32_t mine = VF_KEPT;
@@ -562,13 +585,15 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             if (!greedy && in) xp = logit<BF16>(P.logits + t * P.ld, (uint32_t)d);
             if (!greedy && in && with_q) xq = logit<BF16>(P.draft + t * P.draft_ld, (uint32_t)d);
             const float u = !greedy && t < last ? __ldcg(P.u_accept + t) : 0.f;
+            if (!waited) q4d_pdl_wait();
+            waited = true;
             if (greedy) {
                 mine = !best_of(stat_p + (uint64_t)t * P.chunks, P.chunks, best) ? VF_NONE : t == last ? VF_LAST : best == d ? VF_KEPT : VF_REFUSED;
             } else {
                 RowOf rows[2];
                 rows[0].load(stat_p + (uint64_t)t * P.chunks, P.chunks);
                 rows[1].load(stat_q + (uint64_t)t * P.chunks, with_q ? P.chunks : 0u);
-                if (!rows[0].get(S, p) || (with_q && !rows[1].get(S, q))) {
+                if (!rows[0].get(S, s_pow, p) || (with_q && !rows[1].get(S, s_pow, q))) {
                     mine = VF_NONE;
                 } else if (t == last) {
                     mine = VF_LAST;
@@ -589,6 +614,8 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             }
             out_of_vocab = t < last && !in;
         }
+        if (!waited) q4d_pdl_wait();
+        waited = true;
         __syncthreads();
         if (lane == 0) {
             s_said[warp] = mine;
@@ -618,6 +645,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             break;
         }
     }
+    if (!waited) q4d_pdl_wait();
     if (P.logp)
         for (uint32_t t = stop + 1u + tid; t <= last; t += PICK_THREADS) P.logp[t] = 0.f;
     const bool refused = said == VF_REFUSED && !greedy, open = refused && P.draft;
@@ -629,13 +657,14 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             if (P.logp) P.logp[stop] = 0.f;
             if (said == VF_NONE) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         }
-        if (open) P.choice[r] = {p, q, stop, 1u};
+        if (P.draft && !open) P.choice[r].open = 0u;
+        if (open) P.choice[r] = {S.c, S.drop, 1.0 / p.s, 1.0 / q.s, p.s, p.m, q.m, stop, 1u};
     }
     if (said == VF_NONE || greedy || open) return;
 
     /* ---- from p: the chunk, then the place in it.  The chunk with a certain draft that was refused is summed again without that */
     Weights<BF16> W;
-    W.set(P, stop, p, q, S, false, left_out);
+    W.set(P, stop, p.m, 0.f, 1.0, 0.0, S, false, left_out);
     const uint32_t special = (uint32_t)W.certain < P.vocab ? (uint32_t)((W.certain + W.off) / CHUNK) : 0xffffffffu;
     double without = 0.0;
     if (special != 0xffffffffu) {
@@ -654,7 +683,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     if (warp == 0) {
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
         double left, whole;
-        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_in(stat_at(sp + i), W.p, S); });
+        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_in(stat_at(sp + i), W.p, S, s_pow); });
         if (lane == 0) {
             s_chunk = at;
             s_left = left;
@@ -668,17 +697,22 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
 template <bool BF16>
 __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams P) {
     __shared__ uint32_t s_last, s_chunk, s_over;
-    __shared__ double s_left, s_part[PICK_WARPS];
+    __shared__ double s_left, s_part[PICK_WARPS], s_pow[32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk0 = blockIdx.x;
+    if (tid < 32u) s_pow[tid] = __ldg(g_vf_pow + tid);
     q4d_pdl_wait();
-    const VfChoice *choice = P.choice + r;
-    const float T = temperature(P, r);
-    const Row p = {__ldcg(&choice->p.m), __ldcg(&choice->p.s)}, q = {__ldcg(&choice->q.m), __ldcg(&choice->q.s)};
-    const uint32_t stop = __ldcg(&choice->stop);
-    if (!__ldcg(&choice->open)) return;
+    VfChoice D;
+    {
+        const int4 *from = reinterpret_cast<const int4 *>(P.choice + r);
+        int4 *to = reinterpret_cast<int4 *>(&D);
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(VfChoice) / 16u; i++) to[i] = __ldcg(from + i);
+    }
+    if (!D.open) return;
+    const uint32_t stop = D.stop;
+    const VfScale S(D.c, D.drop);
     Weights<BF16> W;
-    const VfScale S(T);
-    W.set(P, stop, p, q, S, true, -1);
+    W.set(P, stop, D.m_p, D.m_q, D.scale_p, D.scale_q, S, true, -1);
     double *rest = P.rest + (uint64_t)r * P.chunks;
     for (uint32_t chunk = chunk0; chunk < P.chunks; chunk += gridDim.x) {
         const uint32_t i0 = W.begin(chunk) + tid, i1 = W.end(chunk);
@@ -712,7 +746,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
         const bool over_q = whole > 0.0;
         if (!over_q) {           /* p nowhere above q: as if none was refused */
             const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
-            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_in(stat_at(sp + i), W.p, S); });
+            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_in(stat_at(sp + i), W.p, S, s_pow); });
         }
         if (lane == 0) {
             s_chunk = at;
@@ -722,7 +756,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
     }
     __syncthreads();
     W.over_q = s_over;
-    look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
+    look<BF16>(P, W, r, stop, D.sum_p, s_chunk, s_left);
 }
 
 template <bool BF16>
@@ -743,7 +777,7 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     if (!g_q4.ok) return q4i_fail(Q4E_INIT, "verify: library not initialised");
     Q4_REQUIRE(logits && token && start && u_accept && u_next && accepted && next && vocab && n_req && n_tok, "verify: bad argument");
     Q4_REQUIRE(!rows == !keep, "verify: rows and keep go together");
-    Q4_REQUIRE(n_req <= PLAN_MAX_REQ && n_tok <= 0x7fffffffu && vocab <= 0x7fffffffu, "verify: at most 8192 requests, 2^31 - 1 rows and tokens");
+    Q4_REQUIRE(n_req <= PLAN_MAX_REQ && n_tok <= 0x3fffffffu && vocab <= 0x3fffffffu, "verify: at most 8192 requests, 2^30 - 1 rows and tokens");
     Q4_REQUIRE(n_tok == 1u || (ld >= vocab && (!draft || draft_ld >= vocab)), "verify: rows are closer than the vocabulary is wide");
     Q4_REQUIRE(ld < 1ull << 40 && draft_ld < 1ull << 40, "verify: rows are too far apart");
     Q4_REQUIRE(((uintptr_t)logits & (bf16 ? 1u : 3u)) == 0 && ((uintptr_t)draft & (bf16 ? 1u : 3u)) == 0, "verify: logits are not aligned to their type");
@@ -753,7 +787,7 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
     /* a warp's chunks: four, while there are warps for every SM several times over (one session's five drafts: one) */
     const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 64u * (uint64_t)g_q4.sm_count;
-    p.span = all >= 4u * enough ? 4u : all >= 2u * enough ? 2u : 1u;
+    p.span = all >= SPAN * enough ? SPAN : all >= 2u * enough ? 2u : 1u;
     p.spans = (p.chunks + p.span - 1u) / p.span;
     p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
     p.accepted = accepted; p.next = next; p.logp = logp; p.rows = rows; p.keep = keep;
@@ -761,7 +795,7 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t stats = all, rests = draft ? (uint64_t)n_req * p.chunks : 0u, choices = draft ? n_req : 0u;
     if (!q4i_scratch((size_t)(stats * 4u + rests * 2u + choices * (sizeof(VfChoice) / 4u)), 0)) return false;
     p.stat = (VfStat *)g_q4.part;
-    p.rest = (double *)(p.stat + stats);
-    p.choice = (VfChoice *)(p.rest + rests);
+    p.choice = (VfChoice *)(p.stat + stats);
+    p.rest = (double *)(p.choice + choices);
     return bf16 ? verify_launch<true>(p) : verify_launch<false>(p);
 }
