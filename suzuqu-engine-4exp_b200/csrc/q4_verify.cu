@@ -26,10 +26,11 @@ constexpr uint32_t SPAN = 4;
 constexpr uint32_t STAT_BLOCKS = 7, VF_RING = 4;
 constexpr float LARGEST = 3.402823466e38f;
 
-/* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to VfExp's place next to the logit whose bits
- * at is; greedy: at is m's first place */
+/* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to a whole step, whose bits as a float at is (NaN:
+ * relative to m); greedy: at is m's first place */
 struct __align__(16) VfStat { double s; float m; int32_t at; };
-struct Row { float m; double s; };   /* s relative to the place next to m */
+constexpr int32_t NO_STEP = 0x7fffffff;
+struct Row { float m; double s; };   /* s relative to VfExp's place */
 /* of a request: which row decides next (and how), for the launch that looks where p is over q; none: it has been decided */
 struct __align__(16) VfChoice { double c, drop, scale_p, scale_q, sum_p; float m_p, m_q; uint32_t stop, open; };
 
@@ -94,21 +95,20 @@ struct VfScale {
     __device__ __forceinline__ explicit VfScale(float T) : c(STEPS / (double)T), drop(1000.0 * LN2 * (double)T) {}
     __device__ __forceinline__ VfScale(double c_, double drop_) : c(c_), drop(drop_) {}
 };
-/* exp((x - M) / T) for logits x up to some hundred powers of two above M.  fast: relative to the whole step e next to M, as above; it needs steps below 2^40 and
- * a logit 1000 powers of two below M that is still a number.  Else relative to M, by the library's function. */
+/* exp((x - M) / T) for logits x up to some hundred powers of two above M.  fast: relative to the whole step e next to M, as above, where that is a number of 21 bits
+ * and a logit 1000 powers of two below M is still a number.  Else relative to M, by the library's function. */
 struct VfExp {
-    double c, e, m;
+    double c, e, m;              /* e: 0 where not fast */
     float low;                   /* what is below is nothing (2^-1000) */
     bool fast;
     __device__ __forceinline__ void set(float largest, const VfScale &S) {
         m = largest;
         c = S.c;
-        const double at = m * c, far = m - S.drop;
-        fast = fabs(at) < 1099511627776.0 && far > -1e38;
-        e = rint(at);
-        low = (float)far;
+        const double at = m * c;
+        fast = fabs(at) < 2.0e6 && S.drop < 1e35;
+        e = fast ? rint(at) : 0.0;
+        low = (float)(m - S.drop);
     }
-    __device__ __forceinline__ double place() const { return fast ? e : m * c; }   /* what values are relative to, in steps */
     __device__ __forceinline__ double slow(float x) const { return exp2(((double)x - m) * c * (1.0 / 32.0)); }
     /* table: the lane's entry, less its number at the exponent's lowest bits, which the whole step brings along.  By whole warps, x not below low.  The value is f * (what is returned) */
     __device__ __forceinline__ double steps(float x, int2 table, double &f) const {
@@ -120,21 +120,36 @@ struct VfExp {
         f = __hiloint2double(hi + (k << 15), lo);
         return fma(r, fma(r, fma(r, fma(r, fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0), L * L * L / 6.0), L * L / 2.0), L), 1.0);
     }
-    __device__ __forceinline__ double of(float x, int2 table) const {
-        if (!fast) return slow(x);
-        double f;
-        const double y = steps(fmaxf(x, low), table, f);
-        return x < low ? 0.0 : f * y;
+    /* of several at once: a chain of operations of this kind takes 500 cycles, in which others can be at theirs */
+    template <uint32_t N>
+    __device__ __forceinline__ void of(const float (&x)[N], int2 table, double (&w)[N]) const {
+        if (fast) {
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++) {
+                double f;
+                const double y = steps(fmaxf(x[k], low), table, f);
+                w[k] = x[k] < low ? 0.0 : f * y;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++) w[k] = slow(x[k]);
+        }
     }
-    /* what is relative to o's place (a chunk's) as a factor relative to this (its row's) */
-    __device__ __forceinline__ double from(const VfExp &o, const double *pow) const {   /* pow: the table */
-        if (!fast || !o.fast) return exp2((fast || o.fast ? o.place() - place() : (o.m - m) * c) * (1.0 / 32.0));
-        const int32_t k = (int32_t)fmin(fmax(o.e - e, -32000.0), 32000.0);
-        const double x = pow[k & 31];
-        return k <= -32000 ? 0.0 : __hiloint2double(__double2hiint(x) + (k >> 5) * 1048576, __double2loint(x));
+    /* a chunk's sum as one relative to this, its row's; pow: the table */
+    __device__ __forceinline__ double chunk_fast(const VfStat &x, const double *pow) const {   /* both by whole steps */
+        const int32_t k = (int32_t)fminf(fmaxf(__int_as_float(x.at) - (float)e, -32000.f), 32000.f);
+        const double f = pow[k & 31];
+        return k <= -32000 ? 0.0 : x.s * __hiloint2double(__double2hiint(f) + (k >> 5) * 1048576, __double2loint(f));
     }
-    /* log p of logit x, s being its row's sum relative to this */
-    __device__ __forceinline__ float log_p(float x, double s) const { return (float)((fast ? fma((double)x, c, -e) : ((double)x - m) * c) * (LN2 / 32.0) - log(s)); }
+    __device__ __forceinline__ double chunk(const VfStat &x, const double *pow) const {
+        const float at = __int_as_float(x.at);
+        if (fast && x.at != NO_STEP) return chunk_fast(x, pow);
+        if (!(x.s > 0.0)) return 0.0;
+        if (x.at == NO_STEP && !fast) return x.s * slow(x.m);
+        return x.s * exp2(((x.at == NO_STEP ? (double)x.m * c : (double)at) - (fast ? e : m * c)) * (1.0 / 32.0));
+    }
+    /* log p of logit x, log_s being the logarithm of its row's sum relative to this */
+    __device__ __forceinline__ float log_p(float x, double log_s) const { return (float)((fast ? fma((double)x, c, -e) : ((double)x - m) * c) * (LN2 / 32.0) - log_s); }
 };
 __device__ __forceinline__ int2 lane_table() {
     const uint32_t lane = threadIdx.x & 31u;
@@ -204,15 +219,16 @@ struct Piece {
  * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's series, up to r^3: 6e-10, its last roundings 1.5 x 2^-25 x 0.0109: 5e-10;
  * seven additions 7 x 2^-25 x 0.0109: 2.3e-9.  Below 5e-9 in all, and for many tokens far below, as they are not all one way. */
 struct VfFast {
-    float c_hi, c_lo, base, low, high;
+    float c_hi, c_lo, base, low, high, step;
     bool ok;
     double sum;
     __device__ __forceinline__ void set(const VfExp &E, const VfScale &S) {
         constexpr double MAGIC = 12582912.0;   /* 1.5 * 2^23: the sum's low bits are the rounded integer */
-        ok = E.fast && fabs(E.e) < 2.0e6;
+        ok = E.fast;
         c_hi = (float)S.c;
         c_lo = (float)(S.c - (double)c_hi);
         base = (float)(MAGIC - E.e);
+        step = (float)E.e;
         low = (float)(E.m - 0.1 * S.drop);
         high = (float)(E.m + 0.1 * S.drop);
     }
@@ -233,7 +249,7 @@ struct VfFast {
         sum += (double)rest;
     }
 };
-/* a lane's part of a chunk's sum relative to its largest logit, by the slow way */
+/* a lane's part of a chunk's sum relative to its largest logit */
 template <bool BF16>
 __device__ __noinline__ double sum_again(const uint8_t *base, int32_t i0, uint32_t vocab, float largest, float T) {
     VfExp E;
@@ -243,9 +259,12 @@ __device__ __noinline__ double sum_again(const uint8_t *base, int32_t i0, uint32
 #pragma unroll 1
     for (uint32_t k = 0; k < EACH; k++) {
         const uint32_t i = i0 + k * 32u + (threadIdx.x & 31u);   /* below 0: beyond any vocabulary */
-        s += E.of(i < vocab ? logit<BF16>(base, i) : -CUDART_INF_F, table);
+        const float x[1] = {i < vocab ? logit<BF16>(base, i) : -CUDART_INF_F};
+        double w[1];
+        E.of(x, table, w);
+        s += w[0];
     }
-    return s;
+    return E.fast ? s * exp2(fma(-E.m, E.c, E.e) * (1.0 / 32.0)) : s;
 }
 /* greedy rows: a chunk's largest logit and its first place */
 template <bool BF16>
@@ -314,7 +333,7 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
     const uint32_t table = __float_as_uint(near) - (lane << 18);
     VfFast F;
     F.ok = false;
-    F.c_hi = F.c_lo = F.base = F.low = F.high = 0.f;
+    F.c_hi = F.c_lo = F.base = F.low = F.high = F.step = 0.f;
     float ref = -CUDART_INF_F;
     for (uint32_t c = 0; c < chunks; c++, i0 += CHUNK) {
         float m = -CUDART_INF_F;
@@ -353,25 +372,19 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
         }
         const float all = warp_max_nan(m);
         double s = F.sum;
-        float to = ref;
+        int32_t to = __float_as_int(F.step);
         if (finite(all) && (!F.ok || all > F.high || all < F.low)) {
-            to = all;
+            to = NO_STEP;
             s = sum_again<BF16>(base, i0, vocab, all, T);
         }
         s = warp_sum(s);
-        if (lane == 0) out[c] = {finite(all) ? s : 0.0, all, __float_as_int(to)};
+        if (lane == 0) out[c] = {finite(all) ? s : 0.0, all, to};
     }
 }
 
 __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
     const int4 x = __ldcg(reinterpret_cast<const int4 *>(p));
     return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
-}
-/* the sum of a chunk as one of its row's */
-__device__ __forceinline__ double chunk_in(const VfStat &x, const VfExp &row, const VfScale &S, const double *pow) {
-    VfExp E;
-    E.set(__int_as_float(x.at), S);
-    return x.s > 0.0 ? x.s * row.from(E, pow) : 0.0;
 }
 /* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
 struct RowOf {
@@ -385,7 +398,7 @@ struct RowOf {
         chunks = chunks_;
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; k++) {
-            x[k] = {0.0, -CUDART_INF_F, 0};
+            x[k] = {0.0, -CUDART_INF_F, __float_as_int(0.f)};
             if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
         }
     }
@@ -401,10 +414,18 @@ struct RowOf {
         if (!finite(m)) return false;
         VfExp E;
         E.set(m, S);
+        bool steps = E.fast;
 #pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; k++) R.s += chunk_in(x[k], E, S, pow);
+        for (uint32_t k = 0; k < AT_ONCE; k++) steps = steps && x[k].at != NO_STEP;
+        if (__all_sync(0xffffffffu, steps)) {
+#pragma unroll
+            for (uint32_t k = 0; k < AT_ONCE; k++) R.s += E.chunk_fast(x[k], pow);
+        } else {
 #pragma unroll 1
-        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += chunk_in(stat_at(stat + i), E, S, pow);
+            for (uint32_t k = 0; k < AT_ONCE; k++) R.s += E.chunk(x[k], pow);
+        }
+#pragma unroll 1
+        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += E.chunk(stat_at(stat + i), pow);
         R.s = warp_sum(R.s);
         return true;
     }
@@ -486,10 +507,19 @@ struct Weights {
         xp = i < end ? logit<BF16>(row_p, i) : -CUDART_INF_F;
         xq = over_q && i < end ? logit<BF16>(row_q, i) : -CUDART_INF_F;
     }
-    __device__ __forceinline__ double of(float xp, float xq, uint32_t i) const {   /* by whole warps; minus infinity: nothing */
-        const double x = p.of(xp, table);
-        if (over_q) return fmax(__dsub_rn(__dmul_rn(x, scale_p), __dmul_rn(q.of(xq, table), scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
-        return (int32_t)i == certain ? 0.0 : x;
+    template <uint32_t N>
+    __device__ __forceinline__ void of(const float (&xp)[N], const float (&xq)[N], uint32_t i0, uint32_t step, double (&w)[N]) const {   /* of tokens i0, i0 + step ..; by whole warps; minus infinity: nothing */
+        p.of(xp, table, w);
+        if (over_q) {
+            double y[N];
+            q.of(xq, table, y);
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++) w[k] = fmax(__dsub_rn(__dmul_rn(w[k], scale_p), __dmul_rn(y[k], scale_q)), 0.0);   /* both rounded: equal ones leave nothing */
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++)
+                if ((int32_t)(i0 + k * step) == certain) w[k] = 0.0;
+        }
     }
 };
 /* by a block: the token of chunk c at which the running sum passes `left`, and its log p */
@@ -503,11 +533,12 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
     float xp[PICK_EACH], xq[PICK_EACH];
 #pragma unroll
     for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k, i1, xp[k], xq[k]);
+    const double log_s = log(sum_p);   /* while they come */
     double w[PICK_EACH], sum = 0.0;
     int32_t some = -1;
+    W.of(xp, xq, i0, 1u, w);
 #pragma unroll
     for (uint32_t k = 0; k < PICK_EACH; k++) {
-        w[k] = W.of(xp[k], xq[k], i0 + k);
         sum += w[k];
         if (w[k] > 0.0) some = (int32_t)(i0 + k);
     }
@@ -533,7 +564,7 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
         if (s_found == 0xffffffffu)   /* rounding, or u not below 1: the last that can be */
             for (uint32_t k = 0; k < PICK_WARPS; k++) found = max(found, s_some[k]);
         P.next[r] = found;
-        if (P.logp) P.logp[stop] = found >= 0 ? W.p.log_p(logit<BF16>(W.row_p, (uint32_t)found), sum_p) : 0.f;
+        if (P.logp) P.logp[stop] = found >= 0 ? W.p.log_p(logit<BF16>(W.row_p, (uint32_t)found), log_s) : 0.f;
     }
 }
 
@@ -599,15 +630,16 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
                     mine = VF_LAST;
                 } else if (in) {
                     VfExp E;
+                    const float one_p[1] = {xp}, one_q[1] = {xq};
+                    double pd[1] = {0.0}, qd[1] = {1.0}, qs = 1.0;
                     E.set(p.m, S);
-                    const double pd = E.of(xp, table);
-                    double qd = 1.0, qs = 1.0;
+                    E.of(one_p, table, pd);
                     if (with_q) {
                         E.set(q.m, S);
-                        qd = E.of(xq, table);
+                        E.of(one_q, table, qd);
                         qs = q.s;
                     }
-                    mine = (double)u * qd * p.s < pd * qs ? VF_KEPT : VF_REFUSED;   /* u q < p, by both sums */
+                    mine = (double)u * qd[0] * p.s < pd[0] * qs ? VF_KEPT : VF_REFUSED;   /* u q < p, by both sums */
                 } else {
                     mine = VF_REFUSED;
                 }
@@ -631,7 +663,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
             if (P.logp && warp < n) {
                 VfExp E;
                 E.set(p.m, S);
-                P.logp[t] = greedy ? 0.f : E.log_p(xp, p.s);
+                P.logp[t] = greedy ? 0.f : E.log_p(xp, log(p.s));
             }
             if (out_of_vocab && warp <= n) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         }
@@ -669,11 +701,13 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     double without = 0.0;
     if (special != 0xffffffffu) {
         const uint32_t i0 = W.begin(special) + tid, i1 = W.end(special);
-        float xp[PICK_EACH], xq;
+        float xp[PICK_EACH], xq[PICK_EACH];
+        double w[PICK_EACH];
 #pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq);
+        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq[k]);
+        W.of(xp, xq, i0, PICK_THREADS, w);
 #pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) without += W.of(xp[k], 0.f, i0 + k * PICK_THREADS);
+        for (uint32_t k = 0; k < PICK_EACH; k++) without += w[k];
         without = warp_sum(without);
         if (lane == 0) s_part[warp] = without;
         __syncthreads();
@@ -683,7 +717,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     if (warp == 0) {
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
         double left, whole;
-        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : chunk_in(stat_at(sp + i), W.p, S, s_pow); });
+        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : W.p.chunk(stat_at(sp + i), s_pow); });
         if (lane == 0) {
             s_chunk = at;
             s_left = left;
@@ -719,16 +753,19 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
         float xp[PICK_EACH], xq[PICK_EACH];
 #pragma unroll
         for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq[k]);
-        double x = 0.0;
+        double w[PICK_EACH], x = 0.0;
+        W.of(xp, xq, i0, PICK_THREADS, w);
 #pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) x += W.of(xp[k], xq[k], 0u);
+        for (uint32_t k = 0; k < PICK_EACH; k++) x += w[k];
         x = warp_sum(x);
         __syncthreads();         /* the chunk before has been read */
         if (lane == 0) s_part[warp] = x;
         __syncthreads();
-        if (tid == 0) {
-            for (uint32_t k = 1; k < PICK_WARPS; k++) x += s_part[k];
-            __stcg(rest + chunk, x);
+        if (warp == 0) {
+            x = lane < PICK_WARPS ? s_part[lane] : 0.0;
+#pragma unroll
+            for (uint32_t o = PICK_WARPS / 2u; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if (lane == 0) __stcg(rest + chunk, x);
         }
     }
     if (tid == 0) {
@@ -746,7 +783,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
         const bool over_q = whole > 0.0;
         if (!over_q) {           /* p nowhere above q: as if none was refused */
             const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
-            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return chunk_in(stat_at(sp + i), W.p, S, s_pow); });
+            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return W.p.chunk(stat_at(sp + i), s_pow); });
         }
         if (lane == 0) {
             s_chunk = at;
