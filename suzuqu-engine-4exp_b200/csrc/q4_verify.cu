@@ -15,6 +15,7 @@
  * takes some 20.  The first launch is bound by its instructions, 15 per logit, beside memory.
  */
 #include <math_constants.h>
+#include <type_traits>
 
 #include "q4_internal.h"
 #include "q4_pages_scan.h"
@@ -22,8 +23,8 @@
 namespace {
 
 constexpr uint32_t EACH = 64, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-constexpr uint32_t SPAN = 4;
-constexpr uint32_t STAT_BLOCKS = 7, VF_RING = 4;
+constexpr uint32_t SPAN = 3;
+constexpr uint32_t STAT_BLOCKS = 5, VF_RING = 4;
 constexpr float LARGEST = 3.402823466e38f;
 
 /* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to a whole step, whose bits as a float at is (NaN:
@@ -221,7 +222,7 @@ struct Piece {
 struct VfFast {
     float c_hi, c_lo, base, low, high, step;
     bool ok;
-    double sum;
+    double sum[2];
     __device__ __forceinline__ void set(const VfExp &E, const VfScale &S) {
         constexpr double MAGIC = 12582912.0;   /* 1.5 * 2^23: the sum's low bits are the rounded integer */
         ok = E.fast;
@@ -243,10 +244,10 @@ struct VfFast {
             const uint32_t k = __float_as_uint(t);
             const float w = __uint_as_float(__shfl_sync(0xffffffffu, table, k) + (k << 18)), d = __shfl_sync(0xffffffffu, error, k);
             const float q = fmaf(r, fmaf(r, fmaf(r, L * L * L / 6.f, L * L / 2.f), L), d);
-            sum += (double)w;
+            sum[j & 1u] += (double)w;
             rest = fmaf(w, q, rest);
         }
-        sum += (double)rest;
+        sum[0] += (double)rest;
     }
 };
 /* a lane's part of a chunk's sum relative to its largest logit */
@@ -353,25 +354,34 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
                 F.set(E, S);
             }
         }
-        F.sum = 0.0;
+        F.sum[0] = F.sum[1] = 0.0;
 #pragma unroll 1
         for (uint32_t k0 = 0; k0 < CHUNK; k0 += HALF) {
             const int32_t next = i0 + (int32_t)(k0 + HALF);   /* of the next chunk, which lies behind, at last */
             const bool more = k0 + HALF < CHUNK || c + 1u < chunks, inside = more && next >= 0 && next + HALF <= vocab;
             const uint4 *p = reinterpret_cast<const uint4 *>(base + (int64_t)next * (BF16 ? 2 : 4)) + lane;
+            auto take = [&](auto refill) {
 #pragma unroll
-            for (uint32_t k = 0; k < RING; k++) {
-                float x[PER];
-                ring[k].get(x);
-                if (inside) ring[k].v = __ldcs(p + k * 32u);
-                else if (more) ring[k].load(base, next + (int32_t)((k * 32u + lane) * PER), vocab);
+                for (uint32_t k = 0; k < RING; k++) {
+                    float x[PER];
+                    ring[k].get(x);
+                    if constexpr (decltype(refill)::value) ring[k].v = __ldcs(p + k * 32u);
 #pragma unroll
-                for (uint32_t j = 0; j < PER; j += 2u) m = max_nan(m, x[j], x[j + 1u]);
-                F.add(x, table, error);
+                    for (uint32_t j = 0; j < PER; j += 2u) m = max_nan(m, x[j], x[j + 1u]);
+                    F.add(x, table, error);
+                }
+            };
+            if (inside) {
+                take(std::true_type());
+            } else {
+                take(std::false_type());
+                if (more)
+#pragma unroll
+                    for (uint32_t k = 0; k < RING; k++) ring[k].load(base, next + (int32_t)((k * 32u + lane) * PER), vocab);
             }
         }
         const float all = warp_max_nan(m);
-        double s = F.sum;
+        double s = F.sum[0] + F.sum[1];
         int32_t to = __float_as_int(F.step);
         if (finite(all) && (!F.ok || all > F.high || all < F.low)) {
             to = NO_STEP;
@@ -823,7 +833,7 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
     /* a warp's chunks: four, while there are warps for every SM several times over (one session's five drafts: one) */
-    const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 64u * (uint64_t)g_q4.sm_count;
+    const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 40u * (uint64_t)g_q4.sm_count;
     p.span = all >= SPAN * enough ? SPAN : all >= 2u * enough ? 2u : 1u;
     p.spans = (p.chunks + p.span - 1u) / p.span;
     p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
