@@ -42,90 +42,106 @@ struct ForkParams {
 };
 
 /*
- * Fork.  Every block forms the sums over all forks itself, as plan does; then the table entries of whole pages are shared out by threads,
- * the tiles to copy (fork, layer, kv head, 16 rows) by warps.  The last block to finish writes what the others have read: the stack's top
- * and the children's rows.
+ * Fork.  Every block forms the sums over all forks itself, as plan does, and looks up the pages that are copied; then the table entries of whole pages are shared out
+ * by threads, the tiles to copy (fork, layer, kv head, 16 rows) by warps.  The last block to finish writes what the others have read: the
+ * stack's top and the children's rows.
  */
+constexpr uint32_t NOT_SERVED = 0xffffffffu, NO_PAGE = 0xfffffffeu;
 __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P) {
     extern __shared__ uint32_t s_fork[];
-    __shared__ uint64_t s_entries, s_tiles, s_pages;
-    __shared__ uint32_t s_last;
-    uint32_t *owner = s_fork, *entry_end = owner + P.n_req, *tile_end = entry_end + P.n_fork, *page_at = tile_end + P.n_fork;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, mask = (1u << P.page_shift) - 1u;
+    __shared__ uint32_t s_entries, s_tiles, s_pages, s_last;
+    /* of forks: entries and tiles up to and with each; source and place; the page that is copied and the one that it is copied to */
+    uint32_t *owner = s_fork, *entry_end = owner + P.n_req, *tile_end = entry_end + P.n_fork, *places = tile_end + P.n_fork, *old_page = places + P.n_fork, *new_page = old_page + P.n_fork;
+    const uint32_t tid = threadIdx.x, mask = (1u << P.page_shift) - 1u;
     const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
     for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) owner[r] = 0xffffffffu;
     if (tid == 0) s_entries = s_tiles = s_pages = s_last = 0;
     __syncthreads();
     q4d_pdl_wait();
-    const int32_t top = *P.n_free;
-    const uint64_t n_free = top < 0 ? 0u : min((uint32_t)top, P.n_pages);
-    for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS) {   /* a place is the first fork's that names it */
-        const uint32_t d = (uint32_t)__ldcg(P.dst + i);
+    const int32_t top = __ldcg(P.n_free);
+    const uint32_t per = (P.n_fork + PLAN_THREADS - 1u) / PLAN_THREADS, i0 = min(tid * per, P.n_fork), i1 = min(i0 + per, P.n_fork);
+    for (uint32_t i = i0; i < i1; i++) {   /* a place is the first fork's that names it */
+        const uint32_t s = (uint32_t)__ldcg(P.src + i), d = (uint32_t)__ldcg(P.dst + i);
+        places[i] = s < P.n_req && d < P.n_req ? s | d << 16 : NOT_SERVED;   /* up to 8192 of them */
         if (d < P.n_req) atomicMin(owner + d, i);
     }
+    const uint64_t n_free = top < 0 ? 0u : min((uint32_t)top, P.n_pages);
     __syncthreads();
-    const uint32_t per = (P.n_fork + PLAN_THREADS - 1u) / PLAN_THREADS, i0 = min(tid * per, P.n_fork), i1 = min(i0 + per, P.n_fork);
-    auto one = [&](uint32_t i, uint64_t &entries, uint32_t &tiles) -> bool {
-        const uint32_t s = (uint32_t)__ldcg(P.src + i), d = (uint32_t)__ldcg(P.dst + i);
-        const int32_t n = __ldcg(P.len + i);
-        entries = tiles = 0u;
-        if (s >= P.n_req || d >= P.n_req || owner[d] != i || n < 0) return false;
-        const int32_t held = __ldcg(P.rows + s);
-        if (n > max(held, 0) || (uint64_t)max(held, 0) > room || __ldcg(P.rows + d) > 0) return false;
-        entries = (uint32_t)n >> P.page_shift;
-        tiles = (((uint32_t)n & mask) + 15u) >> 4;
-        return true;
-    };
-    uint64_t e_sum = 0, p_sum = 0, t_sum = 0, none = 0, e_all, p_all, t_all, none_all, e;
-    uint32_t t;
     bool any_bad = false;
+    uint64_t e_sum = 0, tp_sum = 0, e_all, tp_all;   /* tp: tiles, and above them pages */
+    auto one = [&](uint32_t i, uint64_t &e, uint64_t &tp) {
+        e = entry_end[i];
+        tp = tile_end[i];
+        if (tp) tp |= 1ull << 32;
+    };
     for (uint32_t i = i0; i < i1; i++) {
-        any_bad |= !one(i, e, t);
-        e_sum += e; t_sum += t; p_sum += t ? 1u : 0u;
+        const uint32_t where = places[i], s = where & 0xffffu, d = where >> 16;
+        bool good = where != NOT_SERVED && owner[d] == i;
+        const int32_t n = good ? __ldcg(P.len + i) : 0, held = good ? __ldcg(P.rows + s) : 0;
+        good = good && n >= 0 && n <= max(held, 0) && (uint64_t)max(held, 0) <= room && __ldcg(P.rows + d) <= 0;
+        any_bad |= !good;
+        places[i] = good ? where : NOT_SERVED;
+        entry_end[i] = good ? (uint32_t)n >> P.page_shift : 0u;
+        tile_end[i] = good ? (((uint32_t)n & mask) + 15u) >> 4 : 0u;
+        uint64_t e, tp;
+        one(i, e, tp);
+        e_sum += e; tp_sum += tp;
     }
-    block_scan2(e_sum, p_sum, e_all, p_all);
-    __syncthreads();
-    block_scan2(t_sum, none, t_all, none_all);
-    uint64_t fit_e = 0, fit_t = 0, fit_p = 0;
+    block_scan2(e_sum, tp_sum, e_all, tp_all);
+    uint64_t fit_e = 0, fit_tp = 0;
+    uint32_t served = i0;        /* behind the thread's last fork that is */
+    bool no_page = false;
     for (uint32_t i = i0; i < i1; i++) {
-        page_at[i] = one(i, e, t) ? (uint32_t)p_sum : 0xffffffffu;   /* 0xffffffff: it cannot be */
-        e_sum += e; t_sum += t; p_sum += t ? 1u : 0u;
-        const bool fits = p_sum <= n_free && e_sum < 0xffffffffu;
-        if (fits) { fit_e = e_sum; fit_t = t_sum; fit_p = p_sum; }
-        entry_end[i] = fits ? (uint32_t)e_sum : 0xffffffffu;   /* 0xffffffff: not served */
-        tile_end[i] = fits ? (uint32_t)t_sum : 0xffffffffu;
+        uint64_t e, tp;
+        one(i, e, tp);
+        const uint32_t before = (uint32_t)(tp_sum >> 32);
+        e_sum += e; tp_sum += tp;
+        const bool fits = (tp_sum >> 32) <= n_free && e_sum < NOT_SERVED;
+        old_page[i] = new_page[i] = NO_PAGE;
+        if (fits && tp) {
+            const uint32_t where = places[i];
+            old_page[i] = (uint32_t)P.table[(size_t)(where & 0xffffu) * P.table_stride + e];   /* behind the whole pages */
+            new_page[i] = (uint32_t)__ldcg(P.free_list + (n_free - 1u - before));
+        }
+        if (fits) { fit_e = e_sum; fit_tp = tp_sum; served = i + 1u; }
+        else places[i] = NOT_SERVED;
+        entry_end[i] = fits ? (uint32_t)e_sum : NOT_SERVED;
+        tile_end[i] = fits ? (uint32_t)tp_sum : NOT_SERVED;
     }
-    if (fit_e) atomicMax((unsigned long long *)&s_entries, (unsigned long long)fit_e);
-    if (fit_t) atomicMax((unsigned long long *)&s_tiles, (unsigned long long)fit_t);
-    if (fit_p) atomicMax((unsigned long long *)&s_pages, (unsigned long long)fit_p);
     __syncthreads();
-    const uint32_t entries = (uint32_t)s_entries, tiles = (uint32_t)s_tiles, pages = (uint32_t)s_pages;
+    if (served > i0 && (served == P.n_fork || entry_end[served] == NOT_SERVED)) {   /* the last one that is served */
+        s_entries = (uint32_t)fit_e;
+        s_tiles = (uint32_t)fit_tp;
+        s_pages = (uint32_t)(fit_tp >> 32);
+    }
+    __syncthreads();
+    const uint32_t entries = s_entries, tiles = s_tiles, pages = s_pages;
     if (blockIdx.x == 0) {
         if (any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-        if (tid == 0 && (p_all > pages || e_all > entries)) atomicOr(P.err, (uint32_t)Q4E_SCRATCH);
+        if (tid == 0 && ((tp_all >> 32) > pages || e_all > entries)) atomicOr(P.err, (uint32_t)Q4E_SCRATCH);
+        for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS)   /* the entry of the page that was copied */
+            if (places[i] != NOT_SERVED && new_page[i] != NO_PAGE) P.table[(size_t)(places[i] >> 16) * P.table_stride + (entry_end[i] - (i ? entry_end[i - 1u] : 0u))] = (int32_t)new_page[i];
     }
-    bool no_page = false;
-    for (uint64_t x = (uint64_t)blockIdx.x * PLAN_THREADS + tid; x < entries; x += (uint64_t)gridDim.x * PLAN_THREADS) {
-        const uint32_t i = first_above(entry_end, P.n_fork, (uint32_t)x), col = (uint32_t)x - (i ? entry_end[i - 1u] : 0u);
-        const int32_t page = P.table[(size_t)__ldcg(P.src + i) * P.table_stride + col];
-        P.table[(size_t)__ldcg(P.dst + i) * P.table_stride + col] = page;
-        if ((uint32_t)page < P.n_pages) atomicAdd(P.shares + page, 1);
-        else no_page = true;
-    }
-    const uint64_t units = (uint64_t)tiles * P.n_layers * P.n_kvh;
-    for (uint64_t u = (uint64_t)blockIdx.x * (PLAN_THREADS / 32u) + (tid >> 5); u < units; u += (uint64_t)gridDim.x * (PLAN_THREADS / 32u)) {
-        const uint64_t lk = u / tiles;
-        const uint32_t x = (uint32_t)(u - lk * tiles), i = first_above(tile_end, P.n_fork, x), tile = x - (i ? tile_end[i - 1u] : 0u);
-        const uint32_t layer = (uint32_t)(lk / P.n_kvh), kh = (uint32_t)(lk - (uint64_t)layer * P.n_kvh), col = (uint32_t)__ldcg(P.len + i) >> P.page_shift;
-        const int32_t old = P.table[(size_t)__ldcg(P.src + i) * P.table_stride + col], page = __ldcg(P.free_list + (n_free - 1u - page_at[i]));
-        if (lk == 0u && tile == 0u && lane == 0u) P.table[(size_t)__ldcg(P.dst + i) * P.table_stride + col] = page;
-        if ((uint32_t)old >= P.n_pages || (uint32_t)page >= P.n_pages) {
+    /* a unit is a tile of all kv heads; of one where there are warps for that (one long prompt's four beams: 2 us less a call) */
+    const uint32_t warps = gridDim.x * (PLAN_THREADS / 32u), at_once = (uint64_t)tiles * P.n_layers * P.n_kvh <= warps ? 1u : P.n_kvh, parts = P.n_kvh / at_once, units = tiles * P.n_layers * parts;
+    const uint64_t page_bytes = (uint64_t)P.n_kvh * P.tiles * P.tile_bytes;
+    for (uint32_t u = blockIdx.x + (tid >> 5) * gridDim.x; u < units; u += warps) {   /* neighbours on different SMs */
+        const uint32_t lk = u / tiles, x = u - lk * tiles, layer = lk / parts, kh0 = lk - layer * parts, i = first_above(tile_end, P.n_fork, x), tile = x - (i ? tile_end[i - 1u] : 0u), from = old_page[i], to = new_page[i];
+        if (from >= P.n_pages || to >= P.n_pages) {
             no_page = true;
             continue;
         }
-        uint8_t *at = P.mem + layer * P.layer_bytes + (uint64_t)(kh * P.tiles + tile) * P.tile_bytes;
-        const uint64_t page_bytes = (uint64_t)P.n_kvh * P.tiles * P.tile_bytes;
-        warp_copy<4>(at + (uint32_t)page * page_bytes, at + (uint32_t)old * page_bytes, P.tile_bytes);
+        uint8_t *at = P.mem + layer * P.layer_bytes + (uint64_t)(kh0 * P.tiles + tile) * P.tile_bytes;
+        const uint8_t *old = at + from * page_bytes;
+        at += to * page_bytes;
+        for (uint32_t k = 0; k < at_once; k++, at += P.tiles * P.tile_bytes, old += P.tiles * P.tile_bytes) warp_copy<9>(at, old, P.tile_bytes);   /* a tile of q8_0 rows of 128 dims at once */
+    }
+    for (uint64_t x = (uint64_t)blockIdx.x * PLAN_THREADS + tid; x < entries; x += (uint64_t)gridDim.x * PLAN_THREADS) {
+        const uint32_t i = first_above(entry_end, P.n_fork, (uint32_t)x), col = (uint32_t)x - (i ? entry_end[i - 1u] : 0u), where = places[i];
+        const int32_t page = P.table[(size_t)(where & 0xffffu) * P.table_stride + col];
+        P.table[(size_t)(where >> 16) * P.table_stride + col] = page;
+        if ((uint32_t)page < P.n_pages) atomicAdd(P.shares + page, 1);
+        else no_page = true;
     }
     if (no_page) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     bool no;
@@ -136,7 +152,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P)
     __syncthreads();
     if (s_last)
         for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS)
-            if (entry_end[i] != 0xffffffffu && page_at[i] != 0xffffffffu) P.rows[__ldcg(P.dst + i)] = __ldcg(P.len + i);
+            if (places[i] != NOT_SERVED) P.rows[places[i] >> 16] = __ldcg(P.len + i);
 }
 
 struct ReleaseParams {
@@ -146,67 +162,92 @@ struct ReleaseParams {
     int32_t *free_list, *n_free, *shares;
     uint32_t *err;
 };
-constexpr uint32_t REL_MAX_BLOCKS = 1024;
-/* between the launches of a call: entries given up, up to and with each request; its rows afterwards; entries of each block with which a page goes back */
-__device__ uint32_t g_rel_end[PLAN_MAX_REQ], g_rel_count[REL_MAX_BLOCKS];
-__device__ int32_t g_rel_rows[PLAN_MAX_REQ];
-__device__ uint32_t g_rel_bad;   /* nothing goes back; zero between calls */
+constexpr uint32_t REL_MAX_BLOCKS = 1024, REL_PROBES = 1u << 22;
+__device__ uint32_t g_rel_count[REL_MAX_BLOCKS];   /* of a call's blocks: pages that go back */
+/* zero between calls: whether nothing goes back, and what has come to the meetings */
+__device__ uint32_t g_rel_bad, g_rel_meet;
 
-/*
- * Release.  The entries that requests give up are numbered in the requests' order.  A page goes back with the last of its entries, if there are
- * as many as it has holders: the first launch counts every page's entries and keeps the largest number, the second counts the pages that go back
- * per block, the third puts them on the stack.  Which entry is a page's last does not depend on the order of the atomics.
- */
-__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_k(const ReleaseParams P) {
-    extern __shared__ uint32_t s_end[];
-    const uint32_t tid = threadIdx.x, mask = (1u << P.page_shift) - 1u;
-    const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
-    q4d_pdl_wait();
-    const uint32_t per = (P.n_req + PLAN_THREADS - 1u) / PLAN_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
-    auto one = [&](uint32_t r, int32_t &after, bool &bad) -> uint32_t {
-        const int32_t h = __ldcg(P.rows + r), k = max(__ldcg(P.keep + r), 0);
-        after = h;
-        bad = h > 0 && (uint64_t)h > room;
-        if (bad || h <= 0 || k >= h) return 0u;
-        if ((uint32_t)k & mask) {   /* its next rows go where others' may be */
-            const int32_t page = P.table[(size_t)r * P.table_stride + ((uint32_t)k >> P.page_shift)];
-            bad = (uint32_t)page < P.n_pages && __ldcg(P.shares + page) > 0;
-            if (bad) return 0u;
+/* all blocks of the launch (at most one per SM, none of which waits for anything before) have come so many times; bounded by 2 s */
+__device__ __forceinline__ void rel_meet(uint32_t times, uint32_t *err) {
+    __syncthreads();
+    if (gridDim.x == 1u) return;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(&g_rel_meet, 1u);
+        unsigned long long t0, t1;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+        for (uint32_t i = 0; i < REL_PROBES; i++) {
+            uint32_t n;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(&g_rel_meet) : "memory");
+            if (n >= times * gridDim.x) break;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+            if (t1 - t0 > 2000000000ull || i == REL_PROBES - 1u) {
+                atomicOr(err, (uint32_t)Q4E_CUDA);
+                atomicOr(&g_rel_bad, 1u);
+                break;
+            }
         }
-        after = k;
-        return (((uint32_t)h + mask) >> P.page_shift) - (((uint32_t)k + mask) >> P.page_shift);
-    };
-    uint64_t sum = 0, all, none = 0, none_all;
-    int32_t after;
-    bool bad, any_bad = false;
-    for (uint32_t r = r0; r < r1; r++) {
-        sum += one(r, after, bad);
-        any_bad |= bad;
-    }
-    block_scan2(sum, none, all, none_all);
-    const bool too_many = all > 0x7fffffffu;
-    for (uint32_t r = r0; r < r1; r++) {
-        sum += one(r, after, bad);
-        s_end[r] = too_many ? 0u : (uint32_t)sum;
-        if (blockIdx.x == 0) {
-            g_rel_end[r] = s_end[r];
-            g_rel_rows[r] = after;
-        }
-    }
-    if (blockIdx.x == 0) {
-        if (any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-        if (too_many && tid == 0) atomicOr(&g_rel_bad, 1u);
+        __threadfence();
     }
     __syncthreads();
-    bool no_page = false;
+}
+
+/*
+ * Release.  The entries that requests give up are numbered in the requests' order, a block has an equal part of them.  A page goes back with the last of its
+ * entries, if there are as many as it has holders: first every page's entries are counted and the largest number kept, then the blocks
+ * count the pages that go back, then they put them on the stack; between these they meet.  Which entry is a page's last does not depend on the
+ * order of the atomics.  (Three launches instead: 14 us for four beams, 21 for 256 answers, as one 9 and 13.)
+ */
+__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleaseParams P) {
+    extern __shared__ uint32_t s_rel[];
+    __shared__ uint32_t s_count, s_before, s_all, s_warp[PLAN_THREADS / 32u], s_last;
+    /* of requests: entries up to and with each, the column of the first, rows afterwards */
+    uint32_t *ends = s_rel, *first = ends + P.n_req;
+    int32_t *rows_after = (int32_t *)(first + P.n_req);
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, mask = (1u << P.page_shift) - 1u;
+    const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
+    if (tid == 0) s_count = s_before = s_all = s_last = 0;
+    q4d_pdl_wait();
+    const int32_t top = __ldcg(P.n_free);
+    const uint32_t per = (P.n_req + PLAN_THREADS - 1u) / PLAN_THREADS, r0 = min(tid * per, P.n_req), r1 = min(r0 + per, P.n_req);
+    uint64_t sum = 0, all_entries, none = 0, none_all;
+    bool any_bad = false;
+    for (uint32_t r = r0; r < r1; r++) {
+        const int32_t h = __ldcg(P.rows + r), k = max(__ldcg(P.keep + r), 0);
+        bool bad = h > 0 && (uint64_t)h > room, gives = !bad && h > 0 && k < h;
+        if (gives && ((uint32_t)k & mask)) {   /* its next rows go where others' may be */
+            const int32_t page = P.table[(size_t)r * P.table_stride + ((uint32_t)k >> P.page_shift)];
+            bad = (uint32_t)page < P.n_pages && __ldcg(P.shares + page) > 0;
+            gives = !bad;
+        }
+        first[r] = ((uint32_t)k + mask) >> P.page_shift;
+        ends[r] = gives ? (((uint32_t)h + mask) >> P.page_shift) - first[r] : 0u;
+        rows_after[r] = gives ? k : h;
+        sum += ends[r];
+        any_bad |= bad;
+    }
+    block_scan2(sum, none, all_entries, none_all);
+    const bool too_many = all_entries > 0x7fffffffu;
+    for (uint32_t r = r0; r < r1; r++) {
+        sum += ends[r];
+        ends[r] = too_many ? 0u : (uint32_t)sum;
+    }
+    if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
+    if (blockIdx.x == 0 && too_many && tid == 0) atomicOr(&g_rel_bad, 1u);
+    __syncthreads();
+    const uint32_t total = too_many ? 0u : (uint32_t)all_entries, share = (total + gridDim.x - 1u) / gridDim.x;
+    const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
     int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
-    const uint32_t total = too_many ? 0u : (uint32_t)all;
-    for (uint64_t x = (uint64_t)blockIdx.x * PLAN_THREADS + tid; x < total; x += (uint64_t)gridDim.x * PLAN_THREADS) {
-        const uint32_t r = first_above(s_end, P.n_req, (uint32_t)x);
-        /* counted from the request's end */
-        const uint32_t pg = (((uint32_t)__ldcg(P.rows + r) + mask) >> P.page_shift) - (s_end[r] - (uint32_t)x);
-        const int32_t page = P.table[(size_t)r * P.table_stride + pg];
-        if ((uint32_t)page < P.n_pages) {
+    auto page_of = [&](uint32_t x) -> uint32_t {
+        const uint32_t r = first_above(ends, P.n_req, x);
+        return (uint32_t)P.table[(size_t)r * P.table_stride + first[r] + (x - (r ? ends[r - 1u] : 0u))];
+    };
+    /* the thread's first entry is looked up once */
+    const uint32_t page0 = x0 + tid < x1 ? page_of((uint32_t)(x0 + tid)) : NO_PAGE;
+    bool no_page = false;
+    for (uint64_t x = x0 + tid; x < x1; x += PLAN_THREADS) {
+        const uint32_t page = x == x0 + tid ? page0 : page_of((uint32_t)x);
+        if (page < P.n_pages) {
             atomicAdd(times + page, 1);
             atomicMax(last + page, (int32_t)x + 1);
         } else {
@@ -214,79 +255,62 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_k(const ReleaseParams
         }
     }
     if (no_page) atomicOr(&g_rel_bad, 1u);
-}
-/* the page of entry x */
-__device__ __forceinline__ int32_t given_page(const ReleaseParams &P, const uint32_t *ends, uint32_t x) {
-    const uint32_t r = first_above(ends, P.n_req, x);
-    const uint32_t pg = (((uint32_t)__ldcg(P.rows + r) + (1u << P.page_shift) - 1u) >> P.page_shift) - (ends[r] - x);
-    return P.table[(size_t)r * P.table_stride + pg];
-}
-__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_count_k(const ReleaseParams P) {
-    extern __shared__ uint32_t s_end[];
-    __shared__ uint32_t s_count;
-    const uint32_t tid = threadIdx.x;
-    if (tid == 0) s_count = 0;
-    q4d_pdl_wait();
-    for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) s_end[r] = __ldcg(g_rel_end + r);
-    __syncthreads();
-    const int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
-    const uint32_t total = s_end[P.n_req - 1u], share = (total + gridDim.x - 1u) / gridDim.x;
-    const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
+    rel_meet(1u, P.err);
+
     uint32_t n = 0;
-    bool bad = false;
+    bool bad = false, mine0 = false;
+    int32_t held0 = 0, given0 = 0;
     for (uint64_t x = x0 + tid; x < x1; x += PLAN_THREADS) {
-        const int32_t page = given_page(P, s_end, (uint32_t)x);
-        if ((uint32_t)page >= P.n_pages || __ldcg(last + page) != (int32_t)x + 1) continue;
+        const bool is0 = x == x0 + tid;
+        const uint32_t page = is0 ? page0 : page_of((uint32_t)x);
+        if (page >= P.n_pages) continue;
         const int32_t held = __ldcg(P.shares + page) + 1, given = __ldcg(times + page);
-        n += given == held;
-        bad |= given > held;
+        const bool mine = __ldcg(last + page) == (int32_t)x + 1;
+        if (is0) { mine0 = mine; held0 = held; given0 = given; }
+        n += mine && given == held;
+        bad |= mine && given > held;
     }
     n = __reduce_add_sync(0xffffffffu, n);
-    if ((tid & 31u) == 0u && n) atomicAdd(&s_count, n);
+    if (lane == 0u && n) atomicAdd(&s_count, n);
     if (bad) atomicOr(&g_rel_bad, 1u);
     __syncthreads();
-    if (tid == 0) g_rel_count[blockIdx.x] = s_count;
-}
-__global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_back_k(const ReleaseParams P) {
-    extern __shared__ uint32_t s_end[];
-    __shared__ uint32_t s_before, s_all, s_warp[PLAN_THREADS / 32u], s_last;
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    if (tid == 0) s_before = s_all = s_last = 0;
-    __syncthreads();
-    q4d_pdl_wait();
-    for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) s_end[r] = __ldcg(g_rel_end + r);
+    if (tid == 0) __stcg(g_rel_count + blockIdx.x, s_count);
+    rel_meet(2u, P.err);
+
     for (uint32_t b = tid; b < gridDim.x; b += PLAN_THREADS) {
-        const uint32_t n = __ldcg(g_rel_count + b);
-        if (n) atomicAdd(&s_all, n);
-        if (n && b < blockIdx.x) atomicAdd(&s_before, n);
+        const uint32_t k = __ldcg(g_rel_count + b);
+        if (k) atomicAdd(&s_all, k);
+        if (k && b < blockIdx.x) atomicAdd(&s_before, k);
     }
-    const int32_t top = *P.n_free;
+    const uint64_t n_free = top < 0 ? 0u : (uint32_t)top;
+    const bool stays = __ldcg(&g_rel_bad) != 0u;
     __syncthreads();
     const uint32_t all = s_all;
-    const uint64_t n_free = top < 0 ? 0u : (uint32_t)top;
-    const bool good = !*(volatile uint32_t *)&g_rel_bad && n_free + all <= P.n_pages;
-    int32_t *times = P.shares + P.n_pages, *last = times + P.n_pages;
-    const uint32_t total = s_end[P.n_req - 1u], share = (total + gridDim.x - 1u) / gridDim.x;
-    const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
+    const bool good = !stays && n_free + all <= P.n_pages;
     uint32_t before = s_before;
     for (uint64_t x = x0; x < x1; x += PLAN_THREADS) {   /* the block stays together */
-        int32_t page = -1;
-        bool mine = false, goes = false;
+        uint32_t page = NO_PAGE;
+        bool goes = false;
         if (x + tid < x1) {
-            page = given_page(P, s_end, (uint32_t)(x + tid));
-            if ((uint32_t)page < P.n_pages) {
+            page = x == x0 ? page0 : page_of((uint32_t)(x + tid));
+            if (page < P.n_pages) {
+                bool mine = mine0;
+                int32_t held = held0, given = given0;
+                if (x != x0) {
+                    mine = __ldcg(last + page) == (int32_t)(x + tid) + 1;
+                    held = __ldcg(P.shares + page) + 1;
+                    given = __ldcg(times + page);
+                }
                 if (!good) {
                     times[page] = last[page] = 0;
-                } else if (__ldcg(last + page) == (int32_t)(x + tid) + 1) {
-                    const int32_t held = __ldcg(P.shares + page) + 1, given = __ldcg(times + page);
-                    mine = true;
+                } else if (mine) {
                     goes = given == held;
                     P.shares[page] = goes ? 0 : held - given - 1;
                     times[page] = last[page] = 0;   /* the others of its entries find that they are not the last, whichever value they read */
                 }
             }
         }
-        const uint32_t votes = __ballot_sync(0xffffffffu, mine && goes);
+        const uint32_t votes = __ballot_sync(0xffffffffu, goes);
         if (lane == 0) s_warp[warp] = __popc(votes);
         __syncthreads();
         uint32_t at = before;
@@ -294,19 +318,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_give_back_k(const ReleaseP
             if (w < warp) at += s_warp[w];
             before += s_warp[w];
         }
-        if (mine && goes) P.free_list[n_free + all - 1u - (at + __popc(votes & ((1u << lane) - 1u)))] = page;
+        if (goes) P.free_list[n_free + all - 1u - (at + __popc(votes & ((1u << lane) - 1u)))] = (int32_t)page;
         __syncthreads();
     }
     bool no;
     if (last_arrives(&g_rel_arrived, !good, no)) {
         if (no) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         else *P.n_free = (int32_t)(n_free + all);
-        g_rel_bad = 0u;
+        g_rel_bad = g_rel_meet = 0u;
         s_last = no ? 0u : 1u;
     }
     __syncthreads();
     if (s_last)
-        for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) P.rows[r] = __ldcg(g_rel_rows + r);
+        for (uint32_t r = tid; r < P.n_req; r += PLAN_THREADS) P.rows[r] = rows_after[r];
 }
 
 struct CompactParams {
@@ -447,6 +471,7 @@ extern "C" bool q4_gpu_pages_fork(const q4_gpu_pages *pg, int32_t *shares, int32
     Q4_REQUIRE(shares && rows && src && dst && len && table && n_req && n_fork && table_stride, "pages_fork: bad argument");
     Q4_REQUIRE(n_req <= PLAN_MAX_REQ && n_fork <= PLAN_MAX_REQ, "pages_fork: at most 8192 requests and forks");
     Q4_REQUIRE((uint64_t)table_stride * pg->page_rows <= 0x7fffffffu, "pages_fork: a block table's rows pass 2^31 - 1");
+    Q4_REQUIRE((uint64_t)n_fork * (pg->page_rows / 16u) * pg->n_layers <= 0x7fffffffu, "pages_fork: too many layers for so many forks");
     ForkParams p = {};
     p.mem = (uint8_t *)pg->mem;
     p.layer_bytes = page_bytes_of(pg) * pg->n_pages;
@@ -458,11 +483,11 @@ extern "C" bool q4_gpu_pages_fork(const q4_gpu_pages *pg, int32_t *shares, int32
     p.free_list = pg->free_list; p.n_free = pg->n_free; p.shares = shares;
     p.err = g_q4.err_d;
     static bool attr = false;
-    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_fork_k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(4u * PLAN_MAX_REQ * sizeof(uint32_t))), "pages_fork smem attribute")) return false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_fork_k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(6u * PLAN_MAX_REQ * sizeof(uint32_t))), "pages_fork smem attribute")) return false;
     attr = true;
     /* a warp per tile to copy, or a thread per entry, up to two blocks per SM */
     const uint64_t tiles = (uint64_t)n_fork * p.tiles * p.n_layers * p.n_kvh, items = tiles * 32u + (uint64_t)n_fork * table_stride, want = (items + PLAN_THREADS - 1u) / PLAN_THREADS, cap = 2u * (uint64_t)g_q4.sm_count;
-    return q4i_launch_pdl("pages_fork launch", q4_pg_fork_k, dim3((unsigned)(want < cap ? want : cap)), PLAN_THREADS, (n_req + 3u * (size_t)n_fork) * sizeof(uint32_t), p);
+    return q4i_launch_pdl("pages_fork launch", q4_pg_fork_k, dim3((unsigned)(want < cap ? want : cap)), PLAN_THREADS, (n_req + 5u * (size_t)n_fork) * sizeof(uint32_t), p);
 }
 
 extern "C" bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table, uint32_t table_stride) {
@@ -478,10 +503,10 @@ extern "C" bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, in
     p.err = g_q4.err_d;
     const dim3 grid(blocks_for((uint64_t)n_req * table_stride));
     if (grid.x > REL_MAX_BLOCKS) return q4i_fail(Q4E_CUDA, "pages_release: more SMs than the counts are for");
-    const size_t smem = n_req * sizeof(uint32_t);
-    return q4i_launch_pdl("pages_release launch", q4_pg_give_k, grid, PLAN_THREADS, smem, p) &&
-           q4i_launch_pdl("pages_release launch", q4_pg_give_count_k, grid, PLAN_THREADS, smem, p) &&
-           q4i_launch_pdl("pages_release launch", q4_pg_give_back_k, grid, PLAN_THREADS, smem, p);
+    static bool attr = false;
+    if (!attr && !q4i_check(cudaFuncSetAttribute(q4_pg_release_k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(3u * PLAN_MAX_REQ * sizeof(uint32_t))), "pages_release smem attribute")) return false;
+    attr = true;
+    return q4i_launch_pdl("pages_release launch", q4_pg_release_k, grid, PLAN_THREADS, 3u * n_req * sizeof(uint32_t), p);
 }
 
 extern "C" bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t *rows, uint32_t n_req, int32_t *table, uint32_t table_stride, int32_t *map) {
