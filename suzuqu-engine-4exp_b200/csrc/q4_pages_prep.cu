@@ -249,8 +249,10 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 template <int KIND, int HD, bool BF16>
 bool prep_launch(PrepParams &p) {
     constexpr uint32_t RPW = 256u / HD;
-    /* warps for every SM, several rounds of them where there is that much */
-    const uint32_t most = 108u * (uint32_t)g_q4.sm_count, want = (most + p.n_tok - 1u) / p.n_tok, q_turns = (p.n_head + RPW - 1u) / RPW, kv_turns = (p.n_kvh + RPW - 1u) / RPW;
+    /* A warp's start (sines, factors) is worth some turns: as many warps as the SMs hold at once, and several rounds of them, the last of which may be part empty,
+     * only where there are many tokens.  us, with 20 warps per SM and with 54: 300 tokens of 24 heads of 256 5.9 and 8.9, 500 of 16 of 128 3.3 and 5.4, 4096 of 24 of
+     * 256 65.9 and 63.1. */
+    const uint32_t most = (p.n_tok < 2048u ? 20u : 54u) * (uint32_t)g_q4.sm_count, want = (most + p.n_tok - 1u) / p.n_tok, q_turns = (p.n_head + RPW - 1u) / RPW, kv_turns = (p.n_kvh + RPW - 1u) / RPW;
     const uint32_t per = (q_turns + kv_turns + want - 1u) / want;
     p.q_per = per < q_turns ? per : q_turns;
     p.kv_per = per < kv_turns ? per : kv_turns;
