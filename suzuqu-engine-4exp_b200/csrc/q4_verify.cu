@@ -22,9 +22,9 @@
 
 namespace {
 
-constexpr uint32_t EACH = 64, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-constexpr uint32_t SPAN = 3;
-constexpr uint32_t STAT_BLOCKS = 5, VF_RING = 4;
+constexpr uint32_t EACH = 32, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
+/* of the first launch: chunks of a warp where there are many, blocks per SM (96 registers: with 72 it is slower), 16-byte pieces on their way to a lane */
+constexpr uint32_t SPAN = 6, STAT_BLOCKS = 5, VF_RING = 4;
 constexpr float LARGEST = 3.402823466e38f;
 
 /* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to a whole step, whose bits as a float at is (NaN:
@@ -398,7 +398,7 @@ __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
 }
 /* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
 struct RowOf {
-    static constexpr uint32_t AT_ONCE = 2;   /* chunks of a lane */
+    static constexpr uint32_t AT_ONCE = 4;   /* chunks of a lane */
     VfStat x[AT_ONCE];
     const VfStat *stat;
     uint32_t chunks;
@@ -832,7 +832,7 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t size = bf16 ? 2u : 4u;
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
-    /* a warp's chunks: four, while there are warps for every SM several times over (one session's five drafts: one) */
+    /* a warp's chunks: as many as leave two rounds of warps for every SM, so that the search for the request and the scale are done once for them (one session's five drafts: one) */
     const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 40u * (uint64_t)g_q4.sm_count;
     p.span = all >= SPAN * enough ? SPAN : all >= 2u * enough ? 2u : 1u;
     p.spans = (p.chunks + p.span - 1u) / p.span;

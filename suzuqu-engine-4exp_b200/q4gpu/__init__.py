@@ -189,11 +189,14 @@ def _dense(t, dtype, n, gpu):
 
 def _rows(t, dtype, n_rows, width, gpu):
     """address and row stride of a tensor [n_rows or more][width or more] of that type on that GPU, whose rows are dense"""
-    apart = t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else width      # a single row has none
-    if t.dtype is not dtype or t.get_device() != gpu or t.dim() != 2 or t.shape[0] < n_rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1) or apart < width:
-        raise RuntimeError("rows of %d numbers of %s on GPU %d are needed, %d of them, not one of %s on %s, %s with strides %s"
-                           % (width, dtype, gpu, n_rows, t.dtype, t.device, tuple(t.shape), t.stride()))
-    return t.data_ptr(), apart
+    if t.dim() == 2:
+        (n, w), (apart, one) = t.shape, t.stride()
+        if n <= 1:                                                         # a single row has no stride
+            apart = width
+        if t.dtype is dtype and t.get_device() == gpu and n >= n_rows and w >= width and (one == 1 or w <= 1) and apart >= width:
+            return t.data_ptr(), apart
+    raise RuntimeError("rows of %d numbers of %s on GPU %d are needed, %d of them, not one of %s on %s, %s with strides %s"
+                       % (width, dtype, gpu, n_rows, t.dtype, t.device, tuple(t.shape), t.stride()))
 
 
 def check(ok, what):
