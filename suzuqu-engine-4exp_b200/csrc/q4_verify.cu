@@ -23,8 +23,8 @@
 namespace {
 
 constexpr uint32_t EACH = 32, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-/* of the first launch: chunks of a warp where there are many, blocks per SM (96 registers: with 72 it is slower), 16-byte pieces on their way to a lane */
-constexpr uint32_t SPAN = 6, STAT_BLOCKS = 5, VF_RING = 4;
+/* of the first launch: chunks of a warp at most, blocks per SM (80 registers: with 64 it is slower), 16-byte pieces on their way to a lane, chunks that are brought to L2 ahead */
+constexpr uint32_t SPAN = 6, STAT_BLOCKS = 6, VF_RING = 4, VF_AHEAD = 2;
 constexpr float LARGEST = 3.402823466e38f;
 
 /* of a chunk: its largest logit m (NaN or +inf: the row is no distribution), the sum of exponentials relative to a whole step, whose bits as a float at is (NaN:
@@ -214,6 +214,20 @@ struct Piece {
     }
 };
 
+/* two floats in a pair of registers */
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ void apart(Two x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two x;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(a), "l"(b), "l"(c));
+    return x;
+}
+
 /* Exponentials for sums, relative to a whole step e of which all that counts lies within 100 powers of two: as VfExp's, but in 32 bits and in two parts.
  * x c comes to whole steps and a rest by a product in two words.  The table's entry is 2^(j / 32) rounded, its error goes into the rest's exponential less 1,
  * q: the value is w + w q, where w is exact and q below 0.0109.  The sums are in 64 bits, but for up to eight w q at a time.  Errors, of the sum: steps 2.25 x 2^-25
@@ -233,21 +247,29 @@ struct VfFast {
         low = (float)(E.m - 0.1 * S.drop);
         high = (float)(E.m + 0.1 * S.drop);
     }
-    /* table: the lane's entry, less its number at the exponent's lowest bits; its error.  By whole warps */
+    /* table: the lane's entry, less its number at the exponent's lowest bits; its error.  By whole warps.  Two logits to an instruction, where there is one for that */
     template <uint32_t N>
     __device__ __forceinline__ void add(const float (&x)[N], uint32_t table, float error) {
         constexpr float L = (float)(LN2 / 32.0);
-        float rest = 0.f;
+        const Two ch = two(c_hi, c_hi), cl = two(c_lo, c_lo), b = two(base, base);
+        Two rest = two(0.f, 0.f);
 #pragma unroll
-        for (uint32_t j = 0; j < N; j++) {
-            const float y = fmaxf(x[j], low), t = fmaf(y, c_hi, base), r = fmaf(y, c_lo, fmaf(y, c_hi, base - t));
-            const uint32_t k = __float_as_uint(t);
-            const float w = __uint_as_float(__shfl_sync(0xffffffffu, table, k) + (k << 18)), d = __shfl_sync(0xffffffffu, error, k);
-            const float q = fmaf(r, fmaf(r, fmaf(r, L * L * L / 6.f, L * L / 2.f), L), d);
-            sum[j & 1u] += (double)w;
-            rest = fmaf(w, q, rest);
+        for (uint32_t j = 0; j < N; j += 2u) {
+            const Two y = two(fmaxf(x[j], low), fmaxf(x[j + 1u], low)), t = fma2(y, ch, b), r = fma2(y, cl, fma2(y, ch, fma2(t, two(-1.f, -1.f), b)));
+            float t0, t1, rest0, rest1;
+            apart(t, t0, t1);
+            const uint32_t k0 = __float_as_uint(t0), k1 = __float_as_uint(t1);
+            const float w0 = __uint_as_float(__shfl_sync(0xffffffffu, table, k0) + (k0 << 18)), w1 = __uint_as_float(__shfl_sync(0xffffffffu, table, k1) + (k1 << 18));
+            const Two d = two(__shfl_sync(0xffffffffu, error, k0), __shfl_sync(0xffffffffu, error, k1));
+            const Two q = fma2(r, fma2(r, fma2(r, two(L * L * L / 6.f, L * L * L / 6.f), two(L * L / 2.f, L * L / 2.f)), two(L, L)), d);
+            rest = fma2(two(w0, w1), q, rest);
+            sum[0] += (double)w0;
+            sum[1] += (double)w1;
+            if (j + 2u == N) {
+                apart(rest, rest0, rest1);
+                sum[0] += (double)(rest0 + rest1);
+            }
         }
-        sum[0] += (double)rest;
     }
 };
 /* a lane's part of a chunk's sum relative to its largest logit */
@@ -304,6 +326,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const VerifyParams P) {
     using V = Piece<BF16>;
     constexpr uint32_t PER = V::PER, RING = V::RING, HALF = RING * 32u * PER;   /* logits of a ring */
+    static_assert(CHUNK % HALF == 0u, "a chunk is whole rings");
     const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.spans, c0 = (unit - row * P.spans) * P.span, c1 = min(c0 + P.span, P.chunks);
     q4d_pdl_wait();
     if (row >= P.rows_all) return;   /* warps behind the last row */
@@ -332,6 +355,15 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
     const double pow = __ldg(g_vf_pow + lane);
     const float near = (float)pow, error = (float)((pow - (double)near) / (double)near);
     const uint32_t table = __float_as_uint(near) - (lane << 18);
+    /* The lines of the chunks behind the next ones to L2: the ring alone keeps too little on its way */
+    constexpr uint32_t AHEAD = VF_AHEAD;
+    auto fetch = [&](int32_t i) {
+        constexpr uint32_t SIZE = BF16 ? 2u : 4u, LINE = 128u / SIZE;
+        i += (int32_t)(lane * LINE);
+        if (lane * LINE < CHUNK && i >= 0 && i < (int32_t)vocab) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + (uint64_t)(uint32_t)i * SIZE));
+    };
+    static_assert(CHUNK * 4u <= 32u * 128u, "a line per lane");
+    for (uint32_t c = 1; c < AHEAD && c < chunks; c++) fetch(i0 + (int32_t)(c * CHUNK));
     VfFast F;
     F.ok = false;
     F.c_hi = F.c_lo = F.base = F.low = F.high = F.step = 0.f;
@@ -355,6 +387,7 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
             }
         }
         F.sum[0] = F.sum[1] = 0.0;
+        if (c + AHEAD < chunks) fetch(i0 + (int32_t)(AHEAD * CHUNK));
 #pragma unroll 1
         for (uint32_t k0 = 0; k0 < CHUNK; k0 += HALF) {
             const int32_t next = i0 + (int32_t)(k0 + HALF);   /* of the next chunk, which lies behind, at last */
@@ -832,9 +865,10 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t size = bf16 ? 2u : 4u;
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
-    /* a warp's chunks: as many as leave two rounds of warps for every SM, so that the search for the request and the scale are done once for them (one session's five drafts: one) */
-    const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, enough = 40u * (uint64_t)g_q4.sm_count;
-    p.span = all >= SPAN * enough ? SPAN : all >= 2u * enough ? 2u : 1u;
+    /* a warp's chunks: as many as leave a round and a half of warps (24 on an SM at once), so that the search for the request and the scale are done once for them: 256 draws
+     * over 32 003 tokens 26.5 us with one, 23.9 with three; 48 x 5 drafts over 131 072 105 with three, 101 with six, 103 with nine */
+    const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, share = all / (36u * (uint64_t)g_q4.sm_count);
+    p.span = share < 1u ? 1u : share < SPAN ? (uint32_t)share : SPAN;
     p.spans = (p.chunks + p.span - 1u) / p.span;
     p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
     p.accepted = accepted; p.next = next; p.logp = logp; p.rows = rows; p.keep = keep;
