@@ -590,14 +590,15 @@ bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t
  *     the draft behind row t is kept while u_accept[t] * q(d) < p(d)         (certain drafts: q(d) = 1, others 0)
  *     next: the first token whose running sum of w exceeds u_next[r] times the whole sum, w = max(p - q, 0) in the row whose draft was
  *     refused (p where that is 0 throughout), w = p in the last row if all are kept
- * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Sums, probabilities and
- * comparisons are in 64 bits.
+ * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Probabilities and comparisons are in 64
+ * bits, a row's sum of exponentials is off by 5e-9 of itself at most.  What row t of draft holds behind a request's last token, and for greedy requests, makes no difference.
  *   accepted, next [n_req]   drafts kept, and the token behind them
  *   logp [n_tok] or NULL     row t's log p of the token that it decided (a kept draft, next), 0 for greedy requests and in rows behind next's
  *   rows, keep [n_req]       or both NULL: keep[r] = rows[r] + accepted[r] + 1, rows[r] being what the request held before the step: for q4_gpu_pages_release
  * A request without tokens: accepted 0, next -1, keep[r] = rows[r].  Logits of minus infinity are tokens that cannot be; a row that is needed and has a NaN, a plus infinity or
  * no token at all, a temperature that is negative or not finite: next -1, status bit 4.  A draft outside the vocabulary is refused, status bit 4.  u in [0, 1).
- * n_req <= 8192.  Scratch (32 bytes per row and 8192 logits) grows outside a capture only. */
+ * n_req <= 8192, n_tok and vocab below 2^30.  Scratch (16 bytes per row and 1024 logits, 64 and 8 per 1024 logits of a request with draft logits) grows outside a capture
+ * only. */
 bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const void *draft, uint64_t draft_ld, uint32_t vocab, const int32_t *token, const int32_t *start,
                    uint32_t n_req, uint32_t n_tok, const float *temp, const float *u_accept, const float *u_next, int32_t *accepted, int32_t *next, float *logp,
                    const int32_t *rows, int32_t *keep);
