@@ -110,8 +110,8 @@ class Case:
         assert self.keep.tolist() == [h + (k + 1 if n else 0) for h, k, n in zip(self.rows.tolist(), accepted, tokens)]
         got = self.logp.cpu().double()
         # rounded to fp32 once.  log p = (x - M) / T - log S: S is off by 5e-9 of itself at most, which is by how much its logarithm is: its terms' exponents by
-        # 2.25 x 2^-25 steps of ln 2 / 32 = 1.5e-9, the last factor of each, e^q - 1 < 0.0109, by 1.5 x 2^-25 of that = 5e-10, up to eight of these added in 32 bits
-        # by 7 x 2^-25 x 0.0109 = 2.3e-9; all else is in 64 bits
+        # 2.25 x 2^-25 steps of ln 2 / 32 = 1.5e-9, the last factor of each, e^q - 1 < 0.0109, by 1.5 x 2^-25 of that = 5e-10 and by its series' fourth term,
+        # q^4 / 24 = 6e-10, up to eight of these added in 32 bits by 7 x 2^-25 x 0.0109 = 2.3e-9; all else is in 64 bits
         assert ((got - logp).abs() <= 2.0**-24 * logp.abs() * (1 + 1e-6) + 5e-9)[: self.live].all()
         assert (got[self.live:] == 5).all()
         return self
@@ -166,6 +166,41 @@ def test_masked_tokens_are_never_drawn(draft):
     start = c.start.tolist()
     for r, (k, n) in enumerate(zip(c.accepted.tolist(), c.next.tolist())):
         assert bool(keep[start[r] + k, n])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("draft", ["logits", "none"])
+def test_tokens_masked_by_the_type_s_lowest_value(bf16, draft):
+    """finite, so that they count where there is nothing else: a row of them alone is flat"""
+    c = Case([2, 0, 3, 1] * 3, 5003, bf16=bf16, draft=draft, seed=20)
+    keep = torch.rand(c.n_tok, c.vocab, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) < 0.02
+    keep[5] = False
+    c.logits.masked_fill_(~keep, torch.finfo(c.logits.dtype).min)
+    c.run().check()
+
+
+@pytest.mark.parametrize("temp", [1e-30, 1e-37, 1e-38, 1e-45])
+def test_temperatures_near_nothing(temp):
+    """the largest logits share everything between them; with a largest of 0 their sizes in steps stay small"""
+    c = Case([1, 0, 2], 5003, temp=[temp] * 3, seed=4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for x in (c.logits, c.draft):
+        x.clamp_(max=-0.01)
+        x[torch.rand(x.shape, device="cuda", generator=g) < 0.01] = 0.0
+    c.run().check()
+
+
+def test_sizes_that_change_along_a_row():
+    """chunks whose logits lie a thousand powers of two and more above or below those before them"""
+    for seed in range(3):
+        c = Case([1, 0, 2], 40000, seed=seed, sharp=1.0, temp=[1.0, 0.05, 20.0])
+        for x in (c.logits, c.draft):
+            x[:, 3000:6000] -= 3000.0
+            x[:, 9000:9100] += 5.0
+            x[:, :1500] -= 900.0
+            x[1, 20000:] += 1500.0
+            x[2, 39999] = 60000.0
+        c.run().check()
 
 
 def test_one_token_left_of_a_row():
