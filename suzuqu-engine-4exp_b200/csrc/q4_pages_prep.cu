@@ -8,7 +8,8 @@
  * The angle is the part of pos * f_i behind the last whole turn.  f_i is kept in turns as a fraction of 2^64, so that the product with
  * the position, modulo 2^64, is that part exactly: an fp32 angle is off by 0.008 at position 262 144, by half a turn at 2^26.
  *
- * Bound by memory: every value is read once and written once.
+ * Bound by memory: every value is read once and written once.  4096 tokens of 24 gated heads of 256 in fp32, 373 MB, take 63 us (90 % of a copy's rate); 16 001 fused
+ * bf16 rows of 32 heads of 128 with 8 kv heads, 394 MB, 78 us (77 %), there beside the issue slots: 63 % busy at the 20 warps that an SM's registers hold.
  */
 #include <math.h>
 #include <string.h>
@@ -17,7 +18,7 @@
 
 namespace {
 
-constexpr uint32_t PREP_THREADS = 32;   /* warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 79 us, in pairs 99, in eights 115) */
+constexpr uint32_t PREP_THREADS = 32;   /* warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115) */
 
 struct PrepParams {
     uint8_t *mem;                /* of the layer */
