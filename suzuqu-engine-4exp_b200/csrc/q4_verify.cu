@@ -16,7 +16,7 @@
  * see every logit, in two parts of 32 bits (VfFast): two additions of 64 bits per logit, and two logits to an instruction in most of the rest.
  *
  * The first launch is bound by its instructions, 18 per logit where the bytes alone are worth 10: 48 requests with 5 drafts over 131 072 tokens,
- * 280 MB, take 101 us in all, 71 in this launch and 43 of memory's; with all of it in 64 bits 206.
+ * 280 MB, take 100 us in all, 71 in this launch and 43 of memory's; with all of it in 64 bits 206.
  */
 #include <math_constants.h>
 #include <type_traits>
@@ -774,11 +774,11 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
 }
 
-/* what p has over q, chunk by chunk; the request's last block to finish looks for next */
+/* what p has over q, chunk by chunk, the next one's logits on their way meanwhile; the request's last block to finish looks for next */
 template <bool BF16>
-__global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams P) {
+__global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const VerifyParams P) {
     __shared__ uint32_t s_last, s_chunk, s_over;
-    __shared__ double s_left, s_part[PICK_WARPS], s_pow[32];
+    __shared__ double s_left, s_part[2][PICK_WARPS], s_pow[32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk0 = blockIdx.x;
     if (tid < 32u) s_pow[tid] = __ldg(g_vf_pow + tid);
     q4d_pdl_wait();
@@ -795,24 +795,33 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_rest_k(const VerifyParams 
     Weights<BF16> W;
     W.set(P, stop, D.m_p, D.m_q, D.scale_p, D.scale_q, S, true, -1);
     double *rest = P.rest + (uint64_t)r * P.chunks;
-    for (uint32_t chunk = chunk0; chunk < P.chunks; chunk += gridDim.x) {
-        const uint32_t i0 = W.begin(chunk) + tid, i1 = W.end(chunk);
-        float xp[PICK_EACH], xq[PICK_EACH];
+    float xp[PICK_EACH], xq[PICK_EACH], xp_next[PICK_EACH], xq_next[PICK_EACH];
+    auto load = [&](uint32_t chunk, float (&p)[PICK_EACH], float (&q)[PICK_EACH]) {
+        const uint32_t i0 = W.begin(chunk) + tid, i1 = chunk < P.chunks ? W.end(chunk) : 0u;
 #pragma unroll
-        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq[k]);
+        for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, p[k], q[k]);
+    };
+    load(chunk0, xp, xq);
+    uint32_t turn = 0;
+    for (uint32_t chunk = chunk0; chunk < P.chunks; chunk += gridDim.x, turn ^= 1u) {
+        load(chunk + gridDim.x, xp_next, xq_next);
         double w[PICK_EACH], x = 0.0;
-        W.of(xp, xq, i0, PICK_THREADS, w);
+        W.of(xp, xq, W.begin(chunk) + tid, PICK_THREADS, w);
 #pragma unroll
         for (uint32_t k = 0; k < PICK_EACH; k++) x += w[k];
         x = warp_sum(x);
-        __syncthreads();         /* the chunk before has been read */
-        if (lane == 0) s_part[warp] = x;
-        __syncthreads();
+        if (lane == 0) s_part[turn][warp] = x;
+        __syncthreads();         /* and the parts of two turns before have been read */
         if (warp == 0) {
-            x = lane < PICK_WARPS ? s_part[lane] : 0.0;
+            x = lane < PICK_WARPS ? s_part[turn][lane] : 0.0;
 #pragma unroll
             for (uint32_t o = PICK_WARPS / 2u; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
             if (lane == 0) __stcg(rest + chunk, x);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < PICK_EACH; k++) {
+            xp[k] = xp_next[k];
+            xq[k] = xq_next[k];
         }
     }
     if (tid == 0) {
