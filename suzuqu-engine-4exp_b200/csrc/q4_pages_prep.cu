@@ -15,8 +15,11 @@
 #include <string.h>
 
 #include "q4_paged.h"
+#include "q4_tc.h"
 
 namespace {
+
+using namespace q4tc;
 
 constexpr uint32_t PREP_THREADS = 32;   /* warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115) */
 
@@ -38,123 +41,271 @@ struct PrepParams {
     q4_gpu_rope rope;
 };
 
-/* eight values of a row, as they lie */
-template <bool BF16>
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+/* eight values of a row, as they lie, the second four of them `apart` bytes behind the first where SPLIT */
+template <bool BF16, bool SPLIT>
 struct Eight {
     uint4 x[BF16 ? 1 : 2];
-    __device__ __forceinline__ void load(const uint8_t *p, bool live) {
+    __device__ __forceinline__ void load(const uint8_t *p, uint32_t apart, bool live) {
+        if constexpr (BF16 && SPLIT) {
+            const uint2 none = make_uint2(0u, 0u), a = live ? __ldcs(reinterpret_cast<const uint2 *>(p)) : none, b = live ? __ldcs(reinterpret_cast<const uint2 *>(p + apart)) : none;
+            x[0] = make_uint4(a.x, a.y, b.x, b.y);
+        } else {
 #pragma unroll
-        for (int i = 0; i < (BF16 ? 1 : 2); i++) x[i] = live ? __ldcs(reinterpret_cast<const uint4 *>(p) + i) : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < (BF16 ? 1 : 2); i++) x[i] = live ? __ldcs(reinterpret_cast<const uint4 *>(p + (i ? SPLIT ? apart : 16u : 0u))) : make_uint4(0u, 0u, 0u, 0u);
+        }
     }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
+    __device__ __forceinline__ void get(uint64_t (&f)[4]) const {   /* two by two */
         const uint32_t *u = reinterpret_cast<const uint32_t *>(x);
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = __uint_as_float(BF16 ? (i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16) : u[BF16 ? 0 : i]);
+        for (int i = 0; i < 4; i++) f[i] = BF16 ? pack2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u)) : pack2(__uint_as_float(u[BF16 ? 0 : 2 * i]), __uint_as_float(u[BF16 ? 0 : 2 * i + 1]));
     }
 };
-__device__ __forceinline__ void eight_floats(const float *p, float (&f)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+__device__ __forceinline__ float4 four_floats(const float *p) { return __ldg(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ float4 four(uint64_t a, uint64_t b) {
+    const float2 x = unpack2(a), y = unpack2(b);
+    return make_float4(x.x, x.y, y.x, y.y);
 }
-__device__ __forceinline__ void store_floats(float *p, const float (&f)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ uint32_t bf16s(uint64_t x) {
+    const float2 f = unpack2(x);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+/* 1 / sqrt(mean x^2 + eps) of a row that LPR lanes hold: 2 units in the last place at most */
+template <uint32_t LPR>
+__device__ __forceinline__ float norm_of(const uint64_t (&x)[4], float eps) {
+    uint64_t s = mul2(x[0], x[0]);
+#pragma unroll
+    for (int i = 1; i < 4; i++) s = fma2(x[i], x[i], s);
+    const float2 two = unpack2(s);
+    float ss = two.x + two.y;
+#pragma unroll
+    for (uint32_t o = LPR / 2u; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return rsqrtf(fmaf(ss, 1.f / (LPR * 8u), eps));
+}
+/* What dims become: r (x fa + y fb), y the pairs' other dims.  Both hold the weights.  on: the twos that are turned; of the others r x fa alone, as the other dim may be infinite */
+template <bool FULL>
+__device__ __forceinline__ void turn(uint64_t (&x)[4], const uint64_t (&y)[4], const uint64_t (&fa)[4], const uint64_t (&fb)[4], uint32_t on, float r) {
+    const uint64_t rr = pack2(r, r);
+    uint64_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint64_t z = mul2(x[i], fa[i]), turned = fma2(y[i], fb[i], z);
+        out[i] = mul2(rr, FULL || (on >> i) & 1u ? turned : z);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = out[i];
 }
 
 /*
  * A warp has a token's queries, or its keys and values, or a part of them where there are few tokens, and keeps what belongs to the token in registers:
  * sines and cosines, with the weights in them.  Lanes hold eight dims of a row each, so that a warp has 1, 2 or 4 rows at a time (hd 256, 128, 64).  The
  * warps' issue slots set the pace beside memory (16 001 rows of a fused bf16 projection 169 us with four dims per lane).  A turn's rows are requested
- * before the one before them is worked at, the first before the token's position is there.
+ * before the one before them is worked at, the first before the token's position is there.  Where pairs lie in two halves a lane has four dims of a query's each and no
+ * other needs them; keys are stored by 16 bytes or quantised by 32 dims, and pass the other dim on between lanes.
  */
 template <int KIND, int HD, bool BF16, bool HALF, bool FULL>
 __global__ void __launch_bounds__(PREP_THREADS) q4_pg_prep_k(const __grid_constant__ PrepParams P) {
     constexpr uint32_t LPR = HD / 8u, RPW = 32u / LPR, U = BF16 ? 2u : 1u, SIZE = BF16 ? 2u : 4u;   /* U: turns at a time, as many bytes on their way in either type */
     const uint32_t lane = threadIdx.x, in = lane % LPR, sub = lane / LPR, unit = blockIdx.x;
     const uint32_t tok = unit / P.units, which = unit - tok * P.units;
-    const bool is_q = which < P.q_units;
-    const uint32_t heads = is_q ? P.n_head : P.n_kvh, per = is_q ? P.q_per : P.kv_per, first = (is_q ? which : which - P.q_units) * per * RPW + sub, behind = min(first - sub + per * RPW, heads);
+    const uint32_t n_rot = P.rope.n_rot, np = n_rot / 2u, quarter = np / 4u;   /* of halves: groups of four dims that have their other ones as many groups behind */
+    /* The warp's lanes take the sines and cosines of the head's pairs, C consecutive ones each, for one another */
+    constexpr uint32_t C = HD / 64u;
+    float cs[C], sn[C];
+    auto angles = [&](int32_t pos) {
+        const uint64_t *turns;             /* as memory: the lanes' addresses differ, which the constant port takes one by one */
+        asm("mov.u64 %0, %1;" : "=l"(turns) : "l"(P.rope.turn));
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++) {
+            const uint64_t angle = (uint64_t)(uint32_t)pos * turns[lane * C + i];
+            sincospif((float)(int32_t)(angle >> 32) * 4.656612873077393e-10f, &sn[i], &cs[i]);   /* 2^-31: half turns */
+            cs[i] *= P.rope.mag;
+            sn[i] *= P.rope.mag;
+        }
+    };
+    auto pair_at = [&](uint32_t pair, uint32_t i, float &c, float &s) {   /* of pair + i, pair a multiple of C; by the whole warp */
+        const uint32_t holder = ((pair + i) / C) & 31u;
+        c = __shfl_sync(0xffffffffu, cs[i % C], holder);
+        s = __shfl_sync(0xffffffffu, sn[i % C], holder);
+    };
+    uint64_t fa[4], fb[4], x[4];
+    uint32_t on = 0;
+    auto interleaved = [&](const float *wn) {
+        float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (wn) {
+            *reinterpret_cast<float4 *>(w) = four_floats(wn + in * 8u);
+            *reinterpret_cast<float4 *>(w + 4) = four_floats(wn + in * 8u + 4u);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            float c, s;
+            pair_at(in * 4u, i, c, s);
+            const bool turns = FULL || in * 4u + i < np;
+            fa[i] = turns ? pack2(w[2 * i] * c, w[2 * i + 1] * c) : pack2(w[2 * i], w[2 * i + 1]);
+            fb[i] = pack2(w[2 * i + 1] * -s, w[2 * i] * s);
+            on |= turns ? 1u << i : 0u;
+        }
+    };
+    auto other_of_two = [&](uint64_t (&y)[4]) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const float2 f = unpack2(x[i]);
+            y[i] = pack2(f.y, f.x);
+        }
+    };
     q4d_pdl_wait();
     const int32_t pos = __ldcg(P.pos + tok);
 
-    /* rows of the group's heads: first, first + RPW .. */
-    const bool two = !is_q || P.gate;      /* a second row: gate or value */
-    const uint32_t step = RPW * HD * (is_q && P.gate ? 2u : 1u) * SIZE;
-    const uint64_t at = (is_q ? tok * P.q_stride : tok * P.kv_stride) + (uint64_t)first * (HD * (is_q && P.gate ? 2u : 1u)) + in * 8u;
-    const uint8_t *pa = (const uint8_t *)(is_q ? P.q : P.k) + at * SIZE, *pb = is_q ? pa + HD * SIZE : (const uint8_t *)P.v + at * SIZE;
-    Eight<BF16> a[U], b[U], a_next[U], b_next[U];
-    auto load = [&](uint32_t head, Eight<BF16> (&x)[U], Eight<BF16> (&y)[U]) {
+    if (which < P.q_units) {
+        const uint32_t first = which * P.q_per * RPW + sub, behind = min(first - sub + P.q_per * RPW, P.n_head);
+        /* the lane's groups of four dims: both sides of its pairs, and those that are not turned as they lie; else next to one another */
+        const uint32_t g0 = HALF && in < quarter ? in : in * 2u, g1 = HALF && in < quarter ? in + quarter : in * 2u + 1u, apart = (g1 - g0) * (4u * SIZE);
+        const uint32_t width = HD * (P.gate ? 2u : 1u), step = RPW * width * SIZE;
+        const uint8_t *pa = (const uint8_t *)P.q + (tok * P.q_stride + (uint64_t)first * width + g0 * 4u) * SIZE, *pb = (const uint8_t *)P.q + (tok * P.q_stride + (uint64_t)first * width + HD + in * 8u) * SIZE;
+        Eight<BF16, HALF> a[U], a_next[U];
+        Eight<BF16, false> b[U], b_next[U];
+        auto load = [&](uint32_t head, Eight<BF16, HALF> (&x)[U], Eight<BF16, false> (&y)[U]) {
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                const bool live = head + u * RPW < behind;
+                x[u].load(pa, apart, live);
+                if (P.gate) y[u].load(pb, 0u, live);
+                pa += step;
+                pb += step;
+            }
+        };
+        load(first, a, b);
+        if (pos < 0) return;
+        angles(pos);
+        const float *wn = P.eps >= 0.f ? P.wq : nullptr;
+        if constexpr (HALF) {
+            float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0;
+            if (wn) {
+                w0 = four_floats(wn + g0 * 4u);
+                w1 = four_floats(wn + g1 * 4u);
+            }
+            const bool turns = FULL || in < quarter;
+            float c[4], s[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++) {
+                pair_at(in * 4u, i, c[i], s[i]);
+                if (!turns) c[i] = 1.f;
+            }
+            fa[0] = pack2(w0.x * c[0], w0.y * c[1]);
+            fa[1] = pack2(w0.z * c[2], w0.w * c[3]);
+            fa[2] = pack2(w1.x * c[0], w1.y * c[1]);
+            fa[3] = pack2(w1.z * c[2], w1.w * c[3]);
+            fb[0] = pack2(w1.x * -s[0], w1.y * -s[1]);
+            fb[1] = pack2(w1.z * -s[2], w1.w * -s[3]);
+            fb[2] = pack2(w0.x * s[0], w0.y * s[1]);
+            fb[3] = pack2(w0.z * s[2], w0.w * s[3]);
+            on = turns ? 0xfu : 0u;
+        } else {
+            interleaved(wn);
+        }
+        for (uint32_t head0 = first; head0 - sub < behind; head0 += RPW * U) {
+            load(head0 + RPW * U, a_next, b_next);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                const uint32_t head = head0 + u * RPW;
+                if (head - sub >= behind) break;
+                a[u].get(x);
+                const float r = P.eps >= 0.f ? norm_of<LPR>(x, P.eps) : 1.f;
+                uint64_t y[4];
+                if constexpr (HALF) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) y[i] = x[i ^ 2u];
+                } else {
+                    other_of_two(y);
+                }
+                turn<FULL>(x, y, fa, fb, on, r);
+                if (head >= behind) continue;
+                const uint64_t to = ((uint64_t)tok * P.n_head + head) * HD;
+                if (P.q_bf16) {
+                    __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(P.q_out) + to + g0 * 4u;
+                    if constexpr (HALF) {
+                        *reinterpret_cast<uint2 *>(out) = make_uint2(bf16s(x[0]), bf16s(x[1]));
+                        *reinterpret_cast<uint2 *>(out + (g1 - g0) * 4u) = make_uint2(bf16s(x[2]), bf16s(x[3]));
+                    } else {
+                        *reinterpret_cast<uint4 *>(out) = make_uint4(bf16s(x[0]), bf16s(x[1]), bf16s(x[2]), bf16s(x[3]));
+                    }
+                } else {
+                    float *out = reinterpret_cast<float *>(P.q_out) + to + g0 * 4u;
+                    *reinterpret_cast<float4 *>(out) = four(x[0], x[1]);
+                    *reinterpret_cast<float4 *>(out + (g1 - g0) * 4u) = four(x[2], x[3]);
+                }
+                if (P.gate) {
+                    b[u].get(x);
+                    float *out = P.gate + to + in * 8u;
+                    *reinterpret_cast<float4 *>(out) = four(x[0], x[1]);
+                    *reinterpret_cast<float4 *>(out + 4) = four(x[2], x[3]);
+                }
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                a[u] = a_next[u];
+                b[u] = b_next[u];
+            }
+        }
+        return;
+    }
+
+    const uint32_t first = (which - P.q_units) * P.kv_per * RPW + sub, behind = min(first - sub + P.kv_per * RPW, P.n_kvh);
+    constexpr uint32_t step = RPW * HD * SIZE;
+    const uint64_t at = (tok * P.kv_stride + (uint64_t)first * HD + in * 8u) * SIZE;
+    const uint8_t *pa = (const uint8_t *)P.k + at, *pb = (const uint8_t *)P.v + at;
+    Eight<BF16, false> a[U], b[U], a_next[U], b_next[U];
+    auto load = [&](uint32_t head, Eight<BF16, false> (&x)[U], Eight<BF16, false> (&y)[U]) {
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
             const bool live = head + u * RPW < behind;
-            x[u].load(pa, live);
-            if (two) y[u].load(pb, live);
+            x[u].load(pa, 0u, live);
+            y[u].load(pb, 0u, live);
             pa += step;
             pb += step;
         }
     };
     load(first, a, b);
-
     if (pos < 0) return;
-    /* The warp's lanes take the sines and cosines of the head's pairs, C consecutive ones each, for one another */
-    const uint32_t n_rot = P.rope.n_rot, np = n_rot / 2u;
-    constexpr uint32_t C = HD / 64u;
-    float cs[C], sn[C];
-    {
-        const uint64_t *turn;              /* as memory: the lanes' addresses differ, which the constant port takes one by one */
-        asm("mov.u64 %0, %1;" : "=l"(turn) : "l"(P.rope.turn));
-#pragma unroll
-        for (uint32_t i = 0; i < C; i++) {
-            const uint64_t angle = (uint64_t)(uint32_t)pos * turn[lane * C + i];
-            sincospif((float)(int32_t)(angle >> 32) * 4.656612873077393e-10f, &sn[i], &cs[i]);   /* 2^-31: half turns */
-            cs[i] *= P.rope.mag;
-            sn[i] *= P.rope.mag;
-        }
-    }
-    /* What a dim is made of: x fa + y fb, y the pair's other dim.  Both hold the weights.  Dims that are not turned: x fa */
-    float fa[8], fb[8];
-    uint32_t on = 0;                       /* dims that are turned */
-    const uint32_t quarter = np / 4u, swap = quarter & 1u;
+    angles(pos);
+    const uint32_t swap = quarter & 1u;
     uint32_t from[2] = {0u, 0u};           /* halves: the lanes where the other dims of the lane's two groups of four lie, in which of its groups is the same for all lanes */
-    {
-        const float *wn = P.eps >= 0.f ? (is_q ? P.wq : P.wk) : nullptr;
-        float w[8];
+    const float *wn = P.eps >= 0.f ? P.wk : nullptr;
+    if constexpr (HALF) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = 1.f;
-        if (wn) eight_floats(wn + in * 8u, w);
-        if constexpr (HALF) {
-#pragma unroll
-            for (uint32_t s = 0; s < 2u; s++) {
-                const uint32_t g = in * 2u + s, other = g < quarter ? g + quarter : g - quarter;
-                const bool turns = FULL || g < 2u * quarter;
-                from[s] = sub * LPR + ((other >> 1) & (LPR - 1u));
-                float v[4] = {1.f, 1.f, 1.f, 1.f};
-                if (wn && turns) *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(wn) + other);
-                const uint32_t pair = (g < quarter ? g : other) * 4u;   /* of the group's first dim */
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) {
-                    const uint32_t k = s * 4u + i, holder = ((pair + i) / C) & 31u;
-                    const float c = __shfl_sync(0xffffffffu, cs[i % C], holder), d = __shfl_sync(0xffffffffu, sn[i % C], holder);
-                    fa[k] = turns ? w[k] * c : w[k];
-                    fb[k] = v[i] * (g < quarter ? -d : d);
-                }
-                on |= turns ? 0xfu << (4u * s) : 0u;
+        for (uint32_t s = 0; s < 2u; s++) {
+            const uint32_t g = in * 2u + s, other = g < quarter ? g + quarter : g - quarter;
+            const bool turns = FULL || g < 2u * quarter;
+            from[s] = sub * LPR + ((other >> 1) & (LPR - 1u));
+            float4 w = make_float4(1.f, 1.f, 1.f, 1.f), v = w;
+            if (wn) {
+                w = four_floats(wn + g * 4u);
+                if (turns) v = four_floats(wn + other * 4u);
             }
-        } else {
+            float c[4], d[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) {
-                const uint32_t pair = in * 4u + i;
-                const float c = __shfl_sync(0xffffffffu, cs[i % C], pair / C), d = __shfl_sync(0xffffffffu, sn[i % C], pair / C);
-                const bool turns = FULL || pair < np;
-                fa[2 * i] = turns ? w[2 * i] * c : w[2 * i];
-                fa[2 * i + 1] = turns ? w[2 * i + 1] * c : w[2 * i + 1];
-                fb[2 * i] = w[2 * i + 1] * -d;
-                fb[2 * i + 1] = w[2 * i] * d;
-                on |= turns ? 3u << (2u * i) : 0u;
+                pair_at((g < quarter ? g : other) * 4u, i, c[i], d[i]);
+                if (!turns) c[i] = 1.f;
+                if (g < quarter) d[i] = -d[i];
             }
+            fa[2 * s] = pack2(w.x * c[0], w.y * c[1]);
+            fa[2 * s + 1] = pack2(w.z * c[2], w.w * c[3]);
+            fb[2 * s] = pack2(v.x * d[0], v.y * d[1]);
+            fb[2 * s + 1] = pack2(v.z * d[2], v.w * d[3]);
+            on |= turns ? 3u << (2u * s) : 0u;
         }
+    } else {
+        interleaved(wn);
     }
-    const int32_t slot = is_q ? -1 : __ldcg(P.slot + tok);
+    const int32_t slot = __ldcg(P.slot + tok);
     const bool keeps = slot >= 0 && (uint32_t)slot < P.slots;
     if (slot >= 0 && !keeps && lane == 0u) atomicOr(P.err, (uint32_t)Q4E_RANGE);
     const uint32_t row = (uint32_t)(keeps ? slot : 0), page = row >> P.page_shift, in_page = row & ((1u << P.page_shift) - 1u), r16 = row & 15u;
@@ -165,75 +316,46 @@ __global__ void __launch_bounds__(PREP_THREADS) q4_pg_prep_k(const __grid_consta
         for (uint32_t u = 0; u < U; u++) {
             const uint32_t head = head0 + u * RPW;
             if (head - sub >= behind) break;
-            const bool live = head < behind;
-            float x[8];
+            const bool live = keeps && head < behind;
             a[u].get(x);
-            float r = 1.f;
-            if (P.eps >= 0.f) {
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-                for (uint32_t o = LPR / 2u; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                r = rsqrtf(fmaf(ss, 1.f / HD, P.eps));   /* 2 units in the last place at most */
-            }
-            float y[8];
+            const float r = P.eps >= 0.f ? norm_of<LPR>(x, P.eps) : 1.f;
+            uint64_t y[4];
             if constexpr (HALF) {
+                float f[8], g[8];
+                *reinterpret_cast<float4 *>(f) = four(x[0], x[1]);
+                *reinterpret_cast<float4 *>(f + 4) = four(x[2], x[3]);
                 if (swap) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) y[i] = __shfl_sync(0xffffffffu, x[i ^ 4u], from[i >> 2]);
+                    for (uint32_t i = 0; i < 8u; i++) g[i] = __shfl_sync(0xffffffffu, f[i ^ 4u], from[i >> 2]);
                 } else {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) y[i] = __shfl_sync(0xffffffffu, x[i], from[i >> 2]);
+                    for (uint32_t i = 0; i < 8u; i++) g[i] = __shfl_sync(0xffffffffu, f[i], from[i >> 2]);
                 }
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) y[i] = pack2(g[2 * i], g[2 * i + 1]);
             } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; i++) y[i] = x[i ^ 1u];
+                other_of_two(y);
             }
+            turn<FULL>(x, y, fa, fb, on, r);
+            uint8_t *tile = P.mem + ((((uint64_t)page * P.n_kvh + head) << (P.page_shift - 4u)) + (in_page >> 4)) * PgTile<KIND, HD>::BYTES;
 #pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) {
-                const float z = x[i] * fa[i];
-                x[i] = r * (FULL || (on >> i) & 1u ? fmaf(y[i], fb[i], z) : z);   /* not turned: the other dim may be infinite */
-            }
-            if (is_q) {
-                if (!live) continue;
-                const uint64_t to = ((uint64_t)tok * P.n_head + head) * HD + in * 8u;
-                if (P.q_bf16) {
-                    __nv_bfloat162 h[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(P.q_out) + to) = *reinterpret_cast<const uint4 *>(h);
-                } else {
-                    store_floats(reinterpret_cast<float *>(P.q_out) + to, x);
-                }
-                if (two) {
-                    b[u].get(x);
-                    store_floats(P.gate + to, x);
-                }
-            } else {
-                uint8_t *tile = P.mem + ((((uint64_t)page * P.n_kvh + head) << (P.page_shift - 4u)) + (in_page >> 4)) * PgTile<KIND, HD>::BYTES;
-#pragma unroll
-                for (uint32_t v = 0; v < 2u; v++) {
-                    if (v) b[u].get(x);
-                    if constexpr (KIND == Q4K_Q8) {   /* four lanes to a block of 32 */
-                        float m = 0.f, d, id;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                        q4d_scale(m, d, id);
-                        if (keeps && live) {
-                            uint8_t *rec = tile + r16 * PgTile<KIND, HD>::ROW;
-                            *reinterpret_cast<uint2 *>(rec + v * HD + in * 8u) = make_uint2(q4d_quant4(make_float4(x[0], x[1], x[2], x[3]), id), q4d_quant4(make_float4(x[4], x[5], x[6], x[7]), id));
-                            if ((in & 3u) == 0u) reinterpret_cast<__half *>(rec + 2u * HD)[v * (HD / 32u) + (in >> 2)] = __float2half_rn(d);
-                        }
-                    } else if (keeps && live) {
-                        __half2 h[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                        uint8_t *dst = tile + v * (PgTile<KIND, HD>::BYTES / 2u) + (in >> 3) * 2048u + r16 * 128u + (((in & 7u) ^ (r16 & 7u)) << 4);
-                        *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(h);
+            for (uint32_t v = 0; v < 2u; v++) {
+                if (v) b[u].get(x);
+                const float4 lo = four(x[0], x[1]), hi = four(x[2], x[3]);
+                if constexpr (KIND == Q4K_Q8) {   /* four lanes to a block of 32 */
+                    float m = fmaxf(fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(lo.z), fabsf(lo.w))), fmaxf(fmaxf(fabsf(hi.x), fabsf(hi.y)), fmaxf(fabsf(hi.z), fabsf(hi.w)))), d, id;
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    q4d_scale(m, d, id);
+                    if (live) {
+                        uint8_t *rec = tile + r16 * PgTile<KIND, HD>::ROW;
+                        *reinterpret_cast<uint2 *>(rec + v * HD + in * 8u) = make_uint2(q4d_quant4(lo, id), q4d_quant4(hi, id));
+                        if ((in & 3u) == 0u) reinterpret_cast<__half *>(rec + 2u * HD)[v * (HD / 32u) + (in >> 2)] = __float2half_rn(d);
                     }
+                } else if (live) {
+                    const __half2 h[4] = {__floats2half2_rn(lo.x, lo.y), __floats2half2_rn(lo.z, lo.w), __floats2half2_rn(hi.x, hi.y), __floats2half2_rn(hi.z, hi.w)};
+                    uint8_t *dst = tile + v * (PgTile<KIND, HD>::BYTES / 2u) + (in >> 3) * 2048u + r16 * 128u + (((in & 7u) ^ (r16 & 7u)) << 4);
+                    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(h);
                 }
             }
         }
