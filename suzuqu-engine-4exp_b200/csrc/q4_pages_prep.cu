@@ -8,8 +8,8 @@
  * The angle is the part of pos * f_i behind the last whole turn.  f_i is kept in turns as a fraction of 2^64, so that the product with
  * the position, modulo 2^64, is that part exactly: an fp32 angle is off by 0.008 at position 262 144, by half a turn at 2^26.
  *
- * Bound by memory: every value is read once and written once.  4096 tokens of 24 gated heads of 256 in fp32, 373 MB, take 63 us (90 % of a copy's rate); 16 001 fused
- * bf16 rows of 32 heads of 128 with 8 kv heads, 394 MB, 78 us (77 %), there beside the issue slots: 63 % busy at the 20 warps that an SM's registers hold.
+ * Bound by memory: every value is read once and written once.  4096 tokens of 24 gated heads of 256 in fp32, 373 MB, take 62 us (92 % of a copy's rate); 16 001 fused
+ * bf16 rows of 32 heads of 128 with 8 kv heads, 394 MB, 75 us (80 %), there beside the issue slots.
  */
 #include <math.h>
 #include <string.h>
@@ -21,7 +21,9 @@ namespace {
 
 using namespace q4tc;
 
-constexpr uint32_t PREP_THREADS = 32;   /* warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115) */
+/* Warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115).  28 of them on an SM, by 72 registers:
+ * 8192 fused rows of 16 heads 31.6 us, 33.5 with up to 96; 32 of them are slower for few tokens (700 tokens of 32 heads 9.2 us, 8.4) */
+constexpr uint32_t PREP_THREADS = 32, PREP_BLOCKS = 28;
 
 struct PrepParams {
     uint8_t *mem;                /* of the layer */
@@ -111,7 +113,7 @@ __device__ __forceinline__ void turn(uint64_t (&x)[4], const uint64_t (&y)[4], c
  * other needs them; keys are stored by 16 bytes or quantised by 32 dims, and pass the other dim on between lanes.
  */
 template <int KIND, int HD, bool BF16, bool HALF, bool FULL>
-__global__ void __launch_bounds__(PREP_THREADS) q4_pg_prep_k(const __grid_constant__ PrepParams P) {
+__global__ void __launch_bounds__(PREP_THREADS, PREP_BLOCKS) q4_pg_prep_k(const __grid_constant__ PrepParams P) {
     constexpr uint32_t LPR = HD / 8u, RPW = 32u / LPR, U = BF16 ? 2u : 1u, SIZE = BF16 ? 2u : 4u;   /* U: turns at a time, as many bytes on their way in either type */
     const uint32_t lane = threadIdx.x, in = lane % LPR, sub = lane / LPR, unit = blockIdx.x;
     const uint32_t tok = unit / P.units, which = unit - tok * P.units;
@@ -372,9 +374,9 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0u; }
 template <int KIND, int HD, bool BF16>
 bool prep_launch(PrepParams &p) {
     constexpr uint32_t RPW = 256u / HD;
-    /* A warp's start (sines, factors) is worth some turns: as many warps as the SMs hold at once, and several rounds of them, the last of which may be part empty,
-     * only where there are many tokens.  us, with 20 warps per SM and with 54: 300 tokens of 24 heads of 256 5.9 and 8.9, 500 of 16 of 128 3.3 and 5.4, 4096 of 24 of
-     * 256 65.9 and 63.1. */
+    /* A warp's start (sines, factors) is worth some turns: no more warps than the SMs hold at once, and several rounds of them, the last of which may be part empty,
+     * only where there are many tokens.  us, with 20 warps per SM and with 54: 300 tokens of 24 heads of 256 6.2 and 8.9, 500 of 16 of 128 3.1 and 5.2, 4096 of 24 of
+     * 256 66.2 and 62.3. */
     const uint32_t most = (p.n_tok < 2048u ? 20u : 54u) * (uint32_t)g_q4.sm_count, want = (most + p.n_tok - 1u) / p.n_tok, q_turns = (p.n_head + RPW - 1u) / RPW, kv_turns = (p.n_kvh + RPW - 1u) / RPW;
     const uint32_t per = (q_turns + kv_turns + want - 1u) / want;
     p.q_per = per < q_turns ? per : q_turns;
