@@ -43,7 +43,9 @@ struct VerifyParams {
     const uint8_t *logits, *draft;
     uint64_t ld, draft_ld;       /* bytes */
     uint32_t vocab, n_req, n_tok;
-    uint32_t chunks, span, spans, rows_all;   /* of a row: chunks, those of a warp, warps; rows: the target's, and the draft's if there are any */
+    uint32_t chunks, span, spans;   /* of a row: chunks, those of a warp, warps */
+    uint32_t levels, across;     /* the order of rows: every levels-th one, then those behind them; levels x across covers n_tok */
+    uint32_t early;              /* rows, in that order, whose drafts are decided on at once; 0: none, and nobody looks */
     const int32_t *token, *start;
     const float *temp, *u_accept, *u_next;
     int32_t *accepted, *next;
@@ -56,6 +58,10 @@ struct VerifyParams {
     uint32_t *err;
 };
 __device__ uint32_t g_vf_arrived[PLAN_MAX_REQ];   /* zero between launches */
+/* of rows with a draft behind them: the warps that have finished, and what became of the draft; zero between calls */
+constexpr uint32_t EARLY_MAX = 1u << 16, EARLY_STOP = 1u << 31, EARLY_NONE = 1u << 30, EARLY_KEPT = 1u << 29;
+__device__ uint32_t g_vf_early[EARLY_MAX];
+__device__ uint32_t g_vf_stop[PLAN_MAX_REQ];      /* of a request: EARLY_MAX less the first row whose draft is not kept; zero: none yet, and between calls */
 __device__ const double g_vf_pow[32] = {          /* 2^(j / 32) */
     1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
     1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
@@ -321,21 +327,54 @@ __device__ __noinline__ void best_in(const uint8_t *base, int32_t i0, uint32_t v
     if (lane == 0) *out = {1.0, all, (int32_t)(i0 + at)};
 }
 
+enum { VF_REFUSED = 0, VF_KEPT = 1, VF_NONE = 2 /* no distribution */, VF_LAST = 3 };
+__device__ __forceinline__ uint32_t said_of(float xp, float xq, float u, const Row &p, const Row &q, bool with_q, const VfScale &S, int2 table);
+template <bool BF16>
+__device__ __noinline__ void decide_early(const VerifyParams &P, uint32_t r, uint32_t t, float T);
+/* a warp has finished with its part of row t; the last of `arrive` of them (0: nobody asks) decides on the draft behind it */
+template <bool BF16>
+__device__ __forceinline__ void row_done(const VerifyParams &P, uint32_t r, uint32_t t, float T, uint32_t arrive) {
+    if (!arrive) return;
+    uint32_t n = 0;
+    if ((threadIdx.x & 31u) == 0u) {   /* who has written its chunks' sums */
+        __threadfence();
+        n = atomicAdd(g_vf_early + t, 1u) + 1u;
+        __threadfence();
+    }
+    if (__shfl_sync(0xffffffffu, n, 0) == arrive) decide_early<BF16>(P, r, t, T);
+}
+
 /*
  * A warp has `span` chunks of a row.  The sums need not be relative to the largest logit but to any within 100 powers of two of it: the largest of the first
  * that the warp sees.  So every logit is taken up once, and its place in the ring is refilled at once from the pieces to come.  Where a
  * chunk's largest logit turns out to lie farther off, it is summed again.
+ *
+ * Rows behind a refused draft are not needed.  EARLY: the last warp of a row decides on the draft behind it, rows are taken in an order in which the requests'
+ * first ones come first (if they bring about as many tokens each), and warps whose row is not needed any more leave.  What such rows leave unwritten is
+ * read, but decides nothing.
  */
-template <bool BF16>
-__global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const VerifyParams P) {
+template <bool BF16, bool EARLY>
+__global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const __grid_constant__ VerifyParams P) {
     using V = Piece<BF16>;
     constexpr uint32_t PER = V::PER, RING = V::RING, HALF = RING * 32u * PER;   /* logits of a ring */
     static_assert(CHUNK % HALF == 0u, "a chunk is whole rings");
-    const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), row = unit / P.spans, c0 = (unit - row * P.spans) * P.span, c1 = min(c0 + P.span, P.chunks);
+    const uint32_t lane = threadIdx.x & 31u, unit = blockIdx.x * VF_WARPS + (threadIdx.x >> 5), turn = unit / P.spans, c0 = (unit - turn * P.spans) * P.span, c1 = min(c0 + P.span, P.chunks);
     q4d_pdl_wait();
-    if (row >= P.rows_all) return;   /* warps behind the last row */
-    const bool drafts = row >= P.n_tok;
-    const uint32_t t = drafts ? row - P.n_tok : row, vocab = P.vocab;
+    bool drafts = false;
+    uint32_t t;
+    bool decides = false;
+    if constexpr (EARLY) {       /* a row and the draft's, one behind the other */
+        const uint32_t nth = P.draft ? turn >> 1 : turn, level = nth / P.across;
+        drafts = P.draft && turn & 1u;
+        t = (nth - level * P.across) * P.levels + level;
+        decides = nth < P.early;
+        if (level >= P.levels || t >= P.n_tok) return;   /* warps behind the last row */
+    } else {
+        if (turn >= P.n_tok * (P.draft ? 2u : 1u)) return;
+        drafts = turn >= P.n_tok;
+        t = drafts ? turn - P.n_tok : turn;
+    }
+    const uint32_t row = drafts ? P.n_tok + t : t, vocab = P.vocab;
     const uint8_t *base = drafts ? P.draft + t * P.draft_ld : P.logits + t * P.ld;
     int32_t i0 = (int32_t)(c0 * CHUNK) - (int32_t)row_begins<BF16>(base);   /* the chunk's first logit */
     V ring[RING];
@@ -343,17 +382,23 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
     for (uint32_t k = 0; k < RING; k++) ring[k].load(base, i0 + (int32_t)((k * 32u + lane) * PER), vocab);
     /* whose row it is, while the logits come */
     float T;
+    uint32_t arrive = 0, r;      /* warps of this row and the draft's, if there is a draft to decide on */
     {
-        const uint32_t r = request_of(P.start, P.n_req, t);
+        r = request_of(P.start, P.n_req, t);
         const int32_t a = __ldcg(P.start + r), b = __ldcg(P.start + r + 1u);
         T = temperature(P, r);
         if ((int32_t)t < a || (int32_t)t >= b || !temperature_ok(T)) return;
         if (drafts && ((int32_t)t + 1 == b || T == 0.f)) return;
+        if (EARLY && a >= 0 && (uint32_t)b <= P.n_tok) {
+            if (decides && (int32_t)t + 1 < b) arrive = P.spans * (P.draft && T != 0.f ? 2u : 1u);
+            if (__ldcg(g_vf_stop + r) > EARLY_MAX - t) return;
+        }
     }
     VfStat *out = P.stat + (uint64_t)row * P.chunks + c0;
     const uint32_t chunks = c1 - c0;
     if (T == 0.f) {
         for (uint32_t c = 0; c < chunks; c++, i0 += CHUNK) best_in<BF16>(base, i0, vocab, out + c);
+        if constexpr (EARLY) row_done<BF16>(P, r, t, T, arrive);
         return;
     }
     const double pow = __ldg(g_vf_pow + lane);
@@ -374,6 +419,8 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
     float ref = -CUDART_INF_F;
     for (uint32_t c = 0; c < chunks; c++, i0 += CHUNK) {
         float m = -CUDART_INF_F;
+        uint32_t word = 0;           /* looked at behind the chunk */
+        if (EARLY) word = __ldcg(g_vf_stop + r);
         if (!finite(ref)) {          /* of what is there: by and large the row's size */
 #pragma unroll
             for (uint32_t k = 0; k < RING; k++) {
@@ -426,7 +473,9 @@ __global__ void __launch_bounds__(VF_THREADS, STAT_BLOCKS) q4_vf_stat_k(const Ve
         }
         s = warp_sum(s);
         if (lane == 0) out[c] = {finite(all) ? s : 0.0, all, to};
+        if (EARLY && word > EARLY_MAX - t) return;
     }
+    if constexpr (EARLY) row_done<BF16>(P, r, t, T, arrive);
 }
 
 __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
@@ -491,6 +540,46 @@ __device__ __forceinline__ bool best_of(const VfStat *stat, uint32_t chunks, int
     const float all = warp_max_nan(m);
     at = __reduce_min_sync(0xffffffffu, m == all ? at : 0x7fffffff);
     return finite(all);
+}
+
+/* whether the draft with logits xp and xq is kept: u q < p, by both sums; by a whole warp */
+__device__ __forceinline__ uint32_t said_of(float xp, float xq, float u, const Row &p, const Row &q, bool with_q, const VfScale &S, int2 table) {
+    VfExp E;
+    const float one_p[1] = {xp}, one_q[1] = {xq};
+    double pd[1] = {0.0}, qd[1] = {1.0}, qs = 1.0;
+    E.set(p.m, S);
+    E.of(one_p, table, pd);
+    if (with_q) {
+        E.set(q.m, S);
+        E.of(one_q, table, qd);
+        qs = q.s;
+    }
+    return (double)u * qd[0] * p.s < pd[0] * qs ? VF_KEPT : VF_REFUSED;
+}
+/* row t and the draft's are done: what becomes of the draft behind t, by a warp */
+template <bool BF16>
+__device__ __noinline__ void decide_early(const VerifyParams &P, uint32_t r, uint32_t t, float T) {
+    const int32_t d = __ldcg(P.token + t + 1u);
+    const bool in = (uint32_t)d < P.vocab, with_q = P.draft != nullptr;
+    const VfStat *stat_p = P.stat + (uint64_t)t * P.chunks;
+    uint32_t said = VF_NONE;
+    if (T == 0.f) {
+        int32_t best;
+        if (best_of(stat_p, P.chunks, best)) said = best == d ? VF_KEPT : VF_REFUSED;
+    } else {
+        float xp = 0.f, xq = 0.f;
+        if (in) xp = logit<BF16>(P.logits + t * P.ld, (uint32_t)d);
+        if (in && with_q) xq = logit<BF16>(P.draft + t * P.draft_ld, (uint32_t)d);
+        const float u = __ldcg(P.u_accept + t);
+        const VfScale S(T);
+        RowOf rows[2];
+        Row p = {}, q = {};
+        rows[0].load(stat_p, P.chunks);
+        rows[1].load(stat_p + (uint64_t)P.n_tok * P.chunks, with_q ? P.chunks : 0u);
+        if (rows[0].get(S, g_vf_pow, p) && (!with_q || rows[1].get(S, g_vf_pow, q))) said = in ? said_of(xp, xq, u, p, q, with_q, S, lane_table()) : (uint32_t)VF_REFUSED;
+    }
+    if ((threadIdx.x & 31u) == 0u && said != VF_KEPT) atomicMax(g_vf_stop + r, EARLY_MAX - t);
+    if ((threadIdx.x & 31u) == 0u) atomicOr(g_vf_early + t, said == VF_KEPT ? EARLY_KEPT : said == VF_NONE ? EARLY_STOP | EARLY_NONE : EARLY_STOP);
 }
 
 /* The place in w_0 w_1 .. w_(n - 1) (of(i, lane's turn): lanes ask for items of their own) at which the running sum passes u times the whole, and what is left for it;
@@ -615,8 +704,6 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
     }
 }
 
-enum { VF_REFUSED = 0, VF_KEPT = 1, VF_NONE = 2 /* no distribution */, VF_LAST = 3 };
-
 template <bool BF16>
 __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams P) {
     __shared__ Row s_p[PICK_WARPS], s_q[PICK_WARPS];
@@ -631,6 +718,9 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     const bool bounds = a >= 0 && b >= a && (uint32_t)b <= P.n_tok;
     if (!bounds || a == b) {
         q4d_pdl_wait();
+        if (P.early && tid == 0) g_vf_stop[r] = 0u;
+        if (P.early)
+            for (int64_t t = (int64_t)max(a, 0) + tid; t < b && t < (int64_t)P.n_tok; t += PICK_THREADS) g_vf_early[t] = 0u;
         if (tid == 0) {
             if (P.draft) P.choice[r].open = 0u;
             P.accepted[r] = 0;
@@ -676,20 +766,13 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
                 } else if (t == last) {
                     mine = VF_LAST;
                 } else if (in) {
-                    VfExp E;
-                    const float one_p[1] = {xp}, one_q[1] = {xq};
-                    double pd[1] = {0.0}, qd[1] = {1.0}, qs = 1.0;
-                    E.set(p.m, S);
-                    E.of(one_p, table, pd);
-                    if (with_q) {
-                        E.set(q.m, S);
-                        E.of(one_q, table, qd);
-                        qs = q.s;
-                    }
-                    mine = (double)u * qd[0] * p.s < pd[0] * qs ? VF_KEPT : VF_REFUSED;   /* u q < p, by both sums */
+                    mine = said_of(xp, xq, u, p, q, with_q, S, table);
                 } else {
                     mine = VF_REFUSED;
                 }
+                /* what the first launch went by, whichever way the sums are rounded here */
+                const uint32_t word = P.early && t < last ? __ldcg(g_vf_early + t) : 0u;
+                if (word & (EARLY_STOP | EARLY_KEPT)) mine = word & EARLY_KEPT ? VF_KEPT : word & EARLY_NONE ? VF_NONE : VF_REFUSED;
             }
             out_of_vocab = t < last && !in;
         }
@@ -725,6 +808,9 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         }
     }
     if (!waited) q4d_pdl_wait();
+    if (P.early && tid == 0) g_vf_stop[r] = 0u;
+    if (P.early)
+        for (uint32_t t = (uint32_t)a + tid; t <= last; t += PICK_THREADS) g_vf_early[t] = 0u;   /* they have been read */
     if (P.logp)
         for (uint32_t t = stop + 1u + tid; t <= last; t += PICK_THREADS) P.logp[t] = 0.f;
     const bool refused = said == VF_REFUSED && !greedy, open = refused && P.draft;
@@ -854,10 +940,11 @@ __global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const VerifyPara
 
 template <bool BF16>
 bool verify_launch(const VerifyParams &p) {
-    const uint64_t warps = (uint64_t)p.rows_all * p.spans, blocks = (warps + VF_WARPS - 1u) / VF_WARPS;
+    const uint64_t warps = (uint64_t)p.levels * p.across * (p.draft ? 2u : 1u) * p.spans, blocks = (warps + VF_WARPS - 1u) / VF_WARPS;
     if (warps > 0x7fffffffu) return q4i_fail(Q4E_ARG, "verify: too many rows for one call");
     const uint32_t rest_blocks = (8u * (uint32_t)g_q4.sm_count + p.n_req - 1u) / p.n_req;   /* of a request; most have nothing to do where few drafts are refused */
-    return q4i_launch_pdl("verify launch", q4_vf_stat_k<BF16>, dim3((unsigned)blocks), VF_THREADS, 0, p) &&
+    return (p.early ? q4i_launch_pdl("verify launch", q4_vf_stat_k<BF16, true>, dim3((unsigned)blocks), VF_THREADS, 0, p)
+                    : q4i_launch_pdl("verify launch", q4_vf_stat_k<BF16, false>, dim3((unsigned)blocks), VF_THREADS, 0, p)) &&
            q4i_launch_pdl("verify launch", q4_vf_pick_k<BF16>, dim3(p.n_req), PICK_THREADS, 0, p) &&
            (!p.draft || q4i_launch_pdl("verify launch", q4_vf_rest_k<BF16>, dim3(rest_blocks < p.chunks ? rest_blocks : p.chunks, p.n_req), PICK_THREADS, 0, p));
 }
@@ -883,7 +970,14 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, share = all / (36u * (uint64_t)g_q4.sm_count);
     p.span = share < 1u ? 1u : share < SPAN ? (uint32_t)share : SPAN;
     p.spans = (p.chunks + p.span - 1u) / p.span;
-    p.n_req = n_req; p.n_tok = n_tok; p.rows_all = n_tok * (draft ? 2u : 1u); p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
+    /* Rows behind refused drafts can be spared where warps come in several rounds; finding out costs a warp a fence and an atomic, and is of no use to the rows of the last two
+     * rounds, which are under way by then.  us, without and with: 256 requests with 8 looked-up drafts, most of them refused, over 50 001 tokens (5.8 rounds) 111 and 60,
+     * 64 with 8 drafts, most of them kept, over 131 072 (7 rounds) 162 and 150, 48 with 5 (3.6 rounds) 99.5 and 101 */
+    const uint64_t warps_of = (uint64_t)p.spans * (draft ? 2u : 1u), at_once = STAT_BLOCKS * VF_WARPS * (uint64_t)g_q4.sm_count;
+    p.early = n_tok > n_req && n_tok <= EARLY_MAX && n_tok * warps_of > 4u * at_once ? n_tok - (uint32_t)(2u * at_once / warps_of) : 0u;
+    p.levels = p.early ? (n_tok + n_req - 1u) / n_req : 1u;
+    p.across = (n_tok + p.levels - 1u) / p.levels;
+    p.n_req = n_req; p.n_tok = n_tok; p.token = token; p.start = start; p.temp = temp; p.u_accept = u_accept; p.u_next = u_next;
     p.accepted = accepted; p.next = next; p.logp = logp; p.rows = rows; p.keep = keep;
     p.err = g_q4.err_d;
     const uint64_t stats = all, rests = draft ? (uint64_t)n_req * p.chunks : 0u, choices = draft ? n_req : 0u;

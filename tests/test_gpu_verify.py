@@ -395,3 +395,68 @@ def test_refusals():
     for bad in (dict(draft=c.draft.double()), dict(draft=c.draft[:, :599]), dict(temp=torch.ones(1, device="cuda")), dict(logp=torch.ones(6))):
         with pytest.raises(RuntimeError):
             c.run(**bad)
+
+
+# ---- so many rows that those behind refused drafts are left out
+@pytest.mark.parametrize("n_req,draft", [(110, "logits"), (200, "none")])
+def test_many_rows(n_req, draft):
+    c = Case([8] * (n_req - 2) + [None, 7], 50001, bf16=True, draft=draft, temp=[1.0, 0.0, 0.7, 1.2], seed=31, idle=3)
+    if draft == "none":                                                     # half of the drafts are likely
+        c.logits.scatter_add_(1, c.token.roll(-1).long()[:, None], 20 * (torch.arange(c.n_tok, device="cuda") % 2).to(c.logits.dtype)[:, None])
+    c.run().check()
+    first = [t.clone() for t in (c.accepted, c.next, c.keep, c.logp)]
+    c.run()
+    assert all(torch.equal(a, b) for a, b in zip(first, (c.accepted, c.next, c.keep, c.logp)))
+
+
+class Many(Case):
+    """a case whose requests can be taken by parts, in which nothing is left out"""
+    def __init__(self, draft):
+        gen = torch.Generator().manual_seed(8)
+        drafts = torch.randint(-1, 9, (5000,), generator=gen).tolist()
+        super().__init__([None if n < 0 else n for n in drafts], 300, draft=draft, temp=[1.0, 0.8, 0.0, 1.0, 0.6, -1.0, 1.1], seed=32, idle=9)
+        kept = torch.rand(self.n_tok, device="cuda") < 0.5
+        self.logits.scatter_add_(1, self.token.roll(-1).long()[:, None], 6 * kept.float()[:, None])
+        self.logits[torch.rand(self.n_tok, device="cuda") < 0.03, 7] = float("nan")
+        self.token[torch.rand(self.n_tok, device="cuda") < 0.03] = 300
+        self.parts = 500
+
+    def by_parts(self):
+        out = [torch.full_like(t, x) for t, x in ((self.accepted, -7), (self.next, -7), (self.keep, -7), (self.logp, 5.0))]
+        for r in range(0, self.n_req, self.parts):
+            n, a, b = self.parts, int(self.start[r]), int(self.start[r + self.parts])
+            q4gpu.verify(self.logits[a:b], self.token[a:b], self.start[r:r + n + 1] - a, self.u_accept[a:b], self.u_next[r:r + n], out[0][r:r + n], out[1][r:r + n],
+                         draft=None if self.draft is None else self.draft[a:b], temp=self.temp[r:r + n], logp=out[3][a:b], rows=self.rows[r:r + n], keep=out[2][r:r + n])
+        return out
+
+    def results(self):
+        return self.accepted, self.next, self.keep, self.logp
+
+
+@pytest.mark.parametrize("draft", ["logits", "none"])
+def test_many_requests_are_their_parts(draft):
+    c = Many(draft)
+    want = c.by_parts()
+    assert lib().q4_gpu_last_error() == 4
+    for _ in range(2):
+        c.logp.fill_(5.0)
+        c.run()
+        assert lib().q4_gpu_last_error() == 4
+        assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
+    # rows behind a first one count: of 5000 requests with 0 to 8 drafts, certain ones kept with 0.3 to 0.4 each, some keep 3 and more (not all 8: 0.35^8 of 500 is 0.1)
+    assert int(c.accepted.max()) >= 3
+
+
+def test_many_rows_with_starts_that_are_none():
+    """they are told, and leave nothing behind for the next call"""
+    c = Many("logits")
+    want = c.by_parts()
+    good = c.start.clone()
+    for at, to in ((17, -5), (18, 2**31 - 1), (400, 0), (2000, c.n_tok + 1), (4990, 3)):
+        c.start[at] = to
+    c.run()
+    assert lib().q4_gpu_last_error() == 4
+    c.start.copy_(good)
+    c.logp.fill_(5.0)
+    c.run()
+    assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
