@@ -460,3 +460,4 @@ def test_many_rows_with_starts_that_are_none():
     c.logp.fill_(5.0)
     c.run()
     assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
+    assert lib().q4_gpu_last_error() == 4                                   # rows that are none, as in the parts
