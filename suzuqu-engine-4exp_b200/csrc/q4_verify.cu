@@ -482,6 +482,11 @@ __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
     const int4 x = __ldcg(reinterpret_cast<const int4 *>(p));
     return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
 }
+__device__ __noinline__ double chunk_any(double c, double e, double m, bool fast, double s, float x_m, int32_t at, const double *pow) {
+    VfExp E;
+    E.c = c; E.e = e; E.m = m; E.fast = fast;
+    return E.chunk({s, x_m, at}, pow);
+}
 /* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
 struct RowOf {
     static constexpr uint32_t AT_ONCE = 4;   /* chunks of a lane */
@@ -518,10 +523,16 @@ struct RowOf {
             for (uint32_t k = 0; k < AT_ONCE; k++) R.s += E.chunk_fast(x[k], pow);
         } else {
 #pragma unroll 1
-            for (uint32_t k = 0; k < AT_ONCE; k++) R.s += E.chunk(x[k], pow);
+            for (uint32_t i = lane; i < min(chunks, 32u * AT_ONCE); i += 32u) {
+                const VfStat y = stat_at(stat + i);
+                R.s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
+            }
         }
 #pragma unroll 1
-        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) R.s += E.chunk(stat_at(stat + i), pow);
+        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) {
+                const VfStat y = stat_at(stat + i);
+                R.s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
+            }
         R.s = warp_sum(R.s);
         return true;
     }
@@ -582,35 +593,76 @@ __device__ __noinline__ void decide_early(const VerifyParams &P, uint32_t r, uin
     if ((threadIdx.x & 31u) == 0u) atomicOr(g_vf_early + t, said == VF_KEPT ? EARLY_KEPT : said == VF_NONE ? EARLY_STOP | EARLY_NONE : EARLY_STOP);
 }
 
-/* The place in w_0 w_1 .. w_(n - 1) (of(i, lane's turn): lanes ask for items of their own) at which the running sum passes u times the whole, and what is left for it;
- * by a whole warp.  A lane sums n / 32 items, then the 32 share out those of the lane in whose sum it lies, and so on.  Where rounding leaves
- * none: the last item with anything in it.  whole: the sum (0: nothing there) */
+/* The chunk of w_0 w_1 .. w_(n - 1) at which the running sum passes u times the whole, and what is left for it; by a whole warp.  A lane sums n / 32 of them (of(i0, i1, w): w_i0
+ * up to w_i1, 0 behind them; N at a time), then all look through those of the lane in whose sum it lies.  Where rounding leaves none: the last one with
+ * anything in it.  whole: the sum (0: nothing there) */
+template <uint32_t N, typename F>
+__device__ __forceinline__ uint32_t place_in(uint32_t n, double u, double &left, double &whole, F of) {
+    const uint32_t lane = threadIdx.x & 31u, step = (n + 31u) / 32u, i0 = min(lane * step, n), i1 = min(i0 + step, n);
+    double w[N], own = 0.0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < step; i += N) {
+        of(min(i0 + i, i1), i1, w);
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) own += w[k];
+    }
+    const double x = warp_scan(own);
+    whole = __shfl_sync(0xffffffffu, x, 31);
+    if (!(whole > 0.0)) return 0u;
+    left = u * whole;
+    const uint32_t above = __ballot_sync(0xffffffffu, x > left && own > 0.0), any = __ballot_sync(0xffffffffu, own > 0.0);
+    const uint32_t l = above ? (uint32_t)__ffs((int)above) - 1u : any ? 31u - (uint32_t)__clz((int)any) : 0u;
+    const double before = __shfl_up_sync(0xffffffffu, x, 1);
+    left = above ? left - __shfl_sync(0xffffffffu, lane ? before : 0.0, (int)l) : CUDART_INF;
+    if (N == 1u) return l;       /* n <= 32 */
+    uint32_t found = 0, last = 0;
+    double sum = 0.0, passed = 0.0;
+    bool there = false;
+#pragma unroll 1
+    for (uint32_t i = 0; i < step; i += N) {
+        if (step > N) of(min(i0 + i, i1), i1, w);
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) {
+            const double v = __shfl_sync(0xffffffffu, w[k], (int)l);
+            if (v > 0.0) last = i + k;
+            if (!there && v > 0.0 && sum + v > left) {
+                there = true;
+                found = i + k;
+                passed = sum;
+            }
+            sum += v;
+        }
+    }
+    left = there ? left - passed : CUDART_INF;
+    return l * step + (there ? found : last);
+}
 template <typename F>
 __device__ __forceinline__ uint32_t place_of(uint32_t n, double u, double &left, double &whole, F of) {
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t lo = 0;
-    bool top = true;
-    left = 0.0;
-    while (top || n > 1u) {
-        const uint32_t step = (n + 31u) / 32u, i0 = min(lane * step, n), i1 = min(i0 + step, n);
-        double own = 0.0;
-#pragma unroll 4
-        for (uint32_t i = i0; i < i1; i++) own += of(lo + i);
-        const double x = warp_scan(own);
-        if (top) {
-            whole = __shfl_sync(0xffffffffu, x, 31);
-            if (!(whole > 0.0)) return 0u;
-            left = u * whole;
-            top = false;
-        }
-        const uint32_t above = __ballot_sync(0xffffffffu, x > left && own > 0.0), any = __ballot_sync(0xffffffffu, own > 0.0);
-        const uint32_t l = above ? (uint32_t)__ffs((int)above) - 1u : any ? 31u - (uint32_t)__clz((int)any) : 0u;
-        const double before = __shfl_up_sync(0xffffffffu, x, 1);
-        left = above ? left - __shfl_sync(0xffffffffu, lane ? before : 0.0, (int)l) : CUDART_INF;
-        n = min(step, n - min(l * step, n));
-        lo += l * step;
+    return n <= 32u ? place_in<1>(n, u, left, whole, of) : place_in<6>(n, u, left, whole, of);
+}
+
+/* N of a row's chunks' sums relative to E; of the one called special: another one */
+template <uint32_t N>
+__device__ __forceinline__ void chunks_of(const VfExp &E, const VfStat *stat, const double *pow, uint32_t special, double other, uint32_t i0, uint32_t i1, double (&w)[N]) {
+    VfStat x[N];
+    bool steps = E.fast;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) {
+        x[k] = {0.0, -CUDART_INF_F, __float_as_int(0.f)};
+        if (i0 + k < i1) x[k] = stat_at(stat + i0 + k);
     }
-    return lo;
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) steps = steps && x[k].at != NO_STEP;
+    if (__all_sync(0xffffffffu, steps)) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) w[k] = E.chunk_fast(x[k], pow);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) w[k] = chunk_any(E.c, E.e, E.m, E.fast, x[k].s, x[k].m, x[k].at, pow);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++)
+        if (i0 + k == special && i0 + k < i1) w[k] = other;
 }
 
 /* a row's tokens by weight: p times its row's sum, without the refused one where drafts are certain, or what p has over q */
@@ -663,9 +715,9 @@ template <bool BF16>
 __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> &W, uint32_t r, uint32_t stop, double sum_p, uint32_t c, double left) {
     __shared__ double s_scan[PICK_WARPS];
     __shared__ int32_t s_some[PICK_WARPS];
-    __shared__ uint32_t s_found;
+    __shared__ unsigned long long s_found;   /* the token, and below it the logit's bits */
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, i0 = W.begin(c) + tid * PICK_EACH, i1 = W.end(c);
-    if (tid == 0) s_found = 0xffffffffu;
+    if (tid == 0) s_found = ~0ull;
     float xp[PICK_EACH], xq[PICK_EACH];
 #pragma unroll
     for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k, i1, xp[k], xq[k]);
@@ -686,21 +738,24 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
     before -= sum;
     for (uint32_t k = 0; k < warp; k++) before += s_scan[k];
     if (before + sum > left && sum > 0.0) {   /* the first token above it; threads behind find later ones */
-        uint32_t found = 0xffffffffu;
+        unsigned long long found = ~0ull;
 #pragma unroll
         for (uint32_t k = 0; k < PICK_EACH; k++) {
             before += w[k];
-            if (before > left && w[k] > 0.0 && found == 0xffffffffu) found = i0 + k;
+            if (before > left && w[k] > 0.0 && found == ~0ull) found = (unsigned long long)(i0 + k) << 32 | __float_as_uint(xp[k]);
         }
-        if (found != 0xffffffffu) atomicMin(&s_found, found);
+        if (found != ~0ull) atomicMin(&s_found, found);
     }
     __syncthreads();
     if (tid == 0) {
-        int32_t found = (int32_t)s_found;
-        if (s_found == 0xffffffffu)   /* rounding, or u not below 1: the last that can be */
+        int32_t found = (int32_t)(s_found >> 32);
+        float x = __uint_as_float((uint32_t)s_found);
+        if (s_found == ~0ull) {  /* rounding, or u not below 1: the last that can be */
             for (uint32_t k = 0; k < PICK_WARPS; k++) found = max(found, s_some[k]);
+            if (found >= 0) x = logit<BF16>(W.row_p, (uint32_t)found);
+        }
         P.next[r] = found;
-        if (P.logp) P.logp[stop] = found >= 0 ? W.p.log_p(logit<BF16>(W.row_p, (uint32_t)found), log_s) : 0.f;
+        if (P.logp) P.logp[stop] = found >= 0 ? W.p.log_p(x, log_s) : 0.f;
     }
 }
 
@@ -850,7 +905,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     if (warp == 0) {
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
         double left, whole;
-        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i) -> double { return i == special ? without : W.p.chunk(stat_at(sp + i), s_pow); });
+        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, special, without, i0, i1, w); });
         if (lane == 0) {
             s_chunk = at;
             s_left = left;
@@ -921,11 +976,14 @@ __global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const VerifyPara
     if (warp == 0) {
         const double u = (double)__ldcg(P.u_next + r);
         double left, whole;
-        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return __ldcg(rest + i); });
+        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) {
+#pragma unroll
+            for (uint32_t k = 0; k < sizeof(w) / sizeof(w[0]); k++) w[k] = i0 + k < i1 ? __ldcg(rest + i0 + k) : 0.0;
+        });
         const bool over_q = whole > 0.0;
         if (!over_q) {           /* p nowhere above q: as if none was refused */
             const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
-            at = place_of(P.chunks, u, left, whole, [&](uint32_t i) -> double { return W.p.chunk(stat_at(sp + i), s_pow); });
+            at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, 0xffffffffu, 0.0, i0, i1, w); });
         }
         if (lane == 0) {
             s_chunk = at;
