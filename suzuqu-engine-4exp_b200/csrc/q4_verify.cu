@@ -503,40 +503,52 @@ struct RowOf {
             if (lane + 32u * k < chunks) x[k] = stat_at(stat + lane + 32u * k);
         }
     }
-    __device__ __forceinline__ bool get(const VfScale &S, const double *pow, Row &R) const {   /* false: no distribution */
-        const uint32_t lane = threadIdx.x & 31u;
+    __device__ __forceinline__ float largest() const {
         float m = -CUDART_INF_F;
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; k++) m = max_nan(m, x[k].m);
 #pragma unroll 1
-        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) m = max_nan(m, __ldcg(&stat[i].m));
-        R.m = m = warp_max_nan(m);
-        R.s = 0.0;
-        if (!finite(m)) return false;
-        VfExp E;
-        E.set(m, S);
+        for (uint32_t i = (threadIdx.x & 31u) + 32u * AT_ONCE; i < chunks; i += 32u) m = max_nan(m, __ldcg(&stat[i].m));
+        return warp_max_nan(m);
+    }
+    __device__ __forceinline__ double own(const VfExp &E, const double *pow) const {   /* the lane's part of S */
+        double s = 0.0;
         bool steps = E.fast;
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; k++) steps = steps && x[k].at != NO_STEP;
-        if (__all_sync(0xffffffffu, steps)) {
+        const bool all = __all_sync(0xffffffffu, steps);
+        if (all) {
 #pragma unroll
-            for (uint32_t k = 0; k < AT_ONCE; k++) R.s += E.chunk_fast(x[k], pow);
-        } else {
-#pragma unroll 1
-            for (uint32_t i = lane; i < min(chunks, 32u * AT_ONCE); i += 32u) {
-                const VfStat y = stat_at(stat + i);
-                R.s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
-            }
+            for (uint32_t k = 0; k < AT_ONCE; k++) s += E.chunk_fast(x[k], pow);
         }
 #pragma unroll 1
-        for (uint32_t i = lane + 32u * AT_ONCE; i < chunks; i += 32u) {
-                const VfStat y = stat_at(stat + i);
-                R.s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
-            }
-        R.s = warp_sum(R.s);
-        return true;
+        for (uint32_t i = (threadIdx.x & 31u) + (all ? 32u * AT_ONCE : 0u); i < chunks; i += 32u) {
+            const VfStat y = stat_at(stat + i);
+            s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
+        }
+        return s;
     }
 };
+/* of p's row, and q's where it has chunks; false: one of them is no distribution */
+__device__ __forceinline__ bool rows_of(const RowOf (&rows)[2], const VfScale &S, const double *pow, Row &p, Row &q) {
+    const bool with_q = rows[1].chunks != 0u;
+    p.m = rows[0].largest();
+    q.m = with_q ? rows[1].largest() : 0.f;
+    p.s = q.s = 0.0;
+    if (!finite(p.m) || !finite(q.m)) return false;
+    VfExp E, F;
+    E.set(p.m, S);
+    F.set(q.m, S);
+    double a = rows[0].own(E, pow), b = with_q ? rows[1].own(F, pow) : 0.0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {   /* side by side */
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    p.s = a;
+    q.s = b;
+    return true;
+}
 /* the first place of a row's largest logit, by a whole warp */
 __device__ __forceinline__ bool best_of(const VfStat *stat, uint32_t chunks, int32_t &at) {
     const uint32_t lane = threadIdx.x & 31u;
@@ -555,17 +567,23 @@ __device__ __forceinline__ bool best_of(const VfStat *stat, uint32_t chunks, int
 
 /* whether the draft with logits xp and xq is kept: u q < p, by both sums; by a whole warp */
 __device__ __forceinline__ uint32_t said_of(float xp, float xq, float u, const Row &p, const Row &q, bool with_q, const VfScale &S, int2 table) {
-    VfExp E;
-    const float one_p[1] = {xp}, one_q[1] = {xq};
-    double pd[1] = {0.0}, qd[1] = {1.0}, qs = 1.0;
+    VfExp E, F;
+    double pd, qd = 1.0, f, g;
     E.set(p.m, S);
-    E.of(one_p, table, pd);
-    if (with_q) {
-        E.set(q.m, S);
-        E.of(one_q, table, qd);
-        qs = q.s;
+    F.set(q.m, S);
+    if (E.fast && F.fast) {      /* side by side */
+        const double y = E.steps(fmaxf(xp, E.low), table, f), z = F.steps(fmaxf(xq, F.low), table, g);
+        pd = xp < E.low ? 0.0 : f * y;
+        if (with_q) qd = xq < F.low ? 0.0 : g * z;
+    } else {
+        const float one_p[1] = {xp}, one_q[1] = {xq};
+        double one[1];
+        E.of(one_p, table, one);
+        pd = one[0];
+        F.of(one_q, table, one);
+        if (with_q) qd = one[0];
     }
-    return (double)u * qd[0] * p.s < pd[0] * qs ? VF_KEPT : VF_REFUSED;
+    return (double)u * qd * p.s < pd * (with_q ? q.s : 1.0) ? VF_KEPT : VF_REFUSED;
 }
 /* row t and the draft's are done: what becomes of the draft behind t, by a warp */
 template <bool BF16>
@@ -587,7 +605,7 @@ __device__ __noinline__ void decide_early(const VerifyParams &P, uint32_t r, uin
         Row p = {}, q = {};
         rows[0].load(stat_p, P.chunks);
         rows[1].load(stat_p + (uint64_t)P.n_tok * P.chunks, with_q ? P.chunks : 0u);
-        if (rows[0].get(S, g_vf_pow, p) && (!with_q || rows[1].get(S, g_vf_pow, q))) said = in ? said_of(xp, xq, u, p, q, with_q, S, lane_table()) : (uint32_t)VF_REFUSED;
+        if (rows_of(rows, S, g_vf_pow, p, q)) said = in ? said_of(xp, xq, u, p, q, with_q, S, lane_table()) : (uint32_t)VF_REFUSED;
     }
     if ((threadIdx.x & 31u) == 0u && said != VF_KEPT) atomicMax(g_vf_stop + r, EARLY_MAX - t);
     if ((threadIdx.x & 31u) == 0u) atomicOr(g_vf_early + t, said == VF_KEPT ? EARLY_KEPT : said == VF_NONE ? EARLY_STOP | EARLY_NONE : EARLY_STOP);
@@ -816,7 +834,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
                 RowOf rows[2];
                 rows[0].load(stat_p + (uint64_t)t * P.chunks, P.chunks);
                 rows[1].load(stat_q + (uint64_t)t * P.chunks, with_q ? P.chunks : 0u);
-                if (!rows[0].get(S, s_pow, p) || (with_q && !rows[1].get(S, s_pow, q))) {
+                if (!rows_of(rows, S, s_pow, p, q)) {
                     mine = VF_NONE;
                 } else if (t == last) {
                     mine = VF_LAST;
