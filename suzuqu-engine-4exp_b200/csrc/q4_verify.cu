@@ -16,7 +16,7 @@
  * see every logit, in two parts of 32 bits (VfFast): two additions of 64 bits per logit, and two logits to an instruction in most of the rest.
  *
  * The first launch is bound by its instructions, 18 per logit where the bytes alone are worth 10: 48 requests with 5 drafts over 131 072 tokens,
- * 280 MB, take 100 us in all, 71 in this launch and 43 of memory's; with all of it in 64 bits 206.
+ * 280 MB, take 97 us in all, 71 in this launch and 43 of memory's; with all of it in 64 bits 206.
  */
 #include <math_constants.h>
 #include <type_traits>
