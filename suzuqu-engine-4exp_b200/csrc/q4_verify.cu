@@ -626,8 +626,8 @@ __device__ __forceinline__ uint32_t place_in(uint32_t n, double u, double &left,
     }
     const double x = warp_scan(own);
     whole = __shfl_sync(0xffffffffu, x, 31);
-    if (!(whole > 0.0)) return 0u;
     left = u * whole;
+    if (!(whole > 0.0)) return 0u;
     const uint32_t above = __ballot_sync(0xffffffffu, x > left && own > 0.0), any = __ballot_sync(0xffffffffu, own > 0.0);
     const uint32_t l = above ? (uint32_t)__ffs((int)above) - 1u : any ? 31u - (uint32_t)__clz((int)any) : 0u;
     const double before = __shfl_up_sync(0xffffffffu, x, 1);

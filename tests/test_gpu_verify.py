@@ -148,6 +148,15 @@ def test_large_vocabulary_and_many_requests():
     Case([0] * 300, 32003, False, seed=4, temp=[0.9, 0.0, 0.5]).run().check()
 
 
+@pytest.mark.parametrize("vocab", [32768 - 3, 32768 + 1, 6 * 32768 + 1, 600001])
+@pytest.mark.parametrize("draft", ["logits", "none"])
+def test_vocabularies_around_a_lane_s_share_of_chunks(vocab, draft):
+    c = Case([2, 0, 1, 3], vocab, draft=draft, temp=[1.0, 3.0, 0.8, 0.0], seed=vocab, sharp=1.5)
+    for u in (0.0, 0.3, 0.9999):
+        c.u_next.fill_(u)
+        c.run().check()
+
+
 @pytest.mark.parametrize("sharp", [0.0, 0.01, 30.0])
 def test_flat_and_sharp(sharp):
     for seed in range(4):
