@@ -44,7 +44,7 @@ struct ForkParams {
 /*
  * Fork.  Every block forms the sums over all forks itself, as plan does, and looks up the pages that are copied; then the table entries of whole pages are shared out
  * by threads, the tiles to copy (fork, layer, kv head, 16 rows) by warps.  The last block to finish writes what the others have read: the
- * stack's top and the children's rows.  256 forks with 104 MB to copy, most of it out of and into L2, 24 us; four of one prompt 6: sums, look-ups that follow
+ * stack's top and the children's rows.  256 forks with 104 MB to copy, most of it out of and into L2, 25 us; four of one prompt 6: sums, look-ups that follow
  * one another and a fence, where the bytes are worth nothing.
  */
 constexpr uint32_t NOT_SERVED = 0xffffffffu, NO_PAGE = 0xfffffffeu;
