@@ -539,7 +539,7 @@ typedef struct q4_gpu_rope {
  *   0  as they are                                                  (factor, orig, fast, slow: ignored)
  *   1  linear   f_i / factor
  *   2  ramp     f_i (1 - s) + f_i / factor s, s rising from 0 to 1 over the pairs, from the one that turns `fast` times in orig positions (rounded
- *               down) to the one that turns `slow` times (rounded up)
+ *               down, 0 at least) to the one that turns `slow` times (rounded up, n_rot - 1 at most: it may lie behind the last pair)
  *   3  smooth   the same with s = 1 - (turns in orig positions - slow) / (fast - slow), between 0 and 1
  * n_rot even, up to 256 (0: no rotation), a multiple of 8 for half; base above 1 (scaling 2 and 3) or 0; factor, orig, mag above 0, fast above
  * slow above 0. */

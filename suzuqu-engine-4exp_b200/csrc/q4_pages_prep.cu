@@ -408,7 +408,8 @@ extern "C" bool q4_gpu_rope_set(q4_gpu_rope *r, uint32_t n_rot, int half, double
     const uint32_t np = n_rot / 2u;
     /* the pair that turns so many times in orig positions */
     auto pair_of = [&](double turns) { return np * log(orig / (turns * two_pi)) / log(base); };
-    const double lo = scaling == 2 ? fmax(0.0, floor(pair_of(fast))) : 0.0, hi = scaling == 2 ? fmin((double)np - 1.0, ceil(pair_of(slow))) : 0.0;
+    /* the slow end may lie behind the last pair, which then is not slowed down fully */
+    const double lo = scaling == 2 ? fmax(0.0, floor(pair_of(fast))) : 0.0, hi = scaling == 2 ? fmin((double)n_rot - 1.0, ceil(pair_of(slow))) : 0.0;
     for (uint32_t i = 0; i < np; i++) {
         double f = pow(base, -2.0 * i / n_rot);
         double s = 0.0;   /* how far it is slowed down */

@@ -66,3 +66,23 @@ def test_refusals(args):
     with pytest.raises(RuntimeError):
         q4gpu.Rope(**args)
     q4gpu.load().q4_gpu_last_error()
+
+
+def ramp(n_rot, base, factor, orig, fast, slow):
+    """radians per position by the definition of the ramp: it ends at the pair that turns `slow` times, which may lie behind the last one; no later than at n_rot - 1"""
+    def pair(turns):                                       # base^(-2 i / n_rot) * orig = 2 pi turns
+        return n_rot * (math.log(orig) - math.log(2 * math.pi * turns)) / (2 * math.log(base))
+    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), n_rot - 1)
+    f = [base ** (-2 * i / n_rot) for i in range(n_rot // 2)]
+    return [x * (1 - s) + x / factor * s for x, s in zip(f, (min(max((i - lo) / (hi - lo), 0.0), 1.0) for i in range(n_rot // 2)))]
+
+
+@pytest.mark.parametrize("n_rot,base,factor,orig,hi", [(128, 1e4, 4.0, 131072, 70), (64, 1e4, 8.0, 65536, 33), (128, 1e4, 4.0, 65536, 65), (64, 1e4, 4.0, 131072, 35), (64, 1e4, 4.0, 32768, 30),
+                                                       (32, 100.0, 2.0, 200000, 31)])
+def test_a_ramp_whose_slow_end_lies_behind_the_last_pair(n_rot, base, factor, orig, hi):
+    """hi: the slow end, worked out by hand; the bounds are those of test_turns"""
+    assert min(math.ceil(n_rot / 2 * math.log(orig / (2 * math.pi)) / math.log(base)), n_rot - 1) == hi
+    r = q4gpu.Rope(n_rot, base, scaling="ramp", factor=factor, orig=orig, fast=32.0, slow=1.0)
+    for i, f in enumerate(ramp(n_rot, base, factor, orig, 32.0, 1.0)):
+        off = (Fraction(r.turn[i], 2**64) - Fraction(f) / TWO_PI) % 1
+        assert min(off, 1 - off) <= Fraction(f) / 2**49 + Fraction(1, 2**52), i
