@@ -803,6 +803,7 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         }
         return;
     }
+    __syncthreads();             /* s_pow: all warps read what the first has put there */
     const bool greedy = T == 0.f;
     const VfStat *stat_p = P.stat, *stat_q = P.stat + (uint64_t)P.n_tok * P.chunks;
     const uint32_t last = (uint32_t)b - 1u;

@@ -470,3 +470,22 @@ def test_many_rows_with_starts_that_are_none():
     c.run()
     assert all(torch.equal(a, b) for a, b in zip(c.results(), want))
     assert lib().q4_gpu_last_error() == 4                                   # rows that are none, as in the parts
+
+
+# ---- what blocks share
+@pytest.mark.parametrize("draft", ["logits", "none"])
+def test_what_other_kernels_left_in_shared_memory(draft):
+    """a launch over 8192 requests that hold nothing leaves zeros on every SM: the decision's table is not read before it is there"""
+    n = 8192
+    pool = q4gpu.PagePool(1, 1, 64, 64, 16)
+    rows, keep = torch.zeros(2, n, dtype=torch.int32, device="cuda").unbind(0)
+    table = torch.zeros(n, 20, dtype=torch.int32, device="cuda")
+    c = Case([7, 3, 5, 9] * 60, 300, draft=draft, seed=33, sharp=0.7)
+    if draft == "none":
+        c.logits[torch.arange(c.n_tok - 1), c.token[1:].long()] += 8.0
+    c.run().check()
+    want = [t.clone() for t in (c.accepted, c.next, c.keep, c.logp)]
+    for _ in range(30):
+        pool.release(rows, keep, table)
+        c.run()
+        assert all(torch.equal(a, b) for a, b in zip((c.accepted, c.next, c.keep, c.logp), want))
