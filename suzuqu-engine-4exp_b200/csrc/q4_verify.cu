@@ -341,7 +341,9 @@ __device__ __forceinline__ void row_done(const VerifyParams &P, uint32_t r, uint
         n = atomicAdd(g_vf_early + t, 1u) + 1u;
         __threadfence();
     }
-    if (__shfl_sync(0xffffffffu, n, 0) == arrive) decide_early<BF16>(P, r, t, T);
+    if (__shfl_sync(0xffffffffu, n, 0) != arrive) return;
+    __syncwarp();                /* a shuffle orders no memory: what the lanes read from here on lies behind the first one's fence */
+    decide_early<BF16>(P, r, t, T);
 }
 
 /*
