@@ -572,7 +572,7 @@ bool q4_gpu_pages_fork(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, u
  * (where keep is less).  A page goes back on the stack with its last holder, in the order of those, and otherwise has a holder less.  A request that
  * would keep only a part of the rows of a page that others hold too is left as it is, status bit 4 (its next rows would overwrite theirs): fork it at
  * that length and release it.  More pages than are out, a page given back by more than hold it, or an entry that is no page of the pool: nothing goes back, rows
- * stay, status bit 4.  Table entries stay as they are.  n_req <= 8192. */
+ * stay, status bit 4; the same with bit 2 too where the launch's blocks do not meet within 2 s.  Table entries stay as they are.  n_req <= 8192. */
 bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows, const int32_t *keep, uint32_t n_req, const int32_t *table,
                           uint32_t table_stride);
 /* Moves the pages in use (those not on the stack) to the low end of the pool, in all layers: page i of those that lie behind it, in ascending

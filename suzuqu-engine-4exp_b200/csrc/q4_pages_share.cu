@@ -164,33 +164,41 @@ struct ReleaseParams {
     uint32_t *err;
 };
 constexpr uint32_t REL_MAX_BLOCKS = 1024, REL_PROBES = 1u << 22;
+static_assert(REL_MAX_BLOCKS * 2u < MEET_BAD, "arrivals stay below the flags");
 __device__ uint32_t g_rel_count[REL_MAX_BLOCKS];   /* of a call's blocks: pages that go back */
-/* zero between calls: whether nothing goes back, and what has come to the meetings */
-__device__ uint32_t g_rel_bad, g_rel_meet;
+__device__ uint32_t g_rel_meet;                    /* where they meet; zero between calls */
 
-/* all blocks of the launch (at most one per SM, none of which waits for anything before) have come so many times; bounded by 2 s */
-__device__ __forceinline__ void rel_meet(uint32_t times, uint32_t *err) {
-    __syncthreads();
-    if (gridDim.x == 1u) return;
+/* All blocks of the launch (at most one per SM, none of which waits for anything before) have come so many times; bounded by 2 s.  What they go by: the word, with bad said by any
+ * thread.  The same for all of a block's threads, and behind the second meeting meet_good is the same for all blocks */
+__device__ __forceinline__ uint32_t rel_meet(uint32_t times, bool bad, uint32_t *err) {
+    __shared__ uint32_t s_word;
+    const bool any = __syncthreads_or(bad);
+    if (gridDim.x == 1u) return times * MEET_HERE | (any ? MEET_BAD : 0u);
     if (threadIdx.x == 0) {
         __threadfence();
-        atomicAdd(&g_rel_meet, 1u);
+        if (any) atomicOr(&g_rel_meet, MEET_BAD);
+        atomicAdd(&g_rel_meet, MEET_HERE);
+        uint32_t word = 0;
         unsigned long long t0, t1;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-        for (uint32_t i = 0; i < REL_PROBES; i++) {
-            uint32_t n;
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(&g_rel_meet) : "memory");
-            if (n >= times * gridDim.x) break;
+        const bool over = pg_within(REL_PROBES, [&]() {
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(word) : "l"(&g_rel_meet) : "memory");
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-            if (t1 - t0 > 2000000000ull || i == REL_PROBES - 1u) {
-                atomicOr(err, (uint32_t)Q4E_CUDA);
-                atomicOr(&g_rel_bad, 1u);
-                break;
-            }
-        }
+            return meet_over(word, gridDim.x, times) || t1 - t0 > 2000000000ull;
+        });
+        if (!over || !meet_over(word, gridDim.x, times))
+            pg_within(4u * REL_MAX_BLOCKS, [&]() {   /* whoever is in between has come, found something bad or given up: three times a block at most */
+                const uint32_t late = meet_given_up(word, gridDim.x, times), seen = late == word ? word : atomicCAS(&g_rel_meet, word, late);
+                const bool done = seen == word;
+                if (done && late != word) atomicOr(err, (uint32_t)Q4E_CUDA);
+                word = done ? late : seen;
+                return done || (word & MEET_LATE);
+            });
         __threadfence();
+        s_word = word;
     }
     __syncthreads();
+    return s_word;
 }
 
 /*
@@ -234,7 +242,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleasePar
         ends[r] = too_many ? 0u : (uint32_t)sum;
     }
     if (blockIdx.x == 0 && any_bad) atomicOr(P.err, (uint32_t)Q4E_RANGE);
-    if (blockIdx.x == 0 && too_many && tid == 0) atomicOr(&g_rel_bad, 1u);
     __syncthreads();
     const uint32_t total = too_many ? 0u : (uint32_t)all_entries, share = (total + gridDim.x - 1u) / gridDim.x;
     const uint64_t x0 = (uint64_t)blockIdx.x * share, x1 = min(x0 + share, (uint64_t)total);
@@ -245,21 +252,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleasePar
     };
     /* the thread's first entry is looked up once */
     const uint32_t page0 = x0 + tid < x1 ? page_of((uint32_t)(x0 + tid)) : NO_PAGE;
-    bool no_page = false;
+    bool bad = too_many;
     for (uint64_t x = x0 + tid; x < x1; x += PLAN_THREADS) {
         const uint32_t page = x == x0 + tid ? page0 : page_of((uint32_t)x);
         if (page < P.n_pages) {
             atomicAdd(times + page, 1);
             atomicMax(last + page, (int32_t)x + 1);
         } else {
-            no_page = true;
+            bad = true;          /* an entry that is no page */
         }
     }
-    if (no_page) atomicOr(&g_rel_bad, 1u);
-    rel_meet(1u, P.err);
+    rel_meet(1u, bad, P.err);
 
     uint32_t n = 0;
-    bool bad = false, mine0 = false;
+    bool mine0 = false;
     int32_t held0 = 0, given0 = 0;
     for (uint64_t x = x0 + tid; x < x1; x += PLAN_THREADS) {
         const bool is0 = x == x0 + tid;
@@ -273,10 +279,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleasePar
     }
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0u && n) atomicAdd(&s_count, n);
-    if (bad) atomicOr(&g_rel_bad, 1u);
     __syncthreads();
     if (tid == 0) __stcg(g_rel_count + blockIdx.x, s_count);
-    rel_meet(2u, P.err);
+    const bool stays = !meet_good(rel_meet(2u, bad, P.err), gridDim.x);
 
     for (uint32_t b = tid; b < gridDim.x; b += PLAN_THREADS) {
         const uint32_t k = __ldcg(g_rel_count + b);
@@ -284,7 +289,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleasePar
         if (k && b < blockIdx.x) atomicAdd(&s_before, k);
     }
     const uint64_t n_free = top < 0 ? 0u : (uint32_t)top;
-    const bool stays = __ldcg(&g_rel_bad) != 0u;
     __syncthreads();
     const uint32_t all = s_all;
     const bool good = !stays && n_free + all <= P.n_pages;
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleasePar
     if (last_arrives(&g_rel_arrived, !good, no)) {
         if (no) atomicOr(P.err, (uint32_t)Q4E_RANGE);
         else *P.n_free = (int32_t)(n_free + all);
-        g_rel_bad = g_rel_meet = 0u;
+        g_rel_meet = 0u;
         s_last = no ? 0u : 1u;
     }
     __syncthreads();
