@@ -110,7 +110,7 @@ struct VfScale {
  * and a logit 1000 powers of two below M is still a number.  Else relative to M, by the library's function. */
 struct VfExp {
     double c, e, m;              /* e: 0 where not fast */
-    float low;                   /* what is below is nothing (2^-1000) */
+    float low;                   /* what is below is nothing (2^-1000), token or chunk: a chunk that counts has a token that does */
     bool fast;
     __device__ __forceinline__ void set(float largest, const VfScale &S) {
         m = largest;
@@ -143,21 +143,22 @@ struct VfExp {
             }
         } else {
 #pragma unroll
-            for (uint32_t k = 0; k < N; k++) w[k] = slow(x[k]);
+            for (uint32_t k = 0; k < N; k++) w[k] = x[k] < low ? 0.0 : slow(x[k]);
         }
     }
-    /* a chunk's sum as one relative to this, its row's; pow: the table */
+    /* A chunk's sum as one relative to this, its row's; pow: the table.  One that counts is above 0, although the logit that it is relative to may lie up to 100 powers of two below its
+     * largest: that is taken as 2^-1000 at least, where it makes no difference beside the row's sum */
     __device__ __forceinline__ double chunk_fast(const VfStat &x, const double *pow) const {   /* both by whole steps */
         const int32_t k = (int32_t)fminf(fmaxf(__int_as_float(x.at) - (float)e, -32000.f), 32000.f);
         const double f = pow[k & 31];
-        return k <= -32000 ? 0.0 : x.s * __hiloint2double(__double2hiint(f) + (k >> 5) * 1048576, __double2loint(f));
+        return x.m < low ? 0.0 : x.s * __hiloint2double(__double2hiint(f) + (k >> 5) * 1048576, __double2loint(f));
     }
     __device__ __forceinline__ double chunk(const VfStat &x, const double *pow) const {
         const float at = __int_as_float(x.at);
         if (fast && x.at != NO_STEP) return chunk_fast(x, pow);
-        if (!(x.s > 0.0)) return 0.0;
+        if (!(x.s > 0.0) || x.m < low) return 0.0;
         if (x.at == NO_STEP && !fast) return x.s * slow(x.m);
-        return x.s * exp2(((x.at == NO_STEP ? (double)x.m * c : (double)at) - (fast ? e : m * c)) * (1.0 / 32.0));
+        return x.s * exp2(fmax(((x.at == NO_STEP ? (double)x.m * c : (double)at) - (fast ? e : m * c)) * (1.0 / 32.0), -1000.0));
     }
     /* log p of logit x, log_s being the logarithm of its row's sum relative to this */
     __device__ __forceinline__ float log_p(float x, double log_s) const { return (float)((fast ? fma((double)x, c, -e) : ((double)x - m) * c) * (LN2 / 32.0) - log_s); }
@@ -484,9 +485,9 @@ __device__ __forceinline__ VfStat stat_at(const VfStat *p) {
     const int4 x = __ldcg(reinterpret_cast<const int4 *>(p));
     return {__hiloint2double(x.y, x.x), __int_as_float(x.z), x.w};
 }
-__device__ __noinline__ double chunk_any(double c, double e, double m, bool fast, double s, float x_m, int32_t at, const double *pow) {
+__device__ __noinline__ double chunk_any(double c, double e, double m, float low, bool fast, double s, float x_m, int32_t at, const double *pow) {
     VfExp E;
-    E.c = c; E.e = e; E.m = m; E.fast = fast;
+    E.c = c; E.e = e; E.m = m; E.low = low; E.fast = fast;
     return E.chunk({s, x_m, at}, pow);
 }
 /* a row's M and S from its chunks', by a whole warp: what is asked for first, so that two rows are on their way at once */
@@ -526,7 +527,7 @@ struct RowOf {
 #pragma unroll 1
         for (uint32_t i = (threadIdx.x & 31u) + (all ? 32u * AT_ONCE : 0u); i < chunks; i += 32u) {
             const VfStat y = stat_at(stat + i);
-            s += chunk_any(E.c, E.e, E.m, E.fast, y.s, y.m, y.at, pow);
+            s += chunk_any(E.c, E.e, E.m, E.low, E.fast, y.s, y.m, y.at, pow);
         }
         return s;
     }
@@ -678,7 +679,7 @@ __device__ __forceinline__ void chunks_of(const VfExp &E, const VfStat *stat, co
         for (uint32_t k = 0; k < N; k++) w[k] = E.chunk_fast(x[k], pow);
     } else {
 #pragma unroll
-        for (uint32_t k = 0; k < N; k++) w[k] = chunk_any(E.c, E.e, E.m, E.fast, x[k].s, x[k].m, x[k].at, pow);
+        for (uint32_t k = 0; k < N; k++) w[k] = chunk_any(E.c, E.e, E.m, E.low, E.fast, x[k].s, x[k].m, x[k].at, pow);
     }
 #pragma unroll
     for (uint32_t k = 0; k < N; k++)

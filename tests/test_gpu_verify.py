@@ -489,3 +489,50 @@ def test_what_other_kernels_left_in_shared_memory(draft):
         pool.release(rows, keep, table)
         c.run()
         assert all(torch.equal(a, b) for a, b in zip((c.accepted, c.next, c.keep, c.logp), want))
+
+
+# ---- tokens that are next to impossible
+def far_below(base, bf16):
+    """five requests whose rows are -inf but for some tokens 2^-1010 to 2^-1040 below the largest, all of them ahead of what else there is; one token of every row takes nearly all"""
+    c = Case([0] * 5, 9000, bf16=bf16, draft="none", seed=34)
+    c.logits.fill_(-INF)
+    c.logits[:, 8000] = base
+    c.logits[0, 600:1024] = base - 704.0     # 2^-1015.6; the first half of the chunk holds nothing
+    c.logits[1, 1023] = base - 720.0
+    c.logits[2, 3000] = base - 704.0
+    c.logits[2, 5000] = base - 672.0         # 2^-969.5: counts
+    c.logits[3, :700] = base - 704.0
+    c.logits[3, 700:900] = base - 688.0      # 2^-992.6
+    return c
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("base", [0.0, 256.0, 131072.0])
+def test_a_draw_of_the_first_token_that_can_be(base, bf16):
+    """a probability below 2^-1000 of the row's largest is none; 131 072 is beyond the steps of the fast exponential (there bf16 has no such differences)"""
+    if bf16 and base:
+        base = -512.0
+    c = far_below(base, bf16)
+    want = [int((c.logits[r].float() >= base - 1000 * math.log(2)).nonzero()[0]) for r in range(5)]
+    c.u_next.fill_(0.0)
+    c.run()
+    assert lib().q4_gpu_last_error() == 0
+    assert c.next.tolist() == want
+    for u in (2.0**-24, 0.5, 1 - 2.0**-24):
+        c.u_next.fill_(u)
+        c.run()
+        assert c.next.tolist() == [8000] * 5 and lib().q4_gpu_last_error() == 0
+
+
+def test_a_draw_behind_a_refused_draft_that_was_all_there_is_ahead():
+    c = Case([1] * 3, 9000, draft="none", seed=35)
+    c.logits.fill_(-INF)
+    c.logits[:, 8000] = 0.0
+    c.logits[:, 40] = -650.0                 # the draft: 2^-938
+    c.logits[:, 2000:2040] = -705.0          # 2^-1017: within 100 powers of two of what its warp saw first, and none
+    c.token.fill_(40)
+    c.u_accept.fill_(0.5)
+    c.u_next.fill_(0.0)
+    c.run()
+    assert lib().q4_gpu_last_error() == 0
+    assert c.accepted.tolist() == [0] * 3 and c.next.tolist() == [8000] * 3
