@@ -783,7 +783,7 @@ __device__ __forceinline__ void look(const VerifyParams &P, const Weights<BF16> 
 template <bool BF16>
 __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams P) {
     __shared__ Row s_p[PICK_WARPS], s_q[PICK_WARPS];
-    __shared__ uint32_t s_said[PICK_WARPS], s_chunk;
+    __shared__ uint32_t s_said[PICK_WARPS], s_chunk, s_alone;
     __shared__ int32_t s_best[PICK_WARPS], s_draft[PICK_WARPS];
     __shared__ double s_left, s_part[PICK_WARPS], s_pow[32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.x;
@@ -926,14 +926,19 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     }
     if (warp == 0) {
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
+        const double u = (double)__ldcg(P.u_next + r);
         double left, whole;
-        const uint32_t at = place_of(P.chunks, (double)__ldcg(P.u_next + r), left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, special, without, i0, i1, w); });
+        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, special, without, i0, i1, w); });
+        const bool alone = !(whole > 0.0);
+        if (alone) at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, 0xffffffffu, 0.0, i0, i1, w); });   /* nothing besides the draft: p itself */
         if (lane == 0) {
             s_chunk = at;
             s_left = left;
+            s_alone = alone;
         }
     }
     __syncthreads();
+    if (s_alone) W.certain = -1;
     look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
 }
 

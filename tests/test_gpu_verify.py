@@ -536,3 +536,21 @@ def test_a_draw_behind_a_refused_draft_that_was_all_there_is_ahead():
     c.run()
     assert lib().q4_gpu_last_error() == 0
     assert c.accepted.tolist() == [0] * 3 and c.next.tolist() == [8000] * 3
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 5000, 40000])
+@pytest.mark.parametrize("u", [1.0, 2.0, float("nan")])
+def test_a_refused_draft_that_is_all_there_is(vocab, u):
+    """max(p - q, 0) is 0 throughout, so that p is drawn from: random numbers that refuse what cannot be"""
+    c = Case([1, 2, 1], vocab, draft="none", seed=36)
+    d = vocab * 3 // 4
+    c.logits.fill_(-INF)
+    c.logits[:, d] = 3.0
+    c.token.fill_(d)
+    c.u_accept.fill_(u)
+    c.run()
+    assert lib().q4_gpu_last_error() == 0
+    # at u = 1 either is right: u S < w with S = w (1 + x), |x| <= 7e-9 as the row's sum is off, holds where x is below 0
+    assert u == 1 or c.accepted.tolist() == [0] * 3
+    assert c.next.tolist() == [d] * 3
+    assert (c.logp[c.start[:-1].long()].abs() <= 7e-9).all()              # log p = 0, by a sum that is off by so much of itself
