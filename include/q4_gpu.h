@@ -591,7 +591,7 @@ bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t
  *     next: the first token whose running sum of w exceeds u_next[r] times the whole sum, w = max(p - q, 0) in the row whose draft was
  *     refused (p where that is 0 throughout), w = p in the last row if all are kept
  * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Probabilities and comparisons are in 64
- * bits, a row's sum of exponentials is off by 5e-9 of itself at most; what is below 2^-1000 of the row's largest exponential counts as 0.  What row t of draft holds behind a request's last token, and for greedy requests, makes no difference.
+ * bits, a row's sum of exponentials is off by 7e-9 of itself at most; what is below 2^-1000 of the row's largest exponential counts as 0.  What row t of draft holds behind a request's last token, and for greedy requests, makes no difference.
  *   accepted, next [n_req]   drafts kept, and the token behind them
  *   logp [n_tok] or NULL     row t's log p of the token that it decided (a kept draft, next), 0 for greedy requests and in rows behind next's
  *   rows, keep [n_req]       or both NULL: keep[r] = rows[r] + accepted[r] + 1, rows[r] being what the request held before the step: for q4_gpu_pages_release

@@ -240,10 +240,11 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
 }
 
 /* Exponentials for sums, relative to a whole step e of which all that counts lies within 100 powers of two: as VfExp's, but in 32 bits and in two parts.
- * x c comes to whole steps and a rest by a product in two words.  The table's entry is 2^(j / 32) rounded, its error goes into the rest's exponential less 1,
- * q: the value is w + w q, where w is exact and q below 0.0109.  The sums are in 64 bits, but for up to eight w q at a time.  Errors, of the sum: steps 2.25 x 2^-25
- * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's series, up to r^3: 6e-10, its last roundings 1.5 x 2^-25 x 0.0109: 5e-10;
- * seven additions 7 x 2^-25 x 0.0109: 2.3e-9.  Below 5e-9 in all, and for many tokens far below, as they are not all one way. */
+ * x c comes to whole steps and a rest by a product in two words.  The step is rounded by c's first word alone: the second, up to 2^-24 of c, adds to the rest, which is
+ * 1/2 at small x c and up to 1/2 + 2e6 x 2^-24 = 0.62 at the largest.  The table's entry is 2^(j / 32) rounded, its error goes into the rest's exponential less 1,
+ * q: the value is w + w q, where w is exact and q below 0.0135.  The sums are in 64 bits, but for up to eight w q at a time.  Errors, of the sum: steps 2.25 x 2^-25
+ * (two roundings, and c's second word over 2^21 steps), times ln 2 / 32: 1.5e-9;  q's series, up to r^3: 0.0135^4 / 24 = 1.4e-9, its last roundings 1.5 x 2^-25 x 0.0135: 6e-10;
+ * seven additions 7 x 2^-25 x 0.0135: 2.8e-9.  Below 7e-9 in all (5e-9 at |x| below 5000 T, where q is below 0.0112), and for many tokens far below, as they are not all one way. */
 struct VfFast {
     float c_hi, c_lo, base, low, high, step;
     bool ok;

@@ -554,3 +554,29 @@ def test_a_refused_draft_that_is_all_there_is(vocab, u):
     assert u == 1 or c.accepted.tolist() == [0] * 3
     assert c.next.tolist() == [d] * 3
     assert (c.logp[c.start[:-1].long()].abs() <= 7e-9).all()              # log p = 0, by a sum that is off by so much of itself
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("limit", [5400.0, 43300.0])
+def test_sums_at_the_largest_sizes_of_the_fast_exponential(limit, bf16):
+    """rows of equal logits, one or many of them, |x / T| up to 2e6 steps of 1/32 of a power of two, where the rest of a step is largest"""
+    n_req, vocab = 600, 2100
+    g = torch.Generator(device="cuda").manual_seed(37)
+    temp = 0.5 + 1.5 * torch.rand(n_req, device="cuda", generator=g)
+    c = Case([0] * n_req, vocab, bf16=bf16, draft="none", seed=37)
+    c.temp = temp
+    sign = torch.where(torch.rand(n_req, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    x = (temp * limit * sign * (0.9 + 0.1 * torch.rand(n_req, device="cuda", generator=g))).to(c.logits.dtype)
+    x = torch.where((x.float() / temp).abs() > limit, (x.float() * 0.99).to(x.dtype), x)
+    assert float((x.float() / temp).abs().max()) <= limit * 1.002
+    many = torch.tensor([1, 2, 8, 64, vocab], device="cuda")[torch.arange(n_req, device="cuda") % 5]
+    c.logits.copy_(torch.where(torch.arange(vocab, device="cuda")[None] < many[:, None], x.float()[:, None], -INF))
+    c.u_next.copy_((torch.arange(n_req, device="cuda") // 5 % 8 + 0.5) / 8)
+    c.run()
+    assert lib().q4_gpu_last_error() == 0
+    # token k of n equal ones has 1 / n: borders at k / n.  Of 64, u = (2 j + 1) / 16 is the one at 4 (2 j + 1): sums that are off by 7e-9 put it on either side
+    at = [u * n for u, n in zip(c.u_next.tolist(), many.tolist())]
+    assert all(got == int(k) or (n == 64 and got == k - 1) for got, k, n in zip(c.next.tolist(), at, many.tolist()))
+    # log p = -log n: its own rounding to fp32, the sum's 7e-9, and the exponent of x over the row's step in 64 bits (2e6 x 2^-53 x ln 2 / 32 and less)
+    want = -many.double().log()
+    assert ((c.logp.double() - want).abs() <= 2.0**-24 * want.abs() * (1 + 1e-6) + 7e-9).all()
