@@ -51,7 +51,7 @@ constexpr uint32_t NOT_SERVED = 0xffffffffu, NO_PAGE = 0xfffffffeu;
 __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P) {
     extern __shared__ uint32_t s_fork[];
     __shared__ uint32_t s_entries, s_tiles, s_pages, s_last;
-    /* of forks: entries and tiles up to and with each; source and place; the page that is copied and the one that it is copied to */
+    /* of places: the fork that fills each; of forks: entries and tiles up to and with each; source and place; the page that is copied and the one that it is copied to */
     uint32_t *owner = s_fork, *entry_end = owner + P.n_req, *tile_end = entry_end + P.n_fork, *places = tile_end + P.n_fork, *old_page = places + P.n_fork, *new_page = old_page + P.n_fork;
     const uint32_t tid = threadIdx.x, mask = (1u << P.page_shift) - 1u;
     const uint64_t room = (uint64_t)P.table_stride << P.page_shift;
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P)
         places[i] = good ? where : NOT_SERVED;
         entry_end[i] = good ? (uint32_t)n >> P.page_shift : 0u;
         tile_end[i] = good ? (((uint32_t)n & mask) + 15u) >> 4 : 0u;
+        old_page[i] = (uint32_t)n;   /* the thread's own until below */
         uint64_t e, tp;
         one(i, e, tp);
         e_sum += e; tp_sum += tp;
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P)
         const uint32_t before = (uint32_t)(tp_sum >> 32);
         e_sum += e; tp_sum += tp;
         const bool fits = (tp_sum >> 32) <= n_free && e_sum < NOT_SERVED;
+        if (fits && places[i] != NOT_SERVED) owner[places[i] >> 16] = old_page[i];   /* from now on the rows of the place: P.len may be P.rows */
         old_page[i] = new_page[i] = NO_PAGE;
         if (fits && tp) {
             const uint32_t where = places[i];
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P)
     __syncthreads();
     if (s_last)
         for (uint32_t i = tid; i < P.n_fork; i += PLAN_THREADS)
-            if (places[i] != NOT_SERVED) P.rows[places[i] >> 16] = __ldcg(P.len + i);
+            if (places[i] != NOT_SERVED) P.rows[places[i] >> 16] = (int32_t)owner[places[i] >> 16];
 }
 
 struct ReleaseParams {

@@ -550,3 +550,24 @@ def test_refusals():
         bare.release(ints([0]), ints([0]), ints([[0, 0]]))
     L.q4_gpu_last_error()
     b.check()
+
+
+def test_lengths_that_are_what_the_requests_hold():
+    """rows given as the lengths too: all forks see them as they were, those that a thread comes to later among them"""
+    n_req, n = 1300, 600
+    pool = q4gpu.PagePool(1, 1, 64, 40, 16)
+    table = torch.full((n_req, 8), -1, dtype=torch.int32, device="cuda")
+    rows, add = torch.zeros(2, n_req, dtype=torch.int32, device="cuda").unbind(0)
+    add[0] = 64
+    start, slot, pos, req = torch.zeros(n_req + 1, dtype=torch.int32, device="cuda"), *torch.zeros(3, 64, dtype=torch.int32, device="cuda").unbind(0)
+    lib().q4_gpu_last_error()
+    pool.plan(rows, add, table, start, slot, pos, req)
+    rows += add
+    dst = torch.arange(512, 512 + n, dtype=torch.int32, device="cuda")      # the first fork's place is the one whose rows are the 512th's length
+    pool.fork(rows, torch.zeros_like(dst), dst, rows[:n], table)
+    assert lib().q4_gpu_last_error() == 0
+    want = torch.zeros(n_req, dtype=torch.int32)
+    want[0] = want[512] = 64
+    assert torch.equal(rows.cpu(), want)
+    assert table[512, :4].tolist() == table[0, :4].tolist() and int((table != -1).sum()) == 8
+    assert int(pool.shares.sum()) == 4
