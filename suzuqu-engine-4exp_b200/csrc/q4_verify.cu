@@ -929,9 +929,14 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
         const VfStat *sp = stat_p + (uint64_t)stop * P.chunks;
         const double u = (double)__ldcg(P.u_next + r);
         double left, whole;
-        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, special, without, i0, i1, w); });
-        const bool alone = !(whole > 0.0);
-        if (alone) at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, 0xffffffffu, 0.0, i0, i1, w); });   /* nothing besides the draft: p itself */
+        uint32_t at, apart = special;
+        bool alone = false;
+#pragma unroll 1
+        for (;; apart = 0xffffffffu) {   /* nothing besides the draft: p itself */
+            at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, apart, without, i0, i1, w); });
+            if (whole > 0.0 || apart == 0xffffffffu) break;
+            alone = true;
+        }
         if (lane == 0) {
             s_chunk = at;
             s_left = left;
