@@ -96,3 +96,35 @@ def test_a_step_replayed_is_the_step_itself(kind):
     q4gpu.use_torch_stream()
     s.pool.release(s.rows, torch.zeros_like(s.rows), s.table)
     assert int(s.pool.n_free[0]) == 120 and L.q4_gpu_last_error() == 0
+
+
+def test_drafts_beside_a_chunk_of_a_prompt():
+    """verify over the rows that the host gathers: drafts and the token before them, of a chunk its last token; what it says to keep is what release takes"""
+    s = Step(q4gpu.KIND_Q8, n_req=3, idle=20)
+    L = lib()
+    L.q4_gpu_last_error()
+    p, held = s.pool, [37, 16, 90]
+    for add in (held, [DRAFTS + 1, 20, 1]):
+        s.add.copy_(torch.tensor(add, dtype=torch.int32))
+        n = sum(add)
+        slot, pos, req = torch.zeros(3, n, dtype=torch.int32, device="cuda").unbind(0)
+        p.plan(s.rows, s.add, s.table, s.start, slot, pos, req)
+        before = s.rows.clone()
+        s.rows.add_(s.start.diff())
+    gathered = torch.tensor([0, 1, 2, 3, DRAFTS + 20, DRAFTS + 21], device="cuda")         # of the step's 25 tokens
+    start = torch.tensor([0, DRAFTS + 1, DRAFTS + 2, DRAFTS + 3], dtype=torch.int32, device="cuda")
+    s.draft.copy_(s.logits)                                     # drafts that are as likely to both: kept
+    token = s.token[:25][gathered].contiguous()
+    token[1:DRAFTS + 1] = s.logits[gathered[:DRAFTS]].argmax(1)
+    rows = before + torch.tensor([0, 19, 0], dtype=torch.int32, device="cuda")
+    u, logits = s.u_accept[:6] * 0.9, s.logits[gathered]
+    q4gpu.verify(logits, token, start, u, s.u_next, s.accepted, s.next, draft=logits.clone(), temp=s.temp, logp=s.logp, rows=rows, keep=s.keep)
+    assert s.accepted.tolist() == [DRAFTS, 0, 0] and all(0 <= x < VOCAB for x in s.next.tolist())
+    assert s.keep.tolist() == [37 + DRAFTS + 1, 36, 91]
+    p.release(s.rows, s.keep, s.table)
+    assert s.rows.tolist() == s.keep.tolist() and L.q4_gpu_last_error() == 0
+    token[2] = (token[2] + 1) % VOCAB                           # a draft that is refused, and its rows' place given back
+    u.fill_(1.0)
+    q4gpu.verify(logits, token, start, u, s.u_next, s.accepted, s.next, temp=s.temp, rows=rows, keep=s.keep)
+    p.release(s.rows, s.keep, s.table)
+    assert s.rows.tolist() == [37 + int(s.accepted[0]) + 1, 36, 91] and L.q4_gpu_last_error() == 0
