@@ -527,7 +527,7 @@ bool q4_gpu_pages_attend(const q4_gpu_pages *pg, uint32_t layer, const void *q, 
  *
  * Rotation of position p: pair i is turned by p * f_i, the pairs being dims (2 i, 2 i + 1) (half = 0) or (i, i + n_rot / 2) (half = 1)
  * of the first n_rot dims; mag is on the turned dims.  turn[i] is f_i in turns as a fraction of 2^64: p * turn[i] modulo 2^64 is the angle
- * without a rounding, at any position. */
+ * without a rounding, at any position; the kernels take sine and cosine of it to 2^-26 of a turn. */
 typedef struct q4_gpu_rope {
     uint32_t n_rot;
     int32_t half;
@@ -579,8 +579,8 @@ bool q4_gpu_pages_release(const q4_gpu_pages *pg, int32_t *shares, int32_t *rows
  * order, to the i-th free one in front.  Then pages [0, n_pages - n_free) are in use and the stack hands out the others in ascending order.  map [n_pages] tells
  * each page's new number (-1: free); shares (may be NULL) move along; the tables' entries of the requests' rows are renamed.  Tables that
  * are not given here are the host's to rename by map.  A stack that names a page twice, or one that is not the pool's: nothing moves, map is the
- * identity, status bit 4; a table's entry that is no page in use stays as it is, status bit 4.  n_req may be 0 (rows and table NULL).  Scratch (4 bytes
- * per page) grows outside a capture only. */
+ * identity, status bit 4; a table's entry that is no page in use stays as it is, status bit 4.  n_req may be 0 (rows and table NULL).  The pool
+ * keeps its n_pages: layers lie that far apart, so what lies behind the pages in use is one piece per layer.  Scratch (4 bytes per page) grows outside a capture only. */
 bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t *rows, uint32_t n_req, int32_t *table, uint32_t table_stride, int32_t *map);
 
 /* Drafted tokens held against the target's distributions, and the token behind the last one that is kept (no counterpart in the reference).  Request r
@@ -592,6 +592,8 @@ bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t
  *     refused (p where that is 0 throughout), w = p in the last row if all are kept
  * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Probabilities and comparisons are in 64
  * bits, a row's sum of exponentials is off by 7e-9 of itself at most; what is below 2^-1000 of the row's largest exponential counts as 0.  What row t of draft holds behind a request's last token, and for greedy requests, makes no difference.
+ * Every token behind a request's first counts as a draft.  A step in which others bring chunks of a prompt has a token, start and logits of its own here, gathered by the
+ * host: a request's drafts and the token before them, of a chunk its last token alone, with rows[r] the number of rows before that.
  *   accepted, next [n_req]   drafts kept, and the token behind them
  *   logp [n_tok] or NULL     row t's log p of the token that it decided (a kept draft, next), 0 for greedy requests and in rows behind next's
  *   rows, keep [n_req]       or both NULL: keep[r] = rows[r] + accepted[r] + 1, rows[r] being what the request held before the step: for q4_gpu_pages_release

@@ -6,7 +6,8 @@
  *     y = x / sqrt(mean x^2 + eps) * w;  (a, b) -> mag (a cos - b sin, a sin + b cos), the angle of pair i being pos * f_i
  *
  * The angle is the part of pos * f_i behind the last whole turn.  f_i is kept in turns as a fraction of 2^64, so that the product with
- * the position, modulo 2^64, is that part exactly: an fp32 angle is off by 0.008 at position 262 144, by half a turn at 2^26.
+ * the position, modulo 2^64, is that part exactly; sine and cosine are taken of it rounded to fp32, 2^-26 of a turn off at most at any position.  An angle
+ * in fp32 throughout is off by 0.008 at position 262 144, by half a turn at 2^26.
  *
  * Bound by memory: every value is read once and written once.  4096 tokens of 24 gated heads of 256 in fp32, 373 MB, take 62 us (92 % of a copy's rate); 16 001 fused
  * bf16 rows of 32 heads of 128 with 8 kv heads, 394 MB, 75 us (80 %), there beside the issue slots.
@@ -21,8 +22,8 @@ namespace {
 
 using namespace q4tc;
 
-/* Warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115).  28 of them on an SM, by 72 registers:
- * 8192 fused rows of 16 heads 31.6 us, 33.5 with up to 96; 32 of them are slower for few tokens (700 tokens of 32 heads 9.2 us, 8.4) */
+/* Warps differ in their turns: a block of several would keep its place for the longest (16 001 fused rows 78 us, in pairs 99, in eights 115).  28 of them on an SM, by 72 registers (forms
+ * that take bf16, and halves of fp32, spill up to 32 bytes, neighbours of fp32 none): 8192 fused rows of 16 heads 31.6 us, 33.5 with up to 96; 32 of them are slower for few tokens (700 tokens of 32 heads 9.2 us, 8.4) */
 constexpr uint32_t PREP_THREADS = 32, PREP_BLOCKS = 28;
 
 struct PrepParams {
@@ -375,8 +376,9 @@ template <int KIND, int HD, bool BF16>
 bool prep_launch(PrepParams &p) {
     constexpr uint32_t RPW = 256u / HD;
     /* A warp's start (sines, factors) is worth some turns: no more warps than the SMs hold at once, and several rounds of them, the last of which may be part empty,
-     * only where there are many tokens.  us, with 20 warps per SM and with 54: 300 tokens of 24 heads of 256 6.2 and 8.9, 500 of 16 of 128 3.1 and 5.2, 4096 of 24 of
-     * 256 66.2 and 62.3. */
+     * only where there are many tokens.  us, with 20 warps per SM and with 54: 300 tokens of 24 heads of 256 6.2 and 8.9, 1000 17.3 and 17.1, 2000 34.4 and 31.9, 3000 47.9 and 46.0,
+     * 4000 65.2 and 61.1; 16 of 128 in fp32 500 3.1 and 5.2, 1000 5.6 and 6.3, 2000 12.6 and 12.0, 3000 18.7 and 17.6; 32 of 128 in bf16 2000 12.9 and 15.0, 3000 18.9 and 19.7, 4000
+     * 22.8 and 22.6; 8 of 64 2000 4.7 and 6.8, 3000 6.9 and 10.3, 4000 9.0 and 9.0.  The sides meet between 1000 tokens (large rows) and 4000 (small ones): one line between them. */
     const uint32_t most = (p.n_tok < 2048u ? 20u : 54u) * (uint32_t)g_q4.sm_count, want = (most + p.n_tok - 1u) / p.n_tok, q_turns = (p.n_head + RPW - 1u) / RPW, kv_turns = (p.n_kvh + RPW - 1u) / RPW;
     const uint32_t per = (q_turns + kv_turns + want - 1u) / want;
     p.q_per = per < q_turns ? per : q_turns;

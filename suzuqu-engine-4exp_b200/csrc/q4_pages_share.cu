@@ -44,8 +44,8 @@ struct ForkParams {
 /*
  * Fork.  Every block forms the sums over all forks itself, as plan does, and looks up the pages that are copied; then the table entries of whole pages are shared out
  * by threads, the tiles to copy (fork, layer, kv head, 16 rows) by warps.  The last block to finish writes what the others have read: the
- * stack's top and the children's rows.  256 forks with 104 MB to copy, most of it out of and into L2, 25 us; four of one prompt 6: sums, look-ups that follow
- * one another and a fence, where the bytes are worth nothing.
+ * stack's top and the children's rows.  Under the profiler 256 forks with 104 MB to copy, most of it out of and into L2, take 25 us, four of
+ * one prompt 9: sums, look-ups that follow one another and a fence, where the bytes are worth nothing.
  */
 constexpr uint32_t NOT_SERVED = 0xffffffffu, NO_PAGE = 0xfffffffeu;
 __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_fork_k(const ForkParams P) {
@@ -207,7 +207,8 @@ __device__ __forceinline__ uint32_t rel_meet(uint32_t times, bool bad, uint32_t 
  * Release.  The entries that requests give up are numbered in the requests' order, a block has an equal part of them.  A page goes back with the last of its
  * entries, if there are as many as it has holders: first every page's entries are counted and the largest number kept, then the blocks
  * count the pages that go back, then they put them on the stack; between these they meet.  Which entry is a page's last does not depend on the
- * order of the atomics.  Bound by those trips to L2.  (Three launches instead: 14 us for four beams, 21 for 256 answers, as one 9 and 13.)
+ * order of the atomics.  Bound by those trips to L2.  (Under the profiler 7 us for four beams, 11 to 12 for 256 answers;
+ * as three launches 14 and 21.)
  */
 __global__ void __launch_bounds__(PLAN_THREADS) q4_pg_release_k(const ReleaseParams P) {
     extern __shared__ uint32_t s_rel[];

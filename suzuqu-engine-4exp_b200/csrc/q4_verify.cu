@@ -27,7 +27,7 @@
 namespace {
 
 constexpr uint32_t EACH = 32, CHUNK = 32u * EACH, VF_THREADS = 128, VF_WARPS = VF_THREADS / 32u, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32u, PICK_EACH = CHUNK / PICK_THREADS;
-/* of the first launch: chunks of a warp at most, blocks per SM (80 registers: with 64 it is slower), 16-byte pieces on their way to a lane, chunks that are brought to L2 ahead */
+/* of the first launch: chunks of a warp at most, blocks per SM (80 registers, 8 to 36 bytes spilled; with 64, which spill more, it is slower), 16-byte pieces on their way to a lane, chunks that are brought to L2 ahead */
 constexpr uint32_t SPAN = 6, STAT_BLOCKS = 6, VF_RING = 4, VF_AHEAD = 2;
 constexpr float LARGEST = 3.402823466e38f;
 
@@ -1056,14 +1056,16 @@ extern "C" bool q4_gpu_verify(const void *logits, int bf16, uint64_t ld, const v
     const uint64_t size = bf16 ? 2u : 4u;
     p.logits = (const uint8_t *)logits; p.draft = (const uint8_t *)draft; p.ld = ld * size; p.draft_ld = draft_ld * size; p.vocab = vocab;
     p.chunks = (uint32_t)((vocab + 16u / size - 1u + CHUNK - 1u) / CHUNK);   /* wherever in a 16-byte piece a row begins */
-    /* a warp's chunks: as many as leave a round and a half of warps (24 on an SM at once), so that the search for the request and the scale are done once for them: 256 draws
-     * over 32 003 tokens 26.5 us with one, 23.9 with three; 48 x 5 drafts over 131 072 105 with three, 101 with six, 103 with nine */
+    /* A warp's chunks: as many as leave a round and a half of warps (24 on an SM at once), so that the search for the request and the scale are done once for them: 48 x 5
+     * drafts over 131 072 tokens 105 us with three, 101 with six, 103 with nine.  A draft row is counted for every token: those behind a request's last one, which are
+     * not read, are known on the device alone.  256 draws over 32 003 tokens come to three with a tensor of draft logits beside them (22.5 us, 26.5 with one; half of the
+     * warps leave at once, the others fill 0.8 of a round) and to one without it (22.7). */
     const uint64_t all = (uint64_t)n_tok * (draft ? 2u : 1u) * p.chunks, share = all / (36u * (uint64_t)g_q4.sm_count);
     p.span = share < 1u ? 1u : share < SPAN ? (uint32_t)share : SPAN;
     p.spans = (p.chunks + p.span - 1u) / p.span;
     /* Rows behind refused drafts can be spared where warps come in several rounds; finding out costs a warp a fence and an atomic, and is of no use to the rows of the last two
-     * rounds, which are under way by then.  us, without and with: 256 requests with 8 looked-up drafts, most of them refused, over 50 001 tokens (5.8 rounds) 111 and 60,
-     * 64 with 8 drafts, most of them kept, over 131 072 (7 rounds) 162 and 150, 48 with 5 (3.6 rounds) 99.5 and 101 */
+     * rounds, which are under way by then.  us, without and with: 256 requests with 8 looked-up drafts, most of them refused, over 50 001 tokens (5.8 rounds) 101 and 54,
+     * 64 with 8 drafts, most of them kept, over 131 072 (7 rounds) 153 and 140, 48 with 5 (3.6 rounds) 95.4 and 96.0 */
     const uint64_t warps_of = (uint64_t)p.spans * (draft ? 2u : 1u), at_once = STAT_BLOCKS * VF_WARPS * (uint64_t)g_q4.sm_count;
     p.early = n_tok > n_req && n_tok <= EARLY_MAX && n_tok * warps_of > 4u * at_once ? n_tok - (uint32_t)(2u * at_once / warps_of) : 0u;
     p.levels = p.early ? (n_tok + n_req - 1u) / n_req : 1u;
