@@ -591,7 +591,9 @@ bool q4_gpu_pages_compact(const q4_gpu_pages *pg, int32_t *shares, const int32_t
  *     next: the first token whose running sum of w exceeds u_next[r] times the whole sum, w = max(p - q, 0) in the row whose draft was
  *     refused (p where that is 0 throughout), w = p in the last row if all are kept
  * A temperature of 0: a draft is kept if it is the largest logit's index (the first of equals), next is that index.  Probabilities and comparisons are in 64
- * bits, a row's sum of exponentials is off by 7e-9 of itself at most; what is below 2^-1000 of the row's largest exponential counts as 0.  What row t of draft holds behind a request's last token, and for greedy requests, makes no difference.
+ * bits, a row's sum of exponentials is off by 7e-9 of itself at most, what w = max(p - q, 0) comes to by a thousandth of itself (where it
+ * is less than 2^-16 in all, by 64-bit roundings of p and q); what is below 2^-1000 of the row's largest exponential counts as 0.  What row t of draft holds behind a request's last
+ * token, and for greedy requests, makes no difference.
  * Every token behind a request's first counts as a draft.  A step in which others bring chunks of a prompt has a token, start and logits of its own here, gathered by the
  * host: a request's drafts and the token before them, of a chunk its last token alone, with rows[r] the number of rows before that.
  *   accepted, next [n_req]   drafts kept, and the token behind them

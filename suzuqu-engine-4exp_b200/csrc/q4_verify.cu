@@ -948,21 +948,87 @@ __global__ void __launch_bounds__(PICK_THREADS) q4_vf_pick_k(const VerifyParams 
     look<BF16>(P, W, r, stop, p.s, s_chunk, s_left);
 }
 
+__device__ __forceinline__ VfChoice choice_at(const VfChoice *p) {
+    VfChoice D;
+    const int4 *from = reinterpret_cast<const int4 *>(p);
+    int4 *to = reinterpret_cast<int4 *>(&D);
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(VfChoice) / 16u; i++) to[i] = __ldcg(from + i);
+    return D;
+}
+/* What p has over q is a difference of numbers that are off by 7e-9 of themselves.  Where it comes to less than this in all (a draft that p and q all but exclude was refused), both
+ * rows are summed again in 64 bits, and chunk by chunk what p has over q by these sums: by a block, 1 over the sums being what comes back.  Above it what p has over q is off by a
+ * thousandth of itself at most.  A draft that was drawn from q is refused so once in 65 536 at most; it costs about 230 us over 131 072 tokens (a block for both rows, twice) */
+constexpr double REST_LITTLE = 1.0 / 65536.0;
+template <bool BF16>
+__device__ __noinline__ double2 rest_again(const VerifyParams &P, uint32_t r) {
+    __shared__ double s_a[PICK_WARPS], s_b[PICK_WARPS];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const VfChoice D = choice_at(P.choice + r);
+    double *rest = P.rest + (uint64_t)r * P.chunks;
+    Weights<BF16> W;
+    W.set(P, D.stop, D.m_p, D.m_q, 1.0, 1.0, VfScale(D.c, D.drop), true, -1);
+    double2 scale = make_double2(1.0, 1.0);
+#pragma unroll 1
+    for (uint32_t over = 0; over < 2u; over++) {
+        double a = 0.0, b = 0.0;
+#pragma unroll 1
+        for (uint32_t chunk = 0; chunk < P.chunks; chunk++) {
+            const uint32_t i0 = W.begin(chunk) + tid, i1 = W.end(chunk);
+            float xp[PICK_EACH], xq[PICK_EACH];
+            double w[PICK_EACH], y[PICK_EACH];
+#pragma unroll
+            for (uint32_t k = 0; k < PICK_EACH; k++) W.load((uint64_t)i0 + k * PICK_THREADS, i1, xp[k], xq[k]);
+            if (over) {
+                W.of(xp, xq, i0, PICK_THREADS, w);
+#pragma unroll
+                for (uint32_t k = 0; k < PICK_EACH; k++) a += w[k];
+            } else {
+                W.p.of(xp, W.table, w);
+                W.q.of(xq, W.table, y);
+#pragma unroll
+                for (uint32_t k = 0; k < PICK_EACH; k++) {
+                    a += w[k];
+                    b += y[k];
+                }
+            }
+            if (!over && chunk + 1u < P.chunks) continue;
+            a = warp_sum(a);
+            b = warp_sum(b);
+            __syncthreads();     /* what was there has been read */
+            if (lane == 0) {
+                s_a[warp] = a;
+                s_b[warp] = b;
+            }
+            __syncthreads();
+            a = b = 0.0;
+            for (uint32_t k = 0; k < PICK_WARPS; k++) {
+                a += s_a[k];
+                b += s_b[k];
+            }
+            if (!over) {
+                scale = make_double2(1.0 / a, 1.0 / b);
+                W.scale_p = scale.x;
+                W.scale_q = scale.y;
+            } else {
+                if (tid == 0) __stcg(rest + chunk, a);
+                a = 0.0;
+            }
+        }
+    }
+    __syncthreads();
+    return scale;
+}
+
 /* what p has over q, chunk by chunk, the next one's logits on their way meanwhile; the request's last block to finish looks for next */
 template <bool BF16>
-__global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const VerifyParams P) {
-    __shared__ uint32_t s_last, s_chunk, s_over;
+__global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const __grid_constant__ VerifyParams P) {
+    __shared__ uint32_t s_last, s_chunk, s_over, s_little;
     __shared__ double s_left, s_part[2][PICK_WARPS], s_pow[32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, r = blockIdx.y, chunk0 = blockIdx.x;
     if (tid < 32u) s_pow[tid] = __ldg(g_vf_pow + tid);
     q4d_pdl_wait();
-    VfChoice D;
-    {
-        const int4 *from = reinterpret_cast<const int4 *>(P.choice + r);
-        int4 *to = reinterpret_cast<int4 *>(&D);
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof(VfChoice) / 16u; i++) to[i] = __ldcg(from + i);
-    }
+    const VfChoice D = choice_at(P.choice + r);
     if (!D.open) return;
     const uint32_t stop = D.stop;
     const VfScale S(D.c, D.drop);
@@ -1006,25 +1072,33 @@ __global__ void __launch_bounds__(PICK_THREADS, 3) q4_vf_rest_k(const VerifyPara
     }
     __syncthreads();
     if (!s_last) return;
-    if (warp == 0) {
-        const double u = (double)__ldcg(P.u_next + r);
-        double left, whole;
-        uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) {
+#pragma unroll 1
+    for (uint32_t again = 0; again < 2u; again++) {
+        if (warp == 0) {
+            const double u = (double)__ldcg(P.u_next + r);
+            double left, whole;
+            uint32_t at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) {
 #pragma unroll
-            for (uint32_t k = 0; k < sizeof(w) / sizeof(w[0]); k++) w[k] = i0 + k < i1 ? __ldcg(rest + i0 + k) : 0.0;
-        });
-        const bool over_q = whole > 0.0;
-        if (!over_q) {           /* p nowhere above q: as if none was refused */
-            const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
-            at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, 0xffffffffu, 0.0, i0, i1, w); });
+                for (uint32_t k = 0; k < sizeof(w) / sizeof(w[0]); k++) w[k] = i0 + k < i1 ? __ldcg(rest + i0 + k) : 0.0;
+            });
+            const bool over_q = whole > 0.0, little = !again && whole < REST_LITTLE;
+            if (!over_q && !little) {   /* p nowhere above q: as if none was refused */
+                const VfStat *sp = P.stat + (uint64_t)stop * P.chunks;
+                at = place_of(P.chunks, u, left, whole, [&](uint32_t i0, uint32_t i1, auto &w) { chunks_of(W.p, sp, s_pow, 0xffffffffu, 0.0, i0, i1, w); });
+            }
+            if (lane == 0) {
+                s_chunk = at;
+                s_left = left;
+                s_over = over_q;
+                s_little = little;
+            }
         }
-        if (lane == 0) {
-            s_chunk = at;
-            s_left = left;
-            s_over = over_q;
-        }
+        __syncthreads();
+        if (!s_little) break;
+        const double2 scale = rest_again<BF16>(P, r);
+        W.scale_p = scale.x;
+        W.scale_q = scale.y;
     }
-    __syncthreads();
     W.over_q = s_over;
     look<BF16>(P, W, r, stop, D.sum_p, s_chunk, s_left);
 }

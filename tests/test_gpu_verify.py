@@ -580,3 +580,31 @@ def test_sums_at_the_largest_sizes_of_the_fast_exponential(limit, bf16):
     # log p = -log n: its own rounding to fp32, the sum's 7e-9, and the exponent of x over the row's step in 64 bits (2e6 x 2^-53 x ln 2 / 32 and less)
     want = -many.double().log()
     assert ((c.logp.double() - want).abs() <= 2.0**-24 * want.abs() * (1 + 1e-6) + 7e-9).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("vocab", [700, 9001, 140001])
+@pytest.mark.parametrize("shift", [14.9, 37.3])
+def test_what_p_has_over_a_q_that_is_nearly_the_same(vocab, bf16, shift):
+    """a token has nearly all of both; what p has over q is 1e-10 and less, far below what their sums may be off by.  Drafts that cannot be are refused"""
+    n_req = 64
+    c = Case([1] * n_req, vocab, bf16=bf16, seed=38, ld=vocab + 3)
+    g = torch.Generator(device="cuda").manual_seed(38)
+    other = shift + torch.linspace(0, 9, c.n_tok, device="cuda")[:, None].to(c.logits.dtype).float()      # softmax knows no shift, but the sums of exponentials are rounded otherwise
+    for x, m in ((c.logits, shift), (c.draft, other[:, 0])):
+        x.fill_(-INF)
+        x[:, vocab // 3] = m
+    over = torch.randint(vocab // 2, vocab, (c.n_tok, 5), device="cuda", generator=g)
+    c.logits.scatter_(1, over, (shift - 24 - 3 * torch.rand(c.n_tok, 5, device="cuda", generator=g)).to(c.logits.dtype))       # 4e-11 and less
+    c.draft.scatter_(1, over[:, :2], (other - 28 - 3 * torch.rand(c.n_tok, 2, device="cuda", generator=g)).to(c.logits.dtype))
+    c.draft[:, 1] = other[:, 0] - 30
+    c.token.fill_(1)
+    c.u_next.copy_((torch.arange(n_req, device="cuda") + 0.5) / n_req)
+    c.run()
+    assert lib().q4_gpu_last_error() == 0 and c.accepted.tolist() == [0] * n_req
+    accepted, nexts, logp, bad = plain(c)
+    # in the definition's own 64 bits what is over is 2^-52 / 1e-11 off at most; of 64 x 6 borders some lie that near a random number by 2^-10 at most
+    for r, (got, want) in enumerate(zip(c.next.tolist(), nexts)):
+        x = softmax(c.logits[2 * r], 1.0) - softmax(c.draft[2 * r], 1.0)
+        s = x.clamp(min=0).cumsum(0) / x.clamp(min=0).sum()
+        assert got == want or min(abs(float(s[k]) - float(c.u_next[r])) for k in over[2 * r].tolist()) < 1e-4, (r, got, want)
