@@ -8,7 +8,7 @@ constexpr uint32_t PLAN_THREADS = 512, PLAN_MAX_REQ = 8192;
 
 /* The word at which the blocks of a launch meet twice: in its lower half the arrivals, above them whether a block found that nothing may come of the call, and whether
  * one gave up waiting.  That it does only while not all have come, in one step with looking.  So a word in which all have come twice does not
- * change any more, one that somebody gave up never becomes good, and all blocks judge alike whenever they look. */
+ * change any more, one that somebody gave up never becomes good, and all blocks decide alike whenever they look. */
 constexpr uint32_t MEET_HERE = 1u, MEET_BAD = 1u << 16, MEET_LATE = 1u << 17;   /* up to 32767 blocks */
 __host__ __device__ inline bool meet_came(uint32_t word, uint32_t blocks, uint32_t times) { return (word & (MEET_BAD - 1u)) >= times * blocks; }
 __host__ __device__ inline bool meet_over(uint32_t word, uint32_t blocks, uint32_t times) { return meet_came(word, blocks, times) || (word & MEET_LATE); }

@@ -1,6 +1,6 @@
 """The word at which release's blocks meet twice: the rules that the kernel goes by, compiled for the host, over every order in which blocks come, find something bad, wait (to the
-end, or until their time is up) and go on.  All have to judge alike, whenever they look: one that lowers a page's holders where another leaves the stack as it is
-would lose the page.  They judge well exactly where all came in time and none found anything bad."""
+end, or until their time is up) and go on.  All have to decide alike, whenever they look: one that lowers a page's holders where another leaves the stack as it is
+would lose the page.  They go on exactly where all came in time and none found anything bad."""
 import os
 import subprocess
 
@@ -78,9 +78,9 @@ int main() {
         for (uint32_t first = 0; first < 4; first++)
             for (uint32_t second = 0; second < 4; second++)
                 for (int in = 0; in < 2; in++)
-                    if (!holds(blocks, first, second, in, true)) return printf("%u blocks, bad %u and %u, %s: they do not judge alike\n", blocks, first, second, in ? "in time" : "late"), 1;
+                    if (!holds(blocks, first, second, in, true)) return printf("%u blocks, bad %u and %u, %s: they do not decide alike\n", blocks, first, second, in ? "in time" : "late"), 1;
     for (uint32_t blocks = 2; blocks <= 5; blocks++)
-        if (holds(blocks, 0u, 0u, false, false)) return printf("%u blocks: the walk does not see one that gives up behind the others' judgement\n", blocks), 1;
+        if (holds(blocks, 0u, 0u, false, false)) return printf("%u blocks: the walk does not see one that gives up behind the others' decision\n", blocks), 1;
     if (meet_came(MEET_BAD | MEET_LATE | 2047u, 1024u, 2u) || !meet_came(MEET_BAD | MEET_LATE | 2048u, 1024u, 2u)) return printf("the flags are counted as blocks\n"), 1;
     printf("ok\n");
     return 0;
@@ -88,7 +88,7 @@ int main() {
 """
 
 
-def test_all_blocks_judge_alike(tmp_path):
+def test_all_blocks_decide_alike(tmp_path):
     src, exe = tmp_path / "meet.cpp", tmp_path / "meet"
     src.write_text(PROGRAM)
     r = subprocess.run(["g++", "-std=c++17", "-O2", "-I", CSRC, "-I", "/usr/local/cuda/include", str(src), "-o", str(exe)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
